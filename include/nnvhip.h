@@ -463,6 +463,68 @@ NNVHIP_API int nnvhip_affine_avgpool2d(nnvhip_ctx* ctx, const nnvhip_avgpool2d* 
 NNVHIP_API int nnvhip_permute_rows(nnvhip_ctx* ctx, int64_t N, const int32_t* src_row, int64_t count,
                         nnvhip_star* const* in, nnvhip_star** out);
 
+/* ---- operators on points and gradients --------------------------------------------------- */
+/* What a program evaluates networks on points and follows gradients with, beside the sets (the reference evaluates layers
+ * point by point, nn/layers/BatchNormalizationLayer.m:118-229, and searches for counterexamples before a reach; it
+ * has no gradients).  Tensors are device memory in C order, of one of the types below.  A call queues its kernels on `stream` (a
+ * hipStream_t; NULL: the default stream) of the context's device and returns; it neither waits nor allocates, uses
+ * nothing of the context's sets or stream, and may be captured into a graph.  A workspace belongs to the call until its kernels are
+ * done; the _workspace functions say how many bytes of device memory (16-byte aligned) it takes for the same
+ * arguments.  Sums, statistics and softmaxes are f32 at least, whatever the type, and each result is rounded once. */
+enum { NNVHIP_TYPE_F32 = 0, NNVHIP_TYPE_BF16 = 1, NNVHIP_TYPE_F16 = 2 };
+
+/* y = (x - mean) * rstd * scale + offset per row, rstd = 1 / sqrt(mean((x - mean)^2) + epsilon).  x: rows x size, row i at
+ * x + i * x_stride elements; y dense; mean, rstd: rows.  scale, offset: size values of param_type (type, or f32), or NULL. */
+NNVHIP_API int nnvhip_layer_norm(nnvhip_ctx* ctx, int type, int param_type, int64_t rows, int64_t size, const void* x,
+                      int64_t x_stride, const void* scale, const void* offset, double epsilon, void* y, float* mean,
+                      float* rstd, void* stream);
+/* dx = rstd * (g - mean(g) - xh * mean(g * xh)) with xh = (x - mean) * rstd, g = dy * scale; dscale = sum over rows of
+ * dy * xh, doffset = sum over rows of dy, in param_type (either may be NULL).  dx dense. */
+NNVHIP_API int nnvhip_layer_norm_backward_workspace(int type, int64_t rows, int64_t size, int64_t* bytes);
+NNVHIP_API int nnvhip_layer_norm_backward(nnvhip_ctx* ctx, int type, int param_type, int64_t rows, int64_t size, const void* dy,
+                               int64_t dy_stride, const void* x, int64_t x_stride, const float* mean, const float* rstd,
+                               const void* scale, void* dx, void* dscale, void* doffset, void* workspace,
+                               int64_t workspace_bytes, void* stream);
+
+/* Attention of `queries` tokens to the `keys` tokens of another sequence.  q: batch x queries x heads x head, k and v:
+ * batch x keys x kv_heads x head, with strides (in elements) for batch, token and head and dense values; consecutive
+ * heads / kv_heads heads share keys and values.  head: 1 to 128.  The keys that count: the first key_lengths[b] of sequence b
+ * (batch values; beyond [0, keys] they are taken as that bound; NULL: all), and of those the ones with key_mask != 0 (batch x keys
+ * bytes with strides; NULL: all).  Keys that do not count are not read into any sum, whatever they hold.
+ *   forward: o = softmax(scale * q k^T) v (dense), lse = log of the softmax's sums (batch x heads x queries); a row for
+ *     which no key counts gives o = 0, lse = -inf.
+ *   backward: go (the gradient of o, strided), o and lse as the forward call gave them; dq, dk, dv dense in the shapes of q, k, v,
+ *     zero where a row or key takes no part.  The order of the sums is fixed: the same inputs give the same bits. */
+typedef struct nnvhip_attention {
+  int64_t type, batch, queries, keys, heads, kv_heads, head;
+  double scale;
+  const void *q, *k, *v;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  const int32_t* key_lengths;
+  const uint8_t* key_mask;
+  int64_t mask_stride[2];
+  void* o;
+  float* lse;
+  const void* go;
+  int64_t go_stride[3];
+  void *dq, *dk, *dv;
+} nnvhip_attention;
+NNVHIP_API int nnvhip_cross_attention_workspace(const nnvhip_attention* d, int64_t* bytes);
+NNVHIP_API int nnvhip_cross_attention(nnvhip_ctx* ctx, const nnvhip_attention* d, void* workspace, int64_t workspace_bytes,
+                           void* stream);
+NNVHIP_API int nnvhip_cross_attention_backward_workspace(const nnvhip_attention* d, int64_t* bytes);
+NNVHIP_API int nnvhip_cross_attention_backward(nnvhip_ctx* ctx, const nnvhip_attention* d, void* workspace,
+                                    int64_t workspace_bytes, void* stream);
+
+/* The norm over all `count` tensors, sqrt(sum of squares), to *norm (device memory; may be NULL), and the tensors scaled
+ * to it: out[k] = in[k] * (norm > threshold ? threshold / norm : 1).  type, n (values), in, out: host arrays of `count` entries that are
+ * read before the call returns; in and out hold device pointers.  out[k] may be in[k]; out NULL: the norm alone.  The
+ * tensors must not overlap otherwise. */
+NNVHIP_API int nnvhip_clip_gradients_workspace(int64_t count, int64_t* bytes);
+NNVHIP_API int nnvhip_clip_gradients(nnvhip_ctx* ctx, int64_t count, const int32_t* type, const int64_t* n, const void* const* in,
+                          void* const* out, double threshold, float* norm, void* workspace, int64_t workspace_bytes,
+                          void* stream);
+
 #ifdef __cplusplus
 }
 #endif

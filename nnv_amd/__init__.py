@@ -10,3 +10,19 @@ from .layers_affine import (AveragePooling2DLayer, BatchNormalizationLayer, Flat
 from .nn import NN  # noqa: F401
 from .sets import Box, ImageStar, SetArray, Star, Zono  # noqa: F401
 from .verify import HalfSpace, verify_specification  # noqa: F401
+
+# The operators on points work on torch tensors; torch is imported when one of them is first used.
+_POINTS = ("layer_norm", "layer_norm_backward", "cross_attention", "cross_attention_backward", "clip_gradients",
+           "LayerNormalizationLayer", "CrossAttentionLayer")
+
+
+def __getattr__(name):
+    if name in _POINTS:
+        from . import points
+        value = globals()[name] = getattr(points, name)
+        return value
+    raise AttributeError("module %r has no attribute %r" % (__name__, name))
+
+
+def __dir__():
+    return sorted(list(globals()) + list(_POINTS))

@@ -30,6 +30,9 @@ SYMBOLS = [
     "nnvhip_estimate_ranges_static", "nnvhip_debug_mailbox_pack", "nnvhip_debug_mailbox_unpack",
     "nnvhip_debug_set_relu_call_number", "nnvhip_reach_layers", "nnvhip_reach_is_one_launch", "nnvhip_relu_reduce_mem",
     "nnvhip_set_switch", "nnvhip_hint_next_fc", "nnvhip_debug_counters", "nnvhip_debug_relu_bounds", "nnvhip_debug_routes", "nnvhip_debug_pool_limit", "nnvhip_debug_fail_copies", "nnvhip_debug_staging", "nnvhip_weight_cache_stats", "nnvhip_weight_cache_release", "nnvhip_debug_weak_weight_hash",
+    "nnvhip_layer_norm", "nnvhip_layer_norm_backward_workspace", "nnvhip_layer_norm_backward",
+    "nnvhip_cross_attention_workspace", "nnvhip_cross_attention", "nnvhip_cross_attention_backward_workspace",
+    "nnvhip_cross_attention_backward", "nnvhip_clip_gradients_workspace", "nnvhip_clip_gradients",
 ]
 
 
@@ -136,6 +139,15 @@ def load():
         "nnvhip_weight_cache_stats": [p, pi64, pi64, pi64],
         "nnvhip_weight_cache_release": [p, pi64],
         "nnvhip_debug_weak_weight_hash": [C.c_int],
+        "nnvhip_layer_norm": [p, C.c_int, C.c_int, i64, i64, p, i64, p, p, dbl, p, p, p, p],
+        "nnvhip_layer_norm_backward_workspace": [C.c_int, i64, i64, p],
+        "nnvhip_layer_norm_backward": [p, C.c_int, C.c_int, i64, i64, p, i64, p, i64, p, p, p, p, p, p, p, i64, p],
+        "nnvhip_cross_attention_workspace": [p, p],
+        "nnvhip_cross_attention": [p, p, p, i64, p],
+        "nnvhip_cross_attention_backward_workspace": [p, p],
+        "nnvhip_cross_attention_backward": [p, p, p, i64, p],
+        "nnvhip_clip_gradients_workspace": [i64, p],
+        "nnvhip_clip_gradients": [p, i64, p, p, p, p, dbl, p, p, i64, p],
     }
     for name, args in sig.items():
         fn = getattr(lib, name)

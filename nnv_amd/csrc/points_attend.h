@@ -1,0 +1,153 @@
+// Attention of points to another sequence's states: what the forward and the backward kernels share.
+//
+//   S = scale q k^T,  lse = log sum over the keys that count of exp(S),  P = exp(S - lse),  o = P v
+//   D = rowsum(do o),  dS = P (do v^T - D),  dq = scale dS k,  dk = scale dS^T q,  dv = P^T do
+//
+// Rows.  The heads / kv_heads heads that share keys and values are taken as more rows of one product: row r of (sequence b,
+// key/value head) is query r % queries of the group's head r / queries.  A tile of keys then serves all of them, a
+// single token of a group of heads fills a tile as far as the group goes, and the gradients of shared keys and values are sums
+// over rows like any other.  lse, D and the partial results are indexed by (b, key/value head, row), which is the
+// (b, head, query) order of the caller's lse.
+//
+// Every product is formed so that what comes out of one is what the next one takes in.  The 32x32 matrix instructions
+// leave lane l column l % 32 and rows 8 (i / 4) + 4 (l / 32) + i % 4 (i = 0 .. 15) of a product, and take as right operand
+// column l % 32 and a slice of the summed index.  So the scores are formed transposed, S^T = k q^T: a lane holds 16 keys of one
+// query, row sums and largest values need one exchange with lane l ^ 32, and P^T is the right operand of o^T = v^T P^T as it
+// stands, if the left operand takes its keys in the same order.
+#pragma once
+#include "points.h"
+
+#include <algorithm>
+
+namespace nnvhip {
+
+typedef float float16_t __attribute__((ext_vector_type(16)));
+
+struct TokenView {   // batch x tokens x heads x head, the last index dense
+  const void* p;
+  int64_t b, t, h;   // strides in elements
+};
+
+struct AttendArgs {
+  TokenView q, k, v, o, go;   // go: the gradient of o
+  void* out;                  // o of the forward pass, dense
+  void *dq, *dk, *dv;         // dense
+  float* lse;                 // batch x heads x queries
+  const int32_t* lengths;     // batch, or null
+  const uint8_t* mask;        // batch x keys, or null
+  int64_t mask_b, mask_k;
+  int batch, queries, keys, kv_heads, group, head;
+  int64_t rows;               // group * queries, below 2^31
+  float scale;
+  int row_tiles, key_tiles, splits;
+  float* delta;               // D, batch x heads x queries
+  float* part;                // partial results of the splits
+  float* part_lse;
+};
+
+__device__ __forceinline__ int keys_that_count(const AttendArgs& a, int b) {
+  return a.lengths ? min(max(a.lengths[b], 0), a.keys) : a.keys;
+}
+__device__ __forceinline__ bool key_counts(const AttendArgs& a, int b, int key, int n) {
+  return key < n && (a.mask == nullptr || a.mask[b * a.mask_b + key * a.mask_k] != 0);
+}
+// offset of row r of (b, kv) in a token view
+__device__ __forceinline__ int64_t row_at(const TokenView& t, const AttendArgs& a, int b, int kv, int64_t r) {
+  const int64_t g = (uint32_t)r / (uint32_t)a.queries, i = r - g * a.queries;
+  return b * t.b + i * t.t + (kv * (int64_t)a.group + g) * t.h;
+}
+// ... and in a dense tensor of that shape
+__device__ __forceinline__ int64_t dense_row_at(const AttendArgs& a, int b, int kv, int64_t r) {
+  const int64_t g = (uint32_t)r / (uint32_t)a.queries, i = r - g * a.queries;
+  return ((b * (int64_t)a.queries + i) * a.kv_heads * a.group + kv * (int64_t)a.group + g) * a.head;
+}
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// the row of a 32x32 product that register i of a lane's half h holds
+__device__ __forceinline__ int product_row(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
+
+struct Four {
+  float v[4];
+};
+// four elements at d, d + 1, ... of a row of `head`; those that do not exist, and all of them if !there, are zero
+template <typename T>
+__device__ __forceinline__ Four load_four(const T* row, int d, int head, bool there) {
+  Four f;
+  if (there && d + 4 <= head) {
+    T t[4];
+    __builtin_memcpy(t, row + d, sizeof(t));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f.v[i] = to_f(t[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f.v[i] = there && d + i < head ? to_f(row[d + i]) : 0.0f;
+  }
+  return f;
+}
+template <typename T>
+__device__ __forceinline__ void store_four(T* row, int d, int head, const float (&f)[4]) {
+  if (d + 4 <= head) {
+    T t[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t[i] = from_f<T>(f[i]);
+    __builtin_memcpy(row + d, t, sizeof(t));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (d + i < head) row[d + i] = from_f<T>(f[i]);
+  }
+}
+
+constexpr int kWaveRows = 32;  // rows of a wave's tile on either side
+
+// 32 rows of a token view as f32 in LDS, rows of DP + 4 floats: a quarter wave's 16-byte reads of one column block then
+// touch every bank once.  NT threads share the work; load() asks for the rows, store() puts what has arrived into LDS.
+template <typename T, int DP, int NT>
+struct Stage {
+  static constexpr int LD = DP + 4, PER = kWaveRows * DP / 4 / NT;
+  Four r[PER];
+  // row(j): pointer of row j; there(j): whether it exists and counts
+  template <class Row, class There>
+  __device__ __forceinline__ void load(Row row, There there, int head, int tid) {
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      const int at = p * NT + tid, j = at / (DP / 4), d = at % (DP / 4) * 4;
+      const bool ok = there(j);
+      r[p] = load_four<T>(ok ? row(j) : (const T*)nullptr, d, head, ok);
+    }
+  }
+  __device__ __forceinline__ void store(float* lds, int tid) {
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      const int at = p * NT + tid, j = at / (DP / 4), d = at % (DP / 4) * 4;
+      __builtin_memcpy(lds + j * LD + d, r[p].v, 16);
+    }
+  }
+};
+
+// The arguments of the kernels from the caller's; what it checks, it reports as `what`.
+int attend_args(const char* what, const nnvhip_attention* d, bool backward, AttendArgs* a);
+// Blocks over which one axis is split so that `blocks` blocks become enough for the chip; no split gets fewer than `least` of the
+// axis' `tiles` tiles.
+inline int split_of(int64_t blocks, int64_t tiles, int64_t least, int64_t want) {
+  if (blocks <= 0 || blocks >= want) return 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(ceil_div(want, blocks), tiles / least), 256));
+}
+
+#define ATTEND_BY_HEAD(CALL, T, ...)                 \
+  do {                                               \
+    if (a.head <= 32) CALL<T, 32>(__VA_ARGS__);      \
+    else if (a.head <= 64) CALL<T, 64>(__VA_ARGS__); \
+    else if (a.head <= 96) CALL<T, 96>(__VA_ARGS__); \
+    else CALL<T, 128>(__VA_ARGS__);                  \
+  } while (0)
+#define ATTEND_BY_TYPE(type, CALL, ...)                                        \
+  do {                                                                         \
+    if ((type) == NNVHIP_TYPE_F32) ATTEND_BY_HEAD(CALL, float, __VA_ARGS__);   \
+    else if ((type) == NNVHIP_TYPE_BF16) ATTEND_BY_HEAD(CALL, bf16_t, __VA_ARGS__); \
+    else ATTEND_BY_HEAD(CALL, f16_t, __VA_ARGS__);                             \
+  } while (0)
+
+}  // namespace nnvhip

@@ -1,0 +1,326 @@
+// Attention of points, forward: the kernels for every type, head size and alignment.
+//
+// The products run on the f32 matrix instructions (v_mfma_f32_32x32x2_f32, 157 TFLOP/s at best), whatever the type of the
+// tensors: f32 tensors keep f32 results, and tensors of 16 bits lose nothing but their final rounding.
+#include "points_attend.h"
+
+#include <algorithm>
+
+#pragma clang fp contract(fast)
+
+namespace nnvhip {
+namespace {
+
+// LDS written by other lanes of the wave (FEW) or of the block
+template <bool FEW>
+__device__ __forceinline__ void lds_barrier() {
+  if constexpr (FEW) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  } else {
+    __syncthreads();
+  }
+}
+
+// One pass over the keys with the running maximum and sum of every query's softmax.
+// FEW = false: a block takes 128 rows, 32 a wave, and its waves share the tiles of keys.
+// FEW = true: a block takes 32 rows and its waves take the tiles of keys in turn, each with LDS of its own; what they found is
+// joined at the end.  For single tokens, where there are many keys for each of a few rows.
+// Where there are too few blocks for the chip, the keys are split over `splits` blocks, and join_kernel puts their results together.
+template <typename T, int DP, bool FEW>
+__global__ __launch_bounds__(256) void attend_kernel(const AttendArgs a) {
+  constexpr int kTile = kWaveRows, LD = DP + 4, NT = FEW ? 64 : 256, STEP = FEW ? 4 : 1;
+  __shared__ float lds[(FEW ? 4 : 1) * 2 * kTile * LD];
+  __shared__ float row_max[4][kTile], row_total[4][kTile];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
+  const int tid = FEW ? lane : threadIdx.x;
+  int64_t at = blockIdx.x;
+  const int split = at % a.splits;
+  at /= a.splits;
+  const int row_tile = at % a.row_tiles;
+  const int bkv = at / a.row_tiles, b = bkv / a.kv_heads, kv = bkv % a.kv_heads;
+  const int n = keys_that_count(a, b);
+  const int tiles = (n + kTile - 1) / kTile, per = (tiles + a.splits - 1) / a.splits;
+  const int t0 = split * per + (FEW ? wave : 0), t1 = min(tiles, split * per + per);
+  const int64_t r = FEW ? (int64_t)row_tile * kTile + col : (int64_t)row_tile * 128 + wave * kTile + col;
+  const bool row_here = r < a.rows;
+  float* ks = lds + (FEW ? wave * 2 * kTile * LD : 0);
+  float* vs = ks + kTile * LD;
+
+  float qf[DP / 8][4];
+  {
+    const T* q = (const T*)a.q.p + (row_here ? row_at(a.q, a, b, kv, r) : 0);
+#pragma unroll
+    for (int c = 0; c < DP / 8; ++c) {
+      const Four f = load_four<T>(q, 8 * c + 4 * h, a.head, row_here);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) qf[c][j] = f.v[j] * (a.scale * kLog2e);
+    }
+  }
+  float16_t acc[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
+  float m = -INFINITY, total = 0.0f;
+
+  const T* kp = (const T*)a.k.p + b * a.k.b + kv * a.k.h;
+  const T* vp = (const T*)a.v.p + b * a.v.b + kv * a.v.h;
+  Stage<T, DP, NT> ks_next, vs_next;
+  bool counts = false;
+  auto fetch = [&](int t) {
+    auto there = [&](int j) { return key_counts(a, b, t * kTile + j, n); };
+    ks_next.load([&](int j) { return kp + (t * kTile + j) * a.k.t; }, there, a.head, tid);
+    vs_next.load([&](int j) { return vp + (t * kTile + j) * a.v.t; }, there, a.head, tid);
+    counts = there(col);
+  };
+  if (t0 < t1) fetch(t0);
+  for (int t = t0; t < t1; t += STEP) {
+    lds_barrier<FEW>();
+    ks_next.store(ks, tid);
+    vs_next.store(vs, tid);
+    const uint32_t valid = (uint32_t)__ballot(counts) >> (4 * h);
+    lds_barrier<FEW>();
+    if (t + STEP < t1) fetch(t + STEP);
+
+    float16_t s;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < DP / 8; ++c) {
+      float kf[4];
+      __builtin_memcpy(kf, ks + col * LD + 8 * c + 4 * h, 16);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[j], qf[c][j], s, 0, 0, 0);
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[i] = (valid >> product_row(i, 0)) & 1 ? s[i] : -INFINITY;
+      top = fmaxf(top, s[i]);
+    }
+    top = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
+    const float base = top == -INFINITY ? 0.0f : top;   // no key of this row counts yet
+    const float fade = exp2_(m - base);
+    m = top;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[i] = exp2_(s[i] - base);
+      sum += s[i];
+    }
+    total = total * fade + sum;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[d][i] *= fade;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vs[product_row(i, h) * LD + d * 32 + col], s[i], acc[d], 0, 0, 0);
+    }
+  }
+  total += __shfl_xor(total, 32, 64);
+
+  const int64_t flat = (int64_t)bkv * a.rows + r;   // of this lane's row
+  if constexpr (!FEW) {
+    if (!row_here) return;
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    const float lse = total == 0.0f ? -INFINITY : (m + log2f(total)) * kLn2;
+    if (h == 0) {
+      if (a.splits > 1) a.part_lse[(int64_t)split * a.batch * a.kv_heads * a.rows + flat] = lse;
+      else a.lse[flat] = lse;
+    }
+    float* part = a.splits > 1 ? a.part + ((int64_t)split * a.batch * a.kv_heads * a.rows + flat) * a.head : nullptr;
+    T* out = (T*)a.out + dense_row_at(a, b, kv, r);
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int i4 = 0; i4 < 4; ++i4) {
+        float f[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = acc[d][4 * i4 + i] * inv;
+        const int at_d = d * 32 + 8 * i4 + 4 * h;
+        if (part) store_four(part, at_d, a.head, f);
+        else store_four(out, at_d, a.head, f);
+      }
+  } else {
+    __syncthreads();
+    float* mine = lds + wave * kTile * LD;   // [row][d] of this wave
+    if (h == 0) {
+      row_max[wave][col] = m;
+      row_total[wave][col] = total;
+    }
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mine[col * LD + d * 32 + product_row(i, h)] = acc[d][i];
+    __syncthreads();
+    for (int e = threadIdx.x; e < kTile * (DP / 4); e += 256) {
+      const int j = e / (DP / 4), d = e % (DP / 4) * 4;
+      const int64_t rj = (int64_t)row_tile * kTile + j;
+      if (rj >= a.rows) continue;
+      float top = row_max[0][j], all = 0.0f, w[4], f[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int k = 1; k < 4; ++k) top = fmaxf(top, row_max[k][j]);
+      const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        w[k] = exp2_(row_max[k][j] - base);
+        all += w[k] * row_total[k][j];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] += w[k] * lds[(k * kTile + j) * LD + d + i];
+      }
+      const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] *= inv;
+      const int64_t fj = (int64_t)bkv * a.rows + rj;
+      const float lse = all == 0.0f ? -INFINITY : (top + log2f(all)) * kLn2;
+      const int64_t sj = (int64_t)split * a.batch * a.kv_heads * a.rows + fj;
+      if (d == 0) (a.splits > 1 ? a.part_lse[sj] : a.lse[fj]) = lse;
+      if (d >= a.head) continue;
+      if (a.splits > 1) store_four(a.part + sj * a.head, d, a.head, f);
+      else store_four((T*)a.out + dense_row_at(a, b, kv, rj), d, a.head, f);
+    }
+  }
+}
+
+// o = sum over splits of exp(lse_s - lse) o_s: a wave per row, in the order of the splits.
+template <typename T>
+__global__ __launch_bounds__(256) void join_kernel(const AttendArgs a) {
+  const int64_t all = (int64_t)a.batch * a.kv_heads * a.rows, flat = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (flat >= all) return;
+  const int lane = threadIdx.x & 63;
+  float top = -INFINITY;
+  for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, a.part_lse[s * all + flat]);
+#pragma unroll
+  for (int k = 32; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor(top, k, 64));
+  const float base = top == -INFINITY ? 0.0f : top;
+  float total = 0.0f, f0 = 0.0f, f1 = 0.0f;
+  for (int s = 0; s < a.splits; ++s) {
+    const float w = exp2_((a.part_lse[s * all + flat] - base) * kLog2e);
+    const float* p = a.part + (s * all + flat) * a.head;
+    total += w;
+    if (lane < a.head) f0 += w * p[lane];
+    if (lane + 64 < a.head) f1 += w * p[lane + 64];
+  }
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  const int bkv = (int)(flat / a.rows), b = bkv / a.kv_heads;
+  T* out = (T*)a.out + dense_row_at(a, b, bkv % a.kv_heads, flat % a.rows);
+  if (lane < a.head) out[lane] = from_f<T>(f0 * inv);
+  if (lane + 64 < a.head) out[lane + 64] = from_f<T>(f1 * inv);
+  if (lane == 0) a.lse[flat] = total == 0.0f ? -INFINITY : base + log2f(total) * kLn2;
+}
+
+// How a forward call is cut: few rows for each head's keys (single tokens) or tiles of 128 rows, and over how many blocks the
+// keys are split.
+struct Cut {
+  bool few;
+  int row_tiles, splits;
+};
+Cut cut_of(const AttendArgs& a) {
+  Cut c;
+  c.few = a.rows <= kWaveRows;
+  c.row_tiles = (int)ceil_div(a.rows, c.few ? kWaveRows : 128);
+  const int64_t blocks = (int64_t)a.batch * a.kv_heads * c.row_tiles;
+  c.splits = split_of(blocks, ceil_div(a.keys, kWaveRows), c.few ? 8 : 4, 512);
+  return c;
+}
+
+template <typename T, int DP>
+void launch_attend(const AttendArgs& a, const Cut& c, hipStream_t st) {
+  const dim3 grid((unsigned)((int64_t)a.batch * a.kv_heads * c.row_tiles * c.splits));
+  if (c.few) hipLaunchKernelGGL((attend_kernel<T, DP, true>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((attend_kernel<T, DP, false>), grid, dim3(256), 0, st, a);
+  if (c.splits > 1)
+    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)ceil_div((int64_t)a.batch * a.kv_heads * a.rows, 4)), dim3(256), 0, st, a);
+}
+
+// strides of the last tokens' rows have to be addressable, the sizes have to fit the kernels' indexes
+int check_sizes(const char* what, const nnvhip_attention* d) {
+  if (!known_type(d->type)) NNV_FAIL(NNVHIP_ERR_ARG, "%s: the values are f32, bf16 or f16", what);
+  if (d->batch < 0 || d->queries < 0 || d->keys < 0) NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: negative size", what);
+  if (d->head < 1 || d->head > 128) NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: heads of 1 to 128 values are supported", what);
+  if (d->heads < 1 || d->kv_heads < 1 || d->heads % d->kv_heads)
+    NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: the number of heads must be a multiple of the number of key/value heads", what);
+  const int64_t most = (int64_t(1) << 31) - 256;
+  if (d->batch > 65535 || d->keys > most || d->heads > 65535 || d->queries > most / d->heads ||
+      d->batch * d->heads * ceil_div(std::max(d->queries, d->keys), 32) > most / 256)
+    NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: too many rows", what);
+  return NNVHIP_OK;
+}
+
+}  // namespace
+
+int attend_args(const char* what, const nnvhip_attention* d, bool backward, AttendArgs* a) {
+  if (!d) NNV_FAIL(NNVHIP_ERR_ARG, "%s: null pointer", what);
+  NNV_TRY(check_sizes(what, d));
+  auto view = [](const void* p, const int64_t (&s)[3]) { return TokenView{p, s[0], s[1], s[2]}; };
+  *a = AttendArgs{};
+  a->q = view(d->q, d->q_stride);
+  a->k = view(d->k, d->k_stride);
+  a->v = view(d->v, d->v_stride);
+  a->go = view(d->go, d->go_stride);
+  a->o = TokenView{d->o, d->queries * d->heads * d->head, d->heads * d->head, d->head};
+  a->out = d->o;
+  a->dq = d->dq;
+  a->dk = d->dk;
+  a->dv = d->dv;
+  a->lse = d->lse;
+  a->lengths = d->key_lengths;
+  a->mask = d->key_mask;
+  a->mask_b = d->mask_stride[0];
+  a->mask_k = d->mask_stride[1];
+  a->batch = (int)d->batch;
+  a->queries = (int)d->queries;
+  a->keys = (int)d->keys;
+  a->kv_heads = (int)d->kv_heads;
+  a->group = (int)(d->heads / d->kv_heads);
+  a->head = (int)d->head;
+  a->rows = d->queries * a->group;
+  a->scale = (float)d->scale;
+  const bool no_rows = d->batch == 0 || d->queries == 0, no_keys = d->batch == 0 || d->keys == 0;
+  if ((!no_rows && (!d->q || !d->o || !d->lse)) || (!no_rows && !no_keys && (!d->k || !d->v)) ||
+      (backward && ((!no_rows && (!d->go || !d->dq)) || (!no_keys && (!d->dk || !d->dv)))))
+    NNV_FAIL(NNVHIP_ERR_ARG, "%s: null pointer", what);
+  return NNVHIP_OK;
+}
+
+}  // namespace nnvhip
+
+using namespace nnvhip;
+
+extern "C" {
+
+int nnvhip_cross_attention_workspace(const nnvhip_attention* d, int64_t* bytes) {
+  if (!d || !bytes) NNV_FAIL(NNVHIP_ERR_ARG, "null pointer");
+  NNV_TRY(check_sizes("nnvhip_cross_attention_workspace", d));
+  AttendArgs a{};
+  a.batch = (int)d->batch;
+  a.kv_heads = (int)d->kv_heads;
+  a.keys = (int)d->keys;
+  a.rows = d->queries * (d->heads / d->kv_heads);
+  const Cut c = cut_of(a);
+  *bytes = c.splits > 1 ? (int64_t)c.splits * d->batch * d->heads * d->queries * (d->head + 1) * (int64_t)sizeof(float) : 0;
+  return NNVHIP_OK;
+}
+
+int nnvhip_cross_attention(nnvhip_ctx* ctx, const nnvhip_attention* d, void* workspace, int64_t workspace_bytes, void* stream) {
+  ENTER_POINT_CALL(ctx);
+  AttendArgs a;
+  NNV_TRY(attend_args("nnvhip_cross_attention", d, false, &a));
+  int64_t need = 0;
+  NNV_TRY(nnvhip_cross_attention_workspace(d, &need));
+  if (need > workspace_bytes || (need && !workspace))
+    NNV_FAIL(NNVHIP_ERR_ARG, "nnvhip_cross_attention: a workspace of %lld bytes is needed", (long long)need);
+  if (a.batch == 0 || a.rows == 0) return NNVHIP_OK;
+  const Cut c = cut_of(a);
+  a.row_tiles = c.row_tiles;
+  a.splits = c.splits;
+  a.part = static_cast<float*>(workspace);
+  a.part_lse = c.splits > 1 ? a.part + (int64_t)c.splits * a.batch * a.kv_heads * a.rows * a.head : nullptr;
+  ATTEND_BY_TYPE(d->type, launch_attend, a, c, (hipStream_t)stream);
+  NNV_HIP_TRY(hipGetLastError());
+  return NNVHIP_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,316 @@
+// Attention of points, backward: the kernels for every type, head size and alignment, on the f32 matrix instructions.
+//
+// Two kernels form dq (a wave per 32 queries, over the keys) and dk, dv (a wave per 32 keys, over the queries of every head that
+// shares them).  Both form S and dP again: seven products instead of the five that one kernel would need, but every
+// gradient is a sum in the registers of one wave, in a fixed order, with no atomics.  What both need of a row besides, D = rowsum(do o),
+// is formed first.  Where one axis gives too few blocks for the chip, the other is split, and sum_kernel adds the parts in order.
+#include "points_attend.h"
+
+#pragma clang fp contract(fast)
+
+namespace nnvhip {
+namespace {
+
+// D = rowsum(do o): 16 lanes a row.
+template <typename T>
+__global__ __launch_bounds__(256) void delta_kernel(const AttendArgs a) {
+  const int64_t flat = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
+  const bool here = flat < (int64_t)a.batch * a.kv_heads * a.rows;
+  const int64_t f = here ? flat : 0;
+  const int bkv = (int)(f / a.rows), b = bkv / a.kv_heads, kv = bkv % a.kv_heads;
+  const T* o = (const T*)a.o.p + row_at(a.o, a, b, kv, f % a.rows);
+  const T* g = (const T*)a.go.p + row_at(a.go, a, b, kv, f % a.rows);
+  float s = 0.0f;
+  for (int d = threadIdx.x % 16 * 4; d < a.head; d += 64) {
+    const Four x = load_four(o, d, a.head, true), y = load_four(g, d, a.head, true);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s += x.v[i] * y.v[i];
+  }
+#pragma unroll
+  for (int k = 8; k > 0; k >>= 1) s += __shfl_xor(s, k, 64);
+  if (here && threadIdx.x % 16 == 0) a.delta[flat] = s;
+}
+
+template <int DP>
+__device__ __forceinline__ void zero(float16_t (&acc)[DP / 32]) {
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
+}
+
+// A product with 32 rows of LDS as left operand and a row's fragments in registers as right one: the sum runs over the head.
+template <int DP>
+__device__ __forceinline__ float16_t over_head(const float* rows, const float (&f)[DP / 8][4], int col, int h) {
+  float16_t s;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+#pragma unroll
+  for (int c = 0; c < DP / 8; ++c) {
+    float x[4];
+    __builtin_memcpy(x, rows + col * (DP + 4) + 8 * c + 4 * h, 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], f[c][j], s, 0, 0, 0);
+  }
+  return s;
+}
+// ... and one whose sum runs over the rows of LDS: acc[d][.] += rows^T p
+template <int DP>
+__device__ __forceinline__ void over_rows(const float* rows, const float16_t& p, float16_t (&acc)[DP / 32], int col, int h) {
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(rows[product_row(i, h) * (DP + 4) + d * 32 + col], p[i], acc[d], 0, 0, 0);
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ void load_fragments(float (&f)[DP / 8][4], const T* row, int h, int head, bool there) {
+#pragma unroll
+  for (int c = 0; c < DP / 8; ++c) {
+    const Four x = load_four(row, 8 * c + 4 * h, head, there);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[c][j] = x.v[j];
+  }
+}
+template <typename T, int DP>
+__device__ __forceinline__ void store_fragments(T* row, const float16_t (&acc)[DP / 32], float by, int h, int head) {
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int i4 = 0; i4 < 4; ++i4) {
+      float f[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = acc[d][4 * i4 + i] * by;
+      store_four(row, d * 32 + 8 * i4 + 4 * h, head, f);
+    }
+}
+
+// lse of a row as the exponent's offset in powers of two; a row without keys takes no part (exp2(s - inf) = 0)
+__device__ __forceinline__ float offset_of(float lse) { return lse == -INFINITY ? INFINITY : lse * kLog2e; }
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void query_grad_kernel(const AttendArgs a) {
+  constexpr int LD = DP + 4, R = kWaveRows;
+  __shared__ float ks[R * LD], vs[R * LD];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
+  int64_t at = blockIdx.x;
+  const int split = at % a.splits;
+  at /= a.splits;
+  const int row_tile = at % a.row_tiles;
+  const int bkv = at / a.row_tiles, b = bkv / a.kv_heads, kv = bkv % a.kv_heads;
+  const int n = keys_that_count(a, b);
+  const int tiles = (n + R - 1) / R, per = (tiles + a.splits - 1) / a.splits;
+  const int t0 = split * per, t1 = min(tiles, t0 + per);
+  const int64_t r = (int64_t)row_tile * 128 + wave * R + col, flat = (int64_t)bkv * a.rows + r;
+  const bool here = r < a.rows;
+  const float lse = here ? a.lse[flat] : -INFINITY;
+  const bool takes_part = here && lse != -INFINITY;
+  const float offset = offset_of(lse), delta = takes_part ? a.delta[flat] : 0.0f, unit = a.scale * kLog2e;
+  float qf[DP / 8][4], gf[DP / 8][4];
+  load_fragments<T, DP>(qf, (const T*)a.q.p + (here ? row_at(a.q, a, b, kv, r) : 0), h, a.head, takes_part);
+  load_fragments<T, DP>(gf, (const T*)a.go.p + (here ? row_at(a.go, a, b, kv, r) : 0), h, a.head, takes_part);
+  float16_t dq[DP / 32];
+  zero<DP>(dq);
+  const T* kp = (const T*)a.k.p + b * a.k.b + kv * a.k.h;
+  const T* vp = (const T*)a.v.p + b * a.v.b + kv * a.v.h;
+  Stage<T, DP, 256> k_next, v_next;
+  bool counts = false;
+  auto fetch = [&](int t) {
+    auto there = [&](int j) { return key_counts(a, b, t * R + j, n); };
+    k_next.load([&](int j) { return kp + (t * R + j) * a.k.t; }, there, a.head, threadIdx.x);
+    v_next.load([&](int j) { return vp + (t * R + j) * a.v.t; }, there, a.head, threadIdx.x);
+    counts = there(col);
+  };
+  if (t0 < t1) fetch(t0);
+  for (int t = t0; t < t1; ++t) {
+    __syncthreads();
+    k_next.store(ks, threadIdx.x);
+    v_next.store(vs, threadIdx.x);
+    const uint32_t valid = (uint32_t)__ballot(counts) >> (4 * h);
+    __syncthreads();
+    if (t + 1 < t1) fetch(t + 1);
+    float16_t s = over_head<DP>(ks, qf, col, h);
+    const float16_t dp = over_head<DP>(vs, gf, col, h);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float p = exp2_(s[i] * unit - offset);
+      s[i] = (valid >> product_row(i, 0)) & 1 ? p * (dp[i] - delta) : 0.0f;
+    }
+    over_rows<DP>(ks, s, dq, col, h);
+  }
+  if (!here) return;
+  if (a.splits > 1)
+    store_fragments<float, DP>(a.part + ((int64_t)split * a.batch * a.kv_heads * a.rows + flat) * a.head, dq, a.scale, h, a.head);
+  else
+    store_fragments<T, DP>((T*)a.dq + dense_row_at(a, b, kv, r), dq, a.scale, h, a.head);
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void key_grad_kernel(const AttendArgs a) {
+  constexpr int LD = DP + 4, R = kWaveRows;
+  __shared__ float qs[R * LD], gs[R * LD], offsets[R], deltas[R];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
+  int64_t at = blockIdx.x;
+  const int split = at % a.splits;
+  at /= a.splits;
+  const int key_tile = at % a.key_tiles;
+  const int bkv = at / a.key_tiles, b = bkv / a.kv_heads, kv = bkv % a.kv_heads;
+  const int n = keys_that_count(a, b);
+  const int key = key_tile * 128 + wave * R + col;
+  const bool here = key < a.keys, counts = key_counts(a, b, key, n);
+  int t0 = 0, t1 = 0;
+  if (key_tile * 128 < n) {   // else no key of the block counts: its gradients are zero
+    const int tiles = (int)((a.rows + R - 1) / R), per = (tiles + a.splits - 1) / a.splits;
+    t0 = split * per;
+    t1 = min(tiles, t0 + per);
+  }
+  float kf[DP / 8][4], vf[DP / 8][4];
+  load_fragments<T, DP>(kf, (const T*)a.k.p + (counts ? b * a.k.b + kv * a.k.h + key * a.k.t : 0), h, a.head, counts);
+  load_fragments<T, DP>(vf, (const T*)a.v.p + (counts ? b * a.v.b + kv * a.v.h + key * a.v.t : 0), h, a.head, counts);
+  const float unit = a.scale * kLog2e;
+  float16_t dk[DP / 32], dv[DP / 32];
+  zero<DP>(dk);
+  zero<DP>(dv);
+  Stage<T, DP, 256> q_next, g_next;
+  float offset = INFINITY, delta = 0.0f;
+  const float* lse = a.lse + (int64_t)bkv * a.rows;
+  auto fetch = [&](int t) {
+    // the rows of a row without keys are not read: what they hold must not reach the sums
+    auto there = [&](int j) { return (int64_t)t * R + j < a.rows && lse[(int64_t)t * R + j] != -INFINITY; };
+    q_next.load([&](int j) { return (const T*)a.q.p + row_at(a.q, a, b, kv, (int64_t)t * R + j); }, there, a.head, threadIdx.x);
+    g_next.load([&](int j) { return (const T*)a.go.p + row_at(a.go, a, b, kv, (int64_t)t * R + j); }, there, a.head, threadIdx.x);
+    if (threadIdx.x < R) {
+      const int64_t r = (int64_t)t * R + threadIdx.x;
+      offset = offset_of(r < a.rows ? lse[r] : -INFINITY);
+      delta = r < a.rows && offset != INFINITY ? a.delta[(int64_t)bkv * a.rows + r] : 0.0f;
+    }
+  };
+  if (t0 < t1) fetch(t0);
+  for (int t = t0; t < t1; ++t) {
+    __syncthreads();
+    q_next.store(qs, threadIdx.x);
+    g_next.store(gs, threadIdx.x);
+    if (threadIdx.x < R) {
+      offsets[threadIdx.x] = offset;
+      deltas[threadIdx.x] = delta;
+    }
+    __syncthreads();
+    if (t + 1 < t1) fetch(t + 1);
+    float16_t s = over_head<DP>(qs, kf, col, h);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = counts ? exp2_(s[i] * unit - offsets[product_row(i, h)]) : 0.0f;
+    over_rows<DP>(gs, s, dv, col, h);
+    const float16_t dp = over_head<DP>(gs, vf, col, h);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] *= dp[i] - deltas[product_row(i, h)];
+    over_rows<DP>(qs, s, dk, col, h);
+  }
+  if (!here) return;
+  const int64_t dense = ((b * (int64_t)a.keys + key) * a.kv_heads + kv) * a.head;
+  if (a.splits > 1) {
+    const int64_t all = (int64_t)a.batch * a.keys * a.kv_heads * a.head;
+    store_fragments<float, DP>(a.part + split * all + dense, dk, a.scale, h, a.head);
+    store_fragments<float, DP>(a.part + (a.splits + split) * all + dense, dv, 1.0f, h, a.head);
+  } else {
+    store_fragments<T, DP>((T*)a.dk + dense, dk, a.scale, h, a.head);
+    store_fragments<T, DP>((T*)a.dv + dense, dv, 1.0f, h, a.head);
+  }
+}
+
+// out[e] = sum over splits of part[s][e], in order
+template <typename T>
+__global__ __launch_bounds__(256) void sum_kernel(const float* __restrict__ part, int splits, int64_t n, T* __restrict__ out) {
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (e >= n) return;
+  float s = 0.0f;
+  for (int k = 0; k < splits; ++k) s += part[k * n + e];
+  out[e] = from_f<T>(s);
+}
+// the same for rows in the order of lse, written in the order of the tensor
+template <typename T>
+__global__ __launch_bounds__(256) void sum_rows_kernel(const AttendArgs a, T* __restrict__ out) {
+  const int64_t all = (int64_t)a.batch * a.kv_heads * a.rows, flat = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (flat >= all) return;
+  const int bkv = (int)(flat / a.rows), b = bkv / a.kv_heads;
+  T* row = out + dense_row_at(a, b, bkv % a.kv_heads, flat % a.rows);
+  for (int d = threadIdx.x & 63; d < a.head; d += 64) {
+    float s = 0.0f;
+    for (int k = 0; k < a.splits; ++k) s += a.part[(k * all + flat) * a.head + d];
+    row[d] = from_f<T>(s);
+  }
+}
+
+struct GradCut {
+  int row_tiles, key_tiles, query_splits, key_splits;
+  int64_t delta, part;   // floats of the workspace
+};
+GradCut grad_cut(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys, int64_t head) {
+  GradCut c;
+  c.row_tiles = (int)ceil_div(rows, 128);
+  c.key_tiles = (int)ceil_div(keys, 128);
+  c.query_splits = split_of(batch * kv_heads * c.row_tiles, ceil_div(keys, kWaveRows), 4, 512);
+  c.key_splits = split_of(batch * kv_heads * c.key_tiles, ceil_div(rows, kWaveRows), 4, 512);
+  c.delta = round_up(batch * kv_heads * rows, 64);
+  const int64_t q = c.query_splits > 1 ? c.query_splits * batch * kv_heads * rows * head : 0;
+  const int64_t k = c.key_splits > 1 ? 2 * c.key_splits * batch * kv_heads * keys * head : 0;
+  c.part = std::max(q, k);
+  return c;
+}
+
+template <typename T, int DP>
+void launch_grad(AttendArgs a, const GradCut& c, hipStream_t st) {
+  const int64_t heads = (int64_t)a.batch * a.kv_heads;
+  if (a.rows > 0) {
+    hipLaunchKernelGGL((delta_kernel<T>), dim3((unsigned)ceil_div(heads * a.rows, 16)), dim3(256), 0, st, a);
+    a.row_tiles = c.row_tiles;
+    a.splits = c.query_splits;
+    hipLaunchKernelGGL((query_grad_kernel<T, DP>), dim3((unsigned)(heads * c.row_tiles * a.splits)), dim3(256), 0, st, a);
+    if (a.splits > 1) hipLaunchKernelGGL((sum_rows_kernel<T>), dim3((unsigned)ceil_div(heads * a.rows, 4)), dim3(256), 0, st, a, (T*)a.dq);
+  }
+  if (a.keys > 0) {
+    a.key_tiles = c.key_tiles;
+    a.splits = c.key_splits;
+    hipLaunchKernelGGL((key_grad_kernel<T, DP>), dim3((unsigned)(heads * c.key_tiles * a.splits)), dim3(256), 0, st, a);
+    if (a.splits > 1) {
+      const int64_t n = heads * a.keys * a.head;
+      hipLaunchKernelGGL((sum_kernel<T>), dim3((unsigned)ceil_div(n, 256)), dim3(256), 0, st, a.part, a.splits, n, (T*)a.dk);
+      hipLaunchKernelGGL((sum_kernel<T>), dim3((unsigned)ceil_div(n, 256)), dim3(256), 0, st, a.part + a.splits * n, a.splits, n, (T*)a.dv);
+    }
+  }
+}
+
+}  // namespace
+}  // namespace nnvhip
+
+using namespace nnvhip;
+
+extern "C" {
+
+int nnvhip_cross_attention_backward_workspace(const nnvhip_attention* d, int64_t* bytes) {
+  int64_t forward = 0;
+  NNV_TRY(nnvhip_cross_attention_workspace(d, &forward));   // checks the sizes
+  if (!bytes) NNV_FAIL(NNVHIP_ERR_ARG, "null pointer");
+  const GradCut c = grad_cut(d->batch, d->kv_heads, d->queries * (d->heads / d->kv_heads), d->keys, d->head);
+  *bytes = (c.delta + c.part) * (int64_t)sizeof(float);
+  return NNVHIP_OK;
+}
+
+int nnvhip_cross_attention_backward(nnvhip_ctx* ctx, const nnvhip_attention* d, void* workspace, int64_t workspace_bytes, void* stream) {
+  ENTER_POINT_CALL(ctx);
+  AttendArgs a;
+  NNV_TRY(attend_args("nnvhip_cross_attention_backward", d, true, &a));
+  int64_t need = 0;
+  NNV_TRY(nnvhip_cross_attention_backward_workspace(d, &need));
+  if (need > workspace_bytes || (need && !workspace))
+    NNV_FAIL(NNVHIP_ERR_ARG, "nnvhip_cross_attention_backward: a workspace of %lld bytes is needed", (long long)need);
+  if (a.batch == 0) return NNVHIP_OK;
+  const GradCut c = grad_cut(a.batch, a.kv_heads, a.rows, a.keys, a.head);
+  a.delta = static_cast<float*>(workspace);
+  a.part = a.delta + c.delta;
+  ATTEND_BY_TYPE(d->type, launch_grad, a, c, (hipStream_t)stream);
+  NNV_HIP_TRY(hipGetLastError());
+  return NNVHIP_OK;
+}
+
+}  // extern "C"

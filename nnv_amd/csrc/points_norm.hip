@@ -1,0 +1,462 @@
+// Layer normalization of points, forward and backward.
+//
+//   mu = mean(x), r = 1 / sqrt(mean((x - mu)^2) + eps), xh = (x - mu) r, y = xh w + b        (per row of `size` values)
+//   g = dy w;  dx = r (g - mean(g) - xh mean(g xh));  dw = sum over rows of dy xh;  db = sum over rows of dy
+//
+// Both are bound by memory: the forward pass reads x and writes y, the backward pass reads x and dy and writes dx, and
+// everything else they do fits under that.  A row is read once: its values stay in the registers of the lanes that hold it,
+// so the variance is a second sum over registers around the mean already known (no difference of large squares).  All
+// sums are f32; what is written in 16 bits is rounded once, at the store.
+#include "points.h"
+
+#include <algorithm>
+
+#pragma clang fp contract(fast)
+
+namespace nnvhip {
+namespace {
+
+constexpr int kThreads = 512;
+
+// Sum of N values over the LPR consecutive lanes that share a row.  Rows of more than a wave add through LDS; `slot` alternates
+// between two sets of partial sums, so that one barrier per sum is enough (a wave can be at most one sum ahead of
+// another, and that one writes the other set).
+template <int LPR, int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], float* lds, int& slot) {
+  constexpr int kIn = LPR < 64 ? LPR : 64;
+#pragma unroll
+  for (int s = kIn / 2; s > 0; s >>= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] += __shfl_xor(v[k], s, 64);
+  if constexpr (LPR > 64) {
+    constexpr int kWaves = LPR / 64;
+    const int wave = threadIdx.x >> 6;
+    float* part = lds + slot * (kThreads / 64 * N);
+    slot ^= 1;
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int k = 0; k < N; ++k) part[wave * N + k] = v[k];
+    __syncthreads();
+    const int first = wave / kWaves * kWaves;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      float s = 0;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) s += part[(first + w) * N + k];
+      v[k] = s;
+    }
+  }
+}
+
+// W: the type of the scale and the offset (T, or float).
+template <typename W>
+__device__ __forceinline__ float param(const W* p, int64_t c, float none) {
+  return p ? to_f(p[c]) : none;
+}
+
+template <typename T, typename W, int LPR, int NV>
+__global__ __launch_bounds__(kThreads) void norm_kernel(const T* __restrict__ x, int64_t x_stride, const W* __restrict__ scale,
+                                                        const W* __restrict__ offset, float eps, int64_t rows, int size,
+                                                        T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
+  constexpr int V = kVec<T>, kRows = kThreads / LPR;
+  __shared__ float lds[2 * kThreads / 64];
+  int slot = 0;
+  const int lane = threadIdx.x % LPR;
+  const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / LPR;
+  const bool here = row < rows;
+  Pack<T> in[NV];
+  float s[1] = {0};
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = (j * LPR + lane) * V;
+    in[j] = load_pack(x + (here ? row : 0) * x_stride + c, here ? size - c : 0);
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[0] += to_f(in[j].v[i]);
+  }
+  row_sum<LPR, 1>(s, lds, slot);
+  const float mu = s[0] / size;
+  float q[1] = {0};
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = (j * LPR + lane) * V;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float d = to_f(in[j].v[i]) - mu;
+      q[0] += c + i < size ? d * d : 0.0f;
+    }
+  }
+  row_sum<LPR, 1>(q, lds, slot);
+  const float r = 1.0f / sqrtf(q[0] / size + eps);
+  if (!here) return;
+  if (lane == 0) {
+    mean[row] = mu;
+    rstd[row] = r;
+  }
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = (j * LPR + lane) * V;
+    if (c >= size) break;
+    Pack<W> w[V / kVec<W> ? V / kVec<W> : 1], b[V / kVec<W> ? V / kVec<W> : 1];
+    constexpr int VW = kVec<W>;
+#pragma unroll
+    for (int k = 0; k < V / VW; ++k) {
+      if (scale) w[k] = load_pack(scale + c + k * VW, size - c - k * VW);
+      if (offset) b[k] = load_pack(offset + c + k * VW, size - c - k * VW);
+    }
+    Pack<T> out;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float v = (to_f(in[j].v[i]) - mu) * r;
+      if (scale) v *= to_f(w[i / VW].v[i % VW]);
+      if (offset) v += to_f(b[i / VW].v[i % VW]);
+      out.v[i] = from_f<T>(v);
+    }
+    store_pack(y + row * (int64_t)size + c, out, size - c);
+  }
+}
+
+// Rows too long for the registers of a block: three passes over the row, the later ones out of the caches.
+template <typename T, typename W>
+__global__ __launch_bounds__(kThreads) void norm_long_kernel(const T* __restrict__ x, int64_t x_stride, const W* __restrict__ scale,
+                                                             const W* __restrict__ offset, float eps, int64_t size,
+                                                             T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
+  constexpr int V = kVec<T>;
+  __shared__ float lds[2 * kThreads / 64];
+  int slot = 0;
+  const int64_t row = blockIdx.x;
+  const T* xr = x + row * x_stride;
+  float s[1] = {0}, q[1] = {0};
+  for (int64_t c = (int64_t)threadIdx.x * V; c < size; c += kThreads * V) {
+    const Pack<T> in = load_pack(xr + c, size - c);
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[0] += to_f(in.v[i]);
+  }
+  row_sum<kThreads, 1>(s, lds, slot);
+  const float mu = s[0] / size;
+  for (int64_t c = (int64_t)threadIdx.x * V; c < size; c += kThreads * V) {
+    const Pack<T> in = load_pack(xr + c, size - c);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float d = to_f(in.v[i]) - mu;
+      q[0] += c + i < size ? d * d : 0.0f;
+    }
+  }
+  row_sum<kThreads, 1>(q, lds, slot);
+  const float r = 1.0f / sqrtf(q[0] / size + eps);
+  if (threadIdx.x == 0) {
+    mean[row] = mu;
+    rstd[row] = r;
+  }
+  for (int64_t c = (int64_t)threadIdx.x * V; c < size; c += kThreads * V) {
+    const Pack<T> in = load_pack(xr + c, size - c);
+    Pack<T> out;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int64_t at = c + i < size ? c + i : size - 1;
+      out.v[i] = from_f<T>((to_f(in.v[i]) - mu) * r * param(scale, at, 1.0f) + param(offset, at, 0.0f));
+    }
+    store_pack(y + row * size + c, out, size - c);
+  }
+}
+
+// The backward pass.  A block's kThreads / LPR groups take rows in turn; every lane keeps the sums of its own columns of dw and
+// db in registers over all rows it sees.  At the end the groups of a block add theirs up in LDS, one after the other,
+// and the block writes one row of partial sums (or the result, when there is one block); column_sum_kernel adds those in
+// order.  No atomics: the same inputs give the same bits.
+template <typename T, typename W, int LPR, int NV>
+__global__ __launch_bounds__(kThreads) void norm_grad_kernel(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ x,
+                                                             int64_t x_stride, const float* __restrict__ mean,
+                                                             const float* __restrict__ rstd, const W* __restrict__ scale,
+                                                             int64_t rows, int size, T* __restrict__ dx, W* __restrict__ dscale,
+                                                             W* __restrict__ doffset, float* __restrict__ part) {
+  constexpr int V = kVec<T>, kRows = kThreads / LPR, E = NV * V;
+  __shared__ float lds[4 * kThreads / 64];
+  __shared__ float sums[2 * LPR * E];
+  int slot = 0;
+  const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
+  float dw[E], db[E], w[E];
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = (j * LPR + lane) * V + i;
+      dw[j * V + i] = db[j * V + i] = 0.0f;
+      w[j * V + i] = c < size ? param(scale, c, 1.0f) : 0.0f;
+    }
+  // every group of a block makes the same number of turns: they share the barriers of row_sum
+  const int64_t turns = (rows + (int64_t)gridDim.x * kRows - 1) / ((int64_t)gridDim.x * kRows);
+  for (int64_t t = 0; t < turns; ++t) {
+    const int64_t row = (t * gridDim.x + blockIdx.x) * kRows + group;
+    const bool here = row < rows;
+    const int64_t at = here ? row : 0;
+    Pack<T> px[NV], pg[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * LPR + lane) * V;
+      px[j] = load_pack(x + at * x_stride + c, here ? size - c : 0);
+      pg[j] = load_pack(dy + at * dy_stride + c, here ? size - c : 0);
+    }
+    const float mu = here ? mean[at] : 0.0f, r = here ? rstd[at] : 0.0f;
+    float s[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float g = to_f(pg[j].v[i]), xh = (to_f(px[j].v[i]) - mu) * r, gw = g * w[j * V + i];
+        dw[j * V + i] += g * xh;   // g is zero where there is no column or no row
+        db[j * V + i] += g;
+        s[0] += gw;
+        s[1] += gw * xh;
+      }
+    row_sum<LPR, 2>(s, lds, slot);
+    const float m0 = s[0] / size, m1 = s[1] / size;
+    if (here) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int c = (j * LPR + lane) * V;
+        if (c >= size) break;
+        Pack<T> out;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float xh = (to_f(px[j].v[i]) - mu) * r;
+          out.v[i] = from_f<T>(r * (to_f(pg[j].v[i]) * w[j * V + i] - m0 - xh * m1));
+        }
+        store_pack(dx + row * (int64_t)size + c, out, size - c);
+      }
+    }
+  }
+  if (dscale == nullptr && doffset == nullptr) return;
+  for (int g = 0; g < kRows; ++g) {
+    if (group == g)
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const int c = (j * LPR + lane) * V + i;
+          sums[c] = (g ? sums[c] : 0.0f) + dw[j * V + i];
+          sums[LPR * E + c] = (g ? sums[LPR * E + c] : 0.0f) + db[j * V + i];
+        }
+    __syncthreads();
+  }
+  for (int c = threadIdx.x; c < size; c += kThreads) {
+    if (gridDim.x == 1) {
+      if (dscale) dscale[c] = from_f<W>(sums[c]);
+      if (doffset) doffset[c] = from_f<W>(sums[LPR * E + c]);
+    } else {
+      part[((int64_t)blockIdx.x * 2 + 0) * size + c] = sums[c];
+      part[((int64_t)blockIdx.x * 2 + 1) * size + c] = sums[LPR * E + c];
+    }
+  }
+}
+
+// Rows too long for registers: dx with the row read twice (the second time out of the caches) ...
+template <typename T, typename W>
+__global__ __launch_bounds__(kThreads) void norm_grad_long_kernel(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ x,
+                                                                  int64_t x_stride, const float* __restrict__ mean,
+                                                                  const float* __restrict__ rstd, const W* __restrict__ scale,
+                                                                  int64_t size, T* __restrict__ dx) {
+  constexpr int V = kVec<T>;
+  __shared__ float lds[4 * kThreads / 64];
+  int slot = 0;
+  const int64_t row = blockIdx.x;
+  const float mu = mean[row], r = rstd[row];
+  float s[2] = {0, 0};
+  for (int64_t c = (int64_t)threadIdx.x * V; c < size; c += kThreads * V) {
+    const Pack<T> px = load_pack(x + row * x_stride + c, size - c), pg = load_pack(dy + row * dy_stride + c, size - c);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float gw = c + i < size ? to_f(pg.v[i]) * param(scale, c + i, 1.0f) : 0.0f;
+      s[0] += gw;
+      s[1] += gw * ((to_f(px.v[i]) - mu) * r);
+    }
+  }
+  row_sum<kThreads, 2>(s, lds, slot);
+  const float m0 = s[0] / size, m1 = s[1] / size;
+  for (int64_t c = (int64_t)threadIdx.x * V; c < size; c += kThreads * V) {
+    const Pack<T> px = load_pack(x + row * x_stride + c, size - c), pg = load_pack(dy + row * dy_stride + c, size - c);
+    Pack<T> out;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float gw = c + i < size ? to_f(pg.v[i]) * param(scale, c + i, 1.0f) : 0.0f;
+      out.v[i] = from_f<T>(r * (gw - m0 - (to_f(px.v[i]) - mu) * r * m1));
+    }
+    store_pack(dx + row * size + c, out, size - c);
+  }
+}
+
+// ... and the sums over rows by a thread per column and chunk of rows.
+template <typename T>
+__global__ __launch_bounds__(256) void norm_grad_columns_kernel(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ x,
+                                                                int64_t x_stride, const float* __restrict__ mean,
+                                                                const float* __restrict__ rstd, int64_t rows, int64_t size,
+                                                                float* __restrict__ part) {
+  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (c >= size) return;
+  const int64_t per = (rows + gridDim.y - 1) / gridDim.y, r0 = blockIdx.y * per, r1 = min(rows, r0 + per);
+  float dw = 0, db = 0;
+  for (int64_t row = r0; row < r1; ++row) {
+    const float g = to_f(dy[row * dy_stride + c]);
+    dw += g * ((to_f(x[row * x_stride + c]) - mean[row]) * rstd[row]);
+    db += g;
+  }
+  part[((int64_t)blockIdx.y * 2 + 0) * size + c] = dw;
+  part[((int64_t)blockIdx.y * 2 + 1) * size + c] = db;
+}
+
+// dscale / doffset = the partial sums added over `parts` rows.  16 columns a block, 16 threads a column; blockIdx.y: which of
+// the two.
+template <typename W>
+__global__ __launch_bounds__(256) void column_sum_kernel(const float* __restrict__ part, int64_t parts, int64_t size,
+                                                         W* __restrict__ dscale, W* __restrict__ doffset) {
+  __shared__ float lds[16][17];
+  W* out = blockIdx.y ? doffset : dscale;
+  if (out == nullptr) return;
+  const int cx = threadIdx.x % 16, py = threadIdx.x / 16;
+  const int64_t c = (int64_t)blockIdx.x * 16 + cx;
+  float s = 0;
+  if (c < size)
+    for (int64_t p = py; p < parts; p += 16) s += part[(p * 2 + blockIdx.y) * size + c];
+  lds[py][cx] = s;
+  __syncthreads();
+  if (py == 0 && c < size) {
+    s = 0;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) s += lds[k][cx];
+    out[c] = from_f<W>(s);
+  }
+}
+
+constexpr int64_t kLongest = 8192;  // values of a row that the registers of a block hold (16 a thread)
+
+// Blocks of the backward pass: every block leaves 8 * size bytes of partial sums, so there are no more than the chip holds at once,
+// and none that would see less than four turns.
+int64_t grad_blocks(int64_t rows, int64_t size, int type) {
+  if (size > kLongest) return std::min<int64_t>(64, std::max<int64_t>(1, ceil_div(rows, 32)));
+  const int64_t per = type == NNVHIP_TYPE_F32 ? 4 : 8;
+  int64_t lpr = per == 8 ? 8 : 16;
+  while (lpr < 64 && lpr * per < size) lpr *= 2;
+  while (lpr * 16 < size) lpr *= 2;
+  return std::max<int64_t>(1, std::min<int64_t>(512, ceil_div(rows, kThreads / lpr * 4)));
+}
+
+template <typename T, typename W, int LPR, int NV>
+void launch_norm(const void* x, int64_t xs, const void* scale, const void* offset, float eps, int64_t rows, int64_t size, void* y,
+                 float* mean, float* rstd, hipStream_t st) {
+  hipLaunchKernelGGL((norm_kernel<T, W, LPR, NV>), dim3((unsigned)ceil_div(rows, kThreads / LPR)), dim3(kThreads), 0, st, (const T*)x,
+                     xs, (const W*)scale, (const W*)offset, eps, rows, (int)size, (T*)y, mean, rstd);
+}
+template <typename T, typename W, int LPR, int NV>
+void launch_norm_grad(const void* dy, int64_t dys, const void* x, int64_t xs, const float* mean, const float* rstd, const void* scale,
+                      int64_t rows, int64_t size, void* dx, void* dscale, void* doffset, float* part, int64_t blocks, hipStream_t st) {
+  hipLaunchKernelGGL((norm_grad_kernel<T, W, LPR, NV>), dim3((unsigned)blocks), dim3(kThreads), 0, st, (const T*)dy, dys, (const T*)x,
+                     xs, mean, rstd, (const W*)scale, rows, (int)size, (T*)dx, (W*)dscale, (W*)doffset, part);
+}
+
+// The lanes that share a row: as few as hold it with one 16-byte load each, up to a wave; then up to 16 values a lane.
+#define NORM_BY_SIZE(CALL, T, W, ...)                                         \
+  do {                                                                        \
+    constexpr int V_ = kVec<T>;                                               \
+    if (size <= 16 * V_ / 2 && V_ == 8) CALL<T, W, 8, 1>(__VA_ARGS__);        \
+    else if (size <= 16 * V_) CALL<T, W, 16, 1>(__VA_ARGS__);                 \
+    else if (size <= 32 * V_) CALL<T, W, 32, 1>(__VA_ARGS__);                 \
+    else if (size <= 64 * V_) CALL<T, W, 64, 1>(__VA_ARGS__);                 \
+    else if (size <= 128 * V_) CALL<T, W, 64, 2>(__VA_ARGS__);                \
+    else if (size <= 1024) CALL<T, W, 64, 16 / V_>(__VA_ARGS__);              \
+    else if (size <= 2048) CALL<T, W, 128, 16 / V_>(__VA_ARGS__);             \
+    else if (size <= 4096) CALL<T, W, 256, 16 / V_>(__VA_ARGS__);             \
+    else CALL<T, W, 512, 16 / V_>(__VA_ARGS__);                               \
+  } while (0)
+
+template <typename T, typename W>
+void norm_forward(const void* x, int64_t xs, const void* scale, const void* offset, float eps, int64_t rows, int64_t size, void* y,
+                  float* mean, float* rstd, hipStream_t st) {
+  if (size > kLongest) {
+    hipLaunchKernelGGL((norm_long_kernel<T, W>), dim3((unsigned)rows), dim3(kThreads), 0, st, (const T*)x, xs, (const W*)scale,
+                       (const W*)offset, eps, size, (T*)y, mean, rstd);
+    return;
+  }
+  NORM_BY_SIZE(launch_norm, T, W, x, xs, scale, offset, eps, rows, size, y, mean, rstd, st);
+}
+
+template <typename T, typename W>
+void norm_backward(const void* dy, int64_t dys, const void* x, int64_t xs, const float* mean, const float* rstd, const void* scale,
+                   int64_t rows, int64_t size, void* dx, void* dscale, void* doffset, float* part, int type, hipStream_t st) {
+  const int64_t blocks = grad_blocks(rows, size, type);
+  if (size > kLongest) {
+    if (rows > 0) hipLaunchKernelGGL((norm_grad_long_kernel<T, W>), dim3((unsigned)rows), dim3(kThreads), 0, st, (const T*)dy, dys, (const T*)x, xs,
+                       mean, rstd, (const W*)scale, size, (T*)dx);
+    if (dscale || doffset)
+      hipLaunchKernelGGL((norm_grad_columns_kernel<T>), dim3((unsigned)ceil_div(size, 256), (unsigned)blocks), dim3(256), 0, st,
+                         (const T*)dy, dys, (const T*)x, xs, mean, rstd, rows, size, part);
+  } else {
+    NORM_BY_SIZE(launch_norm_grad, T, W, dy, dys, x, xs, mean, rstd, scale, rows, size, dx, dscale, doffset, part, blocks, st);
+    if (blocks == 1) return;
+  }
+  if (dscale || doffset)
+    hipLaunchKernelGGL((column_sum_kernel<W>), dim3((unsigned)ceil_div(size, 16), 2), dim3(256), 0, st, part, blocks, size, (W*)dscale,
+                       (W*)doffset);
+}
+
+#define NORM_BY_TYPE(CALL, ...)                                                                 \
+  do {                                                                                          \
+    const bool wide = param_type == NNVHIP_TYPE_F32;                                            \
+    if (type == NNVHIP_TYPE_F32) CALL<float, float>(__VA_ARGS__);                               \
+    else if (type == NNVHIP_TYPE_BF16 && wide) CALL<bf16_t, float>(__VA_ARGS__);                \
+    else if (type == NNVHIP_TYPE_BF16) CALL<bf16_t, bf16_t>(__VA_ARGS__);                       \
+    else if (wide) CALL<f16_t, float>(__VA_ARGS__);                                             \
+    else CALL<f16_t, f16_t>(__VA_ARGS__);                                                       \
+  } while (0)
+
+int check_norm(const char* what, int type, int param_type, int64_t rows, int64_t size) {
+  if (!known_type(type) || !(param_type == type || param_type == NNVHIP_TYPE_F32))
+    NNV_FAIL(NNVHIP_ERR_ARG, "%s: the values are f32, bf16 or f16, scale and offset of the same type or f32", what);
+  if (rows < 0 || size < 1) NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: rows of at least one value are expected", what);
+  if (rows >= (int64_t(1) << 31)) NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: too many rows", what);
+  return NNVHIP_OK;
+}
+
+}  // namespace
+}  // namespace nnvhip
+
+using namespace nnvhip;
+
+extern "C" {
+
+int nnvhip_layer_norm(nnvhip_ctx* ctx, int type, int param_type, int64_t rows, int64_t size, const void* x, int64_t x_stride,
+                      const void* scale, const void* offset, double eps, void* y, float* mean, float* rstd, void* stream) {
+  ENTER_POINT_CALL(ctx);
+  NNV_TRY(check_norm("nnvhip_layer_norm", type, param_type, rows, size));
+  if (rows == 0) return NNVHIP_OK;
+  if (!x || !y || !mean || !rstd) NNV_FAIL(NNVHIP_ERR_ARG, "nnvhip_layer_norm: null pointer");
+  NORM_BY_TYPE(norm_forward, x, x_stride, scale, offset, (float)eps, rows, size, y, mean, rstd, (hipStream_t)stream);
+  NNV_HIP_TRY(hipGetLastError());
+  return NNVHIP_OK;
+}
+
+int nnvhip_layer_norm_backward_workspace(int type, int64_t rows, int64_t size, int64_t* bytes) {
+  if (!bytes) NNV_FAIL(NNVHIP_ERR_ARG, "null pointer");
+  NNV_TRY(check_norm("nnvhip_layer_norm_backward_workspace", type, type, rows, size));
+  const int64_t blocks = grad_blocks(rows, size, type);
+  *bytes = blocks == 1 && size <= kLongest ? 0 : blocks * 2 * size * (int64_t)sizeof(float);
+  return NNVHIP_OK;
+}
+
+int nnvhip_layer_norm_backward(nnvhip_ctx* ctx, int type, int param_type, int64_t rows, int64_t size, const void* dy,
+                               int64_t dy_stride, const void* x, int64_t x_stride, const float* mean, const float* rstd,
+                               const void* scale, void* dx, void* dscale, void* doffset, void* workspace, int64_t workspace_bytes,
+                               void* stream) {
+  ENTER_POINT_CALL(ctx);
+  NNV_TRY(check_norm("nnvhip_layer_norm_backward", type, param_type, rows, size));
+  if (rows > 0 && (!dy || !x || !mean || !rstd || !dx)) NNV_FAIL(NNVHIP_ERR_ARG, "nnvhip_layer_norm_backward: null pointer");
+  int64_t need = 0;
+  NNV_TRY(nnvhip_layer_norm_backward_workspace(type, rows, size, &need));
+  if (need > workspace_bytes || (need && !workspace))
+    NNV_FAIL(NNVHIP_ERR_ARG, "nnvhip_layer_norm_backward: a workspace of %lld bytes is needed", (long long)need);
+  if (rows == 0 && !dscale && !doffset) return NNVHIP_OK;
+  NORM_BY_TYPE(norm_backward, dy, dy_stride, x, x_stride, mean, rstd, scale, rows, size, dx, dscale, doffset, (float*)workspace, type,
+               (hipStream_t)stream);
+  NNV_HIP_TRY(hipGetLastError());
+  return NNVHIP_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,362 @@
+"""Operators on points and gradients: layer normalization, attention to another sequence's states, and the global norm of
+a list of gradients with its clipping.
+
+Sets are what this package reaches; these are what a program runs beside them: a network with such layers is evaluated on
+points of the input box, the gradient of a specification's margin is followed back to the input (see
+``nnv_amd.falsify``) or to the weights, and the step is bounded.  The reference's layers evaluate points as well (e.g.
+nn/layers/BatchNormalizationLayer.m:118-229); it has no gradients, and no counterpart of the two layers here in its reach path.
+
+All arguments and results are torch tensors on the context's GPU: f32, bf16 or f16.  A call is queued on torch's current
+stream of that device, like torch's own operations, and returns without waiting; what it needs besides its results comes from torch's
+allocator.  The layers' sums and statistics are f32 (the gradient norm's squares f64) and each result is rounded once.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import functools
+import struct
+
+import torch
+
+from ._lib import check, default_context
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_INT64 = C.c_int64
+
+
+def _enter(what, ctx, first, *others):
+    """(context, its library, device, stream) for tensors that have to be on that context's GPU."""
+    if not isinstance(first, torch.Tensor):
+        raise TypeError("%s: expected a torch tensor, got %s" % (what, type(first).__name__))
+    device = first.device
+    if device.type != "cuda":
+        raise ValueError("%s: the tensors must be on the GPU" % what)
+    for t in others:
+        if t is not None:
+            if not isinstance(t, torch.Tensor):
+                raise TypeError("%s: expected a torch tensor, got %s" % (what, type(t).__name__))
+            if t.device != device:
+                raise ValueError("%s: the tensors must be on one GPU" % what)
+    ctx = ctx or default_context()
+    if device.index != ctx.device:
+        raise ValueError("%s: the tensors are on GPU %d, the context is GPU %d's" % (what, device.index, ctx.device))
+    return ctx, ctx.lib, device, torch.cuda.current_stream(device).cuda_stream
+
+
+def _type(what, t):
+    k = _TYPES.get(t.dtype)
+    if k is None:
+        raise ValueError("%s: the values must be float32, bfloat16 or float16, not %s" % (what, t.dtype))
+    return k
+
+
+# ---- layer normalization ----------------------------------------------------------------------
+
+
+def _as_rows(x):
+    """(tensor, rows, stride of its rows): x as rows of its last dimension, copied only where they are not evenly spaced."""
+    size = x.shape[-1]
+    if x.is_contiguous():
+        return x, (x.numel() // size if size else 0), size
+    if x.stride(-1) == 1 or size == 1:
+        try:
+            rows = x.view(-1, size)
+            return rows, rows.shape[0], rows.stride(0)
+        except RuntimeError:
+            pass
+    x = x.contiguous()
+    return x, x.numel() // size, size
+
+
+def _norm_params(what, x, scale, offset):
+    t = _type(what, x)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("%s: rows of at least one value are expected" % what)
+    w = t
+    for p in (scale, offset):
+        if p is not None:
+            if p.dim() != 1 or p.shape[0] != x.shape[-1]:
+                raise ValueError("%s: scale and offset have one value per channel (%d), not the shape %s" % (what, x.shape[-1], tuple(p.shape)))
+            w = _type(what, p)
+            if w not in (t, 0):
+                raise ValueError("%s: scale and offset have the type of the values, or float32" % what)
+    if scale is not None and offset is not None and scale.dtype != offset.dtype:
+        raise ValueError("%s: scale and offset must have the same type" % what)
+    return t, w
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def layer_norm(x, scale=None, offset=None, epsilon=1e-5, ctx=None):
+    """y = (x - mean) / sqrt(var + epsilon) * scale + offset over the last dimension of x.
+
+    Returns (y, mean, rstd): y in x's shape and type, the statistics f32, one per row, in x's leading shape;
+    layer_norm_backward takes them.  scale and offset: vectors of x's type or f32, or None."""
+    ctx, lib, device, stream = _enter("layer_norm", ctx, x, scale, offset)
+    t, w = _norm_params("layer_norm", x, scale, offset)
+    if not epsilon >= 0:
+        raise ValueError("layer_norm: epsilon must not be negative")
+    lead, size = x.shape[:-1], x.shape[-1]
+    scale = scale if scale is None else scale.contiguous()
+    offset = offset if offset is None else offset.contiguous()
+    rows_of, rows, stride = _as_rows(x)
+    y = torch.empty(x.shape, dtype=x.dtype, device=device)
+    mean = torch.empty(lead, dtype=torch.float32, device=device)
+    rstd = torch.empty(lead, dtype=torch.float32, device=device)
+    check(lib.nnvhip_layer_norm(ctx.handle, t, w, rows, size, rows_of.data_ptr(), stride, _ptr(scale), _ptr(offset), epsilon,
+                                y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), stream))
+    return y, mean, rstd
+
+
+@functools.lru_cache(maxsize=256)
+def _norm_workspace(lib, t, rows, size):
+    n = _INT64()
+    check(lib.nnvhip_layer_norm_backward_workspace(t, rows, size, C.byref(n)))
+    return n.value
+
+
+def layer_norm_backward(dy, x, mean, rstd, scale=None, ctx=None):
+    """The gradients of layer_norm: (dx, dscale, doffset) from that of its result and its statistics.
+
+    dx has x's type, dscale and doffset the type of scale (x's if scale is None)."""
+    what = "layer_norm_backward"
+    ctx, lib, device, stream = _enter(what, ctx, x, dy, mean, rstd, scale)
+    t, w = _norm_params(what, x, scale, None)
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError("%s: dy must have the shape and type of x" % what)
+    lead, size = x.shape[:-1], x.shape[-1]
+    for s in (mean, rstd):
+        if s.shape != lead or s.dtype != torch.float32:
+            raise ValueError("%s: mean and rstd must be what layer_norm returned" % what)
+    scale = scale if scale is None else scale.contiguous()
+    mean, rstd = mean.contiguous(), rstd.contiguous()
+    xr, rows, xs = _as_rows(x)
+    gr, _, gs = _as_rows(dy)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=device)
+    grads = torch.empty((2, size), dtype=x.dtype if scale is None else scale.dtype, device=device)
+    dscale, doffset = grads.unbind(0)
+    need = _norm_workspace(lib, t, rows, size)
+    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    check(lib.nnvhip_layer_norm_backward(ctx.handle, t, w, rows, size, gr.data_ptr(), gs, xr.data_ptr(), xs, mean.data_ptr(),
+                                         rstd.data_ptr(), _ptr(scale), dx.data_ptr(), dscale.data_ptr(), doffset.data_ptr(),
+                                         _ptr(work), need, stream))
+    return dx, dscale, doffset
+
+
+# ---- attention to another sequence's states ---------------------------------------------------------
+
+# struct nnvhip_attention
+_ATTENTION = struct.Struct("=7qd3Q9qQQ2qQQQ3q3Q")
+
+
+def _dense_values(t):
+    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
+
+
+def _attention_sizes(what, q, k, v, key_lengths, key_mask):
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError("%s: q, k and v are batch x tokens x heads x head" % what)
+    if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise ValueError("%s: q %s, k %s and v %s do not fit together" % (what, tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("%s: q, k and v must have one type" % what)
+    batch, queries, heads, head = q.shape
+    keys, kv_heads = k.shape[1], k.shape[2]
+    if kv_heads < 1 or heads < 1 or heads % kv_heads:
+        raise ValueError("%s: the number of heads must be a multiple of the number of key/value heads" % what)
+    if key_lengths is not None and (key_lengths.shape != (batch,) or key_lengths.dtype not in (torch.int32, torch.int64)):
+        raise ValueError("%s: key_lengths is one whole number per sequence" % what)
+    if key_mask is not None and (key_mask.shape != (batch, keys) or key_mask.dtype not in (torch.bool, torch.uint8)):
+        raise ValueError("%s: key_mask is one truth value per sequence and key" % what)
+    return _type(what, q), batch, queries, keys, heads, kv_heads, head
+
+
+@functools.lru_cache(maxsize=256)
+def _attention_workspace(lib, backward, *sizes):
+    n = _INT64()
+    d = _ATTENTION.pack(*sizes, 0.0, *[0] * 25)
+    fn = lib.nnvhip_cross_attention_backward_workspace if backward else lib.nnvhip_cross_attention_workspace
+    check(fn(d, C.byref(n)))
+    return n.value
+
+
+def _mask_args(key_lengths, key_mask):
+    lengths = None if key_lengths is None else key_lengths.to(torch.int32).contiguous()
+    return lengths, (key_mask.stride() if key_mask is not None else (0, 0))
+
+
+def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None, ctx=None):
+    """softmax(scale * q k^T) v for queries of one sequence and keys and values of another.
+
+    q: batch x queries x heads x head, k and v: batch x keys x kv_heads x head, any strides; consecutive heads / kv_heads
+    heads share keys and values; head is 128 at most.  key_lengths (one number per sequence) and key_mask (truth values,
+    batch x keys) say which keys count; what the others hold is of no effect.  scale: 1 / sqrt(head) if None.
+
+    Returns (o, lse): o in q's shape and type and the logarithm of the softmax's sums, batch x heads x queries, f32.
+    Where no key counts o is zero and lse -inf."""
+    what = "cross_attention"
+    ctx, lib, device, stream = _enter(what, ctx, q, k, v, key_lengths, key_mask)
+    sizes = _attention_sizes(what, q, k, v, key_lengths, key_mask)
+    q, k, v = _dense_values(q), _dense_values(k), _dense_values(v)
+    lengths, mask_stride = _mask_args(key_lengths, key_mask)
+    o = torch.empty(q.shape, dtype=q.dtype, device=device)
+    lse = torch.empty((sizes[1], sizes[4], sizes[2]), dtype=torch.float32, device=device)
+    d = _ATTENTION.pack(*sizes, sizes[6] ** -0.5 if scale is None else scale, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                        *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], _ptr(lengths) or 0, _ptr(key_mask) or 0,
+                        *mask_stride, o.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, 0, 0, 0)
+    need = _attention_workspace(lib, False, *sizes)
+    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    check(lib.nnvhip_cross_attention(ctx.handle, d, _ptr(work), need, stream))
+    return o, lse
+
+
+def cross_attention_backward(do, q, k, v, o, lse, key_lengths=None, key_mask=None, scale=None, ctx=None):
+    """The gradients (dq, dk, dv) of cross_attention, from that of o and from what the forward call returned; the other
+    arguments are that call's.  Rows without keys and keys that do not count get zero."""
+    what = "cross_attention_backward"
+    ctx, lib, device, stream = _enter(what, ctx, q, k, v, key_lengths, key_mask, do, o, lse)
+    sizes = _attention_sizes(what, q, k, v, key_lengths, key_mask)
+    if do.shape != q.shape or do.dtype != q.dtype or o.shape != q.shape or o.dtype != q.dtype:
+        raise ValueError("%s: do and o must have the shape and type of q" % what)
+    if lse.shape != (sizes[1], sizes[4], sizes[2]) or lse.dtype != torch.float32:
+        raise ValueError("%s: lse must be what cross_attention returned" % what)
+    q, k, v, do = _dense_values(q), _dense_values(k), _dense_values(v), _dense_values(do)
+    o, lse = o.contiguous(), lse.contiguous()
+    lengths, mask_stride = _mask_args(key_lengths, key_mask)
+    dq = torch.empty(q.shape, dtype=q.dtype, device=device)
+    dk = torch.empty(k.shape, dtype=q.dtype, device=device)
+    dv = torch.empty(k.shape, dtype=q.dtype, device=device)
+    d = _ATTENTION.pack(*sizes, sizes[6] ** -0.5 if scale is None else scale, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                        *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], _ptr(lengths) or 0, _ptr(key_mask) or 0,
+                        *mask_stride, o.data_ptr(), lse.data_ptr(), do.data_ptr(), *do.stride()[:3], dq.data_ptr(),
+                        dk.data_ptr(), dv.data_ptr())
+    need = _attention_workspace(lib, True, *sizes)
+    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    check(lib.nnvhip_cross_attention_backward(ctx.handle, d, _ptr(work), need, stream))
+    return dq, dk, dv
+
+
+# ---- the norm of all gradients, and clipping ---------------------------------------------------------
+
+
+@functools.lru_cache(maxsize=64)
+def _clip_workspace(lib, count):
+    n = _INT64()
+    check(lib.nnvhip_clip_gradients_workspace(count, C.byref(n)))
+    return n.value
+
+
+def clip_gradients(gradients, threshold, out=None, ctx=None):
+    """The tensors of a list scaled so that the norm over all of them is at most threshold:
+    out[k] = gradients[k] * (norm > threshold ? threshold / norm : 1), norm = sqrt(sum of all squares).
+
+    Returns (the scaled tensors, norm as an f32 tensor of no dimensions); the norm stays on the GPU.  out: tensors of the same shapes
+    and types to write to, e.g. the gradients themselves; new ones if None.  A norm that is infinite or no number is
+    used as it is: the first gives zeros and NaNs, the second leaves the gradients as they are."""
+    what = "clip_gradients"
+    gradients = list(gradients)
+    if not threshold > 0:
+        raise ValueError("%s: the threshold must be positive" % what)
+    if not gradients:
+        ctx = ctx or default_context()
+        return [], torch.zeros((), dtype=torch.float32, device=torch.device("cuda", ctx.device))
+    ctx, lib, device, stream = _enter(what, ctx, *gradients)
+    types = [_type(what, g) for g in gradients]
+    dense = [g if g.is_contiguous() else g.contiguous() for g in gradients]
+    back = None
+    if out is None:
+        out = result = [torch.empty(g.shape, dtype=g.dtype, device=device) for g in gradients]
+    else:
+        out = list(out)
+        if len(out) != len(gradients):
+            raise ValueError("%s: %d gradients and %d tensors to write to" % (what, len(gradients), len(out)))
+        for g, y in zip(gradients, out):
+            if not isinstance(y, torch.Tensor) or y.shape != g.shape or y.dtype != g.dtype or y.device != device:
+                raise ValueError("%s: out must have the shapes, types and device of the gradients" % what)
+        result = out
+        if not all(y.is_contiguous() for y in out):   # through dense tensors, copied back below
+            back = [y for y in out]
+            out = [y if y.is_contiguous() else torch.empty(y.shape, dtype=y.dtype, device=device) for y in out]
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    count = len(gradients)
+    need = _clip_workspace(lib, count)
+    work = torch.empty(need, dtype=torch.uint8, device=device)
+    check(lib.nnvhip_clip_gradients(ctx.handle, count, struct.pack("=%di" % count, *types),
+                                    struct.pack("=%dq" % count, *[g.numel() for g in dense]),
+                                    struct.pack("=%dQ" % count, *[g.data_ptr() for g in dense]),
+                                    struct.pack("=%dQ" % count, *[y.data_ptr() for y in out]), threshold, norm.data_ptr(),
+                                    work.data_ptr(), need, stream))
+    if back is not None:
+        for y, t in zip(back, out):
+            if y is not t:
+                y.copy_(t)
+    return result, norm
+
+
+# ---- layers -------------------------------------------------------------------------------------
+
+
+class LayerNormalizationLayer:
+    """A layer normalization over the channels (the last dimension), with the properties of the reference's normalization layers
+    (name/value constructor, nn/layers/BatchNormalizationLayer.m:33-83).  Scale and Offset are device tensors or None."""
+
+    def __init__(self, **kw):
+        self.Name = kw.get("Name", "LayerNormalizationLayer")
+        self.Scale = kw.get("Scale")
+        self.Offset = kw.get("Offset")
+        self.Epsilon = float(kw.get("Epsilon", 0.00001))
+        known = [p for p in (self.Scale, self.Offset) if p is not None]
+        self.NumChannels = kw.get("NumChannels") or (known[0].shape[0] if known else None)
+
+    def _check(self, x):
+        if self.NumChannels is not None and x.shape[-1] != self.NumChannels:
+            raise ValueError("Inconsistent number of channels between the input and the layer normalization")
+
+    def evaluate(self, x):
+        return self.forward(x)[0]
+
+    def forward(self, x):
+        """(y, what backward takes)."""
+        self._check(x)
+        y, mean, rstd = layer_norm(x, self.Scale, self.Offset, self.Epsilon)
+        return y, (x, mean, rstd)
+
+    def backward(self, dy, saved):
+        """(dx, [dScale, dOffset])."""
+        x, mean, rstd = saved
+        dx, dscale, doffset = layer_norm_backward(dy, x, mean, rstd, self.Scale)
+        return dx, [dscale, doffset]
+
+
+class CrossAttentionLayer:
+    """Attention of NumHeads heads to another sequence's keys and values (NumKeyValueHeads of them, NumHeads if not given);
+    inputs are batch x tokens x channels, the channels of all heads side by side."""
+
+    def __init__(self, NumHeads, NumKeyValueHeads=None, Scale=None, Name="CrossAttentionLayer"):
+        self.Name = Name
+        self.NumHeads = int(NumHeads)
+        self.NumKeyValueHeads = int(NumKeyValueHeads or NumHeads)
+        self.Scale = Scale
+
+    def _heads(self, x, heads):
+        if x.dim() != 3 or x.shape[2] % heads:
+            raise ValueError("The channels of the input must be a multiple of the number of heads")
+        return x.unflatten(2, (heads, x.shape[2] // heads))
+
+    def evaluate(self, q, k, v, key_lengths=None, key_mask=None):
+        return self.forward(q, k, v, key_lengths, key_mask)[0]
+
+    def forward(self, q, k, v, key_lengths=None, key_mask=None):
+        """(o, what backward takes)."""
+        q = self._heads(q, self.NumHeads)
+        k, v = (self._heads(x, self.NumKeyValueHeads) for x in (k, v))
+        o, lse = cross_attention(q, k, v, key_lengths, key_mask, self.Scale)
+        return o.flatten(2), (q, k, v, o, lse, key_lengths, key_mask)
+
+    def backward(self, do, saved):
+        """(dq, dk, dv)."""
+        q, k, v, o, lse, key_lengths, key_mask = saved
+        return tuple(g.flatten(2) for g in cross_attention_backward(self._heads(do, self.NumHeads), q, k, v, o, lse, key_lengths,
+                                                                    key_mask, self.Scale))
