@@ -2,7 +2,7 @@
 //
 // The products run on the f32 matrix instructions (v_mfma_f32_32x32x2_f32, 157 TFLOP/s at best), whatever the type of the
 // tensors: f32 tensors keep f32 results, and tensors of 16 bits lose nothing but their final rounding.
-#include "points_attend.h"
+#include "points_attend16.h"
 
 #include <algorithm>
 
@@ -211,28 +211,29 @@ __global__ __launch_bounds__(256) void join_kernel(const AttendArgs a) {
   if (lane == 0) a.lse[flat] = total == 0.0f ? -INFINITY : base + log2f(total) * kLn2;
 }
 
-// How a forward call is cut: few rows for each head's keys (single tokens) or tiles of 128 rows, and over how many blocks the
-// keys are split.
+// How a forward call is cut: few rows for each head's keys (single tokens) or tiles of many rows (128, or 256 where the 16-bit
+// kernels take the call), and over how many blocks the keys are split.
 struct Cut {
   bool few;
   int row_tiles, splits;
 };
-Cut cut_of(const AttendArgs& a) {
+Cut cut_of(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys, bool by16) {
   Cut c;
-  c.few = a.rows <= kWaveRows;
-  c.row_tiles = (int)ceil_div(a.rows, c.few ? kWaveRows : 128);
-  const int64_t blocks = (int64_t)a.batch * a.kv_heads * c.row_tiles;
-  c.splits = split_of(blocks, ceil_div(a.keys, kWaveRows), c.few ? 8 : 4, 512);
+  c.few = rows <= kWaveRows;
+  c.row_tiles = (int)ceil_div(rows, c.few ? kWaveRows : by16 ? 256 : 128);
+  c.splits = split_of(batch * kv_heads * c.row_tiles, ceil_div(keys, kWaveRows), c.few ? 8 : 4, 512);
   return c;
 }
 
 template <typename T, int DP>
-void launch_attend(const AttendArgs& a, const Cut& c, hipStream_t st) {
-  const dim3 grid((unsigned)((int64_t)a.batch * a.kv_heads * c.row_tiles * c.splits));
-  if (c.few) hipLaunchKernelGGL((attend_kernel<T, DP, true>), grid, dim3(256), 0, st, a);
+void launch_attend(const AttendArgs& a, bool few, hipStream_t st) {
+  const dim3 grid((unsigned)((int64_t)a.batch * a.kv_heads * a.row_tiles * a.splits));
+  if (few) hipLaunchKernelGGL((attend_kernel<T, DP, true>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((attend_kernel<T, DP, false>), grid, dim3(256), 0, st, a);
-  if (c.splits > 1)
-    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)ceil_div((int64_t)a.batch * a.kv_heads * a.rows, 4)), dim3(256), 0, st, a);
+}
+template <typename T, int>
+void launch_join(const AttendArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)ceil_div((int64_t)a.batch * a.kv_heads * a.rows, 4)), dim3(256), 0, st, a);
 }
 
 // strides of the last tokens' rows have to be addressable, the sizes have to fit the kernels' indexes
@@ -294,13 +295,10 @@ extern "C" {
 int nnvhip_cross_attention_workspace(const nnvhip_attention* d, int64_t* bytes) {
   if (!d || !bytes) NNV_FAIL(NNVHIP_ERR_ARG, "null pointer");
   NNV_TRY(check_sizes("nnvhip_cross_attention_workspace", d));
-  AttendArgs a{};
-  a.batch = (int)d->batch;
-  a.kv_heads = (int)d->kv_heads;
-  a.keys = (int)d->keys;
-  a.rows = d->queries * (d->heads / d->kv_heads);
-  const Cut c = cut_of(a);
-  *bytes = c.splits > 1 ? (int64_t)c.splits * d->batch * d->heads * d->queries * (d->head + 1) * (int64_t)sizeof(float) : 0;
+  int splits = 1;   // whichever kernels the alignment of the tensors lets take the call
+  for (const bool by16 : {false, true})
+    splits = std::max(splits, cut_of(d->batch, d->kv_heads, d->queries * (d->heads / d->kv_heads), d->keys, by16).splits);
+  *bytes = splits > 1 ? (int64_t)splits * d->batch * d->heads * d->queries * (d->head + 1) * (int64_t)sizeof(float) : 0;
   return NNVHIP_OK;
 }
 
@@ -313,12 +311,15 @@ int nnvhip_cross_attention(nnvhip_ctx* ctx, const nnvhip_attention* d, void* wor
   if (need > workspace_bytes || (need && !workspace))
     NNV_FAIL(NNVHIP_ERR_ARG, "nnvhip_cross_attention: a workspace of %lld bytes is needed", (long long)need);
   if (a.batch == 0 || a.rows == 0) return NNVHIP_OK;
-  const Cut c = cut_of(a);
+  const bool by16 = attend16_takes(a, (int)d->type);
+  const Cut c = cut_of(a.batch, a.kv_heads, a.rows, a.keys, by16);
   a.row_tiles = c.row_tiles;
   a.splits = c.splits;
   a.part = static_cast<float*>(workspace);
   a.part_lse = c.splits > 1 ? a.part + (int64_t)c.splits * a.batch * a.kv_heads * a.rows * a.head : nullptr;
-  ATTEND_BY_TYPE(d->type, launch_attend, a, c, (hipStream_t)stream);
+  if (by16) launch_attend16(a, (int)d->type, c.few, (hipStream_t)stream);
+  else ATTEND_BY_TYPE(d->type, launch_attend, a, c.few, (hipStream_t)stream);
+  if (c.splits > 1) ATTEND_BY_TYPE(d->type, launch_join, a, (hipStream_t)stream);
   NNV_HIP_TRY(hipGetLastError());
   return NNVHIP_OK;
 }

@@ -1,0 +1,140 @@
+// Attention of points in 16 bits: tiles of rows in LDS, as the bf16 / f16 matrix instructions (32x32x16) take them.
+#pragma once
+#include "lds_dma.h"
+#include "points_attend.h"
+
+namespace nnvhip {
+
+template <typename T>
+struct Half8;
+template <>
+struct Half8<bf16_t> {
+  typedef bf16_t t __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ float16_t mfma(t a, t b, float16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Half8<f16_t> {
+  typedef f16_t t __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ float16_t mfma(t a, t b, float16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <typename T>
+using half8 = typename Half8<T>::t;
+
+typedef short short4_t __attribute__((ext_vector_type(4)));
+
+// ROWS rows of DP values in LDS, row after row, filled by 16-byte transfers from global memory (the head size is a multiple of
+// 8, so a transfer holds values of one row only; those past the head size are zeroed once and never written again).
+//
+// Two readers: over_head takes 16 bytes of 32 rows at one column, over_rows (through the transposing read) 64 bytes of 4 rows
+// at a time.  Both meet every bank once if the 16-byte pieces of a row are exchanged by
+//   piece ^ (row / 4 % 4 + 4 (row % 4 or what of it moves whole groups of four pieces within the row)):
+// four consecutive rows then have the same 64-byte group in different quarters of the 256 bytes that the banks span, and rows 4
+// apart have the same piece in different places of a group.  (Rows of 32 and 96 values do the first by themselves.)
+template <typename T, int DP>
+struct Rows16 {
+  static constexpr int PIECES = DP / 8;
+  static __device__ __forceinline__ int place(int row) {
+    const int low = (row >> 2) & 3;
+    if constexpr (DP == 128) return (row & 3) << 2 | low;
+    if constexpr (DP == 64) return (row >> 1 & 1) << 2 | low;
+    return low;
+  }
+  static __device__ __forceinline__ int at(int row, int piece) { return row * DP + ((piece ^ place(row)) << 3); }
+};
+
+// Left operand of a product over the head: rows first .. first + 31, values 16 c .. 16 c + 15 (lane: row first + col, 8 of them).
+template <typename T, int DP>
+__device__ __forceinline__ half8<T> rows_operand(const T* tile, int first, int c, int col, int h) {
+  half8<T> r;
+  __builtin_memcpy(&r, tile + first * DP + Rows16<T, DP>::at(col, 2 * c + h), 16);
+  return r;
+}
+// Left operand of a product over rows: values 32 d .. 32 d + 31 (lane: value 32 d + col) of the 16 rows first + product_row(0..7, h) of
+// the lane's half: the order in which a product's registers 0-7 (or 8-15, for the 16 rows behind) hold them.
+// ds_read_b64_tr_b16 gives lane i of 16 the i-th value of four rows whose 16 values the lanes 4 j .. 4 j + 3 point to.
+template <typename T, int DP>
+__device__ __forceinline__ half8<T> columns_operand(const T* tile, int first, int d, int lane) {
+  const int h = lane >> 5, j = (lane >> 2) & 3, piece = 4 * d + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+  typedef __attribute__((address_space(3))) short4_t* LdsPtr;
+  short4_t r[2];
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const T* p = tile + first * DP + Rows16<T, DP>::at(8 * half + 4 * h + j, piece) + (lane & 1) * 4;
+    r[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(const __attribute__((address_space(3))) void*)p);
+  }
+  half8<T> f;
+  __builtin_memcpy(&f, r, 16);
+  return f;
+}
+
+// Eight f32 of a product as the right operand of the next one, each rounded to T.
+template <typename T>
+__device__ __forceinline__ half8<T> round8(const float16_t& s, int first) {
+  half8<T> r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = (T)s[first + i];
+  return r;
+}
+
+// The transfers a wave makes for a pair of tiles (a and b) of ROWS rows each: COUNT of 1024 bytes, shared out over WAVES waves.
+template <typename T, int DP, int ROWS, int WAVES>
+struct PairLoad {
+  static constexpr int PIECES = DP / 8, PER_TILE = ROWS * PIECES / 64, COUNT = 2 * PER_TILE / WAVES;
+  static_assert(2 * PER_TILE % WAVES == 0 && ROWS * PIECES % 64 == 0, "transfers come out even");
+  int row[COUNT], value[COUNT];   // of this lane: row of the tile, first value (or -1: behind the head size)
+  // transfer i of this wave: which tile, and where in it
+  __device__ __forceinline__ static int index(int i, int wave) { return i * WAVES + wave; }
+  __device__ __forceinline__ void init(int wave, int lane, int head) {
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) {
+      const int at = index(i, wave) % PER_TILE * 64 + lane;
+      row[i] = at / PIECES;
+      const int piece = at % PIECES ^ Rows16<T, DP>::place(row[i]);
+      value[i] = piece * 8 < head ? piece * 8 : -1;
+    }
+  }
+  // a(row), b(row): pointers to the rows of the tiles; lds: LDS address of tile a, tile b behind it
+  template <class A, class B>
+  __device__ __forceinline__ void issue(A a, B b, unsigned lds, int wave) const {
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) {
+      const int at = index(i, wave);
+      const T* p = at < PER_TILE ? a(row[i]) : b(row[i]);
+      if (value[i] >= 0) lds_dma16_at((const double*)(p + value[i]), __builtin_amdgcn_readfirstlane(lds + at * 1024));
+    }
+  }
+};
+
+// the larger of a value and that of lane l ^ 32
+__device__ __forceinline__ float max_of_halves(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+  return fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
+}
+__device__ __forceinline__ float sum_of_halves(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+  return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+}
+// max(a, b, c) without the extra instructions that make fmaxf quiet signalling NaNs
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+// Block `id` of `total` in an order in which each of the 8 XCDs gets consecutive ones (blocks are dealt to the XCDs in turn):
+// blocks that read the same keys then find them in one L2.
+__device__ __forceinline__ int64_t xcd_order(int64_t id, int64_t total) {
+  const int64_t x = id % 8, base = total / 8, more = total % 8;
+  return x * base + min(x, more) + id / 8;
+}
+
+// A head's row can be moved in 16-byte pieces: head size, strides and start are multiples of 8 values.
+inline bool by_pieces(const TokenView& t, int64_t head) {
+  return head % 8 == 0 && t.b % 8 == 0 && t.t % 8 == 0 && t.h % 8 == 0 && (uintptr_t)t.p % 16 == 0;
+}
+
+// What a launch of the 16-bit kernels for the forward pass needs of the caller; false: the general ones take the call.
+bool attend16_takes(const AttendArgs& a, int type);
+void launch_attend16(const AttendArgs& a, int type, bool few, hipStream_t st);
+
+}  // namespace nnvhip
