@@ -133,8 +133,11 @@ inline bool by_pieces(const TokenView& t, int64_t head) {
   return head % 8 == 0 && t.b % 8 == 0 && t.t % 8 == 0 && t.h % 8 == 0 && (uintptr_t)t.p % 16 == 0;
 }
 
-// What a launch of the 16-bit kernels for the forward pass needs of the caller; false: the general ones take the call.
+// Whether the 16-bit kernels take a call; else the general ones do.
 bool attend16_takes(const AttendArgs& a, int type);
+bool grad16_takes(const AttendArgs& a, int type);
 void launch_attend16(const AttendArgs& a, int type, bool few, hipStream_t st);
+void launch_query_grad16(const AttendArgs& a, hipStream_t st);   // tiles of 256 rows
+void launch_key_grad16(const AttendArgs& a, hipStream_t st);     // tiles of 128 keys
 
 }  // namespace nnvhip

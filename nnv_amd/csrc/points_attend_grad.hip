@@ -4,7 +4,7 @@
 // shares them).  Both form S and dP again: seven products instead of the five that one kernel would need, but every
 // gradient is a sum in the registers of one wave, in a fixed order, with no atomics.  What both need of a row besides, D = rowsum(do o),
 // is formed first.  Where one axis gives too few blocks for the chip, the other is split, and sum_kernel adds the parts in order.
-#include "points_attend.h"
+#include "points_attend16.h"
 
 #pragma clang fp contract(fast)
 
@@ -245,9 +245,9 @@ struct GradCut {
   int row_tiles, key_tiles, query_splits, key_splits;
   int64_t delta, part;   // floats of the workspace
 };
-GradCut grad_cut(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys, int64_t head) {
+GradCut grad_cut(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys, int64_t head, bool by16) {
   GradCut c;
-  c.row_tiles = (int)ceil_div(rows, 128);
+  c.row_tiles = (int)ceil_div(rows, by16 ? 256 : 128);
   c.key_tiles = (int)ceil_div(keys, 128);
   c.query_splits = split_of(batch * kv_heads * c.row_tiles, ceil_div(keys, kWaveRows), 4, 512);
   c.key_splits = split_of(batch * kv_heads * c.key_tiles, ceil_div(rows, kWaveRows), 4, 512);
@@ -259,19 +259,21 @@ GradCut grad_cut(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys, in
 }
 
 template <typename T, int DP>
-void launch_grad(AttendArgs a, const GradCut& c, hipStream_t st) {
+void launch_grad(AttendArgs a, const GradCut& c, bool by16, hipStream_t st) {
   const int64_t heads = (int64_t)a.batch * a.kv_heads;
   if (a.rows > 0) {
     hipLaunchKernelGGL((delta_kernel<T>), dim3((unsigned)ceil_div(heads * a.rows, 16)), dim3(256), 0, st, a);
     a.row_tiles = c.row_tiles;
     a.splits = c.query_splits;
-    hipLaunchKernelGGL((query_grad_kernel<T, DP>), dim3((unsigned)(heads * c.row_tiles * a.splits)), dim3(256), 0, st, a);
+    if (by16) launch_query_grad16(a, st);
+    else hipLaunchKernelGGL((query_grad_kernel<T, DP>), dim3((unsigned)(heads * c.row_tiles * a.splits)), dim3(256), 0, st, a);
     if (a.splits > 1) hipLaunchKernelGGL((sum_rows_kernel<T>), dim3((unsigned)ceil_div(heads * a.rows, 4)), dim3(256), 0, st, a, (T*)a.dq);
   }
   if (a.keys > 0) {
     a.key_tiles = c.key_tiles;
     a.splits = c.key_splits;
-    hipLaunchKernelGGL((key_grad_kernel<T, DP>), dim3((unsigned)(heads * c.key_tiles * a.splits)), dim3(256), 0, st, a);
+    if (by16) launch_key_grad16(a, st);
+    else hipLaunchKernelGGL((key_grad_kernel<T, DP>), dim3((unsigned)(heads * c.key_tiles * a.splits)), dim3(256), 0, st, a);
     if (a.splits > 1) {
       const int64_t n = heads * a.keys * a.head;
       hipLaunchKernelGGL((sum_kernel<T>), dim3((unsigned)ceil_div(n, 256)), dim3(256), 0, st, a.part, a.splits, n, (T*)a.dk);
@@ -291,8 +293,11 @@ int nnvhip_cross_attention_backward_workspace(const nnvhip_attention* d, int64_t
   int64_t forward = 0;
   NNV_TRY(nnvhip_cross_attention_workspace(d, &forward));   // checks the sizes
   if (!bytes) NNV_FAIL(NNVHIP_ERR_ARG, "null pointer");
-  const GradCut c = grad_cut(d->batch, d->kv_heads, d->queries * (d->heads / d->kv_heads), d->keys, d->head);
-  *bytes = (c.delta + c.part) * (int64_t)sizeof(float);
+  *bytes = 0;   // whichever kernels the alignment of the tensors lets take the call
+  for (const bool by16 : {false, true}) {
+    const GradCut c = grad_cut(d->batch, d->kv_heads, d->queries * (d->heads / d->kv_heads), d->keys, d->head, by16);
+    *bytes = std::max(*bytes, (c.delta + c.part) * (int64_t)sizeof(float));
+  }
   return NNVHIP_OK;
 }
 
@@ -305,10 +310,11 @@ int nnvhip_cross_attention_backward(nnvhip_ctx* ctx, const nnvhip_attention* d, 
   if (need > workspace_bytes || (need && !workspace))
     NNV_FAIL(NNVHIP_ERR_ARG, "nnvhip_cross_attention_backward: a workspace of %lld bytes is needed", (long long)need);
   if (a.batch == 0) return NNVHIP_OK;
-  const GradCut c = grad_cut(a.batch, a.kv_heads, a.rows, a.keys, a.head);
+  const bool by16 = grad16_takes(a, (int)d->type);
+  const GradCut c = grad_cut(a.batch, a.kv_heads, a.rows, a.keys, a.head, by16);
   a.delta = static_cast<float*>(workspace);
   a.part = a.delta + c.delta;
-  ATTEND_BY_TYPE(d->type, launch_grad, a, c, (hipStream_t)stream);
+  ATTEND_BY_TYPE(d->type, launch_grad, a, c, by16, (hipStream_t)stream);
   NNV_HIP_TRY(hipGetLastError());
   return NNVHIP_OK;
 }
