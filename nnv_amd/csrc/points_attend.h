@@ -51,6 +51,13 @@ __device__ __forceinline__ int keys_that_count(const AttendArgs& a, int b) {
 __device__ __forceinline__ bool key_counts(const AttendArgs& a, int b, int key, int n) {
   return key < n && (a.mask == nullptr || a.mask[b * a.mask_b + key * a.mask_k] != 0);
 }
+// The same as a number that is zero where the key does not count: a mask's byte as it was loaded, so that nothing waits for it
+// before it is used.
+__device__ __forceinline__ int key_word(const AttendArgs& a, int b, int key, int n) {
+  int w = 0;
+  if (key < n) w = a.mask ? a.mask[b * a.mask_b + key * a.mask_k] : 1;
+  return w;
+}
 // offset of row r of (b, kv) in a token view
 __device__ __forceinline__ int64_t row_at(const TokenView& t, const AttendArgs& a, int b, int kv, int64_t r) {
   const int64_t g = (uint32_t)r / (uint32_t)a.queries, i = r - g * a.queries;

@@ -42,29 +42,77 @@ struct Rows16 {
   static __device__ __forceinline__ int at(int row, int piece) { return row * DP + ((piece ^ place(row)) << 3); }
 };
 
-// Left operand of a product over the head: rows first .. first + 31, values 16 c .. 16 c + 15 (lane: row first + col, 8 of them).
-template <typename T, int DP>
-__device__ __forceinline__ half8<T> rows_operand(const T* tile, int first, int c, int col, int h) {
-  half8<T> r;
-  __builtin_memcpy(&r, tile + first * DP + Rows16<T, DP>::at(col, 2 * c + h), 16);
-  return r;
+// A lane's place in a tile for either reader, from which every other read is an exclusive or with a constant and an offset in the
+// instruction.  (hide() keeps the compiler from holding all those addresses in registers over the loop.)
+__device__ __forceinline__ unsigned hide(unsigned at) {
+  asm("" : "+v"(at));
+  return at;
 }
-// Left operand of a product over rows: values 32 d .. 32 d + 31 (lane: value 32 d + col) of the 16 rows first + product_row(0..7, h) of
-// the lane's half: the order in which a product's registers 0-7 (or 8-15, for the 16 rows behind) hold them.
-// ds_read_b64_tr_b16 gives lane i of 16 the i-th value of four rows whose 16 values the lanes 4 j .. 4 j + 3 point to.
 template <typename T, int DP>
-__device__ __forceinline__ half8<T> columns_operand(const T* tile, int first, int d, int lane) {
-  const int h = lane >> 5, j = (lane >> 2) & 3, piece = 4 * d + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
-  typedef __attribute__((address_space(3))) short4_t* LdsPtr;
+__device__ __forceinline__ unsigned rows_place(int lane) {
+  return 2 * Rows16<T, DP>::at(lane & 31, lane >> 5);
+}
+template <typename T, int DP>
+__device__ __forceinline__ unsigned columns_place(int lane) {
+  const int h = lane >> 5, j = (lane >> 2) & 3, piece = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+  return 2 * (Rows16<T, DP>::at(4 * h + j, piece) + (lane & 1) * 4);
+}
+// Left operand of a product over the head: rows first .. first + 31, values 16 c .. 16 c + 15 (lane: row first + lane % 32, 8 of
+// them).  at: LDS address of the tile + rows_place.
+template <typename T, int DP>
+__device__ __forceinline__ half8<T> rows_operand(unsigned at, int first, int c) {
+  constexpr bool WHOLE = DP == 64 || DP == 128;   // the exchange moves groups of four pieces, too
+  const unsigned x = (at ^ ((WHOLE ? c : c & 1) << 5)) + (WHOLE ? 0 : (c >> 1) * 64) + first * DP * 2;
+  return *(const __attribute__((address_space(3))) half8<T>*)x;
+}
+// Left operand of a product over rows: values 32 d .. 32 d + 31 (lane: value 32 d + lane % 32) of the 16 rows first + product_row(0..7, h)
+// of the lane's half: the order in which a product's registers 0-7 (or 8-15, for the 16 rows behind) hold them.
+// ds_read_b64_tr_b16 gives lane i of 16 the i-th value of four rows whose 16 values the lanes 4 j .. 4 j + 3 point to.
+// at: LDS address of the tile + columns_place.
+template <typename T, int DP>
+__device__ __forceinline__ half8<T> columns_operand(unsigned at, int first, int d) {
+  constexpr bool WHOLE = DP == 64 || DP == 128;
   short4_t r[2];
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    const T* p = tile + first * DP + Rows16<T, DP>::at(8 * half + 4 * h + j, piece) + (lane & 1) * 4;
-    r[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(const __attribute__((address_space(3))) void*)p);
+    const unsigned x = (at ^ (half << 5 | (WHOLE ? d << 6 : 0))) + (WHOLE ? 0 : d * 64) + (first + 8 * half) * DP * 2;
+    r[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)x);
   }
   half8<T> f;
   __builtin_memcpy(&f, r, 16);
   return f;
+}
+
+// s[k] = the product over the head of rows first + 32 k .. first + 32 k + 31 of a tile with a row's operands f.  The LDS reads go two batches of
+// four ahead of the products that use them (left to itself the compiler puts every read right in front of its product), and the
+// products of a batch alternate between the independent results.
+template <typename T, int DP, int K, int MOST = 4>
+__device__ __forceinline__ void over_head(unsigned tile, int first, const half8<T> (&f)[DP / 16], float16_t (&s)[K]) {
+  constexpr int N = K * (DP / 16), BATCH = N % 4 == 0 && MOST == 4 ? 4 : N % 3 == 0 && MOST > 2 ? 3 : 2;
+  half8<T> x[2][BATCH];
+  auto read = [&](int n) {
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int at = n * BATCH + i;
+      x[n & 1][i] = rows_operand<T, DP>(tile, first + 32 * (at % K), at / K);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[k][i] = 0.0f;
+  read(0);
+#pragma unroll
+  for (int n = 0; n < N / BATCH; ++n) {
+    if (n + 1 < N / BATCH) read(n + 1);
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int at = n * BATCH + i;
+      s[at % K] = Half8<T>::mfma(x[n & 1][i], f[at / K], s[at % K]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
 }
 
 // Eight f32 of a product as the right operand of the next one, each rounded to T.
@@ -76,31 +124,41 @@ __device__ __forceinline__ half8<T> round8(const float16_t& s, int first) {
   return r;
 }
 
-// The transfers a wave makes for a pair of tiles (a and b) of ROWS rows each: COUNT of 1024 bytes, shared out over WAVES waves.
+// The transfers a wave makes for a pair of tiles (a and b) of ROWS rows each, PER_TILE transfers of 1024 bytes a tile, shared out
+// over WAVES waves.
 template <typename T, int DP, int ROWS, int WAVES>
 struct PairLoad {
   static constexpr int PIECES = DP / 8, PER_TILE = ROWS * PIECES / 64, COUNT = 2 * PER_TILE / WAVES;
+  static constexpr bool EVEN = PER_TILE % WAVES == 0;        // a wave has the same places in both tiles
+  static constexpr int PLACES = EVEN ? COUNT / 2 : COUNT;
   static_assert(2 * PER_TILE % WAVES == 0 && ROWS * PIECES % 64 == 0, "transfers come out even");
-  int row[COUNT], value[COUNT];   // of this lane: row of the tile, first value (or -1: behind the head size)
-  // transfer i of this wave: which tile, and where in it
-  __device__ __forceinline__ static int index(int i, int wave) { return i * WAVES + wave; }
+  int row[PLACES], value[PLACES];   // of this lane: row of the tile, first value (or -1: behind the head size)
   __device__ __forceinline__ void init(int wave, int lane, int head) {
 #pragma unroll
-    for (int i = 0; i < COUNT; ++i) {
-      const int at = index(i, wave) % PER_TILE * 64 + lane;
+    for (int i = 0; i < PLACES; ++i) {
+      const int at = (i * WAVES + wave) % PER_TILE * 64 + lane;
       row[i] = at / PIECES;
       const int piece = at % PIECES ^ Rows16<T, DP>::place(row[i]);
       value[i] = piece * 8 < head ? piece * 8 : -1;
     }
   }
-  // a(row), b(row): pointers to the rows of the tiles; lds: LDS address of tile a, tile b behind it
-  template <class A, class B>
-  __device__ __forceinline__ void issue(A a, B b, unsigned lds, int wave) const {
+  // where(row): what a and b find a row by; a, b: pointers to the rows of the tiles; lds: LDS address of tile a, tile b behind it
+  template <class Where, class A, class B>
+  __device__ __forceinline__ void issue(Where where, A a, B b, unsigned lds, int wave) const {
 #pragma unroll
-    for (int i = 0; i < COUNT; ++i) {
-      const int at = index(i, wave);
-      const T* p = at < PER_TILE ? a(row[i]) : b(row[i]);
-      if (value[i] >= 0) lds_dma16_at((const double*)(p + value[i]), __builtin_amdgcn_readfirstlane(lds + at * 1024));
+    for (int i = 0; i < PLACES; ++i) {
+      const auto w = where(row[i]);
+      const int at = i * WAVES + wave;
+      if constexpr (EVEN) {
+        const T *pa = a(w) + value[i], *pb = b(w) + value[i];
+        if (value[i] >= 0) {
+          lds_dma16_at((const double*)pa, __builtin_amdgcn_readfirstlane(lds + at * 1024));
+          lds_dma16_at((const double*)pb, __builtin_amdgcn_readfirstlane(lds + (PER_TILE + at) * 1024));
+        }
+      } else {
+        const T* p = (at < PER_TILE ? a(w) : b(w)) + value[i];
+        if (value[i] >= 0) lds_dma16_at((const double*)p, __builtin_amdgcn_readfirstlane(lds + at * 1024));
+      }
     }
   }
 };
@@ -138,6 +196,7 @@ bool attend16_takes(const AttendArgs& a, int type);
 bool grad16_takes(const AttendArgs& a, int type);
 void launch_attend16(const AttendArgs& a, int type, bool few, hipStream_t st);
 void launch_query_grad16(const AttendArgs& a, hipStream_t st);   // tiles of 256 rows
-void launch_key_grad16(const AttendArgs& a, hipStream_t st);     // tiles of 128 keys
+void launch_key_grad16(const AttendArgs& a, hipStream_t st);     // tiles of key_grad16_tile(head) keys
+int key_grad16_tile(int64_t head);
 
 }  // namespace nnvhip

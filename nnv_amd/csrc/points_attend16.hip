@@ -30,7 +30,7 @@ __global__ __launch_bounds__(64 * WAVES) void attend16_kernel(const AttendArgs a
   const int64_t r = FEW ? (int64_t)row_tile * 32 + col : (int64_t)row_tile * (32 * WAVES) + wave * 32 + col;
   const bool row_here = r < a.rows;
   T* mine = lds + (FEW ? wave * 4 * TILE : 0);
-  const unsigned mine_at = lds_addr_of(mine);
+  const unsigned mine_at = lds_addr_of(mine), rows_at = rows_place<T, DP>(lane), columns_at = columns_place<T, DP>(lane);
 
   if (DP != a.head) {   // the columns behind the head size, for good
     half8<T> zero = {};
@@ -62,19 +62,36 @@ __global__ __launch_bounds__(64 * WAVES) void attend16_kernel(const AttendArgs a
   const T* vp = (const T*)a.v.p + b * a.v.b + kv * a.v.h;
   Load load;
   load.init(FEW ? 0 : wave, lane, a.head);
-  bool counts = false;
+  int counts = 0;   // FEW: lane i holds which keys of the i-th tile from here count; else: whether key `lane` of the next tile does
   auto fetch = [&](int t, int buffer) {
     // rows past the last key repeat it: what they hold is not used (see below)
-    load.issue([&](int j) { return kp + (int64_t)min(t * KEYS + j, n - 1) * a.k.t; },
-               [&](int j) { return vp + (int64_t)min(t * KEYS + j, n - 1) * a.v.t; }, mine_at + buffer * (4 * TILE), FEW ? 0 : wave);
-    counts = key_counts(a, b, t * KEYS + (KEYS == 64 ? lane : col), n);
+    load.issue([&](int j) { return min(t * KEYS + j, n - 1); }, [&](int key) { return kp + key * a.k.t; },
+               [&](int key) { return vp + key * a.v.t; }, mine_at + buffer * (4 * TILE), FEW ? 0 : wave);
+    if constexpr (!FEW) counts = key_word(a, b, t * KEYS + lane, n);
   };
   int buffer = 0;
   if (t0 < t1) fetch(t0, 0);
-  for (int t = t0; t < t1; t += STEP, buffer ^= 1) {
-    uint64_t valid = __ballot(counts);
-    T* ks = mine + buffer * 2 * TILE;
-    T* vs = ks + TILE;
+  for (int t = t0, turn = 0; t < t1; t += STEP, buffer ^= 1, ++turn) {
+    uint64_t valid;
+    if constexpr (FEW) {
+      // A mask's bytes are read for 32 tiles at a time: a wait for one of them would be a wait for all transfers behind it.
+      if (a.mask == nullptr) {
+        const int rest = n - t * KEYS;
+        valid = rest >= KEYS ? ~0ull : (1ull << rest) - 1;
+      } else {
+        if (turn % 32 == 0)
+          for (int i = 0; i < 32; ++i) {
+            const uint64_t word = __ballot(t + i * STEP < t1 && key_word(a, b, (t + i * STEP) * KEYS + col, n) != 0);
+            if (lane == i) counts = (int)word;
+          }
+        const uint32_t word = __builtin_amdgcn_readlane(counts, turn % 32);
+        valid = word == ~0u ? ~0ull : word;
+      }
+    } else {
+      valid = __ballot(counts != 0);
+    }
+    T* vs = mine + (buffer * 2 + 1) * TILE;
+    const unsigned ks_at = hide(mine_at + buffer * (4 * TILE) + rows_at), vs_at = hide(mine_at + (buffer * 4 + 2) * TILE + columns_at);
     if constexpr (FEW) {
       // the other pair was read before; its readers are done
       if (t + STEP < t1) {
@@ -104,13 +121,7 @@ __global__ __launch_bounds__(64 * WAVES) void attend16_kernel(const AttendArgs a
     }
 
     float16_t s[KEYS / 32];
-#pragma unroll
-    for (int k = 0; k < KEYS / 32; ++k) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[k][i] = 0.0f;
-#pragma unroll
-      for (int c = 0; c < DP / 16; ++c) s[k] = Half8<T>::mfma(rows_operand<T, DP>(ks, 32 * k, c, col, h), qf[c], s[k]);
-    }
+    over_head<T, DP, KEYS / 32>(ks_at, 0, qf, s);
     if (valid != ~0ull) {
 #pragma unroll
       for (int k = 0; k < KEYS / 32; ++k) {
@@ -151,7 +162,7 @@ __global__ __launch_bounds__(64 * WAVES) void attend16_kernel(const AttendArgs a
       for (int c = 0; c < 2; ++c) {
         const half8<T> p = round8<T>(s[k], 8 * c);
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) acc[d] = Half8<T>::mfma(columns_operand<T, DP>(vs, 32 * k + 16 * c, d, lane), p, acc[d]);
+        for (int d = 0; d < DP / 32; ++d) acc[d] = Half8<T>::mfma(columns_operand<T, DP>(vs_at, 32 * k + 16 * c, d), p, acc[d]);
       }
   }
   total = sum_of_halves(total);

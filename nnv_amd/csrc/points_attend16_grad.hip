@@ -25,22 +25,37 @@ __device__ __forceinline__ void zero(float16_t (&acc)[DP / 32]) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
 }
+// over_head with the operands of the row in LDS as well (16 bytes a lane, 1024 bytes apart), read along with the tile's.
 template <typename T, int DP>
-__device__ __forceinline__ float16_t over_head(const T* tile, int first, const half8<T> (&f)[DP / 16], int col, int h) {
-  float16_t s;
+__device__ __forceinline__ void over_head_parked(unsigned tile, int first, const T* parked, float16_t& s) {
+  constexpr int N = DP / 16, BATCH = 2;
+  half8<T> x[2][BATCH], f[2][BATCH];
+  auto read = [&](int n) {
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      x[n & 1][i] = rows_operand<T, DP>(tile, first, n * BATCH + i);
+      __builtin_memcpy(&f[n & 1][i], parked + 512 * (n * BATCH + i), 16);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
 #pragma unroll
   for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+  read(0);
 #pragma unroll
-  for (int c = 0; c < DP / 16; ++c) s = Half8<T>::mfma(rows_operand<T, DP>(tile, first, c, col, h), f[c], s);
-  return s;
+  for (int n = 0; n < N / BATCH; ++n) {
+    if (n + 1 < N / BATCH) read(n + 1);
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) s = Half8<T>::mfma(x[n & 1][i], f[n & 1][i], s);
+    __builtin_amdgcn_sched_barrier(0);
+  }
 }
 template <typename T, int DP>
-__device__ __forceinline__ void over_rows(const T* tile, int first, const float16_t& p, float16_t (&acc)[DP / 32], int lane) {
+__device__ __forceinline__ void over_rows(unsigned tile, int first, const float16_t& p, float16_t (&acc)[DP / 32]) {
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     const half8<T> f = round8<T>(p, 8 * c);
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d) acc[d] = Half8<T>::mfma(columns_operand<T, DP>(tile, first + 16 * c, d, lane), f, acc[d]);
+    for (int d = 0; d < DP / 32; ++d) acc[d] = Half8<T>::mfma(columns_operand<T, DP>(tile, first + 16 * c, d), f, acc[d]);
   }
 }
 template <typename T, int DP>
@@ -85,7 +100,7 @@ __global__ __launch_bounds__(64 * WAVES) void query_grad16_kernel(const AttendAr
   const int t0 = split * per, t1 = min(tiles, t0 + per);
   const int64_t r = (int64_t)row_tile * (32 * WAVES) + wave * 32 + col, flat = (int64_t)bkv * a.rows + r;
   const bool here = r < a.rows;
-  const unsigned lds_at = lds_addr_of(lds);
+  const unsigned lds_at = lds_addr_of(lds), rows_at = rows_place<T, DP>(lane), columns_at = columns_place<T, DP>(lane);
   if (DP != a.head) zero_all<T, 4 * TILE / 8, 64 * WAVES>(lds);
 
   const float lse = here ? a.lse[flat] : -INFINITY;
@@ -100,38 +115,40 @@ __global__ __launch_bounds__(64 * WAVES) void query_grad16_kernel(const AttendAr
   const T* vp = (const T*)a.v.p + b * a.v.b + kv * a.v.h;
   Load load;
   load.init(wave, lane, a.head);
-  bool counts = false;
+  int counts = 0;
   auto fetch = [&](int t, int buffer) {
-    load.issue([&](int j) { return kp + (int64_t)min(t * KEYS + j, n - 1) * a.k.t; },
-               [&](int j) { return vp + (int64_t)min(t * KEYS + j, n - 1) * a.v.t; }, lds_at + buffer * (4 * TILE), wave);
-    counts = key_counts(a, b, t * KEYS + lane, n);
+    load.issue([&](int j) { return min(t * KEYS + j, n - 1); }, [&](int key) { return kp + key * a.k.t; },
+               [&](int key) { return vp + key * a.v.t; }, lds_at + buffer * (4 * TILE), wave);
+    counts = key_word(a, b, t * KEYS + lane, n);
   };
   int buffer = 0;
   if (t0 < t1) fetch(t0, 0);
   for (int t = t0; t < t1; ++t, buffer ^= 1) {
-    const uint64_t valid = __ballot(counts);
-    T* ks = lds + buffer * 2 * TILE;
-    T* vs = ks + TILE;
+    const uint64_t valid = __ballot(counts != 0);
+    const unsigned pair = lds_at + buffer * (4 * TILE);
+    const unsigned ks_at = hide(pair + rows_at), vs_at = ks_at + 2 * TILE, kc_at = hide(pair + columns_at);
     wait_vm_lds<0>();
     block_barrier();
     if (t + 1 < t1) fetch(t + 1, buffer ^ 1);
     if (valid != ~0ull) {
-      zero_rows<T, DP, KEYS, 64 * WAVES>(ks, valid);
+      zero_rows<T, DP, KEYS, 64 * WAVES>(lds + buffer * 2 * TILE, valid);
       wait_vm_lds<63>();
       block_barrier();
     }
 #pragma unroll
     for (int k = 0; k < KEYS / 32; ++k) {
-      float16_t s = over_head<T, DP>(ks, 32 * k, qf, col, h);
-      const float16_t dp = over_head<T, DP>(vs, 32 * k, gf, col, h);
+      float16_t ps[1], dps[1];
+      over_head<T, DP, 1>(ks_at, 32 * k, qf, ps);
+      over_head<T, DP, 1>(vs_at, 32 * k, gf, dps);
+      float16_t& s = ps[0];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = exp2_(s[i] * unit - offset) * (dp[i] - delta);
+      for (int i = 0; i < 16; ++i) s[i] = exp2_(s[i] * unit - offset) * (dps[0][i] - delta);
       if (valid != ~0ull) {
         const uint32_t word = (uint32_t)(valid >> (32 * k)) >> (4 * h);
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = word >> product_row(i, 0) & 1 ? s[i] : 0.0f;
       }
-      over_rows<T, DP>(ks, 32 * k, s, dq, lane);
+      over_rows<T, DP>(kc_at, 32 * k, s, dq);
     }
   }
   if (!here) return;
@@ -141,11 +158,14 @@ __global__ __launch_bounds__(64 * WAVES) void query_grad16_kernel(const AttendAr
     store_result<T, DP>((T*)a.dq + dense_row_at(a, b, kv, r), dq, a.scale, h, a.head);
 }
 
+// Two waves a SIMD, so that one's exponentials run beside the other's products: 256 registers a wave.  The accumulators take 2 DP of them
+// and the operands of the wave's keys DP / 2, as many again those of its values, which lie in LDS where they would not fit.
 template <typename T, int DP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void key_grad16_kernel(const AttendArgs a) {
+__global__ __launch_bounds__(64 * WAVES, 2) void key_grad16_kernel(const AttendArgs a) {
   constexpr int ROWS = 64, TILE = ROWS * DP;
+  constexpr bool PARKED = DP > 64;   // the values' operands, in LDS
   typedef PairLoad<T, DP, ROWS, WAVES> Load;
-  __shared__ __attribute__((aligned(1024))) T lds[4 * TILE];
+  __shared__ __attribute__((aligned(1024))) T lds[4 * TILE + (PARKED ? WAVES * 32 * DP : 0)];
   __shared__ __attribute__((aligned(16))) float offsets[2][ROWS], deltas[2][ROWS];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
   int64_t at = xcd_order(blockIdx.x, gridDim.x);
@@ -156,7 +176,7 @@ __global__ __launch_bounds__(64 * WAVES) void key_grad16_kernel(const AttendArgs
   const int n = keys_that_count(a, b);
   const int key = key_tile * (32 * WAVES) + wave * 32 + col;
   const bool here = key < a.keys, counts = key_counts(a, b, key, n);
-  const unsigned lds_at = lds_addr_of(lds);
+  const unsigned lds_at = lds_addr_of(lds), rows_at = rows_place<T, DP>(lane), columns_at = columns_place<T, DP>(lane);
   if (DP != a.head) zero_all<T, 4 * TILE / 8, 64 * WAVES>(lds);
   // where no key of the block counts there is nothing to add up (and rows without any key take part in no block)
   const bool any = __syncthreads_or(counts);
@@ -164,8 +184,12 @@ __global__ __launch_bounds__(64 * WAVES) void key_grad16_kernel(const AttendArgs
   const int t0 = split * per, t1 = min(tiles, t0 + per);
 
   half8<T> kf[DP / 16], vf[DP / 16];
+  T* parked = lds + 4 * TILE + wave * (32 * DP) + lane * 8;   // operand c at parked + 512 c; no other wave's
   load_operands<T, DP>(kf, (const T*)a.k.p + (counts ? b * a.k.b + kv * a.k.h + key * a.k.t : 0), h, a.head, counts);
   load_operands<T, DP>(vf, (const T*)a.v.p + (counts ? b * a.v.b + kv * a.v.h + key * a.v.t : 0), h, a.head, counts);
+  if constexpr (PARKED)
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) __builtin_memcpy(parked + 512 * c, &vf[c], 16);
   const float unit = a.scale * kLog2e;
   float16_t dk[DP / 32], dv[DP / 32];
   zero<DP>(dk);
@@ -174,26 +198,36 @@ __global__ __launch_bounds__(64 * WAVES) void key_grad16_kernel(const AttendArgs
   const float* del = a.delta + (int64_t)bkv * a.rows;
   Load load;
   load.init(wave, lane, a.head);
-  float next_offset = 0.0f, next_delta = 0.0f;
+  const T* qp = (const T*)a.q.p + b * a.q.b + kv * (int64_t)a.group * a.q.h;
+  const T* gp = (const T*)a.go.p + b * a.go.b + kv * (int64_t)a.group * a.go.h;
+  const float per_query = 1.0f / a.queries;
+  struct Place {
+    int head, query;
+  };
+  float next_lse = 0.0f, next_delta = 0.0f;
   auto fetch = [&](int t, int buffer) {
-    // rows past the last one repeat it, and are made zeros below
-    auto row = [&](int j) { return min((int64_t)t * ROWS + j, a.rows - 1); };
-    load.issue([&](int j) { return (const T*)a.q.p + row_at(a.q, a, b, kv, row(j)); },
-               [&](int j) { return (const T*)a.go.p + row_at(a.go, a, b, kv, row(j)); }, lds_at + buffer * (4 * TILE), wave);
+    // Head of the group and query of the tile's first row, then of every row: a tile reaches into the next head at most where heads have
+    // ROWS queries, and the quotient is small where they have fewer.  Rows past the last one repeat it, and are made zeros below.
+    const int g0 = (uint32_t)t * ROWS / (uint32_t)a.queries, i0 = t * ROWS - g0 * a.queries, last = (int)a.rows - 1 - g0 * a.queries;
+    auto where = [&](int j) {
+      const int i = min(i0 + j, last);
+      const int more = a.queries >= ROWS ? (int)(i >= a.queries) : (int)((i + 0.5f) * per_query);
+      return Place{g0 + more, i - more * a.queries};
+    };
+    load.issue(where, [&](Place w) { return qp + (w.query * a.q.t + w.head * a.q.h); },
+               [&](Place w) { return gp + (w.query * a.go.t + w.head * a.go.h); }, lds_at + buffer * (4 * TILE), wave);
     if (threadIdx.x < ROWS) {
       const int64_t r = (int64_t)t * ROWS + threadIdx.x;
-      const float x = lse[row(threadIdx.x)];
-      next_offset = r < a.rows && x != -INFINITY ? x * kLog2e : INFINITY;
-      next_delta = r < a.rows ? del[row(threadIdx.x)] : 0.0f;
+      next_lse = r < a.rows ? lse[r] : -INFINITY;
+      next_delta = r < a.rows ? del[r] : 0.0f;
     }
   };
   int buffer = 0;
   if (t0 < t1) fetch(t0, 0);
   for (int t = t0; t < t1; ++t, buffer ^= 1) {
-    T* qs = lds + buffer * 2 * TILE;
-    T* gs = qs + TILE;
+    const unsigned pair = lds_at + buffer * (4 * TILE);
     if (threadIdx.x < ROWS) {
-      offsets[buffer][threadIdx.x] = next_offset;
+      offsets[buffer][threadIdx.x] = next_lse == -INFINITY ? INFINITY : next_lse * kLog2e;
       deltas[buffer][threadIdx.x] = next_delta;
     }
     wait_vm_lds<0>();
@@ -201,34 +235,43 @@ __global__ __launch_bounds__(64 * WAVES) void key_grad16_kernel(const AttendArgs
     if (t + 1 < t1) fetch(t + 1, buffer ^ 1);
     if ((int64_t)(t + 1) * ROWS > a.rows) {
       const uint64_t valid = (1ull << (int)(a.rows - (int64_t)t * ROWS)) - 1;
-      zero_rows<T, DP, ROWS, 64 * WAVES>(qs, valid);
-      zero_rows<T, DP, ROWS, 64 * WAVES>(gs, valid);
+      zero_rows<T, DP, ROWS, 64 * WAVES>(lds + buffer * 2 * TILE, valid);
+      zero_rows<T, DP, ROWS, 64 * WAVES>(lds + (buffer * 2 + 1) * TILE, valid);
       wait_vm_lds<63>();
       block_barrier();
     }
-#pragma unroll
-    for (int k = 0; k < ROWS / 32; ++k) {
-      float16_t s = over_head<T, DP>(qs, 32 * k, kf, col, h);
+#pragma unroll 1
+    for (int k = 0; k < ROWS / 32; ++k) {   // (both at once would need more registers than there are)
+      const unsigned rows_k = rows_at + pair + k * (64 * DP), columns_k = columns_at + pair + k * (64 * DP);
+      const unsigned qs_at = hide(rows_k), gs_at = qs_at + 2 * TILE, qc_at = hide(columns_k), gc_at = qc_at + 2 * TILE;
+      float16_t ps[1], dps[1];
+      over_head<T, DP, 1, DP == 128 ? 2 : 4>(qs_at, 0, kf, ps);
+      float16_t& s = ps[0];
 #pragma unroll
       for (int i4 = 0; i4 < 4; ++i4) {
         float f[4];
         __builtin_memcpy(f, &offsets[buffer][32 * k + 8 * i4 + 4 * h], 16);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[4 * i4 + i] = counts ? exp2_(s[4 * i4 + i] * unit - f[i]) : 0.0f;
+        for (int i = 0; i < 4; ++i) s[4 * i4 + i] = exp2_(s[4 * i4 + i] * unit - f[i]);
       }
-      const float16_t dp = over_head<T, DP>(gs, 32 * k, vf, col, h);
-      over_rows<T, DP>(gs, 32 * k, s, dv, lane);
+      if constexpr (PARKED) over_head_parked<T, DP>(gs_at, 0, parked, dps[0]);
+      else over_head<T, DP, 1>(gs_at, 0, vf, dps);
+      over_rows<T, DP>(gc_at, 0, s, dv);
 #pragma unroll
       for (int i4 = 0; i4 < 4; ++i4) {
         float f[4];
         __builtin_memcpy(f, &deltas[buffer][32 * k + 8 * i4 + 4 * h], 16);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[4 * i4 + i] *= dp[4 * i4 + i] - f[i];
+        for (int i = 0; i < 4; ++i) s[4 * i4 + i] *= dps[0][4 * i4 + i] - f[i];
       }
-      over_rows<T, DP>(qs, 32 * k, s, dk, lane);
+      over_rows<T, DP>(qc_at, 0, s, dk);
     }
   }
   if (!here) return;
+  if (!counts) {   // what the loop made of a column that does not count reached no other one
+    zero<DP>(dk);
+    zero<DP>(dv);
+  }
   const int64_t dense = ((b * (int64_t)a.keys + key) * a.kv_heads + kv) * a.head;
   if (a.splits > 1) {
     const int64_t all = (int64_t)a.batch * a.keys * a.kv_heads * a.head;
@@ -247,12 +290,14 @@ void launch_query(const AttendArgs& a, hipStream_t st) {
 }
 template <typename T, int DP>
 void launch_key(const AttendArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((key_grad16_kernel<T, DP, 4>), dim3((unsigned)((int64_t)a.batch * a.kv_heads * a.key_tiles * a.splits)), dim3(256), 0,
-                     st, a);
+  constexpr int WAVES = DP > 64 ? 8 : 4;
+  hipLaunchKernelGGL((key_grad16_kernel<T, DP, WAVES>), dim3((unsigned)((int64_t)a.batch * a.kv_heads * a.key_tiles * a.splits)),
+                     dim3(64 * WAVES), 0, st, a);
 }
 
 }  // namespace
 
+int key_grad16_tile(int64_t head) { return head > 64 ? 256 : 128; }
 bool grad16_takes(const AttendArgs& a, int type) {
   return type == NNVHIP_TYPE_BF16 && by_pieces(a.q, a.head) && by_pieces(a.k, a.head) && by_pieces(a.v, a.head) && by_pieces(a.go, a.head);
 }
