@@ -140,7 +140,7 @@ int attend_args(const char* what, const nnvhip_attention* d, bool backward, Atte
 // axis' `tiles` tiles.
 inline int split_of(int64_t blocks, int64_t tiles, int64_t least, int64_t want) {
   if (blocks <= 0 || blocks >= want) return 1;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(ceil_div(want, blocks), tiles / least), 256));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want / blocks, tiles / least), 256));
 }
 
 #define ATTEND_BY_HEAD(CALL, T, ...)                 \

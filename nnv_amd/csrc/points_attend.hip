@@ -217,11 +217,11 @@ struct Cut {
   bool few;
   int row_tiles, splits;
 };
-Cut cut_of(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys, bool by16) {
+Cut cut_of(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys, int64_t head, bool by16) {
   Cut c;
   c.few = rows <= kWaveRows;
-  c.row_tiles = (int)ceil_div(rows, c.few ? kWaveRows : by16 ? 256 : 128);
-  c.splits = split_of(batch * kv_heads * c.row_tiles, ceil_div(keys, kWaveRows), c.few ? 8 : 4, 512);
+  c.row_tiles = (int)ceil_div(rows, c.few ? kWaveRows : by16 ? attend16_tile(head) : 128);
+  c.splits = split_of(batch * kv_heads * c.row_tiles, ceil_div(keys, kWaveRows), c.few ? 8 : 4, c.few || (by16 && head > 64) ? 256 : 512);
   return c;
 }
 
@@ -297,7 +297,7 @@ int nnvhip_cross_attention_workspace(const nnvhip_attention* d, int64_t* bytes) 
   NNV_TRY(check_sizes("nnvhip_cross_attention_workspace", d));
   int splits = 1;   // whichever kernels the alignment of the tensors lets take the call
   for (const bool by16 : {false, true})
-    splits = std::max(splits, cut_of(d->batch, d->kv_heads, d->queries * (d->heads / d->kv_heads), d->keys, by16).splits);
+    splits = std::max(splits, cut_of(d->batch, d->kv_heads, d->queries * (d->heads / d->kv_heads), d->keys, d->head, by16).splits);
   *bytes = splits > 1 ? (int64_t)splits * d->batch * d->heads * d->queries * (d->head + 1) * (int64_t)sizeof(float) : 0;
   return NNVHIP_OK;
 }
@@ -312,7 +312,7 @@ int nnvhip_cross_attention(nnvhip_ctx* ctx, const nnvhip_attention* d, void* wor
     NNV_FAIL(NNVHIP_ERR_ARG, "nnvhip_cross_attention: a workspace of %lld bytes is needed", (long long)need);
   if (a.batch == 0 || a.rows == 0) return NNVHIP_OK;
   const bool by16 = attend16_takes(a, (int)d->type);
-  const Cut c = cut_of(a.batch, a.kv_heads, a.rows, a.keys, by16);
+  const Cut c = cut_of(a.batch, a.kv_heads, a.rows, a.keys, a.head, by16);
   a.row_tiles = c.row_tiles;
   a.splits = c.splits;
   a.part = static_cast<float*>(workspace);

@@ -125,43 +125,86 @@ __device__ __forceinline__ half8<T> round8(const float16_t& s, int first) {
 }
 
 // The transfers a wave makes for a pair of tiles (a and b) of ROWS rows each, PER_TILE transfers of 1024 bytes a tile, shared out
-// over WAVES waves.
+// over WAVES waves.  Tiles of evenly spaced rows need no arithmetic on vectors: a scalar address for the tile and an offset that a lane
+// keeps (64-bit products of vectors would take as long as a quarter of a tile's exponentials).
 template <typename T, int DP, int ROWS, int WAVES>
 struct PairLoad {
   static constexpr int PIECES = DP / 8, PER_TILE = ROWS * PIECES / 64, COUNT = 2 * PER_TILE / WAVES;
   static constexpr bool EVEN = PER_TILE % WAVES == 0;        // a wave has the same places in both tiles
   static constexpr int PLACES = EVEN ? COUNT / 2 : COUNT;
   static_assert(2 * PER_TILE % WAVES == 0 && ROWS * PIECES % 64 == 0, "transfers come out even");
-  int row[PLACES], value[PLACES];   // of this lane: row of the tile, first value (or -1: behind the head size)
-  __device__ __forceinline__ void init(int wave, int lane, int head) {
+  unsigned off_a[PLACES], off_b[EVEN ? PLACES : 1];   // bytes behind the tile's address (not EVEN: of whichever tile the place is in)
+  unsigned there;                                     // bit i: place i holds values of the head (not what is behind them)
+  __device__ __forceinline__ static int row(int i, int wave, int lane) { return ((i * WAVES + wave) % PER_TILE * 64 + lane) / PIECES; }
+  __device__ __forceinline__ static int value(int i, int wave, int lane) {
+    const int at = (i * WAVES + wave) % PER_TILE * 64 + lane;
+    return (at % PIECES ^ Rows16<T, DP>::place(at / PIECES)) * 8;
+  }
+  __device__ __forceinline__ void init(int wave, int lane, int head, int64_t stride_a, int64_t stride_b) {
+    there = 0;
 #pragma unroll
     for (int i = 0; i < PLACES; ++i) {
-      const int at = (i * WAVES + wave) % PER_TILE * 64 + lane;
-      row[i] = at / PIECES;
-      const int piece = at % PIECES ^ Rows16<T, DP>::place(row[i]);
-      value[i] = piece * 8 < head ? piece * 8 : -1;
+      const int r = row(i, wave, lane), v = value(i, wave, lane);
+      const bool in_a = EVEN || i * WAVES + wave < PER_TILE;
+      off_a[i] = 2 * (unsigned)(r * (unsigned)(in_a ? stride_a : stride_b) + v);
+      if constexpr (EVEN) off_b[i] = 2 * (unsigned)(r * (unsigned)stride_b + v);
+      there |= v < head ? 1u << i : 0;
     }
   }
-  // where(row): what a and b find a row by; a, b: pointers to the rows of the tiles; lds: LDS address of tile a, tile b behind it
-  template <class Where, class A, class B>
-  __device__ __forceinline__ void issue(Where where, A a, B b, unsigned lds, int wave) const {
+  // tiles whose rows follow one another from pa and pb
+  __device__ __forceinline__ void issue(const T* pa, const T* pb, unsigned lds, int wave) const {
 #pragma unroll
     for (int i = 0; i < PLACES; ++i) {
-      const auto w = where(row[i]);
       const int at = i * WAVES + wave;
-      if constexpr (EVEN) {
-        const T *pa = a(w) + value[i], *pb = b(w) + value[i];
-        if (value[i] >= 0) {
-          lds_dma16_at((const double*)pa, __builtin_amdgcn_readfirstlane(lds + at * 1024));
-          lds_dma16_at((const double*)pb, __builtin_amdgcn_readfirstlane(lds + (PER_TILE + at) * 1024));
+      if (there >> i & 1) {
+        if constexpr (EVEN) {
+          lds_dma16((const double*)pa, off_a[i], __builtin_amdgcn_readfirstlane(lds + at * 1024));
+          lds_dma16((const double*)pb, off_b[i], __builtin_amdgcn_readfirstlane(lds + (PER_TILE + at) * 1024));
+        } else {
+          lds_dma16((const double*)(at < PER_TILE ? pa : pb), off_a[i], __builtin_amdgcn_readfirstlane(lds + at * 1024));
         }
-      } else {
-        const T* p = (at < PER_TILE ? a(w) : b(w)) + value[i];
-        if (value[i] >= 0) lds_dma16_at((const double*)p, __builtin_amdgcn_readfirstlane(lds + at * 1024));
       }
     }
   }
+  // tiles whose rows are anywhere: a(row), b(row) are pointers to them
+  template <class A, class B>
+  __device__ __forceinline__ void issue_any(A a, B b, unsigned lds, int wave, int lane) const {
+#pragma unroll
+    for (int i = 0; i < PLACES; ++i) {
+      const int at = i * WAVES + wave, r = row(i, wave, lane), v = value(i, wave, lane);
+      if (there >> i & 1) {
+        if constexpr (EVEN) {
+          lds_dma16_at((const double*)(a(r) + v), __builtin_amdgcn_readfirstlane(lds + at * 1024));
+          lds_dma16_at((const double*)(b(r) + v), __builtin_amdgcn_readfirstlane(lds + (PER_TILE + at) * 1024));
+        } else {
+          lds_dma16_at((const double*)((at < PER_TILE ? a(r) : b(r)) + v), __builtin_amdgcn_readfirstlane(lds + at * 1024));
+        }
+      }
+    }
+  }
+  // tile t of rows that follow one another from pa and pb and end after n: rows past the last one repeat it
+  __device__ __forceinline__ void issue_tile(int t, int n, const T* pa, int64_t stride_a, const T* pb, int64_t stride_b, unsigned lds, int wave,
+                                             int lane) const {
+    const int first = t * ROWS;
+    if (first + ROWS <= n)
+      issue(pa + first * stride_a, pb + first * stride_b, lds, wave);
+    else
+      issue_any([&](int r) { return pa + min(first + r, n - 1) * stride_a; }, [&](int r) { return pb + min(first + r, n - 1) * stride_b; }, lds,
+                wave, lane);
+  }
 };
+
+// The rows of a tile that do not take part, made zeros by a wave for itself: a weight of zero must meet a zero.  Every wave that reads the
+// tile does so before its own reads, and no wave waits for another.
+template <typename T, int DP, int ROWS>
+__device__ __forceinline__ void zero_rows(T* tile, uint64_t valid, int lane) {
+  half8<T> none = {};
+#pragma unroll 1
+  for (int e = (int)hide(lane); e < ROWS * (DP / 8); e += 64)   // rarely taken: nothing of it is to be kept in registers
+    if (!(valid >> (e / (DP / 8)) & 1)) __builtin_memcpy(tile + e * 8, &none, 16);
+  wait_vm_lds<63>();
+  __builtin_amdgcn_wave_barrier();
+}
 
 // the larger of a value and that of lane l ^ 32
 __device__ __forceinline__ float max_of_halves(float x) {
@@ -178,22 +221,35 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
 }
+// the largest value of K products' registers: in chains that take turns, for one after the other would wait for each result
+template <int K>
+__device__ __forceinline__ float largest(const float16_t (&s)[K]) {
+  float top[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
+#pragma unroll
+  for (int e = 0; e < 16 * K; e += 8)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top[j] = max3(top[j], s[e / 16][e % 16 + 2 * j], s[e / 16][e % 16 + 2 * j + 1]);
+  return max3(max3(top[0], top[1], top[2]), top[3], top[3]);
+}
 
 // Block `id` of `total` in an order in which each of the 8 XCDs gets consecutive ones (blocks are dealt to the XCDs in turn):
-// blocks that read the same keys then find them in one L2.
+// blocks that read the same keys then find them in one L2.  (The sequences of a batch, whose lengths may differ, follow one another
+// within a head: every XCD gets some of each.)
 __device__ __forceinline__ int64_t xcd_order(int64_t id, int64_t total) {
   const int64_t x = id % 8, base = total / 8, more = total % 8;
   return x * base + min(x, more) + id / 8;
 }
 
-// A head's row can be moved in 16-byte pieces: head size, strides and start are multiples of 8 values.
+// A head's row can be moved in 16-byte pieces: head size, strides and start are multiples of 8 values.  And the offsets in a tile of 64 rows
+// fit 31 bits.
 inline bool by_pieces(const TokenView& t, int64_t head) {
-  return head % 8 == 0 && t.b % 8 == 0 && t.t % 8 == 0 && t.h % 8 == 0 && (uintptr_t)t.p % 16 == 0;
+  return t.t >= 0 && t.t < (int64_t(1) << 24) && head % 8 == 0 && t.b % 8 == 0 && t.t % 8 == 0 && t.h % 8 == 0 && (uintptr_t)t.p % 16 == 0;
 }
 
 // Whether the 16-bit kernels take a call; else the general ones do.
 bool attend16_takes(const AttendArgs& a, int type);
 bool grad16_takes(const AttendArgs& a, int type);
+int attend16_tile(int64_t head);   // rows of a block, unless few
 void launch_attend16(const AttendArgs& a, int type, bool few, hipStream_t st);
 void launch_query_grad16(const AttendArgs& a, hipStream_t st);   // tiles of 256 rows
 void launch_key_grad16(const AttendArgs& a, hipStream_t st);     // tiles of key_grad16_tile(head) keys

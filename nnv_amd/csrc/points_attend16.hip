@@ -6,35 +6,39 @@
 namespace nnvhip {
 namespace {
 
-// FEW = false: WAVES waves of 32 rows each share tiles of 64 keys.  FEW = true: 32 rows for the block, whose waves take tiles of 32
-// keys in turn (see attend_kernel, which this is the 16-bit form of).
+// GROUPS groups of WAVES waves each.  FEW = false: the waves of a group take 32 rows each, the same ones in every group, and share tiles
+// of 64 keys, which the groups take in turn.  FEW = true: 32 rows for the block, tiles of 32 keys, groups of one wave.  What the groups
+// found is joined at the end.  (attend_kernel is the f32 form.)
 //
-// The next tile is on its way to LDS (no registers in between) while one is worked on; one barrier a tile.  A weight is rounded to T
-// before the product with the values.  The running maximum is raised only when a row's has grown by more than 2^8: the sums
-// are in f32 and any base serves, so that the accumulators are hardly ever multiplied.
-template <typename T, int DP, int WAVES, bool FEW>
-__global__ __launch_bounds__(64 * WAVES) void attend16_kernel(const AttendArgs a) {
-  constexpr int KEYS = FEW ? 32 : 64, TILE = KEYS * DP, STEP = FEW ? WAVES : 1;
-  typedef PairLoad<T, DP, KEYS, FEW ? 1 : WAVES> Load;
-  __shared__ __attribute__((aligned(1024))) T lds[(FEW ? WAVES : 1) * 2 * 2 * TILE];   // two pairs (k, v), of every wave if FEW
-  __shared__ float row_max[FEW ? WAVES : 1][32], row_total[FEW ? WAVES : 1][32];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
+// Tiles are on their way to LDS (no registers in between) STAGES - 1 ahead of the one that is worked on; one barrier a tile.  A weight is
+// rounded to T before the product with the values.  The running maximum is raised only when a row's has grown by more than 2^8:
+// the sums are in f32 and any base serves, so that the accumulators are hardly ever multiplied.
+template <typename T, int DP, int WAVES, int GROUPS, bool FEW, int STAGES>
+__global__ __launch_bounds__(64 * WAVES * GROUPS, FEW ? 1 : GROUPS > 1 ? 4 : 2) void attend16_kernel(const AttendArgs a) {
+  constexpr int KEYS = FEW ? 32 : 64, TILE = KEYS * DP, THREADS = 64 * WAVES * GROUPS;
+  typedef PairLoad<T, DP, KEYS, WAVES> Load;
+  // STAGES pairs (k, v) of every group; at the end, what the groups found: [group][row][LD values]
+  constexpr int ROWS = 32 * WAVES, LD = DP + 4, TILES = GROUPS * STAGES * 2 * TILE, FOUND = GROUPS > 1 ? GROUPS * ROWS * LD * 2 : 0;
+  __shared__ __attribute__((aligned(1024))) T lds[TILES > FOUND ? TILES : FOUND];
+  __shared__ float row_max[GROUPS][32 * WAVES], row_total[GROUPS][32 * WAVES];
+  const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
+  const int any_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = any_wave / WAVES, wave = any_wave % WAVES;
   int64_t at = xcd_order(blockIdx.x, gridDim.x);
   const int split = at % a.splits;
   at /= a.splits;
   const int row_tile = at % a.row_tiles;
-  const int bkv = at / a.row_tiles, b = bkv / a.kv_heads, kv = bkv % a.kv_heads;
+  const int b = (int)(at / a.row_tiles) % a.batch, kv = (int)(at / a.row_tiles) / a.batch, bkv = b * a.kv_heads + kv;
   const int n = keys_that_count(a, b);
   const int tiles = (n + KEYS - 1) / KEYS, per = (tiles + a.splits - 1) / a.splits;
-  const int t0 = split * per + (FEW ? wave : 0), t1 = min(tiles, split * per + per);
-  const int64_t r = FEW ? (int64_t)row_tile * 32 + col : (int64_t)row_tile * (32 * WAVES) + wave * 32 + col;
+  const int t0 = split * per + group, t1 = min(tiles, split * per + per);
+  const int64_t r = (int64_t)row_tile * (32 * WAVES) + wave * 32 + col;
   const bool row_here = r < a.rows;
-  T* mine = lds + (FEW ? wave * 4 * TILE : 0);
+  T* mine = lds + group * STAGES * 2 * TILE;
   const unsigned mine_at = lds_addr_of(mine), rows_at = rows_place<T, DP>(lane), columns_at = columns_place<T, DP>(lane);
 
   if (DP != a.head) {   // the columns behind the head size, for good
     half8<T> zero = {};
-    for (int e = threadIdx.x; e < (FEW ? WAVES : 1) * 4 * KEYS * (DP / 8); e += 64 * WAVES) __builtin_memcpy(lds + e * 8, &zero, 16);
+    for (int e = threadIdx.x; e < GROUPS * STAGES * 2 * KEYS * (DP / 8); e += THREADS) __builtin_memcpy(lds + e * 8, &zero, 16);
     __syncthreads();
   }
 
@@ -61,67 +65,59 @@ __global__ __launch_bounds__(64 * WAVES) void attend16_kernel(const AttendArgs a
   const T* kp = (const T*)a.k.p + b * a.k.b + kv * a.k.h;
   const T* vp = (const T*)a.v.p + b * a.v.b + kv * a.v.h;
   Load load;
-  load.init(FEW ? 0 : wave, lane, a.head);
-  int counts = 0;   // FEW: lane i holds which keys of the i-th tile from here count; else: whether key `lane` of the next tile does
+  load.init(wave, lane, a.head, a.k.t, a.v.t);
   auto fetch = [&](int t, int buffer) {
-    // rows past the last key repeat it: what they hold is not used (see below)
-    load.issue([&](int j) { return min(t * KEYS + j, n - 1); }, [&](int key) { return kp + key * a.k.t; },
-               [&](int key) { return vp + key * a.v.t; }, mine_at + buffer * (4 * TILE), FEW ? 0 : wave);
-    if constexpr (!FEW) counts = key_word(a, b, t * KEYS + lane, n);
+    load.issue_tile(t, n, kp, a.k.t, vp, a.v.t, mine_at + buffer * (4 * TILE), wave, lane);
   };
+  // which keys of the next 32 tiles count, tile i in lane i
+  unsigned words[KEYS / 32];
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s)
+    if (t0 + s * GROUPS < t1) fetch(t0 + s * GROUPS, s);
   int buffer = 0;
-  if (t0 < t1) fetch(t0, 0);
-  for (int t = t0, turn = 0; t < t1; t += STEP, buffer ^= 1, ++turn) {
+  // the groups of a block make the same number of turns: they share its barriers
+  const int end = FEW ? t1 : t1 + group;
+  for (int t = t0, turn = 0; t < end; t += GROUPS, ++turn) {
     uint64_t valid;
-    if constexpr (FEW) {
-      // A mask's bytes are read for 32 tiles at a time: a wait for one of them would be a wait for all transfers behind it.
-      if (a.mask == nullptr) {
-        const int rest = n - t * KEYS;
-        valid = rest >= KEYS ? ~0ull : (1ull << rest) - 1;
-      } else {
-        if (turn % 32 == 0)
-          for (int i = 0; i < 32; ++i) {
-            const uint64_t word = __ballot(t + i * STEP < t1 && key_word(a, b, (t + i * STEP) * KEYS + col, n) != 0);
-            if (lane == i) counts = (int)word;
-          }
-        const uint32_t word = __builtin_amdgcn_readlane(counts, turn % 32);
-        valid = word == ~0u ? ~0ull : word;
-      }
+    if (a.mask == nullptr) {
+      const int rest = max(n - t * KEYS, 0);
+      valid = rest >= KEYS ? ~0ull : (1ull << rest) - 1;
     } else {
-      valid = __ballot(counts != 0);
+      // A mask's bytes are read for 32 tiles at a time: a wait for one of them is a wait for all transfers ahead of it.
+      if (turn % 32 == 0)
+        for (int i = 0; i < 32; ++i) {
+          const uint64_t word = __ballot(t + i * GROUPS < t1 && key_counts(a, b, (t + i * GROUPS) * KEYS + lane % KEYS, n));
+#pragma unroll
+          for (int k = 0; k < KEYS / 32; ++k) words[k] = lane == i ? (unsigned)(word >> (32 * k)) : words[k];
+        }
+      valid = (unsigned)__builtin_amdgcn_readlane(words[0], turn % 32);
+      valid |= KEYS == 64 ? (uint64_t)(unsigned)__builtin_amdgcn_readlane(words[KEYS / 32 - 1], turn % 32) << 32 : valid << 32;
     }
     T* vs = mine + (buffer * 2 + 1) * TILE;
     const unsigned ks_at = hide(mine_at + buffer * (4 * TILE) + rows_at), vs_at = hide(mine_at + (buffer * 4 + 2) * TILE + columns_at);
+    // the tile after next overwrites the one before this: its readers are done, in this wave or (barrier) in all
+    const int ahead = buffer == 0 ? STAGES - 1 : buffer - 1;
     if constexpr (FEW) {
-      // the other pair was read before; its readers are done
-      if (t + STEP < t1) {
+      if (t + (STAGES - 1) * GROUPS < t1) {
         wait_vm_lds<63>();
-        fetch(t + STEP, buffer ^ 1);
-        wait_vm<Load::COUNT>();
+        fetch(t + (STAGES - 1) * GROUPS, ahead);
+        wait_vm<Load::COUNT * (STAGES - 1)>();
       } else {
         wait_vm<0>();
       }
       __builtin_amdgcn_wave_barrier();
     } else {
-      wait_vm_lds<0>();
+      if (t + (STAGES - 2) * GROUPS < t1) wait_vm_lds<Load::COUNT * (STAGES - 2)>();
+      else wait_vm_lds<0>();
       block_barrier();
-      if (t + STEP < t1) fetch(t + STEP, buffer ^ 1);
+      if (t + (STAGES - 1) * GROUPS < t1) fetch(t + (STAGES - 1) * GROUPS, ahead);
     }
-    if (valid != ~0ull) {   // v's rows that do not count: a weight of zero must meet a zero
-      half8<T> zero = {};
-      for (int e = FEW ? lane : threadIdx.x; e < KEYS * (DP / 8); e += FEW ? 64 : 64 * WAVES)
-        if (!(valid >> (e / (DP / 8)) & 1)) __builtin_memcpy(vs + e * 8, &zero, 16);
-      if constexpr (FEW) {
-        wait_vm_lds<63>();
-        __builtin_amdgcn_wave_barrier();
-      } else {
-        wait_vm_lds<63>();
-        block_barrier();
-      }
-    }
+    buffer = buffer == STAGES - 1 ? 0 : buffer + 1;
+    if (GROUPS > 1 && !FEW && t >= t1) break;   // the group with a tile less has kept the last barrier
+    if (valid != ~0ull) zero_rows<T, DP, KEYS>(vs, valid, lane);
 
     float16_t s[KEYS / 32];
-    over_head<T, DP, KEYS / 32>(ks_at, 0, qf, s);
+    over_head<T, DP, KEYS / 32, (GROUPS > 1 && !FEW ? 2 : 4)>(ks_at, 0, qf, s);
     if (valid != ~0ull) {
 #pragma unroll
       for (int k = 0; k < KEYS / 32; ++k) {
@@ -130,11 +126,7 @@ __global__ __launch_bounds__(64 * WAVES) void attend16_kernel(const AttendArgs a
         for (int i = 0; i < 16; ++i) s[k][i] = word >> product_row(i, 0) & 1 ? s[k][i] : -INFINITY;
       }
     }
-    float top = s[0][0];
-#pragma unroll
-    for (int k = 0; k < KEYS / 32; ++k)
-#pragma unroll
-      for (int i = 0; i < 16; i += 2) top = max3(top, s[k][i], s[k][i + 1]);
+    float top = largest(s);
     top = max_of_halves(top) * unit;
     if (__any(top > base + 8.0f)) {   // also: the first keys of a row that count
       const float next = fmaxf(base, top);
@@ -167,8 +159,9 @@ __global__ __launch_bounds__(64 * WAVES) void attend16_kernel(const AttendArgs a
   }
   total = sum_of_halves(total);
 
-  const int64_t heads_rows = (int64_t)a.batch * a.kv_heads * a.rows, flat = (int64_t)bkv * a.rows + r;
-  if constexpr (!FEW) {
+  const int64_t heads_rows = (int64_t)a.batch * a.kv_heads * a.rows;
+  if constexpr (GROUPS == 1) {
+    const int64_t flat = (int64_t)bkv * a.rows + r;
     if (!row_here) return;
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     const float lse = total == 0.0f ? -INFINITY : (base + log2f(total)) * kLn2;
@@ -187,14 +180,12 @@ __global__ __launch_bounds__(64 * WAVES) void attend16_kernel(const AttendArgs a
         else store_four(out, at_d, a.head, f);
       }
   } else {
-    constexpr int LD = DP + 4;
-    static_assert(32 * LD * sizeof(float) <= 4 * TILE * sizeof(T), "a wave's result fits its tiles");
     __syncthreads();
     float* all_found = (float*)lds;
-    float* found = all_found + wave * (32 * LD);   // [row][value]
+    float* found = all_found + (group * ROWS + wave * 32 + col) * LD;
     if (h == 0) {
-      row_max[wave][col] = base;
-      row_total[wave][col] = total;
+      row_max[group][wave * 32 + col] = base;
+      row_total[group][wave * 32 + col] = total;
     }
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
@@ -203,23 +194,23 @@ __global__ __launch_bounds__(64 * WAVES) void attend16_kernel(const AttendArgs a
         float f[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) f[i] = acc[d][4 * i4 + i];
-        __builtin_memcpy(found + col * LD + d * 32 + 8 * i4 + 4 * h, f, 16);
+        __builtin_memcpy(found + d * 32 + 8 * i4 + 4 * h, f, 16);
       }
     __syncthreads();
-    for (int e = threadIdx.x; e < 32 * (DP / 4); e += 64 * WAVES) {
+    for (int e = threadIdx.x; e < ROWS * (DP / 4); e += THREADS) {
       const int j = e / (DP / 4), d = e % (DP / 4) * 4;
-      const int64_t rj = (int64_t)row_tile * 32 + j;
+      const int64_t rj = (int64_t)row_tile * ROWS + j;
       if (rj >= a.rows) continue;
       float top = row_max[0][j], all = 0.0f, f[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int k = 1; k < WAVES; ++k) top = fmaxf(top, row_max[k][j]);
+      for (int k = 1; k < GROUPS; ++k) top = fmaxf(top, row_max[k][j]);
       const float off = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-      for (int k = 0; k < WAVES; ++k) {
+      for (int k = 0; k < GROUPS; ++k) {
         const float w = exp2_(row_max[k][j] - off);
         all += w * row_total[k][j];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] += w * all_found[(k * 32 + j) * LD + d + i];
+        for (int i = 0; i < 4; ++i) f[i] += w * all_found[(k * ROWS + j) * LD + d + i];
       }
       const float inv = all == 0.0f ? 0.0f : 1.0f / all;
 #pragma unroll
@@ -235,13 +226,21 @@ __global__ __launch_bounds__(64 * WAVES) void attend16_kernel(const AttendArgs a
 
 template <typename T, int DP>
 void launch(const AttendArgs& a, bool few, hipStream_t st) {
-  const dim3 grid((unsigned)((int64_t)a.batch * a.kv_heads * a.row_tiles * a.splits));
-  if (few) hipLaunchKernelGGL((attend16_kernel<T, DP, 4, true>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((attend16_kernel<T, DP, 8, false>), grid, dim3(512), 0, st, a);
+  const int64_t blocks = (int64_t)a.batch * a.kv_heads * a.row_tiles * a.splits;
+  const dim3 grid((unsigned)blocks);
+  if (few) {
+    hipLaunchKernelGGL((attend16_kernel<T, DP, 1, 4, true, 2>), grid, dim3(256), 0, st, a);
+  } else if constexpr (DP > 64) {
+    hipLaunchKernelGGL((attend16_kernel<T, DP, 8, 1, false, 2>), grid, dim3(512), 0, st, a);
+  } else {
+    if (blocks <= 0) hipLaunchKernelGGL((attend16_kernel<T, DP, 4, 2, false, 2>), grid, dim3(512), 0, st, a);
+    else hipLaunchKernelGGL((attend16_kernel<T, DP, 4, 1, false, 3>), grid, dim3(256), 0, st, a);
+  }
 }
 
 }  // namespace
 
+int attend16_tile(int64_t head) { return head > 64 ? 256 : 128; }
 bool attend16_takes(const AttendArgs& a, int type) {
   return type != NNVHIP_TYPE_F32 && by_pieces(a.q, a.head) && by_pieces(a.k, a.head) && by_pieces(a.v, a.head);
 }

@@ -70,13 +70,6 @@ __device__ __forceinline__ void store_result(T* row, const float16_t (&acc)[DP /
       store_four(row, d * 32 + 8 * i4 + 4 * h, head, f);
     }
 }
-// rows of a tile that do not take part, as zeros
-template <typename T, int DP, int ROWS, int THREADS>
-__device__ __forceinline__ void zero_rows(T* tile, uint64_t valid) {
-  half8<T> none = {};
-  for (int e = threadIdx.x; e < ROWS * (DP / 8); e += THREADS)
-    if (!(valid >> (e / (DP / 8)) & 1)) __builtin_memcpy(tile + e * 8, &none, 16);
-}
 template <typename T, int PACKS, int THREADS>
 __device__ __forceinline__ void zero_all(T* lds) {
   half8<T> none = {};
@@ -85,7 +78,7 @@ __device__ __forceinline__ void zero_all(T* lds) {
 }
 
 template <typename T, int DP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void query_grad16_kernel(const AttendArgs a) {
+__global__ __launch_bounds__(64 * WAVES, 2) void query_grad16_kernel(const AttendArgs a) {
   constexpr int KEYS = 64, TILE = KEYS * DP;
   typedef PairLoad<T, DP, KEYS, WAVES> Load;
   __shared__ __attribute__((aligned(1024))) T lds[4 * TILE];
@@ -94,7 +87,7 @@ __global__ __launch_bounds__(64 * WAVES) void query_grad16_kernel(const AttendAr
   const int split = at % a.splits;
   at /= a.splits;
   const int row_tile = at % a.row_tiles;
-  const int bkv = at / a.row_tiles, b = bkv / a.kv_heads, kv = bkv % a.kv_heads;
+  const int b = (int)(at / a.row_tiles) % a.batch, kv = (int)(at / a.row_tiles) / a.batch, bkv = b * a.kv_heads + kv;
   const int n = keys_that_count(a, b);
   const int tiles = (n + KEYS - 1) / KEYS, per = (tiles + a.splits - 1) / a.splits;
   const int t0 = split * per, t1 = min(tiles, t0 + per);
@@ -114,11 +107,10 @@ __global__ __launch_bounds__(64 * WAVES) void query_grad16_kernel(const AttendAr
   const T* kp = (const T*)a.k.p + b * a.k.b + kv * a.k.h;
   const T* vp = (const T*)a.v.p + b * a.v.b + kv * a.v.h;
   Load load;
-  load.init(wave, lane, a.head);
+  load.init(wave, lane, a.head, a.k.t, a.v.t);
   int counts = 0;
   auto fetch = [&](int t, int buffer) {
-    load.issue([&](int j) { return min(t * KEYS + j, n - 1); }, [&](int key) { return kp + key * a.k.t; },
-               [&](int key) { return vp + key * a.v.t; }, lds_at + buffer * (4 * TILE), wave);
+    load.issue_tile(t, n, kp, a.k.t, vp, a.v.t, lds_at + buffer * (4 * TILE), wave, lane);
     counts = key_word(a, b, t * KEYS + lane, n);
   };
   int buffer = 0;
@@ -131,9 +123,7 @@ __global__ __launch_bounds__(64 * WAVES) void query_grad16_kernel(const AttendAr
     block_barrier();
     if (t + 1 < t1) fetch(t + 1, buffer ^ 1);
     if (valid != ~0ull) {
-      zero_rows<T, DP, KEYS, 64 * WAVES>(lds + buffer * 2 * TILE, valid);
-      wait_vm_lds<63>();
-      block_barrier();
+      zero_rows<T, DP, KEYS>(lds + buffer * 2 * TILE, valid, lane);
     }
 #pragma unroll
     for (int k = 0; k < KEYS / 32; ++k) {
@@ -172,7 +162,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void key_grad16_kernel(const AttendA
   const int split = at % a.splits;
   at /= a.splits;
   const int key_tile = at % a.key_tiles;
-  const int bkv = at / a.key_tiles, b = bkv / a.kv_heads, kv = bkv % a.kv_heads;
+  const int b = (int)(at / a.key_tiles) % a.batch, kv = (int)(at / a.key_tiles) / a.batch, bkv = b * a.kv_heads + kv;
   const int n = keys_that_count(a, b);
   const int key = key_tile * (32 * WAVES) + wave * 32 + col;
   const bool here = key < a.keys, counts = key_counts(a, b, key, n);
@@ -197,7 +187,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void key_grad16_kernel(const AttendA
   const float* lse = a.lse + (int64_t)bkv * a.rows;
   const float* del = a.delta + (int64_t)bkv * a.rows;
   Load load;
-  load.init(wave, lane, a.head);
+  load.init(wave, lane, a.head, a.q.t, a.go.t);
   const T* qp = (const T*)a.q.p + b * a.q.b + kv * (int64_t)a.group * a.q.h;
   const T* gp = (const T*)a.go.p + b * a.go.b + kv * (int64_t)a.group * a.go.h;
   const float per_query = 1.0f / a.queries;
@@ -209,13 +199,18 @@ __global__ __launch_bounds__(64 * WAVES, 2) void key_grad16_kernel(const AttendA
     // Head of the group and query of the tile's first row, then of every row: a tile reaches into the next head at most where heads have
     // ROWS queries, and the quotient is small where they have fewer.  Rows past the last one repeat it, and are made zeros below.
     const int g0 = (uint32_t)t * ROWS / (uint32_t)a.queries, i0 = t * ROWS - g0 * a.queries, last = (int)a.rows - 1 - g0 * a.queries;
-    auto where = [&](int j) {
-      const int i = min(i0 + j, last);
-      const int more = a.queries >= ROWS ? (int)(i >= a.queries) : (int)((i + 0.5f) * per_query);
-      return Place{g0 + more, i - more * a.queries};
-    };
-    load.issue(where, [&](Place w) { return qp + (w.query * a.q.t + w.head * a.q.h); },
-               [&](Place w) { return gp + (w.query * a.go.t + w.head * a.go.h); }, lds_at + buffer * (4 * TILE), wave);
+    const unsigned pair = lds_at + buffer * (4 * TILE);
+    if (i0 + ROWS <= a.queries) {
+      load.issue(qp + (i0 * a.q.t + g0 * a.q.h), gp + (i0 * a.go.t + g0 * a.go.h), pair, wave);
+    } else {
+      auto where = [&](int j) {
+        const int i = min(i0 + j, last);
+        const int more = a.queries >= ROWS ? (int)(i >= a.queries) : (int)((i + 0.5f) * per_query);
+        return Place{g0 + more, i - more * a.queries};
+      };
+      auto at_row = [&](const T* p, const TokenView& v, Place w) { return p + (w.query * v.t + w.head * v.h); };
+      load.issue_any([&](int j) { return at_row(qp, a.q, where(j)); }, [&](int j) { return at_row(gp, a.go, where(j)); }, pair, wave, lane);
+    }
     if (threadIdx.x < ROWS) {
       const int64_t r = (int64_t)t * ROWS + threadIdx.x;
       next_lse = r < a.rows ? lse[r] : -INFINITY;
@@ -235,10 +230,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void key_grad16_kernel(const AttendA
     if (t + 1 < t1) fetch(t + 1, buffer ^ 1);
     if ((int64_t)(t + 1) * ROWS > a.rows) {
       const uint64_t valid = (1ull << (int)(a.rows - (int64_t)t * ROWS)) - 1;
-      zero_rows<T, DP, ROWS, 64 * WAVES>(lds + buffer * 2 * TILE, valid);
-      zero_rows<T, DP, ROWS, 64 * WAVES>(lds + (buffer * 2 + 1) * TILE, valid);
-      wait_vm_lds<63>();
-      block_barrier();
+      zero_rows<T, DP, ROWS>(lds + buffer * 2 * TILE, valid, lane);
+      zero_rows<T, DP, ROWS>(lds + (buffer * 2 + 1) * TILE, valid, lane);
     }
 #pragma unroll 1
     for (int k = 0; k < ROWS / 32; ++k) {   // (both at once would need more registers than there are)
