@@ -184,30 +184,67 @@ __global__ __launch_bounds__(256) void attend_kernel(const AttendArgs a) {
   }
 }
 
-// o = sum over splits of exp(lse_s - lse) o_s: a wave per row, in the order of the splits.
-template <typename T>
+// o = sum over splits of exp(lse_s - lse) o_s, in the order of the splits within SLICES slices and of the slices: SLICES * 32 threads a
+// row, four values and every SLICES-th split each.
+template <typename T, int SLICES>
 __global__ __launch_bounds__(256) void join_kernel(const AttendArgs a) {
-  const int64_t all = (int64_t)a.batch * a.kv_heads * a.rows, flat = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (flat >= all) return;
-  const int lane = threadIdx.x & 63;
+  constexpr int ROWS = 8 / SLICES;
+  __shared__ float tops[8], totals[8], found[8][32][4];
+  const int64_t all = (int64_t)a.batch * a.kv_heads * a.rows;
+  const int slot = threadIdx.x / 32, slice = slot % SLICES, lane = threadIdx.x % 32, d = lane * 4;
+  const int64_t flat = (int64_t)blockIdx.x * ROWS + slot / SLICES;
+  const bool here = flat < all;
   float top = -INFINITY;
-  for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, a.part_lse[s * all + flat]);
+  if (here)
+    for (int s = slice * 32 + lane; s < a.splits; s += SLICES * 32) top = fmaxf(top, a.part_lse[s * all + flat]);
 #pragma unroll
-  for (int k = 32; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor(top, k, 64));
-  const float base = top == -INFINITY ? 0.0f : top;
-  float total = 0.0f, f0 = 0.0f, f1 = 0.0f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float w = exp2_((a.part_lse[s * all + flat] - base) * kLog2e);
-    const float* p = a.part + (s * all + flat) * a.head;
-    total += w;
-    if (lane < a.head) f0 += w * p[lane];
-    if (lane + 64 < a.head) f1 += w * p[lane + 64];
+  for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor(top, k, 64));
+  if constexpr (SLICES > 1) {
+    if (lane == 0) tops[slot] = top;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < SLICES; ++k) top = fmaxf(top, tops[slot - slice + k]);
   }
+  const float base = top == -INFINITY ? 0.0f : top;
+  float total = 0.0f, f[4] = {0, 0, 0, 0};
+  if (here)
+    for (int s = slice; s < a.splits; s += SLICES * 4) {
+      Four p[4];
+      float w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int sk = s + k * SLICES;
+        const bool one = sk < a.splits;
+        p[k] = load_four(a.part + ((one ? sk : 0) * all + flat) * a.head, d, a.head, one);
+        w[k] = one ? a.part_lse[sk * all + flat] : -INFINITY;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float e = exp2_((w[k] - base) * kLog2e);
+        total += e;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] += e * p[k].v[i];
+      }
+    }
+  if constexpr (SLICES > 1) {
+    if (lane == 0) totals[slot] = total;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) found[slot][lane][i] = f[i];
+    __syncthreads();
+    if (slice) return;
+#pragma unroll
+    for (int k = 1; k < SLICES; ++k) {
+      total += totals[slot + k];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] += found[slot + k][lane][i];
+    }
+  }
+  if (!here) return;
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] *= inv;
   const int bkv = (int)(flat / a.rows), b = bkv / a.kv_heads;
-  T* out = (T*)a.out + dense_row_at(a, b, bkv % a.kv_heads, flat % a.rows);
-  if (lane < a.head) out[lane] = from_f<T>(f0 * inv);
-  if (lane + 64 < a.head) out[lane + 64] = from_f<T>(f1 * inv);
+  if (d < a.head) store_four((T*)a.out + dense_row_at(a, b, bkv % a.kv_heads, flat % a.rows), d, a.head, f);
   if (lane == 0) a.lse[flat] = total == 0.0f ? -INFINITY : base + log2f(total) * kLn2;
 }
 
@@ -233,7 +270,9 @@ void launch_attend(const AttendArgs& a, bool few, hipStream_t st) {
 }
 template <typename T, int>
 void launch_join(const AttendArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)ceil_div((int64_t)a.batch * a.kv_heads * a.rows, 4)), dim3(256), 0, st, a);
+  const int64_t rows = (int64_t)a.batch * a.kv_heads * a.rows;
+  if (a.splits > 8) hipLaunchKernelGGL((join_kernel<T, 8>), dim3((unsigned)rows), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((join_kernel<T, 1>), dim3((unsigned)ceil_div(rows, 8)), dim3(256), 0, st, a);
 }
 
 // strides of the last tokens' rows have to be addressable, the sizes have to fit the kernels' indexes

@@ -16,12 +16,12 @@
 namespace nnvhip {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 512;   // of the kernels for long rows and of the backward pass
 
-// Sum of N values over the LPR consecutive lanes that share a row.  Rows of more than a wave add through LDS; `slot` alternates
-// between two sets of partial sums, so that one barrier per sum is enough (a wave can be at most one sum ahead of
-// another, and that one writes the other set).
-template <int LPR, int N>
+// Sum of N values over the LPR consecutive lanes that share a row, in a block of THREADS.  Rows of more than a wave add through LDS;
+// `slot` alternates between two sets of partial sums, so that one barrier per sum is enough (a wave can be at most one
+// sum ahead of another, and that one writes the other set).
+template <int LPR, int THREADS, int N>
 __device__ __forceinline__ void row_sum(float (&v)[N], float* lds, int& slot) {
   constexpr int kIn = LPR < 64 ? LPR : 64;
 #pragma unroll
@@ -31,7 +31,7 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float* lds, int& slot) {
   if constexpr (LPR > 64) {
     constexpr int kWaves = LPR / 64;
     const int wave = threadIdx.x >> 6;
-    float* part = lds + slot * (kThreads / 64 * N);
+    float* part = lds + slot * (THREADS / 64 * N);
     slot ^= 1;
     if ((threadIdx.x & 63) == 0)
 #pragma unroll
@@ -53,65 +53,87 @@ template <typename W>
 __device__ __forceinline__ float param(const W* p, int64_t c, float none) {
   return p ? to_f(p[c]) : none;
 }
+// a lane's scales or offsets for a pack of T
+template <typename T, typename W>
+struct Params {
+  Pack<W> p[kVec<T> / kVec<W>];
+  __device__ __forceinline__ void load(const W* from, int c, int size) {
+#pragma unroll
+    for (int k = 0; k < kVec<T> / kVec<W>; ++k) p[k] = load_pack(from + c + k * kVec<W>, from ? size - c - k * kVec<W> : 0);
+  }
+  __device__ __forceinline__ float operator[](int i) const { return to_f(p[i / kVec<W>].v[i % kVec<W>]); }
+};
 
+// LPR lanes a row, NV packs a lane, as many rows a block as its threads hold; a block takes rows in turn.  The next row is asked for
+// before the sums over this one, and the scales and offsets stay in registers over all rows.
 template <typename T, typename W, int LPR, int NV>
-__global__ __launch_bounds__(kThreads) void norm_kernel(const T* __restrict__ x, int64_t x_stride, const W* __restrict__ scale,
-                                                        const W* __restrict__ offset, float eps, int64_t rows, int size,
-                                                        T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
-  constexpr int V = kVec<T>, kRows = kThreads / LPR;
-  __shared__ float lds[2 * kThreads / 64];
+__global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_kernel(const T* __restrict__ x, int64_t x_stride, const W* __restrict__ scale,
+                                                                     const W* __restrict__ offset, float eps, int64_t rows, int size,
+                                                                     T* __restrict__ y, float* __restrict__ mean,
+                                                                     float* __restrict__ rstd) {
+  constexpr int V = kVec<T>, THREADS = LPR > 256 ? LPR : 256, kRows = THREADS / LPR;
+  __shared__ float lds[2 * THREADS / 64];
   int slot = 0;
-  const int lane = threadIdx.x % LPR;
-  const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / LPR;
-  const bool here = row < rows;
-  Pack<T> in[NV];
-  float s[1] = {0};
+  const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
+  Pack<T> in[NV], next[NV];
+  auto fetch = [&](int64_t row, Pack<T>(&to)[NV]) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * LPR + lane) * V;
+      to[j] = load_pack(x + (row < rows ? row : 0) * x_stride + c, row < rows ? size - c : 0);
+    }
+  };
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  int64_t row = (int64_t)blockIdx.x * kRows + group;
+  fetch(row, in);
+  Params<T, W> w[NV], b[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int c = (j * LPR + lane) * V;
-    in[j] = load_pack(x + (here ? row : 0) * x_stride + c, here ? size - c : 0);
-#pragma unroll
-    for (int i = 0; i < V; ++i) s[0] += to_f(in[j].v[i]);
+    w[j].load(scale, (j * LPR + lane) * V, size);
+    b[j].load(offset, (j * LPR + lane) * V, size);
   }
-  row_sum<LPR, 1>(s, lds, slot);
-  const float mu = s[0] / size;
-  float q[1] = {0};
+  // every row of a block's turn takes part in its barriers
+  for (int64_t first = (int64_t)blockIdx.x * kRows; first < rows; first += step, row += step) {
+    if (first + step < rows) fetch(row + step, next);
+    float s[1] = {0};
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int c = (j * LPR + lane) * V;
+    for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float d = to_f(in[j].v[i]) - mu;
-      q[0] += c + i < size ? d * d : 0.0f;
+      for (int i = 0; i < V; ++i) s[0] += to_f(in[j].v[i]);
+    row_sum<LPR, THREADS, 1>(s, lds, slot);
+    const float mu = s[0] / size;
+    float q[1] = {0};
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float d = to_f(in[j].v[i]) - mu;
+        q[0] += (j * LPR + lane) * V + i < size ? d * d : 0.0f;
+      }
+    row_sum<LPR, THREADS, 1>(q, lds, slot);
+    const float r = 1.0f / sqrtf(q[0] / size + eps);
+    if (row < rows) {
+      if (lane == 0) {
+        mean[row] = mu;
+        rstd[row] = r;
+      }
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int c = (j * LPR + lane) * V;
+        if (c >= size) break;
+        Pack<T> out;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          float v = (to_f(in[j].v[i]) - mu) * r;
+          if (scale) v *= w[j][i];
+          if (offset) v += b[j][i];
+          out.v[i] = from_f<T>(v);
+        }
+        store_pack(y + row * (int64_t)size + c, out, size - c);
+      }
     }
-  }
-  row_sum<LPR, 1>(q, lds, slot);
-  const float r = 1.0f / sqrtf(q[0] / size + eps);
-  if (!here) return;
-  if (lane == 0) {
-    mean[row] = mu;
-    rstd[row] = r;
-  }
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int c = (j * LPR + lane) * V;
-    if (c >= size) break;
-    Pack<W> w[V / kVec<W> ? V / kVec<W> : 1], b[V / kVec<W> ? V / kVec<W> : 1];
-    constexpr int VW = kVec<W>;
-#pragma unroll
-    for (int k = 0; k < V / VW; ++k) {
-      if (scale) w[k] = load_pack(scale + c + k * VW, size - c - k * VW);
-      if (offset) b[k] = load_pack(offset + c + k * VW, size - c - k * VW);
-    }
-    Pack<T> out;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      float v = (to_f(in[j].v[i]) - mu) * r;
-      if (scale) v *= to_f(w[i / VW].v[i % VW]);
-      if (offset) v += to_f(b[i / VW].v[i % VW]);
-      out.v[i] = from_f<T>(v);
-    }
-    store_pack(y + row * (int64_t)size + c, out, size - c);
+    for (int j = 0; j < NV; ++j) in[j] = next[j];
   }
 }
 
@@ -131,7 +153,7 @@ __global__ __launch_bounds__(kThreads) void norm_long_kernel(const T* __restrict
 #pragma unroll
     for (int i = 0; i < V; ++i) s[0] += to_f(in.v[i]);
   }
-  row_sum<kThreads, 1>(s, lds, slot);
+  row_sum<kThreads, kThreads, 1>(s, lds, slot);
   const float mu = s[0] / size;
   for (int64_t c = (int64_t)threadIdx.x * V; c < size; c += kThreads * V) {
     const Pack<T> in = load_pack(xr + c, size - c);
@@ -141,7 +163,7 @@ __global__ __launch_bounds__(kThreads) void norm_long_kernel(const T* __restrict
       q[0] += c + i < size ? d * d : 0.0f;
     }
   }
-  row_sum<kThreads, 1>(q, lds, slot);
+  row_sum<kThreads, kThreads, 1>(q, lds, slot);
   const float r = 1.0f / sqrtf(q[0] / size + eps);
   if (threadIdx.x == 0) {
     mean[row] = mu;
@@ -159,10 +181,11 @@ __global__ __launch_bounds__(kThreads) void norm_long_kernel(const T* __restrict
   }
 }
 
-// The backward pass.  A block's kThreads / LPR groups take rows in turn; every lane keeps the sums of its own columns of dw and
-// db in registers over all rows it sees.  At the end the groups of a block add theirs up in LDS, one after the other,
-// and the block writes one row of partial sums (or the result, when there is one block); column_sum_kernel adds those in
-// order.  No atomics: the same inputs give the same bits.
+// The backward pass.  A block's kThreads / LPR groups take rows in turn, the next one asked for ahead; every lane keeps the sums of its
+// own columns of dw and db in registers over all rows it sees.  At the end the groups of a block add theirs up in LDS, one
+// after the other, and the block writes one row of partial sums (or the result, when there is one block); column_sum_kernel
+// adds those in order.  No atomics: the same inputs give the same bits.  One block a CU: every block more would leave
+// 8 * size bytes of partial sums more, and with a row ahead two waves a SIMD keep the memory busy.
 template <typename T, typename W, int LPR, int NV>
 __global__ __launch_bounds__(kThreads) void norm_grad_kernel(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ x,
                                                              int64_t x_stride, const float* __restrict__ mean,
@@ -174,43 +197,49 @@ __global__ __launch_bounds__(kThreads) void norm_grad_kernel(const T* __restrict
   __shared__ float sums[2 * LPR * E];
   int slot = 0;
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
-  float dw[E], db[E], w[E];
-#pragma unroll
-  for (int j = 0; j < NV; ++j)
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int c = (j * LPR + lane) * V + i;
-      dw[j * V + i] = db[j * V + i] = 0.0f;
-      w[j * V + i] = c < size ? param(scale, c, 1.0f) : 0.0f;
-    }
-  // every group of a block makes the same number of turns: they share the barriers of row_sum
-  const int64_t turns = (rows + (int64_t)gridDim.x * kRows - 1) / ((int64_t)gridDim.x * kRows);
-  for (int64_t t = 0; t < turns; ++t) {
-    const int64_t row = (t * gridDim.x + blockIdx.x) * kRows + group;
+  struct Row {
+    Pack<T> x[NV], g[NV];
+    float mu, r;
+  } now, next;
+  auto fetch = [&](int64_t row, Row& to) {
     const bool here = row < rows;
     const int64_t at = here ? row : 0;
-    Pack<T> px[NV], pg[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * LPR + lane) * V;
-      px[j] = load_pack(x + at * x_stride + c, here ? size - c : 0);
-      pg[j] = load_pack(dy + at * dy_stride + c, here ? size - c : 0);
+      to.x[j] = load_pack(x + at * x_stride + c, here ? size - c : 0);
+      to.g[j] = load_pack(dy + at * dy_stride + c, here ? size - c : 0);
     }
-    const float mu = here ? mean[at] : 0.0f, r = here ? rstd[at] : 0.0f;
+    to.mu = here ? mean[at] : 0.0f;
+    to.r = here ? rstd[at] : 0.0f;
+  };
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  int64_t row = (int64_t)blockIdx.x * kRows + group;
+  fetch(row, now);
+  Params<T, W> w[NV];
+  float dw[E], db[E];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) w[j].load(scale, (j * LPR + lane) * V, size);
+#pragma unroll
+  for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.0f;
+  // every row of a block's turn takes part in its barriers
+  for (int64_t first = (int64_t)blockIdx.x * kRows; first < rows; first += step, row += step) {
+    if (first + step < rows) fetch(row + step, next);
+    const float mu = now.mu, r = now.r;
     float s[2] = {0, 0};
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float g = to_f(pg[j].v[i]), xh = (to_f(px[j].v[i]) - mu) * r, gw = g * w[j * V + i];
+        const float g = to_f(now.g[j].v[i]), xh = (to_f(now.x[j].v[i]) - mu) * r, gw = scale ? g * w[j][i] : g;
         dw[j * V + i] += g * xh;   // g is zero where there is no column or no row
         db[j * V + i] += g;
         s[0] += gw;
         s[1] += gw * xh;
       }
-    row_sum<LPR, 2>(s, lds, slot);
+    row_sum<LPR, kThreads, 2>(s, lds, slot);
     const float m0 = s[0] / size, m1 = s[1] / size;
-    if (here) {
+    if (row < rows) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int c = (j * LPR + lane) * V;
@@ -218,33 +247,33 @@ __global__ __launch_bounds__(kThreads) void norm_grad_kernel(const T* __restrict
         Pack<T> out;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float xh = (to_f(px[j].v[i]) - mu) * r;
-          out.v[i] = from_f<T>(r * (to_f(pg[j].v[i]) * w[j * V + i] - m0 - xh * m1));
+          const float g = to_f(now.g[j].v[i]), xh = (to_f(now.x[j].v[i]) - mu) * r;
+          out.v[i] = from_f<T>(r * ((scale ? g * w[j][i] : g) - m0 - xh * m1));
         }
         store_pack(dx + row * (int64_t)size + c, out, size - c);
       }
     }
+    now = next;
   }
   if (dscale == nullptr && doffset == nullptr) return;
   for (int g = 0; g < kRows; ++g) {
     if (group == g)
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int c = (j * LPR + lane) * V + i;
-          sums[c] = (g ? sums[c] : 0.0f) + dw[j * V + i];
-          sums[LPR * E + c] = (g ? sums[LPR * E + c] : 0.0f) + db[j * V + i];
-        }
+      for (int e = 0; e < E; ++e) {   // (a lane's values lie apart, so that neighbouring lanes meet neighbouring banks)
+        const int at = e * LPR + lane;
+        sums[at] = (g ? sums[at] : 0.0f) + dw[e];
+        sums[LPR * E + at] = (g ? sums[LPR * E + at] : 0.0f) + db[e];
+      }
     __syncthreads();
   }
   for (int c = threadIdx.x; c < size; c += kThreads) {
+    const int at = (c / V / LPR * V + c % V) * LPR + c / V % LPR;
     if (gridDim.x == 1) {
-      if (dscale) dscale[c] = from_f<W>(sums[c]);
-      if (doffset) doffset[c] = from_f<W>(sums[LPR * E + c]);
+      if (dscale) dscale[c] = from_f<W>(sums[at]);
+      if (doffset) doffset[c] = from_f<W>(sums[LPR * E + at]);
     } else {
-      part[((int64_t)blockIdx.x * 2 + 0) * size + c] = sums[c];
-      part[((int64_t)blockIdx.x * 2 + 1) * size + c] = sums[LPR * E + c];
+      part[((int64_t)blockIdx.x * 2 + 0) * size + c] = sums[at];
+      part[((int64_t)blockIdx.x * 2 + 1) * size + c] = sums[LPR * E + at];
     }
   }
 }
@@ -270,7 +299,7 @@ __global__ __launch_bounds__(kThreads) void norm_grad_long_kernel(const T* __res
       s[1] += gw * ((to_f(px.v[i]) - mu) * r);
     }
   }
-  row_sum<kThreads, 2>(s, lds, slot);
+  row_sum<kThreads, kThreads, 2>(s, lds, slot);
   const float m0 = s[0] / size, m1 = s[1] / size;
   for (int64_t c = (int64_t)threadIdx.x * V; c < size; c += kThreads * V) {
     const Pack<T> px = load_pack(x + row * x_stride + c, size - c), pg = load_pack(dy + row * dy_stride + c, size - c);
@@ -303,19 +332,25 @@ __global__ __launch_bounds__(256) void norm_grad_columns_kernel(const T* __restr
   part[((int64_t)blockIdx.y * 2 + 1) * size + c] = db;
 }
 
-// dscale / doffset = the partial sums added over `parts` rows.  16 columns a block, 16 threads a column; blockIdx.y: which of
-// the two.
+// dscale / doffset = the partial sums added over `parts` rows.  64 columns a block, 16 threads a column with up to 8 loads on the way;
+// blockIdx.y: which of the two.
 template <typename W>
-__global__ __launch_bounds__(256) void column_sum_kernel(const float* __restrict__ part, int64_t parts, int64_t size,
-                                                         W* __restrict__ dscale, W* __restrict__ doffset) {
-  __shared__ float lds[16][17];
+__global__ __launch_bounds__(1024) void column_sum_kernel(const float* __restrict__ part, int64_t parts, int64_t size,
+                                                          W* __restrict__ dscale, W* __restrict__ doffset) {
+  __shared__ float lds[16][64];
   W* out = blockIdx.y ? doffset : dscale;
   if (out == nullptr) return;
-  const int cx = threadIdx.x % 16, py = threadIdx.x / 16;
-  const int64_t c = (int64_t)blockIdx.x * 16 + cx;
+  const int cx = threadIdx.x % 64, py = threadIdx.x / 64;
+  const int64_t c = (int64_t)blockIdx.x * 64 + cx;
   float s = 0;
   if (c < size)
-    for (int64_t p = py; p < parts; p += 16) s += part[(p * 2 + blockIdx.y) * size + c];
+    for (int64_t p = py; p < parts; p += 16 * 8) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = p + 16 * k < parts ? part[((p + 16 * k) * 2 + blockIdx.y) * size + c] : 0.0f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += v[k];
+    }
   lds[py][cx] = s;
   __syncthreads();
   if (py == 0 && c < size) {
@@ -326,24 +361,25 @@ __global__ __launch_bounds__(256) void column_sum_kernel(const float* __restrict
   }
 }
 
-constexpr int64_t kLongest = 8192;  // values of a row that the registers of a block hold (16 a thread)
+constexpr int64_t kLongest = 8192;  // values of a row that the registers of a block hold
 
-// Blocks of the backward pass: every block leaves 8 * size bytes of partial sums, so there are no more than the chip holds at once,
-// and none that would see less than four turns.
+// Blocks of the backward pass: one a CU, and none that would see less than four turns.
 int64_t grad_blocks(int64_t rows, int64_t size, int type) {
   if (size > kLongest) return std::min<int64_t>(64, std::max<int64_t>(1, ceil_div(rows, 32)));
   const int64_t per = type == NNVHIP_TYPE_F32 ? 4 : 8;
   int64_t lpr = per == 8 ? 8 : 16;
   while (lpr < 64 && lpr * per < size) lpr *= 2;
   while (lpr * 16 < size) lpr *= 2;
-  return std::max<int64_t>(1, std::min<int64_t>(512, ceil_div(rows, kThreads / lpr * 4)));
+  return std::max<int64_t>(1, std::min<int64_t>(256, ceil_div(rows, kThreads / lpr * 4)));
 }
 
 template <typename T, typename W, int LPR, int NV>
 void launch_norm(const void* x, int64_t xs, const void* scale, const void* offset, float eps, int64_t rows, int64_t size, void* y,
                  float* mean, float* rstd, hipStream_t st) {
-  hipLaunchKernelGGL((norm_kernel<T, W, LPR, NV>), dim3((unsigned)ceil_div(rows, kThreads / LPR)), dim3(kThreads), 0, st, (const T*)x,
-                     xs, (const W*)scale, (const W*)offset, eps, rows, (int)size, (T*)y, mean, rstd);
+  constexpr int THREADS = LPR > 256 ? LPR : 256;
+  const int64_t blocks = std::min<int64_t>(ceil_div(rows, THREADS / LPR), 256 * (2048 / THREADS));   // as many as the chip holds
+  hipLaunchKernelGGL((norm_kernel<T, W, LPR, NV>), dim3((unsigned)blocks), dim3(THREADS), 0, st, (const T*)x, xs, (const W*)scale,
+                     (const W*)offset, eps, rows, (int)size, (T*)y, mean, rstd);
 }
 template <typename T, typename W, int LPR, int NV>
 void launch_norm_grad(const void* dy, int64_t dys, const void* x, int64_t xs, const float* mean, const float* rstd, const void* scale,
@@ -393,7 +429,7 @@ void norm_backward(const void* dy, int64_t dys, const void* x, int64_t xs, const
     if (blocks == 1) return;
   }
   if (dscale || doffset)
-    hipLaunchKernelGGL((column_sum_kernel<W>), dim3((unsigned)ceil_div(size, 16), 2), dim3(256), 0, st, part, blocks, size, (W*)dscale,
+    hipLaunchKernelGGL((column_sum_kernel<W>), dim3((unsigned)ceil_div(size, 64), 2), dim3(1024), 0, st, part, blocks, size, (W*)dscale,
                        (W*)doffset);
 }
 
