@@ -3,6 +3,8 @@
 #pragma once
 #include "internal.h"
 
+#include <type_traits>
+
 namespace nnvhip {
 
 using bf16_t = __bf16;
@@ -14,9 +16,19 @@ using f16_t = _Float16;
 template <typename T>
 constexpr int kVec = 16 / (int)sizeof(T);
 
+// (The pack is kept as the four words it is loaded as: taken apart where it is loaded, a pack that is asked for ahead would be
+// waited for at once.)
 template <typename T>
 struct Pack {
-  T v[kVec<T>];
+  unsigned w[4];
+  __device__ __forceinline__ T operator[](int i) const {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, w[i]);
+    else return __builtin_bit_cast(T, (uint16_t)(w[i / 2] >> (16 * (i & 1))));
+  }
+  __device__ __forceinline__ void set(int i, T x) {   // in ascending order: an even element clears its neighbour
+    if constexpr (sizeof(T) == 4) w[i] = __builtin_bit_cast(unsigned, x);
+    else w[i / 2] = i & 1 ? (w[i / 2] & 0xffffu) | (unsigned)__builtin_bit_cast(uint16_t, x) << 16 : (unsigned)__builtin_bit_cast(uint16_t, x);
+  }
 };
 
 // n of the pack's elements exist (n >= kVec: all); the others read as zero and are not touched in memory.
@@ -24,21 +36,21 @@ template <typename T>
 __device__ __forceinline__ Pack<T> load_pack(const T* p, int64_t n) {
   Pack<T> r;
   if (n >= kVec<T>) {
-    __builtin_memcpy(&r, p, sizeof(r));
+    __builtin_memcpy(r.w, p, 16);
   } else {
 #pragma unroll
-    for (int i = 0; i < kVec<T>; ++i) r.v[i] = i < n ? p[i] : (T)0.0f;
+    for (int i = 0; i < kVec<T>; ++i) r.set(i, i < n ? p[i] : (T)0.0f);
   }
   return r;
 }
 template <typename T>
 __device__ __forceinline__ void store_pack(T* p, const Pack<T>& r, int64_t n) {
   if (n >= kVec<T>) {
-    __builtin_memcpy(p, &r, sizeof(r));
+    __builtin_memcpy(p, r.w, 16);
   } else {
 #pragma unroll
     for (int i = 0; i < kVec<T>; ++i)
-      if (i < n) p[i] = r.v[i];
+      if (i < n) p[i] = r[i];
   }
 }
 
@@ -49,6 +61,23 @@ __device__ __forceinline__ float to_f(T x) {
 template <typename T>
 __device__ __forceinline__ T from_f(float x) {  // to nearest, ties to even
   return (T)x;
+}
+
+// Sum over the W consecutive lanes (a power of two) that a lane is one of; every one of them gets it.  On the vector units alone: through
+// LDS the six steps of a wave would take some 100 cycles each.
+template <int W>
+__device__ __forceinline__ float lanes_sum(float x) {
+  auto dpp = [&](auto ctrl) {
+    x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  if constexpr (W >= 2) dpp(std::integral_constant<int, 0xb1>());    // lane ^ 1 (quad_perm)
+  if constexpr (W >= 4) dpp(std::integral_constant<int, 0x4e>());    // lane ^ 2
+  if constexpr (W >= 8) dpp(std::integral_constant<int, 0x141>());   // the other four of eight (row_half_mirror)
+  if constexpr (W >= 16) dpp(std::integral_constant<int, 0x140>());  // the other eight of sixteen (row_mirror)
+  const auto both = [](auto r) { return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]); };
+  if constexpr (W >= 32) x = both(__builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false));
+  if constexpr (W >= 64) x = both(__builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false));
+  return x;
 }
 
 // Selects the context's device for the life of an entry point.  The operators on points run on the stream the caller names

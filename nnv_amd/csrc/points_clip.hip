@@ -58,7 +58,7 @@ __device__ __forceinline__ double tile_squares(const T* p, int64_t n) {
   for (int j = 0; j < kPacks; ++j)
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const double d = (double)to_f(in[j].v[i]);
+      const double d = (double)to_f(in[j][i]);
       s = fma(d, d, s);
     }
   return s;
@@ -103,9 +103,10 @@ __device__ __forceinline__ void tile_scale(const T* p, T* out, int64_t n, float 
 #pragma unroll
   for (int j = 0; j < kPacks; ++j) {
     const int64_t c = (int64_t)(j * kThreads + threadIdx.x) * V;
+    Pack<T> scaled;
 #pragma unroll
-    for (int i = 0; i < V; ++i) in[j].v[i] = from_f<T>(to_f(in[j].v[i]) * f);
-    store_pack(out + c, in[j], n - c);
+    for (int i = 0; i < V; ++i) scaled.set(i, from_f<T>(to_f(in[j][i]) * f));
+    store_pack(out + c, scaled, n - c);
   }
 }
 

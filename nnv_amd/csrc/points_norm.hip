@@ -16,18 +16,17 @@
 namespace nnvhip {
 namespace {
 
-constexpr int kThreads = 512;   // of the kernels for long rows and of the backward pass
+constexpr int kThreads = 512;       // of the kernels for long rows
+constexpr int kAhead = 3;           // rows that a group of lanes has asked for
+constexpr int kGradThreads = 512;   // of the backward pass
 
 // Sum of N values over the LPR consecutive lanes that share a row, in a block of THREADS.  Rows of more than a wave add through LDS;
 // `slot` alternates between two sets of partial sums, so that one barrier per sum is enough (a wave can be at most one
 // sum ahead of another, and that one writes the other set).
 template <int LPR, int THREADS, int N>
 __device__ __forceinline__ void row_sum(float (&v)[N], float* lds, int& slot) {
-  constexpr int kIn = LPR < 64 ? LPR : 64;
 #pragma unroll
-  for (int s = kIn / 2; s > 0; s >>= 1)
-#pragma unroll
-    for (int k = 0; k < N; ++k) v[k] += __shfl_xor(v[k], s, 64);
+  for (int k = 0; k < N; ++k) v[k] = lanes_sum<(LPR < 64 ? LPR : 64)>(v[k]);
   if constexpr (LPR > 64) {
     constexpr int kWaves = LPR / 64;
     const int wave = threadIdx.x >> 6;
@@ -61,11 +60,11 @@ struct Params {
 #pragma unroll
     for (int k = 0; k < kVec<T> / kVec<W>; ++k) p[k] = load_pack(from + c + k * kVec<W>, from ? size - c - k * kVec<W> : 0);
   }
-  __device__ __forceinline__ float operator[](int i) const { return to_f(p[i / kVec<W>].v[i % kVec<W>]); }
+  __device__ __forceinline__ float operator[](int i) const { return to_f(p[i / kVec<W>][i % kVec<W>]); }
 };
 
-// LPR lanes a row, NV packs a lane, as many rows a block as its threads hold; a block takes rows in turn.  The next row is asked for
-// before the sums over this one, and the scales and offsets stay in registers over all rows.
+// LPR lanes a row, NV packs a lane, as many rows a block as its threads hold; a block takes rows in turn.  kAhead rows are on their
+// way while one is worked on, and the scales and offsets stay in registers over all rows.
 template <typename T, typename W, int LPR, int NV>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_kernel(const T* __restrict__ x, int64_t x_stride, const W* __restrict__ scale,
                                                                      const W* __restrict__ offset, float eps, int64_t rows, int size,
@@ -75,7 +74,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_kernel(const T* __
   __shared__ float lds[2 * THREADS / 64];
   int slot = 0;
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
-  Pack<T> in[NV], next[NV];
+  Pack<T> ring[kAhead][NV];
   auto fetch = [&](int64_t row, Pack<T>(&to)[NV]) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -85,33 +84,33 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_kernel(const T* __
   };
   const int64_t step = (int64_t)gridDim.x * kRows;
   int64_t row = (int64_t)blockIdx.x * kRows + group;
-  fetch(row, in);
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) fetch(row + k * step, ring[k]);
   Params<T, W> w[NV], b[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     w[j].load(scale, (j * LPR + lane) * V, size);
     b[j].load(offset, (j * LPR + lane) * V, size);
   }
-  // every row of a block's turn takes part in its barriers
-  for (int64_t first = (int64_t)blockIdx.x * kRows; first < rows; first += step, row += step) {
-    if (first + step < rows) fetch(row + step, next);
+  const float per = 1.0f / size;
+  auto turn = [&](const Pack<T>(&in)[NV]) {
     float s[1] = {0};
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int i = 0; i < V; ++i) s[0] += to_f(in[j].v[i]);
+      for (int i = 0; i < V; ++i) s[0] += to_f(in[j][i]);
     row_sum<LPR, THREADS, 1>(s, lds, slot);
-    const float mu = s[0] / size;
+    const float mu = s[0] / size;   // (times 1 / size, the mean of equal values would not be that value)
     float q[1] = {0};
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float d = to_f(in[j].v[i]) - mu;
+        const float d = to_f(in[j][i]) - mu;
         q[0] += (j * LPR + lane) * V + i < size ? d * d : 0.0f;
       }
     row_sum<LPR, THREADS, 1>(q, lds, slot);
-    const float r = 1.0f / sqrtf(q[0] / size + eps);
+    const float r = 1.0f / sqrtf(q[0] * per + eps);
     if (row < rows) {
       if (lane == 0) {
         mean[row] = mu;
@@ -124,16 +123,26 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_kernel(const T* __
         Pack<T> out;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          float v = (to_f(in[j].v[i]) - mu) * r;
+          float v = (to_f(in[j][i]) - mu) * r;
           if (scale) v *= w[j][i];
           if (offset) v += b[j][i];
-          out.v[i] = from_f<T>(v);
+          out.set(i, from_f<T>(v));
         }
         store_pack(y + row * (int64_t)size + c, out, size - c);
       }
     }
+  };
+  // every row of a block's turn takes part in its barriers
+  for (int64_t first = (int64_t)blockIdx.x * kRows; first < rows;) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) in[j] = next[j];
+    for (int k = 0; k < kAhead; ++k) {
+      if (first < rows) {
+        turn(ring[k]);
+        fetch(row + kAhead * step, ring[k]);
+        first += step;
+        row += step;
+      }
+    }
   }
 }
 
@@ -151,7 +160,7 @@ __global__ __launch_bounds__(kThreads) void norm_long_kernel(const T* __restrict
   for (int64_t c = (int64_t)threadIdx.x * V; c < size; c += kThreads * V) {
     const Pack<T> in = load_pack(xr + c, size - c);
 #pragma unroll
-    for (int i = 0; i < V; ++i) s[0] += to_f(in.v[i]);
+    for (int i = 0; i < V; ++i) s[0] += to_f(in[i]);
   }
   row_sum<kThreads, kThreads, 1>(s, lds, slot);
   const float mu = s[0] / size;
@@ -159,7 +168,7 @@ __global__ __launch_bounds__(kThreads) void norm_long_kernel(const T* __restrict
     const Pack<T> in = load_pack(xr + c, size - c);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float d = to_f(in.v[i]) - mu;
+      const float d = to_f(in[i]) - mu;
       q[0] += c + i < size ? d * d : 0.0f;
     }
   }
@@ -175,32 +184,32 @@ __global__ __launch_bounds__(kThreads) void norm_long_kernel(const T* __restrict
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int64_t at = c + i < size ? c + i : size - 1;
-      out.v[i] = from_f<T>((to_f(in.v[i]) - mu) * r * param(scale, at, 1.0f) + param(offset, at, 0.0f));
+      out.set(i, from_f<T>((to_f(in[i]) - mu) * r * param(scale, at, 1.0f) + param(offset, at, 0.0f)));
     }
     store_pack(y + row * size + c, out, size - c);
   }
 }
 
-// The backward pass.  A block's kThreads / LPR groups take rows in turn, the next one asked for ahead; every lane keeps the sums of its
+// The backward pass.  A block's kGradThreads / LPR groups take rows in turn, kAhead of them on their way; every lane keeps the sums of its
 // own columns of dw and db in registers over all rows it sees.  At the end the groups of a block add theirs up in LDS, one
 // after the other, and the block writes one row of partial sums (or the result, when there is one block); column_sum_kernel
 // adds those in order.  No atomics: the same inputs give the same bits.  One block a CU: every block more would leave
-// 8 * size bytes of partial sums more, and with a row ahead two waves a SIMD keep the memory busy.
+// 8 * size bytes of partial sums more, and with rows ahead two waves a SIMD keep the memory busy.
 template <typename T, typename W, int LPR, int NV>
-__global__ __launch_bounds__(kThreads) void norm_grad_kernel(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ x,
+__global__ __launch_bounds__(kGradThreads) void norm_grad_kernel(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ x,
                                                              int64_t x_stride, const float* __restrict__ mean,
                                                              const float* __restrict__ rstd, const W* __restrict__ scale,
                                                              int64_t rows, int size, T* __restrict__ dx, W* __restrict__ dscale,
                                                              W* __restrict__ doffset, float* __restrict__ part) {
-  constexpr int V = kVec<T>, kRows = kThreads / LPR, E = NV * V;
-  __shared__ float lds[4 * kThreads / 64];
+  constexpr int V = kVec<T>, kRows = kGradThreads / LPR, E = NV * V;
+  __shared__ float lds[4 * kGradThreads / 64];
   __shared__ float sums[2 * LPR * E];
   int slot = 0;
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
   struct Row {
     Pack<T> x[NV], g[NV];
     float mu, r;
-  } now, next;
+  } ring[kAhead];
   auto fetch = [&](int64_t row, Row& to) {
     const bool here = row < rows;
     const int64_t at = here ? row : 0;
@@ -215,30 +224,30 @@ __global__ __launch_bounds__(kThreads) void norm_grad_kernel(const T* __restrict
   };
   const int64_t step = (int64_t)gridDim.x * kRows;
   int64_t row = (int64_t)blockIdx.x * kRows + group;
-  fetch(row, now);
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) fetch(row + k * step, ring[k]);
   Params<T, W> w[NV];
   float dw[E], db[E];
 #pragma unroll
   for (int j = 0; j < NV; ++j) w[j].load(scale, (j * LPR + lane) * V, size);
 #pragma unroll
   for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.0f;
-  // every row of a block's turn takes part in its barriers
-  for (int64_t first = (int64_t)blockIdx.x * kRows; first < rows; first += step, row += step) {
-    if (first + step < rows) fetch(row + step, next);
+  const float per = 1.0f / size;
+  auto turn = [&](const Row& now) {
     const float mu = now.mu, r = now.r;
     float s[2] = {0, 0};
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float g = to_f(now.g[j].v[i]), xh = (to_f(now.x[j].v[i]) - mu) * r, gw = scale ? g * w[j][i] : g;
+        const float g = to_f(now.g[j][i]), xh = (to_f(now.x[j][i]) - mu) * r, gw = scale ? g * w[j][i] : g;
         dw[j * V + i] += g * xh;   // g is zero where there is no column or no row
         db[j * V + i] += g;
         s[0] += gw;
         s[1] += gw * xh;
       }
-    row_sum<LPR, kThreads, 2>(s, lds, slot);
-    const float m0 = s[0] / size, m1 = s[1] / size;
+    row_sum<LPR, kGradThreads, 2>(s, lds, slot);
+    const float m0 = s[0] * per, m1 = s[1] * per;
     if (row < rows) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
@@ -247,13 +256,24 @@ __global__ __launch_bounds__(kThreads) void norm_grad_kernel(const T* __restrict
         Pack<T> out;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float g = to_f(now.g[j].v[i]), xh = (to_f(now.x[j].v[i]) - mu) * r;
-          out.v[i] = from_f<T>(r * ((scale ? g * w[j][i] : g) - m0 - xh * m1));
+          const float g = to_f(now.g[j][i]), xh = (to_f(now.x[j][i]) - mu) * r;
+          out.set(i, from_f<T>(r * ((scale ? g * w[j][i] : g) - m0 - xh * m1)));
         }
         store_pack(dx + row * (int64_t)size + c, out, size - c);
       }
     }
-    now = next;
+  };
+  // every row of a block's turn takes part in its barriers
+  for (int64_t first = (int64_t)blockIdx.x * kRows; first < rows;) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (first < rows) {
+        turn(ring[k]);
+        fetch(row + kAhead * step, ring[k]);
+        first += step;
+        row += step;
+      }
+    }
   }
   if (dscale == nullptr && doffset == nullptr) return;
   for (int g = 0; g < kRows; ++g) {
@@ -266,7 +286,7 @@ __global__ __launch_bounds__(kThreads) void norm_grad_kernel(const T* __restrict
       }
     __syncthreads();
   }
-  for (int c = threadIdx.x; c < size; c += kThreads) {
+  for (int c = threadIdx.x; c < size; c += kGradThreads) {
     const int at = (c / V / LPR * V + c % V) * LPR + c / V % LPR;
     if (gridDim.x == 1) {
       if (dscale) dscale[c] = from_f<W>(sums[at]);
@@ -294,9 +314,9 @@ __global__ __launch_bounds__(kThreads) void norm_grad_long_kernel(const T* __res
     const Pack<T> px = load_pack(x + row * x_stride + c, size - c), pg = load_pack(dy + row * dy_stride + c, size - c);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float gw = c + i < size ? to_f(pg.v[i]) * param(scale, c + i, 1.0f) : 0.0f;
+      const float gw = c + i < size ? to_f(pg[i]) * param(scale, c + i, 1.0f) : 0.0f;
       s[0] += gw;
-      s[1] += gw * ((to_f(px.v[i]) - mu) * r);
+      s[1] += gw * ((to_f(px[i]) - mu) * r);
     }
   }
   row_sum<kThreads, kThreads, 2>(s, lds, slot);
@@ -306,8 +326,8 @@ __global__ __launch_bounds__(kThreads) void norm_grad_long_kernel(const T* __res
     Pack<T> out;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float gw = c + i < size ? to_f(pg.v[i]) * param(scale, c + i, 1.0f) : 0.0f;
-      out.v[i] = from_f<T>(r * (gw - m0 - (to_f(px.v[i]) - mu) * r * m1));
+      const float gw = c + i < size ? to_f(pg[i]) * param(scale, c + i, 1.0f) : 0.0f;
+      out.set(i, from_f<T>(r * (gw - m0 - (to_f(px[i]) - mu) * r * m1)));
     }
     store_pack(dx + row * size + c, out, size - c);
   }
@@ -370,21 +390,21 @@ int64_t grad_blocks(int64_t rows, int64_t size, int type) {
   int64_t lpr = per == 8 ? 8 : 16;
   while (lpr < 64 && lpr * per < size) lpr *= 2;
   while (lpr * 16 < size) lpr *= 2;
-  return std::max<int64_t>(1, std::min<int64_t>(256, ceil_div(rows, kThreads / lpr * 4)));
+  return std::max<int64_t>(1, std::min<int64_t>(256, ceil_div(rows, kGradThreads / lpr * 4)));
 }
 
 template <typename T, typename W, int LPR, int NV>
 void launch_norm(const void* x, int64_t xs, const void* scale, const void* offset, float eps, int64_t rows, int64_t size, void* y,
                  float* mean, float* rstd, hipStream_t st) {
   constexpr int THREADS = LPR > 256 ? LPR : 256;
-  const int64_t blocks = std::min<int64_t>(ceil_div(rows, THREADS / LPR), 256 * (2048 / THREADS));   // as many as the chip holds
+  const int64_t blocks = std::min<int64_t>(ceil_div(rows, THREADS / LPR), 256 * (1024 / THREADS));   // as many as the chip holds at once
   hipLaunchKernelGGL((norm_kernel<T, W, LPR, NV>), dim3((unsigned)blocks), dim3(THREADS), 0, st, (const T*)x, xs, (const W*)scale,
                      (const W*)offset, eps, rows, (int)size, (T*)y, mean, rstd);
 }
 template <typename T, typename W, int LPR, int NV>
 void launch_norm_grad(const void* dy, int64_t dys, const void* x, int64_t xs, const float* mean, const float* rstd, const void* scale,
                       int64_t rows, int64_t size, void* dx, void* dscale, void* doffset, float* part, int64_t blocks, hipStream_t st) {
-  hipLaunchKernelGGL((norm_grad_kernel<T, W, LPR, NV>), dim3((unsigned)blocks), dim3(kThreads), 0, st, (const T*)dy, dys, (const T*)x,
+  hipLaunchKernelGGL((norm_grad_kernel<T, W, LPR, NV>), dim3((unsigned)blocks), dim3(kGradThreads), 0, st, (const T*)dy, dys, (const T*)x,
                      xs, mean, rstd, (const W*)scale, rows, (int)size, (T*)dx, (W*)dscale, (W*)doffset, part);
 }
 
