@@ -229,7 +229,8 @@ void launch(const AttendArgs& a, bool few, hipStream_t st) {
   const int64_t blocks = (int64_t)a.batch * a.kv_heads * a.row_tiles * a.splits;
   const dim3 grid((unsigned)blocks);
   if (few) {
-    hipLaunchKernelGGL((attend16_kernel<T, DP, 1, 4, true, 2>), grid, dim3(256), 0, st, a);
+    constexpr int GROUPS = DP > 64 ? 4 : 8;
+    hipLaunchKernelGGL((attend16_kernel<T, DP, 1, GROUPS, true, 2>), grid, dim3(64 * GROUPS), 0, st, a);
   } else if constexpr (DP > 64) {
     hipLaunchKernelGGL((attend16_kernel<T, DP, 8, 1, false, 2>), grid, dim3(512), 0, st, a);
   } else {

@@ -24,6 +24,10 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _INT64 = C.c_int64
 
 
+_stream_of = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _enter(what, ctx, first, *others):
     """(context, its library, device, stream) for tensors that have to be on that context's GPU."""
     if not isinstance(first, torch.Tensor):
@@ -38,9 +42,10 @@ def _enter(what, ctx, first, *others):
             if t.device != device:
                 raise ValueError("%s: the tensors must be on one GPU" % what)
     ctx = ctx or default_context()
-    if device.index != ctx.device:
-        raise ValueError("%s: the tensors are on GPU %d, the context is GPU %d's" % (what, device.index, ctx.device))
-    return ctx, ctx.lib, device, torch.cuda.current_stream(device).cuda_stream
+    index = device.index
+    if index != ctx.device:
+        raise ValueError("%s: the tensors are on GPU %d, the context is GPU %d's" % (what, index, ctx.device))
+    return ctx, ctx.lib, device, _stream_of(index)
 
 
 def _type(what, t):
@@ -70,13 +75,14 @@ def _as_rows(x):
 
 def _norm_params(what, x, scale, offset):
     t = _type(what, x)
-    if x.dim() < 1 or x.shape[-1] < 1:
+    size = x.shape[-1] if x.dim() else 0
+    if size < 1:
         raise ValueError("%s: rows of at least one value are expected" % what)
     w = t
     for p in (scale, offset):
         if p is not None:
-            if p.dim() != 1 or p.shape[0] != x.shape[-1]:
-                raise ValueError("%s: scale and offset have one value per channel (%d), not the shape %s" % (what, x.shape[-1], tuple(p.shape)))
+            if p.shape != (size,):
+                raise ValueError("%s: scale and offset have one value per channel (%d), not the shape %s" % (what, size, tuple(p.shape)))
             w = _type(what, p)
             if w not in (t, 0):
                 raise ValueError("%s: scale and offset have the type of the values, or float32" % what)
@@ -98,13 +104,14 @@ def layer_norm(x, scale=None, offset=None, epsilon=1e-5, ctx=None):
     t, w = _norm_params("layer_norm", x, scale, offset)
     if not epsilon >= 0:
         raise ValueError("layer_norm: epsilon must not be negative")
-    lead, size = x.shape[:-1], x.shape[-1]
+    shape = x.shape
+    lead, size = shape[:-1], shape[-1]
     scale = scale if scale is None else scale.contiguous()
     offset = offset if offset is None else offset.contiguous()
     rows_of, rows, stride = _as_rows(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=device)
-    mean = torch.empty(lead, dtype=torch.float32, device=device)
-    rstd = torch.empty(lead, dtype=torch.float32, device=device)
+    y = x.new_empty(shape)
+    mean = x.new_empty(lead, dtype=torch.float32)
+    rstd = x.new_empty(lead, dtype=torch.float32)
     check(lib.nnvhip_layer_norm(ctx.handle, t, w, rows, size, rows_of.data_ptr(), stride, _ptr(scale), _ptr(offset), epsilon,
                                 y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), stream))
     return y, mean, rstd
@@ -134,11 +141,11 @@ def layer_norm_backward(dy, x, mean, rstd, scale=None, ctx=None):
     mean, rstd = mean.contiguous(), rstd.contiguous()
     xr, rows, xs = _as_rows(x)
     gr, _, gs = _as_rows(dy)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=device)
-    grads = torch.empty((2, size), dtype=x.dtype if scale is None else scale.dtype, device=device)
-    dscale, doffset = grads.unbind(0)
+    dx = x.new_empty(x.shape)
+    like = x if scale is None else scale
+    dscale, doffset = like.new_empty((size,)), like.new_empty((size,))
     need = _norm_workspace(lib, t, rows, size)
-    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    work = x.new_empty((need,), dtype=torch.uint8) if need else None
     check(lib.nnvhip_layer_norm_backward(ctx.handle, t, w, rows, size, gr.data_ptr(), gs, xr.data_ptr(), xs, mean.data_ptr(),
                                          rstd.data_ptr(), _ptr(scale), dx.data_ptr(), dscale.data_ptr(), doffset.data_ptr(),
                                          _ptr(work), need, stream))
@@ -201,13 +208,13 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None, ctx=No
     sizes = _attention_sizes(what, q, k, v, key_lengths, key_mask)
     q, k, v = _dense_values(q), _dense_values(k), _dense_values(v)
     lengths, mask_stride = _mask_args(key_lengths, key_mask)
-    o = torch.empty(q.shape, dtype=q.dtype, device=device)
-    lse = torch.empty((sizes[1], sizes[4], sizes[2]), dtype=torch.float32, device=device)
+    o = q.new_empty(q.shape)
+    lse = q.new_empty((sizes[1], sizes[4], sizes[2]), dtype=torch.float32)
     d = _ATTENTION.pack(*sizes, sizes[6] ** -0.5 if scale is None else scale, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                         *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], _ptr(lengths) or 0, _ptr(key_mask) or 0,
                         *mask_stride, o.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, 0, 0, 0)
     need = _attention_workspace(lib, False, *sizes)
-    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    work = q.new_empty((need,), dtype=torch.uint8) if need else None
     check(lib.nnvhip_cross_attention(ctx.handle, d, _ptr(work), need, stream))
     return o, lse
 
@@ -225,15 +232,13 @@ def cross_attention_backward(do, q, k, v, o, lse, key_lengths=None, key_mask=Non
     q, k, v, do = _dense_values(q), _dense_values(k), _dense_values(v), _dense_values(do)
     o, lse = o.contiguous(), lse.contiguous()
     lengths, mask_stride = _mask_args(key_lengths, key_mask)
-    dq = torch.empty(q.shape, dtype=q.dtype, device=device)
-    dk = torch.empty(k.shape, dtype=q.dtype, device=device)
-    dv = torch.empty(k.shape, dtype=q.dtype, device=device)
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
     d = _ATTENTION.pack(*sizes, sizes[6] ** -0.5 if scale is None else scale, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                         *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], _ptr(lengths) or 0, _ptr(key_mask) or 0,
                         *mask_stride, o.data_ptr(), lse.data_ptr(), do.data_ptr(), *do.stride()[:3], dq.data_ptr(),
                         dk.data_ptr(), dv.data_ptr())
     need = _attention_workspace(lib, True, *sizes)
-    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    work = q.new_empty((need,), dtype=torch.uint8) if need else None
     check(lib.nnvhip_cross_attention_backward(ctx.handle, d, _ptr(work), need, stream))
     return dq, dk, dv
 
@@ -262,36 +267,44 @@ def clip_gradients(gradients, threshold, out=None, ctx=None):
     if not gradients:
         ctx = ctx or default_context()
         return [], torch.zeros((), dtype=torch.float32, device=torch.device("cuda", ctx.device))
-    ctx, lib, device, stream = _enter(what, ctx, *gradients)
-    types = [_type(what, g) for g in gradients]
-    dense = [g if g.is_contiguous() else g.contiguous() for g in gradients]
-    back = None
-    if out is None:
-        out = result = [torch.empty(g.shape, dtype=g.dtype, device=device) for g in gradients]
-    else:
-        out = list(out)
-        if len(out) != len(gradients):
-            raise ValueError("%s: %d gradients and %d tensors to write to" % (what, len(gradients), len(out)))
-        for g, y in zip(gradients, out):
-            if not isinstance(y, torch.Tensor) or y.shape != g.shape or y.dtype != g.dtype or y.device != device:
-                raise ValueError("%s: out must have the shapes, types and device of the gradients" % what)
-        result = out
-        if not all(y.is_contiguous() for y in out):   # through dense tensors, copied back below
-            back = [y for y in out]
-            out = [y if y.is_contiguous() else torch.empty(y.shape, dtype=y.dtype, device=device) for y in out]
-    norm = torch.empty((), dtype=torch.float32, device=device)
+    first = gradients[0]
+    ctx, lib, device, stream = _enter(what, ctx, first)
+    fresh = out is None
+    result = [torch.empty(g.shape, dtype=g.dtype, device=device) if isinstance(g, torch.Tensor) else None for g in gradients] if fresh else list(out)
     count = len(gradients)
+    if len(result) != count:
+        raise ValueError("%s: %d gradients and %d tensors to write to" % (what, count, len(result)))
+    index, types, sizes, source, target, strided = device.index, [], [], [], [], []
+    for g, y in zip(gradients, result):
+        if not isinstance(g, torch.Tensor):
+            raise TypeError("%s: expected torch tensors, got %s" % (what, type(g).__name__))
+        if g.get_device() != index:
+            raise ValueError("%s: the tensors must be on one GPU" % what)
+        kind = g.dtype
+        if not fresh and (not isinstance(y, torch.Tensor) or y.dtype != kind or y.get_device() != index or y.shape != g.shape):
+            raise ValueError("%s: out must have the shapes, types and device of the gradients" % what)
+        types.append(_TYPES[kind] if kind in _TYPES else _type(what, g))
+        sizes.append(g.numel())
+        if not g.is_contiguous():
+            g = g.contiguous()
+            strided.append((None, g))           # held until the call is queued
+        if not y.is_contiguous():
+            strided.append((y, torch.empty(y.shape, dtype=y.dtype, device=device)))   # through a dense tensor, copied back below
+            y = strided[-1][1]
+        source.append(g.data_ptr())
+        target.append(y.data_ptr())
+    norm = torch.empty((), dtype=torch.float32, device=device)
     need = _clip_workspace(lib, count)
     work = torch.empty(need, dtype=torch.uint8, device=device)
-    check(lib.nnvhip_clip_gradients(ctx.handle, count, struct.pack("=%di" % count, *types),
-                                    struct.pack("=%dq" % count, *[g.numel() for g in dense]),
-                                    struct.pack("=%dQ" % count, *[g.data_ptr() for g in dense]),
-                                    struct.pack("=%dQ" % count, *[y.data_ptr() for y in out]), threshold, norm.data_ptr(),
+    table = struct.pack("=%di%dx%dq%dQ%dQ" % (count, count % 2 * 4, count, count, count), *types, *sizes, *source, *target)
+    at = C.addressof(C.c_char.from_buffer(held := bytearray(table)))
+    longs = at + (count + count % 2) * 4
+    check(lib.nnvhip_clip_gradients(ctx.handle, count, at, longs, longs + 8 * count, longs + 16 * count, threshold, norm.data_ptr(),
                                     work.data_ptr(), need, stream))
-    if back is not None:
-        for y, t in zip(back, out):
-            if y is not t:
-                y.copy_(t)
+    del held
+    for y, t in strided:
+        if y is not None:
+            y.copy_(t)
     return result, norm
 
 
