@@ -28,7 +28,7 @@ __device__ __forceinline__ void lds_barrier() {
 // joined at the end.  For single tokens, where there are many keys for each of a few rows.
 // Where there are too few blocks for the chip, the keys are split over `splits` blocks, and join_kernel puts their results together.
 template <typename T, int DP, bool FEW>
-__global__ __launch_bounds__(256) void attend_kernel(const AttendArgs a) {
+__global__ __launch_bounds__(256, FEW ? 1 : 2) void attend_kernel(const AttendArgs a) {
   constexpr int kTile = kWaveRows, LD = DP + 4, NT = FEW ? 64 : 256, STEP = FEW ? 4 : 1;
   __shared__ float lds[(FEW ? 4 : 1) * 2 * kTile * LD];
   __shared__ float row_max[4][kTile], row_total[4][kTile];

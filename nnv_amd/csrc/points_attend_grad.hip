@@ -54,6 +54,22 @@ __device__ __forceinline__ float16_t over_head(const float* rows, const float (&
   }
   return s;
 }
+// The same with the row's fragments in LDS, 16 bytes a lane, 1024 bytes apart.
+template <int DP>
+__device__ __forceinline__ float16_t over_head_parked(const float* rows, const float* parked, int col, int h) {
+  float16_t s;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+#pragma unroll
+  for (int c = 0; c < DP / 8; ++c) {
+    float x[4], f[4];
+    __builtin_memcpy(x, rows + col * (DP + 4) + 8 * c + 4 * h, 16);
+    __builtin_memcpy(f, parked + 256 * c, 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], f[j], s, 0, 0, 0);
+  }
+  return s;
+}
 // ... and one whose sum runs over the rows of LDS: acc[d][.] += rows^T p
 template <int DP>
 __device__ __forceinline__ void over_rows(const float* rows, const float16_t& p, float16_t (&acc)[DP / 32], int col, int h) {
@@ -90,7 +106,7 @@ __device__ __forceinline__ void store_fragments(T* row, const float16_t (&acc)[D
 __device__ __forceinline__ float offset_of(float lse) { return lse == -INFINITY ? INFINITY : lse * kLog2e; }
 
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void query_grad_kernel(const AttendArgs a) {
+__global__ __launch_bounds__(256, DP <= 96 ? 2 : 1) void query_grad_kernel(const AttendArgs a) {
   constexpr int LD = DP + 4, R = kWaveRows;
   __shared__ float ks[R * LD], vs[R * LD];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
@@ -146,10 +162,13 @@ __global__ __launch_bounds__(256) void query_grad_kernel(const AttendArgs a) {
     store_fragments<T, DP>((T*)a.dq + dense_row_at(a, b, kv, r), dq, a.scale, h, a.head);
 }
 
+// Two waves a SIMD where the registers allow it: heads of up to 96, with the operands of a wave's values in LDS above 64.
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void key_grad_kernel(const AttendArgs a) {
+__global__ __launch_bounds__(256, DP <= 96 ? 2 : 1) void key_grad_kernel(const AttendArgs a) {
   constexpr int LD = DP + 4, R = kWaveRows;
+  constexpr bool PARKED = DP == 96;
   __shared__ float qs[R * LD], gs[R * LD], offsets[R], deltas[R];
+  __shared__ float parked_all[PARKED ? 4 * R * DP : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
   int64_t at = blockIdx.x;
   const int split = at % a.splits;
@@ -168,6 +187,10 @@ __global__ __launch_bounds__(256) void key_grad_kernel(const AttendArgs a) {
   float kf[DP / 8][4], vf[DP / 8][4];
   load_fragments<T, DP>(kf, (const T*)a.k.p + (counts ? b * a.k.b + kv * a.k.h + key * a.k.t : 0), h, a.head, counts);
   load_fragments<T, DP>(vf, (const T*)a.v.p + (counts ? b * a.v.b + kv * a.v.h + key * a.v.t : 0), h, a.head, counts);
+  float* parked = parked_all + (PARKED ? wave * (R * DP) + lane * 4 : 0);
+  if constexpr (PARKED)
+#pragma unroll
+    for (int c = 0; c < DP / 8; ++c) __builtin_memcpy(parked + 256 * c, vf[c], 16);
   const float unit = a.scale * kLog2e;
   float16_t dk[DP / 32], dv[DP / 32];
   zero<DP>(dk);
@@ -201,7 +224,9 @@ __global__ __launch_bounds__(256) void key_grad_kernel(const AttendArgs a) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = counts ? exp2_(s[i] * unit - offsets[product_row(i, h)]) : 0.0f;
     over_rows<DP>(gs, s, dv, col, h);
-    const float16_t dp = over_head<DP>(gs, vf, col, h);
+    float16_t dp;
+    if constexpr (PARKED) dp = over_head_parked<DP>(gs, parked, col, h);
+    else dp = over_head<DP>(gs, vf, col, h);
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] *= dp[i] - deltas[product_row(i, h)];
     over_rows<DP>(qs, s, dk, col, h);
