@@ -83,36 +83,44 @@ __device__ __forceinline__ half8<T> columns_operand(unsigned at, int first, int 
   return f;
 }
 
-// s[k] = the product over the head of rows first + 32 k .. first + 32 k + 31 of a tile with a row's operands f.  The LDS reads go two batches of
-// four ahead of the products that use them (left to itself the compiler puts every read right in front of its product), and the
-// products of a batch alternate between the independent results.
+// s[k] = the product over the head of rows first + 32 k .. first + 32 k + 31 of a tile with a row's operands f.  The LDS reads go a batch
+// (of up to four) ahead of the products that use them (left to itself the compiler puts every read right in front of its product), and
+// the products of a batch alternate between the independent results.  begin() may stand ahead of other work.
 template <typename T, int DP, int K, int MOST = 4>
-__device__ __forceinline__ void over_head(unsigned tile, int first, const half8<T> (&f)[DP / 16], float16_t (&s)[K]) {
-  constexpr int N = K * (DP / 16), BATCH = N % 4 == 0 && MOST == 4 ? 4 : N % 3 == 0 && MOST > 2 ? 3 : 2;
+struct OverHead {
+  static constexpr int N = K * (DP / 16), BATCH = N % 4 == 0 && MOST == 4 ? 4 : N % 3 == 0 && MOST > 2 ? 3 : 2;
   half8<T> x[2][BATCH];
-  auto read = [&](int n) {
+  __device__ __forceinline__ void read(unsigned tile, int first, int n) {
 #pragma unroll
     for (int i = 0; i < BATCH; ++i) {
       const int at = n * BATCH + i;
       x[n & 1][i] = rows_operand<T, DP>(tile, first + 32 * (at % K), at / K);
     }
     __builtin_amdgcn_sched_barrier(0);
-  };
-#pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s[k][i] = 0.0f;
-  read(0);
-#pragma unroll
-  for (int n = 0; n < N / BATCH; ++n) {
-    if (n + 1 < N / BATCH) read(n + 1);
-#pragma unroll
-    for (int i = 0; i < BATCH; ++i) {
-      const int at = n * BATCH + i;
-      s[at % K] = Half8<T>::mfma(x[n & 1][i], f[at / K], s[at % K]);
-    }
-    __builtin_amdgcn_sched_barrier(0);
   }
+  __device__ __forceinline__ void begin(unsigned tile, int first) { read(tile, first, 0); }
+  __device__ __forceinline__ void finish(unsigned tile, int first, const half8<T> (&f)[DP / 16], float16_t (&s)[K]) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[k][i] = 0.0f;
+#pragma unroll
+    for (int n = 0; n < N / BATCH; ++n) {
+      if (n + 1 < N / BATCH) read(tile, first, n + 1);
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const int at = n * BATCH + i;
+        s[at % K] = Half8<T>::mfma(x[n & 1][i], f[at / K], s[at % K]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+};
+template <typename T, int DP, int K, int MOST = 4>
+__device__ __forceinline__ void over_head(unsigned tile, int first, const half8<T> (&f)[DP / 16], float16_t (&s)[K]) {
+  OverHead<T, DP, K, MOST> o;
+  o.begin(tile, first);
+  o.finish(tile, first, f, s);
 }
 
 // Eight f32 of a product as the right operand of the next one, each rounded to T.
@@ -182,17 +190,30 @@ struct PairLoad {
       }
     }
   }
-  // tile t of rows that follow one another from pa and pb and end after n: rows past the last one repeat it
+  // tile ta of a and tile tb of b, of rows that follow one another from pa and pb and end after n: rows past the last one repeat it
+  __device__ __forceinline__ void issue_tiles(int ta, int tb, int n, const T* pa, int64_t stride_a, const T* pb, int64_t stride_b, unsigned lds,
+                                              int wave, int lane) const {
+    const int fa = ta * ROWS, fb = tb * ROWS;
+    if (max(fa, fb) + ROWS <= n)
+      issue(pa + fa * stride_a, pb + fb * stride_b, lds, wave);
+    else
+      issue_any([&](int r) { return pa + min(fa + r, n - 1) * stride_a; }, [&](int r) { return pb + min(fb + r, n - 1) * stride_b; }, lds, wave,
+                lane);
+  }
+  // tile t of both
   __device__ __forceinline__ void issue_tile(int t, int n, const T* pa, int64_t stride_a, const T* pb, int64_t stride_b, unsigned lds, int wave,
                                              int lane) const {
-    const int first = t * ROWS;
-    if (first + ROWS <= n)
-      issue(pa + first * stride_a, pb + first * stride_b, lds, wave);
-    else
-      issue_any([&](int r) { return pa + min(first + r, n - 1) * stride_a; }, [&](int r) { return pb + min(first + r, n - 1) * stride_b; }, lds,
-                wave, lane);
+    issue_tiles(t, t, n, pa, stride_a, pb, stride_b, lds, wave, lane);
   }
 };
+
+// A barrier that no instruction is moved across, in front of which a wave's LDS reads are done.
+__device__ __forceinline__ void phase_barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  wait_vm_lds<63>();
+  block_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+}
 
 // The rows of a tile that do not take part, made zeros by a wave for itself: a weight of zero must meet a zero.  Every wave that reads the
 // tile does so before its own reads, and no wave waits for another.
@@ -234,7 +255,7 @@ __device__ __forceinline__ float largest(const float16_t (&s)[K]) {
 
 // Block `id` of `total` in an order in which each of the 8 XCDs gets consecutive ones (blocks are dealt to the XCDs in turn):
 // blocks that read the same keys then find them in one L2.  (The sequences of a batch, whose lengths may differ, follow one another
-// within a head: every XCD gets some of each.)
+// within a head, beginning with another one in each: every XCD and every CU gets some of each.)
 __device__ __forceinline__ int64_t xcd_order(int64_t id, int64_t total) {
   const int64_t x = id % 8, base = total / 8, more = total % 8;
   return x * base + min(x, more) + id / 8;

@@ -27,12 +27,12 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, FEW ? 1 : GROUPS > 1 ? 4 : 2) 
   const int split = at % a.splits;
   at /= a.splits;
   const int row_tile = at % a.row_tiles;
-  const int b = (int)(at / a.row_tiles) % a.batch, kv = (int)(at / a.row_tiles) / a.batch, bkv = b * a.kv_heads + kv;
+  const int kv = (int)(at / a.row_tiles) / a.batch, b = (int)(at / a.row_tiles + kv) % a.batch, bkv = b * a.kv_heads + kv;
   const int n = keys_that_count(a, b);
   const int tiles = (n + KEYS - 1) / KEYS, per = (tiles + a.splits - 1) / a.splits;
   const int t0 = split * per + group, t1 = min(tiles, split * per + per);
   const int64_t r = (int64_t)row_tile * (32 * WAVES) + wave * 32 + col;
-  const bool row_here = r < a.rows;
+  const bool row_here = r < a.rows, idle = (int64_t)row_tile * (32 * WAVES) + wave * 32 >= a.rows;
   T* mine = lds + group * STAGES * 2 * TILE;
   const unsigned mine_at = lds_addr_of(mine), rows_at = rows_place<T, DP>(lane), columns_at = columns_place<T, DP>(lane);
 
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, FEW ? 1 : GROUPS > 1 ? 4 : 2) 
       if (t + (STAGES - 1) * GROUPS < t1) fetch(t + (STAGES - 1) * GROUPS, ahead);
     }
     buffer = buffer == STAGES - 1 ? 0 : buffer + 1;
-    if (GROUPS > 1 && !FEW && t >= t1) break;   // the group with a tile less has kept the last barrier
+    if (idle || (GROUPS > 1 && !FEW && t >= t1)) continue;   // the barrier was all that was left to do
     if (valid != ~0ull) zero_rows<T, DP, KEYS>(vs, valid, lane);
 
     float16_t s[KEYS / 32];
@@ -224,6 +224,189 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, FEW ? 1 : GROUPS > 1 ? 4 : 2) 
   }
 }
 
+// Many rows: 8 waves of 32 share tiles of 64 keys.  The two waves of a SIMD take turns: while one's products run (the weights of tile t
+// times the values, then the scores of tile t + 1), the other works on its softmax, and a barrier ends every such half.  Left to
+// themselves the waves of a block, which a barrier a tile keeps together anyway, all form products and then all exponentials:
+// the matrix and the vector units of a SIMD, each busy half of the time, took one after the other.
+//
+//   half     0            1            2            3
+//   waves 0-3  products 0   softmax 1    products 1   softmax 2   ...
+//   waves 4-7               products 0   softmax 1    products 1  ...
+//
+// Pair p of tiles in LDS is (keys p + 1, values p): what products p read, in halves 2 p and 2 p + 1.  There are four of them; a wave asks for
+// its share of pair p + 3 when it begins the softmax behind products p, with pair p - 1 out of use.
+template <typename T, int DP>
+__global__ __launch_bounds__(512, 2) void attend16_wide_kernel(const AttendArgs a) {
+  constexpr int KEYS = 64, TILE = KEYS * DP, WAVES = 8;
+  typedef PairLoad<T, DP, KEYS, WAVES> Load;
+  __shared__ __attribute__((aligned(1024))) T lds[8 * TILE];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
+  const bool late = wave >= WAVES / 2;
+  int64_t at = xcd_order(blockIdx.x, gridDim.x);
+  const int split = at % a.splits;
+  at /= a.splits;
+  const int row_tile = at % a.row_tiles;
+  const int kv = (int)(at / a.row_tiles) / a.batch, b = (int)(at / a.row_tiles + kv) % a.batch, bkv = b * a.kv_heads + kv;
+  const int n = keys_that_count(a, b);
+  const int tiles = (n + KEYS - 1) / KEYS, per = (tiles + a.splits - 1) / a.splits;
+  const int t0 = split * per, t1 = min(tiles, t0 + per);
+  const int64_t r = (int64_t)row_tile * (32 * WAVES) + wave * 32 + col;
+  const bool row_here = r < a.rows, idle = (int64_t)row_tile * (32 * WAVES) + wave * 32 >= a.rows;
+  const unsigned lds_at = lds_addr_of(lds), rows_at = rows_place<T, DP>(lane), columns_at = columns_place<T, DP>(lane);
+  if (DP != a.head) {   // the columns behind the head size, for good
+    half8<T> zero = {};
+    for (int e = threadIdx.x; e < 8 * KEYS * (DP / 8); e += 64 * WAVES) __builtin_memcpy(lds + e * 8, &zero, 16);
+    __syncthreads();
+  }
+  // (as in attend16_kernel)
+  const float unit = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
+  half8<T> qf[DP / 16];
+  {
+    const T* q = (const T*)a.q.p + (row_here ? row_at(a.q, a, b, kv, r) : 0);
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+      qf[c] = half8<T>{};
+      if (row_here && 16 * c + 8 * h < a.head) __builtin_memcpy(&qf[c], q + 16 * c + 8 * h, 16);
+      if (a.scale < 0) qf[c] = -qf[c];
+    }
+  }
+  float16_t acc[DP / 32], s[2];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
+  float base = -INFINITY, total = 0.0f;
+  half8<T> p[4];
+  uint64_t valid = 0;
+  unsigned words[2];   // which keys of 32 tiles count, tile i in lane i
+
+  const T* kp = (const T*)a.k.p + b * a.k.b + kv * a.k.h;
+  const T* vp = (const T*)a.v.p + b * a.v.b + kv * a.v.h;
+  Load load;
+  load.init(wave, lane, a.head, a.k.t, a.v.t);
+  const int64_t k_step = KEYS * a.k.t, v_step = KEYS * a.v.t;
+  const T *k_next = kp + t0 * k_step, *v_next = vp + (t0 - 1) * v_step;   // of the pair that is asked for next
+  auto fetch = [&](int pair) {   // what there is not of a pair is replaced by a tile that is not read
+    const unsigned to = lds_at + ((pair - t0) & 3) * (4 * TILE);
+    if (pair >= t0 && (pair + 2) * KEYS <= n) load.issue(k_next, v_next, to, wave);
+    else load.issue_tiles(min(pair + 1, t1 - 1), max(pair, t0), n, kp, a.k.t, vp, a.v.t, to, wave, lane);
+    k_next += k_step;
+    v_next += v_step;
+  };
+  auto softmax = [&](int t) {
+    if (a.mask == nullptr) {
+      const int rest = n - t * KEYS;
+      valid = rest >= KEYS ? ~0ull : (1ull << rest) - 1;
+    } else {
+      if ((t - t0) % 32 == 0)
+        for (int i = 0; i < 32; ++i) {
+          const uint64_t word = __ballot(t + i < t1 && key_counts(a, b, (t + i) * KEYS + lane, n));
+          words[0] = lane == i ? (unsigned)word : words[0];
+          words[1] = lane == i ? (unsigned)(word >> 32) : words[1];
+        }
+      valid = (uint64_t)(unsigned)__builtin_amdgcn_readlane(words[1], (t - t0) % 32) << 32 | (unsigned)__builtin_amdgcn_readlane(words[0], (t - t0) % 32);
+    }
+    if (valid != ~0ull) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t word = (uint32_t)(valid >> (32 * k)) >> (4 * h);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[k][i] = word >> product_row(i, 0) & 1 ? s[k][i] : -INFINITY;
+      }
+    }
+    const float top = max_of_halves(largest(s)) * unit;
+    if (__any(top > base + 8.0f)) {   // also: the first keys of a row that count
+      const float next = fmaxf(base, top);
+      const float fade = next == -INFINITY ? 1.0f : exp2_(base - next);
+      base = next;
+      total *= fade;
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] *= fade;
+    }
+    const float off = base == -INFINITY ? 0.0f : base;
+    float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int i = 8 * c; i < 8 * c + 8; ++i) {
+          s[k][i] = exp2_(s[k][i] * unit - off);
+          sum[i & 1] += s[k][i];
+        }
+        p[2 * k + c] = round8<T>(s[k], 8 * c);
+      }
+    total += sum[0] + sum[1];
+  };
+  auto keys_at = [&](int t) { return hide(lds_at + ((t - t0 - 1) & 3) * (4 * TILE) + rows_at); };
+  auto products = [&](int t) {
+    __builtin_amdgcn_s_setprio(1);
+    if (valid != ~0ull) zero_rows<T, DP, KEYS>(lds + (((t - t0) & 3) * 2 + 1) * TILE, valid, lane);
+    const unsigned vs_at = hide(lds_at + (((t - t0) & 3) * 4 + 2) * TILE + columns_at), ks_at = keys_at(t + 1);
+    OverHead<T, DP, 2> next;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) acc[d] = Half8<T>::mfma(columns_operand<T, DP>(vs_at, 16 * c, d), p[c], acc[d]);
+      if (c == 2) next.begin(ks_at, 0);   // (behind the last tile: read, and not used)
+    }
+    next.finish(ks_at, 0, qf, s);
+    __builtin_amdgcn_s_setprio(0);
+  };
+
+  if (t0 < t1) {
+#pragma unroll
+    for (int k = -1; k < 3; ++k)
+      if (t0 + k < t1) fetch(t0 + k);
+    // pair p has arrived when no more than the pairs behind it are on their way
+    auto arrived = [&](int pair, int asked) {
+      const int behind = min(asked, t1 - 1) - pair;
+      if (behind >= 3) wait_vm<3 * Load::COUNT>();
+      else if (behind == 2) wait_vm<2 * Load::COUNT>();
+      else if (behind == 1) wait_vm<Load::COUNT>();
+      else wait_vm<0>();
+    };
+    arrived(t0 - 1, t0 + 2);
+    phase_barrier();
+    if (!idle) {
+      over_head<T, DP, 2>(keys_at(t0), 0, qf, s);
+      softmax(t0);
+    }
+    arrived(t0, t0 + 2);
+    if (late) phase_barrier();
+    for (int t = t0; t < t1; ++t) {
+      phase_barrier();
+      if (!idle) products(t);
+      if (late) arrived(t + 1, t + 2);
+      if (!late || t + 1 < t1) phase_barrier();
+      if (t + 3 < t1) fetch(t + 3);
+      if (!idle && t + 1 < t1) softmax(t + 1);
+      if (!late) arrived(t + 1, t + 3);
+    }
+  }
+  if (!row_here) return;
+  total = sum_of_halves(total);
+  const int64_t heads_rows = (int64_t)a.batch * a.kv_heads * a.rows, flat = (int64_t)bkv * a.rows + r;
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  const float lse = total == 0.0f ? -INFINITY : (base + log2f(total)) * kLn2;
+  if (h == 0) (a.splits > 1 ? a.part_lse[split * heads_rows + flat] : a.lse[flat]) = lse;
+  float* part = a.splits > 1 ? a.part + (split * heads_rows + flat) * a.head : nullptr;
+  T* out = (T*)a.out + dense_row_at(a, b, kv, r);
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int i4 = 0; i4 < 4; ++i4) {
+      float f[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = acc[d][4 * i4 + i] * inv;
+      const int at_d = d * 32 + 8 * i4 + 4 * h;
+      if (part) store_four(part, at_d, a.head, f);
+      else store_four(out, at_d, a.head, f);
+    }
+}
+
 template <typename T, int DP>
 void launch(const AttendArgs& a, bool few, hipStream_t st) {
   const int64_t blocks = (int64_t)a.batch * a.kv_heads * a.row_tiles * a.splits;
@@ -232,10 +415,10 @@ void launch(const AttendArgs& a, bool few, hipStream_t st) {
     constexpr int GROUPS = DP > 64 ? 4 : 8;
     hipLaunchKernelGGL((attend16_kernel<T, DP, 1, GROUPS, true, 2>), grid, dim3(64 * GROUPS), 0, st, a);
   } else if constexpr (DP > 64) {
-    hipLaunchKernelGGL((attend16_kernel<T, DP, 8, 1, false, 2>), grid, dim3(512), 0, st, a);
+    hipLaunchKernelGGL((attend16_wide_kernel<T, DP>), grid, dim3(512), 0, st, a);
   } else {
     if (blocks <= 0) hipLaunchKernelGGL((attend16_kernel<T, DP, 4, 2, false, 2>), grid, dim3(512), 0, st, a);
-    else hipLaunchKernelGGL((attend16_kernel<T, DP, 4, 1, false, 3>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((attend16_kernel<T, DP, 4, 1, false, 4>), grid, dim3(256), 0, st, a);
   }
 }
 
