@@ -28,24 +28,21 @@ _stream_of = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getC
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _enter(what, ctx, first, *others):
-    """(context, its library, device, stream) for tensors that have to be on that context's GPU."""
-    if not isinstance(first, torch.Tensor):
-        raise TypeError("%s: expected a torch tensor, got %s" % (what, type(first).__name__))
-    device = first.device
-    if device.type != "cuda":
-        raise ValueError("%s: the tensors must be on the GPU" % what)
-    for t in others:
-        if t is not None:
-            if not isinstance(t, torch.Tensor):
-                raise TypeError("%s: expected a torch tensor, got %s" % (what, type(t).__name__))
-            if t.device != device:
+def _enter(what, ctx, *tensors):
+    """(context, its library, stream) for tensors (or None) that have to be on that context's GPU."""
+    try:
+        index = tensors[0].get_device()
+        for t in tensors:
+            if t is not None and t.get_device() != index:
                 raise ValueError("%s: the tensors must be on one GPU" % what)
+    except AttributeError:
+        raise TypeError("%s: expected torch tensors, got %s" % (what, ", ".join(type(t).__name__ for t in tensors))) from None
+    if index < 0:
+        raise ValueError("%s: the tensors must be on the GPU" % what)
     ctx = ctx or default_context()
-    index = device.index
     if index != ctx.device:
         raise ValueError("%s: the tensors are on GPU %d, the context is GPU %d's" % (what, index, ctx.device))
-    return ctx, ctx.lib, device, _stream_of(index)
+    return ctx, ctx.lib, _stream_of(index)
 
 
 def _type(what, t):
@@ -58,11 +55,10 @@ def _type(what, t):
 # ---- layer normalization ----------------------------------------------------------------------
 
 
-def _as_rows(x):
+def _as_rows(x, size):
     """(tensor, rows, stride of its rows): x as rows of its last dimension, copied only where they are not evenly spaced."""
-    size = x.shape[-1]
     if x.is_contiguous():
-        return x, (x.numel() // size if size else 0), size
+        return x, x.numel() // size, size
     if x.stride(-1) == 1 or size == 1:
         try:
             rows = x.view(-1, size)
@@ -100,18 +96,20 @@ def layer_norm(x, scale=None, offset=None, epsilon=1e-5, ctx=None):
 
     Returns (y, mean, rstd): y in x's shape and type, the statistics f32, one per row, in x's leading shape;
     layer_norm_backward takes them.  scale and offset: vectors of x's type or f32, or None."""
-    ctx, lib, device, stream = _enter("layer_norm", ctx, x, scale, offset)
+    ctx, lib, stream = _enter("layer_norm", ctx, x, scale, offset)
     t, w = _norm_params("layer_norm", x, scale, offset)
     if not epsilon >= 0:
         raise ValueError("layer_norm: epsilon must not be negative")
     shape = x.shape
     lead, size = shape[:-1], shape[-1]
-    scale = scale if scale is None else scale.contiguous()
-    offset = offset if offset is None else offset.contiguous()
-    rows_of, rows, stride = _as_rows(x)
-    y = x.new_empty(shape)
+    if scale is not None and not scale.is_contiguous():
+        scale = scale.contiguous()
+    if offset is not None and not offset.is_contiguous():
+        offset = offset.contiguous()
+    rows_of, rows, stride = _as_rows(x, size)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     mean = x.new_empty(lead, dtype=torch.float32)
-    rstd = x.new_empty(lead, dtype=torch.float32)
+    rstd = torch.empty_like(mean)
     check(lib.nnvhip_layer_norm(ctx.handle, t, w, rows, size, rows_of.data_ptr(), stride, _ptr(scale), _ptr(offset), epsilon,
                                 y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), stream))
     return y, mean, rstd
@@ -129,7 +127,7 @@ def layer_norm_backward(dy, x, mean, rstd, scale=None, ctx=None):
 
     dx has x's type, dscale and doffset the type of scale (x's if scale is None)."""
     what = "layer_norm_backward"
-    ctx, lib, device, stream = _enter(what, ctx, x, dy, mean, rstd, scale)
+    ctx, lib, stream = _enter(what, ctx, x, dy, mean, rstd, scale)
     t, w = _norm_params(what, x, scale, None)
     if dy.shape != x.shape or dy.dtype != x.dtype:
         raise ValueError("%s: dy must have the shape and type of x" % what)
@@ -139,11 +137,11 @@ def layer_norm_backward(dy, x, mean, rstd, scale=None, ctx=None):
             raise ValueError("%s: mean and rstd must be what layer_norm returned" % what)
     scale = scale if scale is None else scale.contiguous()
     mean, rstd = mean.contiguous(), rstd.contiguous()
-    xr, rows, xs = _as_rows(x)
-    gr, _, gs = _as_rows(dy)
-    dx = x.new_empty(x.shape)
-    like = x if scale is None else scale
-    dscale, doffset = like.new_empty((size,)), like.new_empty((size,))
+    xr, rows, xs = _as_rows(x, size)
+    gr, _, gs = _as_rows(dy, size)
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+    dscale = (x if scale is None else scale).new_empty((size,))
+    doffset = torch.empty_like(dscale)
     need = _norm_workspace(lib, t, rows, size)
     work = x.new_empty((need,), dtype=torch.uint8) if need else None
     check(lib.nnvhip_layer_norm_backward(ctx.handle, t, w, rows, size, gr.data_ptr(), gs, xr.data_ptr(), xs, mean.data_ptr(),
@@ -190,8 +188,9 @@ def _attention_workspace(lib, backward, *sizes):
 
 
 def _mask_args(key_lengths, key_mask):
-    lengths = None if key_lengths is None else key_lengths.to(torch.int32).contiguous()
-    return lengths, (key_mask.stride() if key_mask is not None else (0, 0))
+    if key_lengths is not None and (key_lengths.dtype != torch.int32 or not key_lengths.is_contiguous()):
+        key_lengths = key_lengths.to(torch.int32).contiguous()
+    return key_lengths, (key_mask.stride() if key_mask is not None else (0, 0))
 
 
 def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None, ctx=None):
@@ -204,11 +203,11 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None, ctx=No
     Returns (o, lse): o in q's shape and type and the logarithm of the softmax's sums, batch x heads x queries, f32.
     Where no key counts o is zero and lse -inf."""
     what = "cross_attention"
-    ctx, lib, device, stream = _enter(what, ctx, q, k, v, key_lengths, key_mask)
+    ctx, lib, stream = _enter(what, ctx, q, k, v, key_lengths, key_mask)
     sizes = _attention_sizes(what, q, k, v, key_lengths, key_mask)
     q, k, v = _dense_values(q), _dense_values(k), _dense_values(v)
     lengths, mask_stride = _mask_args(key_lengths, key_mask)
-    o = q.new_empty(q.shape)
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = q.new_empty((sizes[1], sizes[4], sizes[2]), dtype=torch.float32)
     d = _ATTENTION.pack(*sizes, sizes[6] ** -0.5 if scale is None else scale, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                         *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], _ptr(lengths) or 0, _ptr(key_mask) or 0,
@@ -223,7 +222,7 @@ def cross_attention_backward(do, q, k, v, o, lse, key_lengths=None, key_mask=Non
     """The gradients (dq, dk, dv) of cross_attention, from that of o and from what the forward call returned; the other
     arguments are that call's.  Rows without keys and keys that do not count get zero."""
     what = "cross_attention_backward"
-    ctx, lib, device, stream = _enter(what, ctx, q, k, v, key_lengths, key_mask, do, o, lse)
+    ctx, lib, stream = _enter(what, ctx, q, k, v, key_lengths, key_mask, do, o, lse)
     sizes = _attention_sizes(what, q, k, v, key_lengths, key_mask)
     if do.shape != q.shape or do.dtype != q.dtype or o.shape != q.shape or o.dtype != q.dtype:
         raise ValueError("%s: do and o must have the shape and type of q" % what)
@@ -232,7 +231,7 @@ def cross_attention_backward(do, q, k, v, o, lse, key_lengths=None, key_mask=Non
     q, k, v, do = _dense_values(q), _dense_values(k), _dense_values(v), _dense_values(do)
     o, lse = o.contiguous(), lse.contiguous()
     lengths, mask_stride = _mask_args(key_lengths, key_mask)
-    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
     d = _ATTENTION.pack(*sizes, sizes[6] ** -0.5 if scale is None else scale, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                         *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], _ptr(lengths) or 0, _ptr(key_mask) or 0,
                         *mask_stride, o.data_ptr(), lse.data_ptr(), do.data_ptr(), *do.stride()[:3], dq.data_ptr(),
@@ -267,8 +266,8 @@ def clip_gradients(gradients, threshold, out=None, ctx=None):
     if not gradients:
         ctx = ctx or default_context()
         return [], torch.zeros((), dtype=torch.float32, device=torch.device("cuda", ctx.device))
-    first = gradients[0]
-    ctx, lib, device, stream = _enter(what, ctx, first)
+    ctx, lib, stream = _enter(what, ctx, gradients[0])
+    device = gradients[0].device
     fresh = out is None
     result = [torch.empty(g.shape, dtype=g.dtype, device=device) if isinstance(g, torch.Tensor) else None for g in gradients] if fresh else list(out)
     count = len(gradients)
