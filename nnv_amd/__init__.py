@@ -12,14 +12,15 @@ from .sets import Box, ImageStar, SetArray, Star, Zono  # noqa: F401
 from .verify import HalfSpace, verify_specification  # noqa: F401
 
 # The operators on points work on torch tensors; torch is imported when one of them is first used.
-_POINTS = ("layer_norm", "layer_norm_backward", "cross_attention", "cross_attention_backward", "clip_gradients",
-           "LayerNormalizationLayer", "CrossAttentionLayer")
+_POINTS = {"layer_norm": "points", "layer_norm_backward": "points", "cross_attention": "points", "cross_attention_backward": "points",
+           "clip_gradients": "points", "LayerNormalizationLayer": "points", "CrossAttentionLayer": "points",
+           "CrossAttentionClassifier": "falsify", "falsify_point": "falsify", "train_step": "falsify"}
 
 
 def __getattr__(name):
     if name in _POINTS:
-        from . import points
-        value = globals()[name] = getattr(points, name)
+        import importlib
+        value = globals()[name] = getattr(importlib.import_module("." + _POINTS[name], __name__), name)
         return value
     raise AttributeError("module %r has no attribute %r" % (__name__, name))
 
