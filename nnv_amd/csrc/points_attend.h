@@ -136,11 +136,20 @@ struct Stage {
 
 // The arguments of the kernels from the caller's; what it checks, it reports as `what`.
 int attend_args(const char* what, const nnvhip_attention* d, bool backward, AttendArgs* a);
-// Blocks over which one axis is split so that `blocks` blocks become enough for the chip; no split gets fewer than `least` of the
-// axis' `tiles` tiles.
-inline int split_of(int64_t blocks, int64_t tiles, int64_t least, int64_t want) {
-  if (blocks <= 0 || blocks >= want) return 1;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want / blocks, tiles / least), 256));
+// Over how many blocks one axis of `tiles` tiles is split where there are `blocks` blocks without: the number for which the rounds of
+// `slots` blocks that the chip holds, times the tiles of a block and what starting one costs, take least, the joining of what
+// they leave (where there is any) counted in.  No split gets fewer than `least` tiles.  For 144 blocks of 19 tiles in 512 slots: 3.
+inline int split_of(int64_t blocks, int64_t tiles, int64_t least, int64_t slots, int64_t start, int64_t join) {
+  if (blocks <= 0) return 1;
+  int64_t best = 1, cost = ceil_div(blocks, slots) * (tiles + start);
+  for (int64_t s = 2; s <= std::min<int64_t>(tiles / least, 256) && blocks * s <= 4 * slots; ++s) {
+    const int64_t c = ceil_div(blocks * s, slots) * (ceil_div(tiles, s) + start) + join;
+    if (c < cost) {
+      cost = c;
+      best = s;
+    }
+  }
+  return (int)best;
 }
 
 #define ATTEND_BY_HEAD(CALL, T, ...)                 \

@@ -1,8 +1,8 @@
 // Attention of points, forward: the kernels for every type, head size and alignment.
 //
-// The products run on the f32 matrix instructions (v_mfma_f32_32x32x2_f32, 157 TFLOP/s at best), whatever the type of the
-// tensors: f32 tensors keep f32 results, and tensors of 16 bits lose nothing but their final rounding.
-#include "points_attend16.h"
+// The products are f32 ones, whatever the type of the tensors: f32 tensors keep f32 results, and tensors of 16 bits lose nothing but
+// their final rounding.
+#include "points_attend_split.h"
 
 #include <algorithm>
 
@@ -11,41 +11,124 @@
 namespace nnvhip {
 namespace {
 
-// LDS written by other lanes of the wave (FEW) or of the block
-template <bool FEW>
-__device__ __forceinline__ void lds_barrier() {
-  if constexpr (FEW) {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-  } else {
-    __syncthreads();
+// One pass over the keys with the running maximum and sum of every query's softmax: what both kernels do with the scores of a tile.
+// s: scores in powers of two; valid: which keys count, from this half's on.  Returns what the sums so far are to be multiplied with.
+__device__ __forceinline__ float softmax_step(float16_t& s, uint32_t valid, float& m, float& total) {
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    s[i] = (valid >> product_row(i, 0)) & 1 ? s[i] : -INFINITY;
+    top = fmaxf(top, s[i]);
   }
+  top = fmaxf(m, max_of_halves(top));
+  const float base = top == -INFINITY ? 0.0f : top;   // no key of this row counts yet
+  const float fade = exp2_(m - base);
+  m = top;
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    s[i] = exp2_(s[i] - base);
+    sum += s[i];
+  }
+  total = total * fade + sum;
+  return fade;
 }
 
-// One pass over the keys with the running maximum and sum of every query's softmax.
-// FEW = false: a block takes 128 rows, 32 a wave, and its waves share the tiles of keys.
-// FEW = true: a block takes 32 rows and its waves take the tiles of keys in turn, each with LDS of its own; what they found is
-// joined at the end.  For single tokens, where there are many keys for each of a few rows.
+// Many rows: 32 a wave, 128 a block, whose waves share the tiles of keys; products in pieces.
 // Where there are too few blocks for the chip, the keys are split over `splits` blocks, and join_kernel puts their results together.
-template <typename T, int DP, bool FEW>
-__global__ __launch_bounds__(256, FEW ? 1 : 2) void attend_kernel(const AttendArgs a) {
-  constexpr int kTile = kWaveRows, LD = DP + 4, NT = FEW ? 64 : 256, STEP = FEW ? 4 : 1;
-  __shared__ float lds[(FEW ? 4 : 1) * 2 * kTile * LD];
-  __shared__ float row_max[4][kTile], row_total[4][kTile];
+template <typename T, int DP>
+__global__ __launch_bounds__(256, DP <= 96 ? 2 : 1) void attend_kernel(const AttendArgs a) {
+  constexpr int R = kWaveRows;
+  __shared__ __attribute__((aligned(1024))) bf16_t ks[3 * R * DP], vs[3 * R * DP];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
-  const int tid = FEW ? lane : threadIdx.x;
   int64_t at = blockIdx.x;
   const int split = at % a.splits;
   at /= a.splits;
   const int row_tile = at % a.row_tiles;
   const int bkv = at / a.row_tiles, b = bkv / a.kv_heads, kv = bkv % a.kv_heads;
   const int n = keys_that_count(a, b);
-  const int tiles = (n + kTile - 1) / kTile, per = (tiles + a.splits - 1) / a.splits;
-  const int t0 = split * per + (FEW ? wave : 0), t1 = min(tiles, split * per + per);
-  const int64_t r = FEW ? (int64_t)row_tile * kTile + col : (int64_t)row_tile * 128 + wave * kTile + col;
+  const int tiles = (n + R - 1) / R, per = (tiles + a.splits - 1) / a.splits;
+  const int t0 = split * per, t1 = min(tiles, t0 + per);
+  const int64_t r = (int64_t)row_tile * 128 + wave * R + col;
+  const bool row_here = r < a.rows, idle = (int64_t)row_tile * 128 + wave * R >= a.rows;
+  const unsigned rows_at = rows_place<bf16_t, DP>(lane), columns_at = columns_place<bf16_t, DP>(lane);
+  RowPieces<DP> qf;
+  qf.load((const T*)a.q.p + (row_here ? row_at(a.q, a, b, kv, r) : 0), h, a.head, row_here, a.scale * kLog2e);
+  float16_t acc[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
+  float m = -INFINITY, total = 0.0f;
+  const T* kp = (const T*)a.k.p + b * a.k.b + kv * a.k.h;
+  const T* vp = (const T*)a.v.p + b * a.v.b + kv * a.v.h;
+  SplitStage<T, DP, 256> k_next, v_next;
+  int counts = 0;
+  auto fetch = [&](int t) {
+    auto there = [&](int j) { return key_counts(a, b, t * R + j, n); };
+    k_next.load([&](int j) { return kp + (t * R + j) * a.k.t; }, there, a.head, threadIdx.x);
+    v_next.load([&](int j) { return vp + (t * R + j) * a.v.t; }, there, a.head, threadIdx.x);
+    counts = key_word(a, b, t * R + col, n);
+  };
+  if (t0 < t1) fetch(t0);
+  for (int t = t0; t < t1; ++t) {
+    __syncthreads();
+    k_next.store(ks, threadIdx.x);
+    v_next.store(vs, threadIdx.x);
+    const uint32_t valid = (uint32_t)__ballot(counts != 0) >> (4 * h);
+    __syncthreads();
+    if (t + 1 < t1) fetch(t + 1);
+    if (idle) continue;
+    float16_t s = split_over_head<DP>(hide(lds_addr_of(ks) + rows_at), [&](int k, int c) { return qf.f[k][c]; });
+    const float fade = softmax_step(s, valid, m, total);
+    if (__any(fade != 1.0f))
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] *= fade;
+    split_over_rows<DP>(hide(lds_addr_of(vs) + columns_at), s, acc);
+  }
+  total = sum_of_halves(total);
+  if (!row_here) return;
+  const int64_t flat = (int64_t)bkv * a.rows + r, heads_rows = (int64_t)a.batch * a.kv_heads * a.rows;
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  if (h == 0) (a.splits > 1 ? a.part_lse[split * heads_rows + flat] : a.lse[flat]) = total == 0.0f ? -INFINITY : (m + log2f(total)) * kLn2;
+  float* part = a.splits > 1 ? a.part + (split * heads_rows + flat) * a.head : nullptr;
+  T* out = (T*)a.out + dense_row_at(a, b, kv, r);
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int i4 = 0; i4 < 4; ++i4) {
+      float f[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = acc[d][4 * i4 + i] * inv;
+      const int at_d = d * 32 + 8 * i4 + 4 * h;
+      if (part) store_four(part, at_d, a.head, f);
+      else store_four(out, at_d, a.head, f);
+    }
+}
+
+// Few rows, many keys for each (single tokens): 32 rows for the block, whose four waves take the tiles of keys in turn, each with LDS of its
+// own; what they found is joined at the end.  On the f32 matrix instructions: the keys and values are read once, and cutting each of them into
+// pieces would cost more than the instructions, which keep up with the memory.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attend_few_kernel(const AttendArgs a) {
+  constexpr int R = kWaveRows, LD = DP + 4;
+  __shared__ float lds[4 * 2 * R * LD];
+  __shared__ float row_max[4][R], row_total[4][R];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
+  int64_t at = blockIdx.x;
+  const int split = at % a.splits;
+  at /= a.splits;
+  const int row_tile = at % a.row_tiles;
+  const int bkv = at / a.row_tiles, b = bkv / a.kv_heads, kv = bkv % a.kv_heads;
+  const int n = keys_that_count(a, b);
+  const int tiles = (n + R - 1) / R, per = (tiles + a.splits - 1) / a.splits;
+  const int t0 = split * per + wave, t1 = min(tiles, split * per + per);
+  const int64_t r = (int64_t)row_tile * R + col;
   const bool row_here = r < a.rows;
-  float* ks = lds + (FEW ? wave * 2 * kTile * LD : 0);
-  float* vs = ks + kTile * LD;
+  float* ks = lds + wave * 2 * R * LD;
+  float* vs = ks + R * LD;
 
   float qf[DP / 8][4];
   {
@@ -66,22 +149,26 @@ __global__ __launch_bounds__(256, FEW ? 1 : 2) void attend_kernel(const AttendAr
 
   const T* kp = (const T*)a.k.p + b * a.k.b + kv * a.k.h;
   const T* vp = (const T*)a.v.p + b * a.v.b + kv * a.v.h;
-  Stage<T, DP, NT> ks_next, vs_next;
-  bool counts = false;
+  Stage<T, DP, 64> ks_next, vs_next;
+  int counts = 0;
   auto fetch = [&](int t) {
-    auto there = [&](int j) { return key_counts(a, b, t * kTile + j, n); };
-    ks_next.load([&](int j) { return kp + (t * kTile + j) * a.k.t; }, there, a.head, tid);
-    vs_next.load([&](int j) { return vp + (t * kTile + j) * a.v.t; }, there, a.head, tid);
-    counts = there(col);
+    auto there = [&](int j) { return key_counts(a, b, t * R + j, n); };
+    ks_next.load([&](int j) { return kp + (t * R + j) * a.k.t; }, there, a.head, lane);
+    vs_next.load([&](int j) { return vp + (t * R + j) * a.v.t; }, there, a.head, lane);
+    counts = key_word(a, b, t * R + col, n);
+  };
+  auto wave_barrier = [] {   // LDS written by other lanes of the wave
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
   };
   if (t0 < t1) fetch(t0);
-  for (int t = t0; t < t1; t += STEP) {
-    lds_barrier<FEW>();
-    ks_next.store(ks, tid);
-    vs_next.store(vs, tid);
-    const uint32_t valid = (uint32_t)__ballot(counts) >> (4 * h);
-    lds_barrier<FEW>();
-    if (t + STEP < t1) fetch(t + STEP);
+  for (int t = t0; t < t1; t += 4) {
+    wave_barrier();
+    ks_next.store(ks, lane);
+    vs_next.store(vs, lane);
+    const uint32_t valid = (uint32_t)__ballot(counts != 0) >> (4 * h);
+    wave_barrier();
+    if (t + 4 < t1) fetch(t + 4);
 
     float16_t s;
 #pragma unroll
@@ -93,23 +180,7 @@ __global__ __launch_bounds__(256, FEW ? 1 : 2) void attend_kernel(const AttendAr
 #pragma unroll
       for (int j = 0; j < 4; ++j) s = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[j], qf[c][j], s, 0, 0, 0);
     }
-    float top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s[i] = (valid >> product_row(i, 0)) & 1 ? s[i] : -INFINITY;
-      top = fmaxf(top, s[i]);
-    }
-    top = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
-    const float base = top == -INFINITY ? 0.0f : top;   // no key of this row counts yet
-    const float fade = exp2_(m - base);
-    m = top;
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s[i] = exp2_(s[i] - base);
-      sum += s[i];
-    }
-    total = total * fade + sum;
+    const float fade = softmax_step(s, valid, m, total);
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) {
 #pragma unroll
@@ -119,68 +190,44 @@ __global__ __launch_bounds__(256, FEW ? 1 : 2) void attend_kernel(const AttendAr
         acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vs[product_row(i, h) * LD + d * 32 + col], s[i], acc[d], 0, 0, 0);
     }
   }
-  total += __shfl_xor(total, 32, 64);
+  total = sum_of_halves(total);
 
-  const int64_t flat = (int64_t)bkv * a.rows + r;   // of this lane's row
-  if constexpr (!FEW) {
-    if (!row_here) return;
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    const float lse = total == 0.0f ? -INFINITY : (m + log2f(total)) * kLn2;
-    if (h == 0) {
-      if (a.splits > 1) a.part_lse[(int64_t)split * a.batch * a.kv_heads * a.rows + flat] = lse;
-      else a.lse[flat] = lse;
+  __syncthreads();
+  float* mine = lds + wave * R * LD;   // [row][d] of this wave
+  if (h == 0) {
+    row_max[wave][col] = m;
+    row_total[wave][col] = total;
+  }
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mine[col * LD + d * 32 + product_row(i, h)] = acc[d][i];
+  __syncthreads();
+  for (int e = threadIdx.x; e < R * (DP / 4); e += 256) {
+    const int j = e / (DP / 4), d = e % (DP / 4) * 4;
+    const int64_t rj = (int64_t)row_tile * R + j;
+    if (rj >= a.rows) continue;
+    float top = row_max[0][j], all = 0.0f, w[4], f[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int k = 1; k < 4; ++k) top = fmaxf(top, row_max[k][j]);
+    const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      w[k] = exp2_(row_max[k][j] - base);
+      all += w[k] * row_total[k][j];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] += w[k] * lds[(k * R + j) * LD + d + i];
     }
-    float* part = a.splits > 1 ? a.part + ((int64_t)split * a.batch * a.kv_heads * a.rows + flat) * a.head : nullptr;
-    T* out = (T*)a.out + dense_row_at(a, b, kv, r);
+    const float inv = all == 0.0f ? 0.0f : 1.0f / all;
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-      for (int i4 = 0; i4 < 4; ++i4) {
-        float f[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = acc[d][4 * i4 + i] * inv;
-        const int at_d = d * 32 + 8 * i4 + 4 * h;
-        if (part) store_four(part, at_d, a.head, f);
-        else store_four(out, at_d, a.head, f);
-      }
-  } else {
-    __syncthreads();
-    float* mine = lds + wave * kTile * LD;   // [row][d] of this wave
-    if (h == 0) {
-      row_max[wave][col] = m;
-      row_total[wave][col] = total;
-    }
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) mine[col * LD + d * 32 + product_row(i, h)] = acc[d][i];
-    __syncthreads();
-    for (int e = threadIdx.x; e < kTile * (DP / 4); e += 256) {
-      const int j = e / (DP / 4), d = e % (DP / 4) * 4;
-      const int64_t rj = (int64_t)row_tile * kTile + j;
-      if (rj >= a.rows) continue;
-      float top = row_max[0][j], all = 0.0f, w[4], f[4] = {0, 0, 0, 0};
-#pragma unroll
-      for (int k = 1; k < 4; ++k) top = fmaxf(top, row_max[k][j]);
-      const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        w[k] = exp2_(row_max[k][j] - base);
-        all += w[k] * row_total[k][j];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] += w[k] * lds[(k * kTile + j) * LD + d + i];
-      }
-      const float inv = all == 0.0f ? 0.0f : 1.0f / all;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) f[i] *= inv;
-      const int64_t fj = (int64_t)bkv * a.rows + rj;
-      const float lse = all == 0.0f ? -INFINITY : (top + log2f(all)) * kLn2;
-      const int64_t sj = (int64_t)split * a.batch * a.kv_heads * a.rows + fj;
-      if (d == 0) (a.splits > 1 ? a.part_lse[sj] : a.lse[fj]) = lse;
-      if (d >= a.head) continue;
-      if (a.splits > 1) store_four(a.part + sj * a.head, d, a.head, f);
-      else store_four((T*)a.out + dense_row_at(a, b, kv, rj), d, a.head, f);
-    }
+    for (int i = 0; i < 4; ++i) f[i] *= inv;
+    const int64_t fj = (int64_t)bkv * a.rows + rj;
+    const float lse = all == 0.0f ? -INFINITY : (top + log2f(all)) * kLn2;
+    const int64_t sj = (int64_t)split * a.batch * a.kv_heads * a.rows + fj;
+    if (d == 0) (a.splits > 1 ? a.part_lse[sj] : a.lse[fj]) = lse;
+    if (d >= a.head) continue;
+    if (a.splits > 1) store_four(a.part + sj * a.head, d, a.head, f);
+    else store_four((T*)a.out + dense_row_at(a, b, kv, rj), d, a.head, f);
   }
 }
 
@@ -258,15 +305,18 @@ Cut cut_of(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys, int64_t 
   Cut c;
   c.few = rows <= kWaveRows;
   c.row_tiles = (int)ceil_div(rows, c.few ? kWaveRows : by16 ? attend16_tile(head) : 128);
-  c.splits = split_of(batch * kv_heads * c.row_tiles, ceil_div(keys, kWaveRows), c.few ? 8 : 4, c.few || (by16 && head > 64) ? 256 : 512);
+  // blocks that the chip holds at once; what starting a block, and joining splits, costs in tiles of 32 keys
+  const int64_t slots = c.few || head > (by16 ? 64 : 96) ? 256 : 512;
+  const int64_t start = c.few ? 16 : by16 ? 6 : 2, join = c.few ? 16 : by16 ? 12 : 3;
+  c.splits = split_of(batch * kv_heads * c.row_tiles, ceil_div(keys, kWaveRows), c.few ? 8 : 4, slots, start, join);
   return c;
 }
 
 template <typename T, int DP>
 void launch_attend(const AttendArgs& a, bool few, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)a.batch * a.kv_heads * a.row_tiles * a.splits));
-  if (few) hipLaunchKernelGGL((attend_kernel<T, DP, true>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((attend_kernel<T, DP, false>), grid, dim3(256), 0, st, a);
+  if (few) hipLaunchKernelGGL((attend_few_kernel<T, DP>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((attend_kernel<T, DP>), grid, dim3(256), 0, st, a);
 }
 template <typename T, int>
 void launch_join(const AttendArgs& a, hipStream_t st) {

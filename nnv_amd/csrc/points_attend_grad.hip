@@ -1,10 +1,10 @@
-// Attention of points, backward: the kernels for every type, head size and alignment, on the f32 matrix instructions.
+// Attention of points, backward: the kernels for every type, head size and alignment, with f32 products (points_attend_split.h).
 //
 // Two kernels form dq (a wave per 32 queries, over the keys) and dk, dv (a wave per 32 keys, over the queries of every head that
 // shares them).  Both form S and dP again: seven products instead of the five that one kernel would need, but every
 // gradient is a sum in the registers of one wave, in a fixed order, with no atomics.  What both need of a row besides, D = rowsum(do o),
 // is formed first.  Where one axis gives too few blocks for the chip, the other is split, and sum_kernel adds the parts in order.
-#include "points_attend16.h"
+#include "points_attend_split.h"
 
 #pragma clang fp contract(fast)
 
@@ -39,56 +39,6 @@ __device__ __forceinline__ void zero(float16_t (&acc)[DP / 32]) {
     for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
 }
 
-// A product with 32 rows of LDS as left operand and a row's fragments in registers as right one: the sum runs over the head.
-template <int DP>
-__device__ __forceinline__ float16_t over_head(const float* rows, const float (&f)[DP / 8][4], int col, int h) {
-  float16_t s;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) s[i] = 0.0f;
-#pragma unroll
-  for (int c = 0; c < DP / 8; ++c) {
-    float x[4];
-    __builtin_memcpy(x, rows + col * (DP + 4) + 8 * c + 4 * h, 16);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], f[c][j], s, 0, 0, 0);
-  }
-  return s;
-}
-// The same with the row's fragments in LDS, 16 bytes a lane, 1024 bytes apart.
-template <int DP>
-__device__ __forceinline__ float16_t over_head_parked(const float* rows, const float* parked, int col, int h) {
-  float16_t s;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) s[i] = 0.0f;
-#pragma unroll
-  for (int c = 0; c < DP / 8; ++c) {
-    float x[4], f[4];
-    __builtin_memcpy(x, rows + col * (DP + 4) + 8 * c + 4 * h, 16);
-    __builtin_memcpy(f, parked + 256 * c, 16);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], f[j], s, 0, 0, 0);
-  }
-  return s;
-}
-// ... and one whose sum runs over the rows of LDS: acc[d][.] += rows^T p
-template <int DP>
-__device__ __forceinline__ void over_rows(const float* rows, const float16_t& p, float16_t (&acc)[DP / 32], int col, int h) {
-#pragma unroll
-  for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(rows[product_row(i, h) * (DP + 4) + d * 32 + col], p[i], acc[d], 0, 0, 0);
-}
-
-template <typename T, int DP>
-__device__ __forceinline__ void load_fragments(float (&f)[DP / 8][4], const T* row, int h, int head, bool there) {
-#pragma unroll
-  for (int c = 0; c < DP / 8; ++c) {
-    const Four x = load_four(row, 8 * c + 4 * h, head, there);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) f[c][j] = x.v[j];
-  }
-}
 template <typename T, int DP>
 __device__ __forceinline__ void store_fragments(T* row, const float16_t (&acc)[DP / 32], float by, int h, int head) {
 #pragma unroll
@@ -106,9 +56,9 @@ __device__ __forceinline__ void store_fragments(T* row, const float16_t (&acc)[D
 __device__ __forceinline__ float offset_of(float lse) { return lse == -INFINITY ? INFINITY : lse * kLog2e; }
 
 template <typename T, int DP>
-__global__ __launch_bounds__(256, DP <= 96 ? 2 : 1) void query_grad_kernel(const AttendArgs a) {
-  constexpr int LD = DP + 4, R = kWaveRows;
-  __shared__ float ks[R * LD], vs[R * LD];
+__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void query_grad_kernel(const AttendArgs a) {
+  constexpr int R = kWaveRows;
+  __shared__ __attribute__((aligned(1024))) bf16_t ks[3 * R * DP], vs[3 * R * DP];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
   int64_t at = blockIdx.x;
   const int split = at % a.splits;
@@ -119,41 +69,43 @@ __global__ __launch_bounds__(256, DP <= 96 ? 2 : 1) void query_grad_kernel(const
   const int tiles = (n + R - 1) / R, per = (tiles + a.splits - 1) / a.splits;
   const int t0 = split * per, t1 = min(tiles, t0 + per);
   const int64_t r = (int64_t)row_tile * 128 + wave * R + col, flat = (int64_t)bkv * a.rows + r;
-  const bool here = r < a.rows;
+  const bool here = r < a.rows, idle = (int64_t)row_tile * 128 + wave * R >= a.rows;
   const float lse = here ? a.lse[flat] : -INFINITY;
   const bool takes_part = here && lse != -INFINITY;
   const float offset = offset_of(lse), delta = takes_part ? a.delta[flat] : 0.0f, unit = a.scale * kLog2e;
-  float qf[DP / 8][4], gf[DP / 8][4];
-  load_fragments<T, DP>(qf, (const T*)a.q.p + (here ? row_at(a.q, a, b, kv, r) : 0), h, a.head, takes_part);
-  load_fragments<T, DP>(gf, (const T*)a.go.p + (here ? row_at(a.go, a, b, kv, r) : 0), h, a.head, takes_part);
+  const unsigned rows_at = rows_place<bf16_t, DP>(lane), columns_at = columns_place<bf16_t, DP>(lane);
+  RowPieces<DP> qf, gf;
+  qf.load((const T*)a.q.p + (here ? row_at(a.q, a, b, kv, r) : 0), h, a.head, takes_part, 1.0f);
+  gf.load((const T*)a.go.p + (here ? row_at(a.go, a, b, kv, r) : 0), h, a.head, takes_part, 1.0f);
   float16_t dq[DP / 32];
   zero<DP>(dq);
   const T* kp = (const T*)a.k.p + b * a.k.b + kv * a.k.h;
   const T* vp = (const T*)a.v.p + b * a.v.b + kv * a.v.h;
-  Stage<T, DP, 256> k_next, v_next;
-  bool counts = false;
+  SplitStage<T, DP, 256> k_next, v_next;
+  int counts = 0;
   auto fetch = [&](int t) {
     auto there = [&](int j) { return key_counts(a, b, t * R + j, n); };
     k_next.load([&](int j) { return kp + (t * R + j) * a.k.t; }, there, a.head, threadIdx.x);
     v_next.load([&](int j) { return vp + (t * R + j) * a.v.t; }, there, a.head, threadIdx.x);
-    counts = there(col);
+    counts = key_word(a, b, t * R + col, n);
   };
   if (t0 < t1) fetch(t0);
   for (int t = t0; t < t1; ++t) {
     __syncthreads();
     k_next.store(ks, threadIdx.x);
     v_next.store(vs, threadIdx.x);
-    const uint32_t valid = (uint32_t)__ballot(counts) >> (4 * h);
+    const uint32_t valid = (uint32_t)__ballot(counts != 0) >> (4 * h);
     __syncthreads();
     if (t + 1 < t1) fetch(t + 1);
-    float16_t s = over_head<DP>(ks, qf, col, h);
-    const float16_t dp = over_head<DP>(vs, gf, col, h);
+    if (idle) continue;
+    float16_t s = split_over_head<DP>(hide(lds_addr_of(ks) + rows_at), [&](int k, int c) { return qf.f[k][c]; });
+    const float16_t dp = split_over_head<DP>(hide(lds_addr_of(vs) + rows_at), [&](int k, int c) { return gf.f[k][c]; });
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const float p = exp2_(s[i] * unit - offset);
       s[i] = (valid >> product_row(i, 0)) & 1 ? p * (dp[i] - delta) : 0.0f;
     }
-    over_rows<DP>(ks, s, dq, col, h);
+    split_over_rows<DP>(hide(lds_addr_of(ks) + columns_at), s, dq);
   }
   if (!here) return;
   if (a.splits > 1)
@@ -162,13 +114,14 @@ __global__ __launch_bounds__(256, DP <= 96 ? 2 : 1) void query_grad_kernel(const
     store_fragments<T, DP>((T*)a.dq + dense_row_at(a, b, kv, r), dq, a.scale, h, a.head);
 }
 
-// Two waves a SIMD where the registers allow it: heads of up to 96, with the operands of a wave's values in LDS above 64.
+// Above heads of 64 the pieces of a wave's values lie in LDS: in registers they would be one set too many.
 template <typename T, int DP>
-__global__ __launch_bounds__(256, DP <= 96 ? 2 : 1) void key_grad_kernel(const AttendArgs a) {
-  constexpr int LD = DP + 4, R = kWaveRows;
-  constexpr bool PARKED = DP == 96;
-  __shared__ float qs[R * LD], gs[R * LD], offsets[R], deltas[R];
-  __shared__ float parked_all[PARKED ? 4 * R * DP : 1];
+__global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void key_grad_kernel(const AttendArgs a) {
+  constexpr int R = kWaveRows;
+  constexpr bool PARKED = DP > 64;
+  __shared__ __attribute__((aligned(1024))) bf16_t qs[3 * R * DP], gs[3 * R * DP];
+  __shared__ float offsets[R], deltas[R];
+  __shared__ piece8 parked[PARKED ? 4 : 1][PARKED ? 3 * (DP / 16) : 1][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
   int64_t at = blockIdx.x;
   const int split = at % a.splits;
@@ -177,25 +130,27 @@ __global__ __launch_bounds__(256, DP <= 96 ? 2 : 1) void key_grad_kernel(const A
   const int bkv = at / a.key_tiles, b = bkv / a.kv_heads, kv = bkv % a.kv_heads;
   const int n = keys_that_count(a, b);
   const int key = key_tile * 128 + wave * R + col;
-  const bool here = key < a.keys, counts = key_counts(a, b, key, n);
+  const bool here = key < a.keys, counts = key_counts(a, b, key, n), idle = key_tile * 128 + wave * R >= n;
   int t0 = 0, t1 = 0;
   if (key_tile * 128 < n) {   // else no key of the block counts: its gradients are zero
     const int tiles = (int)((a.rows + R - 1) / R), per = (tiles + a.splits - 1) / a.splits;
     t0 = split * per;
     t1 = min(tiles, t0 + per);
   }
-  float kf[DP / 8][4], vf[DP / 8][4];
-  load_fragments<T, DP>(kf, (const T*)a.k.p + (counts ? b * a.k.b + kv * a.k.h + key * a.k.t : 0), h, a.head, counts);
-  load_fragments<T, DP>(vf, (const T*)a.v.p + (counts ? b * a.v.b + kv * a.v.h + key * a.v.t : 0), h, a.head, counts);
-  float* parked = parked_all + (PARKED ? wave * (R * DP) + lane * 4 : 0);
+  const unsigned rows_at = rows_place<bf16_t, DP>(lane), columns_at = columns_place<bf16_t, DP>(lane);
+  RowPieces<DP> kf, vf;
+  kf.load((const T*)a.k.p + (counts ? b * a.k.b + kv * a.k.h + key * a.k.t : 0), h, a.head, counts, 1.0f);
+  vf.load((const T*)a.v.p + (counts ? b * a.v.b + kv * a.v.h + key * a.v.t : 0), h, a.head, counts, 1.0f);
   if constexpr (PARKED)
 #pragma unroll
-    for (int c = 0; c < DP / 8; ++c) __builtin_memcpy(parked + 256 * c, vf[c], 16);
+    for (int k = 0; k < 3; ++k)
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c) parked[wave][k * (DP / 16) + c][lane] = vf.f[k][c];
   const float unit = a.scale * kLog2e;
   float16_t dk[DP / 32], dv[DP / 32];
   zero<DP>(dk);
   zero<DP>(dv);
-  Stage<T, DP, 256> q_next, g_next;
+  SplitStage<T, DP, 256> q_next, g_next;
   float offset = INFINITY, delta = 0.0f;
   const float* lse = a.lse + (int64_t)bkv * a.rows;
   auto fetch = [&](int t) {
@@ -220,18 +175,24 @@ __global__ __launch_bounds__(256, DP <= 96 ? 2 : 1) void key_grad_kernel(const A
     }
     __syncthreads();
     if (t + 1 < t1) fetch(t + 1);
-    float16_t s = over_head<DP>(qs, kf, col, h);
+    if (idle) continue;
+    float16_t s = split_over_head<DP>(hide(lds_addr_of(qs) + rows_at), [&](int k, int c) { return kf.f[k][c]; });
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = counts ? exp2_(s[i] * unit - offsets[product_row(i, h)]) : 0.0f;
-    over_rows<DP>(gs, s, dv, col, h);
-    float16_t dp;
-    if constexpr (PARKED) dp = over_head_parked<DP>(gs, parked, col, h);
-    else dp = over_head<DP>(gs, vf, col, h);
+    for (int i = 0; i < 16; ++i) s[i] = exp2_(s[i] * unit - offsets[product_row(i, h)]);   // (of a key that does not count: dropped below)
+    split_over_rows<DP>(hide(lds_addr_of(gs) + columns_at), s, dv);
+    const float16_t dp = split_over_head<DP>(hide(lds_addr_of(gs) + rows_at), [&](int k, int c) {
+      if constexpr (PARKED) return parked[wave][k * (DP / 16) + c][lane];
+      else return vf.f[k][c];
+    });
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] *= dp[i] - deltas[product_row(i, h)];
-    over_rows<DP>(qs, s, dk, col, h);
+    split_over_rows<DP>(hide(lds_addr_of(qs) + columns_at), s, dk);
   }
   if (!here) return;
+  if (!counts) {
+    zero<DP>(dk);
+    zero<DP>(dv);
+  }
   const int64_t dense = ((b * (int64_t)a.keys + key) * a.kv_heads + kv) * a.head;
   if (a.splits > 1) {
     const int64_t all = (int64_t)a.batch * a.keys * a.kv_heads * a.head;
@@ -274,8 +235,10 @@ GradCut grad_cut(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys, in
   GradCut c;
   c.row_tiles = (int)ceil_div(rows, by16 ? 256 : 128);
   c.key_tiles = (int)ceil_div(keys, by16 ? key_grad16_tile(head) : 128);
-  c.query_splits = split_of(batch * kv_heads * c.row_tiles, ceil_div(keys, kWaveRows), 4, by16 ? 256 : 512);
-  c.key_splits = split_of(batch * kv_heads * c.key_tiles, ceil_div(rows, kWaveRows), 4, by16 && head > 64 ? 256 : 512);
+  // blocks that the chip holds at once; what starting a block, and adding splits up, costs in tiles of 32 rows
+  const int64_t start = by16 ? 6 : 2, join = by16 ? 12 : 3;
+  c.query_splits = split_of(batch * kv_heads * c.row_tiles, ceil_div(keys, kWaveRows), 4, by16 || head > 64 ? 256 : 512, start, join);
+  c.key_splits = split_of(batch * kv_heads * c.key_tiles, ceil_div(rows, kWaveRows), 4, head > (by16 ? 64 : 32) ? 256 : 512, start, join);
   c.delta = round_up(batch * kv_heads * rows, 64);
   const int64_t q = c.query_splits > 1 ? c.query_splits * batch * kv_heads * rows * head : 0;
   const int64_t k = c.key_splits > 1 ? 2 * c.key_splits * batch * kv_heads * keys * head : 0;
