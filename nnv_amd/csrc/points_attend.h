@@ -54,9 +54,8 @@ __device__ __forceinline__ bool key_counts(const AttendArgs& a, int b, int key, 
 // The same as a number that is zero where the key does not count: a mask's byte as it was loaded, so that nothing waits for it
 // before it is used.
 __device__ __forceinline__ int key_word(const AttendArgs& a, int b, int key, int n) {
-  int w = 0;
-  if (key < n) w = a.mask ? a.mask[b * a.mask_b + key * a.mask_k] : 1;
-  return w;
+  if (a.mask == nullptr) return key < n;
+  return a.mask[b * a.mask_b + min(key, n - 1) * a.mask_k] & (key < n ? 0xff : 0);
 }
 // offset of row r of (b, kv) in a token view
 __device__ __forceinline__ int64_t row_at(const TokenView& t, const AttendArgs& a, int b, int kv, int64_t r) {
@@ -109,27 +108,55 @@ __device__ __forceinline__ void store_four(T* row, int d, int head, const float 
 
 constexpr int kWaveRows = 32;  // rows of a wave's tile on either side
 
-// 32 rows of a token view as f32 in LDS, rows of DP + 4 floats: a quarter wave's 16-byte reads of one column block then
-// touch every bank once.  NT threads share the work; load() asks for the rows, store() puts what has arrived into LDS.
-template <typename T, int DP, int NT>
-struct Stage {
-  static constexpr int LD = DP + 4, PER = kWaveRows * DP / 4 / NT;
-  Four r[PER];
-  // row(j): pointer of row j; there(j): whether it exists and counts
-  template <class Row, class There>
-  __device__ __forceinline__ void load(Row row, There there, int head, int tid) {
+// Four elements as the words they are loaded as (see Pack): what is asked for a tile ahead is taken apart, and found not to
+// count, when it is stored, so that nothing waits for it before.  For the same reason no lane takes another way than its neighbours: what lies
+// behind the head is read from the head's end, and zero when it is stored.
+template <typename T>
+struct RawFour {
+  unsigned w[sizeof(T)];
+  __device__ __forceinline__ void load(const T* row, int d, int head) {   // head is a multiple of 4
+    __builtin_memcpy(w, row + min(d, head - 4), 4 * sizeof(T));
+  }
+  __device__ __forceinline__ void load_any(const T* row, int d, int head) {
+    T t[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t[i] = row[min(d + i, head - 1)];
+    __builtin_memcpy(w, t, sizeof(t));
+  }
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (sizeof(T) == 4) return to_f(__builtin_bit_cast(T, w[i]));
+    else return to_f(__builtin_bit_cast(T, (uint16_t)(w[i / 2] >> (16 * (i & 1)))));
+  }
+};
+
+// 32 rows of a token view on their way to LDS: NT threads, four values of PER rows each.  FOUR: the head is a multiple of 4.
+template <typename T, int DP, int NT, bool FOUR>
+struct RowsAhead {
+  static constexpr int PER = kWaveRows * DP / 4 / NT;
+  RawFour<T> r[PER];
+  int word[PER];
+  // row(j): pointer of row j, one that exists; word(j): what says whether it counts
+  template <class Row, class Word>
+  __device__ __forceinline__ void load(Row row, Word word_of, int head, int tid) {
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
       const int at = p * NT + tid, j = at / (DP / 4), d = at % (DP / 4) * 4;
-      const bool ok = there(j);
-      r[p] = load_four<T>(ok ? row(j) : (const T*)nullptr, d, head, ok);
+      if constexpr (FOUR) r[p].load(row(j), d, head);
+      else r[p].load_any(row(j), d, head);
+      word[p] = word_of(j);
     }
   }
-  __device__ __forceinline__ void store(float* lds, int tid) {
+  // to(j, d, f): takes the values d .. d + 3 of row j; those of a row for which counts(word) is false are zero
+  template <class To, class Counts>
+  __device__ __forceinline__ void store(To to, Counts counts, int head, int tid) const {
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
       const int at = p * NT + tid, j = at / (DP / 4), d = at % (DP / 4) * 4;
-      __builtin_memcpy(lds + j * LD + d, r[p].v, 16);
+      const bool ok = counts(word[p]);
+      float f[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = ok && d + i < head ? r[p][i] : 0.0f;
+      to(j, d, f);
     }
   }
 };

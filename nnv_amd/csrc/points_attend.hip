@@ -36,7 +36,7 @@ __device__ __forceinline__ float softmax_step(float16_t& s, uint32_t valid, floa
 
 // Many rows: 32 a wave, 128 a block, whose waves share the tiles of keys; products in pieces.
 // Where there are too few blocks for the chip, the keys are split over `splits` blocks, and join_kernel puts their results together.
-template <typename T, int DP>
+template <typename T, int DP, bool FOUR>
 __global__ __launch_bounds__(256, DP <= 96 ? 2 : 1) void attend_kernel(const AttendArgs a) {
   constexpr int R = kWaveRows;
   __shared__ __attribute__((aligned(1024))) bf16_t ks[3 * R * DP], vs[3 * R * DP];
@@ -62,19 +62,20 @@ __global__ __launch_bounds__(256, DP <= 96 ? 2 : 1) void attend_kernel(const Att
   float m = -INFINITY, total = 0.0f;
   const T* kp = (const T*)a.k.p + b * a.k.b + kv * a.k.h;
   const T* vp = (const T*)a.v.p + b * a.v.b + kv * a.v.h;
-  SplitStage<T, DP, 256> k_next, v_next;
+  RowsAhead<T, DP, 256, FOUR> k_next, v_next;
   int counts = 0;
   auto fetch = [&](int t) {
-    auto there = [&](int j) { return key_counts(a, b, t * R + j, n); };
-    k_next.load([&](int j) { return kp + (t * R + j) * a.k.t; }, there, a.head, threadIdx.x);
-    v_next.load([&](int j) { return vp + (t * R + j) * a.v.t; }, there, a.head, threadIdx.x);
+    auto word = [&](int j) { return key_word(a, b, t * R + j, n); };
+    k_next.load([&](int j) { return kp + min(t * R + j, n - 1) * a.k.t; }, word, a.head, threadIdx.x);
+    v_next.load([&](int j) { return vp + min(t * R + j, n - 1) * a.v.t; }, word, a.head, threadIdx.x);
     counts = key_word(a, b, t * R + col, n);
   };
   if (t0 < t1) fetch(t0);
   for (int t = t0; t < t1; ++t) {
     __syncthreads();
-    k_next.store(ks, threadIdx.x);
-    v_next.store(vs, threadIdx.x);
+    auto counting = [](int word) { return word != 0; };
+    k_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP>(ks, j, d, f); }, counting, a.head, threadIdx.x);
+    v_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP>(vs, j, d, f); }, counting, a.head, threadIdx.x);
     const uint32_t valid = (uint32_t)__ballot(counts != 0) >> (4 * h);
     __syncthreads();
     if (t + 1 < t1) fetch(t + 1);
@@ -111,7 +112,7 @@ __global__ __launch_bounds__(256, DP <= 96 ? 2 : 1) void attend_kernel(const Att
 // Few rows, many keys for each (single tokens): 32 rows for the block, whose four waves take the tiles of keys in turn, each with LDS of its
 // own; what they found is joined at the end.  On the f32 matrix instructions: the keys and values are read once, and cutting each of them into
 // pieces would cost more than the instructions, which keep up with the memory.
-template <typename T, int DP>
+template <typename T, int DP, bool FOUR>
 __global__ __launch_bounds__(256) void attend_few_kernel(const AttendArgs a) {
   constexpr int R = kWaveRows, LD = DP + 4;
   __shared__ float lds[4 * 2 * R * LD];
@@ -149,12 +150,12 @@ __global__ __launch_bounds__(256) void attend_few_kernel(const AttendArgs a) {
 
   const T* kp = (const T*)a.k.p + b * a.k.b + kv * a.k.h;
   const T* vp = (const T*)a.v.p + b * a.v.b + kv * a.v.h;
-  Stage<T, DP, 64> ks_next, vs_next;
+  RowsAhead<T, DP, 64, FOUR> ks_next, vs_next;
   int counts = 0;
   auto fetch = [&](int t) {
-    auto there = [&](int j) { return key_counts(a, b, t * R + j, n); };
-    ks_next.load([&](int j) { return kp + (t * R + j) * a.k.t; }, there, a.head, lane);
-    vs_next.load([&](int j) { return vp + (t * R + j) * a.v.t; }, there, a.head, lane);
+    auto word = [&](int j) { return key_word(a, b, t * R + j, n); };
+    ks_next.load([&](int j) { return kp + min(t * R + j, n - 1) * a.k.t; }, word, a.head, lane);
+    vs_next.load([&](int j) { return vp + min(t * R + j, n - 1) * a.v.t; }, word, a.head, lane);
     counts = key_word(a, b, t * R + col, n);
   };
   auto wave_barrier = [] {   // LDS written by other lanes of the wave
@@ -164,8 +165,10 @@ __global__ __launch_bounds__(256) void attend_few_kernel(const AttendArgs a) {
   if (t0 < t1) fetch(t0);
   for (int t = t0; t < t1; t += 4) {
     wave_barrier();
-    ks_next.store(ks, lane);
-    vs_next.store(vs, lane);
+    // rows of DP + 4 floats: a quarter wave's 16-byte reads of one column block then touch every bank once
+    auto counting = [](int word) { return word != 0; };
+    ks_next.store([&](int j, int d, const float(&f)[4]) { __builtin_memcpy(ks + j * LD + d, f, 16); }, counting, a.head, lane);
+    vs_next.store([&](int j, int d, const float(&f)[4]) { __builtin_memcpy(vs + j * LD + d, f, 16); }, counting, a.head, lane);
     const uint32_t valid = (uint32_t)__ballot(counts != 0) >> (4 * h);
     wave_barrier();
     if (t + 4 < t1) fetch(t + 4);
@@ -315,8 +318,11 @@ Cut cut_of(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys, int64_t 
 template <typename T, int DP>
 void launch_attend(const AttendArgs& a, bool few, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)a.batch * a.kv_heads * a.row_tiles * a.splits));
-  if (few) hipLaunchKernelGGL((attend_few_kernel<T, DP>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((attend_kernel<T, DP>), grid, dim3(256), 0, st, a);
+  const bool four = a.head % 4 == 0;
+  if (few && four) hipLaunchKernelGGL((attend_few_kernel<T, DP, true>), grid, dim3(256), 0, st, a);
+  else if (few) hipLaunchKernelGGL((attend_few_kernel<T, DP, false>), grid, dim3(256), 0, st, a);
+  else if (four) hipLaunchKernelGGL((attend_kernel<T, DP, true>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((attend_kernel<T, DP, false>), grid, dim3(256), 0, st, a);
 }
 template <typename T, int>
 void launch_join(const AttendArgs& a, hipStream_t st) {

@@ -55,10 +55,14 @@ __device__ __forceinline__ void store_fragments(T* row, const float16_t (&acc)[D
 // lse of a row as the exponent's offset in powers of two; a row without keys takes no part (exp2(s - inf) = 0)
 __device__ __forceinline__ float offset_of(float lse) { return lse == -INFINITY ? INFINITY : lse * kLog2e; }
 
-template <typename T, int DP>
+// Above heads of 64 the pieces of a wave's gradients of o lie in LDS: in registers they would be one set too many, and what is asked for
+// ahead would be moved to the accumulation registers, and waited for, as soon as it is asked for.
+template <typename T, int DP, bool FOUR>
 __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void query_grad_kernel(const AttendArgs a) {
   constexpr int R = kWaveRows;
+  constexpr bool PARKED = DP > 64;
   __shared__ __attribute__((aligned(1024))) bf16_t ks[3 * R * DP], vs[3 * R * DP];
+  __shared__ piece8 parked[PARKED ? 4 : 1][PARKED ? 3 * (DP / 16) : 1][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
   int64_t at = blockIdx.x;
   const int split = at % a.splits;
@@ -77,29 +81,38 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void query_grad_kernel(const
   RowPieces<DP> qf, gf;
   qf.load((const T*)a.q.p + (here ? row_at(a.q, a, b, kv, r) : 0), h, a.head, takes_part, 1.0f);
   gf.load((const T*)a.go.p + (here ? row_at(a.go, a, b, kv, r) : 0), h, a.head, takes_part, 1.0f);
+  if constexpr (PARKED)
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c) parked[wave][k * (DP / 16) + c][lane] = gf.f[k][c];
   float16_t dq[DP / 32];
   zero<DP>(dq);
   const T* kp = (const T*)a.k.p + b * a.k.b + kv * a.k.h;
   const T* vp = (const T*)a.v.p + b * a.v.b + kv * a.v.h;
-  SplitStage<T, DP, 256> k_next, v_next;
+  RowsAhead<T, DP, 256, FOUR> k_next, v_next;
   int counts = 0;
   auto fetch = [&](int t) {
-    auto there = [&](int j) { return key_counts(a, b, t * R + j, n); };
-    k_next.load([&](int j) { return kp + (t * R + j) * a.k.t; }, there, a.head, threadIdx.x);
-    v_next.load([&](int j) { return vp + (t * R + j) * a.v.t; }, there, a.head, threadIdx.x);
+    auto word = [&](int j) { return key_word(a, b, t * R + j, n); };
+    k_next.load([&](int j) { return kp + min(t * R + j, n - 1) * a.k.t; }, word, a.head, threadIdx.x);
+    v_next.load([&](int j) { return vp + min(t * R + j, n - 1) * a.v.t; }, word, a.head, threadIdx.x);
     counts = key_word(a, b, t * R + col, n);
   };
   if (t0 < t1) fetch(t0);
   for (int t = t0; t < t1; ++t) {
     __syncthreads();
-    k_next.store(ks, threadIdx.x);
-    v_next.store(vs, threadIdx.x);
+    auto counting = [](int word) { return word != 0; };
+    k_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP>(ks, j, d, f); }, counting, a.head, threadIdx.x);
+    v_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP>(vs, j, d, f); }, counting, a.head, threadIdx.x);
     const uint32_t valid = (uint32_t)__ballot(counts != 0) >> (4 * h);
     __syncthreads();
     if (t + 1 < t1) fetch(t + 1);
     if (idle) continue;
     float16_t s = split_over_head<DP>(hide(lds_addr_of(ks) + rows_at), [&](int k, int c) { return qf.f[k][c]; });
-    const float16_t dp = split_over_head<DP>(hide(lds_addr_of(vs) + rows_at), [&](int k, int c) { return gf.f[k][c]; });
+    const float16_t dp = split_over_head<DP>(hide(lds_addr_of(vs) + rows_at), [&](int k, int c) {
+      if constexpr (PARKED) return parked[wave][k * (DP / 16) + c][lane];
+      else return gf.f[k][c];
+    });
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const float p = exp2_(s[i] * unit - offset);
@@ -114,8 +127,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void query_grad_kernel(const
     store_fragments<T, DP>((T*)a.dq + dense_row_at(a, b, kv, r), dq, a.scale, h, a.head);
 }
 
-// Above heads of 64 the pieces of a wave's values lie in LDS: in registers they would be one set too many.
-template <typename T, int DP>
+// (as above, with the wave's keys in registers and its values in LDS)
+template <typename T, int DP, bool FOUR>
 __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void key_grad_kernel(const AttendArgs a) {
   constexpr int R = kWaveRows;
   constexpr bool PARKED = DP > 64;
@@ -150,28 +163,31 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void key_grad_kernel(const A
   float16_t dk[DP / 32], dv[DP / 32];
   zero<DP>(dk);
   zero<DP>(dv);
-  SplitStage<T, DP, 256> q_next, g_next;
-  float offset = INFINITY, delta = 0.0f;
+  RowsAhead<T, DP, 256, FOUR> q_next, g_next;
+  constexpr int kNone = (int)0xff800000;   // the bits of -inf
+  float next_lse = -INFINITY, next_delta = 0.0f;
   const float* lse = a.lse + (int64_t)bkv * a.rows;
   auto fetch = [&](int t) {
-    // the rows of a row without keys are not read: what they hold must not reach the sums
-    auto there = [&](int j) { return (int64_t)t * R + j < a.rows && lse[(int64_t)t * R + j] != -INFINITY; };
-    q_next.load([&](int j) { return (const T*)a.q.p + row_at(a.q, a, b, kv, (int64_t)t * R + j); }, there, a.head, threadIdx.x);
-    g_next.load([&](int j) { return (const T*)a.go.p + row_at(a.go, a, b, kv, (int64_t)t * R + j); }, there, a.head, threadIdx.x);
+    // a row without keys (lse = -inf) counts for nothing: what it holds must not reach the sums
+    auto row = [&](int j) { return min((int64_t)t * R + j, a.rows - 1); };
+    auto word = [&](int j) { return (int64_t)t * R + j < a.rows ? __builtin_bit_cast(int, lse[(int64_t)t * R + j]) : kNone; };
+    q_next.load([&](int j) { return (const T*)a.q.p + row_at(a.q, a, b, kv, row(j)); }, word, a.head, threadIdx.x);
+    g_next.load([&](int j) { return (const T*)a.go.p + row_at(a.go, a, b, kv, row(j)); }, word, a.head, threadIdx.x);
     if (threadIdx.x < R) {
       const int64_t r = (int64_t)t * R + threadIdx.x;
-      offset = offset_of(r < a.rows ? lse[r] : -INFINITY);
-      delta = r < a.rows && offset != INFINITY ? a.delta[(int64_t)bkv * a.rows + r] : 0.0f;
+      next_lse = r < a.rows ? lse[r] : -INFINITY;
+      next_delta = r < a.rows ? a.delta[(int64_t)bkv * a.rows + r] : 0.0f;
     }
   };
   if (t0 < t1) fetch(t0);
   for (int t = t0; t < t1; ++t) {
     __syncthreads();
-    q_next.store(qs, threadIdx.x);
-    g_next.store(gs, threadIdx.x);
+    auto counting = [](int word) { return word != kNone; };
+    q_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP>(qs, j, d, f); }, counting, a.head, threadIdx.x);
+    g_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP>(gs, j, d, f); }, counting, a.head, threadIdx.x);
     if (threadIdx.x < R) {
-      offsets[threadIdx.x] = offset;
-      deltas[threadIdx.x] = delta;
+      offsets[threadIdx.x] = offset_of(next_lse);
+      deltas[threadIdx.x] = next_lse == -INFINITY ? 0.0f : next_delta;
     }
     __syncthreads();
     if (t + 1 < t1) fetch(t + 1);
@@ -249,19 +265,22 @@ GradCut grad_cut(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys, in
 template <typename T, int DP>
 void launch_grad(AttendArgs a, const GradCut& c, bool by16, hipStream_t st) {
   const int64_t heads = (int64_t)a.batch * a.kv_heads;
+  const bool four = a.head % 4 == 0;
   if (a.rows > 0) {
     hipLaunchKernelGGL((delta_kernel<T>), dim3((unsigned)ceil_div(heads * a.rows, 16)), dim3(256), 0, st, a);
     a.row_tiles = c.row_tiles;
     a.splits = c.query_splits;
     if (by16) launch_query_grad16(a, st);
-    else hipLaunchKernelGGL((query_grad_kernel<T, DP>), dim3((unsigned)(heads * c.row_tiles * a.splits)), dim3(256), 0, st, a);
+    else if (four) hipLaunchKernelGGL((query_grad_kernel<T, DP, true>), dim3((unsigned)(heads * c.row_tiles * a.splits)), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((query_grad_kernel<T, DP, false>), dim3((unsigned)(heads * c.row_tiles * a.splits)), dim3(256), 0, st, a);
     if (a.splits > 1) hipLaunchKernelGGL((sum_rows_kernel<T>), dim3((unsigned)ceil_div(heads * a.rows, 4)), dim3(256), 0, st, a, (T*)a.dq);
   }
   if (a.keys > 0) {
     a.key_tiles = c.key_tiles;
     a.splits = c.key_splits;
     if (by16) launch_key_grad16(a, st);
-    else hipLaunchKernelGGL((key_grad_kernel<T, DP>), dim3((unsigned)(heads * c.key_tiles * a.splits)), dim3(256), 0, st, a);
+    else if (four) hipLaunchKernelGGL((key_grad_kernel<T, DP, true>), dim3((unsigned)(heads * c.key_tiles * a.splits)), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((key_grad_kernel<T, DP, false>), dim3((unsigned)(heads * c.key_tiles * a.splits)), dim3(256), 0, st, a);
     if (a.splits > 1) {
       const int64_t n = heads * a.keys * a.head;
       hipLaunchKernelGGL((sum_kernel<T>), dim3((unsigned)ceil_div(n, 256)), dim3(256), 0, st, a.part, a.splits, n, (T*)a.dk);

@@ -30,36 +30,19 @@ template <int DP>
 struct Planes {
   static constexpr int VALUES = 32 * DP, BYTES = 2 * VALUES;   // of one plane
 };
-// Rows of a token view on their way to a tile's planes: NT threads, four values at a time.
-template <typename T, int DP, int NT>
-struct SplitStage {
-  static constexpr int PER = 32 * DP / 4 / NT;
-  Four r[PER];
-  template <class Row, class There>
-  __device__ __forceinline__ void load(Row row, There there, int head, int tid) {
+// four values of row j, from d on, into a tile's planes
+template <int DP>
+__device__ __forceinline__ void store_pieces(bf16_t* planes, int j, int d, const float (&f)[4]) {
+  unsigned a[3], b[3];
+  cut_pair(f[0], f[1], a);
+  cut_pair(f[2], f[3], b);
+  bf16_t* to = planes + Rows16<bf16_t, DP>::at(j, d / 8) + d % 8;
 #pragma unroll
-    for (int p = 0; p < PER; ++p) {
-      const int at = p * NT + tid, j = at / (DP / 4), d = at % (DP / 4) * 4;
-      const bool ok = there(j);
-      r[p] = load_four<T>(ok ? row(j) : (const T*)nullptr, d, head, ok);
-    }
+  for (int k = 0; k < 3; ++k) {
+    const unsigned w[2] = {a[k], b[k]};
+    __builtin_memcpy(to + k * Planes<DP>::VALUES, w, 8);
   }
-  __device__ __forceinline__ void store(bf16_t* planes, int tid) {
-#pragma unroll
-    for (int p = 0; p < PER; ++p) {
-      const int at = p * NT + tid, j = at / (DP / 4), d = at % (DP / 4) * 4;
-      unsigned a[3], b[3];
-      cut_pair(r[p].v[0], r[p].v[1], a);
-      cut_pair(r[p].v[2], r[p].v[3], b);
-      bf16_t* to = planes + Rows16<bf16_t, DP>::at(j, d / 8) + d % 8;
-#pragma unroll
-      for (int k = 0; k < 3; ++k) {
-        const unsigned w[2] = {a[k], b[k]};
-        __builtin_memcpy(to + k * Planes<DP>::VALUES, w, 8);
-      }
-    }
-  }
-};
+}
 
 // The operands of a lane's row (values 16 c + 8 h .. + 7), in pieces.
 template <int DP>
@@ -94,18 +77,28 @@ __device__ __forceinline__ void multiply(const piece8 (&x)[3], const piece8& f0,
   rest = Half8<bf16_t>::mfma(x[0], f1, rest);
 }
 
-// The product over the head of a tile's 32 rows with a row's pieces.  at: LDS address of the planes + rows_place; f(k, c): piece k.
+// The product over the head of a tile's 32 rows with a row's pieces.  at: LDS address of the planes + rows_place; f(k, c): piece k.  What
+// one step multiplies is read while the step before it is multiplied (see OverHead).
 template <int DP, class F>
 __device__ __forceinline__ float16_t split_over_head(unsigned at, F f) {
   float16_t s, rest;
 #pragma unroll
   for (int i = 0; i < 16; ++i) s[i] = rest[i] = 0.0f;
+  piece8 x[2][3], y[2][3];
+  auto read = [&](int c) {
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      x[c & 1][k] = rows_operand<bf16_t, DP>(at + k * Planes<DP>::BYTES, 0, c);
+      y[c & 1][k] = f(k, c);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  read(0);
 #pragma unroll
   for (int c = 0; c < DP / 16; ++c) {
-    piece8 x[3];
-#pragma unroll
-    for (int k = 0; k < 3; ++k) x[k] = rows_operand<bf16_t, DP>(at + k * Planes<DP>::BYTES, 0, c);
-    multiply(x, f(0, c), f(1, c), f(2, c), s, rest);
+    if (c + 1 < DP / 16) read(c + 1);
+    multiply(x[c & 1], y[c & 1][0], y[c & 1][1], y[c & 1][2], s, rest);
+    __builtin_amdgcn_sched_barrier(0);
   }
 #pragma unroll
   for (int i = 0; i < 16; ++i) s[i] += rest[i];
@@ -114,24 +107,32 @@ __device__ __forceinline__ float16_t split_over_head(unsigned at, F f) {
 // acc[d] += the product over a tile's 32 rows with a product's registers p.  at: LDS address of the planes + columns_place.
 template <int DP>
 __device__ __forceinline__ void split_over_rows(unsigned at, const float16_t& p, float16_t (&acc)[DP / 32]) {
+  constexpr int N = 2 * (DP / 32);
+  piece8 x[2][3], f[2][3];
+  auto read = [&](int n) {
+#pragma unroll
+    for (int k = 0; k < 3; ++k) x[n & 1][k] = columns_operand<bf16_t, DP>(at + k * Planes<DP>::BYTES, 16 * (n / (DP / 32)), n % (DP / 32));
+  };
+  read(0);
+  __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    piece8 f[3];
     unsigned w[4][3];
 #pragma unroll
     for (int i = 0; i < 4; ++i) cut_pair(p[8 * c + 2 * i], p[8 * c + 2 * i + 1], w[i]);
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
       const unsigned v[4] = {w[0][k], w[1][k], w[2][k], w[3][k]};
-      __builtin_memcpy(&f[k], v, 16);
+      __builtin_memcpy(&f[c][k], v, 16);
     }
+  }
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d) {
-      piece8 x[3];
-#pragma unroll
-      for (int k = 0; k < 3; ++k) x[k] = columns_operand<bf16_t, DP>(at + k * Planes<DP>::BYTES, 16 * c, d);
-      multiply(x, f[0], f[1], f[2], acc[d], acc[d]);
-    }
+  for (int n = 0; n < N; ++n) {
+    if (n + 1 < N) read(n + 1);
+    __builtin_amdgcn_sched_barrier(0);
+    const int c = n / (DP / 32), d = n % (DP / 32);
+    multiply(x[n & 1], f[c][0], f[c][1], f[c][2], acc[d], acc[d]);
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 
