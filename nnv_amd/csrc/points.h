@@ -54,6 +54,41 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T>& r, int64_t n) {
   }
 }
 
+// The pack from element c of a row of `size` elements on, in two parts: ask() for it with no lane taking another way than its neighbours (a
+// lane that had its missing elements set to zero would have to wait for what others are loading into the same registers),
+// and settle() when it is used: what lies behind the row is zero then.  A row shorter than a pack is read element by element.
+template <typename T>
+__device__ __forceinline__ Pack<T> ask_pack(const T* row, int c, int size) {
+  if (size < kVec<T>) return load_pack(row + c, size - c);
+  Pack<T> r;
+  __builtin_memcpy(r.w, row + min(c, size - kVec<T>), 16);
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ Pack<T> settle_pack(const Pack<T>& r, int c, int size) {
+  Pack<T> s;
+  if (size < kVec<T>) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s.w[i] = c < size ? r.w[i] : 0u;
+    return s;
+  }
+  const int missing = c + kVec<T> - size;   // elements that do not exist; the others are the last ones of what was read
+  if (size % kVec<T> == 0) {                // all or none
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s.w[i] = missing > 0 ? 0u : r.w[i];
+    return s;
+  }
+  const int bits = min(max(missing, 0), kVec<T>) * 8 * (int)sizeof(T);
+  const uint64_t lo = (uint64_t)r.w[1] << 32 | r.w[0], hi = (uint64_t)r.w[3] << 32 | r.w[2];
+  const uint64_t down = bits == 0 ? lo : lo >> (bits & 63) | (bits < 64 ? hi << (-bits & 63) : 0);
+  const uint64_t l = bits < 64 ? down : bits < 128 ? hi >> (bits & 63) : 0, u = bits < 64 ? hi >> bits : 0;
+  s.w[0] = (unsigned)l;
+  s.w[1] = (unsigned)(l >> 32);
+  s.w[2] = (unsigned)u;
+  s.w[3] = (unsigned)(u >> 32);
+  return s;
+}
+
 template <typename T>
 __device__ __forceinline__ float to_f(T x) {
   return (float)x;

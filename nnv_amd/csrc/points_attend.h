@@ -134,25 +134,31 @@ template <typename T, int DP, int NT, bool FOUR>
 struct RowsAhead {
   static constexpr int PER = kWaveRows * DP / 4 / NT;
   RawFour<T> r[PER];
-  int word[PER];
-  // row(j): pointer of row j, one that exists; word(j): what says whether it counts
-  template <class Row, class Word>
-  __device__ __forceinline__ void load(Row row, Word word_of, int head, int tid) {
+  struct Words {   // what says of the same rows whether they count
+    int w[PER];
+    template <class Word>
+    __device__ __forceinline__ void load(Word word_of, int tid) {
+#pragma unroll
+      for (int p = 0; p < PER; ++p) w[p] = word_of((p * NT + tid) / (DP / 4));
+    }
+  };
+  // row(j): pointer of row j, one that exists
+  template <class Row>
+  __device__ __forceinline__ void load(Row row, int head, int tid) {
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
       const int at = p * NT + tid, j = at / (DP / 4), d = at % (DP / 4) * 4;
       if constexpr (FOUR) r[p].load(row(j), d, head);
       else r[p].load_any(row(j), d, head);
-      word[p] = word_of(j);
     }
   }
   // to(j, d, f): takes the values d .. d + 3 of row j; those of a row for which counts(word) is false are zero
   template <class To, class Counts>
-  __device__ __forceinline__ void store(To to, Counts counts, int head, int tid) const {
+  __device__ __forceinline__ void store(To to, const Words& words, Counts counts, int head, int tid) const {
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
       const int at = p * NT + tid, j = at / (DP / 4), d = at % (DP / 4) * 4;
-      const bool ok = counts(word[p]);
+      const bool ok = counts(words.w[p]);
       float f[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) f[i] = ok && d + i < head ? r[p][i] : 0.0f;

@@ -63,19 +63,21 @@ __global__ __launch_bounds__(256, DP <= 96 ? 2 : 1) void attend_kernel(const Att
   const T* kp = (const T*)a.k.p + b * a.k.b + kv * a.k.h;
   const T* vp = (const T*)a.v.p + b * a.v.b + kv * a.v.h;
   RowsAhead<T, DP, 256, FOUR> k_next, v_next;
+  typename RowsAhead<T, DP, 256, FOUR>::Words words;
   int counts = 0;
   auto fetch = [&](int t) {
     auto word = [&](int j) { return key_word(a, b, t * R + j, n); };
-    k_next.load([&](int j) { return kp + min(t * R + j, n - 1) * a.k.t; }, word, a.head, threadIdx.x);
-    v_next.load([&](int j) { return vp + min(t * R + j, n - 1) * a.v.t; }, word, a.head, threadIdx.x);
+    words.load(word, threadIdx.x);
+    k_next.load([&](int j) { return kp + min(t * R + j, n - 1) * a.k.t; }, a.head, threadIdx.x);
+    v_next.load([&](int j) { return vp + min(t * R + j, n - 1) * a.v.t; }, a.head, threadIdx.x);
     counts = key_word(a, b, t * R + col, n);
   };
   if (t0 < t1) fetch(t0);
   for (int t = t0; t < t1; ++t) {
     __syncthreads();
     auto counting = [](int word) { return word != 0; };
-    k_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP>(ks, j, d, f); }, counting, a.head, threadIdx.x);
-    v_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP>(vs, j, d, f); }, counting, a.head, threadIdx.x);
+    k_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP>(ks, j, d, f); }, words, counting, a.head, threadIdx.x);
+    v_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP>(vs, j, d, f); }, words, counting, a.head, threadIdx.x);
     const uint32_t valid = (uint32_t)__ballot(counts != 0) >> (4 * h);
     __syncthreads();
     if (t + 1 < t1) fetch(t + 1);
@@ -151,11 +153,13 @@ __global__ __launch_bounds__(256) void attend_few_kernel(const AttendArgs a) {
   const T* kp = (const T*)a.k.p + b * a.k.b + kv * a.k.h;
   const T* vp = (const T*)a.v.p + b * a.v.b + kv * a.v.h;
   RowsAhead<T, DP, 64, FOUR> ks_next, vs_next;
+  typename RowsAhead<T, DP, 64, FOUR>::Words words;
   int counts = 0;
   auto fetch = [&](int t) {
     auto word = [&](int j) { return key_word(a, b, t * R + j, n); };
-    ks_next.load([&](int j) { return kp + min(t * R + j, n - 1) * a.k.t; }, word, a.head, lane);
-    vs_next.load([&](int j) { return vp + min(t * R + j, n - 1) * a.v.t; }, word, a.head, lane);
+    words.load(word, lane);
+    ks_next.load([&](int j) { return kp + min(t * R + j, n - 1) * a.k.t; }, a.head, lane);
+    vs_next.load([&](int j) { return vp + min(t * R + j, n - 1) * a.v.t; }, a.head, lane);
     counts = key_word(a, b, t * R + col, n);
   };
   auto wave_barrier = [] {   // LDS written by other lanes of the wave
@@ -167,8 +171,8 @@ __global__ __launch_bounds__(256) void attend_few_kernel(const AttendArgs a) {
     wave_barrier();
     // rows of DP + 4 floats: a quarter wave's 16-byte reads of one column block then touch every bank once
     auto counting = [](int word) { return word != 0; };
-    ks_next.store([&](int j, int d, const float(&f)[4]) { __builtin_memcpy(ks + j * LD + d, f, 16); }, counting, a.head, lane);
-    vs_next.store([&](int j, int d, const float(&f)[4]) { __builtin_memcpy(vs + j * LD + d, f, 16); }, counting, a.head, lane);
+    ks_next.store([&](int j, int d, const float(&f)[4]) { __builtin_memcpy(ks + j * LD + d, f, 16); }, words, counting, a.head, lane);
+    vs_next.store([&](int j, int d, const float(&f)[4]) { __builtin_memcpy(vs + j * LD + d, f, 16); }, words, counting, a.head, lane);
     const uint32_t valid = (uint32_t)__ballot(counts != 0) >> (4 * h);
     wave_barrier();
     if (t + 4 < t1) fetch(t + 4);

@@ -91,19 +91,21 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void query_grad_kernel(const
   const T* kp = (const T*)a.k.p + b * a.k.b + kv * a.k.h;
   const T* vp = (const T*)a.v.p + b * a.v.b + kv * a.v.h;
   RowsAhead<T, DP, 256, FOUR> k_next, v_next;
+  typename RowsAhead<T, DP, 256, FOUR>::Words words;
   int counts = 0;
   auto fetch = [&](int t) {
     auto word = [&](int j) { return key_word(a, b, t * R + j, n); };
-    k_next.load([&](int j) { return kp + min(t * R + j, n - 1) * a.k.t; }, word, a.head, threadIdx.x);
-    v_next.load([&](int j) { return vp + min(t * R + j, n - 1) * a.v.t; }, word, a.head, threadIdx.x);
+    words.load(word, threadIdx.x);
+    k_next.load([&](int j) { return kp + min(t * R + j, n - 1) * a.k.t; }, a.head, threadIdx.x);
+    v_next.load([&](int j) { return vp + min(t * R + j, n - 1) * a.v.t; }, a.head, threadIdx.x);
     counts = key_word(a, b, t * R + col, n);
   };
   if (t0 < t1) fetch(t0);
   for (int t = t0; t < t1; ++t) {
     __syncthreads();
     auto counting = [](int word) { return word != 0; };
-    k_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP>(ks, j, d, f); }, counting, a.head, threadIdx.x);
-    v_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP>(vs, j, d, f); }, counting, a.head, threadIdx.x);
+    k_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP>(ks, j, d, f); }, words, counting, a.head, threadIdx.x);
+    v_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP>(vs, j, d, f); }, words, counting, a.head, threadIdx.x);
     const uint32_t valid = (uint32_t)__ballot(counts != 0) >> (4 * h);
     __syncthreads();
     if (t + 1 < t1) fetch(t + 1);
@@ -164,6 +166,7 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void key_grad_kernel(const A
   zero<DP>(dk);
   zero<DP>(dv);
   RowsAhead<T, DP, 256, FOUR> q_next, g_next;
+  typename RowsAhead<T, DP, 256, FOUR>::Words words;
   constexpr int kNone = (int)0xff800000;   // the bits of -inf
   float next_lse = -INFINITY, next_delta = 0.0f;
   const float* lse = a.lse + (int64_t)bkv * a.rows;
@@ -171,8 +174,9 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void key_grad_kernel(const A
     // a row without keys (lse = -inf) counts for nothing: what it holds must not reach the sums
     auto row = [&](int j) { return min((int64_t)t * R + j, a.rows - 1); };
     auto word = [&](int j) { return (int64_t)t * R + j < a.rows ? __builtin_bit_cast(int, lse[(int64_t)t * R + j]) : kNone; };
-    q_next.load([&](int j) { return (const T*)a.q.p + row_at(a.q, a, b, kv, row(j)); }, word, a.head, threadIdx.x);
-    g_next.load([&](int j) { return (const T*)a.go.p + row_at(a.go, a, b, kv, row(j)); }, word, a.head, threadIdx.x);
+    words.load(word, threadIdx.x);
+    q_next.load([&](int j) { return (const T*)a.q.p + row_at(a.q, a, b, kv, row(j)); }, a.head, threadIdx.x);
+    g_next.load([&](int j) { return (const T*)a.go.p + row_at(a.go, a, b, kv, row(j)); }, a.head, threadIdx.x);
     if (threadIdx.x < R) {
       const int64_t r = (int64_t)t * R + threadIdx.x;
       next_lse = r < a.rows ? lse[r] : -INFINITY;
@@ -183,8 +187,8 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void key_grad_kernel(const A
   for (int t = t0; t < t1; ++t) {
     __syncthreads();
     auto counting = [](int word) { return word != kNone; };
-    q_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP>(qs, j, d, f); }, counting, a.head, threadIdx.x);
-    g_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP>(gs, j, d, f); }, counting, a.head, threadIdx.x);
+    q_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP>(qs, j, d, f); }, words, counting, a.head, threadIdx.x);
+    g_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP>(gs, j, d, f); }, words, counting, a.head, threadIdx.x);
     if (threadIdx.x < R) {
       offsets[threadIdx.x] = offset_of(next_lse);
       deltas[threadIdx.x] = next_lse == -INFINITY ? 0.0f : next_delta;

@@ -79,7 +79,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_kernel(const T* __
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * LPR + lane) * V;
-      to[j] = load_pack(x + (row < rows ? row : 0) * x_stride + c, row < rows ? size - c : 0);
+      to[j] = ask_pack(x + (row < rows ? row : 0) * x_stride, c, size);
     }
   };
   const int64_t step = (int64_t)gridDim.x * kRows;
@@ -93,7 +93,11 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_kernel(const T* __
     b[j].load(offset, (j * LPR + lane) * V, size);
   }
   const float per = 1.0f / size;
-  auto turn = [&](const Pack<T>(&in)[NV]) {
+  const bool full = size == LPR * NV * V;   // every pack exists
+  auto turn = [&](const Pack<T>(&asked)[NV]) {
+    Pack<T> in[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) in[j] = full ? asked[j] : settle_pack(asked[j], (j * LPR + lane) * V, size);
     float s[1] = {0};
 #pragma unroll
     for (int j = 0; j < NV; ++j)
@@ -216,11 +220,11 @@ __global__ __launch_bounds__(kGradThreads) void norm_grad_kernel(const T* __rest
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * LPR + lane) * V;
-      to.x[j] = load_pack(x + at * x_stride + c, here ? size - c : 0);
-      to.g[j] = load_pack(dy + at * dy_stride + c, here ? size - c : 0);
+      to.x[j] = ask_pack(x + at * x_stride, c, size);
+      to.g[j] = ask_pack(dy + at * dy_stride, c, size);
     }
-    to.mu = here ? mean[at] : 0.0f;
-    to.r = here ? rstd[at] : 0.0f;
+    to.mu = mean[at];
+    to.r = rstd[at];
   };
   const int64_t step = (int64_t)gridDim.x * kRows;
   int64_t row = (int64_t)blockIdx.x * kRows + group;
@@ -233,7 +237,16 @@ __global__ __launch_bounds__(kGradThreads) void norm_grad_kernel(const T* __rest
 #pragma unroll
   for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.0f;
   const float per = 1.0f / size;
-  auto turn = [&](const Row& now) {
+  const bool full = size == LPR * NV * V && rows % step == 0;   // every pack exists, and every row of every turn
+  auto turn = [&](const Row& asked) {
+    Row now;
+    now.mu = asked.mu;
+    now.r = row < rows ? asked.r : 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      now.x[j] = full ? asked.x[j] : settle_pack(asked.x[j], (j * LPR + lane) * V, size);
+      now.g[j] = full ? asked.g[j] : settle_pack(asked.g[j], row < rows ? (j * LPR + lane) * V : size, size);   // (a row that is not there: all zero)
+    }
     const float mu = now.mu, r = now.r;
     float s[2] = {0, 0};
 #pragma unroll
@@ -437,14 +450,14 @@ void norm_forward(const void* x, int64_t xs, const void* scale, const void* offs
 template <typename T, typename W>
 void norm_backward(const void* dy, int64_t dys, const void* x, int64_t xs, const float* mean, const float* rstd, const void* scale,
                    int64_t rows, int64_t size, void* dx, void* dscale, void* doffset, float* part, int type, hipStream_t st) {
-  const int64_t blocks = grad_blocks(rows, size, type);
-  if (size > kLongest) {
-    if (rows > 0) hipLaunchKernelGGL((norm_grad_long_kernel<T, W>), dim3((unsigned)rows), dim3(kThreads), 0, st, (const T*)dy, dys, (const T*)x, xs,
+  const int64_t blocks = rows > 0 ? grad_blocks(rows, size, type) : 0;   // no rows: nothing to read, and sums of no parts
+  if (size > kLongest && rows > 0) {
+    hipLaunchKernelGGL((norm_grad_long_kernel<T, W>), dim3((unsigned)rows), dim3(kThreads), 0, st, (const T*)dy, dys, (const T*)x, xs,
                        mean, rstd, (const W*)scale, size, (T*)dx);
     if (dscale || doffset)
       hipLaunchKernelGGL((norm_grad_columns_kernel<T>), dim3((unsigned)ceil_div(size, 256), (unsigned)blocks), dim3(256), 0, st,
                          (const T*)dy, dys, (const T*)x, xs, mean, rstd, rows, size, part);
-  } else {
+  } else if (rows > 0) {
     NORM_BY_SIZE(launch_norm_grad, T, W, dy, dys, x, xs, mean, rstd, scale, rows, size, dx, dscale, doffset, part, blocks, st);
     if (blocks == 1) return;
   }
