@@ -37,9 +37,9 @@ __device__ __forceinline__ float softmax_step(float16_t& s, uint32_t valid, floa
 // Many rows: 32 a wave, 128 a block, whose waves share the tiles of keys; products in pieces.
 // Where there are too few blocks for the chip, the keys are split over `splits` blocks, and join_kernel puts their results together.
 template <typename T, int DP, bool FOUR>
-__global__ __launch_bounds__(256, DP <= 96 ? 2 : 1) void attend_kernel(const AttendArgs a) {
-  constexpr int R = kWaveRows;
-  __shared__ __attribute__((aligned(1024))) bf16_t ks[3 * R * DP], vs[3 * R * DP];
+__global__ __launch_bounds__(256, DP <= 96 || sizeof(T) == 2 ? 2 : 1) void attend_kernel(const AttendArgs a) {
+  constexpr int R = kWaveRows, PIECES = kPieces<T>;
+  __shared__ __attribute__((aligned(1024))) bf16_t ks[PIECES * R * DP], vs[PIECES * R * DP];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
   int64_t at = blockIdx.x;
   const int split = at % a.splits;
@@ -52,8 +52,9 @@ __global__ __launch_bounds__(256, DP <= 96 ? 2 : 1) void attend_kernel(const Att
   const int64_t r = (int64_t)row_tile * 128 + wave * R + col;
   const bool row_here = r < a.rows, idle = (int64_t)row_tile * 128 + wave * R >= a.rows;
   const unsigned rows_at = rows_place<bf16_t, DP>(lane), columns_at = columns_place<bf16_t, DP>(lane);
-  RowPieces<DP> qf;
-  qf.load((const T*)a.q.p + (row_here ? row_at(a.q, a, b, kv, r) : 0), h, a.head, row_here, a.scale * kLog2e);
+  RowPieces<DP, PIECES> qf;
+  qf.load((const T*)a.q.p + (row_here ? row_at(a.q, a, b, kv, r) : 0), h, a.head, row_here);
+  const float unit = a.scale * kLog2e;
   float16_t acc[DP / 32];
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d)
@@ -76,20 +77,22 @@ __global__ __launch_bounds__(256, DP <= 96 ? 2 : 1) void attend_kernel(const Att
   for (int t = t0; t < t1; ++t) {
     __syncthreads();
     auto counting = [](int word) { return word != 0; };
-    k_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP>(ks, j, d, f); }, words, counting, a.head, threadIdx.x);
-    v_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP>(vs, j, d, f); }, words, counting, a.head, threadIdx.x);
+    k_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP, PIECES>(ks, j, d, f); }, words, counting, a.head, threadIdx.x);
+    v_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP, PIECES>(vs, j, d, f); }, words, counting, a.head, threadIdx.x);
     const uint32_t valid = (uint32_t)__ballot(counts != 0) >> (4 * h);
     __syncthreads();
     if (t + 1 < t1) fetch(t + 1);
     if (idle) continue;
-    float16_t s = split_over_head<DP>(hide(lds_addr_of(ks) + rows_at), [&](int k, int c) { return qf.f[k][c]; });
+    float16_t s = split_over_head<DP, PIECES>(hide(lds_addr_of(ks) + rows_at), [&](int k, int c) { return qf.f[k][c]; });
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] *= unit;
     const float fade = softmax_step(s, valid, m, total);
     if (__any(fade != 1.0f))
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[d][i] *= fade;
-    split_over_rows<DP>(hide(lds_addr_of(vs) + columns_at), s, acc);
+    split_over_rows<DP, PIECES>(hide(lds_addr_of(vs) + columns_at), s, acc);
   }
   total = sum_of_halves(total);
   if (!row_here) return;

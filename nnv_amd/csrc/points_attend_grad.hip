@@ -58,11 +58,11 @@ __device__ __forceinline__ float offset_of(float lse) { return lse == -INFINITY 
 // Above heads of 64 the pieces of a wave's gradients of o lie in LDS: in registers they would be one set too many, and what is asked for
 // ahead would be moved to the accumulation registers, and waited for, as soon as it is asked for.
 template <typename T, int DP, bool FOUR>
-__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void query_grad_kernel(const AttendArgs a) {
-  constexpr int R = kWaveRows;
-  constexpr bool PARKED = DP > 64;
-  __shared__ __attribute__((aligned(1024))) bf16_t ks[3 * R * DP], vs[3 * R * DP];
-  __shared__ piece8 parked[PARKED ? 4 : 1][PARKED ? 3 * (DP / 16) : 1][64];
+__global__ __launch_bounds__(256, DP <= (sizeof(T) == 4 ? 64 : 96) ? 2 : 1) void query_grad_kernel(const AttendArgs a) {
+  constexpr int R = kWaveRows, PIECES = kPieces<T>;
+  constexpr bool PARKED = DP > 64 && PIECES == 3;
+  __shared__ __attribute__((aligned(1024))) bf16_t ks[PIECES * R * DP], vs[PIECES * R * DP];
+  __shared__ piece8 parked[PARKED ? 4 : 1][PARKED ? PIECES * (DP / 16) : 1][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
   int64_t at = blockIdx.x;
   const int split = at % a.splits;
@@ -78,12 +78,12 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void query_grad_kernel(const
   const bool takes_part = here && lse != -INFINITY;
   const float offset = offset_of(lse), delta = takes_part ? a.delta[flat] : 0.0f, unit = a.scale * kLog2e;
   const unsigned rows_at = rows_place<bf16_t, DP>(lane), columns_at = columns_place<bf16_t, DP>(lane);
-  RowPieces<DP> qf, gf;
-  qf.load((const T*)a.q.p + (here ? row_at(a.q, a, b, kv, r) : 0), h, a.head, takes_part, 1.0f);
-  gf.load((const T*)a.go.p + (here ? row_at(a.go, a, b, kv, r) : 0), h, a.head, takes_part, 1.0f);
+  RowPieces<DP, PIECES> qf, gf;
+  qf.load((const T*)a.q.p + (here ? row_at(a.q, a, b, kv, r) : 0), h, a.head, takes_part);
+  gf.load((const T*)a.go.p + (here ? row_at(a.go, a, b, kv, r) : 0), h, a.head, takes_part);
   if constexpr (PARKED)
 #pragma unroll
-    for (int k = 0; k < 3; ++k)
+    for (int k = 0; k < PIECES; ++k)
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c) parked[wave][k * (DP / 16) + c][lane] = gf.f[k][c];
   float16_t dq[DP / 32];
@@ -104,14 +104,14 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void query_grad_kernel(const
   for (int t = t0; t < t1; ++t) {
     __syncthreads();
     auto counting = [](int word) { return word != 0; };
-    k_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP>(ks, j, d, f); }, words, counting, a.head, threadIdx.x);
-    v_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP>(vs, j, d, f); }, words, counting, a.head, threadIdx.x);
+    k_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP, PIECES>(ks, j, d, f); }, words, counting, a.head, threadIdx.x);
+    v_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP, PIECES>(vs, j, d, f); }, words, counting, a.head, threadIdx.x);
     const uint32_t valid = (uint32_t)__ballot(counts != 0) >> (4 * h);
     __syncthreads();
     if (t + 1 < t1) fetch(t + 1);
     if (idle) continue;
-    float16_t s = split_over_head<DP>(hide(lds_addr_of(ks) + rows_at), [&](int k, int c) { return qf.f[k][c]; });
-    const float16_t dp = split_over_head<DP>(hide(lds_addr_of(vs) + rows_at), [&](int k, int c) {
+    float16_t s = split_over_head<DP, PIECES>(hide(lds_addr_of(ks) + rows_at), [&](int k, int c) { return qf.f[k][c]; });
+    const float16_t dp = split_over_head<DP, PIECES>(hide(lds_addr_of(vs) + rows_at), [&](int k, int c) {
       if constexpr (PARKED) return parked[wave][k * (DP / 16) + c][lane];
       else return gf.f[k][c];
     });
@@ -120,7 +120,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void query_grad_kernel(const
       const float p = exp2_(s[i] * unit - offset);
       s[i] = (valid >> product_row(i, 0)) & 1 ? p * (dp[i] - delta) : 0.0f;
     }
-    split_over_rows<DP>(hide(lds_addr_of(ks) + columns_at), s, dq);
+    split_over_rows<DP, PIECES>(hide(lds_addr_of(ks) + columns_at), s, dq);
   }
   if (!here) return;
   if (a.splits > 1)
@@ -131,12 +131,12 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void query_grad_kernel(const
 
 // (as above, with the wave's keys in registers and its values in LDS)
 template <typename T, int DP, bool FOUR>
-__global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void key_grad_kernel(const AttendArgs a) {
-  constexpr int R = kWaveRows;
-  constexpr bool PARKED = DP > 64;
-  __shared__ __attribute__((aligned(1024))) bf16_t qs[3 * R * DP], gs[3 * R * DP];
+__global__ __launch_bounds__(256, DP <= (sizeof(T) == 4 ? 32 : 64) ? 2 : 1) void key_grad_kernel(const AttendArgs a) {
+  constexpr int R = kWaveRows, PIECES = kPieces<T>;
+  constexpr bool PARKED = DP > 64 && PIECES == 3;
+  __shared__ __attribute__((aligned(1024))) bf16_t qs[PIECES * R * DP], gs[PIECES * R * DP];
   __shared__ float offsets[R], deltas[R];
-  __shared__ piece8 parked[PARKED ? 4 : 1][PARKED ? 3 * (DP / 16) : 1][64];
+  __shared__ piece8 parked[PARKED ? 4 : 1][PARKED ? PIECES * (DP / 16) : 1][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
   int64_t at = blockIdx.x;
   const int split = at % a.splits;
@@ -153,12 +153,12 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void key_grad_kernel(const A
     t1 = min(tiles, t0 + per);
   }
   const unsigned rows_at = rows_place<bf16_t, DP>(lane), columns_at = columns_place<bf16_t, DP>(lane);
-  RowPieces<DP> kf, vf;
-  kf.load((const T*)a.k.p + (counts ? b * a.k.b + kv * a.k.h + key * a.k.t : 0), h, a.head, counts, 1.0f);
-  vf.load((const T*)a.v.p + (counts ? b * a.v.b + kv * a.v.h + key * a.v.t : 0), h, a.head, counts, 1.0f);
+  RowPieces<DP, PIECES> kf, vf;
+  kf.load((const T*)a.k.p + (counts ? b * a.k.b + kv * a.k.h + key * a.k.t : 0), h, a.head, counts);
+  vf.load((const T*)a.v.p + (counts ? b * a.v.b + kv * a.v.h + key * a.v.t : 0), h, a.head, counts);
   if constexpr (PARKED)
 #pragma unroll
-    for (int k = 0; k < 3; ++k)
+    for (int k = 0; k < PIECES; ++k)
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c) parked[wave][k * (DP / 16) + c][lane] = vf.f[k][c];
   const float unit = a.scale * kLog2e;
@@ -187,8 +187,8 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void key_grad_kernel(const A
   for (int t = t0; t < t1; ++t) {
     __syncthreads();
     auto counting = [](int word) { return word != kNone; };
-    q_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP>(qs, j, d, f); }, words, counting, a.head, threadIdx.x);
-    g_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP>(gs, j, d, f); }, words, counting, a.head, threadIdx.x);
+    q_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP, PIECES>(qs, j, d, f); }, words, counting, a.head, threadIdx.x);
+    g_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP, PIECES>(gs, j, d, f); }, words, counting, a.head, threadIdx.x);
     if (threadIdx.x < R) {
       offsets[threadIdx.x] = offset_of(next_lse);
       deltas[threadIdx.x] = next_lse == -INFINITY ? 0.0f : next_delta;
@@ -196,17 +196,17 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void key_grad_kernel(const A
     __syncthreads();
     if (t + 1 < t1) fetch(t + 1);
     if (idle) continue;
-    float16_t s = split_over_head<DP>(hide(lds_addr_of(qs) + rows_at), [&](int k, int c) { return kf.f[k][c]; });
+    float16_t s = split_over_head<DP, PIECES>(hide(lds_addr_of(qs) + rows_at), [&](int k, int c) { return kf.f[k][c]; });
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = exp2_(s[i] * unit - offsets[product_row(i, h)]);   // (of a key that does not count: dropped below)
-    split_over_rows<DP>(hide(lds_addr_of(gs) + columns_at), s, dv);
-    const float16_t dp = split_over_head<DP>(hide(lds_addr_of(gs) + rows_at), [&](int k, int c) {
+    split_over_rows<DP, PIECES>(hide(lds_addr_of(gs) + columns_at), s, dv);
+    const float16_t dp = split_over_head<DP, PIECES>(hide(lds_addr_of(gs) + rows_at), [&](int k, int c) {
       if constexpr (PARKED) return parked[wave][k * (DP / 16) + c][lane];
       else return vf.f[k][c];
     });
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] *= dp[i] - deltas[product_row(i, h)];
-    split_over_rows<DP>(hide(lds_addr_of(qs) + columns_at), s, dk);
+    split_over_rows<DP, PIECES>(hide(lds_addr_of(qs) + columns_at), s, dk);
   }
   if (!here) return;
   if (!counts) {
@@ -224,14 +224,21 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void key_grad_kernel(const A
   }
 }
 
-// out[e] = sum over splits of part[s][e], in order
+// dk[e] = sum over splits of part[s][e], in order, and dv[e] of those behind (blockIdx.y)
 template <typename T>
-__global__ __launch_bounds__(256) void sum_kernel(const float* __restrict__ part, int splits, int64_t n, T* __restrict__ out) {
+__global__ __launch_bounds__(256) void sum_kernel(const float* __restrict__ part, int splits, int64_t n, T* __restrict__ dk, T* __restrict__ dv) {
   const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (e >= n) return;
+  part += blockIdx.y * splits * n + e;
   float s = 0.0f;
-  for (int k = 0; k < splits; ++k) s += part[k * n + e];
-  out[e] = from_f<T>(s);
+  for (int k = 0; k < splits; k += 4) {
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = k + i < splits ? part[(k + i) * n] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s += v[i];
+  }
+  (blockIdx.y ? dv : dk)[e] = from_f<T>(s);
 }
 // the same for rows in the order of lse, written in the order of the tensor
 template <typename T>
@@ -287,8 +294,7 @@ void launch_grad(AttendArgs a, const GradCut& c, bool by16, hipStream_t st) {
     else hipLaunchKernelGGL((key_grad_kernel<T, DP, false>), dim3((unsigned)(heads * c.key_tiles * a.splits)), dim3(256), 0, st, a);
     if (a.splits > 1) {
       const int64_t n = heads * a.keys * a.head;
-      hipLaunchKernelGGL((sum_kernel<T>), dim3((unsigned)ceil_div(n, 256)), dim3(256), 0, st, a.part, a.splits, n, (T*)a.dk);
-      hipLaunchKernelGGL((sum_kernel<T>), dim3((unsigned)ceil_div(n, 256)), dim3(256), 0, st, a.part + a.splits * n, a.splits, n, (T*)a.dv);
+      hipLaunchKernelGGL((sum_kernel<T>), dim3((unsigned)ceil_div(n, 256), 2), dim3(256), 0, st, a.part, a.splits, n, (T*)a.dk, (T*)a.dv);
     }
   }
 }

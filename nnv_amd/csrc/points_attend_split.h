@@ -3,21 +3,23 @@
 // each a bf16.  Of the nine products of two such numbers the six largest are formed, exactly, and added up in f32; the three left out are
 // below 2^-24 of the result, where an f32 product rounds as well.  Six products of 32x32x16 take 192 cycles; the f32 instructions
 // (32x32x2) take 512 for the same.
+//
+// Numbers of 16 bits have two pieces (a bf16 one, an f16 two, of 8 and 3 bits): four products are all of theirs.  Two pieces of a softmax's
+// weight, 16 bits, are five more than the result keeps: three products with those.
 #pragma once
 #include "points_attend16.h"
 
 namespace nnvhip {
 
 typedef half8<bf16_t> piece8;
+template <typename T>
+constexpr int kPieces = sizeof(T) == 4 ? 3 : 2;
 
-// The pieces of four numbers, two to a word.  (An infinity's rest is zero, not inf - inf.)
-struct Pieces4 {
-  unsigned w[3][2];
-};
 __device__ __forceinline__ unsigned upper_halves(float a, float b) {   // of a in the lower half of the word, of b in the upper one
   return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, b), __builtin_bit_cast(unsigned, a), 0x07060302);
 }
 __device__ __forceinline__ float cut(float x) { return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, x) & 0xffff0000u); }
+// The pieces of two numbers, each piece of both in a word.  (An infinity's rest is zero, not inf - inf.)
 __device__ __forceinline__ void cut_pair(float a, float b, unsigned (&w)[3]) {
   w[0] = upper_halves(a, b);
   const float a1 = fabsf(a) < INFINITY ? a - cut(a) : 0.0f, b1 = fabsf(b) < INFINITY ? b - cut(b) : 0.0f;
@@ -25,41 +27,41 @@ __device__ __forceinline__ void cut_pair(float a, float b, unsigned (&w)[3]) {
   w[2] = upper_halves(a1 - cut(a1), b1 - cut(b1));
 }
 
-// Tiles of 32 rows in three planes, a Rows16 tile each.
+// Tiles of 32 rows in planes, a Rows16 tile for each piece.
 template <int DP>
 struct Planes {
   static constexpr int VALUES = 32 * DP, BYTES = 2 * VALUES;   // of one plane
 };
 // four values of row j, from d on, into a tile's planes
-template <int DP>
+template <int DP, int PIECES>
 __device__ __forceinline__ void store_pieces(bf16_t* planes, int j, int d, const float (&f)[4]) {
   unsigned a[3], b[3];
   cut_pair(f[0], f[1], a);
   cut_pair(f[2], f[3], b);
   bf16_t* to = planes + Rows16<bf16_t, DP>::at(j, d / 8) + d % 8;
 #pragma unroll
-  for (int k = 0; k < 3; ++k) {
+  for (int k = 0; k < PIECES; ++k) {
     const unsigned w[2] = {a[k], b[k]};
     __builtin_memcpy(to + k * Planes<DP>::VALUES, w, 8);
   }
 }
 
 // The operands of a lane's row (values 16 c + 8 h .. + 7), in pieces.
-template <int DP>
+template <int DP, int PIECES>
 struct RowPieces {
-  piece8 f[3][DP / 16];
+  piece8 f[PIECES][DP / 16];
   template <typename T>
-  __device__ __forceinline__ void load(const T* row, int h, int head, bool there, float by) {
+  __device__ __forceinline__ void load(const T* row, int h, int head, bool there) {
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
       const Four lo = load_four(row, 16 * c + 8 * h, head, there), hi = load_four(row, 16 * c + 8 * h + 4, head, there);
       unsigned w[4][3];
-      cut_pair(lo.v[0] * by, lo.v[1] * by, w[0]);
-      cut_pair(lo.v[2] * by, lo.v[3] * by, w[1]);
-      cut_pair(hi.v[0] * by, hi.v[1] * by, w[2]);
-      cut_pair(hi.v[2] * by, hi.v[3] * by, w[3]);
+      cut_pair(lo.v[0], lo.v[1], w[0]);
+      cut_pair(lo.v[2], lo.v[3], w[1]);
+      cut_pair(hi.v[0], hi.v[1], w[2]);
+      cut_pair(hi.v[2], hi.v[3], w[3]);
 #pragma unroll
-      for (int k = 0; k < 3; ++k) {
+      for (int k = 0; k < PIECES; ++k) {
         const unsigned v[4] = {w[0][k], w[1][k], w[2][k], w[3][k]};
         __builtin_memcpy(&f[k][c], v, 16);
       }
@@ -67,27 +69,29 @@ struct RowPieces {
   }
 };
 
-// The six products of two numbers in pieces: the small ones into `rest`, so that they are added up among themselves first.
-__device__ __forceinline__ void multiply(const piece8 (&x)[3], const piece8& f0, const piece8& f1, const piece8& f2, float16_t& s, float16_t& rest) {
-  rest = Half8<bf16_t>::mfma(x[2], f0, rest);
-  s = Half8<bf16_t>::mfma(x[0], f0, s);
-  rest = Half8<bf16_t>::mfma(x[0], f2, rest);
-  rest = Half8<bf16_t>::mfma(x[1], f1, rest);
-  rest = Half8<bf16_t>::mfma(x[1], f0, rest);
-  rest = Half8<bf16_t>::mfma(x[0], f1, rest);
+// The products of two numbers in pieces: the small ones into `rest`, so that they are added up among themselves first.  ALL: two
+// pieces of either are the whole numbers, and the smallest product counts, too.
+template <int PIECES, bool ALL>
+__device__ __forceinline__ void multiply(const piece8 (&x)[PIECES], const piece8 (&f)[PIECES], float16_t& s, float16_t& rest) {
+  if constexpr (PIECES == 3) rest = Half8<bf16_t>::mfma(x[2], f[0], rest);
+  s = Half8<bf16_t>::mfma(x[0], f[0], s);
+  if constexpr (PIECES == 3) rest = Half8<bf16_t>::mfma(x[0], f[2], rest);
+  if constexpr (PIECES == 3 || ALL) rest = Half8<bf16_t>::mfma(x[1], f[1], rest);
+  rest = Half8<bf16_t>::mfma(x[1], f[0], rest);
+  rest = Half8<bf16_t>::mfma(x[0], f[1], rest);
 }
 
 // The product over the head of a tile's 32 rows with a row's pieces.  at: LDS address of the planes + rows_place; f(k, c): piece k.  What
 // one step multiplies is read while the step before it is multiplied (see OverHead).
-template <int DP, class F>
+template <int DP, int PIECES, class F>
 __device__ __forceinline__ float16_t split_over_head(unsigned at, F f) {
   float16_t s, rest;
 #pragma unroll
   for (int i = 0; i < 16; ++i) s[i] = rest[i] = 0.0f;
-  piece8 x[2][3], y[2][3];
+  piece8 x[2][PIECES], y[2][PIECES];
   auto read = [&](int c) {
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
+    for (int k = 0; k < PIECES; ++k) {
       x[c & 1][k] = rows_operand<bf16_t, DP>(at + k * Planes<DP>::BYTES, 0, c);
       y[c & 1][k] = f(k, c);
     }
@@ -97,7 +101,7 @@ __device__ __forceinline__ float16_t split_over_head(unsigned at, F f) {
 #pragma unroll
   for (int c = 0; c < DP / 16; ++c) {
     if (c + 1 < DP / 16) read(c + 1);
-    multiply(x[c & 1], y[c & 1][0], y[c & 1][1], y[c & 1][2], s, rest);
+    multiply<PIECES, true>(x[c & 1], y[c & 1], s, rest);
     __builtin_amdgcn_sched_barrier(0);
   }
 #pragma unroll
@@ -105,13 +109,13 @@ __device__ __forceinline__ float16_t split_over_head(unsigned at, F f) {
   return s;
 }
 // acc[d] += the product over a tile's 32 rows with a product's registers p.  at: LDS address of the planes + columns_place.
-template <int DP>
+template <int DP, int PIECES>
 __device__ __forceinline__ void split_over_rows(unsigned at, const float16_t& p, float16_t (&acc)[DP / 32]) {
   constexpr int N = 2 * (DP / 32);
-  piece8 x[2][3], f[2][3];
+  piece8 x[2][PIECES], f[2][PIECES];
   auto read = [&](int n) {
 #pragma unroll
-    for (int k = 0; k < 3; ++k) x[n & 1][k] = columns_operand<bf16_t, DP>(at + k * Planes<DP>::BYTES, 16 * (n / (DP / 32)), n % (DP / 32));
+    for (int k = 0; k < PIECES; ++k) x[n & 1][k] = columns_operand<bf16_t, DP>(at + k * Planes<DP>::BYTES, 16 * (n / (DP / 32)), n % (DP / 32));
   };
   read(0);
   __builtin_amdgcn_sched_barrier(0);
@@ -121,7 +125,7 @@ __device__ __forceinline__ void split_over_rows(unsigned at, const float16_t& p,
 #pragma unroll
     for (int i = 0; i < 4; ++i) cut_pair(p[8 * c + 2 * i], p[8 * c + 2 * i + 1], w[i]);
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
+    for (int k = 0; k < PIECES; ++k) {
       const unsigned v[4] = {w[0][k], w[1][k], w[2][k], w[3][k]};
       __builtin_memcpy(&f[c][k], v, 16);
     }
@@ -131,7 +135,7 @@ __device__ __forceinline__ void split_over_rows(unsigned at, const float16_t& p,
     if (n + 1 < N) read(n + 1);
     __builtin_amdgcn_sched_barrier(0);
     const int c = n / (DP / 32), d = n % (DP / 32);
-    multiply(x[n & 1], f[c][0], f[c][1], f[c][2], acc[d], acc[d]);
+    multiply<PIECES, false>(x[n & 1], f[c], acc[d], acc[d]);
     __builtin_amdgcn_sched_barrier(0);
   }
 }

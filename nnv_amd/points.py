@@ -269,29 +269,29 @@ def clip_gradients(gradients, threshold, out=None, ctx=None):
     ctx, lib, stream = _enter(what, ctx, gradients[0])
     device = gradients[0].device
     fresh = out is None
-    result = [torch.empty(g.shape, dtype=g.dtype, device=device) if isinstance(g, torch.Tensor) else None for g in gradients] if fresh else list(out)
+    if not all(isinstance(g, torch.Tensor) for g in gradients):
+        raise TypeError("%s: expected torch tensors" % what)
+    result = [torch.empty(g.shape, dtype=g.dtype, device=device) for g in gradients] if fresh else list(out)
     count = len(gradients)
     if len(result) != count:
         raise ValueError("%s: %d gradients and %d tensors to write to" % (what, count, len(result)))
-    index, types, sizes, source, target, strided = device.index, [], [], [], [], []
-    for g, y in zip(gradients, result):
-        if not isinstance(g, torch.Tensor):
-            raise TypeError("%s: expected torch tensors, got %s" % (what, type(g).__name__))
-        if g.get_device() != index:
-            raise ValueError("%s: the tensors must be on one GPU" % what)
-        kind = g.dtype
-        if not fresh and (not isinstance(y, torch.Tensor) or y.dtype != kind or y.get_device() != index or y.shape != g.shape):
+    tensor, index, dtypes, strided = torch.Tensor, device.index, [g.dtype for g in gradients], []
+    if any(i != index for i in map(tensor.get_device, gradients)):
+        raise ValueError("%s: the tensors must be on one GPU" % what)
+    if not fresh:
+        if not all(isinstance(y, tensor) for y in result) or any(i != index for i in map(tensor.get_device, result)) or \
+                [y.dtype for y in result] != dtypes or not all(map(tensor.is_same_size, result, gradients)):
             raise ValueError("%s: out must have the shapes, types and device of the gradients" % what)
-        types.append(_TYPES[kind] if kind in _TYPES else _type(what, g))
-        sizes.append(g.numel())
-        if not g.is_contiguous():
-            g = g.contiguous()
-            strided.append((None, g))           # held until the call is queued
-        if not y.is_contiguous():
-            strided.append((y, torch.empty(y.shape, dtype=y.dtype, device=device)))   # through a dense tensor, copied back below
-            y = strided[-1][1]
-        source.append(g.data_ptr())
-        target.append(y.data_ptr())
+    types = list(map(_TYPES.get, dtypes))
+    if None in types:
+        _type(what, gradients[types.index(None)])
+    dense, to = gradients, result
+    if not all(map(tensor.is_contiguous, gradients)):
+        dense = [g.contiguous() for g in gradients]
+    if not all(map(tensor.is_contiguous, result)):   # through dense tensors, copied back below
+        to = [y if y.is_contiguous() else torch.empty(y.shape, dtype=y.dtype, device=device) for y in result]
+        strided = [(y, t) for y, t in zip(result, to) if y is not t]
+    sizes, source, target = map(tensor.numel, dense), map(tensor.data_ptr, dense), map(tensor.data_ptr, to)
     norm = torch.empty((), dtype=torch.float32, device=device)
     need = _clip_workspace(lib, count)
     work = torch.empty(need, dtype=torch.uint8, device=device)
@@ -302,8 +302,7 @@ def clip_gradients(gradients, threshold, out=None, ctx=None):
                                     work.data_ptr(), need, stream))
     del held
     for y, t in strided:
-        if y is not None:
-            y.copy_(t)
+        y.copy_(t)
     return result, norm
 
 
