@@ -22,6 +22,7 @@
 namespace nnvhip {
 
 typedef float float16_t __attribute__((ext_vector_type(16)));
+typedef float float4_t __attribute__((ext_vector_type(4)));
 
 struct TokenView {   // batch x tokens x heads x head, the last index dense
   const void* p;

@@ -114,6 +114,39 @@ __global__ __launch_bounds__(256, DP <= 96 || sizeof(T) == 2 ? 2 : 1) void atten
     }
 }
 
+// What the four waves of a block found for its rows ([wave][row][DP + 4 values], with each row's maximum and sum), joined and written.
+template <typename T, int DP, int ROWS>
+__device__ __forceinline__ void join_waves(const AttendArgs& a, const float* found, const float (&row_max)[4][ROWS], const float (&row_total)[4][ROWS],
+                                           int split, int bkv, int row_tile) {
+  constexpr int LD = DP + 4;
+  for (int e = threadIdx.x; e < ROWS * (DP / 4); e += 256) {
+    const int j = e / (DP / 4), d = e % (DP / 4) * 4;
+    const int64_t rj = (int64_t)row_tile * ROWS + j;
+    if (rj >= a.rows) continue;
+    float top = row_max[0][j], all = 0.0f, w[4], f[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int k = 1; k < 4; ++k) top = fmaxf(top, row_max[k][j]);
+    const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      w[k] = exp2_(row_max[k][j] - base);
+      all += w[k] * row_total[k][j];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] += w[k] * found[(k * ROWS + j) * LD + d + i];
+    }
+    const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] *= inv;
+    const int64_t fj = (int64_t)bkv * a.rows + rj;
+    const int b = bkv / a.kv_heads, kv = bkv % a.kv_heads;
+    const float lse = all == 0.0f ? -INFINITY : (top + log2f(all)) * kLn2;
+    const int64_t sj = (int64_t)split * a.batch * a.kv_heads * a.rows + fj;
+    if (d == 0) (a.splits > 1 ? a.part_lse[sj] : a.lse[fj]) = lse;
+    if (d >= a.head) continue;
+    if (a.splits > 1) store_four(a.part + sj * a.head, d, a.head, f);
+    else store_four((T*)a.out + dense_row_at(a, b, kv, rj), d, a.head, f);
+  }}
+
 // Few rows, many keys for each (single tokens): 32 rows for the block, whose four waves take the tiles of keys in turn, each with LDS of its
 // own; what they found is joined at the end.  On the f32 matrix instructions: the keys and values are read once, and cutting each of them into
 // pieces would cost more than the instructions, which keep up with the memory.
@@ -213,32 +246,181 @@ __global__ __launch_bounds__(256) void attend_few_kernel(const AttendArgs a) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) mine[col * LD + d * 32 + product_row(i, h)] = acc[d][i];
   __syncthreads();
-  for (int e = threadIdx.x; e < R * (DP / 4); e += 256) {
-    const int j = e / (DP / 4), d = e % (DP / 4) * 4;
-    const int64_t rj = (int64_t)row_tile * R + j;
-    if (rj >= a.rows) continue;
-    float top = row_max[0][j], all = 0.0f, w[4], f[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int k = 1; k < 4; ++k) top = fmaxf(top, row_max[k][j]);
-    const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      w[k] = exp2_(row_max[k][j] - base);
-      all += w[k] * row_total[k][j];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) f[i] += w[k] * lds[(k * R + j) * LD + d + i];
-    }
-    const float inv = all == 0.0f ? 0.0f : 1.0f / all;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] *= inv;
-    const int64_t fj = (int64_t)bkv * a.rows + rj;
-    const float lse = all == 0.0f ? -INFINITY : (top + log2f(all)) * kLn2;
-    const int64_t sj = (int64_t)split * a.batch * a.kv_heads * a.rows + fj;
-    if (d == 0) (a.splits > 1 ? a.part_lse[sj] : a.lse[fj]) = lse;
-    if (d >= a.head) continue;
-    if (a.splits > 1) store_four(a.part + sj * a.head, d, a.head, f);
-    else store_four((T*)a.out + dense_row_at(a, b, kv, rj), d, a.head, f);
+  join_waves<T, DP, R>(a, lds, row_max, row_total, split, bkv, row_tile);
+}
+
+// 32 rows of f32 on their way from global memory to a wave's own tile in LDS, row after row, with no registers in between: 16 bytes a
+// lane and transfer.  The pieces of a row change places by the row, so that 16 rows' pieces of one column, and (heads of 64 and 128) the two
+// halves of what 32 lanes read of a row each, meet every bank once.
+template <int DP>
+struct FewTile {
+  static constexpr int PIECES = DP / 4, PER = 32 * PIECES / 64;
+  unsigned off[PER], there;   // bytes behind the tile's address; whether place i holds values of the head
+  __device__ __forceinline__ static int place(int row) {
+    if constexpr (DP % 64 == 0) return (row & 3) | (row >> 3 & 1) << 2 | (row >> 2 & 1) << 3;
+    else return row >> 1 & 7;
   }
+  __device__ __forceinline__ static int row(int i, int lane) { return (i * 64 + lane) / PIECES; }
+  __device__ __forceinline__ static int value(int i, int lane) { return ((i * 64 + lane) % PIECES ^ place(row(i, lane))) * 4; }
+  __device__ __forceinline__ void init(int lane, int head, int64_t stride) {
+    there = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      off[i] = 4 * (row(i, lane) * (unsigned)stride + value(i, lane));
+      there |= value(i, lane) < head ? 1u << i : 0;
+    }
+  }
+  // rows 32 t ... of those from p on; past the last of n, that one again.  Every transfer takes part, if not with every lane: it holds a whole row.
+  __device__ __forceinline__ void issue(int t, int n, const float* p, int64_t stride, unsigned lds, int lane) const {
+    if (t * 32 + 32 <= n) {
+      const float* tile = p + t * 32 * stride;
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (there >> i & 1) lds_dma16((const double*)tile, off[i], __builtin_amdgcn_readfirstlane(lds + i * 1024));
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (there >> i & 1)
+          lds_dma16_at((const double*)(p + min(t * 32 + row(i, lane), n - 1) * stride + value(i, lane)), __builtin_amdgcn_readfirstlane(lds + i * 1024));
+    }
+  }
+};
+
+// Up to 16 rows of f32, aligned (single tokens): as attend_few_kernel, on the 16x16x4 instructions.  Lane l holds column l % 16 of a product and
+// its rows 4 (l / 16) + i.  A wave's keys and values go to LDS by themselves, one tile of each: the next keys are asked for when the scores
+// are formed, the next values when they are multiplied, so that always one tile is on its way, mostly two.
+template <int DP>
+__global__ __launch_bounds__(256) void attend_few_f32_kernel(const AttendArgs a) {
+  constexpr int R = 32, TILE = R * DP, LD = DP + 4, ROWS = 16, PER = FewTile<DP>::PER;
+  __shared__ __attribute__((aligned(1024))) float lds[4 * 2 * TILE];
+  __shared__ float row_max[4][ROWS], row_total[4][ROWS];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, q4 = lane >> 4;
+  int64_t at = blockIdx.x;
+  const int split = at % a.splits;
+  const int bkv = at / a.splits, b = bkv / a.kv_heads, kv = bkv % a.kv_heads;
+  const int n = keys_that_count(a, b);
+  const int tiles = (n + R - 1) / R, per = (tiles + a.splits - 1) / a.splits;
+  const int t0 = split * per + wave, t1 = min(tiles, split * per + per);
+  const bool row_here = col < a.rows;
+  float* ks = lds + wave * 2 * TILE;
+  float* vs = ks + TILE;
+  const unsigned ks_at = lds_addr_of(ks), vs_at = ks_at + 4 * TILE;
+  if (DP != a.head) {   // the columns behind the head size, for good
+    for (int e = threadIdx.x; e < 4 * 2 * TILE; e += 256) lds[e] = 0.0f;
+    __syncthreads();
+  }
+  const float* kp = (const float*)a.k.p + b * a.k.b + kv * a.k.h;
+  const float* vp = (const float*)a.v.p + b * a.v.b + kv * a.v.h;
+  FewTile<DP> k_load, v_load;
+  k_load.init(lane, a.head, a.k.t);
+  v_load.init(lane, a.head, a.v.t);
+  if (t0 < t1) {
+    k_load.issue(t0, n, kp, a.k.t, ks_at, lane);
+    v_load.issue(t0, n, vp, a.v.t, vs_at, lane);
+  }
+  Four qf[DP / 16];   // values 16 c + 4 (l / 16) .. + 3 of row l % 16
+#pragma unroll
+  for (int c = 0; c < DP / 16; ++c)
+    qf[c] = load_four((const float*)a.q.p + (row_here ? row_at(a.q, a, b, kv, col) : 0), 16 * c + 4 * q4, a.head, row_here);
+  const float unit = a.scale * kLog2e;
+  float4_t acc[DP / 32][2];   // values 32 d + 8 (l / 16) + 2 i + j of row l % 16 in acc[d][j][i]
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d) acc[d][0] = acc[d][1] = float4_t{0, 0, 0, 0};
+  float base = -INFINITY, total = 0.0f;
+  unsigned words = 0;   // which keys of 32 tiles count, tile i in lane i
+  for (int t = t0, turn = 0; t < t1; t += 4, ++turn) {
+    uint32_t valid;
+    if (a.mask == nullptr) {
+      const int rest = n - t * R;
+      valid = rest >= R ? ~0u : (1u << rest) - 1;
+    } else {
+      // (a wait for one of a mask's bytes is a wait for all transfers ahead of it: those of 32 tiles at a time)
+      if (turn % 32 == 0)
+        for (int i = 0; i < 32; ++i) {
+          const unsigned word = (unsigned)__ballot(t + 4 * i < t1 && key_counts(a, b, (t + 4 * i) * R + lane % R, n));
+          words = lane == i ? word : words;
+        }
+      valid = (unsigned)__builtin_amdgcn_readlane(words, turn % 32);
+    }
+    wave_arrived<PER>();   // the keys; the values may still be on their way
+    float4_t s[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) s[k] = float4_t{0, 0, 0, 0};
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float f[4];
+        __builtin_memcpy(f, ks + (16 * k + col) * DP + ((4 * c + q4) ^ FewTile<DP>::place(16 * k + col)) * 4, 16);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[k] = __builtin_amdgcn_mfma_f32_16x16x4f32(f[j], qf[c].v[j], s[k], 0, 0, 0);
+      }
+    phase_wait();
+    if (t + 4 < t1) k_load.issue(t + 4, n, kp, a.k.t, ks_at, lane);
+    float top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[k][i] = valid >> (16 * k + 4 * q4 + i) & 1 ? s[k][i] * unit : -INFINITY;
+        top = fmaxf(top, s[k][i]);
+      }
+    top = fmaxf(base, max_of_quarters(top));
+    const float off = top == -INFINITY ? 0.0f : top, fade = exp2_(base - off);
+    base = top;
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[k][i] = exp2_(s[k][i] - off);
+        sum += s[k][i];
+      }
+    total = total * fade + sum;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) acc[d][0] *= fade, acc[d][1] *= fade;
+    if (t + 4 < t1) wave_arrived<PER>();
+    else wave_arrived<0>();
+    if (valid != ~0u) {   // a weight of zero must meet a zero
+#pragma unroll 1
+      for (int e = (int)hide(lane); e < R * (DP / 4); e += 64)
+        if (!(valid >> (e / (DP / 4)) & 1)) {
+          const float none[4] = {0, 0, 0, 0};
+          __builtin_memcpy(vs + 4 * e, none, 16);
+        }
+      phase_wait();
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) {
+          const int row = 16 * k + 4 * q4 + i;
+          float f[2];
+          __builtin_memcpy(f, vs + row * DP + ((8 * d + col / 2) ^ FewTile<DP>::place(row)) * 4 + col % 2 * 2, 8);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) acc[d][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(f[j], s[k][i], acc[d][j], 0, 0, 0);
+        }
+    phase_wait();
+    if (t + 4 < t1) v_load.issue(t + 4, n, vp, a.v.t, vs_at, lane);
+  }
+  total = sum_of_quarters(total);
+
+  __syncthreads();
+  float* mine = lds + wave * ROWS * LD;   // [row][d] of this wave
+  if (q4 == 0) {
+    row_max[wave][col] = base;
+    row_total[wave][col] = total;
+  }
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) mine[col * LD + d * 32 + 8 * q4 + 2 * i + j] = acc[d][j][i];
+  __syncthreads();
+  join_waves<float, DP, ROWS>(a, lds, row_max, row_total, split, bkv, 0);
 }
 
 // o = sum over splits of exp(lse_s - lse) o_s, in the order of the splits within SLICES slices and of the slices: SLICES * 32 threads a
@@ -313,19 +495,29 @@ struct Cut {
 };
 Cut cut_of(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys, int64_t head, bool by16) {
   Cut c;
-  c.few = rows <= kWaveRows;
+  c.few = rows <= (by16 ? 2 : 1) * kWaveRows;
   c.row_tiles = (int)ceil_div(rows, c.few ? kWaveRows : by16 ? attend16_tile(head) : 128);
   // blocks that the chip holds at once; what starting a block, and joining splits, costs in tiles of 32 keys
   const int64_t slots = c.few || head > (by16 ? 64 : 96) ? 256 : 512;
   const int64_t start = c.few ? 16 : by16 ? 6 : 2, join = c.few ? 16 : by16 ? 12 : 3;
-  c.splits = split_of(batch * kv_heads * c.row_tiles, ceil_div(keys, kWaveRows), c.few ? 8 : 4, slots, start, join);
+  c.splits = split_of(batch * kv_heads * c.row_tiles, ceil_div(keys, kWaveRows), c.few ? 8 : by16 ? 4 : 2, slots, start, join);
   return c;
+}
+
+// f32 rows can be moved in 16-byte pieces, and the offsets in a tile of 32 fit 31 bits
+inline bool by_fours(const TokenView& t, int64_t head) {
+  return t.t >= 0 && t.t < (int64_t(1) << 24) && head % 4 == 0 && t.b % 4 == 0 && t.t % 4 == 0 && t.h % 4 == 0 && (uintptr_t)t.p % 16 == 0;
 }
 
 template <typename T, int DP>
 void launch_attend(const AttendArgs& a, bool few, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)a.batch * a.kv_heads * a.row_tiles * a.splits));
   const bool four = a.head % 4 == 0;
+  if constexpr (sizeof(T) == 4)
+    if (a.rows <= 16 && by_fours(a.k, a.head) && by_fours(a.v, a.head)) {
+      hipLaunchKernelGGL((attend_few_f32_kernel<DP>), grid, dim3(256), 0, st, a);
+      return;
+    }
   if (few && four) hipLaunchKernelGGL((attend_few_kernel<T, DP, true>), grid, dim3(256), 0, st, a);
   else if (few) hipLaunchKernelGGL((attend_few_kernel<T, DP, false>), grid, dim3(256), 0, st, a);
   else if (four) hipLaunchKernelGGL((attend_kernel<T, DP, true>), grid, dim3(256), 0, st, a);

@@ -207,6 +207,23 @@ struct PairLoad {
   }
 };
 
+// All but the last N transfers of a wave have arrived, and no access to LDS is moved ahead of that.
+template <int N>
+__device__ __forceinline__ void wave_arrived() {
+  __builtin_amdgcn_sched_barrier(0);
+  wait_vm<N>();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+}
+// A wave's LDS accesses are done, and no instruction is moved across.
+__device__ __forceinline__ void phase_wait() {
+  __builtin_amdgcn_sched_barrier(0);
+  wait_vm_lds<63>();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+}
 // A barrier that no instruction is moved across, in front of which a wave's LDS reads are done.
 __device__ __forceinline__ void phase_barrier() {
   __builtin_amdgcn_sched_barrier(0);
@@ -235,6 +252,15 @@ __device__ __forceinline__ float max_of_halves(float x) {
 __device__ __forceinline__ float sum_of_halves(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
   return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+}
+// over the lanes l, l ^ 16, l ^ 32, l ^ 48
+__device__ __forceinline__ float max_of_quarters(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+  return max_of_halves(fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1])));
+}
+__device__ __forceinline__ float sum_of_quarters(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+  return sum_of_halves(__builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]));
 }
 // max(a, b, c) without the extra instructions that make fmaxf quiet signalling NaNs
 __device__ __forceinline__ float max3(float a, float b, float c) {

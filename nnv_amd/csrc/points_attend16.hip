@@ -6,15 +6,17 @@
 namespace nnvhip {
 namespace {
 
-// GROUPS groups of WAVES waves each.  FEW = false: the waves of a group take 32 rows each, the same ones in every group, and share tiles
-// of 64 keys, which the groups take in turn.  FEW = true: 32 rows for the block, tiles of 32 keys, groups of one wave.  What the groups
+// FEW = false (heads of up to 64): four waves take 32 rows each and share tiles of 64 keys.  FEW = true (up to 32 rows, single tokens):
+// 32 rows for the block, whose 8 waves (4 for heads above 64: LDS) are groups that take tiles of 32 keys in turn; what the groups
 // found is joined at the end.  (attend_kernel is the f32 form.)
 //
 // Tiles are on their way to LDS (no registers in between) STAGES - 1 ahead of the one that is worked on; one barrier a tile.  A weight is
 // rounded to T before the product with the values.  The running maximum is raised only when a row's has grown by more than 2^8:
 // the sums are in f32 and any base serves, so that the accumulators are hardly ever multiplied.
-template <typename T, int DP, int WAVES, int GROUPS, bool FEW, int STAGES>
-__global__ __launch_bounds__(64 * WAVES * GROUPS, FEW ? 1 : GROUPS > 1 ? 4 : 2) void attend16_kernel(const AttendArgs a) {
+constexpr int few_groups(int dp) { return dp > 64 ? 4 : 8; }
+template <typename T, int DP, bool FEW>
+__global__ __launch_bounds__(FEW ? 64 * few_groups(DP) : 256, FEW ? 1 : 2) void attend16_kernel(const AttendArgs a) {
+  constexpr int WAVES = FEW ? 1 : 4, GROUPS = FEW ? few_groups(DP) : 1, STAGES = FEW ? 2 : 4;
   constexpr int KEYS = FEW ? 32 : 64, TILE = KEYS * DP, THREADS = 64 * WAVES * GROUPS;
   typedef PairLoad<T, DP, KEYS, WAVES> Load;
   // STAGES pairs (k, v) of every group; at the end, what the groups found: [group][row][LD values]
@@ -75,12 +77,10 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, FEW ? 1 : GROUPS > 1 ? 4 : 2) 
   for (int s = 0; s < STAGES - 1; ++s)
     if (t0 + s * GROUPS < t1) fetch(t0 + s * GROUPS, s);
   int buffer = 0;
-  // the groups of a block make the same number of turns: they share its barriers
-  const int end = FEW ? t1 : t1 + group;
-  for (int t = t0, turn = 0; t < end; t += GROUPS, ++turn) {
+  for (int t = t0, turn = 0; t < t1; t += GROUPS, ++turn) {
     uint64_t valid;
     if (a.mask == nullptr) {
-      const int rest = max(n - t * KEYS, 0);
+      const int rest = n - t * KEYS;
       valid = rest >= KEYS ? ~0ull : (1ull << rest) - 1;
     } else {
       // A mask's bytes are read for 32 tiles at a time: a wait for one of them is a wait for all transfers ahead of it.
@@ -99,13 +99,12 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, FEW ? 1 : GROUPS > 1 ? 4 : 2) 
     const int ahead = buffer == 0 ? STAGES - 1 : buffer - 1;
     if constexpr (FEW) {
       if (t + (STAGES - 1) * GROUPS < t1) {
-        wait_vm_lds<63>();
+        phase_wait();
         fetch(t + (STAGES - 1) * GROUPS, ahead);
-        wait_vm<Load::COUNT * (STAGES - 1)>();
+        wave_arrived<Load::COUNT * (STAGES - 1)>();
       } else {
-        wait_vm<0>();
+        wave_arrived<0>();
       }
-      __builtin_amdgcn_wave_barrier();
     } else {
       if (t + (STAGES - 2) * GROUPS < t1) wait_vm_lds<Load::COUNT * (STAGES - 2)>();
       else wait_vm_lds<0>();
@@ -113,11 +112,11 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, FEW ? 1 : GROUPS > 1 ? 4 : 2) 
       if (t + (STAGES - 1) * GROUPS < t1) fetch(t + (STAGES - 1) * GROUPS, ahead);
     }
     buffer = buffer == STAGES - 1 ? 0 : buffer + 1;
-    if (idle || (GROUPS > 1 && !FEW && t >= t1)) continue;   // the barrier was all that was left to do
+    if (idle) continue;   // the barrier was all that was left to do
     if (valid != ~0ull) zero_rows<T, DP, KEYS>(vs, valid, lane);
 
     float16_t s[KEYS / 32];
-    over_head<T, DP, KEYS / 32, (GROUPS > 1 && !FEW ? 2 : 4)>(ks_at, 0, qf, s);
+    over_head<T, DP, KEYS / 32>(ks_at, 0, qf, s);
     if (valid != ~0ull) {
 #pragma unroll
       for (int k = 0; k < KEYS / 32; ++k) {
@@ -160,7 +159,7 @@ __global__ __launch_bounds__(64 * WAVES * GROUPS, FEW ? 1 : GROUPS > 1 ? 4 : 2) 
   total = sum_of_halves(total);
 
   const int64_t heads_rows = (int64_t)a.batch * a.kv_heads * a.rows;
-  if constexpr (GROUPS == 1) {
+  if constexpr (!FEW) {
     const int64_t flat = (int64_t)bkv * a.rows + r;
     if (!row_here) return;
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
@@ -409,16 +408,13 @@ __global__ __launch_bounds__(512, 2) void attend16_wide_kernel(const AttendArgs 
 
 template <typename T, int DP>
 void launch(const AttendArgs& a, bool few, hipStream_t st) {
-  const int64_t blocks = (int64_t)a.batch * a.kv_heads * a.row_tiles * a.splits;
-  const dim3 grid((unsigned)blocks);
+  const dim3 grid((unsigned)((int64_t)a.batch * a.kv_heads * a.row_tiles * a.splits));
   if (few) {
-    constexpr int GROUPS = DP > 64 ? 4 : 8;
-    hipLaunchKernelGGL((attend16_kernel<T, DP, 1, GROUPS, true, 2>), grid, dim3(64 * GROUPS), 0, st, a);
+    hipLaunchKernelGGL((attend16_kernel<T, DP, true>), grid, dim3(64 * few_groups(DP)), 0, st, a);
   } else if constexpr (DP > 64) {
     hipLaunchKernelGGL((attend16_wide_kernel<T, DP>), grid, dim3(512), 0, st, a);
   } else {
-    if (blocks <= 0) hipLaunchKernelGGL((attend16_kernel<T, DP, 4, 2, false, 2>), grid, dim3(512), 0, st, a);
-    else hipLaunchKernelGGL((attend16_kernel<T, DP, 4, 1, false, 4>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attend16_kernel<T, DP, false>), grid, dim3(256), 0, st, a);
   }
 }
 

@@ -153,7 +153,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void query_grad16_kernel(const Atten
 template <typename T, int DP, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void key_grad16_kernel(const AttendArgs a) {
   constexpr int ROWS = 64, TILE = ROWS * DP;
-  constexpr bool PARKED = DP > 64;   // the values' operands, in LDS
+  constexpr bool PARKED = DP > 96;   // the values' operands, in LDS
   typedef PairLoad<T, DP, ROWS, WAVES> Load;
   __shared__ __attribute__((aligned(1024))) T lds[4 * TILE + (PARKED ? WAVES * 32 * DP : 0)];
   __shared__ __attribute__((aligned(16))) float offsets[2][ROWS], deltas[2][ROWS];

@@ -264,8 +264,8 @@ GradCut grad_cut(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys, in
   c.key_tiles = (int)ceil_div(keys, by16 ? key_grad16_tile(head) : 128);
   // blocks that the chip holds at once; what starting a block, and adding splits up, costs in tiles of 32 rows
   const int64_t start = by16 ? 6 : 2, join = by16 ? 12 : 3;
-  c.query_splits = split_of(batch * kv_heads * c.row_tiles, ceil_div(keys, kWaveRows), 4, by16 || head > 64 ? 256 : 512, start, join);
-  c.key_splits = split_of(batch * kv_heads * c.key_tiles, ceil_div(rows, kWaveRows), 4, head > (by16 ? 64 : 32) ? 256 : 512, start, join);
+  c.query_splits = split_of(batch * kv_heads * c.row_tiles, ceil_div(keys, kWaveRows), 2, by16 || head > 64 ? 256 : 512, start, join);
+  c.key_splits = split_of(batch * kv_heads * c.key_tiles, ceil_div(rows, kWaveRows), 2, head > (by16 ? 64 : 32) ? 256 : 512, start, join);
   c.delta = round_up(batch * kv_heads * rows, 64);
   const int64_t q = c.query_splits > 1 ? c.query_splits * batch * kv_heads * rows * head : 0;
   const int64_t k = c.key_splits > 1 ? 2 * c.key_splits * batch * kv_heads * keys * head : 0;
