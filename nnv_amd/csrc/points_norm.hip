@@ -17,7 +17,6 @@ namespace nnvhip {
 namespace {
 
 constexpr int kThreads = 512;       // of the kernels for long rows
-constexpr int kAhead = 3;           // rows that a group of lanes has asked for
 constexpr int kGradThreads = 512;   // of the backward pass
 
 // Sum of N values over the LPR consecutive lanes that share a row, in a block of THREADS.  Rows of more than a wave add through LDS;
@@ -63,8 +62,11 @@ struct Params {
   __device__ __forceinline__ float operator[](int i) const { return to_f(p[i / kVec<W>][i % kVec<W>]); }
 };
 
-// LPR lanes a row, NV packs a lane, as many rows a block as its threads hold; a block takes rows in turn.  kAhead rows are on their
-// way while one is worked on, and the scales and offsets stay in registers over all rows.
+// LPR lanes a row, NV packs a lane, as many rows a block as its threads hold; a block takes rows in turn.  A group's next row
+// is asked for as soon as the last one is out of the registers that it comes to, and the scales and offsets stay in registers over all rows.
+//
+// Bound by memory: 16384 x 4096 in bf16 takes 53 us, 5.0 TB/s (a copy of 256 MiB: 5.4), 10176 x 2944 in f32 49 us.  One row ahead is enough: with
+// three, which the turn's end asked for, the latter took 59.
 template <typename T, typename W, int LPR, int NV>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_kernel(const T* __restrict__ x, int64_t x_stride, const W* __restrict__ scale,
                                                                      const W* __restrict__ offset, float eps, int64_t rows, int size,
@@ -74,18 +76,17 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_kernel(const T* __
   __shared__ float lds[2 * THREADS / 64];
   int slot = 0;
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
-  Pack<T> ring[kAhead][NV];
-  auto fetch = [&](int64_t row, Pack<T>(&to)[NV]) {
+  Pack<T> next[NV];
+  auto fetch = [&](int64_t row) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * LPR + lane) * V;
-      to[j] = ask_pack(x + (row < rows ? row : 0) * x_stride, c, size);
+      next[j] = ask_pack(x + (row < rows ? row : 0) * x_stride, c, size);
     }
   };
   const int64_t step = (int64_t)gridDim.x * kRows;
   int64_t row = (int64_t)blockIdx.x * kRows + group;
-#pragma unroll
-  for (int k = 0; k < kAhead; ++k) fetch(row + k * step, ring[k]);
+  fetch(row);
   Params<T, W> w[NV], b[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
@@ -94,10 +95,12 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_kernel(const T* __
   }
   const float per = 1.0f / size;
   const bool full = size == LPR * NV * V;   // every pack exists
-  auto turn = [&](const Pack<T>(&asked)[NV]) {
+  // every row of a block's turn takes part in its barriers
+  for (int64_t first = (int64_t)blockIdx.x * kRows; first < rows; first += step, row += step) {
     Pack<T> in[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) in[j] = full ? asked[j] : settle_pack(asked[j], (j * LPR + lane) * V, size);
+    for (int j = 0; j < NV; ++j) in[j] = full ? next[j] : settle_pack(next[j], (j * LPR + lane) * V, size);
+    fetch(row + step);
     float s[1] = {0};
 #pragma unroll
     for (int j = 0; j < NV; ++j)
@@ -133,18 +136,6 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_kernel(const T* __
           out.set(i, from_f<T>(v));
         }
         store_pack(y + row * (int64_t)size + c, out, size - c);
-      }
-    }
-  };
-  // every row of a block's turn takes part in its barriers
-  for (int64_t first = (int64_t)blockIdx.x * kRows; first < rows;) {
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      if (first < rows) {
-        turn(ring[k]);
-        fetch(row + kAhead * step, ring[k]);
-        first += step;
-        row += step;
       }
     }
   }
@@ -194,11 +185,16 @@ __global__ __launch_bounds__(kThreads) void norm_long_kernel(const T* __restrict
   }
 }
 
-// The backward pass.  A block's kGradThreads / LPR groups take rows in turn, kAhead of them on their way; every lane keeps the sums of its
+// The backward pass.  A block's kGradThreads / LPR groups take rows in turn, the next one on its way; every lane keeps the sums of its
 // own columns of dw and db in registers over all rows it sees.  At the end the groups of a block add theirs up in LDS, one
 // after the other, and the block writes one row of partial sums (or the result, when there is one block); column_sum_kernel
 // adds those in order.  No atomics: the same inputs give the same bits.  One block a CU: every block more would leave
-// 8 * size bytes of partial sums more, and with rows ahead two waves a SIMD keep the memory busy.
+// 8 * size bytes of partial sums more, and with a row ahead two waves a SIMD keep the memory busy (12345 x 768 in f32: 30.6 us with 256
+// blocks, 39 with 512, 41 with 128; 16384 x 4096 in bf16: 85, 89 and 132 with the next row asked for at a turn's end).
+//
+// Bound by memory: 16384 x 4096 in bf16 takes 77 us, 5.2 TB/s.  Where rows have more than a wave, the next one is asked for in front of
+// the sums, whose barriers no load is moved across (77 us; at the end of the turn 85).  Where a wave or less has them, the compiler moves the
+// loads itself, and asked for early a row would take registers twice (12345 x 768 in f32: 32.0 us; at the end 30.6).
 template <typename T, typename W, int LPR, int NV>
 __global__ __launch_bounds__(kGradThreads) void norm_grad_kernel(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ x,
                                                              int64_t x_stride, const float* __restrict__ mean,
@@ -213,23 +209,22 @@ __global__ __launch_bounds__(kGradThreads) void norm_grad_kernel(const T* __rest
   struct Row {
     Pack<T> x[NV], g[NV];
     float mu, r;
-  } ring[kAhead];
-  auto fetch = [&](int64_t row, Row& to) {
+  } next;
+  auto fetch = [&](int64_t row) {
     const bool here = row < rows;
     const int64_t at = here ? row : 0;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * LPR + lane) * V;
-      to.x[j] = ask_pack(x + at * x_stride, c, size);
-      to.g[j] = ask_pack(dy + at * dy_stride, c, size);
+      next.x[j] = ask_pack(x + at * x_stride, c, size);
+      next.g[j] = ask_pack(dy + at * dy_stride, c, size);
     }
-    to.mu = mean[at];
-    to.r = rstd[at];
+    next.mu = mean[at];
+    next.r = rstd[at];
   };
   const int64_t step = (int64_t)gridDim.x * kRows;
   int64_t row = (int64_t)blockIdx.x * kRows + group;
-#pragma unroll
-  for (int k = 0; k < kAhead; ++k) fetch(row + k * step, ring[k]);
+  fetch(row);
   Params<T, W> w[NV];
   float dw[E], db[E];
 #pragma unroll
@@ -238,16 +233,18 @@ __global__ __launch_bounds__(kGradThreads) void norm_grad_kernel(const T* __rest
   for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.0f;
   const float per = 1.0f / size;
   const bool full = size == LPR * NV * V && rows % step == 0;   // every pack exists, and every row of every turn
-  auto turn = [&](const Row& asked) {
+  // every row of a block's turn takes part in its barriers
+  for (int64_t first = (int64_t)blockIdx.x * kRows; first < rows; first += step, row += step) {
     Row now;
-    now.mu = asked.mu;
-    now.r = row < rows ? asked.r : 0.0f;
+    now.mu = next.mu;
+    now.r = row < rows ? next.r : 0.0f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      now.x[j] = full ? asked.x[j] : settle_pack(asked.x[j], (j * LPR + lane) * V, size);
-      now.g[j] = full ? asked.g[j] : settle_pack(asked.g[j], row < rows ? (j * LPR + lane) * V : size, size);   // (a row that is not there: all zero)
+      now.x[j] = full ? next.x[j] : settle_pack(next.x[j], (j * LPR + lane) * V, size);
+      now.g[j] = full ? next.g[j] : settle_pack(next.g[j], row < rows ? (j * LPR + lane) * V : size, size);   // (a row that is not there: all zero)
     }
     const float mu = now.mu, r = now.r;
+    if constexpr (LPR > 64) fetch(row + step);
     float s[2] = {0, 0};
 #pragma unroll
     for (int j = 0; j < NV; ++j)
@@ -275,18 +272,7 @@ __global__ __launch_bounds__(kGradThreads) void norm_grad_kernel(const T* __rest
         store_pack(dx + row * (int64_t)size + c, out, size - c);
       }
     }
-  };
-  // every row of a block's turn takes part in its barriers
-  for (int64_t first = (int64_t)blockIdx.x * kRows; first < rows;) {
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      if (first < rows) {
-        turn(ring[k]);
-        fetch(row + kAhead * step, ring[k]);
-        first += step;
-        row += step;
-      }
-    }
+    if constexpr (LPR <= 64) fetch(row + step);
   }
   if (dscale == nullptr && doffset == nullptr) return;
   for (int g = 0; g < kRows; ++g) {
