@@ -1,7 +1,8 @@
 // Attention of points, forward: the kernels for every type, head size and alignment.
 //
-// The products are f32 ones, whatever the type of the tensors: f32 tensors keep f32 results, and tensors of 16 bits lose nothing but
-// their final rounding.
+// The products are f32 ones, whatever the type of the tensors (points_attend_split.h): f32 tensors keep f32 results, and tensors of 16 bits, which
+// come here where their rows cannot be moved in 16-byte pieces, lose nothing but their final rounding.  That costs them: 2 x 4096 x 4096, 32 heads of 128
+// (8 for keys), in bf16 takes 1620 us here and 505 on attend16_wide_kernel; a single token, 2 x 65536 keys of 8 heads of 128, 240 and 94.
 #include "points_attend_split.h"
 
 #include <algorithm>
@@ -36,6 +37,9 @@ __device__ __forceinline__ float softmax_step(float16_t& s, uint32_t valid, floa
 
 // Many rows: 32 a wave, 128 a block, whose waves share the tiles of keys; products in pieces.
 // Where there are too few blocks for the chip, the keys are split over `splits` blocks, and join_kernel puts their results together.
+//
+// Bound by the vector units: cutting numbers into pieces and the softmax take as long as the six products.  4 x 1024 x 1024 in f32, 16 heads of 64:
+// 112 us, 153 TFLOP/s (a large f32 product of a library: 154); 8 heads of 128, one wave a SIMD: 133 us, 129 TFLOP/s.
 template <typename T, int DP, bool FOUR>
 __global__ __launch_bounds__(256, DP <= 96 || sizeof(T) == 2 ? 2 : 1) void attend_kernel(const AttendArgs a) {
   constexpr int R = kWaveRows, PIECES = kPieces<T>;
@@ -149,7 +153,8 @@ __device__ __forceinline__ void join_waves(const AttendArgs& a, const float* fou
 
 // Few rows, many keys for each (single tokens): 32 rows for the block, whose four waves take the tiles of keys in turn, each with LDS of its
 // own; what they found is joined at the end.  On the f32 matrix instructions: the keys and values are read once, and cutting each of them into
-// pieces would cost more than the instructions, which keep up with the memory.
+// pieces would cost more than the instructions.  (64 queries on 8 x 1500 f32 keys, 16 heads of 64: 50 us, in attend_kernel 42; a single token on 16 x 1500:
+// 50 here, 61 there.  So this kernel takes up to 32 rows.)
 template <typename T, int DP, bool FOUR>
 __global__ __launch_bounds__(256) void attend_few_kernel(const AttendArgs a) {
   constexpr int R = kWaveRows, LD = DP + 4;
@@ -289,6 +294,9 @@ struct FewTile {
 // Up to 16 rows of f32, aligned (single tokens): as attend_few_kernel, on the 16x16x4 instructions.  Lane l holds column l % 16 of a product and
 // its rows 4 (l / 16) + i.  A wave's keys and values go to LDS by themselves, one tile of each: the next keys are asked for when the scores
 // are formed, the next values when they are multiplied, so that always one tile is on its way, mostly two.
+//
+// Bound by memory: 2 x 32768 keys of 8 heads of 128 (32 of queries) take 100 us, 5.3 TB/s; in attend_few_kernel, whose rows go through registers, 145.
+// 16 x 1500 keys by length, 16 heads of 64: 38 us, 4.0 TB/s (50).
 template <int DP>
 __global__ __launch_bounds__(256) void attend_few_f32_kernel(const AttendArgs a) {
   constexpr int R = 32, TILE = R * DP, LD = DP + 4, ROWS = 16, PER = FewTile<DP>::PER;
@@ -424,7 +432,8 @@ __global__ __launch_bounds__(256) void attend_few_f32_kernel(const AttendArgs a)
 }
 
 // o = sum over splits of exp(lse_s - lse) o_s, in the order of the splits within SLICES slices and of the slices: SLICES * 32 threads a
-// row, four values and every SLICES-th split each.
+// row, four values and every SLICES-th split each.  Eight slices where there are more than eight splits, else one.  (Single tokens on 2 x 65536 keys, 64
+// rows of 32 splits: 94 us with, 98 without; 64 queries on 8 x 1500 keys, 8192 rows of few splits: 30 us with, 22 without.)
 template <typename T, int SLICES>
 __global__ __launch_bounds__(256) void join_kernel(const AttendArgs a) {
   constexpr int ROWS = 8 / SLICES;
@@ -487,8 +496,15 @@ __global__ __launch_bounds__(256) void join_kernel(const AttendArgs a) {
   if (lane == 0) a.lse[flat] = total == 0.0f ? -INFINITY : base + log2f(total) * kLn2;
 }
 
-// How a forward call is cut: few rows for each head's keys (single tokens) or tiles of many rows (128, or 256 where the 16-bit
-// kernels take the call), and over how many blocks the keys are split.
+// How a forward call is cut: few rows for each head's keys (single tokens) or tiles of many rows (128, or 256 where attend16_wide_kernel
+// takes the call), and over how many blocks the keys are split.
+//
+// Few are up to 64 rows of 16 bits, two tiles: 64 queries on 8 x 1500 keys, 16 heads of 64, take 17.5 us so and 22.3 as many; 96 take 25.5 and 25.0, with heads
+// of 128 on 4096 keys 91 and 64.  (f32: see attend_few_kernel.)
+//
+// Splits (see split_of): without, the single tokens on 2 x 65536 keys take 704 us instead of 94, 4 x 1024 x 1024 in f32 117 instead of 112.  Two tiles of keys are
+// the least for a split in f32: 96 queries on 477 keys, 8 heads of 80, take 20.7 us, with four 24.6.  The costs of a start and of a join in 16 bits
+// are higher, since a tile takes less: with 4 and 5 for 6 and 12, 2 x 538 x 1597, 2 heads of 128, takes 29 us instead of 25, 224 x 512, 16 of 32, 17 instead of 14.
 struct Cut {
   bool few;
   int row_tiles, splits;

@@ -281,7 +281,8 @@ __device__ __forceinline__ float largest(const float16_t (&s)[K]) {
 
 // Block `id` of `total` in an order in which each of the 8 XCDs gets consecutive ones (blocks are dealt to the XCDs in turn):
 // blocks that read the same keys then find them in one L2.  (The sequences of a batch, whose lengths may differ, follow one another
-// within a head, beginning with another one in each: every XCD and every CU gets some of each.)
+// within a head, beginning with another one in each: every XCD and every CU gets some of each.)  In the order of the blocks' numbers 8 x 448 x 1500 by length
+// takes 44.5 us instead of 41.4, the gradients of 4 x 2048 x 2048, 16 heads of 64, 294 instead of 286; heads of 128 the same.
 __device__ __forceinline__ int64_t xcd_order(int64_t id, int64_t total) {
   const int64_t x = id % 8, base = total / 8, more = total % 8;
   return x * base + min(x, more) + id / 8;

@@ -12,7 +12,13 @@ namespace {
 //
 // Tiles are on their way to LDS (no registers in between) STAGES - 1 ahead of the one that is worked on; one barrier a tile.  A weight is
 // rounded to T before the product with the values.  The running maximum is raised only when a row's has grown by more than 2^8:
-// the sums are in f32 and any base serves, so that the accumulators are hardly ever multiplied.
+// the sums are in f32 and any base serves, so that the accumulators are hardly ever multiplied (448 x 1500 by length: 41.4 us, raised with every new
+// maximum 43.0; attend16_wide_kernel's 2 x 4096 x 4096: 516 and 547).
+//
+// FEW is bound by memory: single tokens on 2 x 65536 keys of 8 heads of 128 (32 of queries) take 94 us, 5.0 TB/s; on 16 x 1500 by length, 16 heads of 64, 17.5 us,
+// 4.3 TB/s.  8 groups, where LDS has room for them: 64 such rows on 8 sequences 17.5 us, with 4 groups 23.
+// The other form by the vector units' share of the softmax, and by the last blocks where lengths differ: 8 x 448 x 1500 by length, 16 heads of 64, takes 36 us,
+// 480 TFLOP/s.  (Blocks of 64 rows take 52 us, two groups of four waves 36 to 41, three stages instead of four the same, attend16_wide_kernel 38.)
 constexpr int few_groups(int dp) { return dp > 64 ? 4 : 8; }
 template <typename T, int DP, bool FEW>
 __global__ __launch_bounds__(FEW ? 64 * few_groups(DP) : 256, FEW ? 1 : 2) void attend16_kernel(const AttendArgs a) {
@@ -234,6 +240,9 @@ __global__ __launch_bounds__(FEW ? 64 * few_groups(DP) : 256, FEW ? 1 : 2) void 
 //
 // Pair p of tiles in LDS is (keys p + 1, values p): what products p read, in halves 2 p and 2 p + 1.  There are four of them; a wave asks for
 // its share of pair p + 3 when it begins the softmax behind products p, with pair p - 1 out of use.
+//
+// 2 x 4096 x 4096, 32 heads of 128 (8 for keys): 503 us, 1090 TFLOP/s.  Bound by the power that the products may take: on zeros, where the card keeps its
+// clock, 405 us.  (Waves that do not take turns: 520 us; blocks of four waves 606.)
 template <typename T, int DP>
 __global__ __launch_bounds__(512, 2) void attend16_wide_kernel(const AttendArgs a) {
   constexpr int KEYS = 64, TILE = KEYS * DP, WAVES = 8;

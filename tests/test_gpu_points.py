@@ -248,6 +248,39 @@ def test_attention_large_and_negative_scores(dtype):
     check_attend(q, k, v, scale=0.0, tag="no scale")
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("rows", [15, 16, 17, 32, 33, 63, 64, 65])
+def test_attention_around_the_forms_for_few_rows(rows, dtype):
+    """Rows on either side of what the kernels for few rows take, of one head and of eight that share keys; tiles that the keys end in."""
+    g = gen(rows)
+    for head in (20, 32, 64, 96, 128):
+        check_attend(*make(g, 2, rows, 77, 2, 2, head, dtype), backward=False, tag="%d rows, head %d" % (rows, head))
+    if rows % 8 == 0:
+        check_attend(*make(g, 1, rows // 8, 700, 8, 1, 64, dtype), tag="%d rows of 8 heads" % rows)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_attention_single_tokens_masks_of_many_tiles(dtype):
+    """Masks over more tiles than a wave reads them for at a time, in blocks that take all keys of a sequence; strided keys and values."""
+    import nnv_amd as nnv
+    g = gen(12)
+    b, lk, h, d = 16, 5003, 16, 32
+    q = rand(g, b, 1, h, d, dtype=dtype)
+    kv = rand(g, b, lk, 2, h, d, dtype=dtype)
+    mask = torch.rand(b, lk, generator=g, device="cuda") < 0.3
+    mask[1, :4900] = False
+    mask[2, 128:] = False
+    lengths = torch.randint(0, lk + 1, (b,), generator=g, device="cuda")
+    kv[~mask] = math.nan
+    clean = torch.where(mask[:, :, None, None, None], kv, 0)
+    for kw in (dict(key_mask=mask), dict(key_mask=mask, key_lengths=lengths)):
+        o, lse = nnv.cross_attention(q, kv[:, :, 0], kv[:, :, 1], **kw)
+        eo, el = po.attend(q, clean[:, :, 0], clean[:, :, 1], **kw)
+        bo, bl = po.attend_bounds(q, clean[:, :, 0], clean[:, :, 1], **kw)
+        po.assert_within(lse, el, bl, "lse")
+        po.assert_within(o, eo, bo, "o")
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
 def test_attention_long_keys_few_rows(dtype):
     """Single tokens against many keys: the split over the keys and what joins it."""
