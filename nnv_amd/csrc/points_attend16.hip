@@ -6,17 +6,20 @@
 namespace nnvhip {
 namespace {
 
-// FEW = false (heads of up to 64): four waves take 32 rows each and share tiles of 64 keys.  FEW = true (up to 32 rows, single tokens):
+// FEW = false (heads of up to 64): four waves take 32 rows each and share tiles of 64 keys.  FEW = true (up to 64 rows, single tokens):
 // 32 rows for the block, whose 8 waves (4 for heads above 64: LDS) are groups that take tiles of 32 keys in turn; what the groups
 // found is joined at the end.  (attend_kernel is the f32 form.)
 //
-// Tiles are on their way to LDS (no registers in between) STAGES - 1 ahead of the one that is worked on; one barrier a tile.  A weight is
-// rounded to T before the product with the values.  The running maximum is raised only when a row's has grown by more than 2^8:
-// the sums are in f32 and any base serves, so that the accumulators are hardly ever multiplied (448 x 1500 by length: 41.4 us, raised with every new
-// maximum 43.0; attend16_wide_kernel's 2 x 4096 x 4096: 516 and 547).
+// Tiles are on their way to LDS (no registers in between) STAGES - 1 ahead of the one that is worked on; one barrier a tile.  The running maximum is
+// raised only when a row's has grown by more than 2^8: the sums are in f32 and any base serves, so that the accumulators are hardly ever
+// multiplied (448 x 1500 by length: 41.4 us, raised with every new maximum 43.0; attend16_wide_kernel's 2 x 4096 x 4096: 516 and 547).
 //
-// FEW is bound by memory: single tokens on 2 x 65536 keys of 8 heads of 128 (32 of queries) take 94 us, 5.0 TB/s; on 16 x 1500 by length, 16 heads of 64, 17.5 us,
-// 4.3 TB/s.  8 groups, where LDS has room for them: 64 such rows on 8 sequences 17.5 us, with 4 groups 23.
+// A weight is rounded to T before the product with the values, which adds as much to the error as the result's rounding (bf16: 0.0023 against 64 bits for
+// 0.0017), and takes half the products of two pieces.  FEW, which waits for memory, takes two pieces: what rounding leaves is a second weight (single
+// tokens as below: 18.1 us for 17.7, 93.8 for 93.7).
+//
+// FEW is bound by memory: single tokens on 2 x 65536 keys of 8 heads of 128 (32 of queries) take 94 us, 5.0 TB/s; on 16 x 1500 by length, 16 heads of 64, 18 us,
+// 4.2 TB/s.  8 groups, where LDS has room for them: 64 such rows on 8 sequences 17.5 us, with 4 groups 23.
 // The other form by its two waves a SIMD, which take products and softmax in turn: 8 x 448 x 1500 by length, 16 heads of 64, takes 36 us,
 // 480 TFLOP/s.  (Blocks of 64 rows take 52 us, two groups of four waves 36 to 41, three stages instead of four the same, attend16_wide_kernel 38;
 // the next tile's scores formed among a tile's exponentials 10 % more.)
@@ -159,8 +162,19 @@ __global__ __launch_bounds__(FEW ? 64 * few_groups(DP) : 256, FEW ? 1 : 2) void 
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const half8<T> p = round8<T>(s[k], 8 * c);
+        half8<T> rest = {};
+        if constexpr (FEW) {
+          float16_t left;
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) acc[d] = Half8<T>::mfma(columns_operand<T, DP>(vs_at, 32 * k + 16 * c, d), p, acc[d]);
+          for (int i = 0; i < 8; ++i) left[i] = s[k][8 * c + i] - (float)p[i];
+          rest = round8<T>(left, 0);
+        }
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) {
+          const half8<T> v = columns_operand<T, DP>(vs_at, 32 * k + 16 * c, d);
+          acc[d] = Half8<T>::mfma(v, p, acc[d]);
+          if constexpr (FEW) acc[d] = Half8<T>::mfma(v, rest, acc[d]);
+        }
       }
   }
   total = sum_of_halves(total);
