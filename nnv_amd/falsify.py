@@ -72,8 +72,8 @@ class CrossAttentionClassifier:
 
 
 def falsify_point(network, lb, ub, states, unsafe, starts=8, steps=50, step=0.1, seed=0, key_lengths=None, key_mask=None):
-    """A point of the box [lb, ub] (tokens x channels) whose scores lie in the HalfSpace `unsafe` (G y <= g), as a host array; None if
-    none was found, which says nothing about there being none.
+    """A point of the box [lb, ub] (tokens x channels) whose scores lie in the HalfSpace `unsafe` (G y <= g), as a host array of the
+    states' type (f32 for bf16); None if none was found, which says nothing about there being none.
 
     `starts` points drawn from the box (the first is its centre) descend on the largest row of G y - g, each coordinate by `step` times the
     box's width against the sign of its gradient, and stay in the box.  states: keys x channels."""
@@ -96,7 +96,8 @@ def falsify_point(network, lb, ub, states, unsafe, starts=8, steps=50, step=0.1,
         worst, row = margins.max(1)
         best = int(worst.argmin())
         if float(worst[best]) <= 0 and unsafe.contains(scores[best].double().cpu().numpy()):
-            return x[best].cpu().numpy()
+            point = x[best].cpu()
+            return (point.float() if point.dtype == torch.bfloat16 else point).numpy()
         if k == steps:
             return None
         dx, _ = network.backward(G[row].contiguous(), saved)
