@@ -29,5 +29,5 @@ def box64(lb, ub, dtype, weights, g, **kw):
                          ids=["f32", "bf16", "f16"])
 def test_a_point_of_every_type_is_handed_back(dtype, kept):
     """numpy has no bf16: such a point comes as f32, which holds it."""
-    found = box64([[0.0, 1.0]], [[1.0, 2.0]], dtype, [[1.0, 1.0]], [1e4])
+    found = box64([[0.0, 1.0]], [[1.0, 2.0]], dtype, [[1.0, 1.0]], [1e4], starts=1)
     assert found.dtype == kept and (found == np.array([[0.5, 1.5]])).all()
