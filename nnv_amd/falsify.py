@@ -71,22 +71,37 @@ class CrossAttentionClassifier:
                          pooled.t() @ dscores, dscores.sum(0)]
 
 
+def _bounds_within(lb, ub, like):
+    """(lb, ub) in like's type and on its device, rounded towards the inside of the box that they are given as; None where none of
+    the type's numbers lies between them."""
+    lb, ub = (torch.as_tensor(t, dtype=torch.float64, device="cpu") for t in (lb, ub))
+    if lb.shape != ub.shape or lb.dim() != 2 or not bool((lb <= ub).all()) or not bool((lb.isfinite() & ub.isfinite()).all()):
+        raise ValueError("lb and ub are the bounds of a box of tokens x channels")
+    low, high = lb.to(like.dtype), ub.to(like.dtype)
+    low = torch.where(low.double() < lb, torch.nextafter(low, torch.full_like(low, torch.inf)), low)
+    high = torch.where(high.double() > ub, torch.nextafter(high, torch.full_like(high, -torch.inf)), high)
+    return (low.to(like.device), high.to(like.device)) if bool((low <= high).all()) else None
+
+
 def falsify_point(network, lb, ub, states, unsafe, starts=8, steps=50, step=0.1, seed=0, key_lengths=None, key_mask=None):
     """A point of the box [lb, ub] (tokens x channels) whose scores lie in the HalfSpace `unsafe` (G y <= g), as a host array of the
     states' type (f32 for bf16); None if none was found, which says nothing about there being none.
 
     `starts` points drawn from the box (the first is its centre) descend on the largest row of G y - g, each coordinate by `step` times the
-    box's width against the sign of its gradient, and stay in the box.  states: keys x channels."""
+    box's width against the sign of its gradient, and stay in the box, whose bounds may be finer than the states' type.  states: keys x
+    channels."""
     if not isinstance(unsafe, HalfSpace):
         raise TypeError("unsafe must be a HalfSpace")
-    lb, ub = (torch.as_tensor(t, dtype=states.dtype, device=states.device) for t in (lb, ub))
-    if lb.shape != ub.shape or lb.dim() != 2 or bool((lb > ub).any()):
-        raise ValueError("lb and ub are the bounds of a box of tokens x channels")
+    bounds = _bounds_within(lb, ub, states)
+    if bounds is None:
+        return None
+    lb, ub = bounds
     G = torch.as_tensor(np.asarray(unsafe.G), dtype=states.dtype, device=states.device)
     g = torch.as_tensor(np.asarray(unsafe.g).reshape(-1), dtype=states.dtype, device=states.device)
     r = torch.Generator(device=states.device).manual_seed(seed)
     x = lb + (ub - lb) * torch.rand((starts,) + lb.shape, generator=r, device=states.device, dtype=states.dtype)
-    x[0] = (lb + ub) / 2
+    x[0] = lb / 2 + ub / 2
+    x = torch.minimum(torch.maximum(x, lb), ub)   # (sums are rounded)
     kept = states.expand((starts,) + states.shape)
     spread = None if key_lengths is None else key_lengths.expand(starts).contiguous()
     mask = None if key_mask is None else key_mask.expand(starts, -1)

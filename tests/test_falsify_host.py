@@ -31,3 +31,42 @@ def test_a_point_of_every_type_is_handed_back(dtype, kept):
     """numpy has no bf16: such a point comes as f32, which holds it."""
     found = box64([[0.0, 1.0]], [[1.0, 2.0]], dtype, [[1.0, 1.0]], [1e4], starts=1)
     assert found.dtype == kept and (found == np.array([[0.5, 1.5]])).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_a_point_on_the_boxs_border_is_inside(dtype, sign):
+    """Bounds in 64 bits that the states' type does not hold: the search ends on a border, and that has to be on this side of it."""
+    at = np.array([[0.1, 0.3, 1 / 3, 0.7, 1.1, 2.3]])
+    lb, ub = (at - 1.0, at) if sign > 0 else (-at, 1.0 - at)
+    # only within a hundredth of the largest sums of x: what the steps reach on the border alone
+    limit = -sign * float((ub if sign > 0 else lb).sum())
+    found = box64(lb, ub, dtype, [[-sign] * 6], [limit + 0.1], steps=40)
+    assert found is not None
+    point = np.asarray(found, dtype=np.float64)
+    assert (point >= lb).all() and (point <= ub).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["f32", "bf16", "f16"])
+def test_the_first_points_are_inside(dtype):
+    """Every point is a counterexample, so that the starts themselves are handed back: one of each seed."""
+    r = np.random.default_rng(1)
+    for seed in range(40):
+        lb = r.normal(size=(1, 300))
+        ub = lb + np.maximum(10.0 ** r.uniform(-3, 0), abs(lb) / 64)   # wider than two of bf16's numbers are apart
+        for starts in (1, 2):
+            found = box64(lb, ub, dtype, [[1.0] + [0.0] * 299], [1e4], starts=starts, steps=0, seed=seed)
+            assert found is not None
+            point = np.asarray(found, dtype=np.float64)
+            assert (point >= lb).all() and (point <= ub).all()
+
+
+def test_a_box_without_a_point_of_the_type():
+    assert box64([[0.1]], [[0.1]], torch.float32, [[1.0]], [1e4]) is None
+    assert box64([[0.125]], [[0.125]], torch.float32, [[1.0]], [1e4]) == 0.125
+
+
+def test_boxes_that_are_none():
+    for lb, ub in (([[0.2]], [[0.1]]), ([[np.nan]], [[0.1]]), ([[-np.inf]], [[0.1]]), ([0.1], [0.2])):
+        with pytest.raises(ValueError, match="bounds of a box"):
+            box64(lb, ub, torch.float32, [[1.0]], [1e4])
