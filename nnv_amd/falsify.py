@@ -109,7 +109,7 @@ def falsify_point(network, lb, ub, states, unsafe, starts=8, steps=50, step=0.1,
         scores, saved = network.forward(x, kept, spread, mask)
         margins = scores @ G.t() - g
         worst, row = margins.max(1)
-        best = int(worst.argmin())
+        best = int(worst.nan_to_num(torch.inf, torch.inf, -torch.inf).argmin())   # (a start without scores is not the best one)
         if float(worst[best]) <= 0 and unsafe.contains(scores[best].double().cpu().numpy()):
             point = x[best].cpu()
             return (point.float() if point.dtype == torch.bfloat16 else point).numpy()

@@ -70,3 +70,18 @@ def test_boxes_that_are_none():
     for lb, ub in (([[0.2]], [[0.1]]), ([[np.nan]], [[0.1]]), ([[-np.inf]], [[0.1]]), ([0.1], [0.2])):
         with pytest.raises(ValueError, match="bounds of a box"):
             box64(lb, ub, torch.float32, [[1.0]], [1e4])
+
+
+def test_a_start_without_scores_hides_no_other():
+    """A network that gives NaN for some points: the others are still looked at, and moved."""
+
+    class Broken(Linear):
+        def forward(self, x, states, key_lengths=None, key_mask=None):
+            scores, saved = super().forward(x, states)
+            return torch.where(torch.arange(len(x))[:, None] == 1, torch.nan, scores), saved
+
+    import nnv_amd as nnv
+    states = torch.zeros(1, 1)
+    for limit in (1e4, -0.4):   # met by the first points, and by steps to the lower border
+        found = nnv.falsify_point(Broken(torch.ones(1, 2)), np.zeros((1, 2)) - 0.25, np.ones((1, 2)), states, nnv.HalfSpace([[1.0]], [limit]))
+        assert found is not None and found.sum() <= limit
