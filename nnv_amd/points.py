@@ -187,8 +187,10 @@ def _attention_workspace(lib, backward, *sizes):
     return n.value
 
 
-def _mask_args(key_lengths, key_mask):
+def _mask_args(key_lengths, key_mask, keys):
     if key_lengths is not None and (key_lengths.dtype != torch.int32 or not key_lengths.is_contiguous()):
+        if key_lengths.dtype != torch.int32:   # beyond what 32 bits hold: as beyond the keys
+            key_lengths = key_lengths.clamp(0, keys)
         key_lengths = key_lengths.to(torch.int32).contiguous()
     return key_lengths, (key_mask.stride() if key_mask is not None else (0, 0))
 
@@ -197,8 +199,8 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None, ctx=No
     """softmax(scale * q k^T) v for queries of one sequence and keys and values of another.
 
     q: batch x queries x heads x head, k and v: batch x keys x kv_heads x head, any strides; consecutive heads / kv_heads
-    heads share keys and values; head is 128 at most.  key_lengths (one number per sequence) and key_mask (truth values,
-    batch x keys) say which keys count; what the others hold is of no effect.  scale: 1 / sqrt(head) if None.
+    heads share keys and values; head is 128 at most.  key_lengths (one number per sequence; beyond [0, keys]
+    it is taken as that bound) and key_mask (truth values, batch x keys) say which keys count; what the others hold is of no effect.  scale: 1 / sqrt(head) if None.
 
     Returns (o, lse): o in q's shape and type and the logarithm of the softmax's sums, batch x heads x queries, f32.
     Where no key counts o is zero and lse -inf."""
@@ -206,7 +208,7 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None, ctx=No
     ctx, lib, stream = _enter(what, ctx, q, k, v, key_lengths, key_mask)
     sizes = _attention_sizes(what, q, k, v, key_lengths, key_mask)
     q, k, v = _dense_values(q), _dense_values(k), _dense_values(v)
-    lengths, mask_stride = _mask_args(key_lengths, key_mask)
+    lengths, mask_stride = _mask_args(key_lengths, key_mask, sizes[3])
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = q.new_empty((sizes[1], sizes[4], sizes[2]), dtype=torch.float32)
     d = _ATTENTION.pack(*sizes, sizes[6] ** -0.5 if scale is None else scale, q.data_ptr(), k.data_ptr(), v.data_ptr(),
@@ -230,7 +232,7 @@ def cross_attention_backward(do, q, k, v, o, lse, key_lengths=None, key_mask=Non
         raise ValueError("%s: lse must be what cross_attention returned" % what)
     q, k, v, do = _dense_values(q), _dense_values(k), _dense_values(v), _dense_values(do)
     o, lse = o.contiguous(), lse.contiguous()
-    lengths, mask_stride = _mask_args(key_lengths, key_mask)
+    lengths, mask_stride = _mask_args(key_lengths, key_mask, sizes[3])
     dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
     d = _ATTENTION.pack(*sizes, sizes[6] ** -0.5 if scale is None else scale, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                         *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], _ptr(lengths) or 0, _ptr(key_mask) or 0,

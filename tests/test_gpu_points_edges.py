@@ -1,0 +1,31 @@
+"""The operators on points (nnv_amd.points) on the GPU, where calls are rare: lengths in 64 bits, infinite values in keys that count, scores far
+from zero, weights far below one, gradients whose norm passes f32, many sequences of many keys, and the steady state of the kernels that keep
+several tiles on their way."""
+import math
+
+import pytest
+import torch
+
+from tests import points_oracle as po
+from tests.test_gpu_points import BF16, F16, F32, IDS, TYPES, check_attend, gen, make, rand
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- lengths -------------------------------------------------------------------------------------------------
+
+
+def test_lengths_in_64_bits():
+    """A length beyond the keys is taken as all of them, one below zero as none, whatever its upper half says."""
+    import nnv_amd as nnv
+    lengths = torch.tensor([2 ** 31, 2 ** 32, 2 ** 63 - 1, 2 ** 32 + 5, -2 ** 63, -2 ** 32 + 3, -1, 3, 70], device="cuda")
+    plain = torch.tensor([70, 70, 70, 70, 0, 0, 0, 3, 70], dtype=torch.int32, device="cuda")
+    for dtype in (F32, BF16):
+        g = gen(1)
+        q, k, v = make(g, 9, 5, 70, 2, 1, 64, dtype)
+        do = rand(g, *q.shape, dtype=dtype)
+        o, lse = nnv.cross_attention(q, k, v, lengths)
+        eo, el = nnv.cross_attention(q, k, v, plain)
+        assert torch.equal(o, eo) and torch.equal(lse, el)
+        for a, b in zip(nnv.cross_attention_backward(do, q, k, v, o, lse, lengths), nnv.cross_attention_backward(do, q, k, v, o, lse, plain)):
+            assert torch.equal(a, b)
