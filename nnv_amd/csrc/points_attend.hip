@@ -6,6 +6,8 @@
 #include "points_attend_split.h"
 
 #include <algorithm>
+#include <cfloat>
+#include <cmath>
 
 #pragma clang fp contract(fast)
 
@@ -565,6 +567,7 @@ int check_sizes(const char* what, const nnvhip_attention* d) {
 int attend_args(const char* what, const nnvhip_attention* d, bool backward, AttendArgs* a) {
   if (!d) NNV_FAIL(NNVHIP_ERR_ARG, "%s: null pointer", what);
   NNV_TRY(check_sizes(what, d));
+  if (!(std::fabs(d->scale) <= FLT_MAX)) NNV_FAIL(NNVHIP_ERR_ARG, "%s: the scale must be a finite number of f32", what);
   auto view = [](const void* p, const int64_t (&s)[3]) { return TokenView{p, s[0], s[1], s[2]}; };
   *a = AttendArgs{};
   a->q = view(d->q, d->q_stride);

@@ -160,7 +160,10 @@ def _dense_values(t):
     return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
 
 
-def _attention_sizes(what, q, k, v, key_lengths, key_mask):
+_LARGEST = 3.4028234663852886e38   # of f32
+
+
+def _attention_sizes(what, q, k, v, key_lengths, key_mask, scale):
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError("%s: q, k and v are batch x tokens x heads x head" % what)
     if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
@@ -169,6 +172,10 @@ def _attention_sizes(what, q, k, v, key_lengths, key_mask):
         raise ValueError("%s: q, k and v must have one type" % what)
     batch, queries, heads, head = q.shape
     keys, kv_heads = k.shape[1], k.shape[2]
+    if not 1 <= head <= 128:
+        raise ValueError("%s: heads of 1 to 128 values are supported" % what)
+    if scale is not None and not abs(scale) <= _LARGEST:
+        raise ValueError("%s: the scale must be a finite number of f32" % what)
     if kv_heads < 1 or heads < 1 or heads % kv_heads:
         raise ValueError("%s: the number of heads must be a multiple of the number of key/value heads" % what)
     if key_lengths is not None and (key_lengths.shape != (batch,) or key_lengths.dtype not in (torch.int32, torch.int64)):
@@ -206,7 +213,7 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None, ctx=No
     Where no key counts o is zero and lse -inf."""
     what = "cross_attention"
     ctx, lib, stream = _enter(what, ctx, q, k, v, key_lengths, key_mask)
-    sizes = _attention_sizes(what, q, k, v, key_lengths, key_mask)
+    sizes = _attention_sizes(what, q, k, v, key_lengths, key_mask, scale)
     q, k, v = _dense_values(q), _dense_values(k), _dense_values(v)
     lengths, mask_stride = _mask_args(key_lengths, key_mask, sizes[3])
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
@@ -225,7 +232,7 @@ def cross_attention_backward(do, q, k, v, o, lse, key_lengths=None, key_mask=Non
     arguments are that call's.  Rows without keys and keys that do not count get zero."""
     what = "cross_attention_backward"
     ctx, lib, stream = _enter(what, ctx, q, k, v, key_lengths, key_mask, do, o, lse)
-    sizes = _attention_sizes(what, q, k, v, key_lengths, key_mask)
+    sizes = _attention_sizes(what, q, k, v, key_lengths, key_mask, scale)
     if do.shape != q.shape or do.dtype != q.dtype or o.shape != q.shape or o.dtype != q.dtype:
         raise ValueError("%s: do and o must have the shape and type of q" % what)
     if lse.shape != (sizes[1], sizes[4], sizes[2]) or lse.dtype != torch.float32:

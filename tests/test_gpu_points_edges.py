@@ -29,3 +29,20 @@ def test_lengths_in_64_bits():
         assert torch.equal(o, eo) and torch.equal(lse, el)
         for a, b in zip(nnv.cross_attention_backward(do, q, k, v, o, lse, lengths), nnv.cross_attention_backward(do, q, k, v, o, lse, plain)):
             assert torch.equal(a, b)
+
+
+# ---- arguments -----------------------------------------------------------------------------------------------
+
+
+def test_scales_that_are_no_numbers_and_heads_of_nothing_are_refused():
+    import nnv_amd as nnv
+    for dtype in TYPES:
+        q = torch.zeros(1, 2, 2, 16, device="cuda", dtype=dtype)
+        o, lse = nnv.cross_attention(q, q, q)
+        for scale in (math.nan, math.inf, -math.inf, 1e39):
+            with pytest.raises(ValueError, match="scale"):
+                nnv.cross_attention(q, q, q, scale=scale)
+            with pytest.raises(ValueError, match="scale"):
+                nnv.cross_attention_backward(q, q, q, q, o, lse, scale=scale)
+        with pytest.raises(ValueError, match="1 to 128"):
+            nnv.cross_attention(q[..., :0], q[..., :0], q[..., :0])
