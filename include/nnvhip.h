@@ -491,6 +491,9 @@ NNVHIP_API int nnvhip_layer_norm_backward(nnvhip_ctx* ctx, int type, int param_t
  * heads / kv_heads heads share keys and values.  head: 1 to 128.  The keys that count: the first key_lengths[b] of sequence b
  * (batch values; beyond [0, keys] they are taken as that bound; NULL: all), and of those the ones with key_mask != 0 (batch x keys
  * bytes with strides; NULL: all).  Keys that do not count are not read into any sum, whatever they hold.
+ * At most 65535 sequences and as many heads; keys, and the rows of a key/value head (queries * heads / kv_heads), below 2^31 - 256; tiles of
+ * 128 rows, over all key/value heads and sequences, below 2^23, and in the backward pass tiles of 128 keys as well, and batch * heads * queries
+ * below 2^28.
  *   forward: o = softmax(scale * q k^T) v (dense), lse = log of the softmax's sums (batch x heads x queries); a row for
  *     which no key counts gives o = 0, lse = -inf.
  *   backward: go (the gradient of o, strided), o and lse as the forward call gave them; dq, dk, dv dense in the shapes of q, k, v,

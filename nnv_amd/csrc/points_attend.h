@@ -108,6 +108,7 @@ __device__ __forceinline__ void store_four(T* row, int d, int head, const float 
 }
 
 constexpr int kWaveRows = 32;  // rows of a wave's tile on either side
+constexpr int64_t kMostBlocks = (int64_t(1) << 23) - 1;   // of up to 512 threads: a grid has fewer than 2^32
 
 // Four elements as the words they are loaded as (see Pack): what is asked for a tile ahead is taken apart, and found not to
 // count, when it is stored, so that nothing waits for it before.  For the same reason no lane takes another way than its neighbours: what lies

@@ -548,17 +548,20 @@ void launch_join(const AttendArgs& a, hipStream_t st) {
   else hipLaunchKernelGGL((join_kernel<T, 1>), dim3((unsigned)ceil_div(rows, 8)), dim3(256), 0, st, a);
 }
 
-// strides of the last tokens' rows have to be addressable, the sizes have to fit the kernels' indexes
+// The sizes have to fit the kernels' indexes: a key and a row of a key/value head 31 bits, with room for a tile behind the last one; the rest
+// is counted in 64.  And the threads of a grid have to be below 2^32.
 int check_sizes(const char* what, const nnvhip_attention* d) {
   if (!known_type(d->type)) NNV_FAIL(NNVHIP_ERR_ARG, "%s: the values are f32, bf16 or f16", what);
   if (d->batch < 0 || d->queries < 0 || d->keys < 0) NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: negative size", what);
   if (d->head < 1 || d->head > 128) NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: heads of 1 to 128 values are supported", what);
   if (d->heads < 1 || d->kv_heads < 1 || d->heads % d->kv_heads)
     NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: the number of heads must be a multiple of the number of key/value heads", what);
-  const int64_t most = (int64_t(1) << 31) - 256;
-  if (d->batch > 65535 || d->keys > most || d->heads > 65535 || d->queries > most / d->heads ||
-      d->batch * d->heads * ceil_div(std::max(d->queries, d->keys), 32) > most / 256)
-    NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: too many rows", what);
+  const int64_t most = (int64_t(1) << 31) - 256, group = d->heads / d->kv_heads;
+  if (d->batch > 65535 || d->heads > 65535 || d->keys > most || d->queries > most / group) NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: too many rows", what);
+  for (const bool by16 : {false, true}) {
+    const Cut c = cut_of(d->batch, d->kv_heads, d->queries * group, d->keys, d->head, by16);
+    if (d->batch * d->kv_heads * c.row_tiles * c.splits > kMostBlocks) NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: too many rows", what);
+  }
   return NNVHIP_OK;
 }
 

@@ -318,9 +318,14 @@ int nnvhip_cross_attention_backward_workspace(const nnvhip_attention* d, int64_t
   int64_t forward = 0;
   NNV_TRY(nnvhip_cross_attention_workspace(d, &forward));   // checks the sizes
   if (!bytes) NNV_FAIL(NNVHIP_ERR_ARG, "null pointer");
+  const int64_t heads = d->batch * d->kv_heads;
+  if (ceil_div(d->batch * d->heads * d->queries, 16) > 2 * kMostBlocks)   // delta_kernel's blocks, of 256 threads
+    NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_cross_attention_backward: too many rows");
   *bytes = 0;   // whichever kernels the alignment of the tensors lets take the call
   for (const bool by16 : {false, true}) {
     const GradCut c = grad_cut(d->batch, d->kv_heads, d->queries * (d->heads / d->kv_heads), d->keys, d->head, by16);
+    if (heads * c.row_tiles * c.query_splits > kMostBlocks) NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_cross_attention_backward: too many rows");
+    if (heads * c.key_tiles * c.key_splits > kMostBlocks) NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_cross_attention_backward: too many keys");
     *bytes = std::max(*bytes, (c.delta + c.part) * (int64_t)sizeof(float));
   }
   return NNVHIP_OK;

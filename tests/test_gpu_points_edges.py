@@ -31,6 +31,23 @@ def test_lengths_in_64_bits():
             assert torch.equal(a, b)
 
 
+# ---- sizes ---------------------------------------------------------------------------------------------------
+
+
+def test_many_sequences_of_many_keys():
+    """A token each for 64 sequences of 65536 keys, 64 heads on 8: 17 GB of keys and values, were the sequences not one and the same here."""
+    import nnv_amd as nnv
+    g = gen(4)
+    q, k, v = make(g, 1, 1, 65536, 64, 8, 128, BF16)
+    lengths = torch.arange(64, 0, -1, device="cuda", dtype=torch.int32) * 1024
+    o, lse = nnv.cross_attention(q.expand(64, -1, -1, -1), k.expand(64, -1, -1, -1), v.expand(64, -1, -1, -1), lengths)
+    for i in (0, 1, 40, 63):
+        n = int(lengths[i])
+        (eo, el), (bo, bl) = po.attend(q, k[:, :n], v[:, :n]), po.attend_bounds(q, k[:, :n], v[:, :n])
+        po.assert_within(lse[i:i + 1], el, bl, "lse of sequence %d" % i)
+        po.assert_within(o[i:i + 1], eo, bo, "sequence %d" % i)
+
+
 # ---- arguments -----------------------------------------------------------------------------------------------
 
 
