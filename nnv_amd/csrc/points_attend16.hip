@@ -16,9 +16,10 @@ namespace {
 //
 // A weight is rounded to T before the product with the values, which adds as much to the error as the result's rounding (bf16: 0.0023 against 64 bits for
 // 0.0017), and takes half the products of two pieces.  FEW, which waits for memory, takes two pieces: what rounding leaves is a second weight (single
-// tokens as below: 18.1 us for 17.7, 93.8 for 93.7).
+// tokens as below: 18.0 us for 17.7, 94.5 for 93.7).  The second weights have sums of their own: one may be zero, or below zero, and an infinite value
+// times it is not added to what the weight itself makes of that value.
 //
-// FEW is bound by memory: single tokens on 2 x 65536 keys of 8 heads of 128 (32 of queries) take 94 us, 5.0 TB/s; on 16 x 1500 by length, 16 heads of 64, 18 us,
+// FEW is bound by memory: single tokens on 2 x 65536 keys of 8 heads of 128 (32 of queries) take 94.5 us, 5.0 TB/s; on 16 x 1500 by length, 16 heads of 64, 18 us,
 // 4.2 TB/s.  8 groups, where LDS has room for them: 64 such rows on 8 sequences 17.5 us, with 4 groups 23.
 // The other form by its two waves a SIMD, which take products and softmax in turn: 8 x 448 x 1500 by length, 16 heads of 64, takes 36 us,
 // 480 TFLOP/s.  (Blocks of 64 rows take 52 us, two groups of four waves 36 to 41, three stages instead of four the same, attend16_wide_kernel 38;
@@ -67,11 +68,11 @@ __global__ __launch_bounds__(FEW ? 64 * few_groups(DP) : 256, FEW ? 1 : 2) void 
       if (a.scale < 0) qf[c] = -qf[c];
     }
   }
-  float16_t acc[DP / 32];
+  float16_t acc[DP / 32], second[FEW ? DP / 32 : 1];   // second: of what the weights' rounding leaves
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
+    for (int i = 0; i < 16; ++i) acc[d][i] = second[FEW ? d : 0][i] = 0.0f;
   float base = -INFINITY, total = 0.0f;   // base: of the exponents, in products times unit
 
   const T* kp = (const T*)a.k.p + b * a.k.b + kv * a.k.h;
@@ -145,7 +146,10 @@ __global__ __launch_bounds__(FEW ? 64 * few_groups(DP) : 256, FEW ? 1 : 2) void 
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[d][i] *= fade;
+        for (int i = 0; i < 16; ++i) {
+          acc[d][i] *= fade;
+          if constexpr (FEW) second[d][i] *= fade;
+        }
     }
     const float off = base == -INFINITY ? 0.0f : base;
     float sum[2] = {0.0f, 0.0f};
@@ -173,7 +177,7 @@ __global__ __launch_bounds__(FEW ? 64 * few_groups(DP) : 256, FEW ? 1 : 2) void 
         for (int d = 0; d < DP / 32; ++d) {
           const half8<T> v = columns_operand<T, DP>(vs_at, 32 * k + 16 * c, d);
           acc[d] = Half8<T>::mfma(v, p, acc[d]);
-          if constexpr (FEW) acc[d] = Half8<T>::mfma(v, rest, acc[d]);
+          if constexpr (FEW) second[d] = Half8<T>::mfma(v, rest, second[d]);
         }
       }
   }
@@ -213,7 +217,10 @@ __global__ __launch_bounds__(FEW ? 64 * few_groups(DP) : 256, FEW ? 1 : 2) void 
       for (int i4 = 0; i4 < 4; ++i4) {
         float f[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = acc[d][4 * i4 + i];
+        for (int i = 0; i < 4; ++i) {
+          const float first = acc[d][4 * i4 + i];
+          f[i] = fabsf(first) < INFINITY ? first + second[d][4 * i4 + i] : first;
+        }
         __builtin_memcpy(found + d * 32 + 8 * i4 + 4 * h, f, 16);
       }
     __syncthreads();

@@ -31,6 +31,33 @@ def test_lengths_in_64_bits():
             assert torch.equal(a, b)
 
 
+# ---- infinite values that count --------------------------------------------------------------------------------
+
+
+def check_infinite_values(rows, head, dtype):
+    import nnv_amd as nnv
+    g = gen(rows + head)
+    q, k, v = make(g, 2, rows, 90, 2, 2, head, dtype)
+    v[0, 3, 0, 1], v[0, 70, 0, 1] = math.inf, math.inf
+    v[0, 89, 1, 4] = -math.inf
+    o, lse = nnv.cross_attention(q, k, v)
+    po.assert_within(lse, po.attend(q, k, v)[1], po.attend_bounds(q, k, v)[1], "%d rows, head %d: lse" % (rows, head))
+    po.assert_within(o, po.attend(q, k, v)[0], po.attend_bounds(q, k, v)[0], "%d rows, head %d" % (rows, head))
+    v[1, 5, 0, 2], v[1, 60, 0, 2], v[1, 7, 1, 3] = math.inf, -math.inf, math.nan
+    o, _ = nnv.cross_attention(q, k, v)
+    none = torch.zeros_like(o, dtype=torch.bool)
+    none[1, :, 0, 2] = none[1, :, 1, 3] = True
+    assert torch.equal(torch.isnan(o), none)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("rows", [1, 16, 17, 32, 33, 64, 65, 200])
+def test_infinite_values_of_keys_that_count_in_16_bits(rows, dtype):
+    """A weight is above zero, so that an infinite value makes the result infinite, and nothing else, however many rows there are."""
+    for head in (40, 64, 128):
+        check_infinite_values(rows, head, dtype)
+
+
 # ---- sizes ---------------------------------------------------------------------------------------------------
 
 
