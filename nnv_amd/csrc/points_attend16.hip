@@ -6,6 +6,11 @@
 namespace nnvhip {
 namespace {
 
+// The weights of the softmax are multiples of exp(score - the largest score): in f16 of 2^7, so that what is rounded to T keeps weights down to 2^-32 of the
+// largest (2^-25 without; a million keys of 2^-26 would be lost), and the largest, which the offset may lag behind by 2^8, stays in f16's range.
+template <typename T>
+constexpr float kLift = std::is_same_v<T, f16_t> ? 7.0f : 0.0f;
+
 // FEW = false (heads of up to 64): four waves take 32 rows each and share tiles of 64 keys.  FEW = true (up to 64 rows, single tokens):
 // 32 rows for the block, whose 8 waves (4 for heads above 64: LDS) are groups that take tiles of 32 keys in turn; what the groups
 // found is joined at the end.  (attend_kernel is the f32 form.)
@@ -73,7 +78,7 @@ __global__ __launch_bounds__(FEW ? 64 * few_groups(DP) : 256, FEW ? 1 : 2) void 
   for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[d][i] = second[FEW ? d : 0][i] = 0.0f;
-  float base = -INFINITY, total = 0.0f;   // base: of the exponents, in products times unit
+  float off = -INFINITY, total = 0.0f;   // off: of the exponents, in products times unit
 
   const T* kp = (const T*)a.k.p + b * a.k.b + kv * a.k.h;
   const T* vp = (const T*)a.v.p + b * a.v.b + kv * a.v.h;
@@ -138,10 +143,10 @@ __global__ __launch_bounds__(FEW ? 64 * few_groups(DP) : 256, FEW ? 1 : 2) void 
     }
     float top = largest(s);
     top = max_of_halves(top) * unit;
-    if (__any(top > base + 8.0f)) {   // also: the first keys of a row that count
-      const float next = fmaxf(base, top);
-      const float fade = next == -INFINITY ? 1.0f : exp2_(base - next);
-      base = next;
+    if (__any(top > off + (8.0f + kLift<T>))) {   // also: the first keys of a row that count
+      const float next = fmaxf(off, top - kLift<T>);
+      const float fade = next == -INFINITY ? 1.0f : exp2_(off - next);
+      off = next;
       total *= fade;
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
@@ -151,13 +156,13 @@ __global__ __launch_bounds__(FEW ? 64 * few_groups(DP) : 256, FEW ? 1 : 2) void 
           if constexpr (FEW) second[d][i] *= fade;
         }
     }
-    const float off = base == -INFINITY ? 0.0f : base;
+    const float by = off == -INFINITY ? 0.0f : off;
     float sum[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < KEYS / 32; ++k)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        s[k][i] = exp2_(s[k][i] * unit - off);
+        s[k][i] = exp2_(s[k][i] * unit - by);
         sum[i & 1] += s[k][i];
       }
     total += sum[0] + sum[1];
@@ -188,7 +193,7 @@ __global__ __launch_bounds__(FEW ? 64 * few_groups(DP) : 256, FEW ? 1 : 2) void 
     const int64_t flat = (int64_t)bkv * a.rows + r;
     if (!row_here) return;
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    const float lse = total == 0.0f ? -INFINITY : (base + log2f(total)) * kLn2;
+    const float lse = total == 0.0f ? -INFINITY : (off + log2f(total)) * kLn2;
     if (h == 0) (a.splits > 1 ? a.part_lse[split * heads_rows + flat] : a.lse[flat]) = lse;
     float* part = a.splits > 1 ? a.part + (split * heads_rows + flat) * a.head : nullptr;
     T* out = (T*)a.out + dense_row_at(a, b, kv, r);
@@ -208,7 +213,7 @@ __global__ __launch_bounds__(FEW ? 64 * few_groups(DP) : 256, FEW ? 1 : 2) void 
     float* all_found = (float*)lds;
     float* found = all_found + (group * ROWS + wave * 32 + col) * LD;
     if (h == 0) {
-      row_max[group][wave * 32 + col] = base;
+      row_max[group][wave * 32 + col] = off;
       row_total[group][wave * 32 + col] = total;
     }
 #pragma unroll
@@ -231,10 +236,10 @@ __global__ __launch_bounds__(FEW ? 64 * few_groups(DP) : 256, FEW ? 1 : 2) void 
       float top = row_max[0][j], all = 0.0f, f[4] = {0, 0, 0, 0};
 #pragma unroll
       for (int k = 1; k < GROUPS; ++k) top = fmaxf(top, row_max[k][j]);
-      const float off = top == -INFINITY ? 0.0f : top;
+      const float by = top == -INFINITY ? 0.0f : top;
 #pragma unroll
       for (int k = 0; k < GROUPS; ++k) {
-        const float w = exp2_(row_max[k][j] - off);
+        const float w = exp2_(row_max[k][j] - by);
         all += w * row_total[k][j];
 #pragma unroll
         for (int i = 0; i < 4; ++i) f[i] += w * all_found[(k * ROWS + j) * LD + d + i];
@@ -305,7 +310,7 @@ __global__ __launch_bounds__(512, 2) void attend16_wide_kernel(const AttendArgs 
   for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
-  float base = -INFINITY, total = 0.0f;
+  float off = -INFINITY, total = 0.0f;
   half8<T> p[4];
   uint64_t valid = 0;
   unsigned words[2];   // which keys of 32 tiles count, tile i in lane i
@@ -345,17 +350,17 @@ __global__ __launch_bounds__(512, 2) void attend16_wide_kernel(const AttendArgs 
       }
     }
     const float top = max_of_halves(largest(s)) * unit;
-    if (__any(top > base + 8.0f)) {   // also: the first keys of a row that count
-      const float next = fmaxf(base, top);
-      const float fade = next == -INFINITY ? 1.0f : exp2_(base - next);
-      base = next;
+    if (__any(top > off + (8.0f + kLift<T>))) {   // also: the first keys of a row that count
+      const float next = fmaxf(off, top - kLift<T>);
+      const float fade = next == -INFINITY ? 1.0f : exp2_(off - next);
+      off = next;
       total *= fade;
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[d][i] *= fade;
     }
-    const float off = base == -INFINITY ? 0.0f : base;
+    const float by = off == -INFINITY ? 0.0f : off;
     float sum[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < 2; ++k)
@@ -363,7 +368,7 @@ __global__ __launch_bounds__(512, 2) void attend16_wide_kernel(const AttendArgs 
       for (int c = 0; c < 2; ++c) {
 #pragma unroll
         for (int i = 8 * c; i < 8 * c + 8; ++i) {
-          s[k][i] = exp2_(s[k][i] * unit - off);
+          s[k][i] = exp2_(s[k][i] * unit - by);
           sum[i & 1] += s[k][i];
         }
         p[2 * k + c] = round8<T>(s[k], 8 * c);
@@ -420,7 +425,7 @@ __global__ __launch_bounds__(512, 2) void attend16_wide_kernel(const AttendArgs 
   total = sum_of_halves(total);
   const int64_t heads_rows = (int64_t)a.batch * a.kv_heads * a.rows, flat = (int64_t)bkv * a.rows + r;
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-  const float lse = total == 0.0f ? -INFINITY : (base + log2f(total)) * kLn2;
+  const float lse = total == 0.0f ? -INFINITY : (off + log2f(total)) * kLn2;
   if (h == 0) (a.splits > 1 ? a.part_lse[split * heads_rows + flat] : a.lse[flat]) = lse;
   float* part = a.splits > 1 ? a.part + (split * heads_rows + flat) * a.head : nullptr;
   T* out = (T*)a.out + dense_row_at(a, b, kv, r);

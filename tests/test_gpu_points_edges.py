@@ -58,6 +58,28 @@ def test_infinite_values_of_keys_that_count_in_16_bits(rows, dtype):
         check_infinite_values(rows, head, dtype)
 
 
+# ---- scores and weights at the ends of their range ---------------------------------------------------------------
+
+
+@pytest.mark.parametrize("batch,rows", [(256, 1), (256, 33), (512, 65)])
+def test_many_small_weights_of_f16(batch, rows):
+    """Eight keys of weight 1, one in the first tile of each wave of a block, and 2^20 of some 2^-26: f16's smallest number is 2^-24, and what they hold
+    together is 2^-9 of the result.  A weight may be off by half of f16's last place, or, with the largest at 2^7 or more, by 2^-32.  (The sequences are
+    as many as keep a block with all keys of one; they share their keys.)"""
+    import nnv_amd as nnv
+    n = 1 << 20
+    q = torch.ones(1, rows, 1, 8, dtype=F16, device="cuda").expand(batch, -1, -1, -1)
+    k = torch.full((1, n + 8, 1, 8), -18.02 / 8, dtype=F16, device="cuda")
+    v = torch.ones(1, n + 8, 1, 8, dtype=F16, device="cuda")
+    w = n * math.exp(float(k[0, 0, 0].double().sum()))
+    k[0, :256:32], v[0, :256:32] = 0.0, 0.0
+    o, lse = nnv.cross_attention(q, k.expand(batch, -1, -1, -1), v.expand(batch, -1, -1, -1), scale=1.0)
+    exact = w / (8 + w)
+    assert float((o.double() - exact).abs().max()) <= (n * 2.0 ** -32 + 2 * 2.0 ** -11 * w) / 8
+    # (a sum of n terms, as in the oracle's bounds)
+    assert float((lse.double() - math.log(8 + w)).abs().max()) <= (n + 32) * po.U32
+
+
 # ---- sizes ---------------------------------------------------------------------------------------------------
 
 
