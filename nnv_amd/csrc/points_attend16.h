@@ -48,6 +48,11 @@ __device__ __forceinline__ unsigned hide(unsigned at) {
   asm("" : "+v"(at));
   return at;
 }
+// a value as it is rounded where it stands, not taken into what uses it
+__device__ __forceinline__ float rounded(float x) {
+  asm("" : "+v"(x));
+  return x;
+}
 template <typename T, int DP>
 __device__ __forceinline__ unsigned rows_place(int lane) {
   return 2 * Rows16<T, DP>::at(lane & 31, lane >> 5);

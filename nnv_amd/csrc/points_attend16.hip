@@ -11,6 +11,22 @@ namespace {
 template <typename T>
 constexpr float kLift = std::is_same_v<T, f16_t> ? 7.0f : 0.0f;
 
+// Exponents are score * unit - off in one rounding, off a rounded score * unit: where a rounding is more than a fraction of an exponent, the two do not
+// fit together, and a weight may leave the range of its type.  From there on the products are rounded as off is (round_scores), and off is that of the largest,
+// not lower by kLift, which might be less than half a place.
+constexpr float kFar = 4194304.0f;   // 2^22: places of 1/2
+template <typename T>
+__device__ __forceinline__ float lowered(float top) {
+  return fabsf(top) > kFar ? top : top - kLift<T>;
+}
+template <int K>
+__device__ __forceinline__ void round_scores(float16_t (&s)[K], float unit) {
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[k][i] = rounded(s[k][i] * unit);
+}
+
 // FEW = false (heads of up to 64): four waves take 32 rows each and share tiles of 64 keys.  FEW = true (up to 64 rows, single tokens):
 // 32 rows for the block, whose 8 waves (4 for heads above 64: LDS) are groups that take tiles of 32 keys in turn; what the groups
 // found is joined at the end.  (attend_kernel is the f32 form.)
@@ -79,6 +95,7 @@ __global__ __launch_bounds__(FEW ? 64 * few_groups(DP) : 256, FEW ? 1 : 2) void 
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[d][i] = second[FEW ? d : 0][i] = 0.0f;
   float off = -INFINITY, total = 0.0f;   // off: of the exponents, in products times unit
+  bool far = false;                      // a row's is beyond kFar
 
   const T* kp = (const T*)a.k.p + b * a.k.b + kv * a.k.h;
   const T* vp = (const T*)a.v.p + b * a.v.b + kv * a.v.h;
@@ -144,9 +161,10 @@ __global__ __launch_bounds__(FEW ? 64 * few_groups(DP) : 256, FEW ? 1 : 2) void 
     float top = largest(s);
     top = max_of_halves(top) * unit;
     if (__any(top > off + (8.0f + kLift<T>))) {   // also: the first keys of a row that count
-      const float next = fmaxf(off, top - kLift<T>);
+      const float next = fmaxf(off, lowered<T>(top));
       const float fade = next == -INFINITY ? 1.0f : exp2_(off - next);
       off = next;
+      far = __any(fabsf(off) > kFar);
       total *= fade;
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
@@ -157,12 +175,17 @@ __global__ __launch_bounds__(FEW ? 64 * few_groups(DP) : 256, FEW ? 1 : 2) void 
         }
     }
     const float by = off == -INFINITY ? 0.0f : off;
+    float times = unit;
+    if (far) {
+      round_scores(s, unit);
+      times = 1.0f;
+    }
     float sum[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < KEYS / 32; ++k)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        s[k][i] = exp2_(s[k][i] * unit - by);
+        s[k][i] = exp2_(s[k][i] * times - by);
         sum[i & 1] += s[k][i];
       }
     total += sum[0] + sum[1];
@@ -311,6 +334,7 @@ __global__ __launch_bounds__(512, 2) void attend16_wide_kernel(const AttendArgs 
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
   float off = -INFINITY, total = 0.0f;
+  bool far = false;
   half8<T> p[4];
   uint64_t valid = 0;
   unsigned words[2];   // which keys of 32 tiles count, tile i in lane i
@@ -351,9 +375,10 @@ __global__ __launch_bounds__(512, 2) void attend16_wide_kernel(const AttendArgs 
     }
     const float top = max_of_halves(largest(s)) * unit;
     if (__any(top > off + (8.0f + kLift<T>))) {   // also: the first keys of a row that count
-      const float next = fmaxf(off, top - kLift<T>);
+      const float next = fmaxf(off, lowered<T>(top));
       const float fade = next == -INFINITY ? 1.0f : exp2_(off - next);
       off = next;
+      far = __any(fabsf(off) > kFar);
       total *= fade;
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
@@ -361,6 +386,11 @@ __global__ __launch_bounds__(512, 2) void attend16_wide_kernel(const AttendArgs 
         for (int i = 0; i < 16; ++i) acc[d][i] *= fade;
     }
     const float by = off == -INFINITY ? 0.0f : off;
+    float times = unit;
+    if (far) {
+      round_scores(s, unit);
+      times = 1.0f;
+    }
     float sum[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < 2; ++k)
@@ -368,7 +398,7 @@ __global__ __launch_bounds__(512, 2) void attend16_wide_kernel(const AttendArgs 
       for (int c = 0; c < 2; ++c) {
 #pragma unroll
         for (int i = 8 * c; i < 8 * c + 8; ++i) {
-          s[k][i] = exp2_(s[k][i] * unit - by);
+          s[k][i] = exp2_(s[k][i] * times - by);
           sum[i & 1] += s[k][i];
         }
         p[2 * k + c] = round8<T>(s[k], 8 * c);

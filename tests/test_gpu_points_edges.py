@@ -61,6 +61,28 @@ def test_infinite_values_of_keys_that_count_in_16_bits(rows, dtype):
 # ---- scores and weights at the ends of their range ---------------------------------------------------------------
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, F32], ids=["f16", "bf16", "f32"])
+@pytest.mark.parametrize("head", [64, 128])
+def test_scores_beyond_the_integers_of_f32(head, dtype):
+    """Scores of some 2^28 to 2^32, whose roundings are larger than the distance of any two exponents: the key with the largest score takes all."""
+    import nnv_amd as nnv
+    for rows in (1, 20, 70, 130):
+        g = gen(rows)
+        q, k, v = make(g, 2, rows, 300, 2, 1, head, dtype)
+        size = (1 + torch.rand(2, rows, 2, 1, generator=g, device="cuda") * 3) * 4000
+        q = size.expand(-1, -1, -1, head).to(dtype)
+        order = torch.stack([torch.randperm(300, generator=g, device="cuda") for _ in range(2)])
+        k = (8000.0 + 16 * order)[:, :, None, None].expand(-1, -1, 1, head).to(dtype) * (1 if dtype != BF16 else 1)
+        if dtype == BF16:   # fewer different numbers: the largest one alone
+            k = torch.where(order[:, :, None, None] == 299, 16000.0, 8000.0).expand(-1, -1, 1, head).to(dtype)
+        o, lse = nnv.cross_attention(q, k, v)
+        best = order.argmax(1)
+        expected = torch.stack([v[i, best[i]] for i in range(2)])[:, None].expand(2, rows, 2, head)
+        assert torch.equal(o, expected), "%d rows" % rows
+        exact = (q.double().permute(0, 2, 1, 3)[..., 0] * torch.stack([k[i, best[i], 0, 0] for i in range(2)]).double()[:, None, None]) * head ** 0.5
+        assert float(((lse - exact) / exact).abs().max()) <= (head + 8) * po.U32
+
+
 @pytest.mark.parametrize("batch,rows", [(256, 1), (256, 33), (512, 65)])
 def test_many_small_weights_of_f16(batch, rows):
     """Eight keys of weight 1, one in the first tile of each wave of a block, and 2^20 of some 2^-26: f16's smallest number is 2^-24, and what they hold
