@@ -83,8 +83,8 @@ __global__ __launch_bounds__(256, DP <= 96 || sizeof(T) == 2 ? 2 : 1) void atten
   for (int t = t0; t < t1; ++t) {
     __syncthreads();
     auto counting = [](int word) { return word != 0; };
-    k_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP, PIECES>(ks, j, d, f); }, words, counting, a.head, threadIdx.x);
-    v_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP, PIECES>(vs, j, d, f); }, words, counting, a.head, threadIdx.x);
+    store_tile<DP, PIECES>(k_next, ks, words, counting, a.head, threadIdx.x);
+    store_tile<DP, PIECES>(v_next, vs, words, counting, a.head, threadIdx.x);
     const uint32_t valid = (uint32_t)__ballot(counts != 0) >> (4 * h);
     __syncthreads();
     if (t + 1 < t1) fetch(t + 1);

@@ -63,11 +63,11 @@ __device__ __forceinline__ float offset_of(float lse) { return lse == -INFINITY 
 
 // Above heads of 64 the pieces of a wave's gradients of o lie in LDS: in registers they would be one set too many, and what is asked for
 // ahead would be moved to the accumulation registers, and waited for, as soon as it is asked for (4 x 512 x 512, 8 heads of 128: 156 us, else 171; heads of
-// 80 the same).
+// 80 the same).  In 16 bits heads of up to 96 alone: two waves a SIMD would spill 28 registers (3 x 2304 x 302, 48 heads of 80, 12 for keys, f16: 687 us, else 721).
 template <typename T, int DP, bool FOUR>
 __global__ __launch_bounds__(256, DP <= (sizeof(T) == 4 ? 64 : 96) ? 2 : 1) void query_grad_kernel(const AttendArgs a) {
   constexpr int R = kWaveRows, PIECES = kPieces<T>;
-  constexpr bool PARKED = DP > 64 && PIECES == 3;
+  constexpr bool PARKED = DP > 64 && (PIECES == 3 || DP == 96);
   __shared__ __attribute__((aligned(1024))) bf16_t ks[PIECES * R * DP], vs[PIECES * R * DP];
   __shared__ piece8 parked[PARKED ? 4 : 1][PARKED ? PIECES * (DP / 16) : 1][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
@@ -111,8 +111,8 @@ __global__ __launch_bounds__(256, DP <= (sizeof(T) == 4 ? 64 : 96) ? 2 : 1) void
   for (int t = t0; t < t1; ++t) {
     __syncthreads();
     auto counting = [](int word) { return word != 0; };
-    k_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP, PIECES>(ks, j, d, f); }, words, counting, a.head, threadIdx.x);
-    v_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP, PIECES>(vs, j, d, f); }, words, counting, a.head, threadIdx.x);
+    store_tile<DP, PIECES>(k_next, ks, words, counting, a.head, threadIdx.x);
+    store_tile<DP, PIECES>(v_next, vs, words, counting, a.head, threadIdx.x);
     const uint32_t valid = (uint32_t)__ballot(counts != 0) >> (4 * h);
     __syncthreads();
     if (t + 1 < t1) fetch(t + 1);
@@ -194,8 +194,8 @@ __global__ __launch_bounds__(256, DP <= (sizeof(T) == 4 ? 32 : 64) ? 2 : 1) void
   for (int t = t0; t < t1; ++t) {
     __syncthreads();
     auto counting = [](int word) { return word != kNone; };
-    q_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP, PIECES>(qs, j, d, f); }, words, counting, a.head, threadIdx.x);
-    g_next.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP, PIECES>(gs, j, d, f); }, words, counting, a.head, threadIdx.x);
+    store_tile<DP, PIECES>(q_next, qs, words, counting, a.head, threadIdx.x);
+    store_tile<DP, PIECES>(g_next, gs, words, counting, a.head, threadIdx.x);
     if (threadIdx.x < R) {
       offsets[threadIdx.x] = offset_of(next_lse);
       deltas[threadIdx.x] = next_lse == -INFINITY ? 0.0f : next_delta;

@@ -1,9 +1,10 @@
 // f32 products on the bf16 matrix instructions.  Cut into three pieces of 8 significant bits, an f32 is exactly
-//   x = x0 + x1 + x2,   x0 = the upper 16 bits of x, x1 = those of x - x0, x2 = the rest,
-// each a bf16.  Of the nine products of two such numbers the six largest are formed, exactly, and added up in f32; the three left out are
-// below 2^-24 of the result, where an f32 product rounds as well.  Six products of 32x32x16 take 192 cycles; the f32 instructions
-// (32x32x2) take 512 for the same.  (An infinity's products with pieces of zero are NaN: where a key or a query that counts holds one, so may be
-// the results that would be infinite.)
+//   x = x0 + x1 + x2,   x0 = x rounded to bf16, x1 = x - x0 rounded to bf16, x2 = the rest (8 bits, by then),
+// each a bf16, and a piece no more than 2^-9 of the one before.  Of the nine products of two such numbers the six largest are formed, exactly, and
+// added up in f32; the three left out are below 2^-25 of the result, of either sign, where an f32 product's rounding is up to 2^-24.  (Cut off instead of
+// rounded, pieces are 2^-7 of the one before and have its sign: up to 2^-21 is left out, 0.7 of 2^-24 on the mean, always towards zero.)  Six products of
+// 32x32x16 take 192 cycles; the f32 instructions (32x32x2) take 512 for the same.  (An infinity's products with pieces of zero are NaN: where a key, a
+// query or a value that counts holds one, so may be the results that would be infinite.)
 //
 // Numbers of 16 bits have two pieces (a bf16 one, an f16 two, of 8 and 3 bits): four products are all of theirs.  Two pieces of a softmax's
 // weight, 16 bits, are five more than the result keeps: three products with those.  (The gradients of 3 x 2304 x 302, 48 heads of 80, 12 for keys, in f16: 786 us;
@@ -21,12 +22,45 @@ __device__ __forceinline__ unsigned upper_halves(float a, float b) {   // of a i
   return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, b), __builtin_bit_cast(unsigned, a), 0x07060302);
 }
 __device__ __forceinline__ float cut(float x) { return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, x) & 0xffff0000u); }
-// The pieces of two numbers, each piece of both in a word.  (An infinity's rest is zero, not inf - inf.)
+__device__ __forceinline__ unsigned rounded_halves(float a, float b) {   // the same, to nearest
+  typedef bf16_t bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 r = {(bf16_t)a, (bf16_t)b};
+  return __builtin_bit_cast(unsigned, r);
+}
+__device__ __forceinline__ float lower_half(unsigned w) { return __builtin_bit_cast(float, w << 16); }
+__device__ __forceinline__ float upper_half(unsigned w) { return __builtin_bit_cast(float, w & 0xffff0000u); }
+// The pieces of two numbers, each piece of both in a word.
 __device__ __forceinline__ void cut_pair(float a, float b, unsigned (&w)[3]) {
-  w[0] = upper_halves(a, b);
-  const float a1 = fabsf(a) < INFINITY ? a - cut(a) : 0.0f, b1 = fabsf(b) < INFINITY ? b - cut(b) : 0.0f;
+  w[0] = rounded_halves(a, b);
+  const float a1 = a - lower_half(w[0]), b1 = b - upper_half(w[0]);
+  w[1] = rounded_halves(a1, b1);
+  w[2] = upper_halves(a1 - lower_half(w[1]), b1 - upper_half(w[1]));
+}
+// The same for numbers that bf16 would round to infinity, or that are infinite (their rest is zero, not inf - inf): the first piece cut off.
+constexpr float kRoundsUp = 3.396177e38f;   // below the largest bf16 and half of its last place
+__device__ __forceinline__ void cut_large(float a, float b, unsigned (&w)[3]) {
+  const bool fa = fabsf(a) < INFINITY, fb = fabsf(b) < INFINITY;
+  w[0] = rounded_halves(fa ? cut(a) : a, fb ? cut(b) : b);
+  const float a1 = fa ? a - cut(a) : 0.0f, b1 = fb ? b - cut(b) : 0.0f;
   w[1] = upper_halves(a1, b1);
   w[2] = upper_halves(a1 - cut(a1), b1 - cut(b1));
+}
+// max(x, |a|, |b|); what is no number is left out
+__device__ __forceinline__ float max_of_sizes(float x, float a, float b) {
+  asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(x) : "v"(a), "v"(b));
+  return x;
+}
+// LARGE: with cut_large.  What takes many numbers cuts them the quick way, finds their largest size, and where it is kRoundsUp or more, again the other way: a way
+// chosen number by number is a branch that nothing is moved across (the gradients of 4 x 512 x 512, 8 heads of 128, 160 us instead of 146).
+template <bool LARGE>
+__device__ __forceinline__ void cut_four(const float (&f)[4], unsigned (&a)[3], unsigned (&b)[3]) {
+  if constexpr (LARGE) {
+    cut_large(f[0], f[1], a);
+    cut_large(f[2], f[3], b);
+  } else {
+    cut_pair(f[0], f[1], a);
+    cut_pair(f[2], f[3], b);
+  }
 }
 
 // Tiles of 32 rows in planes, a Rows16 tile for each piece.
@@ -35,11 +69,10 @@ struct Planes {
   static constexpr int VALUES = 32 * DP, BYTES = 2 * VALUES;   // of one plane
 };
 // four values of row j, from d on, into a tile's planes
-template <int DP, int PIECES>
+template <int DP, int PIECES, bool LARGE>
 __device__ __forceinline__ void store_pieces(bf16_t* planes, int j, int d, const float (&f)[4]) {
   unsigned a[3], b[3];
-  cut_pair(f[0], f[1], a);
-  cut_pair(f[2], f[3], b);
+  cut_four<LARGE>(f, a, b);
   bf16_t* to = planes + Rows16<bf16_t, DP>::at(j, d / 8) + d % 8;
 #pragma unroll
   for (int k = 0; k < PIECES; ++k) {
@@ -47,40 +80,59 @@ __device__ __forceinline__ void store_pieces(bf16_t* planes, int j, int d, const
     __builtin_memcpy(to + k * Planes<DP>::VALUES, w, 8);
   }
 }
+// A thread's share of a tile (RowsAhead) into the tile's planes.
+template <int DP, int PIECES, class Ahead, class Counts>
+__device__ __forceinline__ void store_tile(const Ahead& ahead, bf16_t* planes, const typename Ahead::Words& words, Counts counts, int head, int tid) {
+  float top = 0.0f;
+  ahead.store(
+      [&](int j, int d, const float(&f)[4]) {
+        top = max_of_sizes(max_of_sizes(top, f[0], f[1]), f[2], f[3]);
+        store_pieces<DP, PIECES, false>(planes, j, d, f);
+      },
+      words, counts, head, tid);
+  if (__any(top >= kRoundsUp))
+    ahead.store([&](int j, int d, const float(&f)[4]) { store_pieces<DP, PIECES, true>(planes, j, d, f); }, words, counts, head, tid);
+}
 
 // The operands of a lane's row (values 16 c + 8 h .. + 7), in pieces.
 template <int DP, int PIECES>
 struct RowPieces {
   piece8 f[PIECES][DP / 16];
-  template <typename T>
-  __device__ __forceinline__ void load(const T* row, int h, int head, bool there) {
+  template <bool LARGE, typename T>
+  __device__ __forceinline__ float cut_row(const T* row, int h, int head, bool there) {   // returns the largest size
+    float top = 0.0f;
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
       const Four lo = load_four(row, 16 * c + 8 * h, head, there), hi = load_four(row, 16 * c + 8 * h + 4, head, there);
+      top = max_of_sizes(max_of_sizes(top, lo.v[0], lo.v[1]), lo.v[2], lo.v[3]);
+      top = max_of_sizes(max_of_sizes(top, hi.v[0], hi.v[1]), hi.v[2], hi.v[3]);
       unsigned w[4][3];
-      cut_pair(lo.v[0], lo.v[1], w[0]);
-      cut_pair(lo.v[2], lo.v[3], w[1]);
-      cut_pair(hi.v[0], hi.v[1], w[2]);
-      cut_pair(hi.v[2], hi.v[3], w[3]);
+      cut_four<LARGE>(lo.v, w[0], w[1]);
+      cut_four<LARGE>(hi.v, w[2], w[3]);
 #pragma unroll
       for (int k = 0; k < PIECES; ++k) {
         const unsigned v[4] = {w[0][k], w[1][k], w[2][k], w[3][k]};
         __builtin_memcpy(&f[k][c], v, 16);
       }
     }
+    return top;
+  }
+  template <typename T>
+  __device__ __forceinline__ void load(const T* row, int h, int head, bool there) {
+    if (__any(cut_row<false>(row, h, head, there) >= kRoundsUp)) cut_row<true>(row, h, head, there);
   }
 };
 
-// The products of two numbers in pieces: the small ones into `rest`, so that they are added up among themselves first.  ALL: two
-// pieces of either are the whole numbers, and the smallest product counts, too.
+// The products of two numbers in pieces: the small ones into `rest`, or first, so that they are added up among themselves (and a number times one is that
+// number).  ALL: two pieces of either are the whole numbers, and the smallest product counts, too.
 template <int PIECES, bool ALL>
 __device__ __forceinline__ void multiply(const piece8 (&x)[PIECES], const piece8 (&f)[PIECES], float16_t& s, float16_t& rest) {
   if constexpr (PIECES == 3) rest = Half8<bf16_t>::mfma(x[2], f[0], rest);
-  s = Half8<bf16_t>::mfma(x[0], f[0], s);
   if constexpr (PIECES == 3) rest = Half8<bf16_t>::mfma(x[0], f[2], rest);
   if constexpr (PIECES == 3 || ALL) rest = Half8<bf16_t>::mfma(x[1], f[1], rest);
   rest = Half8<bf16_t>::mfma(x[1], f[0], rest);
   rest = Half8<bf16_t>::mfma(x[0], f[1], rest);
+  s = Half8<bf16_t>::mfma(x[0], f[0], s);
 }
 
 // The product over the head of a tile's 32 rows with a row's pieces.  at: LDS address of the planes + rows_place; f(k, c): piece k.  What

@@ -58,6 +58,38 @@ def test_infinite_values_of_keys_that_count_in_16_bits(rows, dtype):
         check_infinite_values(rows, head, dtype)
 
 
+# ---- products of f32 -------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows", [1, 20, 4096])
+def test_products_of_f32_are_rounded_like_f32(rows):
+    """One key, heads of one value: lse is the product.  It is rounded as a product, times scale / ln 2 (a rounded number), in the sum with the
+    logarithm of one, and times ln 2 (a rounded number): five roundings of 2^-24 at most, and what the pieces leave out, below 2^-24."""
+    import nnv_amd as nnv
+    g = gen(rows)
+    q = 1 + torch.rand(64, rows, 1, 1, generator=g, device="cuda")
+    k = 1 + torch.rand(64, 1, 1, 1, generator=g, device="cuda")
+    q[32:], k[32:] = 1.0078124 - (q[32:] - 1) * 2.0 ** -18, 1.0078124    # the largest numbers behind seven zeros
+    q[:, ::2] *= -1
+    _, lse = nnv.cross_attention(q, k, torch.ones_like(k), scale=1.0)
+    exact = (q.double() * k.double())[:, :, 0, 0]
+    err = ((lse[:, 0] - exact) / exact.abs()).abs()
+    assert float(err.max()) <= 6 * po.U32, "%.2f" % (float(err.max()) / po.U32)
+
+
+def test_sums_of_f32_products_have_no_drift():
+    """The mean error of many products is a small part of one rounding, if those go either way: 2^18 of them, each within six, leave a
+    mean below 1/8 beside what the two rounded constants are off."""
+    import nnv_amd as nnv
+    g = gen(3)
+    q = 1 + torch.rand(64, 4096, 1, 1, generator=g, device="cuda")
+    k = 1 + torch.rand(64, 1, 1, 1, generator=g, device="cuda")
+    _, lse = nnv.cross_attention(q, k, torch.ones_like(k), scale=1.0)
+    f = lambda x: float(torch.tensor(x, dtype=F32))  # noqa: E731
+    exact = (q.double() * k.double())[:, :, 0, 0] * (f(1 / math.log(2)) * f(math.log(2)))
+    assert abs(float(((lse[:, 0] - exact) / exact).mean())) <= po.U32 / 8
+
+
 # ---- scores and weights at the ends of their range ---------------------------------------------------------------
 
 
