@@ -89,7 +89,7 @@ __global__ __launch_bounds__(256, DP <= 96 || sizeof(T) == 2 ? 2 : 1) void atten
     __syncthreads();
     if (t + 1 < t1) fetch(t + 1);
     if (idle) continue;
-    float16_t s = split_over_head<DP, PIECES>(hide(lds_addr_of(ks) + rows_at), [&](int k, int c) { return qf.f[k][c]; });
+    float16_t s = split_over_head<DP, PIECES, true>(hide(lds_addr_of(ks) + rows_at), [&](int k, int c) { return qf.f[k][c]; });
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] *= unit;
     const float fade = softmax_step(s, valid, m, total);
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(256, DP <= 96 || sizeof(T) == 2 ? 2 : 1) void atten
       for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[d][i] *= fade;
-    split_over_rows<DP, PIECES>(hide(lds_addr_of(vs) + columns_at), s, acc);
+    split_over_rows<DP, PIECES, true>(hide(lds_addr_of(vs) + columns_at), s, acc);
   }
   total = sum_of_halves(total);
   if (!row_here) return;

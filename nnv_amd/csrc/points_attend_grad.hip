@@ -117,8 +117,8 @@ __global__ __launch_bounds__(256, DP <= (sizeof(T) == 4 ? 64 : 96) ? 2 : 1) void
     __syncthreads();
     if (t + 1 < t1) fetch(t + 1);
     if (idle) continue;
-    float16_t s = split_over_head<DP, PIECES>(hide(lds_addr_of(ks) + rows_at), [&](int k, int c) { return qf.f[k][c]; });
-    const float16_t dp = split_over_head<DP, PIECES>(hide(lds_addr_of(vs) + rows_at), [&](int k, int c) {
+    float16_t s = split_over_head<DP, PIECES, false>(hide(lds_addr_of(ks) + rows_at), [&](int k, int c) { return qf.f[k][c]; });
+    const float16_t dp = split_over_head<DP, PIECES, false>(hide(lds_addr_of(vs) + rows_at), [&](int k, int c) {
       if constexpr (PARKED) return parked[wave][k * (DP / 16) + c][lane];
       else return gf.f[k][c];
     });
@@ -127,7 +127,7 @@ __global__ __launch_bounds__(256, DP <= (sizeof(T) == 4 ? 64 : 96) ? 2 : 1) void
       const float p = exp2_(s[i] * unit - offset);
       s[i] = (valid >> product_row(i, 0)) & 1 ? p * (dp[i] - delta) : 0.0f;
     }
-    split_over_rows<DP, PIECES>(hide(lds_addr_of(ks) + columns_at), s, dq);
+    split_over_rows<DP, PIECES, false>(hide(lds_addr_of(ks) + columns_at), s, dq);
   }
   if (!here) return;
   if (a.splits > 1)
@@ -203,17 +203,17 @@ __global__ __launch_bounds__(256, DP <= (sizeof(T) == 4 ? 32 : 64) ? 2 : 1) void
     __syncthreads();
     if (t + 1 < t1) fetch(t + 1);
     if (idle) continue;
-    float16_t s = split_over_head<DP, PIECES>(hide(lds_addr_of(qs) + rows_at), [&](int k, int c) { return kf.f[k][c]; });
+    float16_t s = split_over_head<DP, PIECES, false>(hide(lds_addr_of(qs) + rows_at), [&](int k, int c) { return kf.f[k][c]; });
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = exp2_(s[i] * unit - offsets[product_row(i, h)]);   // (of a key that does not count: dropped below)
-    split_over_rows<DP, PIECES>(hide(lds_addr_of(gs) + columns_at), s, dv);
-    const float16_t dp = split_over_head<DP, PIECES>(hide(lds_addr_of(gs) + rows_at), [&](int k, int c) {
+    split_over_rows<DP, PIECES, false>(hide(lds_addr_of(gs) + columns_at), s, dv);
+    const float16_t dp = split_over_head<DP, PIECES, false>(hide(lds_addr_of(gs) + rows_at), [&](int k, int c) {
       if constexpr (PARKED) return parked[wave][k * (DP / 16) + c][lane];
       else return vf.f[k][c];
     });
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] *= dp[i] - deltas[product_row(i, h)];
-    split_over_rows<DP, PIECES>(hide(lds_addr_of(qs) + columns_at), s, dk);
+    split_over_rows<DP, PIECES, false>(hide(lds_addr_of(qs) + columns_at), s, dk);
   }
   if (!here) return;
   if (!counts) {

@@ -3,8 +3,12 @@
 // each a bf16, and a piece no more than 2^-9 of the one before.  Of the nine products of two such numbers the six largest are formed, exactly, and
 // added up in f32; the three left out are below 2^-25 of the result, of either sign, where an f32 product's rounding is up to 2^-24.  (Cut off instead of
 // rounded, pieces are 2^-7 of the one before and have its sign: up to 2^-21 is left out, 0.7 of 2^-24 on the mean, always towards zero.)  Six products of
-// 32x32x16 take 192 cycles; the f32 instructions (32x32x2) take 512 for the same.  (An infinity's products with pieces of zero are NaN: where a key, a
-// query or a value that counts holds one, so may be the results that would be infinite.)
+// 32x32x16 take 192 cycles; the f32 instructions (32x32x2) take 512 for the same.
+//
+// An infinity's first piece is all of it, and its products with the other's small pieces are NaN where those are zero.  So a score that is not finite by its
+// first product is that; and the weights that meet values have their pieces cut off, so that none is below zero, and raised to the smallest number at
+// least (cut_weights).  (Asked for only where a tile holds an infinity: 120 us for 4 x 1024 x 1024, 16 heads of 64, always: 117.5.  The gradients of
+// what meets an infinity are infinite or NaN, with or without: there it would take 4 % of the time.)
 //
 // Numbers of 16 bits have two pieces (a bf16 one, an f16 two, of 8 and 3 bits): four products are all of theirs.  Two pieces of a softmax's
 // weight, 16 bits, are five more than the result keeps: three products with those.  (The gradients of 3 x 2304 x 302, 48 heads of 80, 12 for keys, in f16: 786 us;
@@ -61,6 +65,18 @@ __device__ __forceinline__ void cut_four(const float (&f)[4], unsigned (&a)[3], 
     cut_pair(f[0], f[1], a);
     cut_pair(f[2], f[3], b);
   }
+}
+
+// The pieces of two weights: above zero, except for the first one of a weight of zero.
+__device__ __forceinline__ void cut_weights(float a, float b, unsigned (&w)[3]) {
+  typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
+  const ushort2_t least = {0x0080, 0x0080};   // 2^-126
+  const float a1 = a - cut(a), b1 = b - cut(b);
+  w[0] = upper_halves(a, b);
+  w[1] = upper_halves(a1, b1);
+  w[2] = upper_halves(a1 - cut(a1), b1 - cut(b1));
+#pragma unroll
+  for (int k = 1; k < 3; ++k) w[k] = __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(ushort2_t, w[k]), least));
 }
 
 // Tiles of 32 rows in planes, a Rows16 tile for each piece.
@@ -136,8 +152,8 @@ __device__ __forceinline__ void multiply(const piece8 (&x)[PIECES], const piece8
 }
 
 // The product over the head of a tile's 32 rows with a row's pieces.  at: LDS address of the planes + rows_place; f(k, c): piece k.  What
-// one step multiplies is read while the step before it is multiplied (see OverHead).
-template <int DP, int PIECES, class F>
+// one step multiplies is read while the step before it is multiplied (see OverHead).  INFINITE: results that are infinite stay that.
+template <int DP, int PIECES, bool INFINITE, class F>
 __device__ __forceinline__ float16_t split_over_head(unsigned at, F f) {
   float16_t s, rest;
 #pragma unroll
@@ -159,11 +175,12 @@ __device__ __forceinline__ float16_t split_over_head(unsigned at, F f) {
     __builtin_amdgcn_sched_barrier(0);
   }
 #pragma unroll
-  for (int i = 0; i < 16; ++i) s[i] += rest[i];
+  for (int i = 0; i < 16; ++i) s[i] += !INFINITE || fabsf(s[i]) < INFINITY ? rest[i] : 0.0f;
   return s;
 }
-// acc[d] += the product over a tile's 32 rows with a product's registers p.  at: LDS address of the planes + columns_place.
-template <int DP, int PIECES>
+// acc[d] += the product over a tile's 32 rows with a product's registers p.  at: LDS address of the planes + columns_place.  WEIGHTS: none of p is below
+// zero, and infinite numbers of the tile are to stay infinite.
+template <int DP, int PIECES, bool WEIGHTS>
 __device__ __forceinline__ void split_over_rows(unsigned at, const float16_t& p, float16_t (&acc)[DP / 32]) {
   constexpr int N = 2 * (DP / 32);
   piece8 x[2][PIECES], f[2][PIECES];
@@ -177,7 +194,10 @@ __device__ __forceinline__ void split_over_rows(unsigned at, const float16_t& p,
   for (int c = 0; c < 2; ++c) {
     unsigned w[4][3];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) cut_pair(p[8 * c + 2 * i], p[8 * c + 2 * i + 1], w[i]);
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (WEIGHTS) cut_weights(p[8 * c + 2 * i], p[8 * c + 2 * i + 1], w[i]);
+      else cut_pair(p[8 * c + 2 * i], p[8 * c + 2 * i + 1], w[i]);
+    }
 #pragma unroll
     for (int k = 0; k < PIECES; ++k) {
       const unsigned v[4] = {w[0][k], w[1][k], w[2][k], w[3][k]};

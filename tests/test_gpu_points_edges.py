@@ -58,6 +58,35 @@ def test_infinite_values_of_keys_that_count_in_16_bits(rows, dtype):
         check_infinite_values(rows, head, dtype)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("rows", [1, 16, 17, 32, 33, 64, 65, 200])
+def test_infinite_values_where_products_are_cut(rows, dtype):
+    """The same in f32, and in 16 bits with rows that cannot be moved in 16-byte pieces."""
+    for head in (5, 40, 64, 99, 128) if dtype == F32 else (5, 99):
+        check_infinite_values(rows, head, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("rows", [1, 16, 17, 32, 33, 64, 65, 200])
+def test_scores_of_minus_infinity(rows, dtype):
+    """A key whose scores are all -inf, by an infinity in it or in the queries, has no weight."""
+    import nnv_amd as nnv
+    for head in (5, 40, 64, 128):
+        g = gen(rows + head)
+        q, k, v = make(g, 1, rows, 90, 2, 2, head, dtype)
+        q[..., 1] = -q[..., 1].abs() - 0.25
+        k[0, 31, :, 1] = math.inf
+        check_attend(q, k, v, backward=False, tag="%d rows, head %d, keys" % (rows, head))
+        q, k, v = make(g, 1, rows, 90, 2, 2, head, dtype)
+        q[0, rows // 2, :, 2] = math.inf
+        k[..., 2] = -k[..., 2].abs() - 0.25
+        k[0, 50, :, 2] = 0.0                      # inf * 0: no number
+        o, _ = nnv.cross_attention(q, k, v)
+        none = torch.zeros_like(o, dtype=torch.bool)
+        none[0, rows // 2] = True
+        assert torch.equal(torch.isnan(o), none)
+
+
 # ---- products of f32 -------------------------------------------------------------------------------------------
 
 
