@@ -94,8 +94,9 @@ __global__ __launch_bounds__(kThreads) void squares_kernel(const ClipTable t, in
   if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
 
-template <typename T>
-__device__ __forceinline__ void tile_scale(const T* p, T* out, int64_t n, float f) {
+// F: float, or double for a factor that f32 does not hold, or not in full.
+template <typename T, typename F>
+__device__ __forceinline__ void tile_scale(const T* p, T* out, int64_t n, F f) {
   constexpr int V = kVec<T>;
   Pack<T> in[kPacks];
 #pragma unroll
@@ -108,32 +109,40 @@ __device__ __forceinline__ void tile_scale(const T* p, T* out, int64_t n, float 
     const int64_t c = (int64_t)(j * kThreads + threadIdx.x) * V;
     Pack<T> scaled;
 #pragma unroll
-    for (int i = 0; i < V; ++i) scaled.set(i, from_f<T>(to_f(in[j][i]) * f));
+    for (int i = 0; i < V; ++i) scaled.set(i, from_f<T>((float)(to_f(in[j][i]) * f)));
     store_pack(out + c, scaled, n - c);
   }
 }
 
-// Tiles are taken from the last to the first: what the sums read last is still in the caches.
-__global__ __launch_bounds__(kThreads) void clip_kernel(const ClipTable t, int64_t tiles, const double* __restrict__ part, int parts,
-                                                        float threshold, float* __restrict__ norm, int scale) {
-  double s = 0;
-  for (int i = threadIdx.x; i < parts; i += kThreads) s += part[i];
-  s = block_sum(s);
-  const float n = (float)sqrt(s);
-  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = n;
-  if (!scale) return;
-  const float f = n > threshold ? threshold / n : 1.0f;
+template <typename F>
+__device__ __forceinline__ void scale_tiles(const ClipTable& t, int64_t tiles, F f) {
   for (int64_t back = blockIdx.x; back < tiles; back += gridDim.x) {
     const int64_t tile = tiles - 1 - back;
     const int k = tensor_of(t, tile);
     const int type = t.type[k];
     const int64_t per = (int64_t)kThreads * kPacks * (type == NNVHIP_TYPE_F32 ? 4 : 8);
     const int64_t at = (tile - (k ? t.tile_end[k - 1] : 0)) * per;
-    if (f == 1.0f && t.in[k] == t.out[k]) continue;   // nothing changes in place
+    if (f == 1 && t.in[k] == t.out[k]) continue;   // nothing changes in place
     if (type == NNVHIP_TYPE_F32) tile_scale((const float*)t.in[k] + at, (float*)t.out[k] + at, t.n[k] - at, f);
     else if (type == NNVHIP_TYPE_BF16) tile_scale((const bf16_t*)t.in[k] + at, (bf16_t*)t.out[k] + at, t.n[k] - at, f);
     else tile_scale((const f16_t*)t.in[k] + at, (f16_t*)t.out[k] + at, t.n[k] - at, f);
   }
+}
+
+// Tiles are taken from the last to the first: what the sums read last is still in the caches.  The norm of finite f32 gradients may be beyond f32: from some
+// way below that on the factor and its products are f64.
+__global__ __launch_bounds__(kThreads) void clip_kernel(const ClipTable t, int64_t tiles, const double* __restrict__ part, int parts,
+                                                        double threshold, float* __restrict__ norm, int scale) {
+  double s = 0;
+  for (int i = threadIdx.x; i < parts; i += kThreads) s += part[i];
+  s = block_sum(s);
+  const double whole = sqrt(s);
+  const float n = (float)whole, limit = (float)threshold;
+  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = n;
+  if (!scale) return;
+  const float f = n > limit ? limit / n : 1.0f;
+  if (whole > 1e30 || f < 1e-30f) scale_tiles(t, tiles, whole > threshold ? threshold / whole : 1.0);
+  else scale_tiles(t, tiles, f);
 }
 
 }  // namespace
@@ -192,12 +201,12 @@ int nnvhip_clip_gradients(nnvhip_ctx* ctx, int64_t count, const int32_t* type, c
   for (int64_t first = count > 0 ? (count - 1) / kTensors * kTensors : -1; first >= 0 && out; first -= kTensors) {
     const int64_t tiles = fill(first, t), blocks = std::min(tiles, kBlocks);
     if (blocks == 0) continue;
-    hipLaunchKernelGGL(clip_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, st, t, tiles, part, (int)parts, (float)threshold,
+    hipLaunchKernelGGL(clip_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, st, t, tiles, part, (int)parts, threshold,
                        told ? nullptr : norm, 1);
     told = true;
   }
   if (!told && norm)   // nothing to scale: the norm alone
-    hipLaunchKernelGGL(clip_kernel, dim3(1), dim3(kThreads), 0, st, t, (int64_t)0, part, (int)parts, (float)threshold, norm, 0);
+    hipLaunchKernelGGL(clip_kernel, dim3(1), dim3(kThreads), 0, st, t, (int64_t)0, part, (int)parts, threshold, norm, 0);
   NNV_HIP_TRY(hipGetLastError());
   return NNVHIP_OK;
 }

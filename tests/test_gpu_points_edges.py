@@ -195,3 +195,25 @@ def test_scales_that_are_no_numbers_and_heads_of_nothing_are_refused():
                 nnv.cross_attention_backward(q, q, q, q, o, lse, scale=scale)
         with pytest.raises(ValueError, match="1 to 128"):
             nnv.cross_attention(q[..., :0], q[..., :0], q[..., :0])
+
+
+# ---- clipping ------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_clip_a_norm_beyond_f32(dtype):
+    """Finite gradients whose norm f32 does not hold: it is told as infinite, and the gradients are scaled by what it is."""
+    import nnv_amd as nnv
+    grads = [torch.full((1000,), 2e38, device="cuda", dtype=dtype), torch.full((3, 50), -3e38, device="cuda", dtype=dtype),
+             torch.full((20,), 1e30, device="cuda", dtype=dtype)]
+    exact, n = po.clip(grads, 1.0)
+    assert n > 3.5e38
+    got, norm = nnv.clip_gradients(grads, 1.0)
+    assert float(norm) == math.inf
+    for a, e in zip(got, exact):
+        po.assert_within(a, e, 6 * po.U32 * e.abs(), "beyond f32")
+    got, _ = nnv.clip_gradients(grads, 1e39)
+    for a, e in zip(got, po.clip(grads, 1e39)[0]):
+        po.assert_within(a, e, 6 * po.U32 * e.abs(), "a threshold beyond f32")
+    got, _ = nnv.clip_gradients(grads, 1e300)
+    assert all(torch.equal(a, b) for a, b in zip(got, grads))
