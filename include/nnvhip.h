@@ -521,8 +521,8 @@ NNVHIP_API int nnvhip_cross_attention_backward(nnvhip_ctx* ctx, const nnvhip_att
 
 /* The norm over all `count` tensors, sqrt(sum of squares), to *norm (device memory; may be NULL), and the tensors scaled
  * to it: out[k] = in[k] * (norm > threshold ? threshold / norm : 1).  type, n (values), in, out: host arrays of `count` entries that are
- * read before the call returns; in and out hold device pointers.  A norm beyond f32 is told as infinite, and clipped as what it is.  out[k] may be in[k]; out NULL: the norm alone.  The
- * tensors must not overlap otherwise. */
+ * read before the call returns; in and out hold device pointers.  A norm beyond f32 is told as infinite, and clipped as what it is.  out[k] may be in[k]; out NULL: the norm alone.  An out[k]
+ * that overlaps another one, or a gradient otherwise, is refused. */
 NNVHIP_API int nnvhip_clip_gradients_workspace(int64_t count, int64_t* bytes);
 NNVHIP_API int nnvhip_clip_gradients(nnvhip_ctx* ctx, int64_t count, const int32_t* type, const int64_t* n, const void* const* in,
                           void* const* out, double threshold, float* norm, void* workspace, int64_t workspace_bytes,

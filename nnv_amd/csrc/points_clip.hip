@@ -16,6 +16,8 @@
 #include "points.h"
 
 #include <algorithm>
+#include <memory>
+#include <new>
 
 namespace nnvhip {
 namespace {
@@ -145,6 +147,32 @@ __global__ __launch_bounds__(kThreads) void clip_kernel(const ClipTable t, int64
   else scale_tiles(t, tiles, f);
 }
 
+// Whether a tensor that is written to overlaps another one, or the gradient of another one, or its own other than exactly: blocks would read what others
+// wrote.  1: it does, 0: none does, -1: no memory to find out.
+int outputs_overlap(int64_t count, const int32_t* type, const int64_t* n, const void* const* in, void* const* out) {
+  struct Span {
+    uintptr_t begin, end;
+    int64_t k;
+  };
+  const std::unique_ptr<Span[]> spans(new (std::nothrow) Span[count]);
+  if (!spans) return -1;
+  int64_t used = 0;
+  for (int64_t k = 0; k < count; ++k)
+    if (n[k] > 0) spans[used++] = {(uintptr_t)out[k], (uintptr_t)out[k] + (uintptr_t)n[k] * type_size(type[k]), k};
+  Span* const end = spans.get() + used;
+  std::sort(spans.get(), end, [](const Span& a, const Span& b) { return a.begin < b.begin; });
+  for (int64_t i = 1; i < used; ++i)
+    if (spans[i].begin < spans[i - 1].end) return 1;
+  for (int64_t k = 0; k < count; ++k) {
+    if (n[k] == 0) continue;
+    const uintptr_t from = (uintptr_t)in[k], to = from + (uintptr_t)n[k] * type_size(type[k]);
+    // (the spans are apart, so that their ends are in order, too)
+    for (const Span* s = std::upper_bound(spans.get(), end, from, [](uintptr_t x, const Span& b) { return x < b.end; }); s != end && s->begin < to; ++s)
+      if (s->k != k || s->begin != from) return 1;
+  }
+  return 0;
+}
+
 }  // namespace
 }  // namespace nnvhip
 
@@ -173,6 +201,9 @@ int nnvhip_clip_gradients(nnvhip_ctx* ctx, int64_t count, const int32_t* type, c
     if (n[k] < 0) NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_clip_gradients: tensor %lld: a negative size", (long long)k);
     if (n[k] > 0 && (!in[k] || (out && !out[k]))) NNV_FAIL(NNVHIP_ERR_ARG, "nnvhip_clip_gradients: tensor %lld: null pointer", (long long)k);
   }
+  const int overlap = out && count > 0 ? outputs_overlap(count, type, n, in, out) : 0;
+  if (overlap > 0) NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_clip_gradients: a tensor to write to overlaps another one, or another gradient");
+  if (overlap < 0) NNV_FAIL(NNVHIP_ERR_OOM, "nnvhip_clip_gradients: no host memory for %lld tensors", (long long)count);
   hipStream_t st = (hipStream_t)stream;
   double* part = static_cast<double*>(workspace);
   int64_t parts = 0;

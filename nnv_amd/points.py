@@ -266,7 +266,7 @@ def clip_gradients(gradients, threshold, out=None, ctx=None):
     out[k] = gradients[k] * (norm > threshold ? threshold / norm : 1), norm = sqrt(sum of all squares).
 
     Returns (the scaled tensors, norm as an f32 tensor of no dimensions); the norm stays on the GPU.  out: tensors of the same shapes
-    and types to write to, e.g. the gradients themselves; new ones if None.  A norm beyond f32 is told as infinite, and
+    and types to write to, e.g. the gradients themselves, none of which may share memory with another; new ones if None.  A norm beyond f32 is told as infinite, and
     clipped as what it is; one that is infinite, by an infinite gradient, gives zeros and NaNs, and one that is no number leaves the
     gradients as they are."""
     what = "clip_gradients"

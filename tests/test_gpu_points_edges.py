@@ -217,3 +217,30 @@ def test_clip_a_norm_beyond_f32(dtype):
         po.assert_within(a, e, 6 * po.U32 * e.abs(), "a threshold beyond f32")
     got, _ = nnv.clip_gradients(grads, 1e300)
     assert all(torch.equal(a, b) for a, b in zip(got, grads))
+
+def test_clip_refuses_outputs_that_share_memory():
+    """Blocks would read what others have written: the same tensor twice, two in the wrong order, one shifted against its gradient."""
+    import nnv_amd as nnv
+    g = gen(5)
+    store = rand(g, 100000)
+    a, b = store[:40000], store[50000:90000]
+    for grads, out in (([a, a], [a, a]), ([a, b], [b, a]), ([a], [store[1:40001]]), ([b], [store[49999:89999]]),
+                       ([a, b], [torch.empty_like(a), store[39999:79999]]), ([a, store[100:200]], [a, store[100:200]])):
+        with pytest.raises(ValueError, match="overlaps"):
+            nnv.clip_gradients(grads, 1.0, out=out)
+    before = store.clone()
+    exact, _ = po.clip([a, a, b, a[:0]], 1.0)
+    got, _ = nnv.clip_gradients([a, a, b, a[:0]], 1.0)      # read twice, written to new memory
+    assert torch.equal(store, before)
+    for x, e in zip(got, exact):
+        po.assert_within(x, e, 6 * po.U32 * e.abs(), "the same gradient twice")
+    exact, _ = po.clip([a, b, a[:0]], 1.0)
+    got, _ = nnv.clip_gradients([a, b, a[:0]], 1.0, out=[a, torch.empty_like(b), a[:0]])
+    for x, e in zip(got, exact):
+        po.assert_within(x, e, 6 * po.U32 * e.abs(), "in place and not")
+    # next to one another
+    half = [store[:50000], store[50000:]]
+    exact, _ = po.clip(half, 0.5)
+    got, _ = nnv.clip_gradients(half, 0.5, out=half)
+    for x, e in zip(got, exact):
+        po.assert_within(x, e, 6 * po.U32 * e.abs(), "neighbours")
