@@ -343,8 +343,24 @@ class Context:
         return n.value
 
 
+def _default_device() -> int:
+    return int(os.environ.get("NNVHIP_DEVICE", "0"))
+
+
 def default_context() -> Context:
     global _default_ctx
     if _default_ctx is None:
-        _default_ctx = Context(int(os.environ.get("NNVHIP_DEVICE", "0")))
+        _default_ctx = Context(_default_device())
     return _default_ctx
+
+
+_other_ctx = {}
+
+
+def context_on(device: int) -> Context:
+    """The default context if it is (or would be) that GPU's, else one that is made for the GPU once."""
+    if device == (_default_device() if _default_ctx is None else _default_ctx.device):
+        return default_context()
+    if device not in _other_ctx:
+        _other_ctx[device] = Context(device)
+    return _other_ctx[device]

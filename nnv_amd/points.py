@@ -6,7 +6,7 @@ points of the input box, the gradient of a specification's margin is followed ba
 ``nnv_amd.falsify``) or to the weights, and the step is bounded.  The reference's layers evaluate points as well (e.g.
 nn/layers/BatchNormalizationLayer.m:118-229); it has no gradients, and no counterpart of the two layers here in its reach path.
 
-All arguments and results are torch tensors on the context's GPU: f32, bf16 or f16.  A call is queued on torch's current
+All arguments and results are torch tensors on one GPU, that of the context if one is given: f32, bf16 or f16.  A call is queued on torch's current
 stream of that device, like torch's own operations, and returns without waiting; what it needs besides its results comes from torch's
 allocator.  The layers' sums and statistics are f32 (the gradient norm's squares f64) and each result is rounded once.
 """
@@ -18,7 +18,7 @@ import struct
 
 import torch
 
-from ._lib import check, default_context
+from ._lib import check, context_on, default_context
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _INT64 = C.c_int64
@@ -29,7 +29,7 @@ _stream_of = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getC
 
 
 def _enter(what, ctx, *tensors):
-    """(context, its library, stream) for tensors (or None) that have to be on that context's GPU."""
+    """(context, its library, stream) for tensors (or None) that have to be on that context's GPU; ctx None: the one of theirs."""
     try:
         index = tensors[0].get_device()
         for t in tensors:
@@ -39,7 +39,7 @@ def _enter(what, ctx, *tensors):
         raise TypeError("%s: expected torch tensors, got %s" % (what, ", ".join(type(t).__name__ for t in tensors))) from None
     if index < 0:
         raise ValueError("%s: the tensors must be on the GPU" % what)
-    ctx = ctx or default_context()
+    ctx = ctx or context_on(index)
     if index != ctx.device:
         raise ValueError("%s: the tensors are on GPU %d, the context is GPU %d's" % (what, index, ctx.device))
     return ctx, ctx.lib, _stream_of(index)
