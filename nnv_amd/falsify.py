@@ -83,6 +83,7 @@ def _bounds_within(lb, ub, like):
     return (low.to(like.device), high.to(like.device)) if bool((low <= high).all()) else None
 
 
+@torch.no_grad()
 def falsify_point(network, lb, ub, states, unsafe, starts=8, steps=50, step=0.1, seed=0, key_lengths=None, key_mask=None):
     """A point of the box [lb, ub] (tokens x channels) whose scores lie in the HalfSpace `unsafe` (G y <= g), as a host array of the
     states' type (f32 for bf16); None if none was found, which says nothing about there being none.
@@ -119,6 +120,7 @@ def falsify_point(network, lb, ub, states, unsafe, starts=8, steps=50, step=0.1,
         x = torch.minimum(torch.maximum(x - step * (ub - lb) * dx.sign(), lb), ub)
 
 
+@torch.no_grad()
 def train_step(network, x, states, labels, rate, threshold, key_lengths=None, key_mask=None):
     """One step of gradient descent on the cross entropy, the norm of all gradients bounded to `threshold`.  The network's parameters
     are updated in place; returns (loss, norm) as they were before the step, both left on the GPU."""

@@ -8,12 +8,14 @@ nn/layers/BatchNormalizationLayer.m:118-229); it has no gradients, and no counte
 
 All arguments and results are torch tensors on one GPU, that of the context if one is given: f32, bf16 or f16.  A call is queued on torch's current
 stream of that device, like torch's own operations, and returns without waiting; what it needs besides its results comes from torch's
-allocator.  The layers' sums and statistics are f32 (the gradient norm's squares f64) and each result is rounded once.
+allocator.  They are no part of torch's graph: where torch records gradients, tensors that
+require one are refused.  The layers' sums and statistics are f32 (the gradient norm's squares f64) and each result is rounded once.
 """
 from __future__ import annotations
 
 import ctypes as C
 import functools
+import operator
 import struct
 
 import torch
@@ -24,17 +26,27 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _INT64 = C.c_int64
 
 
+_requires_grad = operator.attrgetter("requires_grad")
 _stream_of = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _not_recorded(what):
+    return ValueError("%s: a tensor requires a gradient, which is not recorded here: call it under torch.no_grad() (the backward functions "
+                      "form the gradients)" % what)
 
 
 def _enter(what, ctx, *tensors):
     """(context, its library, stream) for tensors (or None) that have to be on that context's GPU; ctx None: the one of theirs."""
     try:
         index = tensors[0].get_device()
+        recording = torch.is_grad_enabled()
         for t in tensors:
-            if t is not None and t.get_device() != index:
-                raise ValueError("%s: the tensors must be on one GPU" % what)
+            if t is not None:
+                if t.get_device() != index:
+                    raise ValueError("%s: the tensors must be on one GPU" % what)
+                if recording and t.requires_grad:
+                    raise _not_recorded(what)
     except AttributeError:
         raise TypeError("%s: expected torch tensors, got %s" % (what, ", ".join(type(t).__name__ for t in tensors))) from None
     if index < 0:
@@ -292,6 +304,8 @@ def clip_gradients(gradients, threshold, out=None, ctx=None):
         if not all(isinstance(y, tensor) for y in result) or any(i != index for i in map(tensor.get_device, result)) or \
                 [y.dtype for y in result] != dtypes or not all(map(tensor.is_same_size, result, gradients)):
             raise ValueError("%s: out must have the shapes, types and device of the gradients" % what)
+    if torch.is_grad_enabled() and any(map(_requires_grad, gradients if fresh else gradients + result)):
+        raise _not_recorded(what)
     types = list(map(_TYPES.get, dtypes))
     if None in types:
         _type(what, gradients[types.index(None)])

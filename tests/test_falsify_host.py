@@ -15,7 +15,7 @@ class Linear:
         return x.sum(1) @ self.weights.t(), x.shape
 
     def backward(self, dscores, saved):
-        return (dscores @ self.weights)[:, None, :].expand(saved), []
+        return (dscores @ self.weights)[:, None, :].expand(saved), [dscores.sum(0)]
 
 
 def box64(lb, ub, dtype, weights, g, **kw):
@@ -85,3 +85,18 @@ def test_a_start_without_scores_hides_no_other():
     for limit in (1e4, -0.4):   # met by the first points, and by steps to the lower border
         found = nnv.falsify_point(Broken(torch.ones(1, 2)), np.zeros((1, 2)) - 0.25, np.ones((1, 2)), states, nnv.HalfSpace([[1.0]], [limit]))
         assert found is not None and found.sum() <= limit
+
+
+def test_searches_and_training_steps_record_no_gradients():
+    """They follow gradients of their own: weights that require one are no obstacle, and train_step may write to them."""
+    import nnv_amd as nnv
+
+    class Asked(Linear):
+        def forward(self, *args, **kw):
+            assert not torch.is_grad_enabled()
+            return super().forward(*args, **kw)
+
+    net = Asked(torch.ones(1, 2, requires_grad=True))
+    assert nnv.falsify_point(net, np.zeros((1, 2)), np.ones((1, 2)), torch.zeros(1, 1), nnv.HalfSpace([[1.0]], [0.5])) is not None
+    with pytest.raises(ValueError, match="on the GPU"):      # as far as a step goes on the host: to the clipping
+        nnv.train_step(net, torch.ones(2, 1, 2), None, torch.tensor([0, 0]), 0.1, 1.0)

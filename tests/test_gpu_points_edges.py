@@ -196,6 +196,23 @@ def test_scales_that_are_no_numbers_and_heads_of_nothing_are_refused():
         with pytest.raises(ValueError, match="1 to 128"):
             nnv.cross_attention(q[..., :0], q[..., :0], q[..., :0])
 
+def test_tensors_that_require_gradients_are_refused_unless_nobody_asks():
+    """The results are not part of torch's graph: where torch records one, a call says so."""
+    import nnv_amd as nnv
+    x, w = torch.randn(4, 8, device="cuda"), torch.ones(8, device="cuda", requires_grad=True)
+    q, k = torch.randn(1, 2, 2, 16, device="cuda"), torch.randn(1, 3, 2, 16, device="cuda", requires_grad=True)
+    with torch.no_grad():
+        y, mean, rstd = nnv.layer_norm(x, w)
+        o, lse = nnv.cross_attention(q, k, k)
+    for call in (lambda: nnv.layer_norm(x, w), lambda: nnv.layer_norm_backward(x, x, mean, rstd, w), lambda: nnv.cross_attention(q, k, k),
+                 lambda: nnv.cross_attention_backward(q, q, k, k, o, lse), lambda: nnv.clip_gradients([x, w], 1.0),
+                 lambda: nnv.clip_gradients([x], 1.0, out=[torch.empty_like(x).requires_grad_()])):
+        with pytest.raises(ValueError, match="no_grad"):
+            call()
+        with torch.no_grad():
+            call()
+    assert torch.equal(y, nnv.layer_norm(x, w.detach())[0]) and torch.equal(o, nnv.cross_attention(q, k.detach(), k.detach())[0])
+
 
 # ---- clipping ------------------------------------------------------------------------------------------------
 

@@ -3,6 +3,8 @@ import pytest
 
 
 class Tensor:
+    requires_grad = False
+
     def __init__(self, index):
         self.index = index
 
@@ -52,3 +54,17 @@ def test_the_default_contexts_gpu_is_the_environments(contexts, monkeypatch):
     monkeypatch.setenv("NNVHIP_DEVICE", "2")
     assert points._enter("call", None, Tensor(2))[0] is _lib.default_context() and contexts == [2]
     assert points._enter("call", None, Tensor(0))[0].device == 0
+
+
+def test_gradients_that_nobody_records_are_not_lost_silently(contexts):
+    from nnv_amd import points
+    torch = pytest.importorskip("torch")
+
+    class Learnt(Tensor):
+        requires_grad = True
+
+    with pytest.raises(ValueError, match="no_grad"):
+        points._enter("call", None, Tensor(0), None, Learnt(0))
+    with torch.no_grad():
+        assert points._enter("call", None, Tensor(0), None, Learnt(0))[0].device == 0
+    assert points._enter("call", None, Tensor(0), None, Tensor(0))[0].device == 0
