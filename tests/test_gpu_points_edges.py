@@ -261,3 +261,64 @@ def test_clip_refuses_outputs_that_share_memory():
     got, _ = nnv.clip_gradients(half, 0.5, out=half)
     for x, e in zip(got, exact):
         po.assert_within(x, e, 6 * po.U32 * e.abs(), "neighbours")
+
+
+# ---- the steady state of kernels that keep several tiles on their way ------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("head", [48, 72, 80, 96, 128])
+def test_many_tiles_of_keys(head, dtype):
+    """More tiles of keys than the forms for many rows hold at a time, and keys that end next to a tile's and a round's end."""
+    g = gen(head)
+    for rows in (65, 129, 257, 300):
+        for keys in (191, 192, 193, 255, 256, 257, 321, 515):
+            q, k, v = make(g, 2, rows, keys, 2, 1, head, dtype)
+            lengths = torch.tensor([keys, 1 + keys * 3 // 4], dtype=torch.int32, device="cuda")
+            check_attend(q, k, v, backward=keys in (257, 515), tag="%d x %d, head %d" % (rows, keys, head))
+            check_attend(q, k, v, key_lengths=lengths, backward=keys == 321, tag="%d x %d by length, head %d" % (rows, keys, head))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("batch,kv_heads,head", [(1, 2, 128), (1, 2, 32), (8, 32, 72), (8, 32, 128), (8, 64, 32)])
+def test_masks_over_many_tiles_of_keys(batch, kv_heads, head, dtype):
+    """2177 keys, more than a mask is read for at a time, in blocks that take them all (256 of heads above 64, 512 of others) and in blocks
+    that share them; whatever is left out is NaN."""
+    import nnv_amd as nnv
+    g = gen(batch + head)
+    keys = 2177
+    q, k, v = make(g, batch, 65, keys, kv_heads, kv_heads, head, dtype)
+    mask = torch.rand(batch, keys, generator=g, device="cuda") < 0.5
+    mask[0, :2100] = False
+    lengths = torch.randint(2050, keys + 1, (batch,), generator=g, device="cuda")
+    for kw in (dict(key_mask=mask), dict(key_mask=mask, key_lengths=lengths)):
+        counts = po.counting(q, k, kw.get("key_lengths"), mask)[:, :, None, None]
+        o, lse = nnv.cross_attention(q, torch.where(counts, k, math.nan), torch.where(counts, v, math.nan), **kw)
+        for i in range(0, batch, 7):     # (a sequence at a time: the oracle's 64-bit scores)
+            one = dict(key_mask=counts[i:i + 1, :, 0, 0])
+            (eo, el), (bo, bl) = po.attend(q[i:i + 1], k[i:i + 1], v[i:i + 1], **one), po.attend_bounds(q[i:i + 1], k[i:i + 1], v[i:i + 1], **one)
+            po.assert_within(lse[i:i + 1], el, bl, "lse")
+            po.assert_within(o[i:i + 1], eo, bo, "o")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("head", [32, 64, 80, 128])
+def test_masks_of_single_tokens_over_many_tiles_of_keys(head, dtype):
+    """9001 keys in blocks that take them all: eight waves of heads up to 64, four of others, read a mask for 32 tiles each at a time."""
+    import nnv_amd as nnv
+    g = gen(head)
+    batch, keys, heads = 16, 9001, 16
+    q = rand(g, batch, 1, heads, head, dtype=dtype)
+    kv = rand(g, batch, keys, 2, heads, head, dtype=dtype)
+    mask = torch.rand(batch, keys, generator=g, device="cuda") < 0.3
+    mask[1, :8900] = False
+    mask[2, 8000:] = False
+    clean = kv.clone()
+    kv[~mask] = math.nan
+    o, lse = nnv.cross_attention(q, kv[:, :, 0], kv[:, :, 1], key_mask=mask)
+    for i in (0, 1, 2, 15):
+        s = slice(i, i + 1)
+        args, kw = (q[s], clean[s, :, 0], clean[s, :, 1]), dict(key_mask=mask[s])
+        (eo, el), (bo, bl) = po.attend(*args, **kw), po.attend_bounds(*args, **kw)
+        po.assert_within(lse[s], el, bl, "lse")
+        po.assert_within(o[s], eo, bo, "o")
