@@ -474,7 +474,8 @@ NNVHIP_API int nnvhip_permute_rows(nnvhip_ctx* ctx, int64_t N, const int32_t* sr
 enum { NNVHIP_TYPE_F32 = 0, NNVHIP_TYPE_BF16 = 1, NNVHIP_TYPE_F16 = 2 };
 
 /* y = (x - mean) * rstd * scale + offset per row, rstd = 1 / sqrt(mean((x - mean)^2) + epsilon).  x: rows x size, row i at
- * x + i * x_stride elements; y dense; mean, rstd: rows.  scale, offset: size values of param_type (type, or f32), or NULL. */
+ * x + i * x_stride elements; y dense; mean, rstd: rows.  Below 2^31 rows, 2^23 of more than 8192 values.  scale, offset: size values of
+ * param_type (type, or f32), or NULL. */
 NNVHIP_API int nnvhip_layer_norm(nnvhip_ctx* ctx, int type, int param_type, int64_t rows, int64_t size, const void* x,
                       int64_t x_stride, const void* scale, const void* offset, double epsilon, void* y, float* mean,
                       float* rstd, void* stream);

@@ -496,7 +496,8 @@ int check_norm(const char* what, int type, int param_type, int64_t rows, int64_t
   if (!known_type(type) || !(param_type == type || param_type == NNVHIP_TYPE_F32))
     NNV_FAIL(NNVHIP_ERR_ARG, "%s: the values are f32, bf16 or f16, scale and offset of the same type or f32", what);
   if (rows < 0 || size < 1) NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: rows of at least one value are expected", what);
-  if (rows >= (int64_t(1) << 31)) NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: too many rows", what);
+  if (rows >= (int64_t(1) << (size > kLongest ? 23 : 31)))   // (a block of kThreads for each long row: a grid has fewer than 2^32 threads)
+    NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: too many rows", what);
   return NNVHIP_OK;
 }
 

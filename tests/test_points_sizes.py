@@ -44,3 +44,15 @@ def test_what_grids_and_indexes_do_not_hold():
     for kw in (dict(keys=(1 << 31) - 256), dict(batch=4096, keys=1 << 20), dict(batch=65535, queries=1024, heads=8)):
         forward, backward = workspaces(**kw)
         assert forward is not None and backward is None, kw
+
+
+def test_rows_of_layer_norm_that_a_grid_does_not_hold():
+    """Rows beyond a block's registers take a block of 512 threads each."""
+    from nnv_amd import _lib
+    lib, n = _lib.load(), C.c_int64()
+    for rows, size in (((1 << 23) - 1, 8193), (1 << 30, 8192), ((1 << 31) - 1, 64)):
+        _lib.check(lib.nnvhip_layer_norm_backward_workspace(1, rows, size, C.byref(n)))
+        assert n.value > 0
+    for rows, size in ((1 << 23, 8193), (1 << 31, 64)):
+        with pytest.raises(ValueError, match="too many rows"):
+            _lib.check(lib.nnvhip_layer_norm_backward_workspace(1, rows, size, C.byref(n)))
