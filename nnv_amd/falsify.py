@@ -103,7 +103,7 @@ def falsify_point(network, lb, ub, states, unsafe, starts=8, steps=50, step=0.1,
     x = lb + (ub - lb) * torch.rand((starts,) + lb.shape, generator=r, device=states.device, dtype=states.dtype)
     x[0] = lb / 2 + ub / 2
     x = torch.minimum(torch.maximum(x, lb), ub)   # (sums are rounded)
-    kept = states.expand((starts,) + states.shape)
+    kept = states.expand((starts,) + states.shape).contiguous()   # (one matrix of all tokens for the products with the weights)
     spread = None if key_lengths is None else key_lengths.expand(starts).contiguous()
     mask = None if key_mask is None else key_mask.expand(starts, -1)
     for k in range(steps + 1):
