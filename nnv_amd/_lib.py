@@ -359,7 +359,9 @@ _other_ctx = {}
 
 def context_on(device: int) -> Context:
     """The default context if it is (or would be) that GPU's, else one that is made for the GPU once."""
-    if device == (_default_device() if _default_ctx is None else _default_ctx.device):
+    if _default_ctx is not None and _default_ctx.device == device:
+        return _default_ctx
+    if _default_ctx is None and _default_device() == device:
         return default_context()
     if device not in _other_ctx:
         _other_ctx[device] = Context(device)

@@ -26,7 +26,8 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _INT64 = C.c_int64
 
 
-_requires_grad = operator.attrgetter("requires_grad")
+_requires_grad, _dtype = operator.attrgetter("requires_grad"), operator.attrgetter("dtype")
+_records_gradients = torch.is_grad_enabled
 _stream_of = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
@@ -36,19 +37,21 @@ def _not_recorded(what):
                       "form the gradients)" % what)
 
 
-def _enter(what, ctx, *tensors):
-    """(context, its library, stream) for tensors (or None) that have to be on that context's GPU; ctx None: the one of theirs."""
+def _enter(what, ctx, first, *others):
+    """(context, its library, stream) for tensors (others: or None) that have to be on that context's GPU; ctx None: the one of theirs."""
     try:
-        index = tensors[0].get_device()
-        recording = torch.is_grad_enabled()
-        for t in tensors:
+        index, recording = first.get_device(), _records_gradients()
+        asked = recording and first.requires_grad
+        for t in others:
             if t is not None:
                 if t.get_device() != index:
                     raise ValueError("%s: the tensors must be on one GPU" % what)
                 if recording and t.requires_grad:
-                    raise _not_recorded(what)
+                    asked = True
     except AttributeError:
-        raise TypeError("%s: expected torch tensors, got %s" % (what, ", ".join(type(t).__name__ for t in tensors))) from None
+        raise TypeError("%s: expected torch tensors, got %s" % (what, ", ".join(type(t).__name__ for t in (first, *others)))) from None
+    if asked:
+        raise _not_recorded(what)
     if index < 0:
         raise ValueError("%s: the tensors must be on the GPU" % what)
     ctx = ctx or context_on(index)
@@ -267,10 +270,15 @@ def cross_attention_backward(do, q, k, v, o, lse, key_lengths=None, key_mask=Non
 
 
 @functools.lru_cache(maxsize=64)
-def _clip_workspace(lib, count):
+def _clip_plan(lib, count):
+    """(bytes of the workspace, what packs the four arrays of a call, where the second one begins)."""
     n = _INT64()
     check(lib.nnvhip_clip_gradients_workspace(count, C.byref(n)))
-    return n.value
+    return n.value, struct.Struct("=%di%dx%dq%dQ%dQ" % (count, count % 2 * 4, count, count, count)).pack, (count + count % 2) * 4
+
+
+def _all_tensors(values):   # (a set of few members takes a fifth of the time of a loop)
+    return set(map(type, values)) == {torch.Tensor} or all(isinstance(v, torch.Tensor) for v in values)
 
 
 def clip_gradients(gradients, threshold, out=None, ctx=None):
@@ -291,20 +299,21 @@ def clip_gradients(gradients, threshold, out=None, ctx=None):
     ctx, lib, stream = _enter(what, ctx, gradients[0])
     device = gradients[0].device
     fresh = out is None
-    if not all(isinstance(g, torch.Tensor) for g in gradients):
+    tensor, index, strided = torch.Tensor, device.index, []
+    if not _all_tensors(gradients):
         raise TypeError("%s: expected torch tensors" % what)
     result = [torch.empty(g.shape, dtype=g.dtype, device=device) for g in gradients] if fresh else list(out)
     count = len(gradients)
     if len(result) != count:
         raise ValueError("%s: %d gradients and %d tensors to write to" % (what, count, len(result)))
-    tensor, index, dtypes, strided = torch.Tensor, device.index, [g.dtype for g in gradients], []
-    if any(i != index for i in map(tensor.get_device, gradients)):
+    dtypes = list(map(_dtype, gradients))
+    if set(map(tensor.get_device, gradients)) != {index}:
         raise ValueError("%s: the tensors must be on one GPU" % what)
     if not fresh:
-        if not all(isinstance(y, tensor) for y in result) or any(i != index for i in map(tensor.get_device, result)) or \
-                [y.dtype for y in result] != dtypes or not all(map(tensor.is_same_size, result, gradients)):
+        if not _all_tensors(result) or set(map(tensor.get_device, result)) != {index} or list(map(_dtype, result)) != dtypes or \
+                not all(map(tensor.is_same_size, result, gradients)):
             raise ValueError("%s: out must have the shapes, types and device of the gradients" % what)
-    if torch.is_grad_enabled() and any(map(_requires_grad, gradients if fresh else gradients + result)):
+    if _records_gradients() and (any(map(_requires_grad, gradients)) or not fresh and any(map(_requires_grad, result))):
         raise _not_recorded(what)
     types = list(map(_TYPES.get, dtypes))
     if None in types:
@@ -317,11 +326,10 @@ def clip_gradients(gradients, threshold, out=None, ctx=None):
         strided = [(y, t) for y, t in zip(result, to) if y is not t]
     sizes, source, target = map(tensor.numel, dense), map(tensor.data_ptr, dense), map(tensor.data_ptr, to)
     norm = torch.empty((), dtype=torch.float32, device=device)
-    need = _clip_workspace(lib, count)
+    need, pack, second = _clip_plan(lib, count)
     work = torch.empty(need, dtype=torch.uint8, device=device)
-    table = struct.pack("=%di%dx%dq%dQ%dQ" % (count, count % 2 * 4, count, count, count), *types, *sizes, *source, *target)
-    at = C.addressof(C.c_char.from_buffer(held := bytearray(table)))
-    longs = at + (count + count % 2) * 4
+    at = C.addressof(C.c_char.from_buffer(held := bytearray(pack(*types, *sizes, *source, *target))))
+    longs = at + second
     check(lib.nnvhip_clip_gradients(ctx.handle, count, at, longs, longs + 8 * count, longs + 16 * count, threshold, norm.data_ptr(),
                                     work.data_ptr(), need, stream))
     del held
