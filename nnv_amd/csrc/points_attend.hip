@@ -2,7 +2,7 @@
 //
 // The products are f32 ones, whatever the type of the tensors (points_attend_split.h): f32 tensors keep f32 results, and tensors of 16 bits, which
 // come here where their rows cannot be moved in 16-byte pieces, lose nothing but their final rounding.  That costs them: 2 x 4096 x 4096, 32 heads of 128
-// (8 for keys), in bf16 takes 1620 us here and 505 on attend16_wide_kernel; a single token, 2 x 65536 keys of 8 heads of 128, 240 and 94.
+// (8 for keys), in bf16 takes 1620 us here and 508 on attend16_wide_kernel; a single token, 2 x 65536 keys of 8 heads of 128, 240 and 95.
 #include "points_attend_split.h"
 
 #include <algorithm>
@@ -41,7 +41,7 @@ __device__ __forceinline__ float softmax_step(float16_t& s, uint32_t valid, floa
 // Where there are too few blocks for the chip, the keys are split over `splits` blocks, and join_kernel puts their results together.
 //
 // Bound by the vector units: cutting numbers into pieces and the softmax take as long as the six products.  4 x 1024 x 1024 in f32, 16 heads of 64:
-// 112 us, 153 TFLOP/s (a large f32 product of a library: 154); 8 heads of 128, one wave a SIMD: 133 us, 129 TFLOP/s.
+// 120 us, 143 TFLOP/s (a large f32 product of a library: 154), 4 of them for infinities; 8 heads of 128, one wave a SIMD: 132 us, 130 TFLOP/s.
 template <typename T, int DP, bool FOUR>
 __global__ __launch_bounds__(256, DP <= 96 || sizeof(T) == 2 ? 2 : 1) void attend_kernel(const AttendArgs a) {
   constexpr int R = kWaveRows, PIECES = kPieces<T>;
@@ -504,7 +504,7 @@ __global__ __launch_bounds__(256) void join_kernel(const AttendArgs a) {
 // Few are up to 64 rows of 16 bits, two tiles: 64 queries on 8 x 1500 keys, 16 heads of 64, take 17.5 us so and 22.3 as many; 96 take 25.5 and 25.0, with heads
 // of 128 on 4096 keys 91 and 64.  (f32: see attend_few_kernel.)
 //
-// Splits (see split_of): without, the single tokens on 2 x 65536 keys take 704 us instead of 94, 4 x 1024 x 1024 in f32 117 instead of 112.  Two tiles of keys are
+// Splits (see split_of): without, the single tokens on 2 x 65536 keys take 704 us instead of 94, 4 x 1024 x 1024 in f32 5 more.  Two tiles of keys are
 // the least for a split in f32: 96 queries on 477 keys, 8 heads of 80, take 20.7 us, with four 24.6.  The costs of a start and of a join in 16 bits
 // are higher, since a tile takes less: with 4 and 5 for 6 and 12, 2 x 538 x 1597, 2 heads of 128, takes 29 us instead of 25, 224 x 512, 16 of 32, 17 instead of 14.
 struct Cut {

@@ -7,7 +7,7 @@ namespace nnvhip {
 namespace {
 
 // The weights of the softmax are multiples of exp(score - the largest score): in f16 of 2^7, so that what is rounded to T keeps weights down to 2^-32 of the
-// largest (2^-25 without; a million keys of 2^-26 would be lost), and the largest, which the offset may lag behind by 2^8, stays in f16's range.
+// largest (2^-25 without; a million keys of 2^-26 would be lost), and the largest, which the offset may lag behind by 2^8, stays in f16's range.  (A weight that is rounded to zero gives NaN with an infinite value.)
 template <typename T>
 constexpr float kLift = std::is_same_v<T, f16_t> ? 7.0f : 0.0f;
 
@@ -43,7 +43,7 @@ __device__ __forceinline__ void round_scores(float16_t (&s)[K], float unit) {
 // FEW is bound by memory: single tokens on 2 x 65536 keys of 8 heads of 128 (32 of queries) take 94.5 us, 5.0 TB/s; on 16 x 1500 by length, 16 heads of 64, 18 us,
 // 4.2 TB/s.  8 groups, where LDS has room for them: 64 such rows on 8 sequences 17.5 us, with 4 groups 23.
 // The other form by its two waves a SIMD, which take products and softmax in turn: 8 x 448 x 1500 by length, 16 heads of 64, takes 36 us,
-// 480 TFLOP/s.  (Blocks of 64 rows take 52 us, two groups of four waves 36 to 41, three stages instead of four the same, attend16_wide_kernel 38;
+// 475 TFLOP/s.  (Blocks of 64 rows take 52 us, two groups of four waves 36 to 41, three stages instead of four the same, attend16_wide_kernel 38;
 // the next tile's scores formed among a tile's exponentials 10 % more.)
 constexpr int few_groups(int dp) { return dp > 64 ? 4 : 8; }
 template <typename T, int DP, bool FEW>
@@ -291,7 +291,7 @@ __global__ __launch_bounds__(FEW ? 64 * few_groups(DP) : 256, FEW ? 1 : 2) void 
 // Pair p of tiles in LDS is (keys p + 1, values p): what products p read, in halves 2 p and 2 p + 1.  There are four of them; a wave asks for
 // its share of pair p + 3 when it begins the softmax behind products p, with pair p - 1 out of use.
 //
-// 2 x 4096 x 4096, 32 heads of 128 (8 for keys): 503 us, 1090 TFLOP/s.  Bound by the power that the products may take: on zeros, where the card keeps its
+// 2 x 4096 x 4096, 32 heads of 128 (8 for keys): 508 us, 1080 TFLOP/s.  Bound by the power that the products may take: on zeros, where the card keeps its
 // clock, 405 us.  (Waves that do not take turns: 520 us; blocks of four waves 606.)
 template <typename T, int DP>
 __global__ __launch_bounds__(512, 2) void attend16_wide_kernel(const AttendArgs a) {

@@ -8,7 +8,7 @@
 // Bound by the vector units, which cut what the products take into pieces, and by blocks that are too few: 4 x 333 x 577, 12 heads of 80, in f32 take 157 us
 // (5 for D, 92 for dq in 144 blocks, 72 for dk and dv in 240), 47 TFLOP/s of
 // the five products that one kernel would need.  4 x 512 x 512, 8 heads of 128: 156 us.
-// In 16 bits, where points_attend16_grad.hip does not take the call (f16, or rows that cannot be moved in 16-byte pieces): 2 x 1024 x 1024, 16 heads of 64, 151 us;
+// In 16 bits, where points_attend16_grad.hip does not take the call (f16, or rows that cannot be moved in 16-byte pieces): 2 x 1024 x 1024, 16 heads of 64, 141 us;
 // 4 x 2048 x 2048 in bf16 732 us here, 286 there.
 #include "points_attend_split.h"
 
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(256, DP <= (sizeof(T) == 4 ? 64 : 96) ? 2 : 1) void
     store_fragments<T, DP>((T*)a.dq + dense_row_at(a, b, kv, r), dq, a.scale, h, a.head);
 }
 
-// (as above, with the wave's keys in registers and its values in LDS)
+// (as above, with the wave's keys in registers and its values in LDS; in f32 five registers of heads of 128 are spilled)
 template <typename T, int DP, bool FOUR>
 __global__ __launch_bounds__(256, DP <= (sizeof(T) == 4 ? 32 : 64) ? 2 : 1) void key_grad_kernel(const AttendArgs a) {
   constexpr int R = kWaveRows, PIECES = kPieces<T>;

@@ -1,8 +1,8 @@
 // f32 products on the bf16 matrix instructions.  Cut into three pieces of 8 significant bits, an f32 is exactly
 //   x = x0 + x1 + x2,   x0 = x rounded to bf16, x1 = x - x0 rounded to bf16, x2 = the rest (8 bits, by then),
-// each a bf16, and a piece no more than 2^-9 of the one before.  Of the nine products of two such numbers the six largest are formed, exactly, and
-// added up in f32; the three left out are below 2^-25 of the result, of either sign, where an f32 product's rounding is up to 2^-24.  (Cut off instead of
-// rounded, pieces are 2^-7 of the one before and have its sign: up to 2^-21 is left out, 0.7 of 2^-24 on the mean, always towards zero.)  Six products of
+// each a bf16, x1 no more than 2^-8 of x and x2 2^-17.  Of the nine products of two such numbers the six largest are formed, exactly, and
+// added up in f32; the three left out are below 2^-24 of the result, what an f32 product's rounding is, and of either sign.  (Cut off instead of
+// rounded, they are up to 2^-7 and 2^-15 and have its sign: up to 2^-21 is left out, 0.7 of 2^-24 on the mean, always towards zero.)  Six products of
 // 32x32x16 take 192 cycles; the f32 instructions (32x32x2) take 512 for the same.
 //
 // An infinity's first piece is all of it, and its products with the other's small pieces are NaN where those are zero.  So a score that is not finite by its
@@ -11,8 +11,8 @@
 // what meets an infinity are infinite or NaN, with or without: there it would take 4 % of the time.)
 //
 // Numbers of 16 bits have two pieces (a bf16 one, an f16 two, of 8 and 3 bits): four products are all of theirs.  Two pieces of a softmax's
-// weight, 16 bits, are five more than the result keeps: three products with those.  (The gradients of 3 x 2304 x 302, 48 heads of 80, 12 for keys, in f16: 786 us;
-// with three pieces 1214.)
+// weight, 16 bits, are five more than the result keeps: three products with those.  (The gradients of 3 x 2304 x 302, 48 heads of 80, 12 for keys, in f16: 690 us;
+// with three pieces half as much again.)
 #pragma once
 #include "points_attend16.h"
 
@@ -67,7 +67,8 @@ __device__ __forceinline__ void cut_four(const float (&f)[4], unsigned (&a)[3], 
   }
 }
 
-// The pieces of two weights: above zero, except for the first one of a weight of zero.
+// The pieces of two weights: above zero, except for the first one of a weight of zero.  (Cut off, they leave up to 1.5 2^-23 out of their products with
+// rounded pieces, still of either sign.)
 __device__ __forceinline__ void cut_weights(float a, float b, unsigned (&w)[3]) {
   typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
   const ushort2_t least = {0x0080, 0x0080};   // 2^-126

@@ -9,7 +9,9 @@ nn/layers/BatchNormalizationLayer.m:118-229); it has no gradients, and no counte
 All arguments and results are torch tensors on one GPU, that of the context if one is given: f32, bf16 or f16.  A call is queued on torch's current
 stream of that device, like torch's own operations, and returns without waiting; what it needs besides its results comes from torch's
 allocator.  They are no part of torch's graph: where torch records gradients, tensors that
-require one are refused.  The layers' sums and statistics are f32 (the gradient norm's squares f64) and each result is rounded once.
+require one are refused.  The layers' sums and statistics are f32 (the gradient norm's squares f64), and each
+result is rounded once; attention in 16 bits rounds the softmax's weights, and in bf16 the gradients of its scores, in front of the products that take
+them, and its backward pass takes the o that was rounded.
 """
 from __future__ import annotations
 
