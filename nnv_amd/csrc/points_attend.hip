@@ -558,6 +558,8 @@ int check_sizes(const char* what, const nnvhip_attention* d) {
     NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: the number of heads must be a multiple of the number of key/value heads", what);
   const int64_t most = (int64_t(1) << 31) - 256, group = d->heads / d->kv_heads;
   if (d->batch > 65535 || d->heads > 65535 || d->keys > most || d->queries > most / group) NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: too many rows", what);
+  // (at least so many blocks, first, for the sums by which splits are chosen)
+  if (d->batch * d->kv_heads * ceil_div(d->queries * group, 256) > kMostBlocks) NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: too many rows", what);
   for (const bool by16 : {false, true}) {
     const Cut c = cut_of(d->batch, d->kv_heads, d->queries * group, d->keys, d->head, by16);
     if (d->batch * d->kv_heads * c.row_tiles * c.splits > kMostBlocks) NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: too many rows", what);

@@ -321,6 +321,8 @@ int nnvhip_cross_attention_backward_workspace(const nnvhip_attention* d, int64_t
   const int64_t heads = d->batch * d->kv_heads;
   if (ceil_div(d->batch * d->heads * d->queries, 16) > 2 * kMostBlocks)   // delta_kernel's blocks, of 256 threads
     NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_cross_attention_backward: too many rows");
+  if (heads * ceil_div(d->keys, 256) > kMostBlocks)   // (at least so many blocks, as in the forward pass)
+    NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_cross_attention_backward: too many keys");
   *bytes = 0;   // whichever kernels the alignment of the tensors lets take the call
   for (const bool by16 : {false, true}) {
     const GradCut c = grad_cut(d->batch, d->kv_heads, d->queries * (d->heads / d->kv_heads), d->keys, d->head, by16);

@@ -38,10 +38,12 @@ def test_many_keys_for_few_rows(type):
 
 def test_what_grids_and_indexes_do_not_hold():
     for kw in (dict(keys=1 << 31), dict(queries=1 << 31), dict(queries=1 << 30, heads=2), dict(batch=65536), dict(heads=65536),
-               dict(batch=65535, heads=65535, kv_heads=65535), dict(batch=65535, queries=1 << 20)):
+               dict(batch=65535, heads=65535, kv_heads=65535), dict(batch=65535, queries=1 << 20),
+               dict(batch=65535, heads=65535, kv_heads=65535, queries=(1 << 31) - 256, keys=(1 << 31) - 256)):
         assert workspaces(**kw) == (None, None), kw
     # only the backward pass has a block for every tile of keys, and sixteen rows a block
-    for kw in (dict(keys=(1 << 31) - 256), dict(batch=4096, keys=1 << 20), dict(batch=65535, queries=1024, heads=8)):
+    for kw in (dict(keys=(1 << 31) - 256), dict(batch=4096, keys=1 << 20), dict(batch=65535, queries=1024, heads=8),
+               dict(batch=65535, heads=128, kv_heads=128, queries=0, keys=(1 << 31) - 256)):
         forward, backward = workspaces(**kw)
         assert forward is not None and backward is None, kw
 
