@@ -7,7 +7,7 @@
 //
 // An infinity's first piece is all of it, and its products with the other's small pieces are NaN where those are zero.  So a score that is not finite by its
 // first product is that; and the weights that meet values have their pieces cut off, so that none is below zero, and raised to the smallest number at
-// least (cut_weights).  (Asked for only where a tile holds an infinity: 120 us for 4 x 1024 x 1024, 16 heads of 64, always: 117.5.  The gradients of
+// least (cut_weights).  (Asked for only where a tile holds an infinity: 120 us for 4 x 1024 x 1024, 16 heads of 64, as always.  The gradients of
 // what meets an infinity are infinite or NaN, with or without: there it would take 4 % of the time.)
 //
 // Numbers of 16 bits have two pieces (a bf16 one, an f16 two, of 8 and 3 bits): four products are all of theirs.  Two pieces of a softmax's
