@@ -531,6 +531,54 @@ NNVHIP_API int nnvhip_clip_gradients(nnvhip_ctx* ctx, int64_t count, const int32
                           void* const* out, double threshold, float* norm, void* workspace, int64_t workspace_bytes,
                           void* stream);
 
+/* Group normalization with an activation; the channels come last.  x: batch x places x channels, sequence n, place p at
+ * x + n * x_stride[0] + p * x_stride[1] elements, dense channels in `groups` equal groups.  y dense; mean, rstd: batch x groups.
+ *   forward: z = (x - mean) * rstd * scale + offset with mean and rstd = 1 / sqrt(var + epsilon) of a sequence's group over all places,
+ *     y = z, max(z, 0) or z / (1 + exp(-z)).
+ *   backward: dx (dense) from dy, x and the mean and rstd that the forward call gave; dscale, doffset (sums over sequences and
+ *     places) in param_type, either may be NULL.  scale, offset: `channels` values of param_type (type, or f32), or NULL; the
+ *     activation's gradient needs the offset.  max's gradient is zero at zero.
+ * At least one place; channels below 2^24, sequences below 2^23, and of the blocks that sequences, chunks of up to 1024 channels
+ * and parts of the places make, fewer than 2^23. */
+enum { NNVHIP_ACTIVATION_NONE = 0, NNVHIP_ACTIVATION_RELU = 1, NNVHIP_ACTIVATION_SILU = 2 };
+typedef struct nnvhip_group_norm_args {
+  int64_t type, param_type, activation, batch, places, channels, groups;
+  double epsilon;
+  const void* x;
+  int64_t x_stride[2];
+  const void *scale, *offset;
+  void* y;
+  float *mean, *rstd;
+  const void* dy;
+  int64_t dy_stride[2];
+  void *dx, *dscale, *doffset;
+} nnvhip_group_norm_args;
+NNVHIP_API int nnvhip_group_norm_workspace(const nnvhip_group_norm_args* d, int64_t* bytes);
+NNVHIP_API int nnvhip_group_norm(nnvhip_ctx* ctx, const nnvhip_group_norm_args* d, void* workspace, int64_t workspace_bytes, void* stream);
+NNVHIP_API int nnvhip_group_norm_backward_workspace(const nnvhip_group_norm_args* d, int64_t* bytes);
+NNVHIP_API int nnvhip_group_norm_backward(nnvhip_ctx* ctx, const nnvhip_group_norm_args* d, void* workspace, int64_t workspace_bytes,
+                               void* stream);
+
+/* Rotary positions with several axes: pair i of each head's values (values 2 i and 2 i + 1 if interleaved, else i and pairs + i) is turned
+ * by position[axis[i]] * frequency[i] radians, or back by as much if inverse (the gradient); values behind the pairs stay.
+ * in[k]: batch x tokens x heads[k] x head with strides for batch, token and head and dense values, out[k] dense in that shape, neither
+ * overlapping another's out.  positions: batch x tokens x axes with strides.  frequency and axis: host arrays of `pairs`
+ * entries, read before the call returns.  Angles are formed in 64 bits. */
+enum { NNVHIP_POSITION_I32 = 0, NNVHIP_POSITION_I64 = 1, NNVHIP_POSITION_F32 = 2 };
+enum { NNVHIP_ROTATE_TENSORS = 4, NNVHIP_ROTATE_PAIRS = 256 };
+typedef struct nnvhip_rotate_args {
+  int64_t type, batch, tokens, head, tensors, pairs, axes, interleaved, inverse, position_type;
+  const void* positions;
+  int64_t position_stride[3];
+  const double* frequency;
+  const uint8_t* axis;
+  int64_t heads[NNVHIP_ROTATE_TENSORS];
+  const void* in[NNVHIP_ROTATE_TENSORS];
+  void* out[NNVHIP_ROTATE_TENSORS];
+  int64_t in_stride[NNVHIP_ROTATE_TENSORS][3];
+} nnvhip_rotate_args;
+NNVHIP_API int nnvhip_rotate_positions(nnvhip_ctx* ctx, const nnvhip_rotate_args* d, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -14,6 +14,7 @@ from .verify import HalfSpace, verify_specification  # noqa: F401
 # The operators on points work on torch tensors; torch is imported when one of them is first used.
 _POINTS = {"layer_norm": "points", "layer_norm_backward": "points", "cross_attention": "points", "cross_attention_backward": "points",
            "clip_gradients": "points", "LayerNormalizationLayer": "points", "CrossAttentionLayer": "points",
+           "group_norm": "images", "group_norm_backward": "images", "rotate_positions": "images",
            "CrossAttentionClassifier": "falsify", "falsify_point": "falsify", "train_step": "falsify"}
 
 

@@ -33,6 +33,8 @@ SYMBOLS = [
     "nnvhip_layer_norm", "nnvhip_layer_norm_backward_workspace", "nnvhip_layer_norm_backward",
     "nnvhip_cross_attention_workspace", "nnvhip_cross_attention", "nnvhip_cross_attention_backward_workspace",
     "nnvhip_cross_attention_backward", "nnvhip_clip_gradients_workspace", "nnvhip_clip_gradients",
+    "nnvhip_group_norm_workspace", "nnvhip_group_norm", "nnvhip_group_norm_backward_workspace", "nnvhip_group_norm_backward",
+    "nnvhip_rotate_positions",
 ]
 
 
@@ -148,6 +150,11 @@ def load():
         "nnvhip_cross_attention_backward": [p, p, p, i64, p],
         "nnvhip_clip_gradients_workspace": [i64, p],
         "nnvhip_clip_gradients": [p, i64, p, p, p, p, dbl, p, p, i64, p],
+        "nnvhip_group_norm_workspace": [p, p],
+        "nnvhip_group_norm": [p, p, p, i64, p],
+        "nnvhip_group_norm_backward_workspace": [p, p],
+        "nnvhip_group_norm_backward": [p, p, p, i64, p],
+        "nnvhip_rotate_positions": [p, p, p],
     }
     for name, args in sig.items():
         fn = getattr(lib, name)

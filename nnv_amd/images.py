@@ -1,0 +1,201 @@
+"""Operators on points that are images or videos: group normalization with an activation over features whose channels come last,
+rotary positions with several axes (rows and columns, time), and differential attention.
+
+They stand beside the operators of ``nnv_amd.points`` and follow the same rules: torch tensors on one GPU (f32, bf16 or f16), queued on torch's
+current stream of that device, no waiting, workspaces from torch's allocator, no part of torch's graph (tensors that require a
+gradient are refused where torch records one).  Sums and statistics are f32 or more, and each result is rounded once; what attention rounds on
+the way in 16 bits is said at ``differential_attention``.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import functools
+import struct
+
+import torch
+
+from ._lib import check, default_context
+from .points import _INT64, _enter, _ptr, _type
+
+# ---- group normalization ------------------------------------------------------------------------
+
+_ACTIVATIONS = {None: 0, "relu": 1, "silu": 2}
+_GROUP = struct.Struct("=7qdQ2qQQQQQQ2qQQQ")   # struct nnvhip_group_norm_args
+
+
+def _places(x):
+    """x (batch x ... x channels) with its places evenly spaced and its channels dense: (tensor, places, strides of batch and place);
+    copied where they are not."""
+    batch, channels = x.shape[0], x.shape[-1]
+    if x.is_contiguous():
+        places = x.numel() // (batch * channels) if batch else 1
+        return x, places, places * channels, channels
+    if x.stride(-1) == 1 or channels == 1:
+        try:
+            rows = x.view(batch, -1, channels) if x.numel() else None
+        except RuntimeError:
+            rows = None
+        if rows is not None:
+            return rows, rows.shape[1], rows.stride(0), rows.stride(1)
+    return _places(x.contiguous())
+
+
+def _group_params(what, x, groups, scale, offset, activation):
+    t = _type(what, x)
+    if x.dim() < 2:
+        raise ValueError("%s: x is batch x ... x channels" % what)
+    channels = x.shape[-1]
+    if not (isinstance(groups, int) and groups >= 1 and channels >= 1 and channels % groups == 0):
+        raise ValueError("%s: the channels (%d) must come in equal groups, not %s" % (what, channels, groups))
+    if 0 in x.shape[1:]:
+        raise ValueError("%s: at least one place is expected, not the shape %s" % (what, tuple(x.shape)))
+    act = _ACTIVATIONS.get(activation)
+    if act is None:
+        raise ValueError("%s: the activation is None, 'relu' or 'silu', not %r" % (what, activation))
+    w = t
+    for p in (scale, offset):
+        if p is not None:
+            if p.shape != (channels,):
+                raise ValueError("%s: scale and offset have one value per channel (%d), not the shape %s" % (what, channels, tuple(p.shape)))
+            w = _type(what, p)
+            if w not in (t, 0):
+                raise ValueError("%s: scale and offset have the type of the values, or float32" % what)
+    if scale is not None and offset is not None and scale.dtype != offset.dtype:
+        raise ValueError("%s: scale and offset must have the same type" % what)
+    return t, w, act
+
+
+@functools.lru_cache(maxsize=256)
+def _group_workspace(lib, backward, t, batch, places, channels, groups):
+    n = _INT64()
+    d = _GROUP.pack(t, t, 0, batch, places, channels, groups, 0.0, *[0] * 14)
+    check((lib.nnvhip_group_norm_backward_workspace if backward else lib.nnvhip_group_norm_workspace)(d, C.byref(n)))
+    return n.value
+
+
+def _dense(p):
+    return p if p is None or p.is_contiguous() else p.contiguous()
+
+
+def group_norm(x, groups, scale=None, offset=None, epsilon=1e-5, activation=None, ctx=None):
+    """y = act((x - mean) / sqrt(var + epsilon) * scale + offset), mean and var over all places and the channels of a group.
+
+    x: batch x ... x channels; the channels come last, in ``groups`` equal groups of consecutive ones.  activation: None, "relu" or
+    "silu" (z / (1 + exp(-z))).  scale and offset: vectors of x's type or f32, or None.
+    Returns (y, mean, rstd): y in x's shape and type, the statistics f32, batch x groups; group_norm_backward takes them."""
+    what = "group_norm"
+    ctx, lib, stream = _enter(what, ctx, x, scale, offset)
+    t, w, act = _group_params(what, x, groups, scale, offset, activation)
+    if not epsilon >= 0:
+        raise ValueError("group_norm: epsilon must not be negative")
+    batch, channels = x.shape[0], x.shape[-1]
+    scale, offset = _dense(scale), _dense(offset)
+    rows, places, xb, xp = _places(x)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    mean = x.new_empty((batch, groups), dtype=torch.float32)
+    rstd = torch.empty_like(mean)
+    need = _group_workspace(lib, False, t, batch, places, channels, groups)
+    work = x.new_empty((need,), dtype=torch.uint8) if need else None
+    d = _GROUP.pack(t, w, act, batch, places, channels, groups, epsilon, rows.data_ptr(), xb, xp, _ptr(scale) or 0, _ptr(offset) or 0,
+                    y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), 0, 0, 0, 0, 0, 0)
+    check(lib.nnvhip_group_norm(ctx.handle, d, _ptr(work), need, stream))
+    return y, mean, rstd
+
+
+def group_norm_backward(dy, x, mean, rstd, scale=None, offset=None, activation=None, ctx=None):
+    """The gradients of group_norm: (dx, dscale, doffset) from that of its result and its statistics (which say how many groups there are).
+
+    dx has x's type, dscale and doffset the type of scale or offset (x's if both are None).  The gradient of "relu" is zero at zero."""
+    what = "group_norm_backward"
+    ctx, lib, stream = _enter(what, ctx, x, dy, mean, rstd, scale, offset)
+    batch = x.shape[0] if x.dim() else 0
+    for s in (mean, rstd):
+        if s.dim() != 2 or s.shape != mean.shape or s.shape[0] != batch or s.dtype != torch.float32:
+            raise ValueError("%s: mean and rstd must be what group_norm returned" % what)
+    groups = mean.shape[1]
+    t, w, act = _group_params(what, x, groups, scale, offset, activation)
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError("%s: dy must have the shape and type of x" % what)
+    channels = x.shape[-1]
+    scale, offset, mean, rstd = _dense(scale), _dense(offset), _dense(mean), _dense(rstd)
+    rows, places, xb, xp = _places(x)
+    grows, _, gb, gp = _places(dy)
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+    like = scale if scale is not None else offset if offset is not None else x
+    dscale = like.new_empty((channels,))
+    doffset = torch.empty_like(dscale)
+    need = _group_workspace(lib, True, t, batch, places, channels, groups)
+    work = x.new_empty((need,), dtype=torch.uint8) if need else None
+    d = _GROUP.pack(t, w, act, batch, places, channels, groups, 0.0, rows.data_ptr(), xb, xp, _ptr(scale) or 0, _ptr(offset) or 0, 0,
+                    mean.data_ptr(), rstd.data_ptr(), grows.data_ptr(), gb, gp, dx.data_ptr(), dscale.data_ptr(), doffset.data_ptr())
+    check(lib.nnvhip_group_norm_backward(ctx.handle, d, _ptr(work), need, stream))
+    return dx, dscale, doffset
+
+
+# ---- rotary positions ---------------------------------------------------------------------------
+
+_ROTATE_TENSORS, _ROTATE_PAIRS = 4, 256
+_ROTATE = struct.Struct("=10qQ3qQQ4q4Q4Q12q")   # struct nnvhip_rotate_args
+_POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+
+
+@functools.lru_cache(maxsize=64)
+def _frequencies(sections, base, shared):
+    """(frequencies, axes) of the pairs, as arrays that the library reads."""
+    pairs = sum(sections)
+    values, axes = [], []
+    for axis, n in enumerate(sections):
+        for i in range(n):
+            values.append(base ** -((len(values) / pairs) if shared else (i / n)))
+            axes.append(axis)
+    return (C.c_double * pairs)(*values), (C.c_uint8 * pairs)(*axes)
+
+
+def rotate_positions(x, positions, sections, base=10000.0, shared=False, interleaved=False, inverse=False, ctx=None):
+    """x with its heads' values turned by their tokens' positions: rotary positions with several axes.
+
+    x: batch x tokens x heads x head, any strides, or a list of such tensors (queries and keys) whose heads may differ in number.
+    positions: tokens x axes, or batch x tokens x axes (i32, i64 or f32).  sections[a] pairs of a head's values are turned by axis a, one axis after
+    the other; what is behind 2 * sum(sections) values stays.  A pair is (i, i + sum(sections)), or neighbours (2 i, 2 i + 1) if interleaved.  Its angle is
+    position * base^-e with e = (its place in its section) / (pairs of the section), or, if shared, (its place among all pairs) / (all pairs).
+    inverse: turned back, which is the backward pass.
+
+    Returns new tensors, a list if x is one."""
+    what = "rotate_positions"
+    several = not isinstance(x, torch.Tensor)
+    tensors = list(x) if several else [x]
+    if not tensors:
+        raise ValueError("%s: at least one tensor is expected" % what)
+    ctx, lib, stream = _enter(what, ctx, tensors[0], *tensors[1:], positions)
+    sections = tuple(sections)
+    first = tensors[0]
+    t = _type(what, first)
+    if not sections or not all(isinstance(n, int) and n >= 0 for n in sections) or not 1 <= sum(sections) <= _ROTATE_PAIRS or len(sections) > 255:
+        raise ValueError("%s: sections are numbers of pairs, one per axis, %d together at most" % (what, _ROTATE_PAIRS))
+    if not 0 < base < float("inf"):
+        raise ValueError("%s: the base must be positive and finite" % what)
+    for y in tensors:
+        if y.dim() != 4 or y.dtype != first.dtype or y.shape[:2] != first.shape[:2] or y.shape[3] != first.shape[3]:
+            raise ValueError("%s: tensors are batch x tokens x heads x head, alike but for the number of heads" % what)
+    batch, tokens, _, head = first.shape
+    if head < 2 * sum(sections):
+        raise ValueError("%s: heads of %d values do not hold %d pairs" % (what, head, sum(sections)))
+    if positions.dtype not in _POSITIONS or positions.dim() not in (2, 3) or positions.shape[-2:] != (tokens, len(sections)) or \
+            (positions.dim() == 3 and positions.shape[0] != batch):
+        raise ValueError("%s: positions are (batch x) tokens x axes whole numbers or float32, not %s %s" %
+                         (what, positions.dtype, tuple(positions.shape)))
+    stride = positions.stride() if positions.dim() == 3 else (0, *positions.stride())
+    frequency, axis = _frequencies(sections, float(base), bool(shared))
+    done = []
+    for k in range(0, len(tensors), _ROTATE_TENSORS):
+        part = [y if y.stride(3) == 1 or head == 1 else y.contiguous() for y in tensors[k:k + _ROTATE_TENSORS]]
+        out = [torch.empty_like(y, memory_format=torch.contiguous_format) for y in part]
+        none = [0] * (_ROTATE_TENSORS - len(part))
+        strides = [s for y in part for s in y.stride()[:3]]
+        d = _ROTATE.pack(t, batch, tokens, head, len(part), sum(sections), len(sections), bool(interleaved), bool(inverse),
+                         _POSITIONS[positions.dtype], positions.data_ptr(), *stride, C.addressof(frequency), C.addressof(axis),
+                         *[y.shape[2] for y in part], *none, *[y.data_ptr() for y in part], *none, *[y.data_ptr() for y in out], *none,
+                         *strides, *[0] * (12 - len(strides)))
+        check(lib.nnvhip_rotate_positions(ctx.handle, d, stream))
+        done += out
+    return done if several else done[0]

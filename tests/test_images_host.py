@@ -1,0 +1,154 @@
+"""The operators on points that are images or videos as far as they go without a GPU: their refusals, their workspaces, and their
+plain forms in 64 bits (tests/images_oracle.py) against torch's own differentiation."""
+import ctypes as C
+import math
+import os
+
+import pytest
+import torch
+
+from tests import images_oracle as io
+
+LIB = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "nnv_amd", "libnnvhip.so")
+built = pytest.mark.skipif(not os.path.exists(LIB), reason="library not built (python -m nnv_amd.build)")
+
+
+class OnGpu(torch.Tensor):
+    """A host tensor that says it is on GPU 0, for what is checked before anything is launched."""
+
+    @staticmethod
+    def __new__(cls, t):
+        return t.as_subclass(cls)
+
+    def get_device(self):
+        return 0
+
+
+@pytest.fixture
+def no_gpu(monkeypatch):
+    """The operators' checks without a GPU: a context that has no library."""
+    from nnv_amd import images, points
+
+    class Context:
+        lib, handle, device = None, None, 0
+
+    context = Context()
+    monkeypatch.setattr(points, "context_on", lambda index: context)
+    monkeypatch.setattr(points, "_stream_of", lambda index: 0)
+    return images
+
+
+def refused(match, call, *args, error=ValueError, **kw):
+    with pytest.raises(error, match=match):
+        call(*args, **kw)
+
+
+def test_tensors_on_the_host_are_refused():
+    import nnv_amd as nnv
+    x = torch.zeros(2, 3, 4, 8)
+    refused("on the GPU", nnv.group_norm, x, 2)
+    refused("on the GPU", nnv.group_norm_backward, x, x, torch.zeros(2, 2), torch.zeros(2, 2))
+    refused("on the GPU", nnv.rotate_positions, x, torch.zeros(3, 1, dtype=torch.int32), [2])
+    refused("expected torch tensors", nnv.group_norm, 3.0, 2, error=TypeError)
+    refused("expected torch tensors", nnv.rotate_positions, [3.0], x, [2], error=TypeError)
+
+
+def test_refusals_of_group_norm(no_gpu):
+    x, w = OnGpu(torch.zeros(2, 3, 4, 8)), OnGpu(torch.zeros(8))
+    call = no_gpu.group_norm
+    for groups in (0, 3, -2, 2.0, None):
+        refused("equal groups", call, x, groups)
+    refused("batch x", call, OnGpu(torch.zeros(8)), 2)
+    refused("at least one place", call, OnGpu(torch.zeros(2, 0, 8)), 2)
+    refused("activation", call, x, 2, activation="tanh")
+    refused("activation", call, x, 2, activation=False)
+    refused("float32, bfloat16 or float16", call, OnGpu(torch.zeros(2, 3, 8, dtype=torch.float64)), 2)
+    refused("one value per channel", call, x, 2, OnGpu(torch.zeros(4)))
+    refused("type of the values", call, OnGpu(x.bfloat16()), 2, OnGpu(w.half()))
+    refused("same type", call, OnGpu(x.bfloat16()), 2, OnGpu(w.bfloat16()), w)
+    refused("epsilon", call, x, 2, epsilon=-1e-5)
+    refused("epsilon", call, x, 2, epsilon=math.nan)
+    refused("requires a gradient", call, x, 2, OnGpu(torch.zeros(8)).requires_grad_())
+    back, stats = no_gpu.group_norm_backward, OnGpu(torch.zeros(2, 4))
+    refused("shape and type of x", back, OnGpu(torch.zeros(2, 3, 4, 4)), x, stats, stats)
+    refused("shape and type of x", back, OnGpu(x.half()), x, stats, stats)
+    refused("what group_norm returned", back, x, x, stats, OnGpu(torch.zeros(2, 2)))
+    refused("what group_norm returned", back, x, x, OnGpu(torch.zeros(3, 4)), OnGpu(torch.zeros(3, 4)))
+    refused("what group_norm returned", back, x, x, OnGpu(stats.double()), OnGpu(stats.double()))
+    refused("equal groups", back, x, x, OnGpu(torch.zeros(2, 3)), OnGpu(torch.zeros(2, 3)))
+
+
+def test_refusals_of_rotary_positions(no_gpu):
+    x, at = OnGpu(torch.zeros(2, 5, 3, 8)), OnGpu(torch.zeros(5, 2, dtype=torch.int32))
+    call = no_gpu.rotate_positions
+    refused("at least one tensor", call, [], at, [2, 2])
+    for sections in ([], [0, 0], [-1, 3], [1.5, 2], [200, 57]):
+        refused("sections", call, x, at, sections)
+    refused("do not hold", call, x, at, [3, 2])
+    refused("base", call, x, at, [2, 2], base=0.0)
+    refused("base", call, x, at, [2, 2], base=math.inf)
+    refused("alike", call, OnGpu(torch.zeros(2, 5, 8)), at, [2, 2])
+    for other in (torch.zeros(2, 4, 3, 8), torch.zeros(2, 5, 3, 4), torch.zeros(2, 5, 3, 8, dtype=torch.bfloat16)):
+        refused("alike", call, [x, OnGpu(other)], at, [2, 2])
+    for bad in (torch.zeros(5, 3, dtype=torch.int32), torch.zeros(4, 2, dtype=torch.int32), torch.zeros(3, 5, 2, dtype=torch.int32),
+                torch.zeros(5, 2, dtype=torch.float64), torch.zeros(2, dtype=torch.int32)):
+        refused("positions", call, x, OnGpu(bad), [2, 2])
+    refused("float32, bfloat16 or float16", call, OnGpu(x.double()), at, [2, 2])
+
+
+@built
+def test_workspaces_and_their_refusals():
+    from nnv_amd import _lib, images
+    lib, n = _lib.load(), C.c_int64()
+
+    def group(backward=False, **kw):
+        s = dict(type=1, param_type=1, activation=2, batch=4, places=1000, channels=64, groups=8)
+        s.update(kw)
+        fn = lib.nnvhip_group_norm_backward_workspace if backward else lib.nnvhip_group_norm_workspace
+        _lib.check(fn(images._GROUP.pack(*s.values(), 1e-5, *[0] * 14), C.byref(n)))
+        return n.value
+
+    assert group() >= 4 * 8 * 16 and group(backward=True) >= group() + 4 * 64 * 8 and group(batch=0) == 0
+    # what is kept of long places stays a small part of them
+    assert group(backward=True, places=1 << 24, batch=1) < (1 << 24) * 64 * 2 / 16
+    assert group(channels=1 << 20, groups=1) > 0 and group(channels=5000, groups=5000) > 0
+    for kw in (dict(type=3), dict(param_type=2), dict(activation=3), dict(groups=7), dict(groups=0), dict(places=0), dict(channels=0), dict(batch=-1),
+               dict(batch=1 << 23), dict(channels=1 << 24, groups=1), dict(places=1 << 40), dict(batch=1 << 22, channels=2048), dict(places=1 << 39)):
+        for backward in (False, True):
+            with pytest.raises((ValueError, _lib.NNVHipError)):
+                group(backward, **kw)
+
+
+@pytest.mark.parametrize("activation", [None, "relu", "silu"])
+def test_plain_group_norm_is_differentiated_right(activation):
+    torch.manual_seed(3)
+    x, w, b = (torch.randn(*s, dtype=torch.float64, requires_grad=True) for s in ((3, 4, 5, 12), (12,), (12,)))
+    dy = torch.randn(3, 4, 5, 12, dtype=torch.float64)
+    y, mean, rstd = io.group(x, 4, w, b, 1e-5, activation)
+    y.backward(dy)
+    for got, t in zip(io.group_grad(dy, x.detach(), mean.detach(), rstd.detach(), w.detach(), b.detach(), activation), (x, w, b)):
+        assert torch.allclose(got, t.grad, rtol=1e-11, atol=1e-11)
+    plain = torch.nn.functional.group_norm(x.permute(0, 3, 1, 2), 4, w, b, 1e-5).permute(0, 2, 3, 1)
+    act = {None: lambda u: u, "relu": torch.relu, "silu": torch.nn.functional.silu}[activation]
+    assert torch.allclose(y, act(plain), rtol=1e-11, atol=1e-11)
+
+
+def test_plain_rotation_by_hand():
+    x = torch.arange(1.0, 9.0, dtype=torch.float64).view(1, 1, 1, 8)
+    at = torch.tensor([[2, 5]])
+    y = io.rotate(x, at, [1, 2], base=100.0)[0, 0, 0]
+    for i, (t, a, b) in enumerate([(2.0, 1, 4), (5.0, 2, 5), (0.5, 3, 6)]):
+        assert torch.allclose(y[[i, i + 3]], torch.tensor([a * math.cos(t) - b * math.sin(t), a * math.sin(t) + b * math.cos(t)], dtype=torch.float64))
+    assert torch.equal(y[6:], x[0, 0, 0, 6:])
+    z = io.rotate(x, at, [1, 2], base=100.0, shared=True, interleaved=True)[0, 0, 0]
+    for i, t in enumerate([2.0, 5 * 100 ** (-1 / 3), 5 * 100 ** (-2 / 3)]):
+        a, b = x[0, 0, 0, 2 * i], x[0, 0, 0, 2 * i + 1]
+        assert torch.allclose(z[[2 * i, 2 * i + 1]], torch.stack([a * math.cos(t) - b * math.sin(t), a * math.sin(t) + b * math.cos(t)]))
+    # turned back: the gradient
+    assert torch.allclose(io.rotate(io.rotate(x, at, [2, 2]), at, [2, 2], inverse=True), x)
+    # frequencies as the operator forms them
+    from nnv_amd.images import _frequencies
+    f, axes = _frequencies((1, 2), 100.0, True)
+    assert list(axes) == [0, 1, 1] and [round(v, 12) for v in f] == [round(100.0 ** (-i / 3), 12) for i in range(3)]
+    f, axes = _frequencies((2, 1), 100.0, False)
+    assert list(axes) == [0, 0, 1] and list(f) == [1.0, 0.1, 1.0]
