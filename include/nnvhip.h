@@ -579,6 +579,38 @@ typedef struct nnvhip_rotate_args {
 } nnvhip_rotate_args;
 NNVHIP_API int nnvhip_rotate_positions(nnvhip_ctx* ctx, const nnvhip_rotate_args* d, void* stream);
 
+/* Differential attention: o = softmax(scale * q0 k0^T) v - weights[h] * softmax(scale * q1 k1^T) v for each head h.  q: batch x queries x
+ * 2 heads x head (the two maps' queries of a head follow one another), k: batch x keys x 2 kv_heads x head (as well), v: batch x keys x
+ * kv_heads x 2 head; strides, key_lengths and key_mask as in nnvhip_attention, and consecutive heads / kv_heads heads share keys and
+ * values.  head: 1 to 128.  weights: `heads` values of weight_type (type, or f32).  causal: query i sees the keys in front of n - queries + i + 1 alone, n the
+ * sequence's length: the last query's place is the last key's.
+ *   forward: o (dense, batch x queries x heads x 2 head), lse = log of both maps' softmax sums (batch x 2 heads x queries), and, unless NULL,
+ *     second = softmax(scale * q1 k1^T) v, as o lies, which the backward call takes.  A row that sees no key gives zeros, lse = -inf.
+ *   backward: from go (the gradient of o, strided), o, lse and second: dq, dk, dv dense in the shapes of q, k, v, zero where a row or key
+ *     takes no part, and dweights in weight_type.  The order of the sums is fixed.
+ * Sizes are bounded as in nnvhip_attention, with twice the heads. */
+typedef struct nnvhip_differ_args {
+  int64_t type, weight_type, batch, queries, keys, heads, kv_heads, head, causal;
+  double scale;
+  const void *q, *k, *v;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  const void* weights;
+  const int32_t* key_lengths;
+  const uint8_t* key_mask;
+  int64_t mask_stride[2];
+  void* o;
+  float* lse;
+  void* second;
+  const void* go;
+  int64_t go_stride[3];
+  void *dq, *dk, *dv, *dweights;
+} nnvhip_differ_args;
+NNVHIP_API int nnvhip_differential_attention_workspace(const nnvhip_differ_args* d, int64_t* bytes);
+NNVHIP_API int nnvhip_differential_attention(nnvhip_ctx* ctx, const nnvhip_differ_args* d, void* workspace, int64_t workspace_bytes, void* stream);
+NNVHIP_API int nnvhip_differential_attention_backward_workspace(const nnvhip_differ_args* d, int64_t* bytes);
+NNVHIP_API int nnvhip_differential_attention_backward(nnvhip_ctx* ctx, const nnvhip_differ_args* d, void* workspace, int64_t workspace_bytes,
+                                           void* stream);
+
 #ifdef __cplusplus
 }
 #endif

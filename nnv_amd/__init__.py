@@ -15,6 +15,7 @@ from .verify import HalfSpace, verify_specification  # noqa: F401
 _POINTS = {"layer_norm": "points", "layer_norm_backward": "points", "cross_attention": "points", "cross_attention_backward": "points",
            "clip_gradients": "points", "LayerNormalizationLayer": "points", "CrossAttentionLayer": "points",
            "group_norm": "images", "group_norm_backward": "images", "rotate_positions": "images",
+           "differential_attention": "images", "differential_attention_backward": "images",
            "CrossAttentionClassifier": "falsify", "falsify_point": "falsify", "train_step": "falsify"}
 
 

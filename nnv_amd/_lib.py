@@ -34,7 +34,8 @@ SYMBOLS = [
     "nnvhip_cross_attention_workspace", "nnvhip_cross_attention", "nnvhip_cross_attention_backward_workspace",
     "nnvhip_cross_attention_backward", "nnvhip_clip_gradients_workspace", "nnvhip_clip_gradients",
     "nnvhip_group_norm_workspace", "nnvhip_group_norm", "nnvhip_group_norm_backward_workspace", "nnvhip_group_norm_backward",
-    "nnvhip_rotate_positions",
+    "nnvhip_rotate_positions", "nnvhip_differential_attention_workspace", "nnvhip_differential_attention",
+    "nnvhip_differential_attention_backward_workspace", "nnvhip_differential_attention_backward",
 ]
 
 
@@ -155,6 +156,10 @@ def load():
         "nnvhip_group_norm_backward_workspace": [p, p],
         "nnvhip_group_norm_backward": [p, p, p, i64, p],
         "nnvhip_rotate_positions": [p, p, p],
+        "nnvhip_differential_attention_workspace": [p, p],
+        "nnvhip_differential_attention": [p, p, p, i64, p],
+        "nnvhip_differential_attention_backward_workspace": [p, p],
+        "nnvhip_differential_attention_backward": [p, p, p, i64, p],
     }
     for name, args in sig.items():
         fn = getattr(lib, name)

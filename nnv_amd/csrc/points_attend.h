@@ -69,6 +69,11 @@ __device__ __forceinline__ int64_t dense_row_at(const AttendArgs& a, int b, int 
   return ((b * (int64_t)a.queries + i) * a.kv_heads * a.group + kv * (int64_t)a.group + g) * a.head;
 }
 
+// a value as it is rounded where it stands, not taken into what uses it
+__device__ __forceinline__ float rounded(float x) {
+  asm("" : "+v"(x));
+  return x;
+}
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 

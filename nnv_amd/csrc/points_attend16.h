@@ -29,14 +29,15 @@ typedef short short4_t __attribute__((ext_vector_type(4)));
 // at a time.  Both meet every bank once if the 16-byte pieces of a row are exchanged by
 //   piece ^ (row / 4 % 4 + 4 (row % 4 or what of it moves whole groups of four pieces within the row)):
 // four consecutive rows then have the same 64-byte group in different quarters of the 256 bytes that the banks span, and rows 4
-// apart have the same piece in different places of a group.  (Rows of 32 and 96 values do the first by themselves.)
+// apart have the same piece in different places of a group.  (Rows of 32, 96 and 160 values do the first by themselves.)  GROUP: the pieces
+// within which they change places.
 template <typename T, int DP>
 struct Rows16 {
-  static constexpr int PIECES = DP / 8;
+  static constexpr int PIECES = DP / 8, GROUP = DP % 128 == 0 ? 16 : DP % 64 == 0 ? 8 : 4;
   static __device__ __forceinline__ int place(int row) {
     const int low = (row >> 2) & 3;
-    if constexpr (DP == 128) return (row & 3) << 2 | low;
-    if constexpr (DP == 64) return (row >> 1 & 1) << 2 | low;
+    if constexpr (GROUP == 16) return (row & 3) << 2 | low;
+    if constexpr (GROUP == 8) return (row >> 1 & 1) << 2 | low;
     return low;
   }
   static __device__ __forceinline__ int at(int row, int piece) { return row * DP + ((piece ^ place(row)) << 3); }
@@ -47,11 +48,6 @@ struct Rows16 {
 __device__ __forceinline__ unsigned hide(unsigned at) {
   asm("" : "+v"(at));
   return at;
-}
-// a value as it is rounded where it stands, not taken into what uses it
-__device__ __forceinline__ float rounded(float x) {
-  asm("" : "+v"(x));
-  return x;
 }
 template <typename T, int DP>
 __device__ __forceinline__ unsigned rows_place(int lane) {
@@ -66,8 +62,8 @@ __device__ __forceinline__ unsigned columns_place(int lane) {
 // them).  at: LDS address of the tile + rows_place.
 template <typename T, int DP>
 __device__ __forceinline__ half8<T> rows_operand(unsigned at, int first, int c) {
-  constexpr bool WHOLE = DP == 64 || DP == 128;   // the exchange moves groups of four pieces, too
-  const unsigned x = (at ^ ((WHOLE ? c : c & 1) << 5)) + (WHOLE ? 0 : (c >> 1) * 64) + first * DP * 2;
+  constexpr int G = Rows16<T, DP>::GROUP;
+  const unsigned x = (at ^ (c % (G / 2) << 5)) + c / (G / 2) * (G * 16) + first * DP * 2;
   return *(const __attribute__((address_space(3))) half8<T>*)x;
 }
 // Left operand of a product over rows: values 32 d .. 32 d + 31 (lane: value 32 d + lane % 32) of the 16 rows first + product_row(0..7, h)
@@ -76,11 +72,11 @@ __device__ __forceinline__ half8<T> rows_operand(unsigned at, int first, int c) 
 // at: LDS address of the tile + columns_place.
 template <typename T, int DP>
 __device__ __forceinline__ half8<T> columns_operand(unsigned at, int first, int d) {
-  constexpr bool WHOLE = DP == 64 || DP == 128;
+  constexpr int G = Rows16<T, DP>::GROUP;
   short4_t r[2];
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    const unsigned x = (at ^ (half << 5 | (WHOLE ? d << 6 : 0))) + (WHOLE ? 0 : d * 64) + (first + 8 * half) * DP * 2;
+    const unsigned x = (at ^ (half << 5 | d % (G / 4) << 6)) + d / (G / 4) * (G * 16) + (first + 8 * half) * DP * 2;
     r[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)x);
   }
   half8<T> f;

@@ -1,0 +1,364 @@
+// Differential attention of points, backward: the kernels for every type, head size and alignment, with f32 products.
+//
+// As in points_attend_grad.hip two kernels form dq (a wave per 16 queries, both maps) and dk, dv (a wave per 16 keys), each sum in the registers of
+// one wave, in a fixed order, with no atomics.  do v^T, half of what the scores' gradients take, is one product for both maps.  D of both maps and
+// the weights' gradients come first.
+#include "points_differ.h"
+
+#pragma clang fp contract(fast)
+
+namespace nnvhip {
+namespace {
+
+constexpr int kBlockRows = 64;   // rows, or keys, of a block
+
+// D_1 = rowsum(do second), D_0 = rowsum(do o) + w D_1: 16 lanes a row.
+template <typename T, int>
+__global__ __launch_bounds__(256) void differ_delta_kernel(const DifferArgs a) {
+  const int64_t flat = (int64_t)blockIdx.x * 16 + threadIdx.x / 16, all = (int64_t)a.batch * a.kv_heads * a.rows;
+  const bool here = flat < all;
+  const int64_t f = here ? flat : 0, bkv = f / a.rows, r = f % a.rows;
+  const int b = (int)(bkv / a.kv_heads), kv = (int)(bkv % a.kv_heads), size = 2 * a.head;
+  const T* o = (const T*)a.out + wide_row_at(a, b, kv, r);
+  const T* second = (const T*)a.second + wide_row_at(a, b, kv, r);
+  const T* g = (const T*)a.go.p + row_at(a.go, a, b, kv, r);
+  float s[2] = {0, 0};
+  for (int d = threadIdx.x % 16 * 4; d < size; d += 64) {
+    const Four x = load_four(o, d, size, true), z = load_four(second, d, size, true), y = load_four(g, d, size, true);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[0] += x.v[i] * y.v[i];
+      s[1] += z.v[i] * y.v[i];
+    }
+  }
+#pragma unroll
+  for (int k = 8; k > 0; k >>= 1)
+#pragma unroll
+    for (int m = 0; m < 2; ++m) s[m] += __shfl_xor(s[m], k, 64);
+  if (!here || threadIdx.x % 16) return;
+  const bool takes_part = a.lse[lse_at(a, b, kv, r, 0)] != -INFINITY;   // (both maps see the same keys)
+  a.delta[own_row(a, bkv, r, 0)] = takes_part ? s[0] + weight_of<T>(a, head_of_row(a, kv, r)) * s[1] : 0.0f;
+  a.delta[own_row(a, bkv, r, 1)] = takes_part ? s[1] : 0.0f;
+}
+
+// dw of a head: a block adds its rows' D_1, in f64.
+template <typename T, int>
+__global__ __launch_bounds__(256) void differ_weights_kernel(const DifferArgs a) {
+  __shared__ double lds[4];
+  const int head = blockIdx.x, kv = head / a.group, g = head % a.group;
+  double s = 0;
+  for (int b = 0; b < a.batch; ++b) {
+    const float* from = a.delta + own_row(a, b * (int64_t)a.kv_heads + kv, (int64_t)g * a.queries, 1);
+    for (int i = threadIdx.x; i < a.queries; i += 256) s += (double)from[i];
+  }
+#pragma unroll
+  for (int k = 32; k > 0; k >>= 1) s += __shfl_xor(s, k, 64);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x) return;
+  const float all = (float)-(lds[0] + lds[1] + lds[2] + lds[3]);
+  if (a.wide_weights) ((float*)a.dweights)[head] = all;
+  else ((T*)a.dweights)[head] = from_f<T>(all);
+}
+
+// lse of a row as the exponent's offset in powers of two; a row without keys takes no part (exp2(s - inf) = 0)
+__device__ __forceinline__ float offset_of(float lse) { return lse == -INFINITY ? INFINITY : lse * kLog2e; }
+
+template <typename T, int CH, bool FOUR>
+__global__ __launch_bounds__(256, CH <= 6 ? 2 : 1) void differ_query_grad_kernel(const DifferArgs a) {
+  constexpr int R = 32, LD = F32Tile<CH>::LD;
+  __shared__ __attribute__((aligned(16))) float tile[F32Tile<CH>::FLOATS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, q4 = lane >> 4;
+  int64_t at = blockIdx.x;
+  const int split = at % a.splits;
+  at /= a.splits;
+  const int row_tile = a.row_tiles - 1 - (int)(at % a.row_tiles);
+  const int bkv = at / a.row_tiles, b = bkv / a.kv_heads, kv = bkv % a.kv_heads;
+  const int n = keys_that_count(a, b);
+  const int64_t first = (int64_t)row_tile * kBlockRows, last = min(first + kBlockRows, a.rows) - 1;
+  const int tiles = (most_seen(a, first, last, n) + R - 1) / R, per = (tiles + a.splits - 1) / a.splits;
+  const int t0 = split * per, t1 = min(tiles, t0 + per);
+  const int64_t r = first + wave * 16 + col;
+  const bool here = r < a.rows, idle = first + wave * 16 >= a.rows;
+  float offset[2], delta[2];
+#pragma unroll
+  for (int m = 0; m < 2; ++m) offset[m] = offset_of(here ? a.lse[lse_at(a, b, kv, r, m)] : -INFINITY);
+  const bool takes_part = offset[0] < INFINITY;
+#pragma unroll
+  for (int m = 0; m < 2; ++m) delta[m] = takes_part ? a.delta[own_row(a, bkv, r, m)] : 0.0f;
+  const int seen = takes_part ? seen_by(a, r, n) : 0;
+  const float w = here ? weight_of<T>(a, head_of_row(a, kv, r)) : 0.0f, unit = a.scale * kLog2e;
+  float qf[2][CH][4], gf[2 * CH][4];
+#pragma unroll
+  for (int m = 0; m < 2; ++m) f32_operands<T, CH>((const T*)a.q.p + (here ? map_row_at(a.q, a, b, kv, r, m) : 0), q4, a.head, takes_part, qf[m]);
+  f32_operands<T, 2 * CH>((const T*)a.go.p + (here ? row_at(a.go, a, b, kv, r) : 0), q4, 2 * a.head, takes_part, gf);
+  float4_t dq[2][CH];
+#pragma unroll
+  for (int m = 0; m < 2; ++m) f32_zero(dq[m]);
+  const T* kp = (const T*)a.k.p + b * a.k.b + 2 * kv * a.k.h;
+  const T* vp = (const T*)a.v.p + b * a.v.b + kv * a.v.h;
+  TripleAhead<T, CH, 256, FOUR> next;
+  int counts = 0;
+  auto fetch = [&](int t) {
+    next.load([&](int j, int which) { return kp + min(t * R + j, n - 1) * a.k.t + which * a.k.h; }, [&](int j) { return vp + min(t * R + j, n - 1) * a.v.t; },
+              a.head, threadIdx.x);
+    counts = key_word(a, b, t * R + (lane & 31), n);
+  };
+  if (t0 < t1) fetch(t0);
+  for (int t = t0; t < t1; ++t) {
+    __syncthreads();
+    const uint32_t valid = (uint32_t)__ballot(counts != 0);
+    next.store(tile, valid, a.head, threadIdx.x);
+    __syncthreads();
+    if (t + 1 < t1) fetch(t + 1);
+    if (idle) continue;
+    const uint32_t mine = valid & first_bits(seen - t * R);
+    float4_t dp[2];
+    f32_over_head<CH, 2 * CH>(tile + col * LD + 4 * q4 + 32 * CH, gf, dp);
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      float4_t s[2];
+      f32_over_head<CH, CH>(tile + col * LD + 4 * q4 + m * 16 * CH, qf[m], s);
+      const float by = m ? -w : 1.0f;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          s[k][i] = f32_bit(mine, k, i, q4) ? by * exp2_(s[k][i] * unit - offset[m]) * (dp[k][i] - delta[m]) : 0.0f;
+      f32_over_rows<CH, CH>(tile + 4 * q4 * LD + col + m * 16 * CH, s, dq[m]);
+    }
+  }
+  if (!here) return;
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    if (a.splits > 1) f32_store(a.part + (split * own_rows(a) + own_row(a, bkv, r, m)) * a.head, dq[m], a.scale, q4, a.head);
+    else f32_store((T*)a.dq + dense_map_row_at(a, b, kv, r, m), dq[m], a.scale, q4, a.head);
+  }
+}
+
+template <typename T, int CH, bool FOUR>
+__global__ __launch_bounds__(256, CH <= 4 ? 2 : 1) void differ_key_grad_kernel(const DifferArgs a) {
+  constexpr int R = 32, LD = F32Tile<CH>::LD;
+  __shared__ __attribute__((aligned(16))) float tile[F32Tile<CH>::FLOATS];
+  __shared__ __attribute__((aligned(16))) float offsets[2][R], deltas[2][R], weights[R], seen_by_row[R];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, q4 = lane >> 4;
+  int64_t at = blockIdx.x;
+  const int split = at % a.splits;
+  at /= a.splits;
+  const int key_tile = at % a.key_tiles;
+  const int bkv = at / a.key_tiles, b = bkv / a.kv_heads, kv = bkv % a.kv_heads;
+  const int n = keys_that_count(a, b);
+  const int first = key_tile * kBlockRows, key = first + wave * 16 + col;
+  const bool here = key < a.keys, counts = key_counts(a, b, key, n), idle = first + wave * 16 >= n;
+  const int i_min = a.causal ? first - (n - a.queries) : 0;   // the first query that sees one of the block's keys
+  int t0 = 0, t1 = 0;
+  if (first < n) {   // else no key of the block counts: its gradients are zero
+    const int tiles = (int)((a.rows + R - 1) / R), per = (tiles + a.splits - 1) / a.splits;
+    t0 = split * per;
+    t1 = min(tiles, t0 + per);
+  }
+  const int64_t row = here && counts ? key : 0;
+  float kf[2][CH][4], vf[2 * CH][4];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+    f32_operands<T, CH>((const T*)a.k.p + (counts ? b * a.k.b + (2 * kv + m) * a.k.h + row * a.k.t : 0), q4, a.head, counts, kf[m]);
+  f32_operands<T, 2 * CH>((const T*)a.v.p + (counts ? b * a.v.b + kv * a.v.h + row * a.v.t : 0), q4, 2 * a.head, counts, vf);
+  const float unit = a.scale * kLog2e;
+  float4_t dk[2][CH], dv[2 * CH];
+#pragma unroll
+  for (int m = 0; m < 2; ++m) f32_zero(dk[m]);
+  f32_zero(dv);
+  TripleAhead<T, CH, 256, FOUR> next;
+  float next_offset[2] = {INFINITY, INFINITY}, next_delta[2] = {0, 0}, next_weight = 0;
+  int next_seen = 0;
+  auto fetch = [&](int t) {
+    auto row = [&](int j) { return min((int64_t)t * R + j, a.rows - 1); };
+    next.load([&](int j, int which) { return (const T*)a.q.p + map_row_at(a.q, a, b, kv, row(j), which); },
+              [&](int j) { return (const T*)a.go.p + row_at(a.go, a, b, kv, row(j)); }, a.head, threadIdx.x);
+    // (every wave of its own: which rows take part decides what the tile's rows are)
+    const int64_t r = (int64_t)t * R + (lane & 31);
+    const bool is = r < a.rows;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      next_offset[m] = offset_of(is ? a.lse[lse_at(a, b, kv, r, m)] : -INFINITY);
+      next_delta[m] = is ? a.delta[own_row(a, bkv, r, m)] : 0.0f;
+    }
+    next_weight = is ? weight_of<T>(a, head_of_row(a, kv, r)) : 0.0f;
+    next_seen = is ? seen_by(a, r, n) : 0;
+  };
+  int t = next_row_tile(a, t0, R, i_min);
+  if (t < t1) fetch(t);
+  while (t < t1) {
+    __syncthreads();
+    // a row without keys counts for nothing: what it holds must not reach the sums
+    next.store(tile, (uint32_t)__ballot(next_offset[0] < INFINITY), a.head, threadIdx.x);
+    if (threadIdx.x < R) {
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        offsets[m][threadIdx.x] = next_offset[m];
+        deltas[m][threadIdx.x] = next_delta[m];
+      }
+      weights[threadIdx.x] = next_weight;
+      seen_by_row[threadIdx.x] = __builtin_bit_cast(float, next_seen);
+    }
+    __syncthreads();
+    t = next_row_tile(a, t + 1, R, i_min);
+    if (t < t1) fetch(t);
+    if (idle) continue;
+    float4_t s[2][2], dp[2], both[2];
+    bool sees[2][4];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) f32_over_head<CH, CH>(tile + col * LD + 4 * q4 + m * 16 * CH, kf[m], s[m]);
+    f32_over_head<CH, 2 * CH>(tile + col * LD + 4 * q4 + 32 * CH, vf, dp);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = 16 * k + 4 * q4 + i;
+        sees[k][i] = key < __builtin_bit_cast(int, seen_by_row[j]);
+        const float w = weights[j];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) s[m][k][i] = sees[k][i] ? exp2_(s[m][k][i] * unit - offsets[m][j]) : 0.0f;
+        both[k][i] = s[0][k][i] - w * s[1][k][i];
+        s[0][k][i] *= sees[k][i] ? dp[k][i] - deltas[0][j] : 0.0f;
+        s[1][k][i] *= sees[k][i] ? -w * (dp[k][i] - deltas[1][j]) : 0.0f;
+      }
+    f32_over_rows<CH, 2 * CH>(tile + 4 * q4 * LD + col + 32 * CH, both, dv);
+#pragma unroll
+    for (int m = 0; m < 2; ++m) f32_over_rows<CH, CH>(tile + 4 * q4 * LD + col + m * 16 * CH, s[m], dk[m]);
+  }
+  if (!here) return;
+  if (!counts) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) f32_zero(dk[m]);
+    f32_zero(dv);
+  }
+  const int64_t dense = ((b * (int64_t)a.keys + key) * a.kv_heads + kv) * 2 * a.head;   // of dv; of dk's first map as well
+  if (a.splits > 1) {
+    const int64_t all = (int64_t)a.batch * a.keys * a.kv_heads * 2 * a.head;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) f32_store(a.part + split * all + dense + m * a.head, dk[m], a.scale, q4, a.head);
+    f32_store(a.part + (a.splits + split) * all + dense, dv, 1.0f, q4, 2 * a.head);
+  } else {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) f32_store((T*)a.dk + dense + m * a.head, dk[m], a.scale, q4, a.head);
+    f32_store((T*)a.dv + dense, dv, 1.0f, q4, 2 * a.head);
+  }
+}
+
+// dk[e] = sum over splits of part[s][e], in order, and dv[e] of those behind (blockIdx.y)
+template <typename T, int>
+__global__ __launch_bounds__(256) void differ_sum_kernel(const float* __restrict__ part, int splits, int64_t n, T* __restrict__ dk, T* __restrict__ dv) {
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (e >= n) return;
+  part += blockIdx.y * splits * n + e;
+  float s = 0.0f;
+  for (int k = 0; k < splits; k += 4) {
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = k + i < splits ? part[(k + i) * n] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s += v[i];
+  }
+  (blockIdx.y ? dv : dk)[e] = from_f<T>(s);
+}
+// dq's maps' rows from the splits', written in the order of the tensor: a wave a row
+template <typename T, int>
+__global__ __launch_bounds__(256) void differ_sum_rows_kernel(const DifferArgs a) {
+  const int64_t all = own_rows(a), own = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (own >= all) return;
+  const int64_t bkv = own / (2 * a.rows), left = own - bkv * 2 * a.rows, m = left / a.rows;
+  T* row = (T*)a.dq + dense_map_row_at(a, (int)(bkv / a.kv_heads), (int)(bkv % a.kv_heads), left - m * a.rows, (int)m);
+  for (int d = threadIdx.x & 63; d < a.head; d += 64) {
+    float s = 0.0f;
+    for (int k = 0; k < a.splits; ++k) s += a.part[(k * all + own) * a.head + d];
+    row[d] = from_f<T>(s);
+  }
+}
+
+struct GradCut {
+  int row_tiles, key_tiles, query_splits, key_splits;
+  int64_t delta, part;   // floats of the workspace
+};
+GradCut grad_cut(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys, int64_t head) {
+  GradCut c;
+  c.row_tiles = (int)ceil_div(rows, kBlockRows);
+  c.key_tiles = (int)ceil_div(keys, kBlockRows);
+  c.query_splits = split_of(batch * kv_heads * c.row_tiles, ceil_div(keys, 32), 2, head > 96 ? 256 : 512, 2, 3);
+  c.key_splits = split_of(batch * kv_heads * c.key_tiles, ceil_div(rows, 32), 2, head > 64 ? 256 : 512, 2, 3);
+  c.delta = round_up(batch * kv_heads * 2 * rows, 64);
+  const int64_t q = c.query_splits > 1 ? c.query_splits * batch * kv_heads * 2 * rows * head : 0;
+  const int64_t k = c.key_splits > 1 ? 2 * c.key_splits * batch * kv_heads * keys * 2 * head : 0;
+  c.part = std::max(q, k);
+  return c;
+}
+
+template <typename T, int CH>
+void launch_grad(DifferArgs a, const GradCut& c, hipStream_t st) {
+  const int64_t heads = (int64_t)a.batch * a.kv_heads;
+  const bool four = a.head % 4 == 0;
+  if (a.rows > 0 && heads > 0) {
+    hipLaunchKernelGGL((differ_delta_kernel<T, 0>), dim3((unsigned)ceil_div(heads * a.rows, 16)), dim3(256), 0, st, a);
+    a.row_tiles = c.row_tiles;
+    a.splits = c.query_splits;
+    const dim3 grid((unsigned)(heads * c.row_tiles * a.splits));
+    if (four) hipLaunchKernelGGL((differ_query_grad_kernel<T, CH, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((differ_query_grad_kernel<T, CH, false>), grid, dim3(256), 0, st, a);
+    if (a.splits > 1) hipLaunchKernelGGL((differ_sum_rows_kernel<T, 0>), dim3((unsigned)ceil_div(heads * 2 * a.rows, 4)), dim3(256), 0, st, a);
+  } else {
+    a.batch = 0;   // (for the sums over no rows)
+  }
+  hipLaunchKernelGGL((differ_weights_kernel<T, 0>), dim3((unsigned)(a.kv_heads * a.group)), dim3(256), 0, st, a);
+  if (a.keys > 0 && heads > 0) {
+    a.batch = (int)(heads / a.kv_heads);
+    a.key_tiles = c.key_tiles;
+    a.splits = c.key_splits;
+    const dim3 grid((unsigned)(heads * c.key_tiles * a.splits));
+    if (four) hipLaunchKernelGGL((differ_key_grad_kernel<T, CH, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((differ_key_grad_kernel<T, CH, false>), grid, dim3(256), 0, st, a);
+    if (a.splits > 1) {
+      const int64_t n = heads * a.keys * 2 * a.head;
+      hipLaunchKernelGGL((differ_sum_kernel<T, 0>), dim3((unsigned)ceil_div(n, 256), 2), dim3(256), 0, st, a.part, a.splits, n, (T*)a.dk, (T*)a.dv);
+    }
+  }
+}
+
+}  // namespace
+}  // namespace nnvhip
+
+using namespace nnvhip;
+
+extern "C" {
+
+int nnvhip_differential_attention_backward_workspace(const nnvhip_differ_args* d, int64_t* bytes) {
+  int64_t forward = 0;
+  NNV_TRY(nnvhip_differential_attention_workspace(d, &forward));   // checks the sizes
+  if (!bytes) NNV_FAIL(NNVHIP_ERR_ARG, "null pointer");
+  const int64_t heads = d->batch * d->kv_heads, blocks = kMostBlocks;
+  if (ceil_div(d->batch * d->heads * d->queries, 16) > 2 * blocks) NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_differential_attention_backward: too many rows");
+  if (heads * ceil_div(d->keys, kBlockRows) > blocks) NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_differential_attention_backward: too many keys");
+  const GradCut c = grad_cut(d->batch, d->kv_heads, d->queries * (d->heads / d->kv_heads), d->keys, d->head);
+  if (heads * c.row_tiles * c.query_splits > blocks) NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_differential_attention_backward: too many rows");
+  if (heads * c.key_tiles * c.key_splits > blocks || (c.key_splits > 1 && ceil_div(heads * d->keys * 2 * d->head, 256) > blocks))
+    NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_differential_attention_backward: too many keys");
+  *bytes = (c.delta + c.part) * (int64_t)sizeof(float);
+  return NNVHIP_OK;
+}
+
+int nnvhip_differential_attention_backward(nnvhip_ctx* ctx, const nnvhip_differ_args* d, void* workspace, int64_t workspace_bytes, void* stream) {
+  ENTER_POINT_CALL(ctx);
+  DifferArgs a;
+  NNV_TRY(differ_args("nnvhip_differential_attention_backward", d, true, &a));
+  int64_t need = 0;
+  NNV_TRY(nnvhip_differential_attention_backward_workspace(d, &need));
+  if (need > workspace_bytes || (need && !workspace))
+    NNV_FAIL(NNVHIP_ERR_ARG, "nnvhip_differential_attention_backward: a workspace of %lld bytes is needed", (long long)need);
+  const GradCut c = grad_cut(a.batch, a.kv_heads, a.rows, a.keys, a.head);
+  a.delta = static_cast<float*>(workspace);
+  a.part = a.delta + c.delta;
+  DIFFER_BY_TYPE(d->type, launch_grad, a, c, (hipStream_t)stream);
+  NNV_HIP_TRY(hipGetLastError());
+  return NNVHIP_OK;
+}
+
+}  // extern "C"

@@ -14,8 +14,8 @@ import struct
 
 import torch
 
-from ._lib import check, default_context
-from .points import _INT64, _enter, _ptr, _type
+from ._lib import check
+from .points import _INT64, _LARGEST, _dense_values, _enter, _mask_args, _ptr, _type
 
 # ---- group normalization ------------------------------------------------------------------------
 
@@ -199,3 +199,101 @@ def rotate_positions(x, positions, sections, base=10000.0, shared=False, interle
         check(lib.nnvhip_rotate_positions(ctx.handle, d, stream))
         done += out
     return done if several else done[0]
+
+
+# ---- differential attention ---------------------------------------------------------------------
+
+_DIFFER = struct.Struct("=9qd3Q9qQQQ2qQQQQ3q4Q")   # struct nnvhip_differ_args
+
+
+def _differ_sizes(what, q, k, v, weights, key_lengths, key_mask, scale):
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError("%s: q, k and v are batch x tokens x heads x head" % what)
+    batch, queries, heads, head = q.shape
+    keys, kv_heads = v.shape[1], v.shape[2]
+    if k.shape != (batch, keys, 2 * kv_heads, head) or v.shape != (batch, keys, kv_heads, 2 * head):
+        raise ValueError("%s: q %s, k %s and v %s do not fit together" % (what, tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("%s: q, k and v must have one type" % what)
+    if not 1 <= head <= 128:
+        raise ValueError("%s: heads of 1 to 128 values (and as many again in v) are supported" % what)
+    if scale is not None and not abs(scale) <= _LARGEST:
+        raise ValueError("%s: the scale must be a finite number of f32" % what)
+    if heads % 2 or heads < 2 or kv_heads < 1 or heads // 2 % kv_heads:
+        raise ValueError("%s: q has two maps a head, of as many heads as a multiple of the key/value heads" % what)
+    t = _type(what, q)
+    if weights.shape != (heads // 2,):
+        raise ValueError("%s: weights has one value per head (%d), not the shape %s" % (what, heads // 2, tuple(weights.shape)))
+    w = _type(what, weights)
+    if w not in (t, 0):
+        raise ValueError("%s: weights has the type of the values, or float32" % what)
+    if key_lengths is not None and (key_lengths.shape != (batch,) or key_lengths.dtype not in (torch.int32, torch.int64)):
+        raise ValueError("%s: key_lengths is one whole number per sequence" % what)
+    if key_mask is not None and (key_mask.shape != (batch, keys) or key_mask.dtype not in (torch.bool, torch.uint8)):
+        raise ValueError("%s: key_mask is one truth value per sequence and key" % what)
+    return t, w, batch, queries, keys, heads // 2, kv_heads, head
+
+
+@functools.lru_cache(maxsize=256)
+def _differ_workspace(lib, backward, causal, *sizes):
+    n = _INT64()
+    d = _DIFFER.pack(*sizes, causal, 0.0, *[0] * 28)
+    check((lib.nnvhip_differential_attention_backward_workspace if backward else lib.nnvhip_differential_attention_workspace)(d, C.byref(n)))
+    return n.value
+
+
+def differential_attention(q, k, v, weights, key_lengths=None, key_mask=None, causal=False, scale=None, for_backward=False, ctx=None):
+    """softmax(scale * q0 k0^T) v - weights * softmax(scale * q1 k1^T) v: the difference of two attention maps, with a weight per head.
+
+    q: batch x queries x 2 heads x head, the two maps' queries of a head one after the other (2 h and 2 h + 1); k: batch x keys x
+    2 kv_heads x head, as well; v: batch x keys x kv_heads x 2 head; any strides; consecutive heads / kv_heads heads share keys and values; head is 128 at
+    most.  weights: a vector of ``heads`` values of q's type or f32.  key_lengths and key_mask say which keys count, as in
+    cross_attention: what the others hold is of no effect.  causal: query i of a sequence of n keys sees the keys in front of n - queries + i + 1 alone (the
+    last query's place is the last key's); v should then be finite in the keys that count: zero weights of keys that are seen later are multiplied with it.  scale:
+    1 / sqrt(head) if None.
+
+    Returns (o, lse, second): o, batch x queries x heads x 2 head, of q's type; the logarithms of both maps' softmax sums, batch x 2 heads x queries, f32; and, if
+    for_backward, the second map's softmax times v, in o's shape and type, else None.  A query that sees no key has the result 0 and the logarithm -inf."""
+    what = "differential_attention"
+    ctx, lib, stream = _enter(what, ctx, q, k, v, weights, key_lengths, key_mask)
+    sizes = _differ_sizes(what, q, k, v, weights, key_lengths, key_mask, scale)
+    t, w, batch, queries, keys, heads, kv_heads, head = sizes
+    q, k, v, weights = _dense_values(q), _dense_values(k), _dense_values(v), _dense(weights)
+    lengths, mask_stride = _mask_args(key_lengths, key_mask, keys)
+    o = q.new_empty((batch, queries, heads, 2 * head))
+    second = torch.empty_like(o) if for_backward else None
+    lse = q.new_empty((batch, 2 * heads, queries), dtype=torch.float32)
+    d = _DIFFER.pack(*sizes, bool(causal), head ** -0.5 if scale is None else scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3],
+                     *k.stride()[:3], *v.stride()[:3], weights.data_ptr(), _ptr(lengths) or 0, _ptr(key_mask) or 0, *mask_stride, o.data_ptr(),
+                     lse.data_ptr(), _ptr(second) or 0, 0, 0, 0, 0, 0, 0, 0, 0)
+    need = _differ_workspace(lib, False, bool(causal), *sizes)
+    work = q.new_empty((need,), dtype=torch.uint8) if need else None
+    check(lib.nnvhip_differential_attention(ctx.handle, d, _ptr(work), need, stream))
+    return o, lse, second
+
+
+def differential_attention_backward(do, q, k, v, weights, o, lse, second, key_lengths=None, key_mask=None, causal=False, scale=None, ctx=None):
+    """The gradients (dq, dk, dv, dweights) of differential_attention, from that of o and from what the forward call (with for_backward)
+    returned; the other arguments are that call's.  Rows that see no key and keys that do not count get zero.  dweights has the type of weights."""
+    what = "differential_attention_backward"
+    ctx, lib, stream = _enter(what, ctx, q, k, v, weights, key_lengths, key_mask, do, o, lse, second)
+    sizes = _differ_sizes(what, q, k, v, weights, key_lengths, key_mask, scale)
+    t, w, batch, queries, keys, heads, kv_heads, head = sizes
+    for x in (do, o, second):
+        if x is None or x.shape != (batch, queries, heads, 2 * head) or x.dtype != q.dtype:
+            raise ValueError("%s: do, o and second must have the shape and type of what differential_attention returned (for_backward)" % what)
+    if lse.shape != (batch, 2 * heads, queries) or lse.dtype != torch.float32:
+        raise ValueError("%s: lse must be what differential_attention returned" % what)
+    q, k, v, do, weights = _dense_values(q), _dense_values(k), _dense_values(v), _dense_values(do), _dense(weights)
+    o, lse, second = o.contiguous(), lse.contiguous(), second.contiguous()
+    lengths, mask_stride = _mask_args(key_lengths, key_mask, keys)
+    dq, dk, dv = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k, v))
+    dweights = torch.empty_like(weights)
+    d = _DIFFER.pack(*sizes, bool(causal), head ** -0.5 if scale is None else scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3],
+                     *k.stride()[:3], *v.stride()[:3], weights.data_ptr(), _ptr(lengths) or 0, _ptr(key_mask) or 0, *mask_stride, o.data_ptr(),
+                     lse.data_ptr(), second.data_ptr(), do.data_ptr(), *do.stride()[:3], dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                     dweights.data_ptr())
+    need = _differ_workspace(lib, True, bool(causal), *sizes)
+    work = q.new_empty((need,), dtype=torch.uint8) if need else None
+    check(lib.nnvhip_differential_attention_backward(ctx.handle, d, _ptr(work), need, stream))
+    return dq, dk, dv, dweights

@@ -258,3 +258,199 @@ def test_images_on_another_stream_and_in_a_graph():
         torch.cuda.synchronize()
         for a, e in zip(held, fresh):
             assert torch.equal(a, e)
+
+
+# ---- differential attention ---------------------------------------------------------------------
+
+
+def make_differ(g, b, lq, lk, h, hkv, d, dtype, weight_dtype=None):
+    return (rand(g, b, lq, 2 * h, d, dtype=dtype), rand(g, b, lk, 2 * hkv, d, dtype=dtype), rand(g, b, lk, hkv, 2 * d, dtype=dtype),
+            rand(g, h, dtype=weight_dtype or dtype, scale=0.3, shift=0.5))
+
+
+def check_differ(q, k, v, w, backward=True, tag="", **kw):
+    import nnv_amd as nnv
+    o, lse, second = nnv.differential_attention(q, k, v, w, for_backward=backward, **kw)
+    assert o.dtype == q.dtype and (second is None) == (not backward)
+    exact, bounds = io.differ(q, k, v, w, **kw), io.differ_bounds(q, k, v, w, **kw)
+    for name, got, e, bd in zip(("o", "lse", "second"), (o, lse, second), exact, bounds):
+        if got is not None:
+            po.assert_within(got, e, bd, tag + " " + name)
+    if not backward:
+        return o, lse
+    do = rand(gen(q.shape[1]), *o.shape, dtype=q.dtype)
+    grads = nnv.differential_attention_backward(do, q, k, v, w, o, lse, second, **kw)
+    for name, t, got, e, bd in zip(("dq", "dk", "dv", "dweights"), (q, k, v, w), grads, io.differ_grad(do, q, k, v, w, **kw),
+                                   io.differ_grad_bounds(do, q, k, v, w, **kw)):
+        assert got.dtype == t.dtype and got.shape == t.shape
+        po.assert_within(got, e, bd, tag + " " + name)
+    return o, lse
+
+
+# batch, queries, keys, heads, key/value heads, head: single tokens, one key, tiles that do not come out even, rows of several heads in a tile, every template
+DIFFER_SIZES = [(1, 1, 1, 1, 1, 8), (2, 1, 33, 4, 4, 64), (3, 1, 700, 8, 2, 128), (1, 1, 5000, 16, 1, 32), (2, 3, 17, 3, 1, 16), (1, 64, 64, 2, 2, 64), (2, 65, 63, 2, 1, 40),
+                (1, 130, 257, 4, 2, 80), (1, 33, 129, 6, 3, 96), (2, 100, 300, 2, 2, 128), (1, 70, 90, 2, 1, 112), (1, 40, 50, 2, 2, 7), (1, 31, 65, 3, 3, 33), (1, 20, 45, 2, 1, 50),
+                (1, 17, 40, 2, 2, 90), (1, 19, 21, 2, 2, 126), (1, 300, 290, 1, 1, 64), (2, 5, 4000, 4, 4, 48), (1, 16, 64, 20, 4, 24), (1, 513, 40, 2, 1, 72)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("size", DIFFER_SIZES, ids=lambda s: "x".join(map(str, s)))
+def test_differential_attention(size, dtype):
+    b, lq, lk, h, hkv, d = size
+    g = gen(sum(size))
+    q, k, v, w = make_differ(g, *size, dtype)
+    check_differ(q, k, v, w, tag="all")
+    check_differ(q, k, v, w, causal=True, tag="causal")
+    lengths = torch.randint(0, lk + 1, (b,), generator=g, device="cuda", dtype=torch.int32)
+    lengths[0] = lk - lk // 3
+    mask = torch.rand(b, lk, generator=g, device="cuda") < 0.8
+    check_differ(q, k, v, w.float(), key_lengths=lengths, causal=True, tag="lengths, causal")
+    check_differ(q, k, v, w, key_lengths=lengths, key_mask=mask, tag="lengths, mask")
+    check_differ(q, k, v, w, key_mask=mask, causal=True, scale=-0.3, tag="mask, causal")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_differential_attention_without_keys_and_past_the_last(dtype):
+    """Rows that see no key, and what lies in keys that do not count: zeros, -inf, and no trace of it."""
+    import nnv_amd as nnv
+    for d, lq in ((64, 70), (128, 70), (40, 1), (48, 5), (33, 20)):
+        g = gen(d)
+        q, k, v, w = make_differ(g, 4, lq, 150, 4, 2, d, dtype)
+        lengths = torch.tensor([0, 150, 40, 67], device="cuda")
+        mask = torch.ones(4, 150, device="cuda", dtype=torch.bool)
+        mask[1] = False
+        mask[3, 5:60] = False
+        clean_k, clean_v = k.clone(), v.clone()
+        for i, n in enumerate((0, 0, 40, 67)):
+            k[i, n:], v[i, n:] = math.nan, math.inf
+        k[3, 5:60], v[3, 5:60] = -math.inf, math.nan
+        for causal in (False, True):
+            kw = dict(key_lengths=lengths, key_mask=mask, causal=causal)
+            o, lse, second = nnv.differential_attention(q, k, v, w, for_backward=True, **kw)
+            for name, got, e, bd in zip(("o", "lse", "second"), (o, lse, second), io.differ(q, clean_k, clean_v, w, **kw), io.differ_bounds(q, clean_k, clean_v, w, **kw)):
+                po.assert_within(got, e, bd, name)
+            assert (o[:2] == 0).all() and (lse[:2] == -math.inf).all()
+            do = rand(g, *o.shape, dtype=dtype)
+            # what rows without keys hold reaches no gradient either
+            q2, do2 = q.clone(), do.clone()
+            q2[:2], do2[:2] = math.nan, math.inf
+            if causal and lq > 40:
+                q2[2, :lq - 40], do2[2, :lq - 40] = math.inf, math.nan
+            for name, got, e, bd in zip(("dq", "dk", "dv", "dweights"), nnv.differential_attention_backward(do2, q2, k, v, w, o, lse, second, **kw),
+                                        io.differ_grad(do, q, clean_k, clean_v, w, **kw), io.differ_grad_bounds(do, q, clean_k, clean_v, w, **kw)):
+                po.assert_within(got, e, bd, "%s %s" % (causal, name))
+
+
+def test_differential_attention_of_nothing():
+    import nnv_amd as nnv
+    for b, lq, lk in ((0, 5, 7), (2, 0, 7), (2, 5, 0)):
+        q, k, v, w = make_differ(gen(1), b, lq, lk, 4, 2, 32, BF16)
+        o, lse, second = nnv.differential_attention(q, k, v, w, for_backward=True)
+        assert o.shape == (b, lq, 4, 64) and float(o.abs().sum()) == 0 and bool((lse == -math.inf).all())
+        grads = nnv.differential_attention_backward(torch.ones_like(o), q, k, v, w, o, lse, second)
+        assert [t.shape for t in grads] == [q.shape, k.shape, v.shape, w.shape] and all(float(t.abs().sum()) == 0 for t in grads)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_differential_attention_of_views(dtype):
+    """Strides of a joint projection, heads before tokens, odd starts, one sequence's keys for all, masks and lengths with strides."""
+    import nnv_amd as nnv
+    g = gen(31)
+    joint = rand(g, 3, 77, 8 * 64 + 4 * 64 + 2 * 128 + 5, dtype=dtype)
+    w = rand(g, 8, shift=0.5)[::2]
+    for odd in (0, 5):
+        q = joint[..., odd:odd + 512].unflatten(2, (8, 64))
+        k = joint[..., odd + 512:odd + 768].unflatten(2, (4, 64))
+        v = joint[..., odd + 768:odd + 1024].unflatten(2, (2, 128))
+        check_differ(q, k, v, w, causal=True, tag="joint %d" % odd)
+        check_differ(q[:, ::7], k[:1].expand(3, -1, -1, -1), v[:1].expand(3, -1, -1, -1), w, tag="shared %d" % odd)
+    q, k, v, _ = make_differ(g, 2, 50, 60, 4, 2, 32, dtype)
+    mask = torch.rand(60, 2, 3, generator=g, device="cuda") < 0.7
+    lengths = torch.tensor([[59, 0], [13, 0]], device="cuda")[:, 0]
+    check_differ(q.transpose(1, 2).contiguous().transpose(1, 2), k.flip(3).transpose(2, 3).contiguous().transpose(2, 3), v, w, key_mask=mask[:, :, 1].t(),
+                 key_lengths=lengths, tag="transposed")
+    # lengths beyond 32 bits, and below zero
+    beyond = torch.tensor([1 << 40, -(1 << 35)], device="cuda")
+    for a, e in zip(nnv.differential_attention(q, k, v, w, key_lengths=beyond)[:2],
+                    nnv.differential_attention(q, k, v, w, key_lengths=torch.tensor([60, 0], device="cuda"))[:2]):
+        assert torch.equal(a, e)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_differential_attention_with_equal_maps_and_weight_zero(dtype):
+    """A weight of zero is the first map alone, one of one on equal maps leaves nothing."""
+    import nnv_amd as nnv
+    g = gen(41)
+    for lq in (1, 90):
+        q, k, v, w = make_differ(g, 2, lq, 300, 4, 2, 64, dtype)
+        one = nnv.differential_attention(q, k, v, torch.zeros_like(w))[0]
+        e, bd = io.differ(q, k, v, torch.zeros_like(w)), io.differ_bounds(q, k, v, torch.zeros_like(w))
+        po.assert_within(one, e[0], bd[0], "one map")
+        q[:, :, 1::2], k[:, :, 1::2] = q[:, :, ::2], k[:, :, ::2]
+        assert float(nnv.differential_attention(q, k, v, torch.ones_like(w))[0].abs().max()) == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_differential_attention_of_far_scores(dtype):
+    """Scores of some hundreds, weights that nothing is left of, a largest score late in the sequence."""
+    g = gen(43)
+    for lq, lk, d in ((1, 3000, 64), (140, 700, 128), (70, 300, 40)):
+        q, k, v, w = make_differ(g, 1, lq, lk, 2, 1, d, dtype)
+        k[:, lk - 3] = q[:, 0, :2] * 4
+        check_differ(q * 8, k, v, w, tag="%d" % lq)
+        check_differ(q, k, v, w, scale=1e-30, tag="flat %d" % lq)
+        check_differ(q, k, v, w, scale=0.0, tag="zero %d" % lq)
+
+
+def test_differential_attention_gradient_against_differences():
+    import nnv_amd as nnv
+    g = gen(51)
+    q, k, v, w = make_differ(g, 2, 19, 37, 4, 2, 24, F32)
+    kw = dict(causal=True, key_mask=torch.rand(2, 37, generator=g, device="cuda") < 0.8)
+    o, lse, second = nnv.differential_attention(q, k, v, w, for_backward=True, **kw)
+    do = rand(g, *o.shape)
+    grads = nnv.differential_attention_backward(do, q, k, v, w, o, lse, second, **kw)
+    bounds = io.differ_grad_bounds(do, q, k, v, w, **kw)
+    h = 1e-5
+    for i, t in enumerate((q, k, v, w)):
+        d = torch.randn(t.shape, generator=g, device="cuda", dtype=torch.float64)
+        loss = lambda s: float((io.differ(*[u.double() + (s * d if i == j else 0) for j, u in enumerate((q, k, v, w))], **kw)[0] * do.double()).sum())  # noqa: E731
+        slope = (loss(h) - loss(-h)) / (2 * h)
+        size = float((grads[i].double().abs() * d.abs()).sum())
+        allowed = float(((bounds[i] + po.U32 * grads[i].double().abs()) * d.abs()).sum()) + 1e-5 * size + 1e-7
+        assert abs(float((grads[i].double() * d).sum()) - slope) <= allowed
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("size", [(2, 1, 9000, 8, 2, 64), (2, 600, 700, 4, 2, 64), (1, 300, 500, 4, 2, 128), (1, 64, 5000, 2, 1, 96)], ids=lambda s: "x".join(map(str, s)))
+def test_differential_attention_gives_the_same_bits_again_anywhere(size, dtype):
+    """Twice, on another stream, and replayed from a graph among eager calls."""
+    import nnv_amd as nnv
+    g = gen(61)
+    q, k, v, w = make_differ(g, *size, dtype)
+    do = rand(g, size[0], size[1], size[3], 2 * size[5], dtype=dtype)
+    lengths = torch.tensor([size[2] - 30] * size[0], device="cuda", dtype=torch.int32)
+
+    def step():
+        o, lse, second = nnv.differential_attention(q, k, v, w, key_lengths=lengths, causal=True, for_backward=True)
+        return [o, lse, second, *nnv.differential_attention_backward(do, q, k, v, w, o, lse, second, key_lengths=lengths, causal=True)]
+
+    eager = step()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        other = step()
+    torch.cuda.current_stream().wait_stream(s)
+    for a, b, e in zip(step(), other, eager):
+        assert torch.equal(a, e) and torch.equal(b, e)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for n in range(3):
+        q.copy_(rand(gen(200 + n), *q.shape, dtype=dtype))
+        lengths.fill_(size[2] - 100 * n)
+        graph.replay()
+        fresh = step()
+        torch.cuda.synchronize()
+        for a, e in zip(held, fresh):
+            assert torch.equal(a, e)

@@ -152,3 +152,82 @@ def test_plain_rotation_by_hand():
     assert list(axes) == [0, 1, 1] and [round(v, 12) for v in f] == [round(100.0 ** (-i / 3), 12) for i in range(3)]
     f, axes = _frequencies((2, 1), 100.0, False)
     assert list(axes) == [0, 0, 1] and list(f) == [1.0, 0.1, 1.0]
+
+
+def test_refusals_of_differential_attention(no_gpu):
+    import nnv_amd as nnv
+    x = torch.zeros(2, 3, 4, 8)
+    refused("on the GPU", nnv.differential_attention, x, x, torch.zeros(2, 3, 2, 16), torch.zeros(2))
+    q, k, v, w = (OnGpu(torch.zeros(*s)) for s in ((2, 5, 8, 16), (2, 7, 4, 16), (2, 7, 2, 32), (4,)))
+    call = no_gpu.differential_attention
+    refused("batch x tokens", call, OnGpu(q[0]), k, v, w)
+    for bad in ((2, 7, 2, 16), (2, 6, 4, 16), (1, 7, 4, 16), (2, 7, 4, 8)):
+        refused("fit together", call, q, OnGpu(torch.zeros(bad)), v, w)
+    for bad in ((2, 7, 2, 16), (2, 7, 4, 32), (2, 8, 2, 32)):
+        refused("fit together", call, q, k, OnGpu(torch.zeros(bad)), w)
+    refused("one type", call, q, OnGpu(k.half()), v, w)
+    refused("float32, bfloat16 or float16", call, *(OnGpu(t.double()) for t in (q, k, v)), w)
+    refused("1 to 128", call, *(OnGpu(torch.zeros(*s)) for s in ((2, 5, 8, 129), (2, 7, 4, 129), (2, 7, 2, 258))), w)
+    refused("two maps", call, OnGpu(q[:, :, :7]), k, v, w)
+    refused("two maps", call, OnGpu(q[:, :, :6]), k, v, w)
+    refused("two maps", call, OnGpu(q[:, :, :0]), k, v, w)
+    refused("one value per head", call, q, k, v, OnGpu(torch.zeros(8)))
+    refused("type of the values", call, *(OnGpu(t.half()) for t in (q, k, v)), OnGpu(w.bfloat16()))
+    refused("float32, bfloat16 or float16", call, q, k, v, OnGpu(w.double()))
+    refused("key_lengths", call, q, k, v, w, OnGpu(torch.zeros(3, dtype=torch.int32)))
+    refused("key_lengths", call, q, k, v, w, OnGpu(torch.zeros(2)))
+    refused("key_mask", call, q, k, v, w, key_mask=OnGpu(torch.zeros(2, 5, dtype=torch.bool)))
+    refused("finite", call, q, k, v, w, scale=math.inf)
+    refused("finite", call, q, k, v, w, scale=math.nan)
+    back, o, lse = no_gpu.differential_attention_backward, OnGpu(torch.zeros(2, 5, 4, 32)), OnGpu(torch.zeros(2, 8, 5))
+    for bad in (None, OnGpu(torch.zeros(2, 5, 4, 16)), OnGpu(o.half())):
+        refused("for_backward", back, o, q, k, v, w, o, lse, bad)
+    refused("for_backward", back, OnGpu(o[:1]), q, k, v, w, o, lse, o)
+    for bad in (OnGpu(torch.zeros(2, 4, 5)), OnGpu(lse.double())):
+        refused("lse", back, o, q, k, v, w, o, bad, o)
+    refused("requires a gradient", call, q, k, v, OnGpu(torch.zeros(4)).requires_grad_())
+
+
+@built
+def test_workspaces_of_differential_attention_and_their_refusals():
+    from nnv_amd import _lib, images
+    lib, n = _lib.load(), C.c_int64()
+
+    def differ(backward=False, **kw):
+        s = dict(type=1, weight_type=1, batch=2, queries=100, keys=200, heads=4, kv_heads=2, head=64, causal=0)
+        s.update(kw)
+        fn = lib.nnvhip_differential_attention_backward_workspace if backward else lib.nnvhip_differential_attention_workspace
+        _lib.check(fn(images._DIFFER.pack(*s.values(), 0.125, *[0] * 28), C.byref(n)))
+        return n.value
+
+    # one token against many keys is split, a large batch is not; D of both maps' rows in the backward pass
+    assert differ(queries=1, keys=60000) > 0
+    assert differ(batch=64, queries=4096, keys=4096, heads=32, kv_heads=32) == 0
+    assert differ(backward=True) >= 4 * 2 * 2 * 4 * 100
+    for kw in (dict(type=3), dict(weight_type=2), dict(head=0), dict(head=129), dict(heads=3), dict(kv_heads=0), dict(keys=-1), dict(queries=1 << 40),
+               dict(batch=1 << 20), dict(heads=32768), dict(keys=1 << 31), dict(queries=1 << 31), dict(batch=65535, queries=1 << 20),
+               dict(batch=65535, heads=32767, kv_heads=32767, queries=(1 << 31) - 256, keys=(1 << 31) - 256)):
+        for backward in (False, True):
+            with pytest.raises((ValueError, _lib.NNVHipError)):
+                differ(backward, **kw)
+    for kw in (dict(batch=64, heads=64, kv_heads=8, queries=1, keys=65536), dict(heads=8, batch=1, queries=1, keys=1 << 26), dict(batch=1, queries=0), dict(keys=0)):
+        for t in range(3):
+            assert differ(type=t, weight_type=t, **kw) >= 0 and differ(True, type=t, weight_type=t, **kw) >= 0
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_plain_differential_attention_is_differentiated_right(causal):
+    torch.manual_seed(4)
+    q, k, v, w = (torch.randn(*s, dtype=torch.float64, requires_grad=True) for s in ((2, 5, 8, 6), (2, 7, 4, 6), (2, 7, 2, 12), (4,)))
+    kw = dict(key_mask=torch.rand(2, 7) < 0.8, key_lengths=torch.tensor([7, 3]), causal=causal)
+    do = torch.randn(2, 5, 4, 12, dtype=torch.float64)
+    o, lse, second = io.differ(q, k, v, w, **kw)
+    o.backward(do)
+    for got, t in zip(io.differ_grad(do, q.detach(), k.detach(), v.detach(), w.detach(), **kw), (q, k, v, w)):
+        assert torch.allclose(got, t.grad, rtol=1e-10, atol=1e-12)
+    # one row by hand: head 3, whose keys are the second key/value head's
+    at = [j for j in range(7) if kw["key_mask"][0, j] and (not causal or j < 7 - 5 + 2 + 1)]
+    p = [torch.softmax(torch.stack([(q[0, 2, 6 + m] * k[0, j, 2 + m]).sum() * 6 ** -0.5 for j in at]), 0) for m in (0, 1)]
+    assert torch.allclose(o[0, 2, 3], (p[0] - w[3] * p[1]) @ v[0, at, 1]) and torch.allclose(second[0, 2, 3], p[1] @ v[0, at, 1])
+    if causal:     # three keys for five queries: the first two see none
+        assert (o[1, :2] == 0).all() and (lse[1, :, :2] == -math.inf).all()
