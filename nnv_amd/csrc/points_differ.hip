@@ -1,5 +1,5 @@
 // Differential attention of points, forward: the kernel for every type, head size and alignment, with f32 products, and the joining of splits.
-#include "points_differ.h"
+#include "points_differ16.h"
 
 #include <algorithm>
 #include <cfloat>
@@ -181,14 +181,18 @@ __global__ __launch_bounds__(256) void differ_join_kernel(const DifferArgs a) {
   if (a.second) store_four((T*)a.second + wide_row_at(a, b, kv, r), d, 2 * a.head, second);
 }
 
-// How a forward call is cut: tiles of rows, and over how many blocks the keys are split (see split_of).
+// How a forward call is cut: few rows for each head's keys (single tokens, 16 bits) or tiles of many, and over how many blocks the keys are split (see
+// split_of).
 struct Cut {
+  bool few;
   int row_tiles, splits;
 };
-Cut cut_of(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys) {
+Cut cut_of(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys, int64_t head, bool by16) {
   Cut c;
-  c.row_tiles = (int)ceil_div(rows, kRows);
-  c.splits = split_of(batch * kv_heads * c.row_tiles, ceil_div(keys, 32), 2, 512, 2, 3);
+  c.few = by16 && rows <= kDifferFewRows;
+  c.row_tiles = (int)ceil_div(rows, c.few ? kDifferFewRows : by16 ? kDiffer16Rows : kRows);
+  const int64_t start = c.few ? 16 : by16 ? 6 : 2, join = c.few ? 16 : by16 ? 12 : 3;
+  c.splits = split_of(batch * kv_heads * c.row_tiles, ceil_div(keys, 32), c.few ? 8 : by16 ? 4 : 2, by16 ? 256 : 512, start, join);
   return c;
 }
 
@@ -217,9 +221,11 @@ int check_sizes(const char* what, const nnvhip_differ_args* d) {
   const int64_t most = (int64_t(1) << 31) - 256, group = d->heads / d->kv_heads, blocks = kMostBlocks / 2;   // of up to 1024 threads, in two maps
   if (d->batch > 65535 || d->heads > 32767 || d->keys > most || d->queries > most / group) NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: too many rows", what);
   if (d->batch * d->kv_heads * ceil_div(d->queries * group, kRows) > blocks) NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: too many rows", what);
-  const Cut c = cut_of(d->batch, d->kv_heads, d->queries * group, d->keys);
-  if (d->batch * d->kv_heads * c.row_tiles * c.splits > blocks || d->batch * d->heads * d->queries >= (int64_t(1) << (c.splits > 8 ? 23 : 25)))
-    NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: too many rows", what);
+  for (const bool by16 : {false, true}) {
+    const Cut c = cut_of(d->batch, d->kv_heads, d->queries * group, d->keys, d->head, by16);
+    if (d->batch * d->kv_heads * c.row_tiles * c.splits > blocks || d->batch * d->heads * d->queries >= (int64_t(1) << (c.splits > 8 ? 23 : 25)))
+      NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: too many rows", what);
+  }
   return NNVHIP_OK;
 }
 
@@ -272,8 +278,10 @@ extern "C" {
 int nnvhip_differential_attention_workspace(const nnvhip_differ_args* d, int64_t* bytes) {
   if (!bytes) NNV_FAIL(NNVHIP_ERR_ARG, "null pointer");
   NNV_TRY(check_sizes("nnvhip_differential_attention_workspace", d));
-  const Cut c = cut_of(d->batch, d->kv_heads, d->queries * (d->heads / d->kv_heads), d->keys);
-  *bytes = c.splits > 1 ? (int64_t)c.splits * d->batch * d->heads * 2 * d->queries * (2 * d->head + 1) * (int64_t)sizeof(float) : 0;
+  int splits = 1;   // whichever kernels the alignment of the tensors lets take the call
+  for (const bool by16 : {false, true})
+    splits = std::max(splits, cut_of(d->batch, d->kv_heads, d->queries * (d->heads / d->kv_heads), d->keys, d->head, by16).splits);
+  *bytes = splits > 1 ? (int64_t)splits * d->batch * d->heads * 2 * d->queries * (2 * d->head + 1) * (int64_t)sizeof(float) : 0;
   return NNVHIP_OK;
 }
 
@@ -286,12 +294,14 @@ int nnvhip_differential_attention(nnvhip_ctx* ctx, const nnvhip_differ_args* d, 
   if (need > workspace_bytes || (need && !workspace))
     NNV_FAIL(NNVHIP_ERR_ARG, "nnvhip_differential_attention: a workspace of %lld bytes is needed", (long long)need);
   if (a.batch == 0 || a.rows == 0) return NNVHIP_OK;
-  const Cut c = cut_of(a.batch, a.kv_heads, a.rows, a.keys);
+  const bool by16 = differ16_takes(a, (int)d->type);
+  const Cut c = cut_of(a.batch, a.kv_heads, a.rows, a.keys, a.head, by16);
   a.row_tiles = c.row_tiles;
   a.splits = c.splits;
   a.part = static_cast<float*>(workspace);
   a.part_lse = c.splits > 1 ? a.part + (int64_t)c.splits * a.batch * a.kv_heads * a.rows * 2 * 2 * a.head : nullptr;
-  DIFFER_BY_TYPE(d->type, launch_differ, a, (hipStream_t)stream);
+  if (by16) launch_differ16(a, (int)d->type, c.few, (hipStream_t)stream);
+  else DIFFER_BY_TYPE(d->type, launch_differ, a, (hipStream_t)stream);
   if (c.splits > 1) DIFFER_BY_TYPE(d->type, launch_join, a, (hipStream_t)stream);
   NNV_HIP_TRY(hipGetLastError());
   return NNVHIP_OK;

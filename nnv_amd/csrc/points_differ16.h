@@ -1,0 +1,138 @@
+// Differential attention of points in 16 bits: tiles in LDS of the two maps' rows and the wide ones, as the bf16 / f16 matrix instructions take them.
+#pragma once
+#include "points_attend16.h"
+#include "points_differ.h"
+
+namespace nnvhip {
+
+// A tile of ROWS rows: those of the first map (DP values each, the head rounded up to 32), of the second one, and the wide ones (W, twice the head
+// rounded up to 16), each as Rows16 has them, one behind the other.  CH: chunks of 16 values of a map's head.
+template <int CH>
+struct Width16 {
+  static constexpr int W = 32 * CH, DP = (16 * CH + 31) / 32 * 32;
+};
+template <typename T, int CH, int ROWS, int WAVES>
+struct TripleLoad {
+  static constexpr int DP = Width16<CH>::DP, W = Width16<CH>::W;
+  static constexpr int MAP = ROWS * DP, WIDE = ROWS * W, VALUES = 2 * MAP + WIDE;   // values in LDS
+  static constexpr int MAP_COUNT = MAP / 512, WIDE_COUNT = WIDE / 512, TOTAL = 2 * MAP_COUNT + WIDE_COUNT;   // transfers of 1024 bytes
+  static constexpr int PLACES = (TOTAL + WAVES - 1) / WAVES, LEAST = TOTAL / WAVES;   // of a wave: at most, at least
+  unsigned off[PLACES];   // bytes behind the address of the place's tile
+  unsigned there;         // bit i: place i holds values of the head (some lane's of every transfer are)
+  __device__ __forceinline__ static int tile_of(int at) { return at < MAP_COUNT ? 0 : at < 2 * MAP_COUNT ? 1 : 2; }
+  __device__ __forceinline__ static int row(int at, int lane) {
+    const int e = (at < 2 * MAP_COUNT ? at % MAP_COUNT : at - 2 * MAP_COUNT) * 64 + lane;
+    return at < 2 * MAP_COUNT ? e / (DP / 8) : e / (W / 8);
+  }
+  __device__ __forceinline__ static int value(int at, int lane) {
+    const int e = (at < 2 * MAP_COUNT ? at % MAP_COUNT : at - 2 * MAP_COUNT) * 64 + lane;
+    return at < 2 * MAP_COUNT ? (e % (DP / 8) ^ Rows16<T, DP>::place(e / (DP / 8))) * 8 : (e % (W / 8) ^ Rows16<T, W>::place(e / (W / 8))) * 8;
+  }
+  __device__ __forceinline__ void init(int wave, int lane, int head, int64_t map_stride, int64_t wide_stride) {
+    there = 0;
+#pragma unroll
+    for (int i = 0; i < PLACES; ++i) {
+      const int at = i * WAVES + wave;
+      off[i] = 0;
+      if (at >= TOTAL) continue;
+      const int v = value(at, lane);
+      off[i] = 2 * (unsigned)(row(at, lane) * (unsigned)(at < 2 * MAP_COUNT ? map_stride : wide_stride) + v);
+      there |= v < (at < 2 * MAP_COUNT ? head : 2 * head) ? 1u << i : 0;
+    }
+  }
+  // tiles whose rows follow one another from p0, p1 (the maps) and pw
+  __device__ __forceinline__ void issue(const T* p0, const T* p1, const T* pw, unsigned lds, int wave) const {
+#pragma unroll
+    for (int i = 0; i < PLACES; ++i) {
+      const int at = i * WAVES + wave, tile = tile_of(at);
+      if ((i + 1) * WAVES > TOTAL && at >= TOTAL) break;
+      if (there >> i & 1) lds_dma16((const double*)(tile == 0 ? p0 : tile == 1 ? p1 : pw), off[i], __builtin_amdgcn_readfirstlane(lds + at * 1024));
+    }
+  }
+  // rows anywhere: map(j, m), wide(j) are pointers to them
+  template <class Map, class Wide>
+  __device__ __forceinline__ void issue_any(Map map, Wide wide, unsigned lds, int wave, int lane) const {
+#pragma unroll
+    for (int i = 0; i < PLACES; ++i) {
+      const int at = i * WAVES + wave, tile = tile_of(at);
+      if ((i + 1) * WAVES > TOTAL && at >= TOTAL) break;
+      if (there >> i & 1) {
+        const int j = row(at, lane);
+        lds_dma16_at((const double*)((tile == 2 ? wide(j) : map(j, tile)) + value(at, lane)), __builtin_amdgcn_readfirstlane(lds + at * 1024));
+      }
+    }
+  }
+  // tile t of rows that follow one another and end after n: rows past the last one repeat it
+  __device__ __forceinline__ void issue_tile(int t, int n, const T* p, int64_t map_stride, int64_t second_map, const T* pw, int64_t wide_stride,
+                                             unsigned lds, int wave, int lane) const {
+    const int64_t first = (int64_t)t * ROWS;
+    if (first + ROWS <= n) {
+      const T* p0 = p + first * map_stride;
+      issue(p0, p0 + second_map, pw + first * wide_stride, lds, wave);
+    } else {
+      issue_any([&](int j, int m) { return p + min(first + j, (int64_t)n - 1) * map_stride + m * second_map; },
+                [&](int j) { return pw + min(first + j, (int64_t)n - 1) * wide_stride; }, lds, wave, lane);
+    }
+  }
+};
+
+// s[k] = the product over N chunks of 16 values of rows first + 32 k .. + 31 of a tile of rows of DP values with a row's operands f(c).  As OverHead: the
+// reads go a batch ahead of the products.
+template <typename T, int DP, int N, int K, int BATCH, class F>
+__device__ __forceinline__ void over_chunks(unsigned tile, int first, F f, float16_t (&s)[K]) {
+  constexpr int ALL = N * K, STEPS = (ALL + BATCH - 1) / BATCH;
+  half8<T> x[2][BATCH], y[2][BATCH];
+  auto read = [&](int n) {
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int at = n * BATCH + i;
+      if (at >= ALL) continue;
+      x[n & 1][i] = rows_operand<T, DP>(tile, first + 32 * (at % K), at / K);
+      y[n & 1][i] = f(at / K);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[k][i] = 0.0f;
+  read(0);
+#pragma unroll
+  for (int n = 0; n < STEPS; ++n) {
+    if (n + 1 < STEPS) read(n + 1);
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int at = n * BATCH + i;
+      if (at < ALL) s[at % K] = Half8<T>::mfma(x[n & 1][i], y[n & 1][i], s[at % K]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// which keys of a tile of 64 (or 32) keys count, in 32 tiles at a time: a wait for one byte of a mask is a wait for all transfers ahead of it
+template <int KEYS>
+struct KeyWords {
+  unsigned words[KEYS / 32];
+  // of tile t, the turn-th that is asked for, step tiles apart, below t1
+  __device__ __forceinline__ uint64_t operator()(const DifferArgs& a, int b, int n, int t, int t1, int turn, int step, int lane) {
+    if (a.mask == nullptr) {
+      const int rest = n - t * KEYS;
+      return rest >= KEYS ? ~0ull : (1ull << rest) - 1;
+    }
+    if (turn % 32 == 0)
+      for (int i = 0; i < 32; ++i) {
+        const uint64_t word = __ballot(t + i * step < t1 && key_counts(a, b, (t + i * step) * KEYS + lane % KEYS, n));
+#pragma unroll
+        for (int k = 0; k < KEYS / 32; ++k) words[k] = lane == i ? (unsigned)(word >> (32 * k)) : words[k];
+      }
+    uint64_t valid = (unsigned)__builtin_amdgcn_readlane(words[0], turn % 32);
+    return valid | (KEYS == 64 ? (uint64_t)(unsigned)__builtin_amdgcn_readlane(words[KEYS / 32 - 1], turn % 32) << 32 : valid << 32);
+  }
+};
+
+bool differ16_takes(const DifferArgs& a, int type);
+constexpr int kDiffer16Rows = 128;   // of a block
+constexpr int kDifferFewRows = 16;   // of a block of the form for few rows
+void launch_differ16(const DifferArgs& a, int type, bool few, hipStream_t st);
+
+}  // namespace nnvhip
