@@ -16,7 +16,8 @@ OBJ = os.path.join(CSRC, "build")
 LIB = os.path.join(HERE, "libnnvhip.so")
 SOURCES = ["ctx.hip", "sets.hip", "weights.hip", "fc_layer.hip", "fc_window.hip", "fc_skinny.hip", "layers.hip", "gemm.hip", "gemm_seg.hip", "conv.hip", "conv_window.hip", "ranges.hip", "relu.hip", "chain.hip", "spec.hip", "elementwise.hip",
            "points_norm.hip", "points_attend.hip", "points_attend16.hip", "points_attend_grad.hip", "points_attend16_grad.hip", "points_clip.hip",
-           "points_group.hip", "points_rotate.hip", "points_differ.hip", "points_differ16.hip", "points_differ_grad.hip"]
+           "points_group.hip", "points_rotate.hip", "points_differ.hip", "points_differ16.hip", "points_differ_grad.hip",
+           "points_differ16_grad.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-fvisibility=hidden",

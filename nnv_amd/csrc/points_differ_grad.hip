@@ -3,7 +3,7 @@
 // As in points_attend_grad.hip two kernels form dq (a wave per 16 queries, both maps) and dk, dv (a wave per 16 keys), each sum in the registers of
 // one wave, in a fixed order, with no atomics.  do v^T, half of what the scores' gradients take, is one product for both maps.  D of both maps and
 // the weights' gradients come first.
-#include "points_differ.h"
+#include "points_differ16.h"
 
 #pragma clang fp contract(fast)
 
@@ -280,12 +280,14 @@ struct GradCut {
   int row_tiles, key_tiles, query_splits, key_splits;
   int64_t delta, part;   // floats of the workspace
 };
-GradCut grad_cut(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys, int64_t head) {
+GradCut grad_cut(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys, int64_t head, bool by16) {
   GradCut c;
-  c.row_tiles = (int)ceil_div(rows, kBlockRows);
-  c.key_tiles = (int)ceil_div(keys, kBlockRows);
-  c.query_splits = split_of(batch * kv_heads * c.row_tiles, ceil_div(keys, 32), 2, head > 96 ? 256 : 512, 2, 3);
-  c.key_splits = split_of(batch * kv_heads * c.key_tiles, ceil_div(rows, 32), 2, head > 64 ? 256 : 512, 2, 3);
+  c.row_tiles = (int)ceil_div(rows, by16 ? differ_grad16_tile(head) : kBlockRows);
+  c.key_tiles = (int)ceil_div(keys, by16 ? differ_grad16_tile(head) : kBlockRows);
+  // blocks that the chip holds at once; what starting a block, and adding splits up, costs in tiles of 32 rows
+  const int64_t start = by16 ? 6 : 2, join = by16 ? 12 : 3;
+  c.query_splits = split_of(batch * kv_heads * c.row_tiles, ceil_div(keys, 32), 2, by16 || head > 96 ? 256 : 512, start, join);
+  c.key_splits = split_of(batch * kv_heads * c.key_tiles, ceil_div(rows, 32), 2, by16 || head > 64 ? 256 : 512, start, join);
   c.delta = round_up(batch * kv_heads * 2 * rows, 64);
   const int64_t q = c.query_splits > 1 ? c.query_splits * batch * kv_heads * 2 * rows * head : 0;
   const int64_t k = c.key_splits > 1 ? 2 * c.key_splits * batch * kv_heads * keys * 2 * head : 0;
@@ -294,7 +296,7 @@ GradCut grad_cut(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys, in
 }
 
 template <typename T, int CH>
-void launch_grad(DifferArgs a, const GradCut& c, hipStream_t st) {
+void launch_grad(DifferArgs a, const GradCut& c, bool by16, hipStream_t st) {
   const int64_t heads = (int64_t)a.batch * a.kv_heads;
   const bool four = a.head % 4 == 0;
   if (a.rows > 0 && heads > 0) {
@@ -302,7 +304,8 @@ void launch_grad(DifferArgs a, const GradCut& c, hipStream_t st) {
     a.row_tiles = c.row_tiles;
     a.splits = c.query_splits;
     const dim3 grid((unsigned)(heads * c.row_tiles * a.splits));
-    if (four) hipLaunchKernelGGL((differ_query_grad_kernel<T, CH, true>), grid, dim3(256), 0, st, a);
+    if (by16) launch_differ_query_grad16(a, st);
+    else if (four) hipLaunchKernelGGL((differ_query_grad_kernel<T, CH, true>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((differ_query_grad_kernel<T, CH, false>), grid, dim3(256), 0, st, a);
     if (a.splits > 1) hipLaunchKernelGGL((differ_sum_rows_kernel<T, 0>), dim3((unsigned)ceil_div(heads * 2 * a.rows, 4)), dim3(256), 0, st, a);
   } else {
@@ -314,7 +317,8 @@ void launch_grad(DifferArgs a, const GradCut& c, hipStream_t st) {
     a.key_tiles = c.key_tiles;
     a.splits = c.key_splits;
     const dim3 grid((unsigned)(heads * c.key_tiles * a.splits));
-    if (four) hipLaunchKernelGGL((differ_key_grad_kernel<T, CH, true>), grid, dim3(256), 0, st, a);
+    if (by16) launch_differ_key_grad16(a, st);
+    else if (four) hipLaunchKernelGGL((differ_key_grad_kernel<T, CH, true>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((differ_key_grad_kernel<T, CH, false>), grid, dim3(256), 0, st, a);
     if (a.splits > 1) {
       const int64_t n = heads * a.keys * 2 * a.head;
@@ -337,11 +341,14 @@ int nnvhip_differential_attention_backward_workspace(const nnvhip_differ_args* d
   const int64_t heads = d->batch * d->kv_heads, blocks = kMostBlocks;
   if (ceil_div(d->batch * d->heads * d->queries, 16) > 2 * blocks) NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_differential_attention_backward: too many rows");
   if (heads * ceil_div(d->keys, kBlockRows) > blocks) NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_differential_attention_backward: too many keys");
-  const GradCut c = grad_cut(d->batch, d->kv_heads, d->queries * (d->heads / d->kv_heads), d->keys, d->head);
-  if (heads * c.row_tiles * c.query_splits > blocks) NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_differential_attention_backward: too many rows");
-  if (heads * c.key_tiles * c.key_splits > blocks || (c.key_splits > 1 && ceil_div(heads * d->keys * 2 * d->head, 256) > blocks))
-    NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_differential_attention_backward: too many keys");
-  *bytes = (c.delta + c.part) * (int64_t)sizeof(float);
+  *bytes = 0;   // whichever kernels the alignment of the tensors lets take the call
+  for (const bool by16 : {false, true}) {
+    const GradCut c = grad_cut(d->batch, d->kv_heads, d->queries * (d->heads / d->kv_heads), d->keys, d->head, by16);
+    if (heads * c.row_tiles * c.query_splits > blocks) NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_differential_attention_backward: too many rows");
+    if (heads * c.key_tiles * c.key_splits > blocks || (c.key_splits > 1 && ceil_div(heads * d->keys * 2 * d->head, 256) > blocks))
+      NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_differential_attention_backward: too many keys");
+    *bytes = std::max(*bytes, (c.delta + c.part) * (int64_t)sizeof(float));
+  }
   return NNVHIP_OK;
 }
 
@@ -353,10 +360,11 @@ int nnvhip_differential_attention_backward(nnvhip_ctx* ctx, const nnvhip_differ_
   NNV_TRY(nnvhip_differential_attention_backward_workspace(d, &need));
   if (need > workspace_bytes || (need && !workspace))
     NNV_FAIL(NNVHIP_ERR_ARG, "nnvhip_differential_attention_backward: a workspace of %lld bytes is needed", (long long)need);
-  const GradCut c = grad_cut(a.batch, a.kv_heads, a.rows, a.keys, a.head);
+  const bool by16 = differ_grad16_takes(a, (int)d->type);
+  const GradCut c = grad_cut(a.batch, a.kv_heads, a.rows, a.keys, a.head, by16);
   a.delta = static_cast<float*>(workspace);
   a.part = a.delta + c.delta;
-  DIFFER_BY_TYPE(d->type, launch_grad, a, c, (hipStream_t)stream);
+  DIFFER_BY_TYPE(d->type, launch_grad, a, c, by16, (hipStream_t)stream);
   NNV_HIP_TRY(hipGetLastError());
   return NNVHIP_OK;
 }
