@@ -76,6 +76,16 @@ __device__ __forceinline__ int next_row_tile(const DifferArgs& a, int t, int siz
   return (int)(((int64_t)g * q + i_min) / size);           // (of this head: i_min is one of its rows)
 }
 
+// The x-th tile of rows that blocks take, of those of a key/value head.  Causal: those that see most keys first, of all heads of the group, so that the
+// short ones fill what is left at the end.
+__device__ __forceinline__ int row_tile_of(const DifferArgs& a, int x) {
+  const int each = a.row_tiles / a.group;   // tiles of a head, about
+  return a.causal && x < each * a.group ? x % a.group * each + each - 1 - x / a.group : x;
+}
+// Blocks of the kernels over keys.  Causal: a tile of early keys is seen by most rows, one of late keys by few, and a block takes one of either (and
+// where their number is odd, one block the middle one alone).
+__host__ __device__ inline int key_blocks_of(int key_tiles, bool causal) { return causal ? (key_tiles + 1) / 2 : key_tiles; }
+
 // low bits of a word of 32 (or 64) keys: those in front of `seen`
 __device__ __forceinline__ uint32_t first_bits(int seen) { return seen >= 32 ? ~0u : seen <= 0 ? 0u : (1u << seen) - 1; }
 

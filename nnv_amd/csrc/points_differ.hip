@@ -25,7 +25,7 @@ __global__ __launch_bounds__(512, 2) void differ_kernel(const DifferArgs a) {
   int64_t at = blockIdx.x;
   const int split = at % a.splits;
   at /= a.splits;
-  const int row_tile = a.row_tiles - 1 - (int)(at % a.row_tiles);   // causal: those that see most keys first
+  const int row_tile = row_tile_of(a, (int)(at % a.row_tiles));
   const int bkv = at / a.row_tiles, b = bkv / a.kv_heads, kv = bkv % a.kv_heads;
   const int n = keys_that_count(a, b);
   const int64_t first = (int64_t)row_tile * kRows, last = min(first + kRows, a.rows) - 1;

@@ -92,7 +92,7 @@ __global__ __launch_bounds__(512, 2) void differ16_kernel(const DifferArgs a) {
   int64_t at = xcd_order(blockIdx.x, gridDim.x);
   const int split = at % a.splits;
   at /= a.splits;
-  const int row_tile = a.row_tiles - 1 - (int)(at % a.row_tiles);   // causal: those that see most keys first
+  const int row_tile = row_tile_of(a, (int)(at % a.row_tiles));
   const int kv = (int)(at / a.row_tiles) / a.batch, b = (int)(at / a.row_tiles + kv) % a.batch, bkv = b * a.kv_heads + kv;
   const int n = keys_that_count(a, b);
   const int64_t first = (int64_t)row_tile * kDiffer16Rows, last = min(first + kDiffer16Rows, a.rows) - 1;

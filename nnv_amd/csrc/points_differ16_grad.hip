@@ -54,6 +54,8 @@ __device__ __forceinline__ float offset_of(float lse) { return lse == -INFINITY 
 // Heads of up to 64: eight waves, two a SIMD; above, four with all of a SIMD's registers.
 template <int CH>
 constexpr int kWaves = CH <= 4 ? 8 : 4;
+template <int CH>
+constexpr int kKeyWaves = CH <= 4 ? 8 : 4;
 
 // dq of 32 rows a wave, both maps: do v^T is formed once.
 template <typename T, int CH>
@@ -65,7 +67,7 @@ __global__ __launch_bounds__(64 * kWaves<CH>, kWaves<CH> / 4) void differ_query_
   int64_t at = xcd_order(blockIdx.x, gridDim.x);
   const int split = at % a.splits;
   at /= a.splits;
-  const int row_tile = a.row_tiles - 1 - (int)(at % a.row_tiles);
+  const int row_tile = row_tile_of(a, (int)(at % a.row_tiles));
   const int b = (int)(at / a.row_tiles) % a.batch, kv = (int)(at / a.row_tiles) / a.batch, bkv = b * a.kv_heads + kv;
   const int n = keys_that_count(a, b);
   const int64_t first = (int64_t)row_tile * ROWS, last = min(first + ROWS, a.rows) - 1;
@@ -146,174 +148,185 @@ __global__ __launch_bounds__(64 * kWaves<CH>, kWaves<CH> / 4) void differ_query_
 
 // dk of both maps, and dv, of 32 keys a wave.  Two waves a SIMD have no room for the values' operands beside the gradients: they lie in LDS.
 template <typename T, int CH>
-__global__ __launch_bounds__(64 * kWaves<CH>, kWaves<CH> / 4) void differ_key_grad16_kernel(const DifferArgs a) {
-  constexpr int ROWS = 64, WAVES = kWaves<CH>, KEYS = 32 * WAVES, DP = Width16<CH>::DP, W = Width16<CH>::W;
-  constexpr bool PARKED = CH == 3 || CH == 4;
+__global__ __launch_bounds__(64 * kKeyWaves<CH>, kKeyWaves<CH> / 4) void differ_key_grad16_kernel(const DifferArgs a) {
+  constexpr int PARKED = CH == 3 || CH == 4 ? 3 * CH : CH == 8 ? 2 * CH : 0;   // operands in LDS: the values', and the second map's keys'
+  constexpr int ROWS = PARKED ? 32 : 64, WAVES = kKeyWaves<CH>, KEYS = 32 * WAVES, DP = Width16<CH>::DP, W = Width16<CH>::W;
   typedef TripleLoad<T, CH, ROWS, WAVES> Load;
-  __shared__ __attribute__((aligned(1024))) T lds[2 * Load::VALUES + (PARKED ? WAVES * 32 * W : 0)];
+  __shared__ __attribute__((aligned(1024))) T lds[2 * Load::VALUES + WAVES * 512 * PARKED];
   __shared__ __attribute__((aligned(16))) float offsets[2][2][ROWS], deltas[2][2][ROWS], weights[2][ROWS];
   __shared__ int sees[2][ROWS];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
   int64_t at = xcd_order(blockIdx.x, gridDim.x);
   const int split = at % a.splits;
   at /= a.splits;
-  const int key_tile = at % a.key_tiles;
-  const int b = (int)(at / a.key_tiles) % a.batch, kv = (int)(at / a.key_tiles) / a.batch, bkv = b * a.kv_heads + kv;
+  const int blocks = key_blocks_of(a.key_tiles, a.causal), block = at % blocks;
+  const int b = (int)(at / blocks) % a.batch, kv = (int)(at / blocks) / a.batch, bkv = b * a.kv_heads + kv;
   const int n = keys_that_count(a, b);
-  const int first = key_tile * KEYS, key = first + wave * 32 + col;
-  const bool here = key < a.keys, counts = key_counts(a, b, key, n);
-  const int i_min = a.causal ? first - (n - a.queries) : 0;   // the first query that sees one of the block's keys
   const unsigned lds_at = lds_addr_of(lds), rows_at = rows_place<T, DP>(lane), wide_at = rows_place<T, W>(lane) + 4 * Load::MAP;
   const unsigned columns_at = columns_place<T, DP>(lane), wide_columns_at = columns_place<T, W>(lane) + 4 * Load::MAP;
   if (DP != a.head || W != 2 * a.head) zero_lds<T, 2 * Load::VALUES, 64 * WAVES>(lds);
-  // where no key of the block counts there is nothing to add up
-  const bool any = __syncthreads_or(counts);
-  const int tiles = any ? (int)((a.rows + ROWS - 1) / ROWS) : 0, per = (tiles + a.splits - 1) / a.splits;
-  const int t0 = split * per, t1 = min(tiles, t0 + per);
-
-  half8<T> kf[2][CH], vf[2 * CH];
-  T* parked = lds + 2 * Load::VALUES + wave * (32 * W) + lane * 8;   // operand c at parked + 512 c; no other wave's
-#pragma unroll
-  for (int m = 0; m < 2; ++m)
-    load_operands<T, CH>(kf[m], (const T*)a.k.p + (counts ? b * a.k.b + (2 * kv + m) * a.k.h + key * a.k.t : 0), h, a.head, counts);
-  load_operands<T, 2 * CH>(vf, (const T*)a.v.p + (counts ? b * a.v.b + kv * a.v.h + key * a.v.t : 0), h, 2 * a.head, counts);
-  if constexpr (PARKED)
-#pragma unroll
-    for (int c = 0; c < 2 * CH; ++c) __builtin_memcpy(parked + 512 * c, &vf[c], 16);
   const float unit = a.scale * kLog2e;
-  float16_t dk[2][DP / 32], dv[CH];
-#pragma unroll
-  for (int m = 0; m < 2; ++m) zero(dk[m]);
-  zero(dv);
   Load load;
   load.init(wave, lane, a.head, a.q.t, a.go.t);
   const T* qp = (const T*)a.q.p + b * a.q.b + 2 * (kv * (int64_t)a.group) * a.q.h;
   const T* gp = (const T*)a.go.p + b * a.go.b + kv * (int64_t)a.group * a.go.h;
-  float next_offset[2] = {}, next_delta[2] = {}, next_weight = 0.0f;
-  int next_sees = 0;
-  auto fetch = [&](int t, int buffer) {
-    const int64_t r0 = (int64_t)t * ROWS;
-    const int g0 = (uint32_t)r0 / (uint32_t)a.queries, i0 = (int)(r0 - (int64_t)g0 * a.queries);
-    const unsigned stage = lds_at + buffer * (2 * Load::VALUES);
-    if (i0 + ROWS <= a.queries) {
-      const T* p = qp + (i0 * a.q.t + 2 * g0 * a.q.h);
-      load.issue(p, p + a.q.h, gp + (i0 * a.go.t + g0 * a.go.h), stage, wave);
-    } else {   // into the next head, or past the last row, which is repeated and made zeros below
-      auto row = [&](int j) { return (uint32_t)min(r0 + j, a.rows - 1); };
-      load.issue_any([&](int j, int m) { const uint32_t g = row(j) / (uint32_t)a.queries; return qp + ((row(j) - g * a.queries) * a.q.t + (2 * g + m) * a.q.h); },
-                     [&](int j) { const uint32_t g = row(j) / (uint32_t)a.queries; return gp + ((row(j) - g * a.queries) * a.go.t + g * a.go.h); }, stage, wave, lane);
-    }
-    if (threadIdx.x < ROWS) {
-      const int64_t r = r0 + threadIdx.x;
-      const bool is = r < a.rows;
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        next_offset[m] = is ? a.lse[lse_at(a, b, kv, r, m)] : -INFINITY;
-        next_delta[m] = is ? a.delta[own_row(a, bkv, r, m)] : 0.0f;
-      }
-      next_weight = is ? weight_of<T>(a, head_of_row(a, kv, r)) : 0.0f;
-      next_sees = is ? seen_by(a, r, n) : 0;
-    }
-  };
-  int buffer = 0, t = next_row_tile(a, t0, ROWS, i_min);
-  if (t < t1) fetch(t, 0);
-  for (; t < t1; buffer ^= 1) {
-    const unsigned stage = lds_at + buffer * (2 * Load::VALUES);
-    if (threadIdx.x < ROWS) {
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        offsets[buffer][m][threadIdx.x] = offset_of(next_offset[m]);
-        deltas[buffer][m][threadIdx.x] = next_delta[m];
-      }
-      weights[buffer][threadIdx.x] = next_weight;
-      sees[buffer][threadIdx.x] = next_sees;
-    }
-    wait_vm_lds<0>();
-    block_barrier();
-    const int64_t r0 = (int64_t)t * ROWS;
-    t = next_row_tile(a, t + 1, ROWS, i_min);
-    if (t < t1) fetch(t, buffer ^ 1);
-    // rows past the last one, and those that see no key: nothing of them may reach a sum
-    const uint64_t valid = __ballot(offsets[buffer][0][lane] < INFINITY);
-    if (valid != ~0ull) {
-      T* tile = lds + buffer * Load::VALUES;
-      zero_rows<T, DP, ROWS>(tile, valid, lane);
-      zero_rows<T, DP, ROWS>(tile + Load::MAP, valid, lane);
-      zero_rows<T, W, ROWS>(tile + 2 * Load::MAP, valid, lane);
-    }
-    const bool masked = a.causal && fewest_seen(a, r0, min(r0 + ROWS, a.rows) - 1, n) < first + wave * 32 + 32;
 #pragma unroll 1
-    for (int k = 0; k < ROWS / 32; ++k) {
-      const unsigned map_k = stage + k * (64 * DP), wide_k = stage + k * (64 * W);
-      const unsigned qs_at = hide(map_k + rows_at), gs_at = hide(wide_k + wide_at), qc_at = hide(map_k + columns_at), gc_at = hide(wide_k + wide_columns_at);
-      float16_t s[2][1], dp[1], both;
+  for (int key_tile = block;; key_tile = a.key_tiles - 1 - block) {
+    const int first = key_tile * KEYS, key = first + wave * 32 + col;
+    const bool here = key < a.keys, counts = key_counts(a, b, key, n);
+    const int i_min = a.causal ? first - (n - a.queries) : 0;   // the first query that sees one of the block's keys
+    // where no key of the block counts there is nothing to add up
+    const bool any = __syncthreads_or(counts);
+    const int tiles = any ? (int)((a.rows + ROWS - 1) / ROWS) : 0, per = (tiles + a.splits - 1) / a.splits;
+    const int t0 = split * per, t1 = min(tiles, t0 + per);
+
+    half8<T> kf[2][CH], vf[2 * CH];
+    T* parked = lds + 2 * Load::VALUES + wave * (512 * PARKED) + lane * 8;   // operand c at parked + 512 c; no other wave's
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        over_chunks<T, DP, CH, 1, CH >= 6 ? 2 : 4>(qs_at + m * (2 * Load::MAP), 0, [&](int c) { return kf[m][c]; }, s[m]);
+    for (int m = 0; m < 2; ++m)
+      load_operands<T, CH>(kf[m], (const T*)a.k.p + (counts ? b * a.k.b + (2 * kv + m) * a.k.h + key * a.k.t : 0), h, a.head, counts);
+    load_operands<T, 2 * CH>(vf, (const T*)a.v.p + (counts ? b * a.v.b + kv * a.v.h + key * a.v.t : 0), h, 2 * a.head, counts);
 #pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4) {
-          float f[4];
-          __builtin_memcpy(f, &offsets[buffer][m][32 * k + 8 * i4 + 4 * h], 16);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[m][0][4 * i4 + i] = exp2_(s[m][0][4 * i4 + i] * unit - f[i]);
-        }
-      }
-      if (masked)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const bool is = key < sees[buffer][32 * k + product_row(i, h)];
-#pragma unroll
-          for (int m = 0; m < 2; ++m) s[m][0][i] = is ? s[m][0][i] : 0.0f;
-        }
-#pragma unroll
-      for (int i4 = 0; i4 < 4; ++i4) {
-        float f[4];
-        __builtin_memcpy(f, &weights[buffer][32 * k + 8 * i4 + 4 * h], 16);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[1][0][4 * i4 + i] *= -f[i];
-          both[4 * i4 + i] = s[0][0][4 * i4 + i] + s[1][0][4 * i4 + i];
-        }
-      }
-      over_rows<T, W>(gc_at, 0, both, dv);
-      over_chunks<T, W, 2 * CH, 1, CH >= 6 ? 2 : 4>(gs_at, 0, [&](int c) {
-        if constexpr (PARKED) {
-          half8<T> x;
-          __builtin_memcpy(&x, parked + 512 * c, 16);
-          return x;
-        } else {
-          return vf[c];
-        }
-      }, dp);
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-#pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4) {
-          float f[4];
-          __builtin_memcpy(f, &deltas[buffer][m][32 * k + 8 * i4 + 4 * h], 16);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[m][0][4 * i4 + i] *= dp[0][4 * i4 + i] - f[i];
-        }
-        over_rows<T, DP>(qc_at + m * (2 * Load::MAP), 0, s[m][0], dk[m]);
-      }
-    }
-  }
-  if (!here) return;
-  if (!counts) {   // what the loop made of a column that does not count reached no other one
+    for (int c = 0; c < PARKED; ++c) __builtin_memcpy(parked + 512 * c, c < 2 * CH ? &vf[c < 2 * CH ? c : 0] : &kf[1][c < 2 * CH ? 0 : c - 2 * CH], 16);
+    auto operand = [&](int c) {
+      half8<T> x;
+      __builtin_memcpy(&x, parked + 512 * c, 16);
+      return x;
+    };
+    float16_t dk[2][DP / 32], dv[CH];
 #pragma unroll
     for (int m = 0; m < 2; ++m) zero(dk[m]);
     zero(dv);
-  }
-  const int64_t dense = ((b * (int64_t)a.keys + key) * a.kv_heads + kv) * 2 * a.head;
-  if (a.splits > 1) {
-    const int64_t all = (int64_t)a.batch * a.keys * a.kv_heads * 2 * a.head;
+    float next_offset[2] = {}, next_delta[2] = {}, next_weight = 0.0f;
+    int next_sees = 0;
+    auto fetch = [&](int t, int buffer) {
+      const int64_t r0 = (int64_t)t * ROWS;
+      const int g0 = (uint32_t)r0 / (uint32_t)a.queries, i0 = (int)(r0 - (int64_t)g0 * a.queries);
+      const unsigned stage = lds_at + buffer * (2 * Load::VALUES);
+      if (i0 + ROWS <= a.queries) {
+        const T* p = qp + (i0 * a.q.t + 2 * g0 * a.q.h);
+        load.issue(p, p + a.q.h, gp + (i0 * a.go.t + g0 * a.go.h), stage, wave);
+      } else {   // into the next head, or past the last row, which is repeated and made zeros below
+        auto row = [&](int j) { return (uint32_t)min(r0 + j, a.rows - 1); };
+        load.issue_any([&](int j, int m) { const uint32_t g = row(j) / (uint32_t)a.queries; return qp + ((row(j) - g * a.queries) * a.q.t + (2 * g + m) * a.q.h); },
+                       [&](int j) { const uint32_t g = row(j) / (uint32_t)a.queries; return gp + ((row(j) - g * a.queries) * a.go.t + g * a.go.h); }, stage, wave, lane);
+      }
+      if (threadIdx.x < ROWS) {
+        const int64_t r = r0 + threadIdx.x;
+        const bool is = r < a.rows;
 #pragma unroll
-    for (int m = 0; m < 2; ++m) store_result(a.part + split * all + dense + m * a.head, dk[m], a.scale, h, a.head);
-    store_result(a.part + (a.splits + split) * all + dense, dv, 1.0f, h, 2 * a.head);
-  } else {
+        for (int m = 0; m < 2; ++m) {
+          next_offset[m] = is ? a.lse[lse_at(a, b, kv, r, m)] : -INFINITY;
+          next_delta[m] = is ? a.delta[own_row(a, bkv, r, m)] : 0.0f;
+        }
+        next_weight = is ? weight_of<T>(a, head_of_row(a, kv, r)) : 0.0f;
+        next_sees = is ? seen_by(a, r, n) : 0;
+      }
+    };
+    int buffer = 0, t = next_row_tile(a, t0, ROWS, i_min);
+    if (t < t1) fetch(t, 0);
+    for (; t < t1; buffer ^= 1) {
+      const unsigned stage = lds_at + buffer * (2 * Load::VALUES);
+      if (threadIdx.x < ROWS) {
 #pragma unroll
-    for (int m = 0; m < 2; ++m) store_result((T*)a.dk + dense + m * a.head, dk[m], a.scale, h, a.head);
-    store_result((T*)a.dv + dense, dv, 1.0f, h, 2 * a.head);
+        for (int m = 0; m < 2; ++m) {
+          offsets[buffer][m][threadIdx.x] = offset_of(next_offset[m]);
+          deltas[buffer][m][threadIdx.x] = next_delta[m];
+        }
+        weights[buffer][threadIdx.x] = next_weight;
+        sees[buffer][threadIdx.x] = next_sees;
+      }
+      wait_vm_lds<0>();
+      block_barrier();
+      const int64_t r0 = (int64_t)t * ROWS;
+      t = next_row_tile(a, t + 1, ROWS, i_min);
+      if (t < t1) fetch(t, buffer ^ 1);
+      // rows past the last one, and those that see no key: nothing of them may reach a sum
+      const uint64_t valid = __ballot(offsets[buffer][0][lane % ROWS] < INFINITY);
+      if (valid != ~0ull) {
+        T* tile = lds + buffer * Load::VALUES;
+        zero_rows<T, DP, ROWS>(tile, valid, lane);
+        zero_rows<T, DP, ROWS>(tile + Load::MAP, valid, lane);
+        zero_rows<T, W, ROWS>(tile + 2 * Load::MAP, valid, lane);
+      }
+      const bool masked = a.causal && fewest_seen(a, r0, min(r0 + ROWS, a.rows) - 1, n) < first + wave * 32 + 32;
+#pragma unroll 1
+      for (int k = 0; k < ROWS / 32; ++k) {
+        const unsigned map_k = stage + k * (64 * DP), wide_k = stage + k * (64 * W);
+        const unsigned qs_at = hide(map_k + rows_at), gs_at = hide(wide_k + wide_at), qc_at = hide(map_k + columns_at), gc_at = hide(wide_k + wide_columns_at);
+        float16_t s[2][1], dp[1];   // (do v^T first: its operands' registers are then free)
+        over_chunks<T, W, 2 * CH, 1, 2>(gs_at, 0, [&](int c) {
+          if constexpr (PARKED > 0) return operand(c);
+          else return vf[c];
+        }, dp);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          over_chunks<T, DP, CH, 1, 2>(qs_at + m * (2 * Load::MAP), 0, [&](int c) {
+            if (PARKED > 2 * CH && m) return operand(2 * CH + c);
+            else return kf[m][c];
+          }, s[m]);
+#pragma unroll
+          for (int i4 = 0; i4 < 4; ++i4) {
+            float f[4];
+            __builtin_memcpy(f, &offsets[buffer][m][32 * k + 8 * i4 + 4 * h], 16);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[m][0][4 * i4 + i] = exp2_(s[m][0][4 * i4 + i] * unit - f[i]);
+          }
+        }
+        if (masked)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const bool is = key < sees[buffer][32 * k + product_row(i, h)];
+#pragma unroll
+            for (int m = 0; m < 2; ++m) s[m][0][i] = is ? s[m][0][i] : 0.0f;
+          }
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4) {
+          float f[4];
+          __builtin_memcpy(f, &weights[buffer][32 * k + 8 * i4 + 4 * h], 16);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[1][0][4 * i4 + i] *= -f[i];
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          half8<T> both;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) both[i] = (T)(s[0][0][8 * c + i] + s[1][0][8 * c + i]);
+#pragma unroll
+          for (int d = 0; d < CH; ++d) dv[d] = Half8<T>::mfma(columns_operand<T, W>(gc_at, 16 * c, d), both, dv[d]);
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+#pragma unroll
+          for (int i4 = 0; i4 < 4; ++i4) {
+            float f[4];
+            __builtin_memcpy(f, &deltas[buffer][m][32 * k + 8 * i4 + 4 * h], 16);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[m][0][4 * i4 + i] *= dp[0][4 * i4 + i] - f[i];
+          }
+          over_rows<T, DP>(qc_at + m * (2 * Load::MAP), 0, s[m][0], dk[m]);
+        }
+      }
+    }
+    if (here) {
+      if (!counts) {   // what the loop made of a column that does not count reached no other one
+#pragma unroll
+        for (int m = 0; m < 2; ++m) zero(dk[m]);
+        zero(dv);
+      }
+      const int64_t dense = ((b * (int64_t)a.keys + key) * a.kv_heads + kv) * 2 * a.head;
+      if (a.splits > 1) {
+        const int64_t all = (int64_t)a.batch * a.keys * a.kv_heads * 2 * a.head;
+#pragma unroll
+        for (int m = 0; m < 2; ++m) store_result(a.part + split * all + dense + m * a.head, dk[m], a.scale, h, a.head);
+        store_result(a.part + (a.splits + split) * all + dense, dv, 1.0f, h, 2 * a.head);
+      } else {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) store_result((T*)a.dk + dense + m * a.head, dk[m], a.scale, h, a.head);
+        store_result((T*)a.dv + dense, dv, 1.0f, h, 2 * a.head);
+      }
+    }
+    if (key_tile != block || blocks == a.key_tiles || a.key_tiles - 1 - block == block) break;
   }
 }
 
@@ -324,13 +337,14 @@ void launch_query(const DifferArgs& a, hipStream_t st) {
 }
 template <typename T, int CH>
 void launch_key(const DifferArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((differ_key_grad16_kernel<T, CH>), dim3((unsigned)((int64_t)a.batch * a.kv_heads * a.key_tiles * a.splits)), dim3(64 * kWaves<CH>), 0,
+  hipLaunchKernelGGL((differ_key_grad16_kernel<T, CH>), dim3((unsigned)((int64_t)a.batch * a.kv_heads * key_blocks_of(a.key_tiles, a.causal) * a.splits)), dim3(64 * kKeyWaves<CH>), 0,
                      st, a);
 }
 
 }  // namespace
 
 int differ_grad16_tile(int64_t head) { return head <= 64 ? 256 : 128; }
+int differ_key_grad16_tile(int64_t head) { return head <= 64 ? 256 : 128; }
 bool differ_grad16_takes(const DifferArgs& a, int type) {
   return type == NNVHIP_TYPE_BF16 && by_pieces(a.q, a.head) && by_pieces(a.k, a.head) && by_pieces(a.v, a.head) && by_pieces(a.go, a.head);
 }

@@ -72,7 +72,7 @@ __global__ __launch_bounds__(256, CH <= 6 ? 2 : 1) void differ_query_grad_kernel
   int64_t at = blockIdx.x;
   const int split = at % a.splits;
   at /= a.splits;
-  const int row_tile = a.row_tiles - 1 - (int)(at % a.row_tiles);
+  const int row_tile = row_tile_of(a, (int)(at % a.row_tiles));
   const int bkv = at / a.row_tiles, b = bkv / a.kv_heads, kv = bkv % a.kv_heads;
   const int n = keys_that_count(a, b);
   const int64_t first = (int64_t)row_tile * kBlockRows, last = min(first + kBlockRows, a.rows) - 1;
@@ -145,104 +145,109 @@ __global__ __launch_bounds__(256, CH <= 4 ? 2 : 1) void differ_key_grad_kernel(c
   int64_t at = blockIdx.x;
   const int split = at % a.splits;
   at /= a.splits;
-  const int key_tile = at % a.key_tiles;
-  const int bkv = at / a.key_tiles, b = bkv / a.kv_heads, kv = bkv % a.kv_heads;
+  const int blocks = key_blocks_of(a.key_tiles, a.causal), block = at % blocks;
+  const int bkv = at / blocks, b = bkv / a.kv_heads, kv = bkv % a.kv_heads;
   const int n = keys_that_count(a, b);
-  const int first = key_tile * kBlockRows, key = first + wave * 16 + col;
-  const bool here = key < a.keys, counts = key_counts(a, b, key, n), idle = first + wave * 16 >= n;
-  const int i_min = a.causal ? first - (n - a.queries) : 0;   // the first query that sees one of the block's keys
-  int t0 = 0, t1 = 0;
-  if (first < n) {   // else no key of the block counts: its gradients are zero
-    const int tiles = (int)((a.rows + R - 1) / R), per = (tiles + a.splits - 1) / a.splits;
-    t0 = split * per;
-    t1 = min(tiles, t0 + per);
-  }
-  const int64_t row = here && counts ? key : 0;
-  float kf[2][CH][4], vf[2 * CH][4];
-#pragma unroll
-  for (int m = 0; m < 2; ++m)
-    f32_operands<T, CH>((const T*)a.k.p + (counts ? b * a.k.b + (2 * kv + m) * a.k.h + row * a.k.t : 0), q4, a.head, counts, kf[m]);
-  f32_operands<T, 2 * CH>((const T*)a.v.p + (counts ? b * a.v.b + kv * a.v.h + row * a.v.t : 0), q4, 2 * a.head, counts, vf);
   const float unit = a.scale * kLog2e;
-  float4_t dk[2][CH], dv[2 * CH];
-#pragma unroll
-  for (int m = 0; m < 2; ++m) f32_zero(dk[m]);
-  f32_zero(dv);
-  TripleAhead<T, CH, 256, FOUR> next;
-  float next_offset[2] = {INFINITY, INFINITY}, next_delta[2] = {0, 0}, next_weight = 0;
-  int next_seen = 0;
-  auto fetch = [&](int t) {
-    auto row = [&](int j) { return min((int64_t)t * R + j, a.rows - 1); };
-    next.load([&](int j, int which) { return (const T*)a.q.p + map_row_at(a.q, a, b, kv, row(j), which); },
-              [&](int j) { return (const T*)a.go.p + row_at(a.go, a, b, kv, row(j)); }, a.head, threadIdx.x);
-    // (every wave of its own: which rows take part decides what the tile's rows are)
-    const int64_t r = (int64_t)t * R + (lane & 31);
-    const bool is = r < a.rows;
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      next_offset[m] = offset_of(is ? a.lse[lse_at(a, b, kv, r, m)] : -INFINITY);
-      next_delta[m] = is ? a.delta[own_row(a, bkv, r, m)] : 0.0f;
+#pragma unroll 1
+  for (int key_tile = block;; key_tile = a.key_tiles - 1 - block) {
+    const int first = key_tile * kBlockRows, key = first + wave * 16 + col;
+    const bool here = key < a.keys, counts = key_counts(a, b, key, n), idle = first + wave * 16 >= n;
+    const int i_min = a.causal ? first - (n - a.queries) : 0;   // the first query that sees one of the block's keys
+    int t0 = 0, t1 = 0;
+    if (first < n) {   // else no key of the block counts: its gradients are zero
+      const int tiles = (int)((a.rows + R - 1) / R), per = (tiles + a.splits - 1) / a.splits;
+      t0 = split * per;
+      t1 = min(tiles, t0 + per);
     }
-    next_weight = is ? weight_of<T>(a, head_of_row(a, kv, r)) : 0.0f;
-    next_seen = is ? seen_by(a, r, n) : 0;
-  };
-  int t = next_row_tile(a, t0, R, i_min);
-  if (t < t1) fetch(t);
-  while (t < t1) {
-    __syncthreads();
-    // a row without keys counts for nothing: what it holds must not reach the sums
-    next.store(tile, (uint32_t)__ballot(next_offset[0] < INFINITY), a.head, threadIdx.x);
-    if (threadIdx.x < R) {
+    const int64_t row = here && counts ? key : 0;
+    float kf[2][CH][4], vf[2 * CH][4];
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        offsets[m][threadIdx.x] = next_offset[m];
-        deltas[m][threadIdx.x] = next_delta[m];
-      }
-      weights[threadIdx.x] = next_weight;
-      seen_by_row[threadIdx.x] = __builtin_bit_cast(float, next_seen);
-    }
-    __syncthreads();
-    t = next_row_tile(a, t + 1, R, i_min);
-    if (t < t1) fetch(t);
-    if (idle) continue;
-    float4_t s[2][2], dp[2], both[2];
-    bool sees[2][4];
-#pragma unroll
-    for (int m = 0; m < 2; ++m) f32_over_head<CH, CH>(tile + col * LD + 4 * q4 + m * 16 * CH, kf[m], s[m]);
-    f32_over_head<CH, 2 * CH>(tile + col * LD + 4 * q4 + 32 * CH, vf, dp);
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = 16 * k + 4 * q4 + i;
-        sees[k][i] = key < __builtin_bit_cast(int, seen_by_row[j]);
-        const float w = weights[j];
-#pragma unroll
-        for (int m = 0; m < 2; ++m) s[m][k][i] = sees[k][i] ? exp2_(s[m][k][i] * unit - offsets[m][j]) : 0.0f;
-        both[k][i] = s[0][k][i] - w * s[1][k][i];
-        s[0][k][i] *= sees[k][i] ? dp[k][i] - deltas[0][j] : 0.0f;
-        s[1][k][i] *= sees[k][i] ? -w * (dp[k][i] - deltas[1][j]) : 0.0f;
-      }
-    f32_over_rows<CH, 2 * CH>(tile + 4 * q4 * LD + col + 32 * CH, both, dv);
-#pragma unroll
-    for (int m = 0; m < 2; ++m) f32_over_rows<CH, CH>(tile + 4 * q4 * LD + col + m * 16 * CH, s[m], dk[m]);
-  }
-  if (!here) return;
-  if (!counts) {
+    for (int m = 0; m < 2; ++m)
+      f32_operands<T, CH>((const T*)a.k.p + (counts ? b * a.k.b + (2 * kv + m) * a.k.h + row * a.k.t : 0), q4, a.head, counts, kf[m]);
+    f32_operands<T, 2 * CH>((const T*)a.v.p + (counts ? b * a.v.b + kv * a.v.h + row * a.v.t : 0), q4, 2 * a.head, counts, vf);
+    float4_t dk[2][CH], dv[2 * CH];
 #pragma unroll
     for (int m = 0; m < 2; ++m) f32_zero(dk[m]);
     f32_zero(dv);
-  }
-  const int64_t dense = ((b * (int64_t)a.keys + key) * a.kv_heads + kv) * 2 * a.head;   // of dv; of dk's first map as well
-  if (a.splits > 1) {
-    const int64_t all = (int64_t)a.batch * a.keys * a.kv_heads * 2 * a.head;
+    TripleAhead<T, CH, 256, FOUR> next;
+    float next_offset[2] = {INFINITY, INFINITY}, next_delta[2] = {0, 0}, next_weight = 0;
+    int next_seen = 0;
+    auto fetch = [&](int t) {
+      auto row = [&](int j) { return min((int64_t)t * R + j, a.rows - 1); };
+      next.load([&](int j, int which) { return (const T*)a.q.p + map_row_at(a.q, a, b, kv, row(j), which); },
+                [&](int j) { return (const T*)a.go.p + row_at(a.go, a, b, kv, row(j)); }, a.head, threadIdx.x);
+      // (every wave of its own: which rows take part decides what the tile's rows are)
+      const int64_t r = (int64_t)t * R + (lane & 31);
+      const bool is = r < a.rows;
 #pragma unroll
-    for (int m = 0; m < 2; ++m) f32_store(a.part + split * all + dense + m * a.head, dk[m], a.scale, q4, a.head);
-    f32_store(a.part + (a.splits + split) * all + dense, dv, 1.0f, q4, 2 * a.head);
-  } else {
+      for (int m = 0; m < 2; ++m) {
+        next_offset[m] = offset_of(is ? a.lse[lse_at(a, b, kv, r, m)] : -INFINITY);
+        next_delta[m] = is ? a.delta[own_row(a, bkv, r, m)] : 0.0f;
+      }
+      next_weight = is ? weight_of<T>(a, head_of_row(a, kv, r)) : 0.0f;
+      next_seen = is ? seen_by(a, r, n) : 0;
+    };
+    int t = next_row_tile(a, t0, R, i_min);
+    if (t < t1) fetch(t);
+    while (t < t1) {
+      __syncthreads();
+      // a row without keys counts for nothing: what it holds must not reach the sums
+      next.store(tile, (uint32_t)__ballot(next_offset[0] < INFINITY), a.head, threadIdx.x);
+      if (threadIdx.x < R) {
 #pragma unroll
-    for (int m = 0; m < 2; ++m) f32_store((T*)a.dk + dense + m * a.head, dk[m], a.scale, q4, a.head);
-    f32_store((T*)a.dv + dense, dv, 1.0f, q4, 2 * a.head);
+        for (int m = 0; m < 2; ++m) {
+          offsets[m][threadIdx.x] = next_offset[m];
+          deltas[m][threadIdx.x] = next_delta[m];
+        }
+        weights[threadIdx.x] = next_weight;
+        seen_by_row[threadIdx.x] = __builtin_bit_cast(float, next_seen);
+      }
+      __syncthreads();
+      t = next_row_tile(a, t + 1, R, i_min);
+      if (t < t1) fetch(t);
+      if (idle) continue;
+      float4_t s[2][2], dp[2], both[2];
+      bool sees[2][4];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) f32_over_head<CH, CH>(tile + col * LD + 4 * q4 + m * 16 * CH, kf[m], s[m]);
+      f32_over_head<CH, 2 * CH>(tile + col * LD + 4 * q4 + 32 * CH, vf, dp);
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = 16 * k + 4 * q4 + i;
+          sees[k][i] = key < __builtin_bit_cast(int, seen_by_row[j]);
+          const float w = weights[j];
+#pragma unroll
+          for (int m = 0; m < 2; ++m) s[m][k][i] = sees[k][i] ? exp2_(s[m][k][i] * unit - offsets[m][j]) : 0.0f;
+          both[k][i] = s[0][k][i] - w * s[1][k][i];
+          s[0][k][i] *= sees[k][i] ? dp[k][i] - deltas[0][j] : 0.0f;
+          s[1][k][i] *= sees[k][i] ? -w * (dp[k][i] - deltas[1][j]) : 0.0f;
+        }
+      f32_over_rows<CH, 2 * CH>(tile + 4 * q4 * LD + col + 32 * CH, both, dv);
+#pragma unroll
+      for (int m = 0; m < 2; ++m) f32_over_rows<CH, CH>(tile + 4 * q4 * LD + col + m * 16 * CH, s[m], dk[m]);
+    }
+    if (here) {
+      if (!counts) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) f32_zero(dk[m]);
+        f32_zero(dv);
+      }
+      const int64_t dense = ((b * (int64_t)a.keys + key) * a.kv_heads + kv) * 2 * a.head;   // of dv; of dk's first map as well
+      if (a.splits > 1) {
+        const int64_t all = (int64_t)a.batch * a.keys * a.kv_heads * 2 * a.head;
+#pragma unroll
+        for (int m = 0; m < 2; ++m) f32_store(a.part + split * all + dense + m * a.head, dk[m], a.scale, q4, a.head);
+        f32_store(a.part + (a.splits + split) * all + dense, dv, 1.0f, q4, 2 * a.head);
+      } else {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) f32_store((T*)a.dk + dense + m * a.head, dk[m], a.scale, q4, a.head);
+        f32_store((T*)a.dv + dense, dv, 1.0f, q4, 2 * a.head);
+      }
+    }
+    if (key_tile != block || blocks == a.key_tiles || a.key_tiles - 1 - block == block) break;
   }
 }
 
@@ -277,17 +282,18 @@ __global__ __launch_bounds__(256) void differ_sum_rows_kernel(const DifferArgs a
 }
 
 struct GradCut {
-  int row_tiles, key_tiles, query_splits, key_splits;
+  int row_tiles, key_tiles, key_blocks, query_splits, key_splits;
   int64_t delta, part;   // floats of the workspace
 };
-GradCut grad_cut(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys, int64_t head, bool by16) {
+GradCut grad_cut(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys, int64_t head, bool causal, bool by16) {
   GradCut c;
   c.row_tiles = (int)ceil_div(rows, by16 ? differ_grad16_tile(head) : kBlockRows);
-  c.key_tiles = (int)ceil_div(keys, by16 ? differ_grad16_tile(head) : kBlockRows);
+  c.key_tiles = (int)ceil_div(keys, by16 ? differ_key_grad16_tile(head) : kBlockRows);
+  c.key_blocks = key_blocks_of(c.key_tiles, causal);
   // blocks that the chip holds at once; what starting a block, and adding splits up, costs in tiles of 32 rows
   const int64_t start = by16 ? 6 : 2, join = by16 ? 12 : 3;
   c.query_splits = split_of(batch * kv_heads * c.row_tiles, ceil_div(keys, 32), 2, by16 || head > 96 ? 256 : 512, start, join);
-  c.key_splits = split_of(batch * kv_heads * c.key_tiles, ceil_div(rows, 32), 2, by16 || head > 64 ? 256 : 512, start, join);
+  c.key_splits = split_of(batch * kv_heads * c.key_blocks, ceil_div(rows, 32), 2, by16 || head > 64 ? 256 : 512, start, join);
   c.delta = round_up(batch * kv_heads * 2 * rows, 64);
   const int64_t q = c.query_splits > 1 ? c.query_splits * batch * kv_heads * 2 * rows * head : 0;
   const int64_t k = c.key_splits > 1 ? 2 * c.key_splits * batch * kv_heads * keys * 2 * head : 0;
@@ -316,7 +322,7 @@ void launch_grad(DifferArgs a, const GradCut& c, bool by16, hipStream_t st) {
     a.batch = (int)(heads / a.kv_heads);
     a.key_tiles = c.key_tiles;
     a.splits = c.key_splits;
-    const dim3 grid((unsigned)(heads * c.key_tiles * a.splits));
+    const dim3 grid((unsigned)(heads * c.key_blocks * a.splits));
     if (by16) launch_differ_key_grad16(a, st);
     else if (four) hipLaunchKernelGGL((differ_key_grad_kernel<T, CH, true>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((differ_key_grad_kernel<T, CH, false>), grid, dim3(256), 0, st, a);
@@ -343,9 +349,9 @@ int nnvhip_differential_attention_backward_workspace(const nnvhip_differ_args* d
   if (heads * ceil_div(d->keys, kBlockRows) > blocks) NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_differential_attention_backward: too many keys");
   *bytes = 0;   // whichever kernels the alignment of the tensors lets take the call
   for (const bool by16 : {false, true}) {
-    const GradCut c = grad_cut(d->batch, d->kv_heads, d->queries * (d->heads / d->kv_heads), d->keys, d->head, by16);
+    const GradCut c = grad_cut(d->batch, d->kv_heads, d->queries * (d->heads / d->kv_heads), d->keys, d->head, d->causal != 0, by16);
     if (heads * c.row_tiles * c.query_splits > blocks) NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_differential_attention_backward: too many rows");
-    if (heads * c.key_tiles * c.key_splits > blocks || (c.key_splits > 1 && ceil_div(heads * d->keys * 2 * d->head, 256) > blocks))
+    if (heads * c.key_blocks * c.key_splits > blocks || (c.key_splits > 1 && ceil_div(heads * d->keys * 2 * d->head, 256) > blocks))
       NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_differential_attention_backward: too many keys");
     *bytes = std::max(*bytes, (c.delta + c.part) * (int64_t)sizeof(float));
   }
@@ -361,7 +367,7 @@ int nnvhip_differential_attention_backward(nnvhip_ctx* ctx, const nnvhip_differ_
   if (need > workspace_bytes || (need && !workspace))
     NNV_FAIL(NNVHIP_ERR_ARG, "nnvhip_differential_attention_backward: a workspace of %lld bytes is needed", (long long)need);
   const bool by16 = differ_grad16_takes(a, (int)d->type);
-  const GradCut c = grad_cut(a.batch, a.kv_heads, a.rows, a.keys, a.head, by16);
+  const GradCut c = grad_cut(a.batch, a.kv_heads, a.rows, a.keys, a.head, a.causal, by16);
   a.delta = static_cast<float*>(workspace);
   a.part = a.delta + c.delta;
   DIFFER_BY_TYPE(d->type, launch_grad, a, c, by16, (hipStream_t)stream);
