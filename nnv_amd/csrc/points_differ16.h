@@ -17,8 +17,18 @@ struct TripleLoad {
   static constexpr int MAP = ROWS * DP, WIDE = ROWS * W, VALUES = 2 * MAP + WIDE;   // values in LDS
   static constexpr int MAP_COUNT = MAP / 512, WIDE_COUNT = WIDE / 512, TOTAL = 2 * MAP_COUNT + WIDE_COUNT;   // transfers of 1024 bytes
   static constexpr int PLACES = (TOTAL + WAVES - 1) / WAVES, LEAST = TOTAL / WAVES;   // of a wave: at most, at least
-  unsigned off[PLACES];   // bytes behind the address of the place's tile
-  unsigned there;         // bit i: place i holds values of the head (some lane's of every transfer are)
+  // A wave's places of one kind whose rows are a multiple of 16 apart have their pieces in the same order: an offset for each that is not, and the rest goes
+  // into the scalar address (32 places of a single wave would take 32 registers).
+  static constexpr bool EVEN = MAP_COUNT % WAVES == 0 && WIDE_COUNT % WAVES == 0 && WAVES * 512 % DP == 0 && WAVES * 512 % W == 0;
+  static constexpr int MAP_STEP = WAVES * 512 / DP, WIDE_STEP = WAVES * 512 / W;   // rows from one place to the next (EVEN)
+  static constexpr int MAPS = MAP_COUNT / WAVES, WIDES = WIDE_COUNT / WAVES;       // places of a kind of tile
+  static constexpr int least(int x, int y) { return x < y ? x : y; }
+  static constexpr int MAP_OFFS = least(MAPS, 16 / least(16, MAP_STEP)), WIDE_OFFS = least(WIDES, 16 / least(16, WIDE_STEP));
+  static_assert(!EVEN || ((MAP_STEP & (MAP_STEP - 1)) == 0 && (WIDE_STEP & (WIDE_STEP - 1)) == 0), "steps of rows are powers of two");
+  static constexpr int OFFS = EVEN ? MAP_OFFS + WIDE_OFFS : PLACES;
+  unsigned off[OFFS];     // bytes behind the address of the place's tile
+  __device__ __forceinline__ static constexpr int place_of(int i) { return i < MAP_OFFS ? i : 2 * MAPS + i - MAP_OFFS; }   // which an offset is of (EVEN)
+  unsigned there;         // bit i: the place of offset i holds values of the head (some lane's of every transfer are)
   __device__ __forceinline__ static int tile_of(int at) { return at < MAP_COUNT ? 0 : at < 2 * MAP_COUNT ? 1 : 2; }
   __device__ __forceinline__ static int row(int at, int lane) {
     const int e = (at < 2 * MAP_COUNT ? at % MAP_COUNT : at - 2 * MAP_COUNT) * 64 + lane;
@@ -31,8 +41,8 @@ struct TripleLoad {
   __device__ __forceinline__ void init(int wave, int lane, int head, int64_t map_stride, int64_t wide_stride) {
     there = 0;
 #pragma unroll
-    for (int i = 0; i < PLACES; ++i) {
-      const int at = i * WAVES + wave;
+    for (int i = 0; i < OFFS; ++i) {
+      const int at = (EVEN ? place_of(i) : i) * WAVES + wave;
       off[i] = 0;
       if (at >= TOTAL) continue;
       const int v = value(at, lane);
@@ -41,12 +51,18 @@ struct TripleLoad {
     }
   }
   // tiles whose rows follow one another from p0, p1 (the maps) and pw
-  __device__ __forceinline__ void issue(const T* p0, const T* p1, const T* pw, unsigned lds, int wave) const {
+  __device__ __forceinline__ void issue(const T* p0, const T* p1, const T* pw, int64_t map_stride, int64_t wide_stride, unsigned lds, int wave) const {
 #pragma unroll
     for (int i = 0; i < PLACES; ++i) {
       const int at = i * WAVES + wave, tile = tile_of(at);
+      if constexpr (EVEN) {
+        const int j = i < MAPS ? i : i < 2 * MAPS ? i - MAPS : i - 2 * MAPS, each = i < 2 * MAPS ? MAP_OFFS : WIDE_OFFS, o = (i < 2 * MAPS ? 0 : MAP_OFFS) + j % each;
+        const T* p = (i < MAPS ? p0 : i < 2 * MAPS ? p1 : pw) + j / each * each * (i < 2 * MAPS ? MAP_STEP * map_stride : WIDE_STEP * wide_stride);
+        if (there >> o & 1) lds_dma16((const double*)p, off[o], __builtin_amdgcn_readfirstlane(lds + at * 1024));
+        continue;
+      }
       if ((i + 1) * WAVES > TOTAL && at >= TOTAL) break;
-      if (there >> i & 1) lds_dma16((const double*)(tile == 0 ? p0 : tile == 1 ? p1 : pw), off[i], __builtin_amdgcn_readfirstlane(lds + at * 1024));
+      if (there >> i & 1) lds_dma16((const double*)(tile == 0 ? p0 : tile == 1 ? p1 : pw), off[i % OFFS], __builtin_amdgcn_readfirstlane(lds + at * 1024));
     }
   }
   // rows anywhere: map(j, m), wide(j) are pointers to them
@@ -56,7 +72,8 @@ struct TripleLoad {
     for (int i = 0; i < PLACES; ++i) {
       const int at = i * WAVES + wave, tile = tile_of(at);
       if ((i + 1) * WAVES > TOTAL && at >= TOTAL) break;
-      if (there >> i & 1) {
+      const int o = !EVEN ? i : i < MAPS ? i % MAP_OFFS : i < 2 * MAPS ? (i - MAPS) % MAP_OFFS : MAP_OFFS + (i - 2 * MAPS) % WIDE_OFFS;
+      if (there >> o & 1) {
         const int j = row(at, lane);
         lds_dma16_at((const double*)((tile == 2 ? wide(j) : map(j, tile)) + value(at, lane)), __builtin_amdgcn_readfirstlane(lds + at * 1024));
       }
@@ -68,7 +85,7 @@ struct TripleLoad {
     const int64_t first = (int64_t)t * ROWS;
     if (first + ROWS <= n) {
       const T* p0 = p + first * map_stride;
-      issue(p0, p0 + second_map, pw + first * wide_stride, lds, wave);
+      issue(p0, p0 + second_map, pw + first * wide_stride, map_stride, wide_stride, lds, wave);
     } else {
       issue_any([&](int j, int m) { return p + min(first + j, (int64_t)n - 1) * map_stride + m * second_map; },
                 [&](int j) { return pw + min(first + j, (int64_t)n - 1) * wide_stride; }, lds, wave, lane);
@@ -105,6 +122,20 @@ __device__ __forceinline__ void over_chunks(unsigned tile, int first, F f, float
       const int at = n * BATCH + i;
       if (at < ALL) s[at % K] = Half8<T>::mfma(x[n & 1][i], y[n & 1][i], s[at % K]);
     }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// body(c, d, x): the columns 32 d .. of rows first + 16 c .. + 15 of a tile, read one ahead of what uses them
+template <typename T, int DP, int C, class Body>
+__device__ __forceinline__ void over_columns(unsigned tile, int first, Body body) {
+  constexpr int D = DP / 32;
+  half8<T> x[2];
+  x[0] = columns_operand<T, DP>(tile, first, 0);
+#pragma unroll
+  for (int n = 0; n < C * D; ++n) {
+    if (n + 1 < C * D) x[(n + 1) & 1] = columns_operand<T, DP>(tile, first + (n + 1) / D * 16, (n + 1) % D);
+    body(n / D, n % D, x[n & 1]);
     __builtin_amdgcn_sched_barrier(0);
   }
 }

@@ -145,7 +145,7 @@ __global__ __launch_bounds__(512, 2) void differ16_kernel(const DifferArgs a) {
     if (valid != ~0ull) zero_rows<T, W, KEYS>(vs, valid, lane);
 
     float16_t s[2];
-    over_chunks<T, DP, CH, 2, 4>(ks_at, 0, [&](int c) { return qf[c]; }, s);
+    over_chunks<T, DP, CH, 2, CH == 8 ? 2 : 4>(ks_at, 0, [&](int c) { return qf[c]; }, s);
     if (valid != ~0ull || (t + 1) * KEYS > seen_by_all) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) mask_scores(s[k], ((uint32_t)(valid >> (32 * k)) & first_bits(seen - t * KEYS - 32 * k)) >> (4 * h));
@@ -292,20 +292,19 @@ __global__ __launch_bounds__(64 * differ_groups<CH>(), 1) void differ16_few_kern
           acc[d][i] *= fade;
           second[d][i] *= fade;
         }
+    half8<T> p[2], rest[2];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const half8<T> p = round8<T>(s[0], 8 * c);
+      p[c] = round8<T>(s[0], 8 * c);
       float16_t left;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) left[i] = s[0][8 * c + i] - (float)p[i];
-      const half8<T> rest = round8<T>(left, 0);
-#pragma unroll
-      for (int d = 0; d < CH; ++d) {
-        const half8<T> v = columns_operand<T, W>(vs_at, 16 * c, d);
-        acc[d] = Half8<T>::mfma(v, p, acc[d]);
-        second[d] = Half8<T>::mfma(v, rest, second[d]);
-      }
+      for (int i = 0; i < 8; ++i) left[i] = s[0][8 * c + i] - (float)p[c][i];
+      rest[c] = round8<T>(left, 0);
     }
+    over_columns<T, W, 2>(vs_at, 0, [&](int c, int d, const half8<T>& v) {
+      acc[d] = Half8<T>::mfma(v, p[c], acc[d]);
+      second[d] = Half8<T>::mfma(v, rest[c], second[d]);
+    });
   }
   total = sum_of_halves(total);
   __syncthreads();

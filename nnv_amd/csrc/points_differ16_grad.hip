@@ -205,7 +205,7 @@ __global__ __launch_bounds__(64 * kKeyWaves<CH>, kKeyWaves<CH> / 4) void differ_
       const unsigned stage = lds_at + buffer * (2 * Load::VALUES);
       if (i0 + ROWS <= a.queries) {
         const T* p = qp + (i0 * a.q.t + 2 * g0 * a.q.h);
-        load.issue(p, p + a.q.h, gp + (i0 * a.go.t + g0 * a.go.h), stage, wave);
+        load.issue(p, p + a.q.h, gp + (i0 * a.go.t + g0 * a.go.h), a.q.t, a.go.t, stage, wave);
       } else {   // into the next head, or past the last row, which is repeated and made zeros below
         auto row = [&](int j) { return (uint32_t)min(r0 + j, a.rows - 1); };
         load.issue_any([&](int j, int m) { const uint32_t g = row(j) / (uint32_t)a.queries; return qp + ((row(j) - g * a.queries) * a.q.t + (2 * g + m) * a.q.h); },
