@@ -21,7 +21,14 @@ struct DifferArgs : AttendArgs {   // (its lse is the caller's; scale, masks and
   int wide_weights, causal;
   void* second;                    // dense, or null
   void* dweights;
+  float* info;                     // [sequence, key/value head][kInfos][info_rows]: see RowInfo
+  int info_rows;                   // rows, rounded up to kInfoRows
 };
+
+// What the gradients of keys need of a row, as arrays over the rows of a key/value head that a tile's transfer takes as they lie: the exponents' offsets of both
+// maps (infinite for rows without keys, and behind the last one), D of both, the weight with its sign turned, and how many keys the row sees.
+enum RowInfo { kOffset0, kOffset1, kDelta0, kDelta1, kWeight, kSees, kInfos };
+constexpr int kInfoRows = 64;
 
 __device__ __forceinline__ int64_t map_row_at(const TokenView& t, const DifferArgs& a, int b, int kv, int64_t r, int map) {
   const int64_t g = (uint32_t)r / (uint32_t)a.queries, i = r - g * a.queries;
@@ -90,6 +97,9 @@ __host__ __device__ inline int key_blocks_of(int key_tiles, bool causal) { retur
 __device__ __forceinline__ uint32_t first_bits(int seen) { return seen >= 32 ? ~0u : seen <= 0 ? 0u : (1u << seen) - 1; }
 
 int differ_args(const char* what, const nnvhip_differ_args* d, bool backward, DifferArgs* a);
+
+// lse of a row as the exponent's offset in powers of two; a row without keys takes no part (exp2(s - inf) = 0)
+__device__ __forceinline__ float offset_of(float lse) { return lse == -INFINITY ? INFINITY : lse * kLog2e; }
 
 // Which template takes a head size: chunks of 16 values of a map's head, of 32 of v's.
 #define DIFFER_BY_HEAD(CALL, T, ...)                \

@@ -11,7 +11,7 @@ template <int CH>
 struct Width16 {
   static constexpr int W = 32 * CH, DP = (16 * CH + 31) / 32 * 32;
 };
-template <typename T, int CH, int ROWS, int WAVES>
+template <typename T, int CH, int ROWS, int WAVES, bool SAVE = true>   // SAVE: registers, see EVEN
 struct TripleLoad {
   static constexpr int DP = Width16<CH>::DP, W = Width16<CH>::W;
   static constexpr int MAP = ROWS * DP, WIDE = ROWS * W, VALUES = 2 * MAP + WIDE;   // values in LDS
@@ -19,11 +19,11 @@ struct TripleLoad {
   static constexpr int PLACES = (TOTAL + WAVES - 1) / WAVES, LEAST = TOTAL / WAVES;   // of a wave: at most, at least
   // A wave's places of one kind whose rows are a multiple of 16 apart have their pieces in the same order: an offset for each that is not, and the rest goes
   // into the scalar address (32 places of a single wave would take 32 registers).
-  static constexpr bool EVEN = MAP_COUNT % WAVES == 0 && WIDE_COUNT % WAVES == 0 && WAVES * 512 % DP == 0 && WAVES * 512 % W == 0;
+  static constexpr bool EVEN = SAVE && MAP_COUNT % WAVES == 0 && WIDE_COUNT % WAVES == 0 && WAVES * 512 % DP == 0 && WAVES * 512 % W == 0;
   static constexpr int MAP_STEP = WAVES * 512 / DP, WIDE_STEP = WAVES * 512 / W;   // rows from one place to the next (EVEN)
   static constexpr int MAPS = MAP_COUNT / WAVES, WIDES = WIDE_COUNT / WAVES;       // places of a kind of tile
   static constexpr int least(int x, int y) { return x < y ? x : y; }
-  static constexpr int MAP_OFFS = least(MAPS, 16 / least(16, MAP_STEP)), WIDE_OFFS = least(WIDES, 16 / least(16, WIDE_STEP));
+  static constexpr int MAP_OFFS = EVEN ? least(MAPS, 16 / least(16, MAP_STEP)) : 1, WIDE_OFFS = EVEN ? least(WIDES, 16 / least(16, WIDE_STEP)) : 1;
   static_assert(!EVEN || ((MAP_STEP & (MAP_STEP - 1)) == 0 && (WIDE_STEP & (WIDE_STEP - 1)) == 0), "steps of rows are powers of two");
   static constexpr int OFFS = EVEN ? MAP_OFFS + WIDE_OFFS : PLACES;
   unsigned off[OFFS];     // bytes behind the address of the place's tile
@@ -63,6 +63,19 @@ struct TripleLoad {
       }
       if ((i + 1) * WAVES > TOTAL && at >= TOTAL) break;
       if (there >> i & 1) lds_dma16((const double*)(tile == 0 ? p0 : tile == 1 ? p1 : pw), off[i % OFFS], __builtin_amdgcn_readfirstlane(lds + at * 1024));
+    }
+  }
+  // The rows from j0 on and in front of j1, of the same; the others' places are left as they are.  (A scalar address for each run of rows instead of a vector's
+  // for each row.  The number of transfers varies: for those who wait for all of them.)
+  __device__ __forceinline__ void issue_rows(int j0, int j1, const T* p0, const T* p1, const T* pw, unsigned lds, int wave, int lane) const {
+    static_assert(!EVEN, "an offset for every place");
+#pragma unroll
+    for (int i = 0; i < PLACES; ++i) {
+      const int at = i * WAVES + wave, tile = tile_of(at);
+      if ((i + 1) * WAVES > TOTAL && at >= TOTAL) break;
+      const int j = row(at, lane);
+      if ((there >> i & 1) && j >= j0 && j < j1)
+        lds_dma16((const double*)(tile == 0 ? p0 : tile == 1 ? p1 : pw), off[i % OFFS], __builtin_amdgcn_readfirstlane(lds + at * 1024));
     }
   }
   // rows anywhere: map(j, m), wide(j) are pointers to them

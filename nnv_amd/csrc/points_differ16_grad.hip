@@ -49,7 +49,6 @@ __device__ __forceinline__ void zero_lds(T* lds) {
   for (int e = threadIdx.x; e < VALUES / 8; e += THREADS) __builtin_memcpy(lds + e * 8, &none, 16);
   __syncthreads();
 }
-__device__ __forceinline__ float offset_of(float lse) { return lse == -INFINITY ? INFINITY : lse * kLog2e; }
 
 // Heads of up to 64: eight waves, two a SIMD; above, four with all of a SIMD's registers.
 template <int CH>
@@ -151,10 +150,9 @@ template <typename T, int CH>
 __global__ __launch_bounds__(64 * kKeyWaves<CH>, kKeyWaves<CH> / 4) void differ_key_grad16_kernel(const DifferArgs a) {
   constexpr int PARKED = CH == 3 || CH == 4 ? 3 * CH : CH == 8 ? 2 * CH : 0;   // operands in LDS: the values', and the second map's keys'
   constexpr int ROWS = PARKED ? 32 : 64, WAVES = kKeyWaves<CH>, KEYS = 32 * WAVES, DP = Width16<CH>::DP, W = Width16<CH>::W;
-  typedef TripleLoad<T, CH, ROWS, WAVES> Load;
+  typedef TripleLoad<T, CH, ROWS, WAVES, false> Load;
   __shared__ __attribute__((aligned(1024))) T lds[2 * Load::VALUES + WAVES * 512 * PARKED];
-  __shared__ __attribute__((aligned(16))) float offsets[2][2][ROWS], deltas[2][2][ROWS], weights[2][ROWS];
-  __shared__ int sees[2][ROWS];
+  __shared__ __attribute__((aligned(1024))) float info[2][kInfos * ROWS < 256 ? 256 : 512];   // [buffer][RowInfo * ROWS + row]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
   int64_t at = xcd_order(blockIdx.x, gridDim.x);
   const int split = at % a.splits;
@@ -197,52 +195,46 @@ __global__ __launch_bounds__(64 * kKeyWaves<CH>, kKeyWaves<CH> / 4) void differ_
 #pragma unroll
     for (int m = 0; m < 2; ++m) zero(dk[m]);
     zero(dv);
-    float next_offset[2] = {}, next_delta[2] = {}, next_weight = 0.0f;
-    int next_sees = 0;
     auto fetch = [&](int t, int buffer) {
       const int64_t r0 = (int64_t)t * ROWS;
-      const int g0 = (uint32_t)r0 / (uint32_t)a.queries, i0 = (int)(r0 - (int64_t)g0 * a.queries);
+      int g = (int)((uint32_t)r0 / (uint32_t)a.queries), i = (int)(r0 - (int64_t)g * a.queries);
       const unsigned stage = lds_at + buffer * (2 * Load::VALUES);
-      if (i0 + ROWS <= a.queries) {
-        const T* p = qp + (i0 * a.q.t + 2 * g0 * a.q.h);
-        load.issue(p, p + a.q.h, gp + (i0 * a.go.t + g0 * a.go.h), a.q.t, a.go.t, stage, wave);
-      } else {   // into the next head, or past the last row, which is repeated and made zeros below
-        auto row = [&](int j) { return (uint32_t)min(r0 + j, a.rows - 1); };
-        load.issue_any([&](int j, int m) { const uint32_t g = row(j) / (uint32_t)a.queries; return qp + ((row(j) - g * a.queries) * a.q.t + (2 * g + m) * a.q.h); },
-                       [&](int j) { const uint32_t g = row(j) / (uint32_t)a.queries; return gp + ((row(j) - g * a.queries) * a.go.t + g * a.go.h); }, stage, wave, lane);
-      }
-      if (threadIdx.x < ROWS) {
-        const int64_t r = r0 + threadIdx.x;
-        const bool is = r < a.rows;
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          next_offset[m] = is ? a.lse[lse_at(a, b, kv, r, m)] : -INFINITY;
-          next_delta[m] = is ? a.delta[own_row(a, bkv, r, m)] : 0.0f;
+      const T *q = qp + (i * a.q.t + 2 * g * a.q.h), *go = gp + (i * a.go.t + g * a.go.h);
+      if (i + ROWS <= a.queries) {
+        load.issue(q, q + a.q.h, go, a.q.t, a.go.t, stage, wave);
+      } else {   // head after head; rows past the last one stay what they are, and are made zeros below
+        for (int j = 0; j < ROWS && g < a.group; ++g) {
+          const int end = min(ROWS, j + a.queries - i);
+          load.issue_rows(j, end, q, q + a.q.h, go, stage, wave, lane);
+          // (the next head's row 0 is at row `end` of the tile)
+          q = qp + (2 * (g + 1) * a.q.h - end * a.q.t);
+          go = gp + ((g + 1) * a.go.h - end * a.go.t);
+          j = end;
+          i = 0;
         }
-        next_weight = is ? weight_of<T>(a, head_of_row(a, kv, r)) : 0.0f;
-        next_sees = is ? seen_by(a, r, n) : 0;
+      }
+      if (wave == 0) {   // kInfos * ROWS floats, four a lane and transfer
+        const float* from = a.info + bkv * (int64_t)kInfos * a.info_rows + r0;
+#pragma unroll
+        for (int k = 0; k < kInfos * ROWS / 256 + (kInfos * ROWS % 256 != 0); ++k) {
+          const int array = (k * 64 + lane) / (ROWS / 4);
+          if (array < kInfos)
+            lds_dma16((const double*)from, 4 * ((unsigned)array * a.info_rows + (k * 64 + lane) % (ROWS / 4) * 4),
+                      __builtin_amdgcn_readfirstlane(lds_addr_of(info[buffer]) + k * 1024));
+        }
       }
     };
     int buffer = 0, t = next_row_tile(a, t0, ROWS, i_min);
     if (t < t1) fetch(t, 0);
     for (; t < t1; buffer ^= 1) {
       const unsigned stage = lds_at + buffer * (2 * Load::VALUES);
-      if (threadIdx.x < ROWS) {
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          offsets[buffer][m][threadIdx.x] = offset_of(next_offset[m]);
-          deltas[buffer][m][threadIdx.x] = next_delta[m];
-        }
-        weights[buffer][threadIdx.x] = next_weight;
-        sees[buffer][threadIdx.x] = next_sees;
-      }
       wait_vm_lds<0>();
       block_barrier();
       const int64_t r0 = (int64_t)t * ROWS;
       t = next_row_tile(a, t + 1, ROWS, i_min);
       if (t < t1) fetch(t, buffer ^ 1);
       // rows past the last one, and those that see no key: nothing of them may reach a sum
-      const uint64_t valid = __ballot(offsets[buffer][0][lane % ROWS] < INFINITY);
+      const uint64_t valid = __ballot(info[buffer][kOffset0 * ROWS + lane % ROWS] < INFINITY);
       if (valid != ~0ull) {
         T* tile = lds + buffer * Load::VALUES;
         zero_rows<T, DP, ROWS>(tile, valid, lane);
@@ -260,7 +252,7 @@ __global__ __launch_bounds__(64 * kKeyWaves<CH>, kKeyWaves<CH> / 4) void differ_
           else return vf[c];
         }, dp);
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
+        for (int m = 1; m >= 0; --m) {   // (the one whose keys are read from LDS first)
           over_chunks<T, DP, CH, 1, 2>(qs_at + m * (2 * Load::MAP), 0, [&](int c) {
             if (PARKED > 2 * CH && m) return operand(2 * CH + c);
             else return kf[m][c];
@@ -268,7 +260,7 @@ __global__ __launch_bounds__(64 * kKeyWaves<CH>, kKeyWaves<CH> / 4) void differ_
 #pragma unroll
           for (int i4 = 0; i4 < 4; ++i4) {
             float f[4];
-            __builtin_memcpy(f, &offsets[buffer][m][32 * k + 8 * i4 + 4 * h], 16);
+            __builtin_memcpy(f, &info[buffer][(kOffset0 + m) * ROWS + 32 * k + 8 * i4 + 4 * h], 16);
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[m][0][4 * i4 + i] = exp2_(s[m][0][4 * i4 + i] * unit - f[i]);
           }
@@ -276,16 +268,16 @@ __global__ __launch_bounds__(64 * kKeyWaves<CH>, kKeyWaves<CH> / 4) void differ_
         if (masked)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const bool is = key < sees[buffer][32 * k + product_row(i, h)];
+            const bool is = key < __builtin_bit_cast(int, info[buffer][kSees * ROWS + 32 * k + product_row(i, h)]);
 #pragma unroll
             for (int m = 0; m < 2; ++m) s[m][0][i] = is ? s[m][0][i] : 0.0f;
           }
 #pragma unroll
         for (int i4 = 0; i4 < 4; ++i4) {
           float f[4];
-          __builtin_memcpy(f, &weights[buffer][32 * k + 8 * i4 + 4 * h], 16);
+          __builtin_memcpy(f, &info[buffer][kWeight * ROWS + 32 * k + 8 * i4 + 4 * h], 16);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[1][0][4 * i4 + i] *= -f[i];
+          for (int i = 0; i < 4; ++i) s[1][0][4 * i4 + i] *= f[i];
         }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -300,7 +292,7 @@ __global__ __launch_bounds__(64 * kKeyWaves<CH>, kKeyWaves<CH> / 4) void differ_
 #pragma unroll
           for (int i4 = 0; i4 < 4; ++i4) {
             float f[4];
-            __builtin_memcpy(f, &deltas[buffer][m][32 * k + 8 * i4 + 4 * h], 16);
+            __builtin_memcpy(f, &info[buffer][(kDelta0 + m) * ROWS + 32 * k + 8 * i4 + 4 * h], 16);
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[m][0][4 * i4 + i] *= dp[0][4 * i4 + i] - f[i];
           }
@@ -346,7 +338,7 @@ void launch_key(const DifferArgs& a, hipStream_t st) {
 int differ_grad16_tile(int64_t head) { return head <= 64 ? 256 : 128; }
 int differ_key_grad16_tile(int64_t head) { return head <= 64 ? 256 : 128; }
 bool differ_grad16_takes(const DifferArgs& a, int type) {
-  return type == NNVHIP_TYPE_BF16 && by_pieces(a.q, a.head) && by_pieces(a.k, a.head) && by_pieces(a.v, a.head) && by_pieces(a.go, a.head);
+  return type == NNVHIP_TYPE_BF16 && by_pieces(a.q, a.head) && by_pieces(a.k, a.head) && by_pieces(a.v, a.head) && by_pieces(a.go, a.head) && a.rows < (1 << 27);   // (kInfos * rows floats within 32 bits)
 }
 void launch_differ_query_grad16(const DifferArgs& a, hipStream_t st) { DIFFER_BY_HEAD(launch_query, bf16_t, a, st); }
 void launch_differ_key_grad16(const DifferArgs& a, hipStream_t st) { DIFFER_BY_HEAD(launch_key, bf16_t, a, st); }

@@ -15,10 +15,15 @@ constexpr int kBlockRows = 64;   // rows, or keys, of a block
 // D_1 = rowsum(do second), D_0 = rowsum(do o) + w D_1: 16 lanes a row.
 template <typename T, int>
 __global__ __launch_bounds__(256) void differ_delta_kernel(const DifferArgs a) {
-  const int64_t flat = (int64_t)blockIdx.x * 16 + threadIdx.x / 16, all = (int64_t)a.batch * a.kv_heads * a.rows;
-  const bool here = flat < all;
-  const int64_t f = here ? flat : 0, bkv = f / a.rows, r = f % a.rows;
+  const int64_t flat = (int64_t)blockIdx.x * 16 + threadIdx.x / 16, per = a.info ? a.info_rows : a.rows, all = (int64_t)a.batch * a.kv_heads * per;
+  if (flat >= all) return;   // (the lanes of a row go together)
+  const int64_t bkv = flat / per, r = flat % per;
   const int b = (int)(bkv / a.kv_heads), kv = (int)(bkv % a.kv_heads), size = 2 * a.head;
+  float* info = a.info ? a.info + bkv * kInfos * per + r : nullptr;
+  if (r >= a.rows) {
+    if (threadIdx.x % 16 < kInfos) info[threadIdx.x % 16 * per] = threadIdx.x % 16 <= kOffset1 ? INFINITY : 0.0f;
+    return;
+  }
   const T* o = (const T*)a.out + wide_row_at(a, b, kv, r);
   const T* second = (const T*)a.second + wide_row_at(a, b, kv, r);
   const T* g = (const T*)a.go.p + row_at(a.go, a, b, kv, r);
@@ -35,10 +40,16 @@ __global__ __launch_bounds__(256) void differ_delta_kernel(const DifferArgs a) {
   for (int k = 8; k > 0; k >>= 1)
 #pragma unroll
     for (int m = 0; m < 2; ++m) s[m] += __shfl_xor(s[m], k, 64);
-  if (!here || threadIdx.x % 16) return;
-  const bool takes_part = a.lse[lse_at(a, b, kv, r, 0)] != -INFINITY;   // (both maps see the same keys)
-  a.delta[own_row(a, bkv, r, 0)] = takes_part ? s[0] + weight_of<T>(a, head_of_row(a, kv, r)) * s[1] : 0.0f;
-  a.delta[own_row(a, bkv, r, 1)] = takes_part ? s[1] : 0.0f;
+  if (threadIdx.x % 16) return;
+  const float lse[2] = {a.lse[lse_at(a, b, kv, r, 0)], a.lse[lse_at(a, b, kv, r, 1)]};
+  const bool takes_part = lse[0] != -INFINITY;   // (both maps see the same keys)
+  const float w = weight_of<T>(a, head_of_row(a, kv, r)), d0 = takes_part ? s[0] + w * s[1] : 0.0f, d1 = takes_part ? s[1] : 0.0f;
+  a.delta[own_row(a, bkv, r, 0)] = d0;
+  a.delta[own_row(a, bkv, r, 1)] = d1;
+  if (!info) return;
+  const float values[kInfos] = {offset_of(lse[0]), offset_of(lse[1]), d0, d1, -w, __builtin_bit_cast(float, seen_by(a, r, keys_that_count(a, b)))};
+#pragma unroll
+  for (int k = 0; k < kInfos; ++k) info[k * per] = values[k];
 }
 
 // dw of a head: a block adds its rows' D_1, in f64.
@@ -60,9 +71,6 @@ __global__ __launch_bounds__(256) void differ_weights_kernel(const DifferArgs a)
   if (a.wide_weights) ((float*)a.dweights)[head] = all;
   else ((T*)a.dweights)[head] = from_f<T>(all);
 }
-
-// lse of a row as the exponent's offset in powers of two; a row without keys takes no part (exp2(s - inf) = 0)
-__device__ __forceinline__ float offset_of(float lse) { return lse == -INFINITY ? INFINITY : lse * kLog2e; }
 
 template <typename T, int CH, bool FOUR>
 __global__ __launch_bounds__(256, CH <= 6 ? 2 : 1) void differ_query_grad_kernel(const DifferArgs a) {
@@ -283,7 +291,7 @@ __global__ __launch_bounds__(256) void differ_sum_rows_kernel(const DifferArgs a
 
 struct GradCut {
   int row_tiles, key_tiles, key_blocks, query_splits, key_splits;
-  int64_t delta, part;   // floats of the workspace
+  int64_t delta, info, part;   // floats of the workspace
 };
 GradCut grad_cut(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys, int64_t head, bool causal, bool by16) {
   GradCut c;
@@ -295,6 +303,7 @@ GradCut grad_cut(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys, in
   c.query_splits = split_of(batch * kv_heads * c.row_tiles, ceil_div(keys, 32), 2, by16 || head > 96 ? 256 : 512, start, join);
   c.key_splits = split_of(batch * kv_heads * c.key_blocks, ceil_div(rows, 32), 2, by16 || head > 64 ? 256 : 512, start, join);
   c.delta = round_up(batch * kv_heads * 2 * rows, 64);
+  c.info = by16 ? batch * kv_heads * kInfos * round_up(rows, kInfoRows) : 0;
   const int64_t q = c.query_splits > 1 ? c.query_splits * batch * kv_heads * 2 * rows * head : 0;
   const int64_t k = c.key_splits > 1 ? 2 * c.key_splits * batch * kv_heads * keys * 2 * head : 0;
   c.part = std::max(q, k);
@@ -306,7 +315,7 @@ void launch_grad(DifferArgs a, const GradCut& c, bool by16, hipStream_t st) {
   const int64_t heads = (int64_t)a.batch * a.kv_heads;
   const bool four = a.head % 4 == 0;
   if (a.rows > 0 && heads > 0) {
-    hipLaunchKernelGGL((differ_delta_kernel<T, 0>), dim3((unsigned)ceil_div(heads * a.rows, 16)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((differ_delta_kernel<T, 0>), dim3((unsigned)ceil_div(heads * (a.info ? a.info_rows : a.rows), 16)), dim3(256), 0, st, a);
     a.row_tiles = c.row_tiles;
     a.splits = c.query_splits;
     const dim3 grid((unsigned)(heads * c.row_tiles * a.splits));
@@ -345,7 +354,7 @@ int nnvhip_differential_attention_backward_workspace(const nnvhip_differ_args* d
   NNV_TRY(nnvhip_differential_attention_workspace(d, &forward));   // checks the sizes
   if (!bytes) NNV_FAIL(NNVHIP_ERR_ARG, "null pointer");
   const int64_t heads = d->batch * d->kv_heads, blocks = kMostBlocks;
-  if (ceil_div(d->batch * d->heads * d->queries, 16) > 2 * blocks) NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_differential_attention_backward: too many rows");
+  if (ceil_div(heads * round_up(d->queries * (d->heads / d->kv_heads), kInfoRows), 16) > 2 * blocks) NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_differential_attention_backward: too many rows");
   if (heads * ceil_div(d->keys, kBlockRows) > blocks) NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_differential_attention_backward: too many keys");
   *bytes = 0;   // whichever kernels the alignment of the tensors lets take the call
   for (const bool by16 : {false, true}) {
@@ -353,7 +362,7 @@ int nnvhip_differential_attention_backward_workspace(const nnvhip_differ_args* d
     if (heads * c.row_tiles * c.query_splits > blocks) NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_differential_attention_backward: too many rows");
     if (heads * c.key_blocks * c.key_splits > blocks || (c.key_splits > 1 && ceil_div(heads * d->keys * 2 * d->head, 256) > blocks))
       NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_differential_attention_backward: too many keys");
-    *bytes = std::max(*bytes, (c.delta + c.part) * (int64_t)sizeof(float));
+    *bytes = std::max(*bytes, (c.delta + c.info + c.part) * (int64_t)sizeof(float));
   }
   return NNVHIP_OK;
 }
@@ -369,7 +378,9 @@ int nnvhip_differential_attention_backward(nnvhip_ctx* ctx, const nnvhip_differ_
   const bool by16 = differ_grad16_takes(a, (int)d->type);
   const GradCut c = grad_cut(a.batch, a.kv_heads, a.rows, a.keys, a.head, a.causal, by16);
   a.delta = static_cast<float*>(workspace);
-  a.part = a.delta + c.delta;
+  a.info = c.info ? a.delta + c.delta : nullptr;
+  a.info_rows = (int)round_up(a.rows, kInfoRows);
+  a.part = a.delta + c.delta + c.info;
   DIFFER_BY_TYPE(d->type, launch_grad, a, c, by16, (hipStream_t)stream);
   NNV_HIP_TRY(hipGetLastError());
   return NNVHIP_OK;
