@@ -93,6 +93,35 @@ __device__ __forceinline__ int row_tile_of(const DifferArgs& a, int x) {
 // where their number is odd, one block the middle one alone).
 __host__ __device__ inline int key_blocks_of(int key_tiles, bool causal) { return causal ? (key_tiles + 1) / 2 : key_tiles; }
 
+// Where a block works: (sequence, key/value head) and one of `each` blocks of it.  Blocks are dealt to the 8 XCDs in turn, and those of a key/value head
+// go to one, whose L2 then holds its keys; sequences go by length, the longest first, so that short blocks fill what is left at the end.
+// (8 x 577 x 1000 by length, 12 heads of 40, 480 blocks: in the order of their numbers 64 us, two of the longest one after the other.)
+struct BlockPlace {
+  int b, kv, x;
+};
+__device__ __forceinline__ BlockPlace block_place(const DifferArgs& a, int64_t id, int64_t each) {
+  const int64_t groups = (int64_t)a.batch * a.kv_heads, whole = groups / 8 * 8 * each;
+  int64_t group, x;
+  if (id < whole) {
+    group = id / 8 / each * 8 + id % 8;
+    x = id / 8 % each;
+  } else {
+    group = groups / 8 * 8 + (id - whole) / each;
+    x = (id - whole) % each;
+  }
+  BlockPlace p{(int)(group / a.kv_heads), (int)(group % a.kv_heads), (int)x};
+  if (a.lengths != nullptr && a.batch <= 64 && a.batch > 1) {   // the sequence of that rank
+    const int lane = threadIdx.x & 63, mine = lane < a.batch ? min(max(a.lengths[lane], 0), a.keys) : -1;
+    int rank = 0;
+    for (int j = 0; j < a.batch; ++j) {
+      const int other = __builtin_amdgcn_readlane(mine, j);
+      rank += other > mine || (other == mine && j < lane);
+    }
+    p.b = __builtin_ctzll(__ballot(lane < a.batch && rank == p.b));
+  }
+  return p;
+}
+
 // low bits of a word of 32 (or 64) keys: those in front of `seen`
 __device__ __forceinline__ uint32_t first_bits(int seen) { return seen >= 32 ? ~0u : seen <= 0 ? 0u : (1u << seen) - 1; }
 

@@ -22,11 +22,8 @@ __global__ __launch_bounds__(512, 2) void differ_kernel(const DifferArgs a) {
   __shared__ __attribute__((aligned(16))) float tile[F32Tile<CH>::FLOATS > 4 * 16 * W ? F32Tile<CH>::FLOATS : 4 * 16 * W];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, q4 = lane >> 4;
   const int map = wave & 1, part_of = wave >> 1;
-  int64_t at = blockIdx.x;
-  const int split = at % a.splits;
-  at /= a.splits;
-  const int row_tile = row_tile_of(a, (int)(at % a.row_tiles));
-  const int bkv = at / a.row_tiles, b = bkv / a.kv_heads, kv = bkv % a.kv_heads;
+  const BlockPlace at = block_place(a, blockIdx.x, (int64_t)a.row_tiles * a.splits);
+  const int b = at.b, kv = at.kv, bkv = b * a.kv_heads + kv, split = at.x % a.splits, row_tile = row_tile_of(a, at.x / a.splits);
   const int n = keys_that_count(a, b);
   const int64_t first = (int64_t)row_tile * kRows, last = min(first + kRows, a.rows) - 1;
   const int tiles = (most_seen(a, first, last, n) + R - 1) / R, per = (tiles + a.splits - 1) / a.splits;
@@ -151,10 +148,9 @@ __global__ __launch_bounds__(256) void differ_join_kernel(const DifferArgs a) {
     if (d < 2 * a.head)
       for (int k = slice; k < a.splits; k += SLICES) {
         const float w = exp2_((a.part_lse[k * rows + own] - base) * kLog2e) * inv;
-        if (w == 0.0f) continue;   // (a part without keys, or too small to count)
         const Four x = load_four(a.part + (k * rows + own) * 2 * a.head, d, 2 * a.head, true);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[m][i] += w * x.v[i];
+        for (int i = 0; i < 4; ++i) f[m][i] += w == 0.0f ? 0.0f : w * x.v[i];   // (a part without keys holds zeros; one too small to count may be infinite)
       }
   }
   if constexpr (SLICES > 1) {
@@ -205,7 +201,7 @@ void launch_differ(const DifferArgs& a, hipStream_t st) {
 template <typename T, int>
 void launch_join(const DifferArgs& a, hipStream_t st) {
   const int64_t rows = (int64_t)a.batch * a.kv_heads * a.rows;
-  if (a.splits > 8) hipLaunchKernelGGL((differ_join_kernel<T, 4>), dim3((unsigned)rows), dim3(256), 0, st, a);
+  if (a.splits > 8 || (a.splits > 2 && rows <= 4096)) hipLaunchKernelGGL((differ_join_kernel<T, 4>), dim3((unsigned)rows), dim3(256), 0, st, a);
   else hipLaunchKernelGGL((differ_join_kernel<T, 1>), dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, a);
 }
 

@@ -69,6 +69,7 @@ struct TripleLoad {
   // for each row.  The number of transfers varies: for those who wait for all of them.)
   __device__ __forceinline__ void issue_rows(int j0, int j1, const T* p0, const T* p1, const T* pw, unsigned lds, int wave, int lane) const {
     static_assert(!EVEN, "an offset for every place");
+    lane = (int)hide(lane);
 #pragma unroll
     for (int i = 0; i < PLACES; ++i) {
       const int at = i * WAVES + wave, tile = tile_of(at);
@@ -81,6 +82,7 @@ struct TripleLoad {
   // rows anywhere: map(j, m), wide(j) are pointers to them
   template <class Map, class Wide>
   __device__ __forceinline__ void issue_any(Map map, Wide wide, unsigned lds, int wave, int lane) const {
+    lane = (int)hide(lane);   // (rarely taken: nothing of it is to be kept in registers)
 #pragma unroll
     for (int i = 0; i < PLACES; ++i) {
       const int at = i * WAVES + wave, tile = tile_of(at);
@@ -92,17 +94,23 @@ struct TripleLoad {
       }
     }
   }
-  // tile t of rows that follow one another and end after n: rows past the last one repeat it
+  // Tile ta of the maps and tile tb of the wide rows, of rows that follow one another and end after n: rows past the last one repeat it (and ones in
+  // front of the first one that).
+  __device__ __forceinline__ void issue_tiles(int ta, int tb, int n, const T* p, int64_t map_stride, int64_t second_map, const T* pw, int64_t wide_stride,
+                                              unsigned lds, int wave, int lane) const {
+    const int64_t fa = (int64_t)ta * ROWS, fb = (int64_t)tb * ROWS;
+    if (fb >= 0 && max(fa, fb) + ROWS <= n) {
+      const T* p0 = p + fa * map_stride;
+      issue(p0, p0 + second_map, pw + fb * wide_stride, map_stride, wide_stride, lds, wave);
+    } else {
+      issue_any([&](int j, int m) { return p + min(fa + j, (int64_t)n - 1) * map_stride + m * second_map; },
+                [&](int j) { return pw + min(max(fb + j, (int64_t)0), (int64_t)n - 1) * wide_stride; }, lds, wave, lane);
+    }
+  }
+  // tile t of all
   __device__ __forceinline__ void issue_tile(int t, int n, const T* p, int64_t map_stride, int64_t second_map, const T* pw, int64_t wide_stride,
                                              unsigned lds, int wave, int lane) const {
-    const int64_t first = (int64_t)t * ROWS;
-    if (first + ROWS <= n) {
-      const T* p0 = p + first * map_stride;
-      issue(p0, p0 + second_map, pw + first * wide_stride, map_stride, wide_stride, lds, wave);
-    } else {
-      issue_any([&](int j, int m) { return p + min(first + j, (int64_t)n - 1) * map_stride + m * second_map; },
-                [&](int j) { return pw + min(first + j, (int64_t)n - 1) * wide_stride; }, lds, wave, lane);
-    }
+    issue_tiles(t, t, n, p, map_stride, second_map, pw, wide_stride, lds, wave, lane);
   }
 };
 

@@ -75,25 +75,23 @@ __device__ __forceinline__ void zero_lds(T* lds) {
 }
 
 // Many rows: a wave takes 32 rows of one map, eight waves share tiles of 64 keys: four groups of rows, both maps, whose two waves are of one SIMD.  Tiles are
-// on their way to LDS STAGES - 1 ahead; one barrier a tile.  At the end the second map's result meets the first one's in LDS, lane by lane.
+// on their way to LDS STAGES - 1 ahead; one barrier a tile.  (The two waves of a SIMD taking turns at products and softmax, as attend16_wide_kernel's
+// do: 4096 x 4096, heads of 128, 530 us instead of 471, 577 x 1000, heads of 40, 76 instead of 65: with values twice as wide the products take longer than the
+// softmax beside them.)  At the end the second map's result meets the first one's in LDS, lane by lane.
+// (Four stages where they fit and every wave has as many transfers: 2 x 2048 x 2048, 16 heads of 64, 126 us, with two 136.  Else two: heads of 40 as above 64 us,
+// with four 67, of 96 109 us, with three 112.)
 template <int CH>
-constexpr int differ_stages() {
-  constexpr int stage = 64 * (2 * Width16<CH>::DP + Width16<CH>::W) * 2;
-  return 147456 / stage < 4 ? 147456 / stage : 4;
-}
+constexpr int differ_stages = CH == 2 || CH == 4 ? 4 : 2;
 template <typename T, int CH>
 __global__ __launch_bounds__(512, 2) void differ16_kernel(const DifferArgs a) {
-  constexpr int KEYS = 64, STAGES = differ_stages<CH>(), DP = Width16<CH>::DP, W = Width16<CH>::W;
+  constexpr int KEYS = 64, STAGES = differ_stages<CH>, DP = Width16<CH>::DP, W = Width16<CH>::W;
   typedef TripleLoad<T, CH, KEYS, 8> Load;
   __shared__ __attribute__((aligned(1024))) T lds[STAGES * Load::VALUES];
   static_assert(STAGES >= 2 && STAGES * Load::VALUES * 2 >= 4 * 32 * W * 4, "the second map's result fits the tiles' place");
   const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int map = wave >> 2, part_of = wave & 3;
-  int64_t at = xcd_order(blockIdx.x, gridDim.x);
-  const int split = at % a.splits;
-  at /= a.splits;
-  const int row_tile = row_tile_of(a, (int)(at % a.row_tiles));
-  const int kv = (int)(at / a.row_tiles) / a.batch, b = (int)(at / a.row_tiles + kv) % a.batch, bkv = b * a.kv_heads + kv;
+  const BlockPlace at = block_place(a, blockIdx.x, (int64_t)a.row_tiles * a.splits);
+  const int b = at.b, kv = at.kv, bkv = b * a.kv_heads + kv, split = at.x % a.splits, row_tile = row_tile_of(a, at.x / a.splits);
   const int n = keys_that_count(a, b);
   const int64_t first = (int64_t)row_tile * kDiffer16Rows, last = min(first + kDiffer16Rows, a.rows) - 1;
   const int tiles = (most_seen(a, first, last, n) + KEYS - 1) / KEYS, per = (tiles + a.splits - 1) / a.splits;
@@ -227,11 +225,8 @@ __global__ __launch_bounds__(64 * differ_groups<CH>(), 1) void differ16_few_kern
   __shared__ __attribute__((aligned(1024))) T lds[TILES > FOUND ? TILES : FOUND];
   __shared__ float col_max[GROUPS][32], col_total[GROUPS][32];
   const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5, group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int64_t at = xcd_order(blockIdx.x, gridDim.x);
-  const int split = at % a.splits;
-  at /= a.splits;
-  const int row_tile = at % a.row_tiles;
-  const int kv = (int)(at / a.row_tiles) / a.batch, b = (int)(at / a.row_tiles + kv) % a.batch, bkv = b * a.kv_heads + kv;
+  const BlockPlace at = block_place(a, blockIdx.x, (int64_t)a.row_tiles * a.splits);
+  const int b = at.b, kv = at.kv, bkv = b * a.kv_heads + kv, split = at.x % a.splits, row_tile = at.x / a.splits;
   const int n = keys_that_count(a, b);
   const int64_t first = (int64_t)row_tile * kDifferFewRows, last = min(first + kDifferFewRows, a.rows) - 1;
   const int tiles = (most_seen(a, first, last, n) + KEYS - 1) / KEYS, per = (tiles + a.splits - 1) / a.splits;

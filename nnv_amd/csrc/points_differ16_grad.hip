@@ -63,11 +63,8 @@ __global__ __launch_bounds__(64 * kWaves<CH>, kWaves<CH> / 4) void differ_query_
   typedef TripleLoad<T, CH, KEYS, WAVES> Load;
   __shared__ __attribute__((aligned(1024))) T lds[2 * Load::VALUES];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
-  int64_t at = xcd_order(blockIdx.x, gridDim.x);
-  const int split = at % a.splits;
-  at /= a.splits;
-  const int row_tile = row_tile_of(a, (int)(at % a.row_tiles));
-  const int b = (int)(at / a.row_tiles) % a.batch, kv = (int)(at / a.row_tiles) / a.batch, bkv = b * a.kv_heads + kv;
+  const BlockPlace at = block_place(a, blockIdx.x, (int64_t)a.row_tiles * a.splits);
+  const int b = at.b, kv = at.kv, bkv = b * a.kv_heads + kv, split = at.x % a.splits, row_tile = row_tile_of(a, at.x / a.splits);
   const int n = keys_that_count(a, b);
   const int64_t first = (int64_t)row_tile * ROWS, last = min(first + ROWS, a.rows) - 1;
   const int tiles = (most_seen(a, first, last, n) + KEYS - 1) / KEYS, per = (tiles + a.splits - 1) / a.splits;
@@ -154,11 +151,9 @@ __global__ __launch_bounds__(64 * kKeyWaves<CH>, kKeyWaves<CH> / 4) void differ_
   __shared__ __attribute__((aligned(1024))) T lds[2 * Load::VALUES + WAVES * 512 * PARKED];
   __shared__ __attribute__((aligned(1024))) float info[2][kInfos * ROWS < 256 ? 256 : 512];   // [buffer][RowInfo * ROWS + row]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
-  int64_t at = xcd_order(blockIdx.x, gridDim.x);
-  const int split = at % a.splits;
-  at /= a.splits;
-  const int blocks = key_blocks_of(a.key_tiles, a.causal), block = at % blocks;
-  const int b = (int)(at / blocks) % a.batch, kv = (int)(at / blocks) / a.batch, bkv = b * a.kv_heads + kv;
+  const int blocks = key_blocks_of(a.key_tiles, a.causal);
+  const BlockPlace at = block_place(a, blockIdx.x, (int64_t)blocks * a.splits);
+  const int b = at.b, kv = at.kv, bkv = b * a.kv_heads + kv, split = at.x % a.splits, block = at.x / a.splits;
   const int n = keys_that_count(a, b);
   const unsigned lds_at = lds_addr_of(lds), rows_at = rows_place<T, DP>(lane), wide_at = rows_place<T, W>(lane) + 4 * Load::MAP;
   const unsigned columns_at = columns_place<T, DP>(lane), wide_columns_at = columns_place<T, W>(lane) + 4 * Load::MAP;

@@ -77,11 +77,8 @@ __global__ __launch_bounds__(256, CH <= 6 ? 2 : 1) void differ_query_grad_kernel
   constexpr int R = 32, LD = F32Tile<CH>::LD;
   __shared__ __attribute__((aligned(16))) float tile[F32Tile<CH>::FLOATS];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, q4 = lane >> 4;
-  int64_t at = blockIdx.x;
-  const int split = at % a.splits;
-  at /= a.splits;
-  const int row_tile = row_tile_of(a, (int)(at % a.row_tiles));
-  const int bkv = at / a.row_tiles, b = bkv / a.kv_heads, kv = bkv % a.kv_heads;
+  const BlockPlace at = block_place(a, blockIdx.x, (int64_t)a.row_tiles * a.splits);
+  const int b = at.b, kv = at.kv, bkv = b * a.kv_heads + kv, split = at.x % a.splits, row_tile = row_tile_of(a, at.x / a.splits);
   const int n = keys_that_count(a, b);
   const int64_t first = (int64_t)row_tile * kBlockRows, last = min(first + kBlockRows, a.rows) - 1;
   const int tiles = (most_seen(a, first, last, n) + R - 1) / R, per = (tiles + a.splits - 1) / a.splits;
@@ -150,11 +147,9 @@ __global__ __launch_bounds__(256, CH <= 4 ? 2 : 1) void differ_key_grad_kernel(c
   __shared__ __attribute__((aligned(16))) float tile[F32Tile<CH>::FLOATS];
   __shared__ __attribute__((aligned(16))) float offsets[2][R], deltas[2][R], weights[R], seen_by_row[R];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, q4 = lane >> 4;
-  int64_t at = blockIdx.x;
-  const int split = at % a.splits;
-  at /= a.splits;
-  const int blocks = key_blocks_of(a.key_tiles, a.causal), block = at % blocks;
-  const int bkv = at / blocks, b = bkv / a.kv_heads, kv = bkv % a.kv_heads;
+  const int blocks = key_blocks_of(a.key_tiles, a.causal);
+  const BlockPlace at = block_place(a, blockIdx.x, (int64_t)blocks * a.splits);
+  const int b = at.b, kv = at.kv, bkv = b * a.kv_heads + kv, split = at.x % a.splits, block = at.x / a.splits;
   const int n = keys_that_count(a, b);
   const float unit = a.scale * kLog2e;
 #pragma unroll 1
