@@ -4,11 +4,12 @@
 //   xh = (x - mu) r, z = xh w + b, y = act(z);  act: z, max(z, 0) or z / (1 + exp(-z))
 //   h = dy act'(z);  dx = r (h w - mean(h w) - xh mean(h w xh));  dw = sum over n, p of h xh;  db = sum over n, p of h
 //
-// Both directions are bound by memory: the forward pass reads x and writes y, the backward pass reads x and dy and writes dx.  A sequence's
-// group does not fit a block in general, so that each direction is two launches: one leaves sums of parts of the places, the
-// other adds them (in order: no atomics, the same inputs give the same bits) and reads again what the caches may still hold.
+// Both directions are bound by memory: the forward pass reads x and writes y, the backward pass reads x and dy and writes dx.  Where all places of a
+// sequence's group (or of a few, next to one another) fit a block's registers, a block takes them, and everything is read once (the resident
+// kernels below).  Else each direction is two launches: one leaves sums of parts of the places, the other adds them (in order: no
+// atomics, the same inputs give the same bits) and reads again what the caches may still hold.
 //
-// A block takes a part of the places of a chunk of channels: whole groups, or a part of a wide one.  Its threads are (pack of
+// There a block takes a part of the places of a chunk of channels: whole groups, or a part of a wide one.  Its threads are (pack of
 // 16 bytes of channels) x (places): rows are read as they lie in memory, whatever the groups are.  The sums of x and x^2 are f64:
 // the memory's rate asks for some 1e13 f64 operations a second, a quarter of what the f64 pipes give, and a mean far from zero then
 // costs the variance nothing.
@@ -21,7 +22,7 @@
 namespace nnvhip {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
 constexpr int kWide = 1024;   // channels of a chunk, at most
 constexpr int kAhead = 4;     // places that a thread has on the way
 
@@ -40,6 +41,7 @@ struct GroupArgs {
   int batch, channels, groups, each;
   int width, chunks, per_group;   // channels of a chunk; chunks of all channels; of a group, where it is wider than a chunk
   int splits, wide_params;        // wide_params: scale and offset are f32
+  int resident, threads;          // packs of a thread of the resident form (0: the other one), and its threads
   float eps;
 };
 
@@ -236,20 +238,23 @@ __global__ __launch_bounds__(kThreads) void group_apply_kernel(const GroupArgs a
   });
 }
 
+__device__ __forceinline__ float apart(float x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
 // h = dy act'(z).  Which side of zero z is on decides a whole gradient: next to zero it is formed in 64 bits.
 template <typename T, int ACT>
 __device__ __forceinline__ float through(float dy, float x, float xh, float mu, float r, float w, float b) {
   if constexpr (ACT == kRelu) {
     const float z = xh * w + b;
     bool on = z > 0.0f;
-    if (fabsf(z) <= 4e-7f * (fabsf(xh * w) + fabsf(b))) on = ((double)x - (double)mu) * (double)r * (double)w + (double)b > 0.0;
+    if (fabsf(z) <= 4e-7f * (fabsf(xh * w) + fabsf(b)))   // (formed where it is needed: kept, the parameters in 64 bits would take 64 registers)
+      on = ((double)apart(x) - (double)apart(mu)) * (double)apart(r) * (double)apart(w) + (double)apart(b) > 0.0;
     return on ? dy : z == z ? 0.0f : z;
   }
   if constexpr (ACT == kSilu) {
-    const float z = xh * w + b, e = exp_minus<T>(z), sig = over<T>(1.0f, 1.0f + e);
-    // act' = sig (1 + z (1 - sig)), 1 - sig = e sig, which is 1 where e is beyond f32 (and sig zero)
-    const float rest = e < 1e30f ? e * sig : 1.0f;
-    return dy * (sig * (1.0f + z * rest));
+    const float z = xh * w + b, sig = over<T>(1.0f, 1.0f + exp_minus<T>(z));
+    return dy * (sig * (1.0f + z * (1.0f - sig)));
   }
   return dy;
 }
@@ -290,17 +295,24 @@ __global__ __launch_bounds__(kThreads) void group_grad_sums_kernel(const GroupAr
     }
   }
   __syncthreads();
-  for (int col = threadIdx.x; col < c.size; col += kThreads) {
+  for (int e = threadIdx.x; e < c.size * 8; e += kThreads) {   // 8 threads a channel, of one wave
+    const int col = e >> 3;
     float s = 0, q = 0;
-    for (int k = 0; k < rows; ++k) {
+    for (int k = e & 7; k < rows; k += 8) {
       s += lds[0][k * packs * V + col];
       q += lds[1][k * packs * V + col];
     }
+#pragma unroll
+    for (int k = 4; k > 0; k >>= 1) {
+      s += __shfl_xor(s, k, 64);
+      q += __shfl_xor(q, k, 64);
+    }
+    if (e & 7) continue;
     float* to = a.columns + (((int64_t)c.n * a.splits + c.split) * a.channels + c.first + col) * 2;
     to[0] = s;
     to[1] = q;
     const float w = param<T>(a, a.scale, c.first + col, 1.0f);
-    lds[0][col] = s * w;   // (row 0 of this column, which no other thread reads)
+    lds[0][col] = s * w;   // (row 0 of this channel, whose readers are these threads)
     lds[1][col] = q * w;
   }
   __syncthreads();
@@ -365,7 +377,7 @@ __global__ __launch_bounds__(kThreads) void group_grad_apply_kernel(const GroupA
   __syncthreads();
   const int packs = (c.size + V - 1) / V, rows = kThreads / packs, tx = threadIdx.x % packs, ty = threadIdx.x / packs, left = c.size - tx * V;
   if (ty >= rows) return;
-  float mu[V], r[V], w[V], b[V], m0[V], m1[V];
+  float mu[V], r[V], w[V], b[V], rw[V], m0[V], m1[V];   // the means times r
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int col = min(tx * V + i, c.size - 1), j = a.per_group > 1 ? 0 : col / a.each;
@@ -374,8 +386,9 @@ __global__ __launch_bounds__(kThreads) void group_grad_apply_kernel(const GroupA
     r[i] = a.rstd[g];
     w[i] = param<T>(a, a.scale, c.first + col, 1.0f);
     b[i] = param<T>(a, a.offset, c.first + col, 0.0f);
-    m0[i] = mean_h[j];
-    m1[i] = mean_hx[j];
+    rw[i] = r[i] * w[i];
+    m0[i] = r[i] * mean_h[j];
+    m1[i] = r[i] * mean_hx[j];
   }
   const T* const at[2] = {(const T*)a.x + c.n * a.x_b + c.first + tx * V, (const T*)a.dy + c.n * a.dy_b + c.first + tx * V};
   const int64_t stride[2] = {a.x_p, a.dy_p};
@@ -387,15 +400,291 @@ __global__ __launch_bounds__(kThreads) void group_grad_apply_kernel(const GroupA
     for (int i = 0; i < V; ++i) {
       const float x = to_f(p[0][i]), xh = (x - mu[i]) * r[i];
       const float h = through<T, ACT>(to_f(p[1][i]), x, xh, mu[i], r[i], w[i], b[i]);
-      dx.set(i, from_f<T>(r[i] * (h * w[i] - m0[i] - xh * m1[i])));
+      dx.set(i, from_f<T>(h * rw[i] - (m0[i] + xh * m1[i])));
     }
     store_pack(out + place * a.channels, dx, left);
   });
 }
 
+// ---- resident: all places of a chunk of whole groups in a block's registers ----------------------------------
+
+constexpr int kFour = 4;   // channels a thread takes of a place
+
+// four channels of a place, as the words they are loaded as
+template <typename T>
+struct Quad {
+  unsigned w[sizeof(T)];
+  __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(w, p, 4 * sizeof(T)); }
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (sizeof(T) == 4) return to_f(__builtin_bit_cast(T, w[i]));
+    else return to_f(__builtin_bit_cast(T, (uint16_t)(w[i / 2] >> (16 * (i & 1)))));
+  }
+};
+template <typename T>
+__device__ __forceinline__ void store_quad(T* p, const float (&f)[4]) {
+  T t[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) t[i] = from_f<T>(f[i]);
+  __builtin_memcpy(p, t, sizeof(t));
+}
+
+// The chunk of a block, whose neighbours share the lines of memory that its places lie in: the chunks of a sequence are one XCD's.  (Blocks are dealt
+// to the 8 XCDs in turn.)
+struct Resident {
+  int n, first;        // sequence, first channel
+  int quads, rows;     // threads of a place; places at a time
+  int tx, ty;
+};
+__device__ __forceinline__ Resident resident_of(const GroupArgs& a) {
+  const int64_t id = blockIdx.x, whole = (int64_t)a.batch / 8 * 8 * a.chunks;
+  Resident c;
+  int k;
+  if (id < whole) {
+    c.n = (int)(id / 8 / a.chunks * 8 + id % 8);
+    k = (int)(id / 8 % a.chunks);
+  } else {
+    c.n = (int)(a.batch / 8 * 8 + (id - whole) / a.chunks);
+    k = (int)((id - whole) % a.chunks);
+  }
+  c.first = k * a.width;
+  c.quads = a.width / kFour;
+  c.rows = blockDim.x / c.quads;
+  c.tx = threadIdx.x % c.quads;
+  c.ty = threadIdx.x / c.quads;
+  return c;
+}
+
+// Sums over the rows of a block, and the channels of each of its groups, of two numbers a thread and channel; sums[j]: of group j, for all threads.  Waves take
+// the groups in turn, or share one; the order is fixed.  columns(col, s, q): the sums of a channel, for who wants them.
+template <typename N, class Columns>
+__device__ __forceinline__ void resident_sums(const GroupArgs& a, const Resident& c, const N (&s)[kFour], const N (&q)[kFour], char* lds, double (*sums)[2],
+                                              Columns columns) {
+  N* one = (N*)lds;                                  // [rows][width]
+  N* two = one + (int64_t)c.rows * a.width;
+  if (c.ty < c.rows)
+#pragma unroll
+    for (int i = 0; i < kFour; ++i) {
+      one[c.ty * a.width + c.tx * kFour + i] = s[i];
+      two[c.ty * a.width + c.tx * kFour + i] = q[i];
+    }
+  __syncthreads();
+  // channels first: every 8 threads (or fewer) add one channel's rows
+  for (int e = threadIdx.x; e < a.width * 8; e += blockDim.x) {
+    const int col = e >> 3;
+    N x = 0, y = 0;
+    for (int k = e & 7; k < c.rows; k += 8) {
+      x += one[k * a.width + col];
+      y += two[k * a.width + col];
+    }
+    // (the 8 threads are of one wave, and all of them are here: blocks have a multiple of 64 threads, and so has their work)
+#pragma unroll
+    for (int k = 4; k > 0; k >>= 1) {
+      x += __shfl_xor(x, k, 64);
+      y += __shfl_xor(y, k, 64);
+    }
+    if ((e & 7) == 0) {
+      columns(col, x, y);
+      one[col] = x;   // (row 0 of this channel: its reader is among these threads, and done)
+      two[col] = y;
+    }
+  }
+  __syncthreads();
+  const int groups = a.width / a.each, lanes = a.each > 64 ? 64 : 8, at = threadIdx.x % lanes;   // of a group
+  for (int j = threadIdx.x / lanes; j < groups; j += blockDim.x / lanes) {
+    double x = 0, y = 0;
+    for (int e = at; e < a.each; e += lanes) {
+      x += (double)one[j * a.each + e];
+      y += (double)two[j * a.each + e];
+    }
+    for (int k = lanes >> 1; k > 0; k >>= 1) {
+      x += __shfl_xor(x, k, 64);
+      y += __shfl_xor(y, k, 64);
+    }
+    if (at == 0) {
+      sums[j][0] = x;
+      sums[j][1] = y;
+    }
+  }
+  __syncthreads();
+}
+
+constexpr int kResidentWide = 512;   // channels of a resident chunk, at most: its threads
+
+template <typename T, int NP>
+__global__ __launch_bounds__(1024) void group_resident_kernel(const GroupArgs a, int activation) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ double sums[kResidentWide][2];
+  const Resident c = resident_of(a);
+  const bool on = c.ty < c.rows;
+  const int places = (int)a.places;
+  const T* x = (const T*)a.x + c.n * a.x_b + c.first + c.tx * kFour;
+  Quad<T> in[NP];
+#pragma unroll
+  for (int k = 0; k < NP; ++k) in[k].load(x + min(c.ty + k * c.rows, places - 1) * a.x_p);
+  float w[kFour], b[kFour], mu[kFour];
+#pragma unroll
+  for (int i = 0; i < kFour; ++i) {
+    w[i] = param<T>(a, a.scale, c.first + c.tx * kFour + i, 1.0f);
+    b[i] = param<T>(a, a.offset, c.first + c.tx * kFour + i, 0.0f);
+  }
+  double s[kFour] = {}, q[kFour] = {};
+#pragma unroll
+  for (int k = 0; k < NP; ++k)
+    if (on && c.ty + k * c.rows < places)
+#pragma unroll
+      for (int i = 0; i < kFour; ++i) {
+        const double v = (double)in[k][i];
+        s[i] += v;
+        q[i] = fma(v, v, q[i]);
+      }
+  resident_sums(a, c, s, q, lds, sums, [](int, double&, double&) {});
+  const double inv = 1.0 / ((double)a.places * a.each);
+  const int groups = a.width / a.each;
+  for (int j = threadIdx.x; j < groups; j += blockDim.x) {
+    const double m = sums[j][0] * inv, var = sums[j][1] * inv - m * m;
+    const int64_t g = (int64_t)c.n * a.groups + c.first / a.each + j;
+    a.mean[g] = (float)m;
+    a.rstd[g] = (float)(1.0 / sqrt((var < 0 ? 0.0 : var) + (double)a.eps));   // (NaN stays)
+    sums[j][0] = m;
+    sums[j][1] = (double)a.rstd[g];
+  }
+  __syncthreads();
+  if (!on) return;
+#pragma unroll
+  for (int i = 0; i < kFour; ++i) {
+    const int j = (c.tx * kFour + i) / a.each;
+    mu[i] = (float)sums[j][0];
+    w[i] *= (float)sums[j][1];
+  }
+  T* out = (T*)a.out + (c.n * a.places * a.channels + c.first + c.tx * kFour);
+  auto write = [&](auto act) {
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      const int place = c.ty + k * c.rows;
+      if (place < places) {
+        float y[kFour];
+#pragma unroll
+        for (int i = 0; i < kFour; ++i) y[i] = activate<T, decltype(act)::value>((in[k][i] - mu[i]) * w[i] + b[i]);
+        store_quad(out + (int64_t)place * a.channels, y);
+      }
+    }
+  };
+  if (activation == kSilu) write(std::integral_constant<int, kSilu>());
+  else if (activation == kRelu) write(std::integral_constant<int, kRelu>());
+  else write(std::integral_constant<int, kNone>());
+}
+
+template <typename T, int NP>
+__global__ __launch_bounds__(1024) void group_grad_resident_kernel(const GroupArgs a, int activation) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ double sums[kResidentWide][2];
+  const Resident c = resident_of(a);
+  const bool on = c.ty < c.rows;
+  const int places = (int)a.places;
+  const T* x = (const T*)a.x + c.n * a.x_b + c.first + c.tx * kFour;
+  const T* dy = (const T*)a.dy + c.n * a.dy_b + c.first + c.tx * kFour;
+  Quad<T> in[NP], go[NP];
+#pragma unroll
+  for (int k = 0; k < NP; ++k) {
+    in[k].load(x + min(c.ty + k * c.rows, places - 1) * a.x_p);
+    go[k].load(dy + min(c.ty + k * c.rows, places - 1) * a.dy_p);
+  }
+  float w[kFour], b[kFour], mu[kFour], r[kFour];
+#pragma unroll
+  for (int i = 0; i < kFour; ++i) {
+    const int col = c.first + c.tx * kFour + i;
+    const int64_t g = (int64_t)c.n * a.groups + col / a.each;
+    mu[i] = a.mean[g];
+    r[i] = a.rstd[g];
+    w[i] = param<T>(a, a.scale, col, 1.0f);
+    b[i] = param<T>(a, a.offset, col, 0.0f);
+  }
+  T* out = (T*)a.out + (c.n * a.places * a.channels + c.first + c.tx * kFour);
+  auto all = [&](auto act) {
+    constexpr int ACT = decltype(act)::value;
+    float s[kFour] = {}, q[kFour] = {};
+#pragma unroll
+    for (int k = 0; k < NP; ++k)
+      if (on && c.ty + k * c.rows < places)
+#pragma unroll
+        for (int i = 0; i < kFour; ++i) {
+          const float v = in[k][i], xh = (v - mu[i]) * r[i], h = through<T, ACT>(go[k][i], v, xh, mu[i], r[i], w[i], b[i]);
+          s[i] += h;
+          q[i] += h * xh;
+        }
+    float* columns = a.columns + ((int64_t)c.n * a.channels + c.first) * 2;
+    // (the groups' sums are of h w: the weight of a channel times its sums)
+    resident_sums(a, c, s, q, lds, sums, [&](int col, float& sum, float& product) {
+      columns[col * 2] = sum;
+      columns[col * 2 + 1] = product;
+      const float weight = param<T>(a, a.scale, c.first + col, 1.0f);
+      sum *= weight;
+      product *= weight;
+    });
+    if (!on) return;
+    const double inv = 1.0 / ((double)a.places * a.each);
+    float rw[kFour], m0[kFour], m1[kFour];
+#pragma unroll
+    for (int i = 0; i < kFour; ++i) {
+      const int j = (c.tx * kFour + i) / a.each;
+      rw[i] = r[i] * w[i];
+      m0[i] = r[i] * (float)(sums[j][0] * inv);
+      m1[i] = r[i] * (float)(sums[j][1] * inv);
+    }
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      const int place = c.ty + k * c.rows;
+      if (place < places) {
+        float dx[kFour];
+#pragma unroll
+        for (int i = 0; i < kFour; ++i) {
+          const float v = in[k][i], xh = (v - mu[i]) * r[i], h = through<T, ACT>(go[k][i], v, xh, mu[i], r[i], w[i], b[i]);
+          dx[i] = h * rw[i] - (m0[i] + xh * m1[i]);
+        }
+        store_quad(out + (int64_t)place * a.channels, dx);
+      }
+    }
+  };
+  if (activation == kSilu) all(std::integral_constant<int, kSilu>());
+  else if (activation == kRelu) all(std::integral_constant<int, kRelu>());
+  else all(std::integral_constant<int, kNone>());
+}
+template <typename T, int>
+__global__ __launch_bounds__(kThreads) void group_columns_kernel(const GroupArgs a) {
+  add_columns<T>(a, blockIdx.x);
+}
+
 constexpr int kMostPlaces = 128;   // that a thread adds, in f32 in the backward pass
 
-// Sizes to chunks and splits.  Four blocks a CU, and no thread with fewer places than it has on the way or more than kMostPlaces.
+// The resident form takes a call where a chunk of whole groups, of four channels' multiples and 32 bytes at least, leaves a thread few enough places to
+// hold, and where there are many chunks, or short ones.  Forward, 16 x 64 x 64 x 320 in bf16, 21 places a thread: 28 us, in two launches 33.  Of x and dy
+// a thread holds ten places each (twice as many take more registers than 1024 threads have: 57 us, in two launches 50); 40 chunks of 21 places
+// (5 x 53 x 79 x 96 in f32) take 26 us.
+constexpr int kPacks = 22, kGradPacks = 10;
+bool plan_resident(GroupArgs* a, int type, bool backward) {
+  const int size = type_size(type);
+  a->each = a->channels / a->groups;
+  for (int together = 1; together <= 16 && together <= a->groups; ++together) {
+    const int64_t width = (int64_t)together * a->each;
+    if (a->groups % together || width % kFour || width * size < 32) continue;
+    if (width > kResidentWide || (int64_t)a->batch * (a->groups / together) >= (1 << 21)) return false;   // (of 1024 threads: a grid has fewer than 2^32)
+    const int quads = (int)width / kFour;
+    const int64_t rows = std::min<int64_t>(1024 / quads, a->places), packs = ceil_div(a->places, rows);
+    if (packs > (backward ? kGradPacks : kPacks) || (packs > 5 && a->batch * (a->groups / together) < 128)) return false;
+    a->width = (int)width;
+    a->chunks = a->groups / together;
+    a->per_group = a->splits = 1;
+    a->per = a->places;
+    a->resident = (int)packs;
+    a->threads = (int)round_up(rows * quads, 64);
+    return true;
+  }
+  return false;
+}
+
+// Sizes to chunks and splits.  A block a CU, whose start (the parts' sums, the channels' parameters) costs as much as some
+// ten places a thread (the gradient of 16 x 64 x 64 x 320: 22 + 28 us; two blocks a CU 23 + 31, eight of 256 threads 30 + 51), and no thread with fewer places than it has
+// on the way or more than kMostPlaces.
 void plan(GroupArgs* a, int type) {
   const int64_t v = 16 / type_size(type);
   a->each = a->channels / a->groups;
@@ -411,7 +700,7 @@ void plan(GroupArgs* a, int type) {
   }
   const int64_t rows = kThreads / ceil_div(std::min(a->width, a->channels), v), blocks = std::max<int64_t>(1, (int64_t)a->batch * a->chunks);
   const int64_t most = std::max<int64_t>(1, ceil_div(a->places, rows * kAhead));
-  const int64_t splits = std::max(std::min(std::max<int64_t>(1, ceil_div(1024, blocks)), most), ceil_div(a->places, rows * kMostPlaces));
+  const int64_t splits = std::max(std::min(std::max<int64_t>(1, ceil_div(256, blocks)), most), ceil_div(a->places, rows * kMostPlaces));
   a->per = std::max<int64_t>(1, ceil_div(a->places, splits));
   a->splits = (int)std::max<int64_t>(1, ceil_div(a->places, a->per));
 }
@@ -429,7 +718,7 @@ int group_args(const char* what, const nnvhip_group_norm_args* d, bool backward,
   a->places = d->places;
   a->channels = (int)d->channels;
   a->groups = (int)d->groups;
-  plan(a, (int)d->type);
+  if (!plan_resident(a, (int)d->type, backward)) plan(a, (int)d->type);
   // (a grid has fewer than 2^32 threads, and the backward pass has blocks for its columns' sums)
   if ((int64_t)a->batch * a->chunks * a->splits + ceil_div(a->channels, kColumns) >= (int64_t(1) << 23)) NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: too many values", what);
   a->x = d->x;
@@ -450,8 +739,29 @@ int group_args(const char* what, const nnvhip_group_norm_args* d, bool backward,
   return NNVHIP_OK;
 }
 
-int64_t part_bytes(const GroupArgs& a) { return (int64_t)a.batch * a.splits * a.per_group * a.groups * 2 * (int64_t)sizeof(double); }
+int64_t part_bytes(const GroupArgs& a) { return a.resident ? 0 : (int64_t)a.batch * a.splits * a.per_group * a.groups * 2 * (int64_t)sizeof(double); }
 int64_t column_bytes(const GroupArgs& a) { return (int64_t)a.batch * a.splits * a.channels * 2 * (int64_t)sizeof(float); }
+
+template <typename T, int NP>
+void launch_resident(const GroupArgs& a, int activation, bool backward, hipStream_t st) {
+  const dim3 grid((unsigned)((int64_t)a.batch * a.chunks)), block(a.threads);
+  const int rows = a.threads / (a.width / kFour);
+  const size_t lds = (size_t)rows * a.width * 2 * (backward ? sizeof(float) : sizeof(double));
+  if (!backward) hipLaunchKernelGGL((group_resident_kernel<T, NP>), grid, block, lds, st, a, activation);
+  else if constexpr (NP <= kGradPacks) hipLaunchKernelGGL((group_grad_resident_kernel<T, NP>), grid, block, lds, st, a, activation);
+}
+template <typename T>
+void resident(const GroupArgs& a, int activation, bool backward, hipStream_t st) {
+  if (a.batch > 0) {
+    if (a.resident <= 1) launch_resident<T, 1>(a, activation, backward, st);
+    else if (a.resident <= 2) launch_resident<T, 2>(a, activation, backward, st);
+    else if (a.resident <= 5) launch_resident<T, 5>(a, activation, backward, st);
+    else if (a.resident <= 10) launch_resident<T, 10>(a, activation, backward, st);
+    else launch_resident<T, 22>(a, activation, backward, st);
+  }
+  if (backward && (a.dscale || a.doffset))
+    hipLaunchKernelGGL((group_columns_kernel<T, 0>), dim3((unsigned)ceil_div(a.channels, kColumns)), dim3(kThreads), 0, st, a);
+}
 
 template <typename T, int ACT>
 void forward(const GroupArgs& a, hipStream_t st) {
@@ -479,6 +789,13 @@ void backward(const GroupArgs& a, hipStream_t st) {
     else GROUP_BY_ACTIVATION(CALL, f16_t, act, __VA_ARGS__);                           \
   } while (0)
 
+#define GROUP_RESIDENT(type, ...)                                     \
+  do {                                                                \
+    if ((type) == NNVHIP_TYPE_F32) resident<float>(__VA_ARGS__);      \
+    else if ((type) == NNVHIP_TYPE_BF16) resident<bf16_t>(__VA_ARGS__); \
+    else resident<f16_t>(__VA_ARGS__);                                \
+  } while (0)
+
 }  // namespace
 }  // namespace nnvhip
 
@@ -501,10 +818,11 @@ int nnvhip_group_norm(nnvhip_ctx* ctx, const nnvhip_group_norm_args* d, void* wo
   if (a.batch == 0) return NNVHIP_OK;
   if (!a.x || !a.out || !a.mean || !a.rstd) NNV_FAIL(NNVHIP_ERR_ARG, "nnvhip_group_norm: null pointer");
   if (!(d->epsilon >= 0)) NNV_FAIL(NNVHIP_ERR_ARG, "nnvhip_group_norm: epsilon must not be negative");
-  if (!workspace || workspace_bytes < part_bytes(a))
+  if (workspace_bytes < part_bytes(a) || (part_bytes(a) && !workspace))
     NNV_FAIL(NNVHIP_ERR_ARG, "nnvhip_group_norm: a workspace of %lld bytes is needed", (long long)part_bytes(a));
   a.part = (double*)workspace;
-  GROUP_BY_TYPE(forward, d->type, d->activation, a, (hipStream_t)stream);
+  if (a.resident) GROUP_RESIDENT(d->type, a, (int)d->activation, false, (hipStream_t)stream);
+  else GROUP_BY_TYPE(forward, d->type, d->activation, a, (hipStream_t)stream);
   NNV_HIP_TRY(hipGetLastError());
   return NNVHIP_OK;
 }
@@ -529,7 +847,8 @@ int nnvhip_group_norm_backward(nnvhip_ctx* ctx, const nnvhip_group_norm_args* d,
     a.part = (double*)workspace;
     a.columns = (float*)((char*)workspace + part_bytes(a));
   }
-  GROUP_BY_TYPE(backward, d->type, d->activation, a, (hipStream_t)stream);
+  if (a.resident) GROUP_RESIDENT(d->type, a, (int)d->activation, true, (hipStream_t)stream);
+  else GROUP_BY_TYPE(backward, d->type, d->activation, a, (hipStream_t)stream);
   NNV_HIP_TRY(hipGetLastError());
   return NNVHIP_OK;
 }
