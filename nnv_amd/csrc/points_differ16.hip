@@ -211,7 +211,8 @@ __global__ __launch_bounds__(512, 2) void differ16_kernel(const DifferArgs a) {
 
 // Few rows (single tokens): 16 rows for the block, and a product's 32 columns are their first maps and their second ones, so that the values are multiplied with
 // both at once.  (The scores of each map's keys are formed for all columns, of which half are taken.)  The block's waves take tiles of 32 keys in
-// turn, each with LDS of its own, two stages; what they found is joined at the end.  Bound by memory.  Weights in two pieces, as in attend16_kernel.
+// turn, each with LDS of its own, two stages; what they found is joined at the end.  Bound by memory, so that weights go in two pieces: what their rounding leaves is
+// a second weight.
 template <int CH>
 constexpr int differ_groups() {
   constexpr int two_stages = 2 * 32 * (2 * Width16<CH>::DP + Width16<CH>::W) * 2;
@@ -242,11 +243,11 @@ __global__ __launch_bounds__(64 * differ_groups<CH>(), 1) void differ16_few_kern
   const float unit = unit_of(a.scale);
   half8<T> qf[CH];
   query_operands<T, CH>(qf, (const T*)a.q.p + (here ? map_row_at(a.q, a, b, kv, r, map) : 0), h, a.head, here, a.scale);
-  float16_t acc[CH], second[CH];   // second: of what the weights' rounding leaves
+  float16_t acc[CH];
 #pragma unroll
   for (int d = 0; d < CH; ++d)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[d][i] = second[d][i] = 0.0f;
+    for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
   float off = -INFINITY, total = 0.0f;
   bool far = false;
   const T* kp = (const T*)a.k.p + b * a.k.b + 2 * kv * a.k.h;
@@ -283,10 +284,7 @@ __global__ __launch_bounds__(64 * differ_groups<CH>(), 1) void differ16_few_kern
 #pragma unroll
       for (int d = 0; d < CH; ++d)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          acc[d][i] *= fade;
-          second[d][i] *= fade;
-        }
+        for (int i = 0; i < 16; ++i) acc[d][i] *= fade;
     half8<T> p[2], rest[2];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -298,7 +296,7 @@ __global__ __launch_bounds__(64 * differ_groups<CH>(), 1) void differ16_few_kern
     }
     over_columns<T, W, 2>(vs_at, 0, [&](int c, int d, const half8<T>& v) {
       acc[d] = Half8<T>::mfma(v, p[c], acc[d]);
-      second[d] = Half8<T>::mfma(v, rest[c], second[d]);
+      acc[d] = Half8<T>::mfma(v, rest[c], acc[d]);
     });
   }
   total = sum_of_halves(total);
@@ -313,12 +311,7 @@ __global__ __launch_bounds__(64 * differ_groups<CH>(), 1) void differ16_few_kern
   for (int d = 0; d < CH; ++d)
 #pragma unroll
     for (int i4 = 0; i4 < 4; ++i4) {
-      float f[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float one = acc[d][4 * i4 + i];
-        f[i] = fabsf(one) < INFINITY ? one + second[d][4 * i4 + i] : one;
-      }
+      const float f[4] = {acc[d][4 * i4], acc[d][4 * i4 + 1], acc[d][4 * i4 + 2], acc[d][4 * i4 + 3]};
       __builtin_memcpy(found + d * 32 + 8 * i4 + 4 * h, f, 16);
     }
   __syncthreads();
