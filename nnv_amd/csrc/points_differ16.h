@@ -189,7 +189,7 @@ void launch_differ16(const DifferArgs& a, int type, bool few, hipStream_t st);
 bool differ_grad16_takes(const DifferArgs& a, int type);
 int differ_grad16_tile(int64_t head);       // rows of a block
 int differ_key_grad16_tile(int64_t head);   // keys
-void launch_differ_query_grad16(const DifferArgs& a, hipStream_t st);
-void launch_differ_key_grad16(const DifferArgs& a, hipStream_t st);
+void launch_differ_query_grad16(const DifferArgs& a, int type, hipStream_t st);
+void launch_differ_key_grad16(const DifferArgs& a, int type, hipStream_t st);
 
 }  // namespace nnvhip

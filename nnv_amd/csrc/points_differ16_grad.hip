@@ -1,6 +1,10 @@
-// Differential attention of points in bf16, backward, on v_mfma_f32_32x32x16_bf16: the 16-bit forms of differ_query_grad_kernel and
-// differ_key_grad_kernel.  The weights' difference and the scores' gradients are rounded to bf16 in front of the products that use them, as in
-// points_attend16_grad.hip (and f16 stays away for the reason given there).
+// Differential attention of points in 16 bits, backward, on v_mfma_f32_32x32x16_{bf16,f16}: the 16-bit forms of differ_query_grad_kernel and
+// differ_key_grad_kernel.  The weights' difference and the scores' gradients are rounded to 16 bits in front of the products that use them.
+//
+// f16 does not hold the scores' gradients as they are: weights far below one times differences of any size.  What a lane rounds is all of one column of the
+// product that takes it, and so of one row of the result; a power of two that brings the column's largest value so far to 2^14 (Lift) is taken out of the
+// result at the end, and when a larger value comes the sums so far are scaled, as a softmax's are: what is below 2^-38 of the largest is lost, what is above 2^-28
+// keeps all bits.
 #include "points_differ16.h"
 
 #pragma clang fp contract(fast)
@@ -8,6 +12,12 @@
 namespace nnvhip {
 namespace {
 
+// max(x, |a|, |b|)
+__device__ __forceinline__ float max3_of_sizes(float x, float a, float b) {
+  float r;
+  asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(r) : "v"(x), "v"(a), "v"(b));
+  return r;
+}
 template <typename T, int N>
 __device__ __forceinline__ void load_operands(half8<T> (&f)[N], const T* row, int h, int size, bool there) {
 #pragma unroll
@@ -23,6 +33,41 @@ __device__ __forceinline__ void zero(float16_t (&acc)[N]) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
 }
+// The power of two by which a column's values are rounded in f16 (bf16: none).
+template <typename T>
+struct Lift {
+  static constexpr bool USED = std::is_same_v<T, f16_t>;
+  float up = USED ? 0x1p40f : 1.0f;
+  // M sets of values of a column, in this lane and l ^ 32: what has been added up of them so far is scaled where a value is larger than any before
+  template <int M, int N>
+  __device__ __forceinline__ void raise(float16_t (*s)[1], float16_t (&acc)[M][N]) {
+    if constexpr (USED) {
+      float top = 0.0f;
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) top = max3_of_sizes(top, s[m][0][i], s[m][0][i + 1]);
+      top = max_of_halves(top);
+      if (__any(top * up > 32768.0f)) {
+        // (an infinite or missing value is not lifted, and does what it would)
+        const float next = top * up > 32768.0f && top < INFINITY ? __builtin_amdgcn_ldexpf(1.0f, 14 - __builtin_amdgcn_frexp_expf(top)) : up, fade = next / up;
+        up = next;
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int d = 0; d < N; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[m][d][i] *= fade;
+      }
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[m][0][i] *= up;
+    }
+  }
+  __device__ __forceinline__ float down() const { return USED ? 1.0f / up : 1.0f; }
+};
+
 // acc[d] += the product over 32 rows, from `first` on, of a tile of rows of DP values with p, rounded
 template <typename T, int DP>
 __device__ __forceinline__ void over_rows(unsigned tile, int first, const float16_t& p, float16_t (&acc)[DP / 32]) {
@@ -89,9 +134,10 @@ __global__ __launch_bounds__(64 * kWaves<CH>, kWaves<CH> / 4) void differ_query_
 #pragma unroll
   for (int m = 0; m < 2; ++m) load_operands<T, CH>(qf[m], (const T*)a.q.p + (here ? map_row_at(a.q, a, b, kv, r, m) : 0), h, a.head, takes_part);
   load_operands<T, 2 * CH>(gf, (const T*)a.go.p + (here ? row_at(a.go, a, b, kv, r) : 0), h, 2 * a.head, takes_part);
-  float16_t dq[2][DP / 32];
+  float16_t dq[2][1][DP / 32];
+  Lift<T> lift[2];
 #pragma unroll
-  for (int m = 0; m < 2; ++m) zero(dq[m]);
+  for (int m = 0; m < 2; ++m) zero(dq[m][0]);
   const T* kp = (const T*)a.k.p + b * a.k.b + 2 * kv * a.k.h;
   const T* vp = (const T*)a.v.p + b * a.v.b + kv * a.v.h;
   Load load;
@@ -130,15 +176,16 @@ __global__ __launch_bounds__(64 * kWaves<CH>, kWaves<CH> / 4) void differ_query_
         if (masked)
 #pragma unroll
           for (int i = 0; i < 16; ++i) s[m][0][i] = word >> product_row(i, 0) & 1 ? s[m][0][i] : 0.0f;
-        over_rows<T, DP>(kc_at + m * (2 * Load::MAP), 0, s[m][0], dq[m]);
+        lift[m].raise(&s[m], dq[m]);
+        over_rows<T, DP>(kc_at + m * (2 * Load::MAP), 0, s[m][0], dq[m][0]);
       }
     }
   }
   if (!here) return;
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
-    if (a.splits > 1) store_result(a.part + (split * own_rows(a) + own_row(a, bkv, r, m)) * a.head, dq[m], a.scale, h, a.head);
-    else store_result((T*)a.dq + dense_map_row_at(a, b, kv, r, m), dq[m], a.scale, h, a.head);
+    if (a.splits > 1) store_result(a.part + (split * own_rows(a) + own_row(a, bkv, r, m)) * a.head, dq[m][0], a.scale * lift[m].down(), h, a.head);
+    else store_result((T*)a.dq + dense_map_row_at(a, b, kv, r, m), dq[m][0], a.scale * lift[m].down(), h, a.head);
   }
 }
 
@@ -163,6 +210,13 @@ __global__ __launch_bounds__(64 * kKeyWaves<CH>, kKeyWaves<CH> / 4) void differ_
   load.init(wave, lane, a.head, a.q.t, a.go.t);
   const T* qp = (const T*)a.q.p + b * a.q.b + 2 * (kv * (int64_t)a.group) * a.q.h;
   const T* gp = (const T*)a.go.p + b * a.go.b + kv * (int64_t)a.group * a.go.h;
+  // the weights' difference is at most 1 + |w|: in f16 of 2^14 (the largest, all bits down to 2^-28)
+  float wide_up = 1.0f;
+  if constexpr (Lift<T>::USED) {
+    float most = 0.0f;
+    for (int g = 0; g < a.group; ++g) most = fmaxf(most, fabsf(weight_of<T>(a, kv * a.group + g)));
+    if (most < INFINITY) wide_up = __builtin_amdgcn_ldexpf(1.0f, 14 - __builtin_amdgcn_frexp_expf(1.0f + most));
+  }
 #pragma unroll 1
   for (int key_tile = block;; key_tile = a.key_tiles - 1 - block) {
     const int first = key_tile * KEYS, key = first + wave * 32 + col;
@@ -187,6 +241,7 @@ __global__ __launch_bounds__(64 * kKeyWaves<CH>, kKeyWaves<CH> / 4) void differ_
       return x;
     };
     float16_t dk[2][DP / 32], dv[CH];
+    Lift<T> lift;
 #pragma unroll
     for (int m = 0; m < 2; ++m) zero(dk[m]);
     zero(dv);
@@ -278,7 +333,7 @@ __global__ __launch_bounds__(64 * kKeyWaves<CH>, kKeyWaves<CH> / 4) void differ_
         for (int c = 0; c < 2; ++c) {
           half8<T> both;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) both[i] = (T)(s[0][0][8 * c + i] + s[1][0][8 * c + i]);
+          for (int i = 0; i < 8; ++i) both[i] = (T)((s[0][0][8 * c + i] + s[1][0][8 * c + i]) * wide_up);
 #pragma unroll
           for (int d = 0; d < CH; ++d) dv[d] = Half8<T>::mfma(columns_operand<T, W>(gc_at, 16 * c, d), both, dv[d]);
         }
@@ -291,7 +346,12 @@ __global__ __launch_bounds__(64 * kKeyWaves<CH>, kKeyWaves<CH> / 4) void differ_
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[m][0][4 * i4 + i] *= dp[0][4 * i4 + i] - f[i];
           }
-          over_rows<T, DP>(qc_at + m * (2 * Load::MAP), 0, s[m][0], dk[m]);
+          if constexpr (!Lift<T>::USED) over_rows<T, DP>(qc_at + m * (2 * Load::MAP), 0, s[m][0], dk[m]);
+        }
+        if constexpr (Lift<T>::USED) {
+          lift.raise(s, dk);
+#pragma unroll
+          for (int m = 0; m < 2; ++m) over_rows<T, DP>(qc_at + m * (2 * Load::MAP), 0, s[m][0], dk[m]);
         }
       }
     }
@@ -305,12 +365,12 @@ __global__ __launch_bounds__(64 * kKeyWaves<CH>, kKeyWaves<CH> / 4) void differ_
       if (a.splits > 1) {
         const int64_t all = (int64_t)a.batch * a.keys * a.kv_heads * 2 * a.head;
 #pragma unroll
-        for (int m = 0; m < 2; ++m) store_result(a.part + split * all + dense + m * a.head, dk[m], a.scale, h, a.head);
-        store_result(a.part + (a.splits + split) * all + dense, dv, 1.0f, h, 2 * a.head);
+        for (int m = 0; m < 2; ++m) store_result(a.part + split * all + dense + m * a.head, dk[m], a.scale * lift.down(), h, a.head);
+        store_result(a.part + (a.splits + split) * all + dense, dv, 1.0f / wide_up, h, 2 * a.head);
       } else {
 #pragma unroll
-        for (int m = 0; m < 2; ++m) store_result((T*)a.dk + dense + m * a.head, dk[m], a.scale, h, a.head);
-        store_result((T*)a.dv + dense, dv, 1.0f, h, 2 * a.head);
+        for (int m = 0; m < 2; ++m) store_result((T*)a.dk + dense + m * a.head, dk[m], a.scale * lift.down(), h, a.head);
+        store_result((T*)a.dv + dense, dv, 1.0f / wide_up, h, 2 * a.head);
       }
     }
     if (key_tile != block || blocks == a.key_tiles || a.key_tiles - 1 - block == block) break;
@@ -333,9 +393,15 @@ void launch_key(const DifferArgs& a, hipStream_t st) {
 int differ_grad16_tile(int64_t head) { return head <= 64 ? 256 : 128; }
 int differ_key_grad16_tile(int64_t head) { return head <= 64 ? 256 : 128; }
 bool differ_grad16_takes(const DifferArgs& a, int type) {
-  return type == NNVHIP_TYPE_BF16 && by_pieces(a.q, a.head) && by_pieces(a.k, a.head) && by_pieces(a.v, a.head) && by_pieces(a.go, a.head) && a.rows < (1 << 27);   // (kInfos * rows floats within 32 bits)
+  return type != NNVHIP_TYPE_F32 && by_pieces(a.q, a.head) && by_pieces(a.k, a.head) && by_pieces(a.v, a.head) && by_pieces(a.go, a.head) && a.rows < (1 << 27);   // (kInfos * rows floats within 32 bits)
 }
-void launch_differ_query_grad16(const DifferArgs& a, hipStream_t st) { DIFFER_BY_HEAD(launch_query, bf16_t, a, st); }
-void launch_differ_key_grad16(const DifferArgs& a, hipStream_t st) { DIFFER_BY_HEAD(launch_key, bf16_t, a, st); }
+void launch_differ_query_grad16(const DifferArgs& a, int type, hipStream_t st) {
+  if (type == NNVHIP_TYPE_BF16) DIFFER_BY_HEAD(launch_query, bf16_t, a, st);
+  else DIFFER_BY_HEAD(launch_query, f16_t, a, st);
+}
+void launch_differ_key_grad16(const DifferArgs& a, int type, hipStream_t st) {
+  if (type == NNVHIP_TYPE_BF16) DIFFER_BY_HEAD(launch_key, bf16_t, a, st);
+  else DIFFER_BY_HEAD(launch_key, f16_t, a, st);
+}
 
 }  // namespace nnvhip

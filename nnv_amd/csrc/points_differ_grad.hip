@@ -305,6 +305,8 @@ GradCut grad_cut(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys, in
   return c;
 }
 
+template <typename T>
+constexpr int kType = std::is_same_v<T, float> ? NNVHIP_TYPE_F32 : std::is_same_v<T, bf16_t> ? NNVHIP_TYPE_BF16 : NNVHIP_TYPE_F16;
 template <typename T, int CH>
 void launch_grad(DifferArgs a, const GradCut& c, bool by16, hipStream_t st) {
   const int64_t heads = (int64_t)a.batch * a.kv_heads;
@@ -314,7 +316,7 @@ void launch_grad(DifferArgs a, const GradCut& c, bool by16, hipStream_t st) {
     a.row_tiles = c.row_tiles;
     a.splits = c.query_splits;
     const dim3 grid((unsigned)(heads * c.row_tiles * a.splits));
-    if (by16) launch_differ_query_grad16(a, st);
+    if (by16) launch_differ_query_grad16(a, kType<T>, st);
     else if (four) hipLaunchKernelGGL((differ_query_grad_kernel<T, CH, true>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((differ_query_grad_kernel<T, CH, false>), grid, dim3(256), 0, st, a);
     if (a.splits > 1) hipLaunchKernelGGL((differ_sum_rows_kernel<T, 0>), dim3((unsigned)ceil_div(heads * 2 * a.rows, 4)), dim3(256), 0, st, a);
@@ -327,7 +329,7 @@ void launch_grad(DifferArgs a, const GradCut& c, bool by16, hipStream_t st) {
     a.key_tiles = c.key_tiles;
     a.splits = c.key_splits;
     const dim3 grid((unsigned)(heads * c.key_blocks * a.splits));
-    if (by16) launch_differ_key_grad16(a, st);
+    if (by16) launch_differ_key_grad16(a, kType<T>, st);
     else if (four) hipLaunchKernelGGL((differ_key_grad_kernel<T, CH, true>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((differ_key_grad_kernel<T, CH, false>), grid, dim3(256), 0, st, a);
     if (a.splits > 1) {

@@ -454,3 +454,20 @@ def test_differential_attention_gives_the_same_bits_again_anywhere(size, dtype):
         torch.cuda.synchronize()
         for a, e in zip(held, fresh):
             assert torch.equal(a, e)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_differential_attention_gradients_of_every_size(dtype):
+    """Rows whose gradients are 2^-12 to 2^9 of the others', the largest ones last; weights of either sign beyond one."""
+    import nnv_amd as nnv
+    for d, lq, lk in ((64, 200, 333), (128, 70, 140), (40, 300, 90)):
+        g = gen(71)
+        q, k, v, w = make_differ(g, 2, lq, lk, 4, 2, d, dtype)
+        w[0], w[1] = -3.0, 17.0
+        kw = dict(causal=lk > lq)
+        o, lse, second = nnv.differential_attention(q, k, v, w, for_backward=True, **kw)
+        by = 2.0 ** (torch.arange(lq, device="cuda") * 21 // lq - 12)
+        do = (rand(g, *o.shape) * by[None, :, None, None]).to(dtype)
+        grads = nnv.differential_attention_backward(do, q, k, v, w, o, lse, second, **kw)
+        for name, got, e, bd in zip(("dq", "dk", "dv", "dweights"), grads, io.differ_grad(do, q, k, v, w, **kw), io.differ_grad_bounds(do, q, k, v, w, **kw)):
+            po.assert_within(got, e, bd, "%d %s" % (d, name))
