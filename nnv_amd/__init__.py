@@ -15,7 +15,8 @@ from .verify import HalfSpace, verify_specification  # noqa: F401
 _POINTS = {"layer_norm": "points", "layer_norm_backward": "points", "cross_attention": "points", "cross_attention_backward": "points",
            "clip_gradients": "points", "LayerNormalizationLayer": "points", "CrossAttentionLayer": "points",
            "group_norm": "images", "group_norm_backward": "images", "rotate_positions": "images",
-           "differential_attention": "images", "differential_attention_backward": "images",
+           "differential_attention": "images", "differential_attention_backward": "images", "GroupNormalizationLayer": "images",
+           "DifferentialAttentionLayer": "images", "GridAttentionClassifier": "falsify",
            "CrossAttentionClassifier": "falsify", "falsify_point": "falsify", "train_step": "falsify"}
 
 

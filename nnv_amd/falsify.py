@@ -3,7 +3,8 @@ together on a network that the set layers do not cover.
 
 A verifier looks for a counterexample before it reaches (the reference's NN evaluates samples of the input box, nn/NN.m); where a
 gradient is to be had, the search follows it.  ``CrossAttentionClassifier`` is a small network for that: points are sequences of
-tokens that attend to the states of another sequence.  ``falsify_point`` moves points of a box towards a HalfSpace of unsafe outputs
+tokens that attend to the states of another sequence; ``GridAttentionClassifier`` is one for images and videos, whose tokens have places in a
+grid.  ``falsify_point`` moves points of a box towards a HalfSpace of unsafe outputs
 and returns one whose output lies in it, checked against the HalfSpace itself; ``train_step`` is one step of gradient descent on
 the cross entropy of labelled points, e.g. of counterexamples, with the norm of all gradients bounded.
 """
@@ -12,6 +13,7 @@ from __future__ import annotations
 import numpy as np
 import torch
 
+from .images import DifferentialAttentionLayer, GroupNormalizationLayer
 from .points import CrossAttentionLayer, LayerNormalizationLayer, clip_gradients
 from .verify import HalfSpace
 
@@ -61,14 +63,80 @@ class CrossAttentionClassifier:
         p = self.parameters
         x, states, y, norm, o, attend, pooled = saved
 
-        def by_weights(inputs, gradient):      # sum over batch and tokens
-            return inputs.flatten(0, -2).t() @ gradient.flatten(0, -2)
-
         dz = ((dscores @ p["Wc"].t()) / x.shape[1])[:, None, :].expand(x.shape).contiguous()
         dq, dk, dv = self.attend.backward(dz @ p["Wo"].t(), attend)
         dx, (dscale, doffset) = self.norm.backward(dq @ p["Wq"].t(), norm)
-        return dz + dx, [dscale, doffset, by_weights(y, dq), by_weights(states, dk), by_weights(states, dv), by_weights(o, dz),
+        return dz + dx, [dscale, doffset, _by_weights(y, dq), _by_weights(states, dk), _by_weights(states, dv), _by_weights(o, dz),
                          pooled.t() @ dscores, dscores.sum(0)]
+
+
+class GridAttentionClassifier:
+    """scores = mean over tokens of (x + attention(norm(x) Wq; states Wk, states Wv) Wo) Wc + bc for tokens that are the places of a grid (rows and
+    columns of an image, time as well in a video): the norm is a group normalization over all places with "silu" behind it, the attention is
+    differential, and queries and keys are turned by their places' positions.
+
+    x: batch x tokens x channels, the places of Grid in the order of its last axis; states: batch x keys x (their channels), those of StateGrid, with key_lengths or a key_mask
+    where some do not count.  Sections: pairs of a head's values for each axis."""
+
+    PARAMETERS = ("Scale", "Offset", "Wq", "Wk", "Wv", "Weights", "Wo", "Wc", "bc")
+
+    def __init__(self, Grid, StateGrid, NumGroups, NumHeads, Sections, NumKeyValueHeads=None, Rotary=None, **parameters):
+        missing = [n for n in self.PARAMETERS if n not in parameters]
+        if missing:
+            raise ValueError("parameters missing: " + ", ".join(missing))
+        if not len(Grid) == len(StateGrid) == len(Sections):
+            raise ValueError("Grid, StateGrid and Sections have the same axes")
+        self.parameters = {n: parameters[n] for n in self.PARAMETERS}
+        self.norm = GroupNormalizationLayer(NumGroups, Scale=parameters["Scale"], Offset=parameters["Offset"], Activation="silu")
+        self.attend = DifferentialAttentionLayer(NumHeads, parameters["Weights"], NumKeyValueHeads, Sections=Sections, Rotary=Rotary)
+        self.positions, self.state_positions = (self.places(grid, parameters["Wq"].device) for grid in (Grid, StateGrid))
+
+    @staticmethod
+    def places(grid, device):
+        """The positions of a grid's places: tokens x axes."""
+        axes = torch.meshgrid(*[torch.arange(n, dtype=torch.int32) for n in grid], indexing="ij")
+        return torch.stack([a.reshape(-1) for a in axes], 1).to(device)
+
+    @staticmethod
+    def random(channels, state_channels, classes, Grid, StateGrid, NumGroups, NumHeads, Sections, NumKeyValueHeads=None, head=32, seed=0,
+               dtype=torch.float32, device="cuda"):
+        """A network with random weights, for examples and tests."""
+        g = torch.Generator().manual_seed(seed)
+        kv = NumKeyValueHeads or NumHeads
+
+        def w(n_in, n_out):
+            return (torch.randn(n_in, n_out, generator=g) / n_in ** 0.5).to(dtype).to(device)
+
+        return GridAttentionClassifier(Grid, StateGrid, NumGroups, NumHeads, Sections, NumKeyValueHeads, Scale=torch.ones(channels, dtype=dtype, device=device),
+                                       Offset=torch.zeros(channels, dtype=dtype, device=device), Wq=w(channels, 2 * NumHeads * head),
+                                       Wk=w(state_channels, 2 * kv * head), Wv=w(state_channels, 2 * kv * head),
+                                       Weights=torch.full((NumHeads,), 0.5, dtype=dtype, device=device), Wo=w(2 * NumHeads * head, channels),
+                                       Wc=w(channels, classes), bc=torch.zeros(classes, dtype=dtype, device=device))
+
+    def evaluate(self, x, states, key_lengths=None, key_mask=None):
+        return self.forward(x, states, key_lengths, key_mask)[0]
+
+    def forward(self, x, states, key_lengths=None, key_mask=None):
+        """(scores: batch x classes, what backward takes)."""
+        p = self.parameters
+        y, norm = self.norm.forward(x)
+        o, attend = self.attend.forward(y @ p["Wq"], states @ p["Wk"], states @ p["Wv"], self.positions, self.state_positions, key_lengths, key_mask)
+        pooled = (x + o @ p["Wo"]).mean(1)
+        return pooled @ p["Wc"] + p["bc"], (x, states, y, norm, o, attend, pooled)
+
+    def backward(self, dscores, saved):
+        """(dx, gradients of the parameters in the order of PARAMETERS)."""
+        p = self.parameters
+        x, states, y, norm, o, attend, pooled = saved
+        dz = ((dscores @ p["Wc"].t()) / x.shape[1])[:, None, :].expand(x.shape).contiguous()
+        dq, dk, dv, dweights = self.attend.backward(dz @ p["Wo"].t(), attend)
+        dx, (dscale, doffset) = self.norm.backward(dq @ p["Wq"].t(), norm)
+        return dz + dx, [dscale, doffset, _by_weights(y, dq), _by_weights(states, dk), _by_weights(states, dv), dweights, _by_weights(o, dz),
+                         pooled.t() @ dscores, dscores.sum(0)]
+
+
+def _by_weights(inputs, gradient):      # sum over batch and tokens
+    return inputs.flatten(0, -2).t() @ gradient.flatten(0, -2)
 
 
 def _bounds_within(lb, ub, like):

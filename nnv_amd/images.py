@@ -297,3 +297,89 @@ def differential_attention_backward(do, q, k, v, weights, o, lse, second, key_le
     work = q.new_empty((need,), dtype=torch.uint8) if need else None
     check(lib.nnvhip_differential_attention_backward(ctx.handle, d, _ptr(work), need, stream))
     return dq, dk, dv, dweights
+
+
+# ---- layers -------------------------------------------------------------------------------------
+
+
+class GroupNormalizationLayer:
+    """A group normalization over NumGroups groups of the channels (the last dimension) and all places, with an Activation behind it (None, "relu"
+    or "silu"); properties as of the reference's normalization layers (nn/layers/BatchNormalizationLayer.m:33-83).  Scale and Offset are
+    device tensors or None."""
+
+    def __init__(self, NumGroups, **kw):
+        self.Name = kw.get("Name", "GroupNormalizationLayer")
+        self.NumGroups = int(NumGroups)
+        self.Scale = kw.get("Scale")
+        self.Offset = kw.get("Offset")
+        self.Epsilon = float(kw.get("Epsilon", 0.00001))
+        self.Activation = kw.get("Activation")
+        known = [p for p in (self.Scale, self.Offset) if p is not None]
+        self.NumChannels = kw.get("NumChannels") or (known[0].shape[0] if known else None)
+
+    def evaluate(self, x):
+        return self.forward(x)[0]
+
+    def forward(self, x):
+        """(y, what backward takes)."""
+        if self.NumChannels is not None and x.shape[-1] != self.NumChannels:
+            raise ValueError("Inconsistent number of channels between the input and the group normalization")
+        y, mean, rstd = group_norm(x, self.NumGroups, self.Scale, self.Offset, self.Epsilon, self.Activation)
+        return y, (x, mean, rstd)
+
+    def backward(self, dy, saved):
+        """(dx, [dScale, dOffset])."""
+        x, mean, rstd = saved
+        dx, dscale, doffset = group_norm_backward(dy, x, mean, rstd, self.Scale, self.Offset, self.Activation)
+        return dx, [dscale, doffset]
+
+
+class DifferentialAttentionLayer:
+    """Differential attention of NumHeads heads (two maps each) to keys and values of NumKeyValueHeads (NumHeads if not given); Weights: the second map's
+    weight in each head.  Inputs are batch x tokens x channels, the channels of all heads (and maps) side by side; with Sections, queries and keys are turned by the
+    positions that go with them (rotate_positions, Rotary: its other arguments)."""
+
+    def __init__(self, NumHeads, Weights, NumKeyValueHeads=None, Causal=False, Scale=None, Sections=None, Rotary=None, Name="DifferentialAttentionLayer"):
+        self.Name = Name
+        self.NumHeads = int(NumHeads)
+        self.NumKeyValueHeads = int(NumKeyValueHeads or NumHeads)
+        self.Weights = Weights
+        self.Causal = bool(Causal)
+        self.Scale = Scale
+        self.Sections = None if Sections is None else tuple(Sections)
+        self.Rotary = dict(Rotary or {})
+
+    def _heads(self, x, heads):
+        if x.dim() != 3 or x.shape[2] % heads:
+            raise ValueError("The channels of the input must be a multiple of the number of heads and maps")
+        return x.unflatten(2, (heads, x.shape[2] // heads))
+
+    def _turn(self, q, k, q_positions, k_positions, inverse=False):
+        if self.Sections is None:
+            return q, k
+        if q_positions is k_positions:
+            return rotate_positions([q, k], q_positions, self.Sections, inverse=inverse, **self.Rotary)
+        return tuple(rotate_positions(x, at, self.Sections, inverse=inverse, **self.Rotary) for x, at in ((q, q_positions), (k, k_positions)))
+
+    def evaluate(self, q, k, v, q_positions=None, k_positions=None, key_lengths=None, key_mask=None):
+        return self._forward(q, k, v, q_positions, k_positions, key_lengths, key_mask, False)[0]
+
+    def forward(self, q, k, v, q_positions=None, k_positions=None, key_lengths=None, key_mask=None):
+        """(o, what backward takes)."""
+        return self._forward(q, k, v, q_positions, k_positions, key_lengths, key_mask, True)
+
+    def _forward(self, q, k, v, q_positions, k_positions, key_lengths, key_mask, for_backward):
+        if self.Sections is not None and (q_positions is None or k_positions is None):
+            raise ValueError("Queries and keys that are turned need positions")
+        q, k, v = self._heads(q, 2 * self.NumHeads), self._heads(k, 2 * self.NumKeyValueHeads), self._heads(v, self.NumKeyValueHeads)
+        q, k = self._turn(q, k, q_positions, k_positions)
+        masks = {"key_lengths": key_lengths, "key_mask": key_mask, "causal": self.Causal, "scale": self.Scale}
+        o, lse, second = differential_attention(q, k, v, self.Weights, for_backward=for_backward, **masks)
+        return o.flatten(2), (q, k, v, o, lse, second, q_positions, k_positions, masks)
+
+    def backward(self, do, saved):
+        """(dq, dk, dv, dWeights)."""
+        q, k, v, o, lse, second, q_positions, k_positions, masks = saved
+        dq, dk, dv, dweights = differential_attention_backward(self._heads(do, self.NumHeads), q, k, v, self.Weights, o, lse, second, **masks)
+        dq, dk = self._turn(dq, dk, q_positions, k_positions, inverse=True)
+        return dq.flatten(2), dk.flatten(2), dv.flatten(2), dweights
