@@ -51,6 +51,14 @@ __device__ __forceinline__ float to_weights(float16_t (&s)[K], float unit, float
   total += sum[0] + sum[1];
   return fade;
 }
+// what rounding eight weights to p leaves
+template <typename T>
+__device__ __forceinline__ half8<T> rest8(const float16_t& s, const half8<T>& p, int first) {
+  half8<T> r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = (T)(s[first + i] - (float)p[i]);
+  return r;
+}
 // keys that do not take part: -inf.  word: of 32 keys, from this half's on
 __device__ __forceinline__ void mask_scores(float16_t& s, uint32_t word) {
 #pragma unroll
@@ -84,6 +92,7 @@ template <int CH>
 constexpr int differ_stages = CH == 2 || CH == 4 ? 4 : 2;
 template <typename T, int CH>
 __global__ __launch_bounds__(512, 2) void differ16_kernel(const DifferArgs a) {
+  constexpr bool TWO = std::is_same_v<T, f16_t>;
   constexpr int KEYS = 64, STAGES = differ_stages<CH>, DP = Width16<CH>::DP, W = Width16<CH>::W;
   typedef TripleLoad<T, CH, KEYS, 8> Load;
   __shared__ __attribute__((aligned(1024))) T lds[STAGES * Load::VALUES];
@@ -159,8 +168,14 @@ __global__ __launch_bounds__(512, 2) void differ16_kernel(const DifferArgs a) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const half8<T> p = round8<T>(s[k], 8 * c);
+        half8<T> rest = {};
+        if constexpr (TWO) rest = rest8<T>(s[k], p, 8 * c);
 #pragma unroll
-        for (int d = 0; d < CH; ++d) acc[d] = Half8<T>::mfma(columns_operand<T, W>(vs_at, 32 * k + 16 * c, d), p, acc[d]);
+        for (int d = 0; d < CH; ++d) {
+          const half8<T> x = columns_operand<T, W>(vs_at, 32 * k + 16 * c, d);
+          acc[d] = Half8<T>::mfma(x, p, acc[d]);
+          if constexpr (TWO) acc[d] = Half8<T>::mfma(x, rest, acc[d]);
+        }
       }
   }
   total = sum_of_halves(total);
@@ -289,10 +304,7 @@ __global__ __launch_bounds__(64 * differ_groups<CH>(), 1) void differ16_few_kern
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       p[c] = round8<T>(s[0], 8 * c);
-      float16_t left;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) left[i] = s[0][8 * c + i] - (float)p[c][i];
-      rest[c] = round8<T>(left, 0);
+      rest[c] = rest8<T>(s[0], p[c], 8 * c);
     }
     over_columns<T, W, 2>(vs_at, 0, [&](int c, int d, const half8<T>& v) {
       acc[d] = Half8<T>::mfma(v, p[c], acc[d]);

@@ -136,6 +136,7 @@ __global__ __launch_bounds__(64 * kWaves<CH>, kWaves<CH> / 4) void differ_query_
   load_operands<T, 2 * CH>(gf, (const T*)a.go.p + (here ? row_at(a.go, a, b, kv, r) : 0), h, 2 * a.head, takes_part);
   float16_t dq[2][1][DP / 32];
   Lift<T> lift[2];
+  float dot = 0.0f;   // D_1 again, of the weights and dP: what the weights' gradients add up (second is rounded)
 #pragma unroll
   for (int m = 0; m < 2; ++m) zero(dq[m][0]);
   const T* kp = (const T*)a.k.p + b * a.k.b + 2 * kv * a.k.h;
@@ -167,21 +168,31 @@ __global__ __launch_bounds__(64 * kWaves<CH>, kWaves<CH> / 4) void differ_query_
       float16_t dp[1], s[2][1];
       over_chunks<T, W, 2 * CH, 1, 4>(vs_at, 0, [&](int c) { return gf[c]; }, dp);
       const uint32_t word = ((uint32_t)(valid >> (32 * k)) & first_bits(seen - t * KEYS - 32 * k)) >> (4 * h);
+      if (masked)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dp[0][i] = word >> product_row(i, 0) & 1 ? dp[0][i] : 0.0f;
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         over_chunks<T, DP, CH, 1, 4>(ks_at + m * (2 * Load::MAP), 0, [&](int c) { return qf[m][c]; }, s[m]);
         const float by = m ? -w : 1.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[m][0][i] = exp2_(s[m][0][i] * unit - offset[m]) * (by * (dp[0][i] - delta[m]));
+        for (int i = 0; i < 16; ++i) s[m][0][i] = exp2_(s[m][0][i] * unit - offset[m]);
         if (masked)
 #pragma unroll
           for (int i = 0; i < 16; ++i) s[m][0][i] = word >> product_row(i, 0) & 1 ? s[m][0][i] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if (m) dot += s[m][0][i] * dp[0][i];
+          s[m][0][i] *= by * (dp[0][i] - delta[m]);
+        }
         lift[m].raise(&s[m], dq[m]);
         over_rows<T, DP>(kc_at + m * (2 * Load::MAP), 0, s[m][0], dq[m][0]);
       }
     }
   }
+  dot = sum_of_halves(dot);
   if (!here) return;
+  if (h == 0) a.dots[(split * (int64_t)a.batch * a.kv_heads + bkv) * a.rows + r] = dot;
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
     if (a.splits > 1) store_result(a.part + (split * own_rows(a) + own_row(a, bkv, r, m)) * a.head, dq[m][0], a.scale * lift[m].down(), h, a.head);

@@ -52,22 +52,32 @@ __global__ __launch_bounds__(256) void differ_delta_kernel(const DifferArgs a) {
   for (int k = 0; k < kInfos; ++k) info[k * per] = values[k];
 }
 
-// dw of a head: a block adds its rows' D_1, in f64.
+// dw of a head: a block adds its rows' D_1 (of all splits, where the kernel of dq found it), in f64.
 template <typename T, int>
-__global__ __launch_bounds__(256) void differ_weights_kernel(const DifferArgs a) {
-  __shared__ double lds[4];
+__global__ __launch_bounds__(1024) void differ_weights_kernel(const DifferArgs a) {
+  __shared__ double lds[16];
   const int head = blockIdx.x, kv = head / a.group, g = head % a.group;
   double s = 0;
-  for (int b = 0; b < a.batch; ++b) {
-    const float* from = a.delta + own_row(a, b * (int64_t)a.kv_heads + kv, (int64_t)g * a.queries, 1);
-    for (int i = threadIdx.x; i < a.queries; i += 256) s += (double)from[i];
+  const int sets = a.dots ? a.splits * a.batch : a.batch;
+  for (int k = 0; k < sets; ++k) {
+    const int64_t bkv = k % a.batch * (int64_t)a.kv_heads + kv;
+    const float* from = a.dots ? a.dots + (k / a.batch * (int64_t)a.batch * a.kv_heads + bkv) * a.rows + (int64_t)g * a.queries
+                               : a.delta + own_row(a, bkv, (int64_t)g * a.queries, 1);
+    int i = threadIdx.x;
+    for (; i + 3 * 1024 < a.queries; i += 4 * 1024) {
+      const float x[4] = {from[i], from[i + 1024], from[i + 2048], from[i + 3072]};
+      s += ((double)x[0] + (double)x[1]) + ((double)x[2] + (double)x[3]);
+    }
+    for (; i < a.queries; i += 1024) s += (double)from[i];
   }
 #pragma unroll
   for (int k = 32; k > 0; k >>= 1) s += __shfl_xor(s, k, 64);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
   __syncthreads();
   if (threadIdx.x) return;
-  const float all = (float)-(lds[0] + lds[1] + lds[2] + lds[3]);
+  double sum = 0;
+  for (int k = 0; k < 16; ++k) sum += lds[k];
+  const float all = (float)-sum;
   if (a.wide_weights) ((float*)a.dweights)[head] = all;
   else ((T*)a.dweights)[head] = from_f<T>(all);
 }
@@ -286,7 +296,7 @@ __global__ __launch_bounds__(256) void differ_sum_rows_kernel(const DifferArgs a
 
 struct GradCut {
   int row_tiles, key_tiles, key_blocks, query_splits, key_splits;
-  int64_t delta, info, part;   // floats of the workspace
+  int64_t delta, info, dots, part;   // floats of the workspace
 };
 GradCut grad_cut(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys, int64_t head, bool causal, bool by16) {
   GradCut c;
@@ -299,6 +309,7 @@ GradCut grad_cut(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys, in
   c.key_splits = split_of(batch * kv_heads * c.key_blocks, ceil_div(rows, 32), 2, by16 || head > 64 ? 256 : 512, start, join);
   c.delta = round_up(batch * kv_heads * 2 * rows, 64);
   c.info = by16 ? batch * kv_heads * kInfos * round_up(rows, kInfoRows) : 0;
+  c.dots = by16 ? round_up(c.query_splits * batch * kv_heads * rows, 64) : 0;
   const int64_t q = c.query_splits > 1 ? c.query_splits * batch * kv_heads * 2 * rows * head : 0;
   const int64_t k = c.key_splits > 1 ? 2 * c.key_splits * batch * kv_heads * keys * 2 * head : 0;
   c.part = std::max(q, k);
@@ -323,7 +334,7 @@ void launch_grad(DifferArgs a, const GradCut& c, bool by16, hipStream_t st) {
   } else {
     a.batch = 0;   // (for the sums over no rows)
   }
-  hipLaunchKernelGGL((differ_weights_kernel<T, 0>), dim3((unsigned)(a.kv_heads * a.group)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((differ_weights_kernel<T, 0>), dim3((unsigned)(a.kv_heads * a.group)), dim3(1024), 0, st, a);
   if (a.keys > 0 && heads > 0) {
     a.batch = (int)(heads / a.kv_heads);
     a.key_tiles = c.key_tiles;
@@ -359,7 +370,7 @@ int nnvhip_differential_attention_backward_workspace(const nnvhip_differ_args* d
     if (heads * c.row_tiles * c.query_splits > blocks) NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_differential_attention_backward: too many rows");
     if (heads * c.key_blocks * c.key_splits > blocks || (c.key_splits > 1 && ceil_div(heads * d->keys * 2 * d->head, 256) > blocks))
       NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_differential_attention_backward: too many keys");
-    *bytes = std::max(*bytes, (c.delta + c.info + c.part) * (int64_t)sizeof(float));
+    *bytes = std::max(*bytes, (c.delta + c.info + c.dots + c.part) * (int64_t)sizeof(float));
   }
   return NNVHIP_OK;
 }
@@ -377,7 +388,8 @@ int nnvhip_differential_attention_backward(nnvhip_ctx* ctx, const nnvhip_differ_
   a.delta = static_cast<float*>(workspace);
   a.info = c.info ? a.delta + c.delta : nullptr;
   a.info_rows = (int)round_up(a.rows, kInfoRows);
-  a.part = a.delta + c.delta + c.info;
+  a.dots = c.dots ? a.delta + c.delta + c.info : nullptr;
+  a.part = a.delta + c.delta + c.info + c.dots;
   DIFFER_BY_TYPE(d->type, launch_grad, a, c, by16, (hipStream_t)stream);
   NNV_HIP_TRY(hipGetLastError());
   return NNVHIP_OK;
