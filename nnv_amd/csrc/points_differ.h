@@ -123,6 +123,17 @@ __device__ __forceinline__ BlockPlace block_place(const DifferArgs& a, int64_t i
   return p;
 }
 
+// store_four where sizes are multiples of four: no code for what is behind the last one (of which the 16-bit kernels had more than of all else, and
+// fetched it from memory where they run for a few microseconds)
+template <typename T>
+__device__ __forceinline__ void put_four(T* row, int d, int size, const float (&f)[4]) {
+  if (d >= size) return;
+  T t[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) t[i] = from_f<T>(f[i]);
+  __builtin_memcpy(row + d, t, sizeof(t));
+}
+
 // low bits of a word of 32 (or 64) keys: those in front of `seen`
 __device__ __forceinline__ uint32_t first_bits(int seen) { return seen >= 32 ? ~0u : seen <= 0 ? 0u : (1u << seen) - 1; }
 
@@ -236,12 +247,13 @@ __device__ __forceinline__ void f32_zero(float4_t (&acc)[N]) {
 #pragma unroll
   for (int d = 0; d < N; ++d) acc[d] = float4_t{0, 0, 0, 0};
 }
-template <typename T, int N>
+template <bool FOUR, typename T, int N>
 __device__ __forceinline__ void f32_store(T* row, const float4_t (&acc)[N], float by, int q4, int size) {
 #pragma unroll
   for (int d = 0; d < N; ++d) {
     const float f[4] = {acc[d][0] * by, acc[d][1] * by, acc[d][2] * by, acc[d][3] * by};
-    store_four(row, 16 * d + 4 * q4, size, f);
+    if constexpr (FOUR) put_four(row, 16 * d + 4 * q4, size, f);
+    else store_four(row, 16 * d + 4 * q4, size, f);
   }
 }
 // which of the 8 keys (or rows) 16 k + 4 q4 + i of 32 a lane's registers are

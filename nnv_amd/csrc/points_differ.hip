@@ -90,7 +90,7 @@ __global__ __launch_bounds__(512, 2) void differ_kernel(const DifferArgs a) {
     if (!here) return;
     const int64_t own = split * own_rows(a) + own_row(a, bkv, r, map);
     if (q4 == 0) a.part_lse[own] = lse;
-    f32_store(a.part + own * 2 * a.head, acc, inv, q4, 2 * a.head);
+    f32_store<FOUR>(a.part + own * 2 * a.head, acc, inv, q4, 2 * a.head);
     return;
   }
   if (here && q4 == 0) a.lse[lse_at(a, b, kv, r, map)] = lse;
@@ -102,7 +102,7 @@ __global__ __launch_bounds__(512, 2) void differ_kernel(const DifferArgs a) {
       const float f[4] = {acc[d][0] * inv, acc[d][1] * inv, acc[d][2] * inv, acc[d][3] * inv};
       __builtin_memcpy(found + 256 * d, f, 16);
     }
-    if (a.second && here) f32_store((T*)a.second + wide_row_at(a, b, kv, r), acc, inv, q4, 2 * a.head);
+    if (a.second && here) f32_store<FOUR>((T*)a.second + wide_row_at(a, b, kv, r), acc, inv, q4, 2 * a.head);
   }
   __syncthreads();
   if (map || !here) return;
@@ -114,7 +114,7 @@ __global__ __launch_bounds__(512, 2) void differ_kernel(const DifferArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[d][i] = rounded(acc[d][i] * inv) - w * f[i];   // (of equal maps and a weight of one nothing is left)
   }
-  f32_store((T*)a.out + wide_row_at(a, b, kv, r), acc, 1.0f, q4, 2 * a.head);
+  f32_store<FOUR>((T*)a.out + wide_row_at(a, b, kv, r), acc, 1.0f, q4, 2 * a.head);
 }
 
 // The parts of a row's two maps, joined: 64 lanes (four values each, of up to 256) a row, SLICES of which take the splits in turn.

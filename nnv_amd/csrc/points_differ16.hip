@@ -190,7 +190,7 @@ __global__ __launch_bounds__(512, 2) void differ16_kernel(const DifferArgs a) {
 #pragma unroll
       for (int i4 = 0; i4 < 4; ++i4) {
         const float f[4] = {acc[d][4 * i4] * inv, acc[d][4 * i4 + 1] * inv, acc[d][4 * i4 + 2] * inv, acc[d][4 * i4 + 3] * inv};
-        store_four(a.part + own * size, d * 32 + 8 * i4 + 4 * h, size, f);
+        put_four(a.part + own * size, d * 32 + 8 * i4 + 4 * h, size, f);
       }
     return;
   }
@@ -206,7 +206,7 @@ __global__ __launch_bounds__(512, 2) void differ16_kernel(const DifferArgs a) {
       for (int i4 = 0; i4 < 4; ++i4) {
         const float f[4] = {acc[d][4 * i4] * inv, acc[d][4 * i4 + 1] * inv, acc[d][4 * i4 + 2] * inv, acc[d][4 * i4 + 3] * inv};
         __builtin_memcpy(found + 256 * (4 * d + i4), f, 16);
-        if (a.second && here) store_four((T*)a.second + dense, d * 32 + 8 * i4 + 4 * h, size, f);
+        if (a.second && here) put_four((T*)a.second + dense, d * 32 + 8 * i4 + 4 * h, size, f);
       }
   }
   __syncthreads();
@@ -220,7 +220,7 @@ __global__ __launch_bounds__(512, 2) void differ16_kernel(const DifferArgs a) {
       __builtin_memcpy(f, found + 256 * (4 * d + i4), 16);
 #pragma unroll
       for (int i = 0; i < 4; ++i) f[i] = rounded(acc[d][4 * i4 + i] * inv) - w * f[i];
-      store_four((T*)a.out + dense, d * 32 + 8 * i4 + 4 * h, size, f);
+      put_four((T*)a.out + dense, d * 32 + 8 * i4 + 4 * h, size, f);
     }
 }
 
@@ -354,15 +354,15 @@ __global__ __launch_bounds__(64 * differ_groups<CH>(), 1) void differ16_few_kern
       for (int i = 0; i < 4; ++i) f[m][i] = rounded(f[m][i] * inv);
       const int64_t own = split * own_rows(a) + own_row(a, bkv, rj, m);
       if (d == 0) (a.splits > 1 ? a.part_lse[own] : a.lse[lse_at(a, b, kv, rj, m)]) = lse;
-      if (a.splits > 1 && d < size) store_four(a.part + own * size, d, size, f[m]);
+      if (a.splits > 1 && d < size) put_four(a.part + own * size, d, size, f[m]);
     }
     if (a.splits > 1 || d >= size) continue;
     const int64_t dense = wide_row_at(a, b, kv, rj);
-    if (a.second) store_four((T*)a.second + dense, d, size, f[1]);
+    if (a.second) put_four((T*)a.second + dense, d, size, f[1]);
     const float w = weight_of<T>(a, head_of_row(a, kv, rj));
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[0][i] -= w * f[1][i];
-    store_four((T*)a.out + dense, d, size, f[0]);
+    put_four((T*)a.out + dense, d, size, f[0]);
   }
 }
 

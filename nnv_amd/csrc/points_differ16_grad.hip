@@ -85,7 +85,7 @@ __device__ __forceinline__ void store_result(T* row, const float16_t (&acc)[N], 
 #pragma unroll
     for (int i4 = 0; i4 < 4; ++i4) {
       const float f[4] = {acc[d][4 * i4] * by, acc[d][4 * i4 + 1] * by, acc[d][4 * i4 + 2] * by, acc[d][4 * i4 + 3] * by};
-      store_four(row, d * 32 + 8 * i4 + 4 * h, size, f);
+      put_four(row, d * 32 + 8 * i4 + 4 * h, size, f);
     }
 }
 template <typename T, int VALUES, int THREADS>

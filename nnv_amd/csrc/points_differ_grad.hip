@@ -146,8 +146,8 @@ __global__ __launch_bounds__(256, CH <= 6 ? 2 : 1) void differ_query_grad_kernel
   if (!here) return;
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
-    if (a.splits > 1) f32_store(a.part + (split * own_rows(a) + own_row(a, bkv, r, m)) * a.head, dq[m], a.scale, q4, a.head);
-    else f32_store((T*)a.dq + dense_map_row_at(a, b, kv, r, m), dq[m], a.scale, q4, a.head);
+    if (a.splits > 1) f32_store<FOUR>(a.part + (split * own_rows(a) + own_row(a, bkv, r, m)) * a.head, dq[m], a.scale, q4, a.head);
+    else f32_store<FOUR>((T*)a.dq + dense_map_row_at(a, b, kv, r, m), dq[m], a.scale, q4, a.head);
   }
 }
 
@@ -252,12 +252,12 @@ __global__ __launch_bounds__(256, CH <= 4 ? 2 : 1) void differ_key_grad_kernel(c
       if (a.splits > 1) {
         const int64_t all = (int64_t)a.batch * a.keys * a.kv_heads * 2 * a.head;
 #pragma unroll
-        for (int m = 0; m < 2; ++m) f32_store(a.part + split * all + dense + m * a.head, dk[m], a.scale, q4, a.head);
-        f32_store(a.part + (a.splits + split) * all + dense, dv, 1.0f, q4, 2 * a.head);
+        for (int m = 0; m < 2; ++m) f32_store<FOUR>(a.part + split * all + dense + m * a.head, dk[m], a.scale, q4, a.head);
+        f32_store<FOUR>(a.part + (a.splits + split) * all + dense, dv, 1.0f, q4, 2 * a.head);
       } else {
 #pragma unroll
-        for (int m = 0; m < 2; ++m) f32_store((T*)a.dk + dense + m * a.head, dk[m], a.scale, q4, a.head);
-        f32_store((T*)a.dv + dense, dv, 1.0f, q4, 2 * a.head);
+        for (int m = 0; m < 2; ++m) f32_store<FOUR>((T*)a.dk + dense + m * a.head, dk[m], a.scale, q4, a.head);
+        f32_store<FOUR>((T*)a.dv + dense, dv, 1.0f, q4, 2 * a.head);
       }
     }
     if (key_tile != block || blocks == a.key_tiles || a.key_tiles - 1 - block == block) break;

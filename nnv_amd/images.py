@@ -151,6 +151,17 @@ def _frequencies(sections, base, shared):
     return (C.c_double * pairs)(*values), (C.c_uint8 * pairs)(*axes)
 
 
+@functools.lru_cache(maxsize=64)
+def _turns(sections, base, shared):
+    """(pairs, axes, addresses of _frequencies, which they belong to) of a call's arguments, or the error."""
+    if not sections or not all(isinstance(n, int) and n >= 0 for n in sections) or not 1 <= sum(sections) <= _ROTATE_PAIRS or len(sections) > 255:
+        raise ValueError("rotate_positions: sections are numbers of pairs, one per axis, %d together at most" % _ROTATE_PAIRS)
+    if not 0 < base < float("inf"):
+        raise ValueError("rotate_positions: the base must be positive and finite")
+    held = _frequencies(sections, float(base), shared)
+    return sum(sections), len(sections), C.addressof(held[0]), C.addressof(held[1]), held
+
+
 def rotate_positions(x, positions, sections, base=10000.0, shared=False, interleaved=False, inverse=False, ctx=None):
     """x with its heads' values turned by their tokens' positions: rotary positions with several axes.
 
@@ -167,35 +178,35 @@ def rotate_positions(x, positions, sections, base=10000.0, shared=False, interle
     if not tensors:
         raise ValueError("%s: at least one tensor is expected" % what)
     ctx, lib, stream = _enter(what, ctx, tensors[0], *tensors[1:], positions)
-    sections = tuple(sections)
     first = tensors[0]
     t = _type(what, first)
-    if not sections or not all(isinstance(n, int) and n >= 0 for n in sections) or not 1 <= sum(sections) <= _ROTATE_PAIRS or len(sections) > 255:
-        raise ValueError("%s: sections are numbers of pairs, one per axis, %d together at most" % (what, _ROTATE_PAIRS))
-    if not 0 < base < float("inf"):
-        raise ValueError("%s: the base must be positive and finite" % what)
-    for y in tensors:
-        if y.dim() != 4 or y.dtype != first.dtype or y.shape[:2] != first.shape[:2] or y.shape[3] != first.shape[3]:
-            raise ValueError("%s: tensors are batch x tokens x heads x head, alike but for the number of heads" % what)
+    pairs, axes, frequency, axis, _ = _turns(tuple(sections), base, bool(shared))
+    if first.dim() != 4:
+        raise ValueError("%s: tensors are batch x tokens x heads x head, alike but for the number of heads" % what)
     batch, tokens, _, head = first.shape
-    if head < 2 * sum(sections):
-        raise ValueError("%s: heads of %d values do not hold %d pairs" % (what, head, sum(sections)))
-    if positions.dtype not in _POSITIONS or positions.dim() not in (2, 3) or positions.shape[-2:] != (tokens, len(sections)) or \
-            (positions.dim() == 3 and positions.shape[0] != batch):
-        raise ValueError("%s: positions are (batch x) tokens x axes whole numbers or float32, not %s %s" %
-                         (what, positions.dtype, tuple(positions.shape)))
-    stride = positions.stride() if positions.dim() == 3 else (0, *positions.stride())
-    frequency, axis = _frequencies(sections, float(base), bool(shared))
+    for y in tensors[1:]:
+        if y.dim() != 4 or y.dtype != first.dtype or y.shape[:2] != first.shape[:2] or y.shape[3] != head:
+            raise ValueError("%s: tensors are batch x tokens x heads x head, alike but for the number of heads" % what)
+    if head < 2 * pairs:
+        raise ValueError("%s: heads of %d values do not hold %d pairs" % (what, head, pairs))
+    kind, shape, stride = _POSITIONS.get(positions.dtype), positions.shape, positions.stride()
+    if len(shape) == 2:
+        stride = (0, *stride)
+    if kind is None or len(shape) not in (2, 3) or shape[-2:] != (tokens, axes) or (len(shape) == 3 and shape[0] != batch):
+        raise ValueError("%s: positions are (batch x) tokens x axes whole numbers or float32, not %s %s" % (what, positions.dtype, tuple(shape)))
+    fixed = (t, batch, tokens, head)
+    turned = (pairs, axes, bool(interleaved), bool(inverse), kind, positions.data_ptr(), *stride, frequency, axis)
     done = []
     for k in range(0, len(tensors), _ROTATE_TENSORS):
         part = [y if y.stride(3) == 1 or head == 1 else y.contiguous() for y in tensors[k:k + _ROTATE_TENSORS]]
         out = [torch.empty_like(y, memory_format=torch.contiguous_format) for y in part]
-        none = [0] * (_ROTATE_TENSORS - len(part))
-        strides = [s for y in part for s in y.stride()[:3]]
-        d = _ROTATE.pack(t, batch, tokens, head, len(part), sum(sections), len(sections), bool(interleaved), bool(inverse),
-                         _POSITIONS[positions.dtype], positions.data_ptr(), *stride, C.addressof(frequency), C.addressof(axis),
-                         *[y.shape[2] for y in part], *none, *[y.data_ptr() for y in part], *none, *[y.data_ptr() for y in out], *none,
-                         *strides, *[0] * (12 - len(strides)))
+        none = (0,) * (_ROTATE_TENSORS - len(part))
+        heads, strides = [], []
+        for y in part:
+            heads.append(y.shape[2])
+            strides += y.stride()[:3]
+        d = _ROTATE.pack(*fixed, len(part), *turned, *heads, *none, *[y.data_ptr() for y in part], *none, *[y.data_ptr() for y in out], *none,
+                         *strides, *none, *none, *none)
         check(lib.nnvhip_rotate_positions(ctx.handle, d, stream))
         done += out
     return done if several else done[0]

@@ -108,7 +108,9 @@ def test_workspaces_and_their_refusals():
         _lib.check(fn(images._GROUP.pack(*s.values(), 1e-5, *[0] * 14), C.byref(n)))
         return n.value
 
-    assert group() >= 4 * 8 * 16 and group(backward=True) >= group() + 4 * 64 * 8 and group(batch=0) == 0
+    # sums of parts of the places, where they are too many for a block; sums of the channels in the backward pass
+    assert group() == 0 and group(places=1 << 20) >= 4 * 8 * 16 and group(backward=True) >= 4 * 64 * 8 and group(batch=0) == 0
+    assert group(backward=True, places=1 << 20) >= group(places=1 << 20) + 4 * 64 * 8
     # what is kept of long places stays a small part of them
     assert group(backward=True, places=1 << 24, batch=1) < (1 << 24) * 64 * 2 / 16
     assert group(channels=1 << 20, groups=1) > 0 and group(channels=5000, groups=5000) > 0
