@@ -91,8 +91,12 @@ __device__ __forceinline__ int row_tile_of(const DifferArgs& a, int x) {
   return a.causal && x < each * a.group ? x % a.group * each + each - 1 - x / a.group : x;
 }
 // Blocks of the kernels over keys.  Causal: a tile of early keys is seen by most rows, one of late keys by few, and a block takes one of either (and
-// where their number is odd, one block the middle one alone).
-__host__ __device__ inline int key_blocks_of(int key_tiles, bool causal) { return causal ? (key_tiles + 1) / 2 : key_tiles; }
+// where their number is odd, one block the middle one alone).  Not where the tiles are few, or few of the keys are hidden from any row (8 x 16 x 504, 2 heads
+// of 96: 29 us, in pairs 49; 2 x 4096 x 4096, 16 / 4 heads of 64: 650, in pairs 430).
+__host__ __device__ inline int key_blocks_of(int key_tiles, int64_t queries, int64_t keys, bool causal) {
+  return causal && key_tiles >= 6 && queries >= keys / 2 ? (key_tiles + 1) / 2 : key_tiles;
+}
+__device__ __forceinline__ int key_blocks_of(const DifferArgs& a) { return key_blocks_of(a.key_tiles, a.queries, a.keys, a.causal); }
 
 // Where a block works: (sequence, key/value head) and one of `each` blocks of it.  Blocks are dealt to the 8 XCDs in turn, and those of a key/value head
 // go to one, whose L2 then holds its keys; sequences go by length, the longest first, so that short blocks fill what is left at the end.

@@ -209,7 +209,7 @@ __global__ __launch_bounds__(64 * kKeyWaves<CH>, kKeyWaves<CH> / 4) void differ_
   __shared__ __attribute__((aligned(1024))) T lds[2 * Load::VALUES + WAVES * 512 * PARKED];
   __shared__ __attribute__((aligned(1024))) float info[2][kInfos * ROWS < 256 ? 256 : 512];   // [buffer][RowInfo * ROWS + row]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
-  const int blocks = key_blocks_of(a.key_tiles, a.causal);
+  const int blocks = key_blocks_of(a);
   const BlockPlace at = block_place(a, blockIdx.x, (int64_t)blocks * a.splits);
   const int b = at.b, kv = at.kv, bkv = b * a.kv_heads + kv, split = at.x % a.splits, block = at.x / a.splits;
   const int n = keys_that_count(a, b);
@@ -395,7 +395,7 @@ void launch_query(const DifferArgs& a, hipStream_t st) {
 }
 template <typename T, int CH>
 void launch_key(const DifferArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((differ_key_grad16_kernel<T, CH>), dim3((unsigned)((int64_t)a.batch * a.kv_heads * key_blocks_of(a.key_tiles, a.causal) * a.splits)), dim3(64 * kKeyWaves<CH>), 0,
+  hipLaunchKernelGGL((differ_key_grad16_kernel<T, CH>), dim3((unsigned)((int64_t)a.batch * a.kv_heads * key_blocks_of(a.key_tiles, a.queries, a.keys, a.causal) * a.splits)), dim3(64 * kKeyWaves<CH>), 0,
                      st, a);
 }
 

@@ -58,17 +58,17 @@ __global__ __launch_bounds__(1024) void differ_weights_kernel(const DifferArgs a
   __shared__ double lds[16];
   const int head = blockIdx.x, kv = head / a.group, g = head % a.group;
   double s = 0;
-  const int sets = a.dots ? a.splits * a.batch : a.batch;
-  for (int k = 0; k < sets; ++k) {
+  // a wave takes 256 rows of a set at a time
+  const int sets = a.dots ? a.splits * a.batch : a.batch, each = (a.queries + 255) / 256;
+  for (int64_t unit = threadIdx.x >> 6; unit < sets * (int64_t)each; unit += 16) {
+    const int k = (int)(unit / each), first = (int)(unit - k * (int64_t)each) * 256 + (threadIdx.x & 63);
     const int64_t bkv = k % a.batch * (int64_t)a.kv_heads + kv;
     const float* from = a.dots ? a.dots + (k / a.batch * (int64_t)a.batch * a.kv_heads + bkv) * a.rows + (int64_t)g * a.queries
                                : a.delta + own_row(a, bkv, (int64_t)g * a.queries, 1);
-    int i = threadIdx.x;
-    for (; i + 3 * 1024 < a.queries; i += 4 * 1024) {
-      const float x[4] = {from[i], from[i + 1024], from[i + 2048], from[i + 3072]};
-      s += ((double)x[0] + (double)x[1]) + ((double)x[2] + (double)x[3]);
-    }
-    for (; i < a.queries; i += 1024) s += (double)from[i];
+    float x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = first + 64 * j < a.queries ? from[first + 64 * j] : 0.0f;
+    s += ((double)x[0] + (double)x[1]) + ((double)x[2] + (double)x[3]);
   }
 #pragma unroll
   for (int k = 32; k > 0; k >>= 1) s += __shfl_xor(s, k, 64);
@@ -157,7 +157,7 @@ __global__ __launch_bounds__(256, CH <= 4 ? 2 : 1) void differ_key_grad_kernel(c
   __shared__ __attribute__((aligned(16))) float tile[F32Tile<CH>::FLOATS];
   __shared__ __attribute__((aligned(16))) float offsets[2][R], deltas[2][R], weights[R], seen_by_row[R];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, q4 = lane >> 4;
-  const int blocks = key_blocks_of(a.key_tiles, a.causal);
+  const int blocks = key_blocks_of(a);
   const BlockPlace at = block_place(a, blockIdx.x, (int64_t)blocks * a.splits);
   const int b = at.b, kv = at.kv, bkv = b * a.kv_heads + kv, split = at.x % a.splits, block = at.x / a.splits;
   const int n = keys_that_count(a, b);
@@ -298,11 +298,11 @@ struct GradCut {
   int row_tiles, key_tiles, key_blocks, query_splits, key_splits;
   int64_t delta, info, dots, part;   // floats of the workspace
 };
-GradCut grad_cut(int64_t batch, int64_t kv_heads, int64_t rows, int64_t keys, int64_t head, bool causal, bool by16) {
+GradCut grad_cut(int64_t batch, int64_t kv_heads, int64_t queries, int64_t rows, int64_t keys, int64_t head, bool causal, bool by16) {
   GradCut c;
   c.row_tiles = (int)ceil_div(rows, by16 ? differ_grad16_tile(head) : kBlockRows);
   c.key_tiles = (int)ceil_div(keys, by16 ? differ_key_grad16_tile(head) : kBlockRows);
-  c.key_blocks = key_blocks_of(c.key_tiles, causal);
+  c.key_blocks = key_blocks_of(c.key_tiles, queries, keys, causal);
   // blocks that the chip holds at once; what starting a block, and adding splits up, costs in tiles of 32 rows
   const int64_t start = by16 ? 6 : 2, join = by16 ? 12 : 3;
   c.query_splits = split_of(batch * kv_heads * c.row_tiles, ceil_div(keys, 32), 2, by16 || head > 96 ? 256 : 512, start, join);
@@ -366,7 +366,7 @@ int nnvhip_differential_attention_backward_workspace(const nnvhip_differ_args* d
   if (heads * ceil_div(d->keys, kBlockRows) > blocks) NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_differential_attention_backward: too many keys");
   *bytes = 0;   // whichever kernels the alignment of the tensors lets take the call
   for (const bool by16 : {false, true}) {
-    const GradCut c = grad_cut(d->batch, d->kv_heads, d->queries * (d->heads / d->kv_heads), d->keys, d->head, d->causal != 0, by16);
+    const GradCut c = grad_cut(d->batch, d->kv_heads, d->queries, d->queries * (d->heads / d->kv_heads), d->keys, d->head, d->causal != 0, by16);
     if (heads * c.row_tiles * c.query_splits > blocks) NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_differential_attention_backward: too many rows");
     if (heads * c.key_blocks * c.key_splits > blocks || (c.key_splits > 1 && ceil_div(heads * d->keys * 2 * d->head, 256) > blocks))
       NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_differential_attention_backward: too many keys");
@@ -384,7 +384,7 @@ int nnvhip_differential_attention_backward(nnvhip_ctx* ctx, const nnvhip_differ_
   if (need > workspace_bytes || (need && !workspace))
     NNV_FAIL(NNVHIP_ERR_ARG, "nnvhip_differential_attention_backward: a workspace of %lld bytes is needed", (long long)need);
   const bool by16 = differ_grad16_takes(a, (int)d->type);
-  const GradCut c = grad_cut(a.batch, a.kv_heads, a.rows, a.keys, a.head, a.causal, by16);
+  const GradCut c = grad_cut(a.batch, a.kv_heads, a.queries, a.rows, a.keys, a.head, a.causal, by16);
   a.delta = static_cast<float*>(workspace);
   a.info = c.info ? a.delta + c.delta : nullptr;
   a.info_rows = (int)round_up(a.rows, kInfoRows);
