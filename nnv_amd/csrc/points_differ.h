@@ -143,7 +143,7 @@ __device__ __forceinline__ uint32_t first_bits(int seen) { return seen >= 32 ? ~
 
 int differ_args(const char* what, const nnvhip_differ_args* d, bool backward, DifferArgs* a);
 
-// lse of a row as the exponent's offset in powers of two; a row without keys takes no part (exp2(s - inf) = 0)
+// lse of a row as the exponent's offset in powers of two; a row without keys takes no part (exp2(s - inf) = 0), one with missing values does
 __device__ __forceinline__ float offset_of(float lse) { return lse == -INFINITY ? INFINITY : lse * kLog2e; }
 
 // Which template takes a head size: chunks of 16 values of a map's head, of 32 of v's.

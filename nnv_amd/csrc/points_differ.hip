@@ -219,7 +219,7 @@ int check_sizes(const char* what, const nnvhip_differ_args* d) {
   if (d->batch * d->kv_heads * ceil_div(d->queries * group, kRows) > blocks) NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: too many rows", what);
   for (const bool by16 : {false, true}) {
     const Cut c = cut_of(d->batch, d->kv_heads, d->queries * group, d->keys, d->head, by16);
-    if (d->batch * d->kv_heads * c.row_tiles * c.splits > blocks || d->batch * d->heads * d->queries >= (int64_t(1) << (c.splits > 8 ? 23 : 25)))
+    if (d->batch * d->kv_heads * c.row_tiles * c.splits > blocks || (c.splits > 1 && d->batch * d->heads * d->queries >= (int64_t(1) << 23)))
       NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: too many rows", what);
   }
   return NNVHIP_OK;

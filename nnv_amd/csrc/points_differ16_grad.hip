@@ -125,7 +125,7 @@ __global__ __launch_bounds__(64 * kWaves<CH>, kWaves<CH> / 4) void differ_query_
   float offset[2], delta[2];
 #pragma unroll
   for (int m = 0; m < 2; ++m) offset[m] = offset_of(here ? a.lse[lse_at(a, b, kv, r, m)] : -INFINITY);
-  const bool takes_part = offset[0] < INFINITY;
+  const bool takes_part = offset[0] != INFINITY;
 #pragma unroll
   for (int m = 0; m < 2; ++m) delta[m] = takes_part ? a.delta[own_row(a, bkv, r, m)] : 0.0f;
   const int seen = takes_part ? seen_by(a, r, n) : 0;
@@ -295,7 +295,7 @@ __global__ __launch_bounds__(64 * kKeyWaves<CH>, kKeyWaves<CH> / 4) void differ_
       t = next_row_tile(a, t + 1, ROWS, i_min);
       if (t < t1) fetch(t, buffer ^ 1);
       // rows past the last one, and those that see no key: nothing of them may reach a sum
-      const uint64_t valid = __ballot(info[buffer][kOffset0 * ROWS + lane % ROWS] < INFINITY);
+      const uint64_t valid = __ballot(info[buffer][kOffset0 * ROWS + lane % ROWS] != INFINITY);
       if (valid != ~0ull) {
         T* tile = lds + buffer * Load::VALUES;
         zero_rows<T, DP, ROWS>(tile, valid, lane);

@@ -98,7 +98,7 @@ __global__ __launch_bounds__(256, CH <= 6 ? 2 : 1) void differ_query_grad_kernel
   float offset[2], delta[2];
 #pragma unroll
   for (int m = 0; m < 2; ++m) offset[m] = offset_of(here ? a.lse[lse_at(a, b, kv, r, m)] : -INFINITY);
-  const bool takes_part = offset[0] < INFINITY;
+  const bool takes_part = offset[0] != INFINITY;
 #pragma unroll
   for (int m = 0; m < 2; ++m) delta[m] = takes_part ? a.delta[own_row(a, bkv, r, m)] : 0.0f;
   const int seen = takes_part ? seen_by(a, r, n) : 0;
@@ -206,7 +206,7 @@ __global__ __launch_bounds__(256, CH <= 4 ? 2 : 1) void differ_key_grad_kernel(c
     while (t < t1) {
       __syncthreads();
       // a row without keys counts for nothing: what it holds must not reach the sums
-      next.store(tile, (uint32_t)__ballot(next_offset[0] < INFINITY), a.head, threadIdx.x);
+      next.store(tile, (uint32_t)__ballot(next_offset[0] != INFINITY), a.head, threadIdx.x);
       if (threadIdx.x < R) {
 #pragma unroll
         for (int m = 0; m < 2; ++m) {

@@ -158,7 +158,7 @@ def _turns(sections, base, shared):
         raise ValueError("rotate_positions: sections are numbers of pairs, one per axis, %d together at most" % _ROTATE_PAIRS)
     if not 0 < base < float("inf"):
         raise ValueError("rotate_positions: the base must be positive and finite")
-    held = _frequencies(sections, float(base), shared)
+    held = _frequencies(sections, base, shared)
     return sum(sections), len(sections), C.addressof(held[0]), C.addressof(held[1]), held
 
 
@@ -180,7 +180,7 @@ def rotate_positions(x, positions, sections, base=10000.0, shared=False, interle
     ctx, lib, stream = _enter(what, ctx, tensors[0], *tensors[1:], positions)
     first = tensors[0]
     t = _type(what, first)
-    pairs, axes, frequency, axis, _ = _turns(tuple(sections), base, bool(shared))
+    pairs, axes, frequency, axis, _ = _turns(tuple(sections), float(base), bool(shared))
     if first.dim() != 4:
         raise ValueError("%s: tensors are batch x tokens x heads x head, alike but for the number of heads" % what)
     batch, tokens, _, head = first.shape
@@ -285,7 +285,8 @@ def differential_attention(q, k, v, weights, key_lengths=None, key_mask=None, ca
 
 def differential_attention_backward(do, q, k, v, weights, o, lse, second, key_lengths=None, key_mask=None, causal=False, scale=None, ctx=None):
     """The gradients (dq, dk, dv, dweights) of differential_attention, from that of o and from what the forward call (with for_backward)
-    returned; the other arguments are that call's.  Rows that see no key and keys that do not count get zero.  dweights has the type of weights."""
+    returned; the other arguments are that call's.  Rows that see no key and keys that do not count get zero.  A value of q or do that is not finite reaches the
+    gradients of all keys that count (causal as well: zero weights are multiplied with it).  dweights has the type of weights."""
     what = "differential_attention_backward"
     ctx, lib, stream = _enter(what, ctx, q, k, v, weights, key_lengths, key_mask, do, o, lse, second)
     sizes = _differ_sizes(what, q, k, v, weights, key_lengths, key_mask, scale)

@@ -471,3 +471,112 @@ def test_differential_attention_gradients_of_every_size(dtype):
         grads = nnv.differential_attention_backward(do, q, k, v, w, o, lse, second, **kw)
         for name, got, e, bd in zip(("dq", "dk", "dv", "dweights"), grads, io.differ_grad(do, q, k, v, w, **kw), io.differ_grad_bounds(do, q, k, v, w, **kw)):
             po.assert_within(got, e, bd, "%d %s" % (d, name))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_a_missing_value_shows_where_it_counts(dtype):
+    """A query with a missing value: its row has none of o, lse and dq, the other rows keep theirs, and the gradients of the keys that it sees have none."""
+    import nnv_amd as nnv
+    for d, lq, lk in ((64, 90, 150), (40, 1, 70), (128, 40, 33)):
+        g = gen(81)
+        q, k, v, w = make_differ(g, 2, lq, lk, 4, 2, d, dtype)
+        mask = torch.rand(2, lk, generator=g, device="cuda") < 0.8
+        clean, row = q.clone(), lq // 2
+        q[1, row] = math.nan
+        o, lse, second = nnv.differential_attention(q, k, v, w, key_mask=mask, for_backward=True)
+        exact, bounds = io.differ(clean, k, v, w, key_mask=mask), io.differ_bounds(clean, k, v, w, key_mask=mask)
+        others = torch.ones(2, lq, dtype=torch.bool, device="cuda")
+        others[1, row] = False
+        for name, got, e, bd in zip(("o", "lse", "second"), (o, lse, second), exact, bounds):
+            if name == "lse":
+                got, e, bd = (x.transpose(1, 2) for x in (got, e, bd))
+            assert got[1, row].isnan().all()
+            po.assert_within(got[others], e[others], bd[others], name)
+        do = rand(g, *o.shape, dtype=dtype)
+        dq, dk, dv, dw = nnv.differential_attention_backward(do, q, k, v, w, o, lse, second, key_mask=mask)
+        e, bd = io.differ_grad(do, clean, k, v, w, key_mask=mask)[0], io.differ_grad_bounds(do, clean, k, v, w, key_mask=mask)[0]
+        assert dq[1, row].isnan().all() and dw.isnan().all()
+        po.assert_within(dq[others], e[others], bd[others], "dq")
+        for x in (dk, dv):
+            assert x[1][mask[1]].isnan().all() and (x[1][~mask[1]] == 0).all() and x[0].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_differential_attention_of_many_sequences_by_length(dtype):
+    """More sequences than a wave has lanes; keys that are the queries themselves."""
+    g = gen(91)
+    for lq in (1, 20):
+        q, k, v, w = make_differ(g, 70, lq, 45, 2, 1, 32, dtype)
+        lengths = torch.randint(0, 46, (70,), generator=g, device="cuda", dtype=torch.int32)
+        check_differ(q, k, v, w, key_lengths=lengths, causal=True, tag="%d" % lq)
+    q = rand(g, 3, 50, 4, 64, dtype=dtype)
+    check_differ(q, q, rand(g, 3, 50, 2, 128, dtype=dtype), w, causal=True, tag="self")
+
+
+def far(g, shape, strides, dtype):
+    """A tensor of random values that lie far apart."""
+    last = sum((n - 1) * s for n, s in zip(shape, strides)) + 1
+    x = torch.empty(last, dtype=dtype, device="cuda").as_strided(shape, strides)
+    return x.copy_(rand(g, *shape, dtype=dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_offsets_past_32_bits(dtype):
+    """Tokens, places and sequences more than 2^31 elements apart, and results longer than that."""
+    import nnv_amd as nnv
+    g, most = gen(95), 1 << 31
+    for lq in (1, 70):
+        for b, token in ((1, 1 << 22), (2, 1 << 9)):
+            lk, batch = 600, most + (1 << 14)
+            q, w = rand(g, b, lq, 8, 64, dtype=dtype), rand(g, 4, dtype=dtype)
+            k = far(g, (b, lk, 2, 64), (batch, token, 64, 1), dtype)
+            v = far(g, (b, lk, 1, 128), (batch, token, 128, 1), dtype)
+            do = rand(g, b, lq, 4, 128, dtype=dtype)
+            found = []
+            for kk, vv in ((k, v), (k.contiguous(), v.contiguous())):
+                o, lse, second = nnv.differential_attention(q, kk, vv, w, causal=True, for_backward=True)
+                found.append([o, lse, second, *nnv.differential_attention_backward(do, q, kk, vv, w, o, lse, second, causal=True)])
+            for a, e in zip(*found):
+                assert torch.equal(a, e)
+            del k, v, kk, vv
+    q = far(g, (1, 550, 8, 64), (0, 1 << 22, 64, 1), dtype)
+    k, v = rand(g, 1, 90, 2, 64, dtype=dtype), rand(g, 1, 90, 1, 128, dtype=dtype)
+    found = []
+    for qq in (q, q.contiguous()):
+        o, lse, second = nnv.differential_attention(qq, k, v, w, for_backward=True)
+        do = far(gen(96), o.shape, (0, 1 << 22, 128, 1), dtype)
+        found.append([o, *nnv.differential_attention_backward(do, qq, k, v, w, o, lse, second)])
+        del do
+    for a, e in zip(*found):
+        assert torch.equal(a, e)
+    del q, qq
+    # q, o and dq of more than 2^31 elements: the last sequences
+    q = torch.zeros(4100, 128, 64, 64, dtype=dtype, device="cuda")
+    q[-2:] = rand(g, 2, 128, 64, 64, dtype=dtype)
+    k, v, w = rand(g, 4100, 3, 4, 64, dtype=dtype), rand(g, 4100, 3, 2, 128, dtype=dtype), rand(g, 32, dtype=dtype)
+    o, lse, second = nnv.differential_attention(q, k, v, w, for_backward=True)
+    dq, dk, dv, _ = nnv.differential_attention_backward(o, q, k, v, w, o, lse, second)
+    one = nnv.differential_attention(q[-2:], k[-2:], v[-2:], w, for_backward=True)
+    for a, e in zip((o, lse, second), one):
+        assert torch.equal(a[-2:], e)
+    for a, e in zip((dq, dk, dv), nnv.differential_attention_backward(one[0], q[-2:], k[-2:], v[-2:], w, *one)):
+        assert torch.allclose(a[-2:].float(), e.float(), rtol=2e-2, atol=1e-5)
+    del q, o, second, dq
+    x = far(g, (1, 700, 64), (0, 1 << 22, 1), dtype)
+    dy = rand(g, 1, 700, 64, dtype=dtype)
+    y, mean, rstd = nnv.group_norm(x, 8)
+    for a, e in zip((y, mean, rstd, *nnv.group_norm_backward(dy, x, mean, rstd)),
+                    (lambda z: (*z, *nnv.group_norm_backward(dy, x.contiguous(), *z[1:])))(nnv.group_norm(x.contiguous(), 8))):
+        assert torch.equal(a, e)
+    x = far(g, (1, 700, 2, 64), (0, 1 << 22, 64, 1), dtype)
+    at = torch.arange(700, device="cuda", dtype=torch.int32)[:, None]
+    assert torch.equal(nnv.rotate_positions(x, at, [32]), nnv.rotate_positions(x.contiguous(), at, [32]))
+    x = rand(g, 1, 20, 32, 128, dtype=dtype).repeat(1, 26300, 1, 1)   # 2^31 and 6 millions
+    at = torch.arange(20, device="cuda", dtype=torch.int32)[:, None].repeat(26300, 1)
+    y = nnv.rotate_positions(x, at, [64])
+    assert torch.equal(y[:, -20:], y[:, :20]) and torch.equal(y[:, :20], nnv.rotate_positions(x[:, :20], at[:20], [64]))
+    del y
+    y, mean, rstd = nnv.group_norm(x.view(2, -1, 128), 4)
+    assert torch.equal(y[0], y[1])
+    dx, dscale, _ = nnv.group_norm_backward(x.view(2, -1, 128), x.view(2, -1, 128), mean, rstd)
+    assert torch.equal(dx[0], dx[1]) and torch.equal(mean[0], mean[1])

@@ -212,7 +212,7 @@ def test_workspaces_of_differential_attention_and_their_refusals():
         for backward in (False, True):
             with pytest.raises((ValueError, _lib.NNVHipError)):
                 differ(backward, **kw)
-    for kw in (dict(batch=64, heads=64, kv_heads=8, queries=1, keys=65536), dict(heads=8, batch=1, queries=1, keys=1 << 26), dict(batch=1, queries=0), dict(keys=0)):
+    for kw in (dict(batch=64, heads=32, kv_heads=32, queries=32768, keys=4096), dict(batch=64, heads=64, kv_heads=8, queries=1, keys=65536), dict(heads=8, batch=1, queries=1, keys=1 << 26), dict(batch=1, queries=0), dict(keys=0)):
         for t in range(3):
             assert differ(type=t, weight_type=t, **kw) >= 0 and differ(True, type=t, weight_type=t, **kw) >= 0
 
