@@ -23,13 +23,14 @@ struct DifferArgs : AttendArgs {   // (its lse is the caller's; scale, masks and
   void* dweights;
   float* info;                     // [sequence, key/value head][kInfos][info_rows]: see RowInfo
   int info_rows;                   // rows, rounded up to kInfoRows
-  float* dots;                     // D_1 as the 16-bit form finds it, [split][sequence, key/value head][row]; else null
+  float* dots;                     // D as the 16-bit form finds it, [split][sequence, key/value head][map][row]; else null
 };
 
 // What the gradients of keys need of a row, as arrays over the rows of a key/value head that a tile's transfer takes as they lie: the exponents' offsets of both
 // maps (infinite for rows without keys, and behind the last one), D of both, the weight with its sign turned, and how many keys the row sees.
 enum RowInfo { kOffset0, kOffset1, kDelta0, kDelta1, kWeight, kSees, kInfos };
 constexpr int kInfoRows = 64;
+__device__ __forceinline__ float* info_at(const DifferArgs& a, int64_t bkv, int64_t r, int which) { return a.info + (bkv * kInfos + which) * a.info_rows + r; }
 
 __device__ __forceinline__ int64_t map_row_at(const TokenView& t, const DifferArgs& a, int b, int kv, int64_t r, int map) {
   const int64_t g = (uint32_t)r / (uint32_t)a.queries, i = r - g * a.queries;

@@ -5,6 +5,15 @@
 
 namespace nnvhip {
 
+// what rounding eight weights to p leaves
+template <typename T>
+__device__ __forceinline__ half8<T> rest8(const float16_t& s, const half8<T>& p, int first) {
+  half8<T> r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = (T)(s[first + i] - (float)p[i]);
+  return r;
+}
+
 // A tile of ROWS rows: those of the first map (DP values each, the head rounded up to 32), of the second one, and the wide ones (W, twice the head
 // rounded up to 16), each as Rows16 has them, one behind the other.  CH: chunks of 16 values of a map's head.
 template <int CH>

@@ -63,8 +63,7 @@ __global__ __launch_bounds__(1024) void differ_weights_kernel(const DifferArgs a
   for (int64_t unit = threadIdx.x >> 6; unit < sets * (int64_t)each; unit += 16) {
     const int k = (int)(unit / each), first = (int)(unit - k * (int64_t)each) * 256 + (threadIdx.x & 63);
     const int64_t bkv = k % a.batch * (int64_t)a.kv_heads + kv;
-    const float* from = a.dots ? a.dots + (k / a.batch * (int64_t)a.batch * a.kv_heads + bkv) * a.rows + (int64_t)g * a.queries
-                               : a.delta + own_row(a, bkv, (int64_t)g * a.queries, 1);
+    const float* from = (a.dots ? a.dots + k / a.batch * own_rows(a) : a.delta) + own_row(a, bkv, (int64_t)g * a.queries, 1);
     float x[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) x[j] = first + 64 * j < a.queries ? from[first + 64 * j] : 0.0f;
@@ -280,13 +279,18 @@ __global__ __launch_bounds__(256) void differ_sum_kernel(const float* __restrict
   }
   (blockIdx.y ? dv : dk)[e] = from_f<T>(s);
 }
-// dq's maps' rows from the splits', written in the order of the tensor: a wave a row
+// dq's maps' rows from the splits', written in the order of the tensor, and D of the 16-bit form: a wave a row
 template <typename T, int>
 __global__ __launch_bounds__(256) void differ_sum_rows_kernel(const DifferArgs a) {
   const int64_t all = own_rows(a), own = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (own >= all) return;
   const int64_t bkv = own / (2 * a.rows), left = own - bkv * 2 * a.rows, m = left / a.rows;
   T* row = (T*)a.dq + dense_map_row_at(a, (int)(bkv / a.kv_heads), (int)(bkv % a.kv_heads), left - m * a.rows, (int)m);
+  if (a.dots && (threadIdx.x & 63) == 0) {
+    float s = 0.0f;
+    for (int k = 0; k < a.splits; ++k) s += a.dots[k * all + own];
+    *info_at(a, bkv, left - m * a.rows, kDelta0 + (int)m) = s;
+  }
   for (int d = threadIdx.x & 63; d < a.head; d += 64) {
     float s = 0.0f;
     for (int k = 0; k < a.splits; ++k) s += a.part[(k * all + own) * a.head + d];
@@ -309,7 +313,7 @@ GradCut grad_cut(int64_t batch, int64_t kv_heads, int64_t queries, int64_t rows,
   c.key_splits = split_of(batch * kv_heads * c.key_blocks, ceil_div(rows, 32), 2, by16 || head > 64 ? 256 : 512, start, join);
   c.delta = round_up(batch * kv_heads * 2 * rows, 64);
   c.info = by16 ? batch * kv_heads * kInfos * round_up(rows, kInfoRows) : 0;
-  c.dots = by16 ? round_up(c.query_splits * batch * kv_heads * rows, 64) : 0;
+  c.dots = by16 ? round_up(c.query_splits * batch * kv_heads * 2 * rows, 64) : 0;
   const int64_t q = c.query_splits > 1 ? c.query_splits * batch * kv_heads * 2 * rows * head : 0;
   const int64_t k = c.key_splits > 1 ? 2 * c.key_splits * batch * kv_heads * keys * 2 * head : 0;
   c.part = std::max(q, k);
