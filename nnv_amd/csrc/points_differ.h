@@ -105,9 +105,9 @@ __device__ __forceinline__ int key_blocks_of(const DifferArgs& a) { return key_b
 struct BlockPlace {
   int b, kv, x;
 };
-__device__ __forceinline__ BlockPlace block_place(const DifferArgs& a, int64_t id, int64_t each) {
-  const int64_t groups = (int64_t)a.batch * a.kv_heads, whole = groups / 8 * 8 * each;
-  int64_t group, x;
+__device__ __forceinline__ BlockPlace block_place(const DifferArgs& a, uint32_t id, uint32_t each) {   // (a grid has fewer blocks than 2^23)
+  const uint32_t groups = (uint32_t)a.batch * a.kv_heads, whole = groups / 8 * 8 * each;
+  uint32_t group, x;
   if (id < whole) {
     group = id / 8 / each * 8 + id % 8;
     x = id / 8 % each;
@@ -115,7 +115,7 @@ __device__ __forceinline__ BlockPlace block_place(const DifferArgs& a, int64_t i
     group = groups / 8 * 8 + (id - whole) / each;
     x = (id - whole) % each;
   }
-  BlockPlace p{(int)(group / a.kv_heads), (int)(group % a.kv_heads), (int)x};
+  BlockPlace p{(int)(group / (uint32_t)a.kv_heads), (int)(group % (uint32_t)a.kv_heads), (int)x};
   if (a.lengths != nullptr && a.batch <= 64 && a.batch > 1) {   // the sequence of that rank
     const int lane = threadIdx.x & 63, mine = lane < a.batch ? min(max(a.lengths[lane], 0), a.keys) : -1;
     int rank = 0;

@@ -94,8 +94,8 @@ __global__ __launch_bounds__(512, 2) void differ16_kernel(const DifferArgs a) {
   static_assert(STAGES >= 2 && STAGES * Load::VALUES * 2 >= 4 * 32 * W * 4, "the second map's result fits the tiles' place");
   const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int map = wave >> 2, part_of = wave & 3;
-  const BlockPlace at = block_place(a, blockIdx.x, (int64_t)a.row_tiles * a.splits);
-  const int b = at.b, kv = at.kv, bkv = b * a.kv_heads + kv, split = at.x % a.splits, row_tile = row_tile_of(a, at.x / a.splits);
+  const BlockPlace at = block_place(a, blockIdx.x, (uint32_t)a.row_tiles * a.splits);
+  const int b = at.b, kv = at.kv, bkv = b * a.kv_heads + kv, split = (uint32_t)at.x % (uint32_t)a.splits, row_tile = row_tile_of(a, (uint32_t)at.x / (uint32_t)a.splits);
   const int n = keys_that_count(a, b);
   const int64_t first = (int64_t)row_tile * kDiffer16Rows, last = min(first + kDiffer16Rows, a.rows) - 1;
   const int tiles = (most_seen(a, first, last, n) + KEYS - 1) / KEYS, per = (tiles + a.splits - 1) / a.splits;
@@ -243,7 +243,7 @@ __global__ __launch_bounds__(64 * differ_groups<CH>(), 1) void differ16_few_kern
   __shared__ __attribute__((aligned(1024))) T lds[TILES > FOUND ? TILES : FOUND];
   __shared__ float col_max[GROUPS][32], col_total[GROUPS][32];
   const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5, group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const BlockPlace at = block_place(a, blockIdx.x, (int64_t)a.row_tiles * a.splits);
+  const BlockPlace at = block_place(a, blockIdx.x, (uint32_t)a.row_tiles * a.splits);
   const int b = at.b, kv = at.kv, bkv = b * a.kv_heads + kv, split = at.x % a.splits, row_tile = at.x / a.splits;
   const int n = keys_that_count(a, b);
   const int64_t first = (int64_t)row_tile * kDifferFewRows, last = min(first + kDifferFewRows, a.rows) - 1;

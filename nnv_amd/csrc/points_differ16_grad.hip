@@ -7,6 +7,9 @@
 // product that takes it, and so of one row of the result; a power of two that brings the column's largest value so far to 2^14 (Lift) is taken out of the
 // result at the end, and when a larger value comes the sums so far are scaled, as a softmax's are: what is below 2^-38 of the largest is lost, what is above 2^-28
 // keeps all bits.
+//
+// 2 x 4096 x 4096, 16 heads of 64, 4 for keys, causal, in bf16: dq 310 to 335 us, dk and dv 425 to 450.  Matrix units are busy 36 and 35 % of it, LDS 15 and 31: two waves a
+// SIMD, whose exponentials, roundings and reads from LDS follow one another between the products.  More waves would not have the registers.
 #include "points_differ16.h"
 
 #pragma clang fp contract(fast)
@@ -116,8 +119,8 @@ __global__ __launch_bounds__(64 * kWaves<CH>, kWaves<CH> / 4) void differ_query_
   typedef TripleLoad<T, CH, KEYS, WAVES> Load;
   __shared__ __attribute__((aligned(1024))) T lds[2 * Load::VALUES];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
-  const BlockPlace at = block_place(a, blockIdx.x, (int64_t)a.row_tiles * a.splits);
-  const int b = at.b, kv = at.kv, bkv = b * a.kv_heads + kv, split = at.x % a.splits, row_tile = row_tile_of(a, at.x / a.splits);
+  const BlockPlace at = block_place(a, blockIdx.x, (uint32_t)a.row_tiles * a.splits);
+  const int b = at.b, kv = at.kv, bkv = b * a.kv_heads + kv, split = (uint32_t)at.x % (uint32_t)a.splits, row_tile = row_tile_of(a, (uint32_t)at.x / (uint32_t)a.splits);
   const int n = keys_that_count(a, b);
   const int64_t first = (int64_t)row_tile * ROWS, last = min(first + ROWS, a.rows) - 1;
   const int tiles = (most_seen(a, first, last, n) + KEYS - 1) / KEYS, per = (tiles + a.splits - 1) / a.splits;
@@ -222,8 +225,8 @@ __global__ __launch_bounds__(64 * kKeyWaves<CH>, kKeyWaves<CH> / 4) void differ_
   __shared__ __attribute__((aligned(1024))) float info[2][kInfos * ROWS < 256 ? 256 : 512];   // [buffer][RowInfo * ROWS + row]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
   const int blocks = key_blocks_of(a);
-  const BlockPlace at = block_place(a, blockIdx.x, (int64_t)blocks * a.splits);
-  const int b = at.b, kv = at.kv, bkv = b * a.kv_heads + kv, split = at.x % a.splits, block = at.x / a.splits;
+  const BlockPlace at = block_place(a, blockIdx.x, (uint32_t)blocks * a.splits);
+  const int b = at.b, kv = at.kv, bkv = b * a.kv_heads + kv, split = (uint32_t)at.x % (uint32_t)a.splits, block = (uint32_t)at.x / (uint32_t)a.splits;
   const int n = keys_that_count(a, b);
   const unsigned lds_at = lds_addr_of(lds), rows_at = rows_place<T, DP>(lane), wide_at = rows_place<T, W>(lane) + 4 * Load::MAP;
   const unsigned columns_at = columns_place<T, DP>(lane), wide_columns_at = columns_place<T, W>(lane) + 4 * Load::MAP;

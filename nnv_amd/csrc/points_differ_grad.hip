@@ -3,6 +3,9 @@
 // As in points_attend_grad.hip two kernels form dq (a wave per 16 queries, both maps) and dk, dv (a wave per 16 keys), each sum in the registers of
 // one wave, in a fixed order, with no atomics.  do v^T, half of what the scores' gradients take, is one product for both maps.  D of both maps and
 // the weights' gradients come first.
+//
+// Bound by the f32 matrix instructions (4 x 1024 x 1024, 16 heads of 64: dq 475 us, dk and dv 740; 4 x 333 x 577, 6 heads of 40: 49 and 68, matrix units busy 48
+// and 44 %: blocks of six or seven tiles, in whose beginning and end nothing is multiplied).  Two buffers in LDS, and so one barrier a tile instead of two, measured the same.
 #include "points_differ16.h"
 
 #pragma clang fp contract(fast)
@@ -15,10 +18,11 @@ constexpr int kBlockRows = 64;   // rows, or keys, of a block
 // D_1 = rowsum(do second), D_0 = rowsum(do o) + w D_1: 16 lanes a row.
 template <typename T, int>
 __global__ __launch_bounds__(256) void differ_delta_kernel(const DifferArgs a) {
-  const int64_t flat = (int64_t)blockIdx.x * 16 + threadIdx.x / 16, per = a.info ? a.info_rows : a.rows, all = (int64_t)a.batch * a.kv_heads * per;
-  if (flat >= all) return;   // (the lanes of a row go together)
-  const int64_t bkv = flat / per, r = flat % per;
-  const int b = (int)(bkv / a.kv_heads), kv = (int)(bkv % a.kv_heads), size = 2 * a.head;
+  const uint32_t flat = blockIdx.x * 16 + threadIdx.x / 16, per = a.info ? a.info_rows : (uint32_t)a.rows;   // (fewer than 2^28)
+  if (flat >= (int64_t)a.batch * a.kv_heads * per) return;   // (the lanes of a row go together)
+  const uint32_t own = flat / per;
+  const int64_t bkv = own, r = flat - own * per;
+  const int b = own / (uint32_t)a.kv_heads, kv = own - b * a.kv_heads, size = 2 * a.head;
   float* info = a.info ? a.info + bkv * kInfos * per + r : nullptr;
   if (r >= a.rows) {
     if (threadIdx.x % 16 < kInfos) info[threadIdx.x % 16 * per] = threadIdx.x % 16 <= kOffset1 ? INFINITY : 0.0f;
@@ -59,11 +63,12 @@ __global__ __launch_bounds__(1024) void differ_weights_kernel(const DifferArgs a
   const int head = blockIdx.x, kv = head / a.group, g = head % a.group;
   double s = 0;
   // a wave takes 256 rows of a set at a time
-  const int sets = a.dots ? a.splits * a.batch : a.batch, each = (a.queries + 255) / 256;
-  for (int64_t unit = threadIdx.x >> 6; unit < sets * (int64_t)each; unit += 16) {
-    const int k = (int)(unit / each), first = (int)(unit - k * (int64_t)each) * 256 + (threadIdx.x & 63);
-    const int64_t bkv = k % a.batch * (int64_t)a.kv_heads + kv;
-    const float* from = (a.dots ? a.dots + k / a.batch * own_rows(a) : a.delta) + own_row(a, bkv, (int64_t)g * a.queries, 1);
+  const uint32_t sets = a.dots ? a.splits * a.batch : a.batch, each = ((uint32_t)a.queries + 255) / 256;
+  for (uint32_t unit = threadIdx.x >> 6; unit < sets * each; unit += 16) {   // (fewer than 2^31)
+    const uint32_t k = unit / each, split = k / (uint32_t)a.batch;
+    const int first = (unit - k * each) * 256 + (threadIdx.x & 63);
+    const int64_t bkv = (int64_t)(k - split * a.batch) * a.kv_heads + kv;
+    const float* from = (a.dots ? a.dots + split * own_rows(a) : a.delta) + own_row(a, bkv, (int64_t)g * a.queries, 1);
     float x[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) x[j] = first + 64 * j < a.queries ? from[first + 64 * j] : 0.0f;
@@ -86,8 +91,8 @@ __global__ __launch_bounds__(256, CH <= 6 ? 2 : 1) void differ_query_grad_kernel
   constexpr int R = 32, LD = F32Tile<CH>::LD;
   __shared__ __attribute__((aligned(16))) float tile[F32Tile<CH>::FLOATS];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, q4 = lane >> 4;
-  const BlockPlace at = block_place(a, blockIdx.x, (int64_t)a.row_tiles * a.splits);
-  const int b = at.b, kv = at.kv, bkv = b * a.kv_heads + kv, split = at.x % a.splits, row_tile = row_tile_of(a, at.x / a.splits);
+  const BlockPlace at = block_place(a, blockIdx.x, (uint32_t)a.row_tiles * a.splits);
+  const int b = at.b, kv = at.kv, bkv = b * a.kv_heads + kv, split = (uint32_t)at.x % (uint32_t)a.splits, row_tile = row_tile_of(a, (uint32_t)at.x / (uint32_t)a.splits);
   const int n = keys_that_count(a, b);
   const int64_t first = (int64_t)row_tile * kBlockRows, last = min(first + kBlockRows, a.rows) - 1;
   const int tiles = (most_seen(a, first, last, n) + R - 1) / R, per = (tiles + a.splits - 1) / a.splits;
@@ -157,8 +162,8 @@ __global__ __launch_bounds__(256, CH <= 4 ? 2 : 1) void differ_key_grad_kernel(c
   __shared__ __attribute__((aligned(16))) float offsets[2][R], deltas[2][R], weights[R], seen_by_row[R];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, q4 = lane >> 4;
   const int blocks = key_blocks_of(a);
-  const BlockPlace at = block_place(a, blockIdx.x, (int64_t)blocks * a.splits);
-  const int b = at.b, kv = at.kv, bkv = b * a.kv_heads + kv, split = at.x % a.splits, block = at.x / a.splits;
+  const BlockPlace at = block_place(a, blockIdx.x, (uint32_t)blocks * a.splits);
+  const int b = at.b, kv = at.kv, bkv = b * a.kv_heads + kv, split = (uint32_t)at.x % (uint32_t)a.splits, block = (uint32_t)at.x / (uint32_t)a.splits;
   const int n = keys_that_count(a, b);
   const float unit = a.scale * kLog2e;
 #pragma unroll 1
@@ -284,12 +289,14 @@ template <typename T, int>
 __global__ __launch_bounds__(256) void differ_sum_rows_kernel(const DifferArgs a) {
   const int64_t all = own_rows(a), own = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (own >= all) return;
-  const int64_t bkv = own / (2 * a.rows), left = own - bkv * 2 * a.rows, m = left / a.rows;
-  T* row = (T*)a.dq + dense_map_row_at(a, (int)(bkv / a.kv_heads), (int)(bkv % a.kv_heads), left - m * a.rows, (int)m);
+  const uint32_t rows = (uint32_t)a.rows, set = (uint32_t)own / rows, b = set / 2 / (uint32_t)a.kv_heads;   // (a call that is split has fewer than 2^23 rows)
+  const int64_t bkv = set / 2, r = own - (int64_t)set * rows;
+  const int m = set % 2;
+  T* row = (T*)a.dq + dense_map_row_at(a, b, (int)bkv - b * a.kv_heads, r, m);
   if (a.dots && (threadIdx.x & 63) == 0) {
     float s = 0.0f;
     for (int k = 0; k < a.splits; ++k) s += a.dots[k * all + own];
-    *info_at(a, bkv, left - m * a.rows, kDelta0 + (int)m) = s;
+    *info_at(a, bkv, r, kDelta0 + m) = s;
   }
   for (int d = threadIdx.x & 63; d < a.head; d += 64) {
     float s = 0.0f;

@@ -13,6 +13,9 @@
 // 16 bytes of channels) x (places): rows are read as they lie in memory, whatever the groups are.  The sums of x and x^2 are f64:
 // the memory's rate asks for some 1e13 f64 operations a second, a quarter of what the f64 pipes give, and a mean far from zero then
 // costs the variance nothing.
+//
+// 16 x 64 x 64 x 320 in bf16: 26 us forward (3.2 TB/s: a block reads all it has before it writes, and one fits a CU), 54 backward (24 + 28 us a kernel: x and dy are read
+// twice, the second time partly from the caches); 5 x 53 x 79 x 96 in f32 backward 17; 4 x 8 x 8 x 256 forward 5.5 us, a launch and one latency of memory.
 #include "points.h"
 
 #include <algorithm>

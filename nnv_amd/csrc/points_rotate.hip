@@ -5,7 +5,8 @@
 //
 // Bound by memory: each value is read and written once.  A block takes the heads of a few tokens and forms the tokens' cosines and
 // sines once, in LDS.  Angles are counted in turns and in f64: position * (frequency / 2 pi), of which the whole turns are dropped, so
-// that far positions lose nothing; what is left goes through sincospif.
+// that far positions lose nothing; what is left goes through sincospif.  (2 x 19200 tokens of 32 heads of 128 in bf16: 122 us, 5.15 TB/s; 16 tokens: 4.3 us,
+// of which the launch is most; 3 x 1577 tokens of 24 heads of 80 in f32: 17 us among other calls, 4.2 TB/s.)
 #include "points.h"
 
 #include <algorithm>
