@@ -56,17 +56,17 @@ __global__ __launch_bounds__(256) void differ_delta_kernel(const DifferArgs a) {
   for (int k = 0; k < kInfos; ++k) info[k * per] = values[k];
 }
 
-// dw of a head: a block adds its rows' D_1 (of all splits, where the kernel of dq found it), in f64.
-template <typename T, int>
-__global__ __launch_bounds__(1024) void differ_weights_kernel(const DifferArgs a) {
+// dw of a head: a block adds its rows' D_1 (of all splits, where the kernel of dq found it), in f64.  splits: of that kernel.
+constexpr int kRowsOfAWave = 256;
+template <typename T>
+__device__ __forceinline__ void add_weights(const DifferArgs& a, int splits, int head) {
   __shared__ double lds[16];
-  const int head = blockIdx.x, kv = head / a.group, g = head % a.group;
+  const int kv = head / a.group, g = head % a.group, waves = blockDim.x >> 6;
   double s = 0;
-  // a wave takes 256 rows of a set at a time
-  const uint32_t sets = a.dots ? a.splits * a.batch : a.batch, each = ((uint32_t)a.queries + 255) / 256;
-  for (uint32_t unit = threadIdx.x >> 6; unit < sets * each; unit += 16) {   // (fewer than 2^31)
+  const uint32_t sets = a.dots ? splits * a.batch : a.batch, each = ((uint32_t)a.queries + kRowsOfAWave - 1) / kRowsOfAWave;
+  for (uint32_t unit = threadIdx.x >> 6; unit < sets * each; unit += waves) {   // (fewer than 2^31)
     const uint32_t k = unit / each, split = k / (uint32_t)a.batch;
-    const int first = (unit - k * each) * 256 + (threadIdx.x & 63);
+    const int first = (unit - k * each) * kRowsOfAWave + (threadIdx.x & 63);
     const int64_t bkv = (int64_t)(k - split * a.batch) * a.kv_heads + kv;
     const float* from = (a.dots ? a.dots + split * own_rows(a) : a.delta) + own_row(a, bkv, (int64_t)g * a.queries, 1);
     float x[4];
@@ -80,10 +80,14 @@ __global__ __launch_bounds__(1024) void differ_weights_kernel(const DifferArgs a
   __syncthreads();
   if (threadIdx.x) return;
   double sum = 0;
-  for (int k = 0; k < 16; ++k) sum += lds[k];
+  for (int k = 0; k < waves; ++k) sum += lds[k];
   const float all = (float)-sum;
   if (a.wide_weights) ((float*)a.dweights)[head] = all;
   else ((T*)a.dweights)[head] = from_f<T>(all);
+}
+template <typename T, int>
+__global__ __launch_bounds__(1024) void differ_weights_kernel(const DifferArgs a) {
+  add_weights<T>(a, a.splits, blockIdx.x);
 }
 
 template <typename T, int CH, bool FOUR>
@@ -268,12 +272,18 @@ __global__ __launch_bounds__(256, CH <= 4 ? 2 : 1) void differ_key_grad_kernel(c
   }
 }
 
-// dk[e] = sum over splits of part[s][e], in order, and dv[e] of those behind (blockIdx.y)
+// dk[e] = sum over splits of part[s][e], in order, and dv[e] of those behind (the second half of the blocks).  The first `heads` blocks add the weights' gradients.
 template <typename T, int>
-__global__ __launch_bounds__(256) void differ_sum_kernel(const float* __restrict__ part, int splits, int64_t n, T* __restrict__ dk, T* __restrict__ dv) {
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+__global__ __launch_bounds__(256) void differ_sum_kernel(const DifferArgs a, int heads, int query_splits, int64_t n) {
+  if ((int)blockIdx.x < heads) {
+    add_weights<T>(a, query_splits, blockIdx.x);
+    return;
+  }
+  const uint32_t half = (gridDim.x - heads) / 2, which = blockIdx.x - heads >= half;
+  const int64_t e = (int64_t)(blockIdx.x - heads - which * half) * 256 + threadIdx.x;
   if (e >= n) return;
-  part += blockIdx.y * splits * n + e;
+  const int splits = a.splits;
+  const float* __restrict__ part = a.part + which * splits * n + e;
   float s = 0.0f;
   for (int k = 0; k < splits; k += 4) {
     float v[4];
@@ -282,7 +292,7 @@ __global__ __launch_bounds__(256) void differ_sum_kernel(const float* __restrict
 #pragma unroll
     for (int i = 0; i < 4; ++i) s += v[i];
   }
-  (blockIdx.y ? dv : dk)[e] = from_f<T>(s);
+  ((T*)(which ? a.dv : a.dk))[e] = from_f<T>(s);
 }
 // dq's maps' rows from the splits', written in the order of the tensor, and D of the 16-bit form: a wave a row
 template <typename T, int>
@@ -345,7 +355,10 @@ void launch_grad(DifferArgs a, const GradCut& c, bool by16, hipStream_t st) {
   } else {
     a.batch = 0;   // (for the sums over no rows)
   }
-  hipLaunchKernelGGL((differ_weights_kernel<T, 0>), dim3((unsigned)(a.kv_heads * a.group)), dim3(1024), 0, st, a);
+  // the weights' gradients beside the sums of dk and dv, where there are such and a wave there takes sixteen turns at most
+  const int64_t turns = ceil_div((a.dots ? a.splits : 1) * (int64_t)a.batch * ceil_div(a.queries, kRowsOfAWave), 4);
+  const int beside = a.batch > 0 && a.keys > 0 && c.key_splits > 1 && turns <= 16 ? a.kv_heads * a.group : 0, query_splits = a.splits;
+  if (!beside) hipLaunchKernelGGL((differ_weights_kernel<T, 0>), dim3((unsigned)(a.kv_heads * a.group)), dim3(1024), 0, st, a);
   if (a.keys > 0 && heads > 0) {
     a.batch = (int)(heads / a.kv_heads);
     a.key_tiles = c.key_tiles;
@@ -356,7 +369,7 @@ void launch_grad(DifferArgs a, const GradCut& c, bool by16, hipStream_t st) {
     else hipLaunchKernelGGL((differ_key_grad_kernel<T, CH, false>), grid, dim3(256), 0, st, a);
     if (a.splits > 1) {
       const int64_t n = heads * a.keys * 2 * a.head;
-      hipLaunchKernelGGL((differ_sum_kernel<T, 0>), dim3((unsigned)ceil_div(n, 256), 2), dim3(256), 0, st, a.part, a.splits, n, (T*)a.dk, (T*)a.dv);
+      hipLaunchKernelGGL((differ_sum_kernel<T, 0>), dim3((unsigned)(beside + 2 * ceil_div(n, 256))), dim3(256), 0, st, a, beside, query_splits, n);
     }
   }
 }

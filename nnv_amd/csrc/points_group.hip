@@ -715,7 +715,7 @@ int group_args(const char* what, const nnvhip_group_norm_args* d, bool backward,
   if (d->activation < kNone || d->activation > kSilu) NNV_FAIL(NNVHIP_ERR_ARG, "%s: the activation is none, relu or silu", what);
   if (d->batch < 0 || d->places < 1 || d->channels < 1 || d->groups < 1 || d->channels % d->groups)
     NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: at least one place and channel are expected, the channels in equal groups", what);
-  if (d->channels >= (1 << 24) || d->batch >= (1 << 23) || d->places >= (int64_t(1) << 40))
+  if (d->channels >= (1 << 24) || d->batch >= (1 << 23) || d->places >= (int64_t(1) << 36))
     NNV_FAIL(NNVHIP_ERR_SHAPE, "%s: too many values", what);
   a->batch = (int)d->batch;
   a->places = d->places;

@@ -115,7 +115,7 @@ def test_workspaces_and_their_refusals():
     assert group(backward=True, places=1 << 24, batch=1) < (1 << 24) * 64 * 2 / 16
     assert group(channels=1 << 20, groups=1) > 0 and group(channels=5000, groups=5000) > 0
     for kw in (dict(type=3), dict(param_type=2), dict(activation=3), dict(groups=7), dict(groups=0), dict(places=0), dict(channels=0), dict(batch=-1),
-               dict(batch=1 << 23), dict(channels=1 << 24, groups=1), dict(places=1 << 40), dict(batch=1 << 22, channels=2048), dict(places=1 << 39)):
+               dict(batch=1 << 23), dict(channels=1 << 24, groups=1), dict(places=1 << 40), dict(batch=1 << 22, channels=2048), dict(places=1 << 39), dict(places=1 << 36, channels=1, groups=1)):
         for backward in (False, True):
             with pytest.raises((ValueError, _lib.NNVHipError)):
                 group(backward, **kw)
