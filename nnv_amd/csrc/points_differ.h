@@ -91,6 +91,15 @@ __device__ __forceinline__ int row_tile_of(const DifferArgs& a, int x) {
   const int each = a.row_tiles / a.group;   // tiles of a head, about
   return a.causal && x < each * a.group ? x % a.group * each + each - 1 - x / a.group : x;
 }
+// Where the tiles of `size` rows of a split of a block over keys begin, of those of which a row may see one of its keys, from a head's row i_min on: all splits
+// get as many such rows.  (8 x 2552 x 640 causal, 4 / 2 heads of 32, five splits: with as many tiles each, 20 of one had rows that see a key, of another none.)
+__device__ __forceinline__ int first_row_tile(const DifferArgs& a, int split, int size, int i_min) {
+  const uint32_t splits = a.splits, q = a.queries, skipped = min(max(i_min, 0), a.queries), each = q - skipped;
+  if (split == 0 || each == 0) return 0;
+  if (split == a.splits) return (int)((a.rows + size - 1) / size);
+  const uint32_t all = each * a.group, at = all / splits * split + all % splits * split / splits, head = at / each;
+  return (int)((head * q + skipped + (at - head * each)) / (uint32_t)size);
+}
 // Blocks of the kernels over keys.  Causal: a tile of early keys is seen by most rows, one of late keys by few, and a block takes one of either (and
 // where their number is odd, one block the middle one alone).  Not where the tiles are few, or few of the keys are hidden from any row (8 x 16 x 504, 2 heads
 // of 96: 29 us, in pairs 49; 2 x 4096 x 4096, 16 / 4 heads of 64: 650, in pairs 430).

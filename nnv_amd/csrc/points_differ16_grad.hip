@@ -250,8 +250,7 @@ __global__ __launch_bounds__(64 * kKeyWaves<CH>, kKeyWaves<CH> / 4) void differ_
     const int i_min = a.causal ? first - (n - a.queries) : 0;   // the first query that sees one of the block's keys
     // where no key of the block counts there is nothing to add up
     const bool any = __syncthreads_or(counts);
-    const int tiles = any ? (int)((a.rows + ROWS - 1) / ROWS) : 0, per = (tiles + a.splits - 1) / a.splits;
-    const int t0 = split * per, t1 = min(tiles, t0 + per);
+    const int t0 = first_row_tile(a, split, ROWS, i_min), t1 = any ? first_row_tile(a, split + 1, ROWS, i_min) : 0;
 
     half8<T> kf[2][CH], vf[2 * CH];
     T* parked = lds + 2 * Load::VALUES + wave * (512 * PARKED) + lane * 8;   // operand c at parked + 512 c; no other wave's

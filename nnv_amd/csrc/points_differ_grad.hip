@@ -177,9 +177,8 @@ __global__ __launch_bounds__(256, CH <= 4 ? 2 : 1) void differ_key_grad_kernel(c
     const int i_min = a.causal ? first - (n - a.queries) : 0;   // the first query that sees one of the block's keys
     int t0 = 0, t1 = 0;
     if (first < n) {   // else no key of the block counts: its gradients are zero
-      const int tiles = (int)((a.rows + R - 1) / R), per = (tiles + a.splits - 1) / a.splits;
-      t0 = split * per;
-      t1 = min(tiles, t0 + per);
+      t0 = first_row_tile(a, split, R, i_min);
+      t1 = first_row_tile(a, split + 1, R, i_min);
     }
     const int64_t row = here && counts ? key : 0;
     float kf[2][CH][4], vf[2 * CH][4];
@@ -324,10 +323,13 @@ GradCut grad_cut(int64_t batch, int64_t kv_heads, int64_t queries, int64_t rows,
   c.row_tiles = (int)ceil_div(rows, by16 ? differ_grad16_tile(head) : kBlockRows);
   c.key_tiles = (int)ceil_div(keys, by16 ? differ_key_grad16_tile(head) : kBlockRows);
   c.key_blocks = key_blocks_of(c.key_tiles, queries, keys, causal);
-  // blocks that the chip holds at once; what starting a block, and adding splits up, costs in tiles of 32 rows
-  const int64_t start = by16 ? 6 : 2, join = by16 ? 12 : 3;
-  c.query_splits = split_of(batch * kv_heads * c.row_tiles, ceil_div(keys, 32), 2, by16 || head > 96 ? 256 : 512, start, join);
-  c.key_splits = split_of(batch * kv_heads * c.key_blocks, ceil_div(rows, 32), 2, by16 || head > 64 ? 256 : 512, start, join);
+  // blocks that the chip holds at once; what starting a block, and adding splits up, costs in tiles of 32 rows.  A tile takes the 16-bit kernels a microsecond or more: a launch is
+  // three, and so are 12 MB of parts.  (2 x 200 x 300, 4 heads of 40 in f16: 59 us, with twelve for every sum 95; 8 x 577 x 1000, 12 heads of 64: 275, with four 314.)
+  const int64_t start = by16 ? 6 : 2, heads = batch * kv_heads;
+  auto join = [&](int64_t values) { return by16 ? 3 + 16 * values / 4000000 : 3; };   // of f32, of two splits, written and read
+  c.query_splits = split_of(heads * c.row_tiles, ceil_div(keys, 32), 2, by16 || head > 96 ? 256 : 512, start, join(heads * 2 * rows * head));
+  const int64_t useful = causal ? std::min(queries, keys) * (rows / std::max<int64_t>(queries, 1)) : rows;   // rows that see a key
+  c.key_splits = split_of(heads * c.key_blocks, ceil_div(useful, 32), 2, by16 || head > 64 ? 256 : 512, start, join(heads * 4 * keys * head));
   c.delta = round_up(batch * kv_heads * 2 * rows, 64);
   c.info = by16 ? batch * kv_heads * kInfos * round_up(rows, kInfoRows) : 0;
   c.dots = by16 ? round_up(c.query_splits * batch * kv_heads * 2 * rows, 64) : 0;
