@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import struct
+from numbers import Integral
 
 import torch
 
@@ -45,7 +46,7 @@ def _group_params(what, x, groups, scale, offset, activation):
     if x.dim() < 2:
         raise ValueError("%s: x is batch x ... x channels" % what)
     channels = x.shape[-1]
-    if not (isinstance(groups, int) and groups >= 1 and channels >= 1 and channels % groups == 0):
+    if not ((isinstance(groups, int) or isinstance(groups, Integral)) and groups >= 1 and channels >= 1 and channels % groups == 0):
         raise ValueError("%s: the channels (%d) must come in equal groups, not %s" % (what, channels, groups))
     if 0 in x.shape[1:]:
         raise ValueError("%s: at least one place is expected, not the shape %s" % (what, tuple(x.shape)))
@@ -154,7 +155,7 @@ def _frequencies(sections, base, shared):
 @functools.lru_cache(maxsize=64)
 def _turns(sections, base, shared):
     """(pairs, axes, addresses of _frequencies, which they belong to) of a call's arguments, or the error."""
-    if not sections or not all(isinstance(n, int) and n >= 0 for n in sections) or not 1 <= sum(sections) <= _ROTATE_PAIRS or len(sections) > 255:
+    if not sections or not all(isinstance(n, Integral) and n >= 0 for n in sections) or not 1 <= sum(sections) <= _ROTATE_PAIRS or len(sections) > 255:
         raise ValueError("rotate_positions: sections are numbers of pairs, one per axis, %d together at most" % _ROTATE_PAIRS)
     if not 0 < base < float("inf"):
         raise ValueError("rotate_positions: the base must be positive and finite")

@@ -2,6 +2,7 @@
 values where they can go wrong."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -580,3 +581,46 @@ def test_offsets_past_32_bits(dtype):
     assert torch.equal(y[0], y[1])
     dx, dscale, _ = nnv.group_norm_backward(x.view(2, -1, 128), x.view(2, -1, 128), mean, rstd)
     assert torch.equal(dx[0], dx[1]) and torch.equal(mean[0], mean[1])
+
+
+def test_images_in_calls_at_once_and_graphs_of_one_pool():
+    """Three streams with calls of their own at once, two graphs that share memory replayed in turn, gradients that are one number, the same tensor several times."""
+    import nnv_amd as nnv
+    g = gen(97)
+    q, k, v, w = make_differ(g, 2, 200, 300, 4, 1, 64, BF16)
+    do = torch.ones(1, 1, 1, 1, dtype=BF16, device="cuda").expand(2, 200, 4, 128)
+    x, scale = rand(g, 2, 40, 50, 64, dtype=BF16), rand(g, 64, dtype=BF16)
+
+    def step():
+        o, lse, second = nnv.differential_attention(q, k, v, w, causal=True, for_backward=True)
+        y, mean, rstd = nnv.group_norm(x, 8, scale, activation="silu")
+        return [o, lse, second, *nnv.differential_attention_backward(do, q, k, v, w, o, lse, second, causal=True), y, *nnv.group_norm_backward(y, x, mean, rstd, scale, None, "silu")]
+
+    eager = step()
+    whole = nnv.differential_attention_backward(do.contiguous(), q, k, v, w, *eager[:3], causal=True)
+    assert all(torch.equal(a, e) for a, e in zip(eager[3:7], whole))
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    found = [None] * 3
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                found[i] = step()
+    torch.cuda.synchronize()
+    for f in found:
+        assert all(torch.equal(a, e) for a, e in zip(f, eager))
+    graphs, held = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for i, graph in enumerate(graphs):
+        with torch.cuda.graph(graph, pool=graphs[0].pool() if i else None):
+            held.append(step())
+    for n in range(3):
+        q.copy_(rand(gen(300 + n), *q.shape, dtype=BF16))
+        for i in (1, 0, 1):
+            graphs[i].replay()
+            fresh = step()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, e) for a, e in zip(held[i], fresh))
+    at = torch.arange(200, device="cuda")[:, None].expand(200, 2)
+    turned = nnv.rotate_positions([q] * 6, at, np.array([16, 16]))
+    assert all(torch.equal(t, nnv.rotate_positions(q, at.contiguous(), (16, 16))) for t in turned)
+    assert torch.equal(nnv.group_norm(x, np.int64(8))[0], nnv.group_norm(x, 8)[0])
