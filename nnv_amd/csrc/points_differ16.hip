@@ -80,10 +80,9 @@ __device__ __forceinline__ void zero_lds(T* lds) {
 // softmax beside them.)  At the end the second map's result meets the first one's in LDS, lane by lane.
 // (Four stages where they fit and every wave has as many transfers: 2 x 2048 x 2048, 16 heads of 64, 126 us, with two 136.  Else two: heads of 40 as above 64 us,
 // with four 67, of 96 109 us, with three 112.)
-// A map's weights are rounded to 16 bits in front of the product with v, and where the map counts for as much as the other one, half of them in two pieces: the rounded ones
-// and what that left.  The difference of the maps is smaller than either: with rounded weights alone the result is up to 1.6 times as far off as its own rounding (bf16: 0.0026
-// for 0.0017), with half of them in two pieces 0.0023, with all 0.0019.  (4096 x 4096, 16 heads of 128, causal: 450, 487, 528 us; 2048 x 2048, 16 heads
-// of 64: 131, 156, 171.)  With a weight of 0.6 it is the first map's.
+// A map's weights go into the product with v in two pieces of 16 bits each, the rounded ones and what that left, all of them: the difference of the maps is smaller than either, so that
+// rounded weights alone leave the result up to 1.6 times as far off as its own rounding (bf16: 0.0026 for 0.0017), and what is off must not go by where a key lies.
+// (2 x 4096 x 4096, 16 heads of 128, causal: 583 us, with rounded weights alone 450; 8 x 577 x 1000 by length, 12 heads of 40: 64 us.)
 template <int CH>
 constexpr int differ_stages = CH == 2 || CH == 4 ? 4 : 2;
 template <typename T, int CH>
@@ -119,9 +118,6 @@ __global__ __launch_bounds__(512, 2) void differ16_kernel(const DifferArgs a) {
     for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
   float off = -INFINITY, total = 0.0f;   // off: of the exponents, in products times unit
   bool far = false;                      // a row's is beyond kFar
-  // weights in two pieces (see above): where the other map's share is not a good deal larger
-  const float share = here ? fabsf(weight_of<T>(a, head_of_row(a, kv, r))) : 0.0f;
-  const bool two = __any(here && (map ? !(share < 0.75f) : !(0.75f * share > 1.0f)));
 
   const T* kp = (const T*)a.k.p + b * a.k.b + 2 * kv * a.k.h;
   const T* vp = (const T*)a.v.p + b * a.v.b + kv * a.v.h;
@@ -174,9 +170,8 @@ __global__ __launch_bounds__(512, 2) void differ16_kernel(const DifferArgs a) {
           for (int d = 0; d < SOME; ++d) x[d] = columns_operand<T, W>(vs_at, 32 * k + 16 * c, d0 + d);
 #pragma unroll
           for (int d = 0; d < SOME; ++d) acc[d0 + d] = Half8<T>::mfma(x[d], p, acc[d0 + d]);
-          if (c == 0 && two)
 #pragma unroll
-            for (int d = 0; d < SOME; ++d) acc[d0 + d] = Half8<T>::mfma(x[d], rest, acc[d0 + d]);
+          for (int d = 0; d < SOME; ++d) acc[d0 + d] = Half8<T>::mfma(x[d], rest, acc[d0 + d]);
         }
       }
   }

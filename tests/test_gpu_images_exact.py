@@ -1,0 +1,80 @@
+"""What the operators on points that are images or videos owe to the last bit of their results' type: nothing but the result is rounded to 16 bits where a
+second piece can hold what a first one leaves, in whatever order the keys lie; infinities that count stay infinite; masks and tiles that go on for long."""
+import math
+
+import pytest
+import torch
+
+from tests import images_oracle as io
+from tests import points_oracle as po
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+TYPES, IDS = [F32, BF16, F16], ["f32", "bf16", "f16"]
+
+
+def gen(seed=0):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def rand(g, *shape, dtype=F32, scale=1.0, shift=0.0):
+    return (torch.randn(*shape, generator=g, device="cuda") * scale + shift).to(dtype)
+
+
+def make_differ(g, b, lq, lk, h, hkv, d, dtype):
+    return (rand(g, b, lq, 2 * h, d, dtype=dtype), rand(g, b, lk, 2 * hkv, d, dtype=dtype), rand(g, b, lk, hkv, 2 * d, dtype=dtype),
+            rand(g, h, scale=0.1, shift=0.6))
+
+
+def check_differ(q, k, v, w, clean=None, tag="", **kw):
+    """Forward and backward against the 64-bit forms (of `clean` keys and values, where those that do not count hold something else)."""
+    import nnv_amd as nnv
+    ck, cv = clean or (k, v)
+    o, lse, second = nnv.differential_attention(q, k, v, w, for_backward=True, **kw)
+    for name, got, e, bd in zip(("o", "lse", "second"), (o, lse, second), io.differ(q, ck, cv, w, **kw), io.differ_bounds(q, ck, cv, w, **kw)):
+        po.assert_within(got, e, bd, tag + " " + name)
+    do = rand(gen(q.shape[1]), *o.shape, dtype=q.dtype)
+    grads = nnv.differential_attention_backward(do, q, k, v, w, o, lse, second, **kw)
+    for name, got, e, bd in zip(("dq", "dk", "dv", "dweights"), grads, io.differ_grad(do, q, ck, cv, w, **kw), io.differ_grad_bounds(do, q, ck, cv, w, **kw)):
+        po.assert_within(got, e, bd, tag + " " + name)
+
+
+def off(got, exact):
+    """How far a tensor is from what it should be, relative to that, as root mean squares."""
+    return float((got.double() - exact).norm() / exact.norm())
+
+
+def assert_rounded_once(got, exact, name):
+    """No further off than a rounding at the end: two pieces hold 2^-16 (bf16) or 2^-22 (f16) of a number, sums and exponents in f32 some 1e-6, whose squares are nothing
+    beside that of a rounding (0.0017, 0.00021); 2 % are left for them."""
+    own = off(exact.to(got.dtype), exact)
+    assert off(got, exact) <= 1.02 * own, "%s: %.3g off, its rounding is %.3g" % (name, off(got, exact), own)
+
+
+def lopsided(g, b, lq, lk, h, hkv, d, dtype, heavy):
+    """Keys that nearly all weight is on, or nearly none, by their place among 32 that follow one another."""
+    q, k, v, w = make_differ(g, b, lq, lk, h, hkv, d, dtype)
+    place = torch.arange(lk, device="cuda") % 32 // 16
+    q[..., 0], k[..., 0] = d ** 0.5, ((place == heavy).float() * 6 - 3)[None, :, None].to(dtype)
+    return q, k, v, w
+
+
+# queries, keys, head: single tokens, rows that fill a tile of few, many rows; heads of every template in 16 bits
+SIZES = [(1, 3000, 64), (3, 500, 128), (90, 1000, 64), (70, 600, 128), (150, 400, 40), (100, 300, 80), (65, 333, 96), (40, 257, 24)]
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize("size", SIZES, ids=lambda s: "x".join(map(str, s)))
+def test_results_are_rounded_once_in_whatever_order_the_keys_lie(size, dtype):
+    import nnv_amd as nnv
+    lq, lk, d = size
+    for heavy in (0, 1, 2):      # 2: no such keys
+        for weight in (0.6, 1.0, -2.5):
+            g = gen(lq + lk + heavy)
+            q, k, v, w = lopsided(g, 2, lq, lk, 4, 2, d, dtype, heavy)
+            w = w - 0.6 + weight
+            o, _, second = nnv.differential_attention(q, k, v, w, for_backward=True)
+            exact = io.differ(q, k, v, w)
+            assert_rounded_once(second, exact[2], "second, %d" % heavy)
+            assert_rounded_once(o, exact[0], "o, %d, %g" % (heavy, weight))
