@@ -1,5 +1,5 @@
 // Differential attention of points in 16 bits, backward, on v_mfma_f32_32x32x16_{bf16,f16}: the 16-bit forms of differ_query_grad_kernel and
-// differ_key_grad_kernel.  The weights' difference and the scores' gradients are rounded to 16 bits in front of the products that use them, the latter partly in two pieces
+// differ_key_grad_kernel.  The weights' difference is rounded to 16 bits in front of the product that uses it; the scores' gradients go into theirs in two pieces
 // (over_rows).  dq takes D from the rounded o and second; on the way it finds D again as the sum of weights times dP, in f32, which the gradients of weights and keys take:
 // a row that sees one key has a scores' gradient of zero, and what rounding makes of it would reach dk.
 //
@@ -73,9 +73,9 @@ struct Lift {
   __device__ __forceinline__ float down() const { return USED ? 1.0f / up : 1.0f; }
 };
 
-// acc[d] += the product over 32 rows, from `first` on, of a tile of rows of DP values with p, rounded; of half of them also with what the rounding left.  (The
-// scores' gradients cancel: of rounded ones alone dq and dk are up to 1.6 times as far off as their own rounding, 0.0026 for 0.0017 in bf16; of these 0.0021, and of two pieces
-// everywhere 0.0018.  2 x 4096 x 4096, 16 / 4 heads of 64, causal: dq 290, 335, 365 us, dk and dv 440, 470, 505.)
+// acc[d] += the product over 32 rows, from `first` on, of a tile of rows of DP values with p in two pieces, rounded and what that left.  (The scores' gradients
+// cancel: of rounded ones alone dq and dk are up to 1.6 times as far off as their own rounding, 0.0026 for 0.0017 in bf16.  The gradients of 2 x 4096 x 4096, 16 / 4 heads of 64,
+// causal, take 854 us, with rounded ones alone 710.)
 template <typename T, int DP>
 __device__ __forceinline__ void over_rows(unsigned tile, int first, const float16_t& p, float16_t (&acc)[DP / 32]) {
 #pragma unroll
@@ -85,7 +85,7 @@ __device__ __forceinline__ void over_rows(unsigned tile, int first, const float1
     for (int d = 0; d < DP / 32; ++d) {
       const half8<T> x = columns_operand<T, DP>(tile, first + 16 * c, d);
       acc[d] = Half8<T>::mfma(x, f, acc[d]);
-      if (c == 0) acc[d] = Half8<T>::mfma(x, left, acc[d]);
+      acc[d] = Half8<T>::mfma(x, left, acc[d]);
     }
   }
 }

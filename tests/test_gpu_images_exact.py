@@ -78,3 +78,44 @@ def test_results_are_rounded_once_in_whatever_order_the_keys_lie(size, dtype):
             exact = io.differ(q, k, v, w)
             assert_rounded_once(second, exact[2], "second, %d" % heavy)
             assert_rounded_once(o, exact[0], "o, %d, %g" % (heavy, weight))
+
+
+def exact_gradients(do, q, k, v, w, o, second, **kw):
+    """(dq, dk, dv, dweights) in f64, dq with D from the o and second of the call, as the operator has it; and what dweights may be off by: sums in f32."""
+    scale, group = q.shape[3] ** -0.5, q.shape[2] // k.shape[2]
+    _, dk, dv, dw = io.differ_grad(do, q, k, v, w, **kw)
+    c = io.seen(q, k, kw.get("key_lengths"), kw.get("key_mask"), kw.get("causal", False))
+    maps, vh = io._split_maps(q, k, v, c)
+    g = torch.where(c.any(2)[:, None, :, None], do.double().permute(0, 2, 1, 3), 0.0).contiguous()
+    dp, share = io._matmul(g, vh), w.double()[None, :, None, None]
+    rows = lambda x: (g * x.double().permute(0, 2, 1, 3)).sum(-1, keepdim=True)  # noqa: E731
+    deltas = [rows(o) + share * rows(second), rows(second)]
+    dq = [torch.matmul((-share if m else 1.0) * io._softmax(qm, km, c, scale)[0] * (dp - deltas[m]) * scale, km) for m, (qm, km) in enumerate(maps)]
+    size = (io._softmax(*maps[1], c, scale)[0] * io._matmul(g.abs(), vh.abs())).sum((0, 2, 3))
+    return io._by_map(*dq), dk, dv, dw, (k.shape[1] + 2 * q.shape[3] + 100) * po.U32 * size
+
+
+def gradients(dtype, size, heavy, **kw):
+    import nnv_amd as nnv
+    lq, lk, d = size
+    g = gen(lq + lk + heavy)
+    q, k, v, w = lopsided(g, 2, lq, lk, 4, 2, d, dtype, heavy)
+    q[:, :, 1::2, 1], k[:, :, 1::2, 1] = q[:, :, 1::2, 0], -k[:, :, 1::2, 0]      # (the second map's heavy keys are the others)
+    q[:, :, 1::2, 0] = 0
+    o, lse, second = nnv.differential_attention(q, k, v, w, for_backward=True, **kw)
+    do = rand(g, *o.shape, dtype=dtype)
+    return nnv.differential_attention_backward(do, q, k, v, w, o, lse, second, **kw), exact_gradients(do, q, k, v, w, o, second, **kw)
+
+
+GRAD_SIZES = [(90, 1000, 64), (300, 333, 64), (70, 600, 128), (150, 400, 40), (100, 300, 80), (65, 333, 96), (40, 257, 24), (8, 500, 96)]
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize("size", GRAD_SIZES, ids=lambda s: "x".join(map(str, s)))
+def test_gradients_of_queries_and_keys_are_rounded_once(size, dtype):
+    for heavy in (0, 1, 2):
+        for causal in (False, True):
+            got, exact = gradients(dtype, size, heavy, causal=causal)
+            for i, name in enumerate(("dq", "dk")):
+                assert_rounded_once(got[i], exact[i], "%s %d %s" % (name, heavy, causal))
+            assert ((got[3].double() - exact[3]).abs() <= exact[4]).all()
