@@ -1,6 +1,5 @@
 // Differential attention of points in 16 bits, backward, on v_mfma_f32_32x32x16_{bf16,f16}: the 16-bit forms of differ_query_grad_kernel and
-// differ_key_grad_kernel.  The weights' difference is rounded to 16 bits in front of the product that uses it; the scores' gradients go into theirs in two pieces
-// (over_rows).  dq takes D from the rounded o and second; on the way it finds D again as the sum of weights times dP, in f32, which the gradients of weights and keys take:
+// differ_key_grad_kernel.  The weights' difference and the scores' gradients go into their products in two pieces of 16 bits each.  dq takes D from the rounded o and second; on the way it finds D again as the sum of weights times dP, in f32, which the gradients of weights and keys take:
 // a row that sees one key has a scores' gradient of zero, and what rounding makes of it would reach dk.
 //
 // f16 does not hold the scores' gradients as they are: weights far below one times differences of any size.  What a lane rounds is all of one column of the
@@ -356,11 +355,19 @@ __global__ __launch_bounds__(64 * kKeyWaves<CH>, kKeyWaves<CH> / 4) void differ_
         }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          half8<T> both;
+          half8<T> both, left;   // in two pieces, as the scores' gradients
 #pragma unroll
-          for (int i = 0; i < 8; ++i) both[i] = (T)((s[0][0][8 * c + i] + s[1][0][8 * c + i]) * wide_up);
+          for (int i = 0; i < 8; ++i) {
+            const float x = (s[0][0][8 * c + i] + s[1][0][8 * c + i]) * wide_up;
+            both[i] = (T)x;
+            left[i] = (T)(x - (float)both[i]);
+          }
 #pragma unroll
-          for (int d = 0; d < CH; ++d) dv[d] = Half8<T>::mfma(columns_operand<T, W>(gc_at, 16 * c, d), both, dv[d]);
+          for (int d = 0; d < CH; ++d) {
+            const half8<T> x = columns_operand<T, W>(gc_at, 16 * c, d);
+            dv[d] = Half8<T>::mfma(x, both, dv[d]);
+            dv[d] = Half8<T>::mfma(x, left, dv[d]);
+          }
         }
 #pragma unroll
         for (int m = 0; m < 2; ++m) {

@@ -267,9 +267,8 @@ def differential_attention(q, k, v, weights, key_lengths=None, key_mask=None, ca
     Returns (o, lse, second): o, batch x queries x heads x 2 head, of q's type; the logarithms of both maps' softmax sums, batch x 2 heads x queries, f32; and, if
     for_backward, the second map's softmax times v, in o's shape and type, else None.  A query that sees no key has the result 0 and the logarithm -inf.
 
-    In 16 bits the maps' weights, and in the backward pass the gradients of the scores, go into their products in two pieces that hold all but 2^-16 of them (2^-22 in f16), so that a
-    result is off by its own rounding alone.  In the backward pass dq takes D, the sum of do times each map's result, from the o and second that were rounded, and the weights' difference in front of dv
-    is rounded: dv is up to 0.0025 off, where one rounding at the end gives 0.0017 (bf16)."""
+    In 16 bits the maps' weights, and in the backward pass their difference and the gradients of the scores, go into their products in two pieces that hold all but 2^-16 of them (2^-22
+    in f16), so that a result is off by its own rounding alone.  But dq takes D, the sum of do times each map's result, from the o and second that were rounded."""
     what = "differential_attention"
     ctx, lib, stream = _enter(what, ctx, q, k, v, weights, key_lengths, key_mask)
     sizes = _differ_sizes(what, q, k, v, weights, key_lengths, key_mask, scale)

@@ -119,3 +119,12 @@ def test_gradients_of_queries_and_keys_are_rounded_once(size, dtype):
             for i, name in enumerate(("dq", "dk")):
                 assert_rounded_once(got[i], exact[i], "%s %d %s" % (name, heavy, causal))
             assert ((got[3].double() - exact[3]).abs() <= exact[4]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize("size", GRAD_SIZES + [(700, 5, 64)], ids=lambda s: "x".join(map(str, s)))
+def test_gradients_of_values_are_rounded_once(size, dtype):
+    for heavy in (0, 1, 2):
+        for causal in (False, True):
+            got, exact = gradients(dtype, size, heavy, causal=causal)
+            assert_rounded_once(got[2], exact[2], "dv %d %s" % (heavy, causal))
