@@ -42,31 +42,25 @@ template <typename T>
 struct Lift {
   static constexpr bool USED = std::is_same_v<T, f16_t>;
   float up = USED ? 0x1p40f : 1.0f;
-  // M sets of values of a column, in this lane and l ^ 32: what has been added up of them so far is scaled where a value is larger than any before
-  template <int M, int N>
-  __device__ __forceinline__ void raise(float16_t (*s)[1], float16_t (&acc)[M][N]) {
+  // values of a column, in this lane and l ^ 32: what has been added up of them so far is scaled where a value is larger than any before
+  template <int N>
+  __device__ __forceinline__ void raise(float16_t& s, float16_t (&acc)[N]) {
     if constexpr (USED) {
       float top = 0.0f;
 #pragma unroll
-      for (int m = 0; m < M; ++m)
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) top = max3_of_sizes(top, s[m][0][i], s[m][0][i + 1]);
+      for (int i = 0; i < 16; i += 2) top = max3_of_sizes(top, s[i], s[i + 1]);
       top = max_of_halves(top);
       if (__any(top * up > 32768.0f)) {
         // (an infinite or missing value is not lifted, and does what it would)
         const float next = top * up > 32768.0f && top < INFINITY ? __builtin_amdgcn_ldexpf(1.0f, 14 - __builtin_amdgcn_frexp_expf(top)) : up, fade = next / up;
         up = next;
 #pragma unroll
-        for (int m = 0; m < M; ++m)
+        for (int d = 0; d < N; ++d)
 #pragma unroll
-          for (int d = 0; d < N; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[m][d][i] *= fade;
+          for (int i = 0; i < 16; ++i) acc[d][i] *= fade;
       }
 #pragma unroll
-      for (int m = 0; m < M; ++m)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[m][0][i] *= up;
+      for (int i = 0; i < 16; ++i) s[i] *= up;
     }
   }
   __device__ __forceinline__ float down() const { return USED ? 1.0f / up : 1.0f; }
@@ -144,11 +138,11 @@ __global__ __launch_bounds__(64 * kWaves<CH>, kWaves<CH> / 4) void differ_query_
 #pragma unroll
   for (int m = 0; m < 2; ++m) load_operands<T, CH>(qf[m], (const T*)a.q.p + (here ? map_row_at(a.q, a, b, kv, r, m) : 0), h, a.head, takes_part);
   load_operands<T, 2 * CH>(gf, (const T*)a.go.p + (here ? row_at(a.go, a, b, kv, r) : 0), h, 2 * a.head, takes_part);
-  float16_t dq[2][1][DP / 32];
+  float16_t dq[2][DP / 32];
   Lift<T> lift[2];
   float dot[2] = {0.0f, 0.0f};   // D again, of the weights and dP, for the weights' and the keys' gradients (o and second are rounded)
 #pragma unroll
-  for (int m = 0; m < 2; ++m) zero(dq[m][0]);
+  for (int m = 0; m < 2; ++m) zero(dq[m]);
   const T* kp = (const T*)a.k.p + b * a.k.b + 2 * kv * a.k.h;
   const T* vp = (const T*)a.v.p + b * a.v.b + kv * a.v.h;
   Load load;
@@ -195,8 +189,8 @@ __global__ __launch_bounds__(64 * kWaves<CH>, kWaves<CH> / 4) void differ_query_
           dot[m] += s[m][0][i] * dp[0][i];
           s[m][0][i] *= by * (dp[0][i] - delta[m]);
         }
-        lift[m].raise(&s[m], dq[m]);
-        over_rows<T, DP>(kc_at + m * (2 * Load::MAP), 0, s[m][0], dq[m][0]);
+        lift[m].raise(s[m][0], dq[m]);
+        over_rows<T, DP>(kc_at + m * (2 * Load::MAP), 0, s[m][0], dq[m]);
       }
     }
   }
@@ -209,8 +203,8 @@ __global__ __launch_bounds__(64 * kWaves<CH>, kWaves<CH> / 4) void differ_query_
       a.dots[split * own_rows(a) + own_row(a, bkv, r, m)] = dot[m];
       if (a.splits == 1) *info_at(a, bkv, r, kDelta0 + m) = dot[m];   // else differ_sum_rows_kernel does
     }
-    if (a.splits > 1) store_result(a.part + (split * own_rows(a) + own_row(a, bkv, r, m)) * a.head, dq[m][0], a.scale * lift[m].down(), h, a.head);
-    else store_result((T*)a.dq + dense_map_row_at(a, b, kv, r, m), dq[m][0], a.scale * lift[m].down(), h, a.head);
+    if (a.splits > 1) store_result(a.part + (split * own_rows(a) + own_row(a, bkv, r, m)) * a.head, dq[m], a.scale * lift[m].down(), h, a.head);
+    else store_result((T*)a.dq + dense_map_row_at(a, b, kv, r, m), dq[m], a.scale * lift[m].down(), h, a.head);
   }
 }
 
@@ -265,7 +259,7 @@ __global__ __launch_bounds__(64 * kKeyWaves<CH>, kKeyWaves<CH> / 4) void differ_
       return x;
     };
     float16_t dk[2][DP / 32], dv[CH];
-    Lift<T> lift;
+    Lift<T> lift[2];
 #pragma unroll
     for (int m = 0; m < 2; ++m) zero(dk[m]);
     zero(dv);
@@ -378,12 +372,8 @@ __global__ __launch_bounds__(64 * kKeyWaves<CH>, kKeyWaves<CH> / 4) void differ_
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[m][0][4 * i4 + i] *= dp[0][4 * i4 + i] - f[i];
           }
-          if constexpr (!Lift<T>::USED) over_rows<T, DP>(qc_at + m * (2 * Load::MAP), 0, s[m][0], dk[m]);
-        }
-        if constexpr (Lift<T>::USED) {
-          lift.raise(s, dk);
-#pragma unroll
-          for (int m = 0; m < 2; ++m) over_rows<T, DP>(qc_at + m * (2 * Load::MAP), 0, s[m][0], dk[m]);
+          lift[m].raise(s[m][0], dk[m]);
+          over_rows<T, DP>(qc_at + m * (2 * Load::MAP), 0, s[m][0], dk[m]);
         }
       }
     }
@@ -397,11 +387,11 @@ __global__ __launch_bounds__(64 * kKeyWaves<CH>, kKeyWaves<CH> / 4) void differ_
       if (a.splits > 1) {
         const int64_t all = (int64_t)a.batch * a.keys * a.kv_heads * 2 * a.head;
 #pragma unroll
-        for (int m = 0; m < 2; ++m) store_result(a.part + split * all + dense + m * a.head, dk[m], a.scale * lift.down(), h, a.head);
+        for (int m = 0; m < 2; ++m) store_result(a.part + split * all + dense + m * a.head, dk[m], a.scale * lift[m].down(), h, a.head);
         store_result(a.part + (a.splits + split) * all + dense, dv, 1.0f / wide_up, h, 2 * a.head);
       } else {
 #pragma unroll
-        for (int m = 0; m < 2; ++m) store_result((T*)a.dk + dense + m * a.head, dk[m], a.scale * lift.down(), h, a.head);
+        for (int m = 0; m < 2; ++m) store_result((T*)a.dk + dense + m * a.head, dk[m], a.scale * lift[m].down(), h, a.head);
         store_result((T*)a.dv + dense, dv, 1.0f / wide_up, h, 2 * a.head);
       }
     }

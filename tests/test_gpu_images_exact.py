@@ -128,3 +128,22 @@ def test_gradients_of_values_are_rounded_once(size, dtype):
         for causal in (False, True):
             got, exact = gradients(dtype, size, heavy, causal=causal)
             assert_rounded_once(got[2], exact[2], "dv %d %s" % (heavy, causal))
+
+
+@pytest.mark.parametrize("size", [(90, 200, 64), (70, 150, 128), (60, 333, 40)], ids=lambda s: "x".join(map(str, s)))
+def test_f16_keeps_the_bits_of_small_gradients_beside_large_ones(size):
+    """The second map's keys in f16, whose gradients are 2^-24 of the first one's: each map's are lifted for themselves.  (As test_gradients_..._rounded_once: no further off
+    than their own rounding.)"""
+    import nnv_amd as nnv
+    lq, lk, d = size
+    g = gen(5)
+    q, k, v, w = make_differ(g, 2, lq, lk, 4, 2, d, F16)
+    w = w * 2.0 ** -24
+    o, lse, second = nnv.differential_attention(q, k, v, w, for_backward=True)
+    do = (rand(g, *o.shape) * 8192).to(F16)
+    got = nnv.differential_attention_backward(do, q, k, v, w, o, lse, second)
+    exact = exact_gradients(do, q, k, v, w, o, second)
+    for i, name in enumerate(("dq", "dk")):
+        for m in (0, 1):
+            assert bool(exact[i][:, :, m::2].abs().max() < 2.0 ** 15)
+            assert_rounded_once(got[i][:, :, m::2], exact[i][:, :, m::2], "%s of map %d" % (name, m))
