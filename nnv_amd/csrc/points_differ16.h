@@ -5,13 +5,25 @@
 
 namespace nnvhip {
 
-// what rounding eight weights to p leaves
-template <typename T>
-__device__ __forceinline__ half8<T> rest8(const float16_t& s, const half8<T>& p, int first) {
-  half8<T> r;
+// Eight values in two pieces: p, rounded towards zero, and what that leaves (to 2^-16 of the value in bf16, 2^-22 in f16).  Both have the value's sign, and
+// the second one is not zero where the first one is not (2^-23 of the value are added to it): an infinite number times either piece is the same infinity, and their sum no
+// NaN.  (In f16 the second piece of a value below 2^-13 may be zero.)  value(i): the i-th one
+template <typename T, class Value>
+__device__ __forceinline__ void pieces8(Value value, half8<T>& p, half8<T>& rest) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = (T)(s[first + i] - (float)p[i]);
-  return r;
+  for (int i = 0; i < 8; i += 2) {
+    const float x[2] = {value(i), value(i + 1)};   // (floats of their own: the bits of a vector's element are taken of its first one)
+    if constexpr (std::is_same_v<T, f16_t>) {
+      const auto two = __builtin_amdgcn_cvt_pkrtz(x[0], x[1]);
+      p[i] = (T)two[0];
+      p[i + 1] = (T)two[1];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) p[i + j] = __builtin_bit_cast(T, (uint16_t)(__builtin_bit_cast(unsigned, x[j]) >> 16));
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) rest[i + j] = (T)fmaf(x[j], 1.0f + 0x1p-23f, -(float)p[i + j]);
+  }
 }
 
 // A tile of ROWS rows: those of the first map (DP values each, the head rounded up to 32), of the second one, and the wide ones (W, twice the head

@@ -80,9 +80,9 @@ __device__ __forceinline__ void zero_lds(T* lds) {
 // softmax beside them.)  At the end the second map's result meets the first one's in LDS, lane by lane.
 // (Four stages where they fit and every wave has as many transfers: 2 x 2048 x 2048, 16 heads of 64, 126 us, with two 136.  Else two: heads of 40 as above 64 us,
 // with four 67, of 96 109 us, with three 112.)
-// A map's weights go into the product with v in two pieces of 16 bits each, the rounded ones and what that left, all of them: the difference of the maps is smaller than either, so that
+// A map's weights go into the product with v in two pieces of 16 bits each (pieces8), all of them: the difference of the maps is smaller than either, so that
 // rounded weights alone leave the result up to 1.6 times as far off as its own rounding (bf16: 0.0026 for 0.0017), and what is off must not go by where a key lies.
-// (2 x 4096 x 4096, 16 heads of 128, causal: 583 us, with rounded weights alone 450; 8 x 577 x 1000 by length, 12 heads of 40: 64 us.)
+// (2 x 4096 x 4096, 16 heads of 128, causal: 572 us, with rounded weights alone 450; 8 x 577 x 1000 by length, 12 heads of 40: 61 us.)
 template <int CH>
 constexpr int differ_stages = CH == 2 || CH == 4 ? 4 : 2;
 template <typename T, int CH>
@@ -161,7 +161,8 @@ __global__ __launch_bounds__(512, 2) void differ16_kernel(const DifferArgs a) {
     for (int k = 0; k < 2; ++k)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const half8<T> p = round8<T>(s[k], 8 * c), rest = rest8<T>(s[k], p, 8 * c);
+        half8<T> p, rest;
+        pieces8<T>([&](int i) { return s[k][8 * c + i]; }, p, rest);
         constexpr int SOME = CH % 4 == 0 ? 4 : CH % 3 == 0 ? 3 : CH;
 #pragma unroll
         for (int d0 = 0; d0 < CH; d0 += SOME) {
@@ -299,10 +300,7 @@ __global__ __launch_bounds__(64 * differ_groups<CH>(), 1) void differ16_few_kern
         for (int i = 0; i < 16; ++i) acc[d][i] *= fade;
     half8<T> p[2], rest[2];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      p[c] = round8<T>(s[0], 8 * c);
-      rest[c] = rest8<T>(s[0], p[c], 8 * c);
-    }
+    for (int c = 0; c < 2; ++c) pieces8<T>([&](int i) { return s[0][8 * c + i]; }, p[c], rest[c]);
     over_columns<T, W, 2>(vs_at, 0, [&](int c, int d, const half8<T>& v) {
       acc[d] = Half8<T>::mfma(v, p[c], acc[d]);
       acc[d] = Half8<T>::mfma(v, rest[c], acc[d]);

@@ -66,14 +66,15 @@ struct Lift {
   __device__ __forceinline__ float down() const { return USED ? 1.0f / up : 1.0f; }
 };
 
-// acc[d] += the product over 32 rows, from `first` on, of a tile of rows of DP values with p in two pieces, rounded and what that left.  (The scores' gradients
+// acc[d] += the product over 32 rows, from `first` on, of a tile of rows of DP values with p in two pieces.  (The scores' gradients
 // cancel: of rounded ones alone dq and dk are up to 1.6 times as far off as their own rounding, 0.0026 for 0.0017 in bf16.  The gradients of 2 x 4096 x 4096, 16 / 4 heads of 64,
-// causal, take 854 us, with rounded ones alone 710.)
+// causal, take 862 us, with rounded ones alone 710.)
 template <typename T, int DP>
 __device__ __forceinline__ void over_rows(unsigned tile, int first, const float16_t& p, float16_t (&acc)[DP / 32]) {
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    const half8<T> f = round8<T>(p, 8 * c), left = rest8<T>(p, f, 8 * c);
+    half8<T> f, left;
+    pieces8<T>([&](int i) { return p[8 * c + i]; }, f, left);
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) {
       const half8<T> x = columns_operand<T, DP>(tile, first + 16 * c, d);
@@ -350,12 +351,7 @@ __global__ __launch_bounds__(64 * kKeyWaves<CH>, kKeyWaves<CH> / 4) void differ_
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           half8<T> both, left;   // in two pieces, as the scores' gradients
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float x = (s[0][0][8 * c + i] + s[1][0][8 * c + i]) * wide_up;
-            both[i] = (T)x;
-            left[i] = (T)(x - (float)both[i]);
-          }
+          pieces8<T>([&](int i) { return (s[0][0][8 * c + i] + s[1][0][8 * c + i]) * wide_up; }, both, left);
 #pragma unroll
           for (int d = 0; d < CH; ++d) {
             const half8<T> x = columns_operand<T, W>(gc_at, 16 * c, d);

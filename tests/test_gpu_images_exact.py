@@ -147,3 +147,30 @@ def test_f16_keeps_the_bits_of_small_gradients_beside_large_ones(size):
         for m in (0, 1):
             assert bool(exact[i][:, :, m::2].abs().max() < 2.0 ** 15)
             assert_rounded_once(got[i][:, :, m::2], exact[i][:, :, m::2], "%s of map %d" % (name, m))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_an_infinite_value_that_counts_stays_infinite(dtype):
+    """Of a weight in two pieces neither makes an infinite value a NaN: second is infinite there, and so is o where the weight's sign adds the maps up."""
+    import nnv_amd as nnv
+    for lq, lk, d in ((1, 300, 64), (1, 70, 128), (16, 200, 40), (90, 200, 64), (70, 150, 128), (40, 333, 48)):
+        for flat in (False, True):      # flat: every weight is a power of two, and its second piece would be zero
+            g = gen(lq + d)
+            q, k, v, w = make_differ(g, 2, lq, lk, 4, 2, d, dtype)
+            q = (q * (0.0 if flat else 0.3)).to(dtype)
+            w = -w
+            for at, value in ((3, math.inf), (20, -math.inf), (lk - 1, math.inf)):
+                v[1, at, 0, at % (2 * d)] = value
+            o, _, second = nnv.differential_attention(q, k, v, w, for_backward=True)
+            exact, bounds = io.differ(q, k, v, w), io.differ_bounds(q, k, v, w)
+            assert bool(exact[2].isinf().any()) and not bool(exact[2].isnan().any())
+            for name, got, e, bd in (("o", o, exact[0], bounds[0]), ("second", second, exact[2], bounds[2])):
+                po.assert_within(got, e, bd, "%d %d %s %s" % (lq, d, flat, name))
+            # and an infinite gradient of the result is infinite in dv of every key
+            v = rand(g, *v.shape, dtype=dtype)
+            o, lse, second = nnv.differential_attention(q, k, v, w, for_backward=True)
+            do = rand(g, *o.shape, dtype=dtype)
+            do[1, lq // 2, 1, 5], do[1, 0, 3, 7] = math.inf, -math.inf
+            got, exact = (f(do, q, k, v, w, *s)[2] for f, s in ((nnv.differential_attention_backward, (o, lse, second)), (io.differ_grad, ())))
+            assert bool((exact[1, :, 0, 5] == math.inf).all()) and bool((exact[1, :, 1, 7] == -math.inf).all())
+            po.assert_within(got, exact, io.differ_grad_bounds(do, q, k, v, w)[2], "%d %d %s dv" % (lq, d, flat))
