@@ -23,7 +23,7 @@ struct DifferArgs : AttendArgs {   // (its lse is the caller's; scale, masks and
   void* dweights;
   float* info;                     // [sequence, key/value head][kInfos][info_rows]: see RowInfo
   int info_rows;                   // rows, rounded up to kInfoRows
-  float* dots;                     // D as the 16-bit form finds it, [split][sequence, key/value head][map][row]; else null
+  float* dots;                     // D of 16-bit tensors as the kernel of dq finds it, [split][sequence, key/value head][map][row]; else null
 };
 
 // What the gradients of keys need of a row, as arrays over the rows of a key/value head that a tile's transfer takes as they lie: the exponents' offsets of both

@@ -2,7 +2,8 @@
 //
 // As in points_attend_grad.hip two kernels form dq (a wave per 16 queries, both maps) and dk, dv (a wave per 16 keys), each sum in the registers of
 // one wave, in a fixed order, with no atomics.  do v^T, half of what the scores' gradients take, is one product for both maps.  D of both maps and
-// the weights' gradients come first.
+// the weights' gradients come first.  Of 16-bit tensors, whose o and second are rounded, the kernel of dq finds D again on its way, as the sum of weights times dP in f32, which the gradients
+// of weights and keys take: a row that sees one key has a scores' gradient of zero, and what rounding makes of it would reach dk.
 //
 // Bound by the f32 matrix instructions (4 x 1024 x 1024, 16 heads of 64: dq 475 us, dk and dv 740; 4 x 333 x 577, 6 heads of 40: 49 and 68, matrix units busy 48
 // and 44 %: blocks of six or seven tiles, in whose beginning and end nothing is multiplied).  Two buffers in LDS, and so one barrier a tile instead of two, measured the same.
@@ -14,6 +15,8 @@ namespace nnvhip {
 namespace {
 
 constexpr int kBlockRows = 64;   // rows, or keys, of a block
+template <typename T>
+constexpr bool kHalves = sizeof(T) == 2;
 
 // D_1 = rowsum(do second), D_0 = rowsum(do o) + w D_1: 16 lanes a row.
 template <typename T, int>
@@ -116,6 +119,7 @@ __global__ __launch_bounds__(256, CH <= 6 ? 2 : 1) void differ_query_grad_kernel
   for (int m = 0; m < 2; ++m) f32_operands<T, CH>((const T*)a.q.p + (here ? map_row_at(a.q, a, b, kv, r, m) : 0), q4, a.head, takes_part, qf[m]);
   f32_operands<T, 2 * CH>((const T*)a.go.p + (here ? row_at(a.go, a, b, kv, r) : 0), q4, 2 * a.head, takes_part, gf);
   float4_t dq[2][CH];
+  float dot[2] = {0.0f, 0.0f};   // of 16-bit tensors D again, for the gradients of weights and keys (o and second are rounded)
 #pragma unroll
   for (int m = 0; m < 2; ++m) f32_zero(dq[m]);
   const T* kp = (const T*)a.k.p + b * a.k.b + 2 * kv * a.k.h;
@@ -146,12 +150,27 @@ __global__ __launch_bounds__(256, CH <= 6 ? 2 : 1) void differ_query_grad_kernel
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          s[k][i] = f32_bit(mine, k, i, q4) ? by * exp2_(s[k][i] * unit - offset[m]) * (dp[k][i] - delta[m]) : 0.0f;
+        for (int i = 0; i < 4; ++i) {
+          const bool sees = f32_bit(mine, k, i, q4);
+          const float p = exp2_(s[k][i] * unit - offset[m]);
+          if constexpr (kHalves<T>) dot[m] += sees ? p * dp[k][i] : 0.0f;
+          s[k][i] = sees ? by * p * (dp[k][i] - delta[m]) : 0.0f;
+        }
       f32_over_rows<CH, CH>(tile + 4 * q4 * LD + col + m * 16 * CH, s, dq[m]);
     }
   }
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+    if constexpr (kHalves<T>) dot[m] = quarters_sum(dot[m]);
   if (!here) return;
+  if constexpr (kHalves<T>) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+      if (q4 == 0) {
+        a.dots[split * own_rows(a) + own_row(a, bkv, r, m)] = dot[m];
+        if (a.splits == 1) a.delta[own_row(a, bkv, r, m)] = dot[m];   // (the row's own, read above.  Else differ_sum_rows_kernel does)
+      }
+  }
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
     if (a.splits > 1) f32_store<FOUR>(a.part + (split * own_rows(a) + own_row(a, bkv, r, m)) * a.head, dq[m], a.scale, q4, a.head);
@@ -293,7 +312,7 @@ __global__ __launch_bounds__(256) void differ_sum_kernel(const DifferArgs a, int
   }
   ((T*)(which ? a.dv : a.dk))[e] = from_f<T>(s);
 }
-// dq's maps' rows from the splits', written in the order of the tensor, and D of the 16-bit form: a wave a row
+// dq's maps' rows from the splits', written in the order of the tensor, and D of 16-bit tensors: a wave a row
 template <typename T, int>
 __global__ __launch_bounds__(256) void differ_sum_rows_kernel(const DifferArgs a) {
   const int64_t all = own_rows(a), own = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -305,7 +324,7 @@ __global__ __launch_bounds__(256) void differ_sum_rows_kernel(const DifferArgs a
   if (a.dots && (threadIdx.x & 63) == 0) {
     float s = 0.0f;
     for (int k = 0; k < a.splits; ++k) s += a.dots[k * all + own];
-    *info_at(a, bkv, r, kDelta0 + m) = s;
+    (a.info ? *info_at(a, bkv, r, kDelta0 + m) : a.delta[own]) = s;
   }
   for (int d = threadIdx.x & 63; d < a.head; d += 64) {
     float s = 0.0f;
@@ -318,7 +337,7 @@ struct GradCut {
   int row_tiles, key_tiles, key_blocks, query_splits, key_splits;
   int64_t delta, info, dots, part;   // floats of the workspace
 };
-GradCut grad_cut(int64_t batch, int64_t kv_heads, int64_t queries, int64_t rows, int64_t keys, int64_t head, bool causal, bool by16) {
+GradCut grad_cut(int64_t batch, int64_t kv_heads, int64_t queries, int64_t rows, int64_t keys, int64_t head, bool causal, bool halves, bool by16) {
   GradCut c;
   c.row_tiles = (int)ceil_div(rows, by16 ? differ_grad16_tile(head) : kBlockRows);
   c.key_tiles = (int)ceil_div(keys, by16 ? differ_key_grad16_tile(head) : kBlockRows);
@@ -332,7 +351,7 @@ GradCut grad_cut(int64_t batch, int64_t kv_heads, int64_t queries, int64_t rows,
   c.key_splits = split_of(heads * c.key_blocks, ceil_div(useful, 32), 2, by16 || head > 64 ? 256 : 512, start, join(heads * 4 * keys * head));
   c.delta = round_up(batch * kv_heads * 2 * rows, 64);
   c.info = by16 ? batch * kv_heads * kInfos * round_up(rows, kInfoRows) : 0;
-  c.dots = by16 ? round_up(c.query_splits * batch * kv_heads * 2 * rows, 64) : 0;
+  c.dots = halves ? round_up(c.query_splits * batch * kv_heads * 2 * rows, 64) : 0;
   const int64_t q = c.query_splits > 1 ? c.query_splits * batch * kv_heads * 2 * rows * head : 0;
   const int64_t k = c.key_splits > 1 ? 2 * c.key_splits * batch * kv_heads * keys * 2 * head : 0;
   c.part = std::max(q, k);
@@ -392,7 +411,7 @@ int nnvhip_differential_attention_backward_workspace(const nnvhip_differ_args* d
   if (heads * ceil_div(d->keys, kBlockRows) > blocks) NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_differential_attention_backward: too many keys");
   *bytes = 0;   // whichever kernels the alignment of the tensors lets take the call
   for (const bool by16 : {false, true}) {
-    const GradCut c = grad_cut(d->batch, d->kv_heads, d->queries, d->queries * (d->heads / d->kv_heads), d->keys, d->head, d->causal != 0, by16);
+    const GradCut c = grad_cut(d->batch, d->kv_heads, d->queries, d->queries * (d->heads / d->kv_heads), d->keys, d->head, d->causal != 0, d->type != NNVHIP_TYPE_F32, by16);
     if (heads * c.row_tiles * c.query_splits > blocks) NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_differential_attention_backward: too many rows");
     if (heads * c.key_blocks * c.key_splits > blocks || (c.key_splits > 1 && ceil_div(heads * d->keys * 2 * d->head, 256) > blocks))
       NNV_FAIL(NNVHIP_ERR_SHAPE, "nnvhip_differential_attention_backward: too many keys");
@@ -410,7 +429,7 @@ int nnvhip_differential_attention_backward(nnvhip_ctx* ctx, const nnvhip_differ_
   if (need > workspace_bytes || (need && !workspace))
     NNV_FAIL(NNVHIP_ERR_ARG, "nnvhip_differential_attention_backward: a workspace of %lld bytes is needed", (long long)need);
   const bool by16 = differ_grad16_takes(a, (int)d->type);
-  const GradCut c = grad_cut(a.batch, a.kv_heads, a.queries, a.rows, a.keys, a.head, a.causal, by16);
+  const GradCut c = grad_cut(a.batch, a.kv_heads, a.queries, a.rows, a.keys, a.head, a.causal, d->type != NNVHIP_TYPE_F32, by16);
   a.delta = static_cast<float*>(workspace);
   a.info = c.info ? a.delta + c.delta : nullptr;
   a.info_rows = (int)round_up(a.rows, kInfoRows);

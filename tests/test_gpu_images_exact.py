@@ -174,3 +174,39 @@ def test_an_infinite_value_that_counts_stays_infinite(dtype):
             got, exact = (f(do, q, k, v, w, *s)[2] for f, s in ((nnv.differential_attention_backward, (o, lse, second)), (io.differ_grad, ())))
             assert bool((exact[1, :, 0, 5] == math.inf).all()) and bool((exact[1, :, 1, 7] == -math.inf).all())
             po.assert_within(got, exact, io.differ_grad_bounds(do, q, k, v, w)[2], "%d %d %s dv" % (lq, d, flat))
+
+
+# heads that are no multiple of 8, which the kernels with products in f32 take
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize("size", [(90, 400, 60), (70, 200, 33), (9, 900, 126), (300, 40, 50)], ids=lambda s: "x".join(map(str, s)))
+def test_gradients_of_odd_heads_are_rounded_once(size, dtype):
+    for heavy in (0, 2):
+        for causal in (False, True):
+            got, exact = gradients(dtype, size, heavy, causal=causal)
+            for i, name in enumerate(("dq", "dk", "dv")):
+                assert_rounded_once(got[i], exact[i], "%s %d %s" % (name, heavy, causal))
+            assert ((got[3].double() - exact[3]).abs() <= exact[4]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_a_row_that_sees_one_key_has_no_gradient_for_it(dtype):
+    """Its weight is one whatever the score: what dk is beside zero comes of sums in f32, not of the o and second that were rounded to 16 bits."""
+    import nnv_amd as nnv
+    for lq, lk, d in ((40, 50, 64), (70, 90, 128), (100, 30, 40), (40, 50, 60), (33, 70, 7), (1, 20, 64)):
+        g = gen(d)
+        q, k, v, w = make_differ(g, 2, lq, lk, 4, 2, d, dtype)
+        lengths = torch.ones(2, dtype=torch.int32, device="cuda")
+        o, lse, second = nnv.differential_attention(q, k, v, w, key_lengths=lengths, for_backward=True)
+        do = rand(g, *o.shape, dtype=dtype)
+        dk = nnv.differential_attention_backward(do, q, k, v, w, o, lse, second, key_lengths=lengths)[1]
+        assert (dk[:, 1:] == 0).all()
+        # a weight is off by what its score (twice: in lse as well) and its exponent are, D by the sums of do v; both times do v
+        size = q.shape[3] ** -0.5
+        heads = lambda x, n: x.double().abs().repeat_interleave(n, 2)  # noqa: E731   (key/value heads to heads)
+        k0, v0, qa = heads(k[:, 0].view(2, 1, 2, 2 * d), 2).view(2, 1, 8, d), heads(v[:, :1], 2), q.double().abs()
+        score = (qa * k0).sum(-1) * size
+        dp = (do.double().abs() * v0).sum(-1).repeat_interleave(2, 2)
+        off = (2 * (d + 16) * score + 8 * score + 4 * d + 64) * po.U32
+        by = torch.stack([torch.ones(4, device="cuda"), w.abs() + 0], 1).flatten().double() + w.abs().double().max()   # (the first map's D is formed from o and second)
+        bound = ((size * by * off * dp)[..., None] * qa).sum(1).view(2, 2, 2, 2, d).sum(2).reshape(2, 4, d)
+        assert (dk[:, 0].double().abs() <= bound + po.TINY[dtype]).all(), (lq, lk, d)
