@@ -1,5 +1,6 @@
 // Differential attention of points in 16 bits, backward, on v_mfma_f32_32x32x16_{bf16,f16}: the 16-bit forms of differ_query_grad_kernel and
-// differ_key_grad_kernel.  The weights' difference and the scores' gradients go into their products in two pieces of 16 bits each.  dq takes D from the rounded o and second; on the way it finds D again as the sum of weights times dP, in f32, which the gradients of weights and keys take:
+// differ_key_grad_kernel.  The weights' difference and the scores' gradients go into their products in two pieces of 16 bits each.  dq takes D from
+// the rounded o and second, but where keys are few (kTwice); on the way it finds D again as the sum of weights times dP, in f32, which the gradients of weights and keys take:
 // a row that sees one key has a scores' gradient of zero, and what rounding makes of it would reach dk.
 //
 // f16 does not hold the scores' gradients as they are: weights far below one times differences of any size.  What a lane rounds is all of one column of the
@@ -68,7 +69,7 @@ struct Lift {
 
 // acc[d] += the product over 32 rows, from `first` on, of a tile of rows of DP values with p in two pieces.  (The scores' gradients
 // cancel: of rounded ones alone dq and dk are up to 1.6 times as far off as their own rounding, 0.0026 for 0.0017 in bf16.  The gradients of 2 x 4096 x 4096, 16 / 4 heads of 64,
-// causal, take 862 us, with rounded ones alone 710.)
+// causal, take 874 us, with rounded ones alone 710.)
 template <typename T, int DP>
 __device__ __forceinline__ void over_rows(unsigned tile, int first, const float16_t& p, float16_t (&acc)[DP / 32]) {
 #pragma unroll
@@ -154,49 +155,60 @@ __global__ __launch_bounds__(64 * kWaves<CH>, kWaves<CH> / 4) void differ_query_
     counts = key_word(a, b, t * KEYS + lane, n);
   };
   int buffer = 0;
-  if (t0 < t1) fetch(t0, 0);
-  for (int t = t0; t < t1; ++t, buffer ^= 1) {
-    const uint64_t valid = __ballot(counts != 0);
-    const unsigned stage = lds_at + buffer * (2 * Load::VALUES);
-    wait_vm_lds<0>();
-    block_barrier();
-    if (t + 1 < t1) fetch(t + 1, buffer ^ 1);
-    if (idle || t * KEYS >= seen_by_any) continue;
-    if (valid != ~0ull) {   // the maps' keys, which a gradient of zero meets
-      zero_rows<T, DP, KEYS>(lds + buffer * Load::VALUES, valid, lane);
-      zero_rows<T, DP, KEYS>(lds + buffer * Load::VALUES + Load::MAP, valid, lane);
-    }
-    const bool masked = valid != ~0ull || (t + 1) * KEYS > seen_by_all;
 #pragma unroll 1
-    for (int k = 0; k < KEYS / 32; ++k) {
-      const unsigned map_k = stage + k * (64 * DP), ks_at = hide(map_k + rows_at), vs_at = hide(stage + k * (64 * W) + wide_at), kc_at = hide(map_k + columns_at);
-      float16_t dp[1], s[2][1];
-      over_chunks<T, W, 2 * CH, 1, 4>(vs_at, 0, [&](int c) { return gf[c]; }, dp);
-      const uint32_t word = ((uint32_t)(valid >> (32 * k)) & first_bits(seen - t * KEYS - 32 * k)) >> (4 * h);
-      if (masked)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) dp[0][i] = word >> product_row(i, 0) & 1 ? dp[0][i] : 0.0f;
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        over_chunks<T, DP, CH, 1, 4>(ks_at + m * (2 * Load::MAP), 0, [&](int c) { return qf[m][c]; }, s[m]);
-        const float by = m ? -w : 1.0f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[m][0][i] = exp2_(s[m][0][i] * unit - offset[m]);
+  for (int sweep = tiles * KEYS <= kTwice ? 0 : 1; sweep < 2; ++sweep) {   // the first one, if any, for D alone, of all splits' keys
+    const int first_tile = sweep ? t0 : 0, end = sweep ? t1 : tiles;
+    if (first_tile < end) fetch(first_tile, buffer);   // (where the tile before the last one was)
+    for (int t = first_tile; t < end; ++t, buffer ^= 1) {
+      const uint64_t valid = __ballot(counts != 0);
+      const unsigned stage = lds_at + buffer * (2 * Load::VALUES);
+      wait_vm_lds<0>();
+      block_barrier();
+      if (t + 1 < end) fetch(t + 1, buffer ^ 1);
+      if (idle || t * KEYS >= seen_by_any) continue;
+      if (valid != ~0ull) {   // the maps' keys, which a gradient of zero meets
+        zero_rows<T, DP, KEYS>(lds + buffer * Load::VALUES, valid, lane);
+        zero_rows<T, DP, KEYS>(lds + buffer * Load::VALUES + Load::MAP, valid, lane);
+      }
+      const bool masked = valid != ~0ull || (t + 1) * KEYS > seen_by_all;
+#pragma unroll 1
+      for (int k = 0; k < KEYS / 32; ++k) {
+        const unsigned map_k = stage + k * (64 * DP), ks_at = hide(map_k + rows_at), vs_at = hide(stage + k * (64 * W) + wide_at), kc_at = hide(map_k + columns_at);
+        float16_t dp[1], s[2][1];
+        over_chunks<T, W, 2 * CH, 1, 4>(vs_at, 0, [&](int c) { return gf[c]; }, dp);
+        const uint32_t word = ((uint32_t)(valid >> (32 * k)) & first_bits(seen - t * KEYS - 32 * k)) >> (4 * h);
         if (masked)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) s[m][0][i] = word >> product_row(i, 0) & 1 ? s[m][0][i] : 0.0f;
+          for (int i = 0; i < 16; ++i) dp[0][i] = word >> product_row(i, 0) & 1 ? dp[0][i] : 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          dot[m] += s[m][0][i] * dp[0][i];
-          s[m][0][i] *= by * (dp[0][i] - delta[m]);
+        for (int m = 0; m < 2; ++m) {
+          over_chunks<T, DP, CH, 1, 4>(ks_at + m * (2 * Load::MAP), 0, [&](int c) { return qf[m][c]; }, s[m]);
+          const float by = m ? -w : 1.0f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[m][0][i] = exp2_(s[m][0][i] * unit - offset[m]);
+          if (masked)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[m][0][i] = word >> product_row(i, 0) & 1 ? s[m][0][i] : 0.0f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            dot[m] += s[m][0][i] * dp[0][i];
+            s[m][0][i] *= by * (dp[0][i] - delta[m]);
+          }
+          if (sweep == 0) continue;
+          lift[m].raise(s[m][0], dq[m]);
+          over_rows<T, DP>(kc_at + m * (2 * Load::MAP), 0, s[m][0], dq[m]);
         }
-        lift[m].raise(s[m][0], dq[m]);
-        over_rows<T, DP>(kc_at + m * (2 * Load::MAP), 0, s[m][0], dq[m]);
       }
     }
-  }
 #pragma unroll
-  for (int m = 0; m < 2; ++m) dot[m] = sum_of_halves(dot[m]);
+    for (int m = 0; m < 2; ++m) dot[m] = sum_of_halves(dot[m]);
+    if (sweep) break;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      delta[m] = dot[m];
+      dot[m] = 0.0f;
+    }
+  }
   if (!here) return;
 #pragma unroll
   for (int m = 0; m < 2; ++m) {

@@ -131,37 +131,48 @@ __global__ __launch_bounds__(256, CH <= 6 ? 2 : 1) void differ_query_grad_kernel
               a.head, threadIdx.x);
     counts = key_word(a, b, t * R + (lane & 31), n);
   };
-  if (t0 < t1) fetch(t0);
-  for (int t = t0; t < t1; ++t) {
-    __syncthreads();
-    const uint32_t valid = (uint32_t)__ballot(counts != 0);
-    next.store(tile, valid, a.head, threadIdx.x);
-    __syncthreads();
-    if (t + 1 < t1) fetch(t + 1);
-    if (idle) continue;
-    const uint32_t mine = valid & first_bits(seen - t * R);
-    float4_t dp[2];
-    f32_over_head<CH, 2 * CH>(tile + col * LD + 4 * q4 + 32 * CH, gf, dp);
+#pragma unroll 1
+  for (int sweep = kHalves<T> && tiles * R <= kTwice ? 0 : 1; sweep < 2; ++sweep) {   // the first one, if any, for D alone, of all splits' keys
+    const int first_tile = sweep ? t0 : 0, end = sweep ? t1 : tiles;
+    if (first_tile < end) fetch(first_tile);
+    for (int t = first_tile; t < end; ++t) {
+      __syncthreads();
+      const uint32_t valid = (uint32_t)__ballot(counts != 0);
+      next.store(tile, valid, a.head, threadIdx.x);
+      __syncthreads();
+      if (t + 1 < end) fetch(t + 1);
+      if (idle) continue;
+      const uint32_t mine = valid & first_bits(seen - t * R);
+      float4_t dp[2];
+      f32_over_head<CH, 2 * CH>(tile + col * LD + 4 * q4 + 32 * CH, gf, dp);
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        float4_t s[2];
+        f32_over_head<CH, CH>(tile + col * LD + 4 * q4 + m * 16 * CH, qf[m], s);
+        const float by = m ? -w : 1.0f;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool sees = f32_bit(mine, k, i, q4);
+            const float p = exp2_(s[k][i] * unit - offset[m]);
+            if constexpr (kHalves<T>) dot[m] += sees ? p * dp[k][i] : 0.0f;
+            s[k][i] = sees ? by * p * (dp[k][i] - delta[m]) : 0.0f;
+          }
+        if (kHalves<T> && sweep == 0) continue;
+        f32_over_rows<CH, CH>(tile + 4 * q4 * LD + col + m * 16 * CH, s, dq[m]);
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+      if constexpr (kHalves<T>) dot[m] = quarters_sum(dot[m]);
+    if (sweep) break;
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-      float4_t s[2];
-      f32_over_head<CH, CH>(tile + col * LD + 4 * q4 + m * 16 * CH, qf[m], s);
-      const float by = m ? -w : 1.0f;
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool sees = f32_bit(mine, k, i, q4);
-          const float p = exp2_(s[k][i] * unit - offset[m]);
-          if constexpr (kHalves<T>) dot[m] += sees ? p * dp[k][i] : 0.0f;
-          s[k][i] = sees ? by * p * (dp[k][i] - delta[m]) : 0.0f;
-        }
-      f32_over_rows<CH, CH>(tile + 4 * q4 * LD + col + m * 16 * CH, s, dq[m]);
+      delta[m] = dot[m];
+      dot[m] = 0.0f;
     }
   }
-#pragma unroll
-  for (int m = 0; m < 2; ++m)
-    if constexpr (kHalves<T>) dot[m] = quarters_sum(dot[m]);
   if (!here) return;
   if constexpr (kHalves<T>) {
 #pragma unroll

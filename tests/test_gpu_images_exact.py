@@ -81,7 +81,7 @@ def test_results_are_rounded_once_in_whatever_order_the_keys_lie(size, dtype):
 
 
 def exact_gradients(do, q, k, v, w, o, second, **kw):
-    """(dq, dk, dv, dweights) in f64, dq with D from the o and second of the call, as the operator has it; and what dweights may be off by: sums in f32."""
+    """(dq, dk, dv, dweights) in f64, of more than 256 keys dq with D from the o and second of the call, as the operator has it; and what dweights may be off by: sums in f32."""
     scale, group = q.shape[3] ** -0.5, q.shape[2] // k.shape[2]
     _, dk, dv, dw = io.differ_grad(do, q, k, v, w, **kw)
     c = io.seen(q, k, kw.get("key_lengths"), kw.get("key_mask"), kw.get("causal", False))
@@ -89,7 +89,7 @@ def exact_gradients(do, q, k, v, w, o, second, **kw):
     g = torch.where(c.any(2)[:, None, :, None], do.double().permute(0, 2, 1, 3), 0.0).contiguous()
     dp, share = io._matmul(g, vh), w.double()[None, :, None, None]
     rows = lambda x: (g * x.double().permute(0, 2, 1, 3)).sum(-1, keepdim=True)  # noqa: E731
-    deltas = [rows(o) + share * rows(second), rows(second)]
+    deltas = [rows(o) + share * rows(second), rows(second)] if k.shape[1] > 256 else [(io._softmax(*m, c, scale)[0] * dp).sum(-1, keepdim=True) for m in maps]
     dq = [torch.matmul((-share if m else 1.0) * io._softmax(qm, km, c, scale)[0] * (dp - deltas[m]) * scale, km) for m, (qm, km) in enumerate(maps)]
     size = (io._softmax(*maps[1], c, scale)[0] * io._matmul(g.abs(), vh.abs())).sum((0, 2, 3))
     return io._by_map(*dq), dk, dv, dw, (k.shape[1] + 2 * q.shape[3] + 100) * po.U32 * size
@@ -210,3 +210,37 @@ def test_a_row_that_sees_one_key_has_no_gradient_for_it(dtype):
         by = torch.stack([torch.ones(4, device="cuda"), w.abs() + 0], 1).flatten().double() + w.abs().double().max()   # (the first map's D is formed from o and second)
         bound = ((size * by * off * dp)[..., None] * qa).sum(1).view(2, 2, 2, 2, d).sum(2).reshape(2, 4, d)
         assert (dk[:, 0].double().abs() <= bound + po.TINY[dtype]).all(), (lq, lk, d)
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize("size", [(64, 16, 64), (200, 30, 40), (1, 130, 128), (300, 256, 64), (250, 256, 96), (300, 250, 60), (40, 3, 33), (150, 200, 128)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_gradients_of_queries_with_few_keys_are_rounded_once(size, dtype):
+    """D is that of the weights, not of the o and second that were rounded to 16 bits."""
+    import nnv_amd as nnv
+    lq, lk, d = size
+    for causal in (False, True):
+        g = gen(sum(size))
+        q, k, v, w = lopsided(g, 2, lq, lk, 4, 2, d, dtype, 2)
+        lengths = torch.tensor([lk, lk // 2 + 1], dtype=torch.int32, device="cuda")
+        mask = torch.rand(2, lk, generator=g, device="cuda") < 0.9
+        for kw in ({}, {"key_lengths": lengths}, {"key_mask": mask}):
+            o, lse, second = nnv.differential_attention(q, k, v, w, for_backward=True, causal=causal, **kw)
+            do = rand(g, *o.shape, dtype=dtype)
+            exact = io.differ_grad(do, q, k, v, w, causal=causal, **kw)
+            for name, got, e in zip(("dq", "dk", "dv"), nnv.differential_attention_backward(do, q, k, v, w, o, lse, second, causal=causal, **kw), exact):
+                assert_rounded_once(got, e, "%s %s" % (name, causal))
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=IDS[1:])
+def test_early_rows_of_a_causal_call_are_rounded_once(dtype):
+    """Those whose block sees 256 keys: blocks of 256 rows for heads of 64, of 128 above."""
+    import nnv_amd as nnv
+    for n, d, first in ((700, 64, 256), (600, 128, 256)):
+        g = gen(n)
+        q, k, v, w = make_differ(g, 2, n, n, 2, 2, d, dtype)
+        o, lse, second = nnv.differential_attention(q, k, v, w, for_backward=True, causal=True)
+        do = rand(g, *o.shape, dtype=dtype)
+        dq = nnv.differential_attention_backward(do, q, k, v, w, o, lse, second, causal=True)[0]
+        exact = io.differ_grad(do, q, k, v, w, causal=True)[0]
+        assert_rounded_once(dq[:, :first], exact[:, :first], "%d" % d)
