@@ -242,11 +242,11 @@ __global__ __launch_bounds__(64 * kKeyWaves<CH>, kKeyWaves<CH> / 4) void differ_
   load.init(wave, lane, a.head, a.q.t, a.go.t);
   const T* qp = (const T*)a.q.p + b * a.q.b + 2 * (kv * (int64_t)a.group) * a.q.h;
   const T* gp = (const T*)a.go.p + b * a.go.b + kv * (int64_t)a.group * a.go.h;
-  // the weights' difference is at most 1 + |w|: in f16 of 2^14 (the largest, all bits down to 2^-28)
+  // the weights' difference is at most 1 + |w|: in f16 of 2^14 (the largest, all bits down to 2^-28).  (Without rows there may be no weights, and there is nothing to lift.)
   float wide_up = 1.0f;
   if constexpr (Lift<T>::USED) {
     float most = 0.0f;
-    for (int g = 0; g < a.group; ++g) most = fmaxf(most, fabsf(weight_of<T>(a, kv * a.group + g)));
+    for (int g = 0; g < a.group && a.rows > 0; ++g) most = fmaxf(most, fabsf(weight_of<T>(a, kv * a.group + g)));
     if (most < INFINITY) wide_up = __builtin_amdgcn_ldexpf(1.0f, 14 - __builtin_amdgcn_frexp_expf(1.0f + most));
   }
 #pragma unroll 1

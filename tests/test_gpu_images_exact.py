@@ -244,3 +244,21 @@ def test_early_rows_of_a_causal_call_are_rounded_once(dtype):
         dq = nnv.differential_attention_backward(do, q, k, v, w, o, lse, second, causal=True)[0]
         exact = io.differ_grad(do, q, k, v, w, causal=True)[0]
         assert_rounded_once(dq[:, :first], exact[:, :first], "%d" % d)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_backward_of_no_queries_through_c_reads_no_weights(dtype):
+    """The C call takes NULL for what it has no rows of: the keys' gradients are zero."""
+    from nnv_amd import _lib, images
+    from nnv_amd._lib import context_on
+    ctx = context_on(0)
+    t = TYPES.index(dtype)
+    k, v = torch.ones(2, 40, 4, 64, dtype=dtype, device="cuda"), torch.ones(2, 40, 2, 128, dtype=dtype, device="cuda")
+    dk, dv, dw = torch.full_like(k, 7), torch.full_like(v, 7), torch.full((4,), 7.0, dtype=dtype, device="cuda")
+    d = images._DIFFER.pack(t, t, 2, 0, 40, 4, 2, 64, 0, 0.125, 0, k.data_ptr(), v.data_ptr(), 0, 8 * 64, 64, *k.stride()[:3], *v.stride()[:3], 0, 0, 0, 0, 0, 0, 0, 0, 0,
+                            0, 4 * 128, 128, 0, dk.data_ptr(), dv.data_ptr(), dw.data_ptr())
+    need = images._differ_workspace(ctx.lib, True, False, t, t, 2, 0, 40, 4, 2, 64)
+    work = torch.empty(max(1, need), dtype=torch.uint8, device="cuda")
+    _lib.check(ctx.lib.nnvhip_differential_attention_backward(ctx.handle, d, work.data_ptr(), need, torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    assert (dk == 0).all() and (dv == 0).all() and (dw == 0).all()
