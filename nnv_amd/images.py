@@ -181,7 +181,7 @@ def rotate_positions(x, positions, sections, base=10000.0, shared=False, interle
     ctx, lib, stream = _enter(what, ctx, tensors[0], *tensors[1:], positions)
     first = tensors[0]
     t = _type(what, first)
-    pairs, axes, frequency, axis, _ = _turns(tuple(sections), float(base), bool(shared))
+    pairs, axes, frequency, axis, held = _turns(tuple(sections), float(base), bool(shared))   # held: what the addresses are of
     if first.dim() != 4:
         raise ValueError("%s: tensors are batch x tokens x heads x head, alike but for the number of heads" % what)
     batch, tokens, _, head = first.shape
@@ -210,6 +210,7 @@ def rotate_positions(x, positions, sections, base=10000.0, shared=False, interle
                          *strides, *none, *none, *none)
         check(lib.nnvhip_rotate_positions(ctx.handle, d, stream))
         done += out
+    del held
     return done if several else done[0]
 
 

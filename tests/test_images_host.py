@@ -96,6 +96,34 @@ def test_refusals_of_rotary_positions(no_gpu):
     refused("float32, bfloat16 or float16", call, OnGpu(x.double()), at, [2, 2])
 
 
+def test_frequencies_live_as_long_as_a_call_that_reads_them(no_gpu, monkeypatch):
+    """The library is handed their addresses: other calls, which push them out of the caches meanwhile, must not free them."""
+    import gc
+    import weakref
+
+    from nnv_amd import points
+
+    held, read = [], []
+
+    class Library:
+        @staticmethod
+        def nnvhip_rotate_positions(handle, d, stream):
+            no_gpu._turns.cache_clear()
+            no_gpu._frequencies.cache_clear()
+            gc.collect()
+            read.append([array() is not None for array in held])
+            return 0
+
+    class Context:
+        lib, handle, device = Library, None, 0
+
+    monkeypatch.setattr(points, "context_on", lambda index: Context)
+    held += [weakref.ref(array) for array in no_gpu._frequencies((2, 1), 77.0, False)]
+    x, at = OnGpu(torch.zeros(2, 5, 3, 8)), OnGpu(torch.zeros(5, 2, dtype=torch.int32))
+    no_gpu.rotate_positions([x] * 5, at, [2, 1], base=77.0)
+    assert read == [[True, True]] * 2
+
+
 @built
 def test_workspaces_and_their_refusals():
     from nnv_amd import _lib, images
