@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import operator
 import struct
 from numbers import Integral
 
@@ -152,11 +153,14 @@ def _frequencies(sections, base, shared):
     return (C.c_double * pairs)(*values), (C.c_uint8 * pairs)(*axes)
 
 
+_SECTIONS = "rotate_positions: sections are numbers of pairs, one per axis, %d together at most" % _ROTATE_PAIRS
+
+
 @functools.lru_cache(maxsize=64)
 def _turns(sections, base, shared):
-    """(pairs, axes, addresses of _frequencies, which they belong to) of a call's arguments, or the error."""
-    if not sections or not all(isinstance(n, Integral) and n >= 0 for n in sections) or not 1 <= sum(sections) <= _ROTATE_PAIRS or len(sections) > 255:
-        raise ValueError("rotate_positions: sections are numbers of pairs, one per axis, %d together at most" % _ROTATE_PAIRS)
+    """(pairs, axes, addresses of _frequencies, which they belong to) of a call's arguments, or the error.  sections: ints (a cache takes 2.0 for 2)."""
+    if not sections or min(sections) < 0 or not 1 <= sum(sections) <= _ROTATE_PAIRS or len(sections) > 255:
+        raise ValueError(_SECTIONS)
     if not 0 < base < float("inf"):
         raise ValueError("rotate_positions: the base must be positive and finite")
     held = _frequencies(sections, base, shared)
@@ -181,7 +185,11 @@ def rotate_positions(x, positions, sections, base=10000.0, shared=False, interle
     ctx, lib, stream = _enter(what, ctx, tensors[0], *tensors[1:], positions)
     first = tensors[0]
     t = _type(what, first)
-    pairs, axes, frequency, axis, held = _turns(tuple(sections), float(base), bool(shared))   # held: what the addresses are of
+    try:
+        sections = tuple(map(operator.index, sections))
+    except TypeError:
+        raise ValueError(_SECTIONS) from None
+    pairs, axes, frequency, axis, held = _turns(sections, float(base), bool(shared))   # held: what the addresses are of
     if first.dim() != 4:
         raise ValueError("%s: tensors are batch x tokens x heads x head, alike but for the number of heads" % what)
     batch, tokens, _, head = first.shape

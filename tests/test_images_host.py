@@ -4,6 +4,7 @@ import ctypes as C
 import math
 import os
 
+import numpy as np
 import pytest
 import torch
 
@@ -94,6 +95,14 @@ def test_refusals_of_rotary_positions(no_gpu):
                 torch.zeros(5, 2, dtype=torch.float64), torch.zeros(2, dtype=torch.int32)):
         refused("positions", call, x, OnGpu(bad), [2, 2])
     refused("float32, bfloat16 or float16", call, OnGpu(x.double()), at, [2, 2])
+
+
+def test_sections_that_are_no_whole_numbers_are_refused_whatever_was_called_before(no_gpu):
+    x, at = OnGpu(torch.zeros(2, 5, 3, 8)), OnGpu(torch.zeros(5, 3, dtype=torch.int32))   # (positions of other axes: refused after the sections)
+    for accepted in ([1, 2], (np.int64(1), np.int32(2)), np.array([1, 2])):
+        refused("positions", no_gpu.rotate_positions, x, at, accepted)
+        for sections in ([1.0, 2.0], [1, 2.0], (np.float32(1), 2), [1, None], ["1", 2]):
+            refused("sections", no_gpu.rotate_positions, x, at, sections)
 
 
 def test_frequencies_live_as_long_as_a_call_that_reads_them(no_gpu, monkeypatch):
