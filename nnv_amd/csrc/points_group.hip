@@ -10,9 +10,9 @@
 // atomics, the same inputs give the same bits) and reads again what the caches may still hold.
 //
 // There a block takes a part of the places of a chunk of channels: whole groups, or a part of a wide one.  Its threads are (pack of
-// 16 bytes of channels) x (places): rows are read as they lie in memory, whatever the groups are.  The sums of x and x^2 are f64:
-// the memory's rate asks for some 1e13 f64 operations a second, a quarter of what the f64 pipes give, and a mean far from zero then
-// costs the variance nothing.
+// 16 bytes of channels) x (places): rows are read as they lie in memory, whatever the groups are.  The sums are f64, which the memory's
+// rate asks some 1e13 operations a second of, a third of what the f64 pipes give, and they are of x - c and (x - c)^2, c the group's first value: a mean far from zero costs the variance
+// nothing, for the variance is no less than a share of (c - mean)^2, and that of equal values is zero.
 //
 // 16 x 64 x 64 x 320 in bf16: 26 us forward (3.2 TB/s: a block reads all it has before it writes, and one fits a CU), 54 backward (24 + 28 us a kernel: x and dy are read
 // twice, the second time partly from the caches); 5 x 53 x 79 x 96 in f32 backward 17; 4 x 8 x 8 x 256 forward 5.5 us, a launch and one latency of memory.
@@ -134,21 +134,30 @@ __device__ __forceinline__ void over_places(const T* const (&at)[N], const int64
   }
 }
 
+// what a group's values are counted from: its first one, or zero where that is not finite
+template <typename T>
+__device__ __forceinline__ float origin_of(const GroupArgs& a, int n, int group) {
+  const float x = to_f(((const T*)a.x)[n * a.x_b + (int64_t)group * a.each]);
+  return fabsf(x) < INFINITY ? x : 0.0f;
+}
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void group_sums_kernel(const GroupArgs a) {
   constexpr int V = kVec<T>;
   __shared__ double lds[2][kThreads * V];
   const Chunk c = chunk_of(a, blockIdx.x);
   const int packs = (c.size + V - 1) / V, rows = kThreads / packs, tx = threadIdx.x % packs, ty = threadIdx.x / packs;
-  double s[V] = {}, q[V] = {};
+  double s[V] = {}, q[V] = {}, from[V];
   if (ty < rows) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) from[i] = (double)origin_of<T>(a, c.n, (c.first + min(tx * V + i, c.size - 1)) / a.each);
     const T* const at[1] = {(const T*)a.x + c.n * a.x_b + c.first + tx * V};
     const int64_t stride[1] = {a.x_p};
     const int64_t p0 = c.split * a.per, p1 = min(a.places, p0 + a.per);
     over_places<T, 1>(at, stride, p0, p1, ty, rows, c.size - tx * V, [&](int64_t, const Pack<T>(&p)[1]) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const double x = (double)to_f(p[0][i]);
+        const double x = (double)to_f(p[0][i]) - from[i];
         s[i] += x;
         q[i] = fma(x, x, q[i]);
       }
@@ -194,6 +203,7 @@ __device__ __forceinline__ float activate(float z) {
 }
 
 // Where a group's sums over the parts end up: mean and rstd of the chunk's groups.
+template <typename T>
 __device__ __forceinline__ void statistics(const GroupArgs& a, const Chunk& c, float* mean, float* rstd) {
   const int parts = a.splits * a.per_group;
   const double inv = 1.0 / ((double)a.places * a.each);
@@ -203,7 +213,7 @@ __device__ __forceinline__ void statistics(const GroupArgs& a, const Chunk& c, f
     v[1] = from[((int64_t)e * a.groups + j) * 2 + 1];
   }, [&](int j, const double(&v)[2]) {
     const double m = v[0] * inv, var = v[1] * inv - m * m;
-    mean[j] = (float)m;
+    mean[j] = (float)((double)origin_of<T>(a, c.n, c.group + j) + m);
     rstd[j] = (float)(1.0 / sqrt((var < 0 ? 0.0 : var) + (double)a.eps));   // (NaN stays)
     if (c.split == 0 && c.sub == 0) {
       a.mean[(int64_t)c.n * a.groups + c.group + j] = mean[j];
@@ -218,7 +228,7 @@ __global__ __launch_bounds__(kThreads) void group_apply_kernel(const GroupArgs a
   constexpr int V = kVec<T>;
   __shared__ float mean[kWide], rstd[kWide];
   const Chunk c = chunk_of(a, gridDim.x - 1 - blockIdx.x);   // what was read last is in the caches
-  statistics(a, c, mean, rstd);
+  statistics<T>(a, c, mean, rstd);
   const int packs = (c.size + V - 1) / V, rows = kThreads / packs, tx = threadIdx.x % packs, ty = threadIdx.x / packs, left = c.size - tx * V;
   if (ty >= rows) return;
   float mu[V], times[V], plus[V];
@@ -524,9 +534,10 @@ __global__ __launch_bounds__(1024) void group_resident_kernel(const GroupArgs a,
   Quad<T> in[NP];
 #pragma unroll
   for (int k = 0; k < NP; ++k) in[k].load(x + min(c.ty + k * c.rows, places - 1) * a.x_p);
-  float w[kFour], b[kFour], mu[kFour];
+  float w[kFour], b[kFour], mu[kFour], from[kFour];
 #pragma unroll
   for (int i = 0; i < kFour; ++i) {
+    from[i] = origin_of<T>(a, c.n, (c.first + c.tx * kFour + i) / a.each);
     w[i] = param<T>(a, a.scale, c.first + c.tx * kFour + i, 1.0f);
     b[i] = param<T>(a, a.offset, c.first + c.tx * kFour + i, 0.0f);
   }
@@ -536,7 +547,7 @@ __global__ __launch_bounds__(1024) void group_resident_kernel(const GroupArgs a,
     if (on && c.ty + k * c.rows < places)
 #pragma unroll
       for (int i = 0; i < kFour; ++i) {
-        const double v = (double)in[k][i];
+        const double v = (double)in[k][i] - (double)from[i];
         s[i] += v;
         q[i] = fma(v, v, q[i]);
       }
@@ -544,7 +555,7 @@ __global__ __launch_bounds__(1024) void group_resident_kernel(const GroupArgs a,
   const double inv = 1.0 / ((double)a.places * a.each);
   const int groups = a.width / a.each;
   for (int j = threadIdx.x; j < groups; j += blockDim.x) {
-    const double m = sums[j][0] * inv, var = sums[j][1] * inv - m * m;
+    const double off = sums[j][0] * inv, var = sums[j][1] * inv - off * off, m = (double)origin_of<T>(a, c.n, c.first / a.each + j) + off;
     const int64_t g = (int64_t)c.n * a.groups + c.first / a.each + j;
     a.mean[g] = (float)m;
     a.rstd[g] = (float)(1.0 / sqrt((var < 0 ? 0.0 : var) + (double)a.eps));   // (NaN stays)

@@ -262,3 +262,47 @@ def test_backward_of_no_queries_through_c_reads_no_weights(dtype):
     _lib.check(ctx.lib.nnvhip_differential_attention_backward(ctx.handle, d, work.data_ptr(), need, torch.cuda.current_stream().cuda_stream))
     torch.cuda.synchronize()
     assert (dk == 0).all() and (dv == 0).all() and (dw == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("places", [1, 40, 300, 70001], ids=str)
+def test_group_norm_of_a_mean_far_from_zero(places, dtype):
+    """Groups of equal values have no spread whatever the values are, and of a small spread the variance keeps its bits: sums in f64 of differences from a value of the group, which lose
+    less than 2^-53 n of a variance of n values."""
+    import nnv_amd as nnv
+    for channels, groups in ((16, 4), (40, 8), (6, 3), (1030, 2)):
+        if places * channels > 1 << 22:
+            continue
+        b = torch.arange(float(channels), device="cuda") - 8
+        for value in (1000.1, 10000.3, -60000.7, 7.1e-3):
+            x = torch.full((2, places, channels), value, device="cuda").to(dtype)
+            y, mean, rstd = nnv.group_norm(x, groups, None, b, 1e-5)
+            assert (mean == x[0, 0, 0].float()).all() and torch.equal(y.float(), b.to(dtype).float().expand(2, places, channels))
+            assert ((rstd.double() * 1e-5 ** 0.5 - 1).abs() <= 2 * po.U32).all()      # (its own rounding, and that of epsilon)
+        # f32 values next to one another around a far mean; one that lies far from the others, in front and behind
+        if dtype == F32 and places > 1:
+            g = gen(places)
+            far = torch.tensor([1000.0, -30000.0], device="cuda")[:, None, None] + torch.randint(0, 9, (2, places, channels), generator=g, device="cuda") / 512
+            out = far.clone()
+            out[0, 0, 0], out[1, -1, -1] = 3e7, -1e30
+            for x in (far, out):
+                _, mean, rstd = nnv.group_norm(x, groups, None, None, 1e-5)
+                _, e_mean, e_rstd = io.group(x, groups, None, None, 1e-5, None)
+                n = places * channels // groups
+                assert ((mean.double() - e_mean).abs() <= 1.01 * po.U32 * e_mean.abs()).all()
+                assert ((rstd.double() / e_rstd - 1).abs() <= (1.5 + n * 2.0 ** -27) * po.U32 * 1.0).all()
+
+
+def test_group_norm_whose_first_value_is_infinite():
+    """Its mean is infinite, as that of any group with such a value, and the other groups know nothing of it."""
+    import nnv_amd as nnv
+    for places in (40, 5000):
+        x = rand(gen(places), 2, places, 16, shift=100.0)
+        clean = x.clone()
+        x[0, 0, 4], x[1, 0, 8] = math.inf, math.nan
+        y, mean, _ = nnv.group_norm(x, 4)
+        e, e_mean, _ = nnv.group_norm(clean, 4)
+        assert mean[0, 1] == math.inf and mean[1, 2].isnan() and y[0, :, 4:8].isnan().all() and y[1, :, 8:12].isnan().all()
+        for n, hit in ((0, 1), (1, 2)):
+            others = [j for j in range(4) if j != hit]
+            assert torch.equal(mean[n, others], e_mean[n, others]) and all(torch.equal(y[n, :, 4 * j:4 * j + 4], e[n, :, 4 * j:4 * j + 4]) for j in others)
