@@ -536,11 +536,7 @@ __global__ __launch_bounds__(1024) void group_resident_kernel(const GroupArgs a,
   for (int k = 0; k < NP; ++k) in[k].load(x + min(c.ty + k * c.rows, places - 1) * a.x_p);
   float w[kFour], b[kFour], mu[kFour], from[kFour];
 #pragma unroll
-  for (int i = 0; i < kFour; ++i) {
-    from[i] = origin_of<T>(a, c.n, (c.first + c.tx * kFour + i) / a.each);
-    w[i] = param<T>(a, a.scale, c.first + c.tx * kFour + i, 1.0f);
-    b[i] = param<T>(a, a.offset, c.first + c.tx * kFour + i, 0.0f);
-  }
+  for (int i = 0; i < kFour; ++i) from[i] = origin_of<T>(a, c.n, (c.first + c.tx * kFour + i) / a.each);
   double s[kFour] = {}, q[kFour] = {};
 #pragma unroll
   for (int k = 0; k < NP; ++k)
@@ -564,11 +560,13 @@ __global__ __launch_bounds__(1024) void group_resident_kernel(const GroupArgs a,
   }
   __syncthreads();
   if (!on) return;
+  // (the parameters are read here: ahead of the sums they take registers that the places need; 16 x 32 x 32 x 640 in bf16: 21.3 us instead of 17.1)
 #pragma unroll
   for (int i = 0; i < kFour; ++i) {
     const int j = (c.tx * kFour + i) / a.each;
     mu[i] = (float)sums[j][0];
-    w[i] *= (float)sums[j][1];
+    w[i] = param<T>(a, a.scale, c.first + c.tx * kFour + i, 1.0f) * (float)sums[j][1];
+    b[i] = param<T>(a, a.offset, c.first + c.tx * kFour + i, 0.0f);
   }
   T* out = (T*)a.out + (c.n * a.places * a.channels + c.first + c.tx * kFour);
   auto write = [&](auto act) {
