@@ -45,7 +45,7 @@ struct GroupArgs {
   int width, chunks, per_group;   // channels of a chunk; chunks of all channels; of a group, where it is wider than a chunk
   int splits, wide_params;        // wide_params: scale and offset are f32
   int resident, threads;          // packs of a thread of the resident form (0: the other one), and its threads
-  float eps;
+  double eps;
 };
 
 struct Chunk {
@@ -214,7 +214,7 @@ __device__ __forceinline__ void statistics(const GroupArgs& a, const Chunk& c, f
   }, [&](int j, const double(&v)[2]) {
     const double m = v[0] * inv, var = v[1] * inv - m * m;
     mean[j] = (float)((double)origin_of<T>(a, c.n, c.group + j) + m);
-    rstd[j] = (float)(1.0 / sqrt((var < 0 ? 0.0 : var) + (double)a.eps));   // (NaN stays)
+    rstd[j] = (float)(1.0 / sqrt((var < 0 ? 0.0 : var) + a.eps));   // (NaN stays)
     if (c.split == 0 && c.sub == 0) {
       a.mean[(int64_t)c.n * a.groups + c.group + j] = mean[j];
       a.rstd[(int64_t)c.n * a.groups + c.group + j] = rstd[j];
@@ -554,7 +554,7 @@ __global__ __launch_bounds__(1024) void group_resident_kernel(const GroupArgs a,
     const double off = sums[j][0] * inv, var = sums[j][1] * inv - off * off, m = (double)origin_of<T>(a, c.n, c.first / a.each + j) + off;
     const int64_t g = (int64_t)c.n * a.groups + c.first / a.each + j;
     a.mean[g] = (float)m;
-    a.rstd[g] = (float)(1.0 / sqrt((var < 0 ? 0.0 : var) + (double)a.eps));   // (NaN stays)
+    a.rstd[g] = (float)(1.0 / sqrt((var < 0 ? 0.0 : var) + a.eps));   // (NaN stays)
     sums[j][0] = m;
     sums[j][1] = (double)a.rstd[g];
   }
@@ -747,7 +747,7 @@ int group_args(const char* what, const nnvhip_group_norm_args* d, bool backward,
   a->mean = d->mean;
   a->rstd = d->rstd;
   a->wide_params = d->param_type == NNVHIP_TYPE_F32;
-  a->eps = (float)d->epsilon;
+  a->eps = d->epsilon;
   return NNVHIP_OK;
 }
 

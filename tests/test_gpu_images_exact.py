@@ -306,3 +306,12 @@ def test_group_norm_whose_first_value_is_infinite():
         for n, hit in ((0, 1), (1, 2)):
             others = [j for j in range(4) if j != hit]
             assert torch.equal(mean[n, others], e_mean[n, others]) and all(torch.equal(y[n, :, 4 * j:4 * j + 4], e[n, :, 4 * j:4 * j + 4]) for j in others)
+
+
+def test_group_norm_takes_epsilon_in_64_bits():
+    """Of equal values rstd is 1 / sqrt(epsilon), also of one that f32 does not hold."""
+    import nnv_amd as nnv
+    for places in (40, 70001):
+        for epsilon in (1e-5, 1.0 / 3, 1e-42, 1e-60):
+            rstd = nnv.group_norm(torch.full((1, places, 8), 3.5, device="cuda"), 2, epsilon=epsilon)[2]
+            assert ((rstd.double() * math.sqrt(epsilon) - 1).abs() <= 1.01 * po.U32).all()
