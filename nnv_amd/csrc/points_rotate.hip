@@ -5,7 +5,7 @@
 //
 // Bound by memory: each value is read and written once.  A block takes the heads of a few tokens and forms the tokens' cosines and
 // sines once, in LDS.  Angles are counted in turns and in f64: position * (frequency / 2 pi), of which the whole turns are dropped, so
-// that far positions lose nothing; what is left goes through sincospif.  (2 x 19200 tokens of 32 heads of 128 in bf16: 122 us, 5.15 TB/s; 16 tokens: 4.3 us,
+// that far positions lose nothing; what is left goes through sincospif, rounded to f32, and what that rounding leaves turns the result by as much.  (2 x 19200 tokens of 32 heads of 128 in bf16: 122 us, 5.15 TB/s; 16 tokens: 4.3 us,
 // of which the launch is most; 3 x 1577 tokens of 24 heads of 80 in f32: 17 us among other calls, 4.2 TB/s.)
 #include "points.h"
 
@@ -54,11 +54,12 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(const RotateArgs a) {
   const int here = (int)min((int64_t)a.per_block, a.all - token0), slice = blockIdx.x % a.slices;
   for (int e = threadIdx.x; e < here * a.pairs; e += kThreads) {
     const int k = e / a.pairs, i = e - k * a.pairs;
-    const double turns = position(a, token0 + k, a.axis[i]) * a.turns[i], left = turns - rint(turns);
+    const double turns = position(a, token0 + k, a.axis[i]) * a.turns[i], left = 2.0 * (turns - rint(turns));
+    const float half = (float)left, rest = (float)(left - (double)half) * 3.14159265f;
     float s, c;
-    sincospif(2.0f * (float)left, &s, &c);
-    cosines[e] = c;
-    sines[e] = s * a.sign;
+    sincospif(half, &s, &c);
+    cosines[e] = c - s * rest;
+    sines[e] = (s + c * rest) * a.sign;
   }
   __syncthreads();
   const int total = a.first[a.tensors], work = here * total;

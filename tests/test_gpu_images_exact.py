@@ -315,3 +315,30 @@ def test_group_norm_takes_epsilon_in_64_bits():
         for epsilon in (1e-5, 1.0 / 3, 1e-42, 1e-60):
             rstd = nnv.group_norm(torch.full((1, places, 8), 3.5, device="cuda"), 2, epsilon=epsilon)[2]
             assert ((rstd.double() * math.sqrt(epsilon) - 1).abs() <= 1.01 * po.U32).all()
+
+
+def test_rotary_positions_keep_the_bits_of_the_angle():
+    """Next to multiples of a quarter turn a sine or cosine is as small as what is left of the angle there, and has its bits: a few units in the last place, and of the angle 2^-53 of the whole one."""
+    import nnv_amd as nnv
+    at = torch.tensor([3, 11, 14, 22, 33, 44, 355, 710, 1065, 52174, 208341, 312689, 0, 1, 2, 100], device="cuda")
+    for interleaved in (False, True):
+        for inverse in (False, True):
+            x = torch.zeros(1, len(at), 1, 2, device="cuda")
+            x[..., 0] = 1.0
+            y = nnv.rotate_positions(x, at[:, None], [1], interleaved=interleaved, inverse=inverse)[0, :, 0].double()
+            angle = at.double() * (-1 if inverse else 1)
+            exact = torch.stack([torch.cos(angle), torch.sin(angle)], 1)
+            assert ((y - exact).abs() <= 8 * po.U32 * exact.abs() + (8 * at.double() * 2.0 ** -53)[:, None]).all()
+
+
+def test_rotary_positions_in_f32_are_as_far_off_as_rounded_cosines():
+    """No further than products and sums in f32 with cosines and sines that were rounded once, but for a tenth."""
+    import nnv_amd as nnv
+    g = gen(3)
+    x = rand(g, 2, 3000, 4, 64)
+    at = torch.randint(0, 5000, (3000, 2), generator=g, device="cuda")
+    y, exact = nnv.rotate_positions(x, at, [16, 16]), io.rotate(x, at, [16, 16])
+    angle = torch.cat([at[:, a, None].double() * 10000.0 ** -(torch.arange(16, device="cuda", dtype=torch.float64) / 16) for a in (0, 1)], 1)[None, :, None]
+    c, s, u, w = torch.cos(angle).float(), torch.sin(angle).float(), x[..., :32], x[..., 32:]
+    plain = torch.cat([u * c - w * s, u * s + w * c], -1)
+    assert off(y, exact) <= 1.1 * off(plain, exact)
