@@ -301,7 +301,7 @@ def differential_attention(q, k, v, weights, key_lengths=None, key_mask=None, ca
 def differential_attention_backward(do, q, k, v, weights, o, lse, second, key_lengths=None, key_mask=None, causal=False, scale=None, ctx=None):
     """The gradients (dq, dk, dv, dweights) of differential_attention, from that of o and from what the forward call (with for_backward)
     returned; the other arguments are that call's.  Rows that see no key and keys that do not count get zero.  A value of q or do that is not finite reaches the
-    gradients of all keys that count (causal as well: zero weights are multiplied with it).  dweights has the type of weights."""
+    gradients of all keys that count, and causal one of k those of queries that do not see it (zero weights are multiplied with them).  dweights has the type of weights."""
     what = "differential_attention_backward"
     ctx, lib, stream = _enter(what, ctx, q, k, v, weights, key_lengths, key_mask, do, o, lse, second)
     sizes = _differ_sizes(what, q, k, v, weights, key_lengths, key_mask, scale)

@@ -342,3 +342,56 @@ def test_rotary_positions_in_f32_are_as_far_off_as_rounded_cosines():
     c, s, u, w = torch.cos(angle).float(), torch.sin(angle).float(), x[..., :32], x[..., 32:]
     plain = torch.cat([u * c - w * s, u * s + w * c], -1)
     assert off(y, exact) <= 1.1 * off(plain, exact)
+
+
+# Causal calls whose blocks take two tiles of keys, an early and a late one (six tiles or more: of 256 keys in 16 bits, 128 for heads above 64, of 64 in f32), an even and an odd number of them
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("size", [(800, 1400, 64, 6), (800, 1600, 40, 7), (400, 700, 128, 6), (450, 850, 96, 7), (250, 420, 64, 0), (200, 380, 33, 0)], ids=lambda s: "x".join(map(str, s[:3])))
+def test_gradients_of_keys_in_paired_tiles(size, dtype):
+    lq, lk, d, tiles = size
+    assert dtype == F32 or tiles == 0 or -(-lk // (256 if d <= 64 else 128)) == tiles
+    assert dtype != F32 or tiles or -(-lk // 64) in (6, 7)
+    g = gen(lk)
+    q, k, v, w = make_differ(g, 2, lq, lk, 2, 1, d, dtype)
+    check_differ(q, k, v, w, causal=True, tag="all")
+    lengths = torch.tensor([lk - 70, lq // 2 + 3], dtype=torch.int32, device="cuda")      # (the second one shorter than the queries: its first rows see no key)
+    mask = torch.rand(2, lk, generator=g, device="cuda") < 0.9
+    clean = (k.clone(), v.clone())
+    for i, n in enumerate(lengths.tolist()):
+        k[i, n:], v[i, n:] = math.nan, math.inf
+    check_differ(q, k, v, w, clean, causal=True, key_lengths=lengths, tag="lengths")
+    check_differ(q, k, v, w, clean, causal=True, key_lengths=lengths, key_mask=mask, tag="lengths, mask")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("size", [(16, 40, 4500, 16, 16, 64), (64, 1, 20000, 8, 4, 32), (32, 2, 9000, 8, 8, 128)], ids=lambda s: "x".join(map(str, s)))
+def test_masks_of_many_tiles(size, dtype):
+    """More tiles in a row than a mask is read for at a time (32, of 64 keys, or of 32 that eight or two groups of waves take in turn), with no period, and what is left out far behind holds anything."""
+    import nnv_amd as nnv
+    from nnv_amd import _lib, images
+    b, lq, lk, h, hkv, d = size
+    lib = _lib.load()
+    t = TYPES.index(dtype)
+    need = images._differ_workspace(lib, False, False, t, 0, *size)
+    splits = max(1, need // (b * h * 2 * lq * (2 * d + 1) * 4))
+    assert lk // (64 if lq > 16 else 32 * {32: 8, 128: 2}[d]) // splits > 32
+    g = gen(lk)
+    q, k, v, w = make_differ(g, *size, dtype)
+    mask = torch.rand(b, lk, generator=g, device="cuda") < 0.7
+    mask[:, lk // 2:] &= torch.rand(b, lk - lk // 2, generator=g, device="cuda") < 0.5
+    clean = (k.clone(), v.clone())
+    k[~mask], v[~mask] = math.nan, math.inf
+    for causal in (False, True):
+        o, lse, second = nnv.differential_attention(q, k, v, w, key_mask=mask, causal=causal, for_backward=True)
+        kw = {"key_mask": mask, "causal": causal}
+        for i in range(0, b, 8):      # (some sequences at a time: the 64-bit forms are large)
+            part = [x[i:i + 8] for x in (q, *clean)] + [w]
+            at = {"key_mask": mask[i:i + 8], "causal": causal}
+            for name, got, e, bd in zip(("o", "lse", "second"), (o, lse, second), io.differ(*part, **at), io.differ_bounds(*part, **at)):
+                po.assert_within(got[i:i + 8], e, bd, "%s %s" % (name, causal))
+        if lq > 16:
+            do = rand(g, *o.shape, dtype=dtype)
+            grads = nnv.differential_attention_backward(do, q, k, v, w, o, lse, second, **kw)
+            exact, bounds = (f(do[:2], q[:2], clean[0][:2], clean[1][:2], w, key_mask=mask[:2], causal=causal) for f in (io.differ_grad, io.differ_grad_bounds))
+            for name, got, e, bd in zip(("dq", "dk", "dv"), grads, exact, bounds):
+                po.assert_within(got[:2], e, bd, "%s %s" % (name, causal))
