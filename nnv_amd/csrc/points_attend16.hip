@@ -6,27 +6,6 @@
 namespace nnvhip {
 namespace {
 
-// The weights of the softmax are multiples of exp(score - the largest score): in f16 of 2^7, so that what is rounded to T keeps weights down to 2^-32 of the
-// largest (2^-25 without; a million keys of 2^-26 would be lost), and the largest, which the offset may lag behind by 2^8, stays in f16's range.  (A weight that is rounded to zero gives NaN with an infinite value.)
-template <typename T>
-constexpr float kLift = std::is_same_v<T, f16_t> ? 7.0f : 0.0f;
-
-// Exponents are score * unit - off in one rounding, off a rounded score * unit: where a rounding is more than a fraction of an exponent, the two do not
-// fit together, and a weight may leave the range of its type.  From there on the products are rounded as off is (round_scores), and off is that of the largest,
-// not lower by kLift, which might be less than half a place.
-constexpr float kFar = 4194304.0f;   // 2^22: places of 1/2
-template <typename T>
-__device__ __forceinline__ float lowered(float top) {
-  return fabsf(top) > kFar ? top : top - kLift<T>;
-}
-template <int K>
-__device__ __forceinline__ void round_scores(float16_t (&s)[K], float unit) {
-#pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s[k][i] = rounded(s[k][i] * unit);
-}
-
 // FEW = false (heads of up to 64): four waves take 32 rows each and share tiles of 64 keys.  FEW = true (up to 64 rows, single tokens):
 // 32 rows for the block, whose 8 waves (4 for heads above 64: LDS) are groups that take tiles of 32 keys in turn; what the groups
 // found is joined at the end.  (attend_kernel is the f32 form.)

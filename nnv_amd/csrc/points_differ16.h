@@ -203,6 +203,13 @@ struct KeyWords {
   }
 };
 
+template <typename T, int VALUES, int THREADS>
+__device__ __forceinline__ void zero_lds(T* lds) {
+  half8<T> none = {};
+  for (int e = threadIdx.x; e < VALUES / 8; e += THREADS) __builtin_memcpy(lds + e * 8, &none, 16);
+  __syncthreads();
+}
+
 bool differ16_takes(const DifferArgs& a, int type);
 constexpr int kDiffer16Rows = 128;   // of a block
 constexpr int kDifferFewRows = 16;   // of a block of the form for few rows

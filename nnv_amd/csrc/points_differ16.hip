@@ -1,5 +1,5 @@
 // Differential attention of points in 16 bits, forward, on v_mfma_f32_32x32x16_{bf16,f16}.  What is said of the softmax's weights, their lift
-// in f16 and of scores that are far from zero in points_attend16.hip holds here.
+// in f16 and of scores that are far from zero in points_attend16.h holds here.
 #include "points_differ16.h"
 
 #pragma clang fp contract(fast)
@@ -7,20 +7,6 @@
 namespace nnvhip {
 namespace {
 
-template <typename T>
-constexpr float kLift = std::is_same_v<T, f16_t> ? 7.0f : 0.0f;
-constexpr float kFar = 4194304.0f;   // 2^22: places of 1/2
-template <typename T>
-__device__ __forceinline__ float lowered(float top) {
-  return fabsf(top) > kFar ? top : top - kLift<T>;
-}
-template <int K>
-__device__ __forceinline__ void round_scores(float16_t (&s)[K], float unit) {
-#pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s[k][i] = rounded(s[k][i] * unit);
-}
 // A tile's scores (of a lane's row, masked) to weights: raises the running maximum where it has grown by more than 2^8; returns what the sums so far are
 // to be multiplied with (1 mostly).
 template <typename T, int K>
@@ -66,12 +52,6 @@ __device__ __forceinline__ void query_operands(half8<T> (&f)[CH], const T* q, in
     if (here && 16 * c + 8 * h < head) __builtin_memcpy(&f[c], q + 16 * c + 8 * h, 16);
     if (scale < 0) f[c] = -f[c];
   }
-}
-template <typename T, int VALUES, int THREADS>
-__device__ __forceinline__ void zero_lds(T* lds) {
-  half8<T> none = {};
-  for (int e = threadIdx.x; e < VALUES / 8; e += THREADS) __builtin_memcpy(lds + e * 8, &none, 16);
-  __syncthreads();
 }
 
 // Many rows: a wave takes 32 rows of one map, eight waves share tiles of 64 keys: four groups of rows, both maps, whose two waves are of one SIMD.  Tiles are

@@ -94,12 +94,6 @@ __device__ __forceinline__ void store_result(T* row, const float16_t (&acc)[N], 
       put_four(row, d * 32 + 8 * i4 + 4 * h, size, f);
     }
 }
-template <typename T, int VALUES, int THREADS>
-__device__ __forceinline__ void zero_lds(T* lds) {
-  half8<T> none = {};
-  for (int e = threadIdx.x; e < VALUES / 8; e += THREADS) __builtin_memcpy(lds + e * 8, &none, 16);
-  __syncthreads();
-}
 
 // Heads of up to 64: eight waves, two a SIMD; above, four with all of a SIMD's registers.
 template <int CH>
