@@ -32,7 +32,7 @@ enum RowInfo { kOffset0, kOffset1, kDelta0, kDelta1, kWeight, kSees, kInfos };
 constexpr int kInfoRows = 64;
 // Of 16-bit tensors, whose o and second are rounded, D of a block of rows that see up to so many keys is found by going through the keys twice: what D of rounded values leaves in dq is large
 // where keys are few (in bf16 a causal call of 64 x 16 has dq 1.4 times as far off as its rounding, 1000 x 1000 1.07, not causal 1.01), and for long rows going twice would take
-// the gradients of 4096 x 4096, 16 heads of 64, 1081 us instead of 874.
+// the gradients of 4096 x 4096, 16 heads of 64, 1081 us instead of 865.
 constexpr int kTwice = 256;
 __device__ __forceinline__ float* info_at(const DifferArgs& a, int64_t bkv, int64_t r, int which) { return a.info + (bkv * kInfos + which) * a.info_rows + r; }
 

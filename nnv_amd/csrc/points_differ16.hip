@@ -56,13 +56,14 @@ __device__ __forceinline__ void query_operands(half8<T> (&f)[CH], const T* q, in
 
 // Many rows: a wave takes 32 rows of one map, eight waves share tiles of 64 keys: four groups of rows, both maps, whose two waves are of one SIMD.  Tiles are
 // on their way to LDS STAGES - 1 ahead; one barrier a tile.  (The two waves of a SIMD taking turns at products and softmax, as attend16_wide_kernel's
-// do: 4096 x 4096, heads of 128, 530 us instead of 471, 577 x 1000, heads of 40, 76 instead of 65: with values twice as wide the products take longer than the
+// do, with rounded weights: 4096 x 4096, heads of 128, 530 us instead of 471, 577 x 1000, heads of 40, 76 instead of 65: with values twice as wide the products take longer than the
 // softmax beside them.)  At the end the second map's result meets the first one's in LDS, lane by lane.
-// (Four stages where they fit and every wave has as many transfers: 2 x 2048 x 2048, 16 heads of 64, 126 us, with two 136.  Else two: heads of 40 as above 64 us,
+// (Four stages where they fit and every wave has as many transfers; with rounded weights, 2 x 2048 x 2048, 16 heads of 64: 126 us, with two 136.  Else two: heads of 40 as above 64 us,
 // with four 67, of 96 109 us, with three 112.)
 // A map's weights go into the product with v in two pieces of 16 bits each (pieces8), all of them: the difference of the maps is smaller than either, so that
 // rounded weights alone leave the result up to 1.6 times as far off as its own rounding (bf16: 0.0026 for 0.0017), and what is off must not go by where a key lies.
-// (2 x 4096 x 4096, 16 heads of 128, causal: 572 us, with rounded weights alone 450; 8 x 577 x 1000 by length, 12 heads of 40: 61 us.)
+// (2 x 4096 x 4096, 16 heads of 128, causal: 567 us, 1210 TFLOP/s, matrix units busy 62 %, with rounded weights alone 450; 8 x 577 x 1000 by length, 12 heads of 40: 61 us, matrix units busy
+// 34 %.)
 template <int CH>
 constexpr int differ_stages = CH == 2 || CH == 4 ? 4 : 2;
 template <typename T, int CH>

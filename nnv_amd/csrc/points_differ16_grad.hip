@@ -8,8 +8,9 @@
 // result at the end, and when a larger value comes the sums so far are scaled, as a softmax's are: what is below 2^-38 of the largest is lost, what is above 2^-28
 // keeps all bits.
 //
-// 2 x 4096 x 4096, 16 heads of 64, 4 for keys, causal, in bf16: dq 310 to 335 us, dk and dv 425 to 450.  Matrix units are busy 36 and 35 % of it, LDS 15 and 31: two waves a
-// SIMD, whose exponentials, roundings and reads from LDS follow one another between the products.  More waves would not have the registers.
+// 2 x 4096 x 4096, 16 heads of 64, 4 for keys, causal, in bf16: dq 346 to 373 us, dk and dv 461 to 501.  Matrix units are busy 38 and 44 % of it, LDS 14 and 30: two waves a
+// SIMD, whose exponentials, roundings and reads from LDS follow one another between the products.  More waves would not have the registers.  (Those of the keys' kernel that
+// do not fit, in scratch: 5 for heads of 49 to 64, 10 above 96; in f16 8, 6 for heads of 65 to 80, 86 to 96, 165 above.)
 #include "points_differ16.h"
 
 #pragma clang fp contract(fast)
@@ -69,7 +70,7 @@ struct Lift {
 
 // acc[d] += the product over 32 rows, from `first` on, of a tile of rows of DP values with p in two pieces.  (The scores' gradients
 // cancel: of rounded ones alone dq and dk are up to 1.6 times as far off as their own rounding, 0.0026 for 0.0017 in bf16.  The gradients of 2 x 4096 x 4096, 16 / 4 heads of 64,
-// causal, take 874 us, with rounded ones alone 710.)
+// causal, take 865 us, with rounded ones alone 710.)
 template <typename T, int DP>
 __device__ __forceinline__ void over_rows(unsigned tile, int first, const float16_t& p, float16_t (&acc)[DP / 32]) {
 #pragma unroll

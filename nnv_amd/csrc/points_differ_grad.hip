@@ -6,7 +6,8 @@
 // of weights and keys take: a row that sees one key has a scores' gradient of zero, and what rounding makes of it would reach dk.
 //
 // Bound by the f32 matrix instructions (4 x 1024 x 1024, 16 heads of 64: dq 475 us, dk and dv 740; 4 x 333 x 577, 6 heads of 40: 49 and 68, matrix units busy 48
-// and 44 %: blocks of six or seven tiles, in whose beginning and end nothing is multiplied).  Two buffers in LDS, and so one barrier a tile instead of two, measured the same.
+// and 44 %: blocks of six or seven tiles, in whose beginning and end nothing is multiplied).  Two buffers in LDS, and so one barrier a tile instead of two, measured the same.  Heads of 65 to 96,
+// and those that are no multiple of 4, have some registers in scratch (dq of heads of 92 in f32 125, of 90 208; dk and dv of 92 50, of 126 189): 4 x 333 x 577, 6 heads of 92 take 352 us, of 90 594.
 #include "points_differ16.h"
 
 #pragma clang fp contract(fast)
@@ -354,7 +355,7 @@ GradCut grad_cut(int64_t batch, int64_t kv_heads, int64_t queries, int64_t rows,
   c.key_tiles = (int)ceil_div(keys, by16 ? differ_key_grad16_tile(head) : kBlockRows);
   c.key_blocks = key_blocks_of(c.key_tiles, queries, keys, causal);
   // blocks that the chip holds at once; what starting a block, and adding splits up, costs in tiles of 32 rows.  A tile takes the 16-bit kernels a microsecond or more: a launch is
-  // three, and so are 12 MB of parts.  (2 x 200 x 300, 4 heads of 40 in f16: 59 us, with twelve for every sum 95; 8 x 577 x 1000, 12 heads of 64: 275, with four 314.)
+  // three, and so are 12 MB of parts.  (With half of the second pieces, 2 x 200 x 300, 4 heads of 40 in f16: 59 us, with twelve for every sum 95; 8 x 577 x 1000, 12 heads of 64: 275, with four 314.)
   const int64_t start = by16 ? 6 : 2, heads = batch * kv_heads;
   auto join = [&](int64_t values) { return by16 ? 3 + 16 * values / 4000000 : 3; };   // of f32, of two splits, written and read
   c.query_splits = split_of(heads * c.row_tiles, ceil_div(keys, 32), 2, by16 || head > 96 ? 256 : 512, start, join(heads * 2 * rows * head));

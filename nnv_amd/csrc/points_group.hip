@@ -14,8 +14,8 @@
 // rate asks some 1e13 operations a second of, a third of what the f64 pipes give, and they are of x - c and (x - c)^2, c the group's first value: a mean far from zero costs the variance
 // nothing, for the variance is no less than a share of (c - mean)^2, and that of equal values is zero.
 //
-// 16 x 64 x 64 x 320 in bf16: 26 us forward (3.2 TB/s: a block reads all it has before it writes, and one fits a CU), 54 backward (24 + 28 us a kernel: x and dy are read
-// twice, the second time partly from the caches); 5 x 53 x 79 x 96 in f32 backward 17; 4 x 8 x 8 x 256 forward 5.5 us, a launch and one latency of memory.
+// 16 x 64 x 64 x 320 in bf16: 26 us forward (3.2 TB/s: a block of two groups of 10 channels reads all it has before it writes, and one fits a CU), 54 backward (24 + 27 us a kernel: x and dy are read
+// twice, the second time partly from the caches); 5 x 53 x 79 x 96 in f32 backward 17; 4 x 8 x 8 x 256 forward 5.8 us, a launch and one latency of memory.
 #include "points.h"
 
 #include <algorithm>
@@ -670,7 +670,7 @@ constexpr int kMostPlaces = 128;   // that a thread adds, in f32 in the backward
 
 // The resident form takes a call where a chunk of whole groups, of four channels' multiples and 32 bytes at least, leaves a thread few enough places to
 // hold, and where there are many chunks, or short ones.  Forward, 16 x 64 x 64 x 320 in bf16, 21 places a thread: 28 us, in two launches 33.  Of x and dy
-// a thread holds ten places each (twice as many take more registers than 1024 threads have: 57 us, in two launches 50); 40 chunks of 21 places
+// a thread holds ten places each (twice as many take more registers than 1024 threads have: 57 us, in two launches 54); 40 chunks of 21 places
 // (5 x 53 x 79 x 96 in f32) take 26 us.
 constexpr int kPacks = 22, kGradPacks = 10;
 bool plan_resident(GroupArgs* a, int type, bool backward) {
