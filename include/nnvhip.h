@@ -588,7 +588,8 @@ NNVHIP_API int nnvhip_rotate_positions(nnvhip_ctx* ctx, const nnvhip_rotate_args
  *     second = softmax(scale * q1 k1^T) v, as o lies, which the backward call takes.  A row that sees no key gives zeros, lse = -inf.
  *   backward: from go (the gradient of o, strided), o, lse and second: dq, dk, dv dense in the shapes of q, k, v, zero where a row or key
  *     takes no part, and dweights in weight_type.  The order of the sums is fixed.
- * In 16 bits weights, their difference and scores' gradients go into their products as two numbers each; sums and exponents are f32.
+ * In 16 bits weights, their difference and scores' gradients go into their products as two numbers each; sums and exponents are f32.  dq of rows that see
+ * more than 256 keys takes the sums of go times o and second as these were rounded.
  * Sizes are bounded as in nnvhip_attention, with twice the heads. */
 typedef struct nnvhip_differ_args {
   int64_t type, weight_type, batch, queries, keys, heads, kv_heads, head, causal;

@@ -279,7 +279,7 @@ def differential_attention(q, k, v, weights, key_lengths=None, key_mask=None, ca
     In 16 bits the maps' weights, and in the backward pass their difference and the gradients of the scores, go into their products in two pieces that hold all but 2^-16 of them (2^-22
     in f16), so that a result is off by its own rounding alone.  But rows that see more
     than 256 keys take D, the sum of do times each map's result, for dq from the o and second that were rounded: dq is mostly up to 1.1 times as far off as its rounding (0.0018 for 0.0017 in bf16), up
-    to 1.4 times where a mask leaves few of the keys, and 2.3 times with heads of a few values."""
+    to 1.4 times where a mask leaves few of the keys, and 2.5 times with heads of a few values."""
     what = "differential_attention"
     ctx, lib, stream = _enter(what, ctx, q, k, v, weights, key_lengths, key_mask)
     sizes = _differ_sizes(what, q, k, v, weights, key_lengths, key_mask, scale)
